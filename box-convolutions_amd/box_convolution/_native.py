@@ -57,6 +57,17 @@ _SIGNATURES["boxconv_integral_image_int"] = (_i, [_vp, _vp, _i, _i64, _i, _i, _v
 _SIGNATURES["boxconv_integral_image_half_f32"] = (_i, [_vp, _i, _vp, _i64, _i, _i, _vp, _sz, _vp])
 _SIGNATURES["boxconv_forward_fused_f32"] = (_i, [_vp] * 6 + [_i] + [_vp] * 3 + [_i] * 8 + [_vp])
 
+_SIGNATURES["boxconv_group_norm_workspace_bytes"] = (_sz, [_i64, _i64, _i, _i, _i, _i])
+_SIGNATURES["boxconv_group_norm_forward"] = (
+    _i, [_vp] * 3 + [_i] + [_vp] * 4 + [_i, _i64, _i64, _i, _i, _f, _i, _vp, _sz, _vp])
+_SIGNATURES["boxconv_group_norm_backward"] = (
+    _i, [_vp] * 3 + [_i] + [_vp] * 8 + [_i, _i64, _i64, _i, _i, _i, _vp, _sz, _vp])
+_SIGNATURES["boxconv_linear_workspace_bytes"] = (_sz, [_i64, _i64, _i64, _i, _i])
+_SIGNATURES["boxconv_linear_forward"] = (
+    _i, [_vp, _i64, _vp, _vp, _vp, _i64, _vp, _vp, _i, _i64, _i64, _i64, _i, _vp, _sz, _vp])
+_SIGNATURES["boxconv_linear_backward"] = (
+    _i, [_vp, _i64] + [_vp] * 7 + [_i, _i64, _i64, _i64, _i, _vp, _sz, _vp])
+
 EXPORTED_SYMBOLS = tuple(sorted(_SIGNATURES))
 
 # element type codes BOXCONV_F32 / BOXCONV_F16 / BOXCONV_BF16 (include/boxconv.h)
@@ -622,10 +633,165 @@ def training_forward(input, x_min, x_max, y_min, y_max, reparametrization_h, rep
     return integrated, output, real.unbind(0)
 
 
+# ---- operators around a box convolution (channels-last data) ------------------------------------
+
+# activation codes BOXCONV_ACT_* (include/boxconv.h)
+ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3}
+
+
+def _operator_dtype(t, what):
+    try:
+        return _FUSED_OUTPUT[t.dtype]
+    except KeyError:
+        raise RuntimeError("box_convolution: %s must be float32, float16 or bfloat16, got %s"
+                           % (what, t.dtype)) from None
+
+
+def _activation(name):
+    try:
+        return ACTIVATIONS[name]
+    except (KeyError, TypeError):
+        raise RuntimeError("box_convolution: activation must be None, 'relu', 'silu' or 'gelu', got %r" % (name,)) from None
+
+
+def _operator_workspace_bytes(fn, *key):
+    key = (fn,) + key
+    n = _workspace_bytes.get(key)
+    if n is None:
+        n = _workspace_bytes[key] = getattr(load(), fn)(*key[1:])
+    return n
+
+
+def _norm_parameters(input, channels, weight, bias):
+    """(weight, bias, their dtype code): contiguous vectors of `channels` values, both float32 or both
+    of the input's type."""
+    kind, out = None, []
+    for name, p in (("weight", weight), ("bias", bias)):
+        if p is not None:
+            if p.device != input.device or p.dim() != 1 or p.size(0) != channels:
+                raise RuntimeError("box_convolution: %s must hold %d values on %s" % (name, channels, input.device))
+            if p.dtype not in (torch.float32, input.dtype) or kind not in (None, p.dtype):
+                raise RuntimeError("box_convolution: weight and bias must both be float32 or both of the input's type")
+            kind = p.dtype
+            p = p.contiguous()
+        out.append(p)
+    return out[0], out[1], _FUSED_OUTPUT[kind or torch.float32]
+
+
+def _same_as(t, like, what):
+    if t.device != like.device or t.dtype != like.dtype or t.shape != like.shape:
+        raise RuntimeError("box_convolution: %s must have the shape %s, type %s and device %s, got %s, %s, %s"
+                           % (what, tuple(like.shape), like.dtype, like.device, tuple(t.shape), t.dtype, t.device))
+    return t
+
+
+def group_norm_forward(input, num_groups, weight, bias, residual, activation, eps, keep_statistics):
+    """``act(group_norm(input) * weight + bias + residual)`` of a contiguous ``[B, ..., C]`` tensor
+    (include/boxconv.h, boxconv_group_norm_forward). Returns ``(output, mean, rstd)``, the last two
+    ``None`` unless ``keep_statistics``."""
+    B, C = input.size(0), input.size(-1)
+    dtype, act = _FUSED_OUTPUT[input.dtype], ACTIVATIONS[activation]
+    weight, bias, param_dtype = _norm_parameters(input, C, weight, bias)
+    output, mean, rstd = torch.empty_like(input), None, None
+    if keep_statistics:
+        mean, rstd = torch.empty((2, B, num_groups), dtype=torch.float32, device=input.device).unbind(0)
+    if input.numel() == 0:
+        return output, mean, rstd
+    pixels = input.numel() // (B * C)
+    with _on_device(input.device):
+        nbytes = _operator_workspace_bytes("boxconv_group_norm_workspace_bytes", B, pixels, C, num_groups, dtype, 0)
+        stream = _stream(input.device)
+        ws = _workspace(nbytes, input.device, stream)
+        rc = load().boxconv_group_norm_forward(
+            _ptr(input), _ptr(weight), _ptr(bias), param_dtype, _ptr(residual), _ptr(output), _ptr(mean), _ptr(rstd),
+            dtype, B, pixels, C, num_groups, eps, act, _ptr(ws), nbytes, stream)
+    _check(rc, "group_norm")
+    return output, mean, rstd
+
+
+def group_norm_backward(input, num_groups, weight, bias, residual, activation, mean, rstd, grad_output, needs):
+    """Gradients of ``group_norm_forward``, all tensors contiguous ``[B, ..., C]``. ``needs``: whether
+    input, weight, bias and residual need theirs; returns the four, ``None`` where not."""
+    B, C = input.size(0), input.size(-1)
+    dtype, act = _FUSED_OUTPUT[input.dtype], ACTIVATIONS[activation]
+    weight, bias, param_dtype = _norm_parameters(input, C, weight, bias)
+    kind = {0: torch.float32, 1: torch.float16, 2: torch.bfloat16}[param_dtype]
+    empty = input.numel() == 0
+    grads = [torch.empty_like(input) if needs[0] else None,
+             (torch.zeros if empty else torch.empty)(C, dtype=kind, device=input.device) if needs[1] else None,
+             (torch.zeros if empty else torch.empty)(C, dtype=kind, device=input.device) if needs[2] else None,
+             torch.empty_like(input) if needs[3] else None]
+    if empty:
+        return grads
+    pixels = input.numel() // (B * C)
+    with _on_device(input.device):
+        nbytes = _operator_workspace_bytes("boxconv_group_norm_workspace_bytes", B, pixels, C, num_groups, dtype, 1)
+        stream = _stream(input.device)
+        ws = _workspace(nbytes, input.device, stream)
+        rc = load().boxconv_group_norm_backward(
+            _ptr(input), _ptr(weight), _ptr(bias), param_dtype, _ptr(residual), _ptr(grad_output), _ptr(mean), _ptr(rstd),
+            *[_ptr(g) for g in grads], dtype, B, pixels, C, num_groups, act, _ptr(ws), nbytes, stream)
+    _check(rc, "group_norm backward")
+    return grads
+
+
+def linear_forward(input, weight, bias, residual, activation, keep_slope):
+    """``act(input @ weight.T + bias + residual)`` of a ``[rows, K]`` tensor with contiguous rows
+    (include/boxconv.h, boxconv_linear_forward). Returns ``(output, kept)``: what the backward
+    takes besides, ``None`` unless ``keep_slope`` and the activation has one."""
+    rows, K = input.shape
+    N = weight.size(0)
+    dtype, act = _FUSED_OUTPUT[input.dtype], ACTIVATIONS[activation]
+    output = torch.empty((rows, N), dtype=input.dtype, device=input.device)
+    slope = None
+    if keep_slope and act >= 2:
+        slope = torch.empty((rows, N), dtype=torch.float32 if dtype == 0 else torch.int16, device=input.device)
+    if output.numel() > 0:
+        with _on_device(input.device):
+            nbytes = _operator_workspace_bytes("boxconv_linear_workspace_bytes", rows, K, N, dtype, 0)
+            stream = _stream(input.device)
+            ws = _workspace(nbytes, input.device, stream)
+            rc = load().boxconv_linear_forward(
+                _ptr(input), input.stride(0), _ptr(weight), _ptr(bias), _ptr(residual),
+                0 if residual is None else residual.stride(0), _ptr(output), _ptr(slope), dtype, rows, K, N, act,
+                _ptr(ws), nbytes, stream)
+        _check(rc, "linear")
+    return output, slope if act >= 2 else output if keep_slope and act == 1 else None
+
+
+def linear_backward(input, weight, kept, activation, grad_output, needs):
+    """Gradients of ``linear_forward``; ``grad_output`` contiguous. ``needs``: whether input, weight, bias
+    and residual need theirs; returns the four, ``None`` where not."""
+    rows, K = input.shape
+    N = weight.size(0)
+    dtype, act = _FUSED_OUTPUT[input.dtype], ACTIVATIONS[activation]
+    none = rows == 0 or N == 0
+    new = torch.zeros if none or K == 0 else torch.empty
+    grads = [new((rows, K), dtype=input.dtype, device=input.device) if needs[0] else None,
+             new((N, K), dtype=input.dtype, device=input.device) if needs[1] else None,
+             new((N,), dtype=input.dtype, device=input.device) if needs[2] else None,
+             None]
+    if needs[3]:                 # without an activation the residual's gradient is grad_output itself
+        grads[3] = grad_output if act == 0 else torch.empty_like(grad_output)
+    if not none:
+        with _on_device(input.device):
+            nbytes = _operator_workspace_bytes("boxconv_linear_workspace_bytes", rows, K, N, dtype, 1)
+            stream = _stream(input.device)
+            ws = _workspace(nbytes, input.device, stream)
+            rc = load().boxconv_linear_backward(
+                _ptr(input), input.stride(0), _ptr(weight), _ptr(grad_output), _ptr(kept),
+                *[_ptr(g) for g in grads[:3]], _ptr(grads[3]) if act else None, dtype, rows, K, N, act, _ptr(ws), nbytes,
+                stream)
+        _check(rc, "linear backward")
+    return grads
+
+
 KERNEL_NAMES = ("band_colsum", "band_prefix", "band_scan", "forward_rows", "forward_quads", "forward_narrow", "forward_narrow_unaligned",
                 "grad_output_stream", "grad_input_cols", "grad_input_taps", "param_grad_finalize", "fill_zero", "fill_marker", "clip",
                 "forward_gather", "grad_input_gather", "grad_params_gather", "int_row_prefix",
-                "int_col_prefix")
+                "int_col_prefix", "norm_statistics", "norm_join", "norm_apply", "norm_small", "norm_any", "norm_sums",
+                "norm_join_sums", "norm_grad", "norm_small_grad", "norm_parameter", "norm_any_sums", "norm_any_grad", "linear",
+                "linear_dx", "linear_dweight", "linear_slope", "join_parts", "join_bias")
 
 
 def reload_switches():

@@ -40,11 +40,15 @@ def _inst(tag, t, tg, part, same):
 
 SOURCES = [(s, s.replace(".hip", ".o"), []) for s in
            ("box_sampling.hip", "integral_image.hip", "integral_image_int.hip", "box_misc.hip",
-            "boxconv_c_abi.hip")]
+            "boxconv_c_abi.hip", "operators_c_abi.hip", "group_norm.hip")]
 for _tag, _t, _tg in (("f32", "float", "float"), ("f64", "double", "double"),
                       ("f16", "float", "f16_t"), ("bf16", "float", "bf16_t")):
     for _part in (1, 2, 9) + ((3, 4, 5, 6, 7, 8) if _t == "float" else ()):
         SOURCES.append(_inst(_tag, _t, _tg, _part, _t == _tg))
+for _tag, _t in (("f32", "float"), ("f16", "_Float16"), ("bf16", "__bf16")):
+    SOURCES.append(("linear.hip", "linear_%s.o" % _tag, ["-DBOXCONV_INST_T=" + _t]))
+OPERATOR_HEADERS = ["activation.hpp", "operators_host.hpp", "linear_tile.hpp"]     # only included by the sources below
+OPERATOR_SOURCES = ("operators_c_abi.hip", "group_norm.hip", "linear.hip")
 HEADERS = ["boxconv_device.hpp", "boxconv_host.hpp", "box_sampling_common.hpp", "box_sampling_impl.hpp", "narrow_rows.hpp", "forward_tail.hpp",
            os.path.join("..", "..", "include", "boxconv.h")]
 
@@ -103,13 +107,14 @@ def build(force=False, verbose=True):
     os.makedirs(OBJ_DIR, exist_ok=True)
     hipcc = _hipcc()
     header_paths = [os.path.normpath(os.path.join(CSRC, h)) for h in HEADERS] + [os.path.abspath(__file__)]
+    operator_paths = header_paths + [os.path.join(CSRC, h) for h in OPERATOR_HEADERS]
     jobs = []
     objs = []
     for src, obj_name, defines in SOURCES:
         src_path = os.path.join(CSRC, src)
         obj = os.path.join(OBJ_DIR, obj_name)
         objs.append(obj)
-        if force or _stale(obj, [src_path] + header_paths):
+        if force or _stale(obj, [src_path] + (operator_paths if src in OPERATOR_SOURCES else header_paths)):
             jobs.append([hipcc] + HIPCC_FLAGS + defines + ["-c", src_path, "-o", obj])
 
     def run(cmd):

@@ -57,8 +57,10 @@ void profile_after(const char* name, hipStream_t stream) {
 }  // namespace boxconv
 
 namespace {
-
 thread_local char g_error[512] = "";
+}  // namespace
+
+namespace boxconv {
 
 int fail(int code, const char* fmt, ...) {
     va_list ap;
@@ -72,6 +74,13 @@ int hip_result(hipError_t e, const char* what) {
     if (e == hipSuccess) return 0;
     return fail(static_cast<int>(e), "%s: %s", what, hipGetErrorString(e));
 }
+
+}  // namespace boxconv
+
+namespace {
+
+using boxconv::fail;
+using boxconv::hip_result;
 
 constexpr int64_t kMaxElems = (int64_t(1) << 31) - 1;
 

@@ -291,6 +291,10 @@ void profile_after(const char* name, hipStream_t stream);
         ::boxconv::profile_after(NAME, STREAM);                                   \
     } while (0)
 
+// boxconv_last_error()'s message for this thread, and `code`; 0 or the code and message of a HIP error.
+int fail(int code, const char* fmt, ...);
+int hip_result(hipError_t e, const char* what);
+
 constexpr int kMaxRowStreamWidth = 4096;       // float32 rows; float64 rows half of that
 constexpr int kMaxScanRowsWidth = 4096;        // widest row the one-workgroup-per-row integral kernels take
 constexpr int kMaxWideningWidth = 2048;        // widest float16 / bfloat16 row the integral image reads directly

@@ -1,0 +1,996 @@
+// Group norm with a residual and an activation on channels-last data, forward and backward.
+//
+//   m = pixels * channels / groups values per (batch item b, group g);  mean, var over them;  rstd = 1/sqrt(var + eps)
+//   u = (x - mean) * rstd;  z = u * weight[c] + bias[c] + residual;  y = act(z)
+//   dz = dy * act'(z);  dweight[c] = sum dz*u;  dbias[c] = sum dz;  dresidual = dz
+//   dx = rstd * (weight[c]*dz - (s1 + u*s2)/m),  s1, s2 = sums over the group of weight*dz and weight*dz*u
+//
+// A batch item is one run of pixels * channels elements. Lane t of a workgroup takes 16-byte vectors t, t + T, t + 2T, ... of
+// it, with T (at most the workgroup's threads) a multiple of the vectors after which the channels repeat: the channels of a
+// lane's elements then never change, so per-channel values and sums sit in registers, whatever the number of channels.
+#include "activation.hpp"
+#include "boxconv_host.hpp"
+#include "operators_host.hpp"
+
+namespace boxconv {
+
+namespace {
+
+constexpr int kUnroll = 8;             // vectors a lane requests before it uses the first one, in the statistics
+
+// How a workgroup's lanes lie over one batch item (or, in the one-launch kernels, over `slab` of its channels).
+struct Lanes {
+    int64_t total;        // elements of a batch item
+    int64_t stride;       // elements from a lane's vector to its next one
+    int channels, slab;   // channels in all; channels a workgroup covers (all of them, or whole groups and whole vectors)
+    int active;           // lanes that take part
+    int phase;            // lanes after which the channels repeat
+};
+
+template <class T>
+struct Item {
+    static constexpr int V = Vec<T>::kLen;
+    typedef typename Vec<T>::Type Packed;
+    // First element of lane t (relative to the batch item), channels [c0, c0 + slab).
+    static __device__ __forceinline__ int64_t offset(const Lanes& L, int t, int c0) {
+        return static_cast<int64_t>(t / L.phase) * (L.slab == L.channels ? L.phase * V : L.channels) + c0 + (t % L.phase) * V;
+    }
+    // Elements [off, off + V) of an item of `total`: V of them, fewer at its end, zeros beyond it.
+    static __device__ __forceinline__ Packed load(const T* p, int64_t off, int64_t total) {
+        if (off + V <= total) return *reinterpret_cast<const Packed*>(p + off);
+        Packed v = {};
+        for (int j = 0; j < V; ++j)
+            if (off + j < total) v[j] = p[off + j];
+        return v;
+    }
+    static __device__ __forceinline__ void store(T* p, int64_t off, int64_t total, Packed v) {
+        if (off + V <= total) {
+            *reinterpret_cast<Packed*>(p + off) = v;
+            return;
+        }
+        for (int j = 0; j < V; ++j)
+            if (off + j < total) p[off + j] = v[j];
+    }
+};
+
+// Sum over `width` (a power of two, at most 64) neighbouring lanes.
+__device__ __forceinline__ float sum_over(float v, int width) {
+    for (int d = width >> 1; d > 0; d >>= 1) v += __shfl_xor(v, d);
+    return v;
+}
+
+// Lanes that share a group when the workgroup's threads walk over `groups` of them: a power of two.
+__device__ __forceinline__ int lanes_per_group(int threads, int groups) {
+    int w = 64;
+    while (w > 1 && w * groups > threads) w >>= 1;
+    return w;
+}
+
+// Per-slot statistics of a workgroup's lanes to per-group ones: count, mean and sum of squared deviations. Means are joined
+// before deviations, so nothing cancels however far the mean is from zero. `put(g, n, mean, m2)` gets the groups that start
+// at channel c0, counted from 0.
+template <int V, class Put>
+__device__ __forceinline__ void join_statistics(const float (&mean)[V], const float (&m2)[V], const float (&count)[V], float* lds,
+                                                const Lanes& L, int per_group, Put put) {
+    const int t = threadIdx.x, slots = L.active * V;
+    float *smean = lds, *sm2 = lds + slots, *sn = lds + 2 * slots;
+    if (t < L.active) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            smean[t * V + j] = mean[j];
+            sm2[t * V + j] = m2[j];
+            sn[t * V + j] = count[j];
+        }
+    }
+    __syncthreads();
+    // slots t*V + j with (t % phase)*V + j = c (mod slab) hold channel c: slot c + slab*k for every k
+    const int groups = L.slab / per_group, width = lanes_per_group(blockDim.x, groups), per_channel = slots / L.slab;
+    for (int g0 = 0; g0 < groups; g0 += blockDim.x / width) {
+        const int g = g0 + t / width;
+        const bool live = g < groups;
+        float n = 0.0f, sum = 0.0f;
+        if (live)
+            for (int i = t % width; i < per_group * per_channel; i += width) {
+                const int s = g * per_group + i % per_group + L.slab * (i / per_group);
+                n += sn[s];
+                sum = fmaf(sn[s], smean[s], sum);
+            }
+        n = sum_over(n, width);
+        const float mu = n > 0.0f ? sum_over(sum, width) / n : 0.0f;
+        float dev = 0.0f;
+        if (live)
+            for (int i = t % width; i < per_group * per_channel; i += width) {
+                const int s = g * per_group + i % per_group + L.slab * (i / per_group);
+                const float d = smean[s] - mu;
+                dev += sm2[s] + sn[s] * d * d;
+            }
+        dev = sum_over(dev, width);
+        if (live && t % width == 0) put(g, n, mu, dev);
+    }
+}
+
+// Sums per slot to sums per channel of the slab (channel counted from 0): put(c, sum a, sum b).
+template <int V, class Put>
+__device__ __forceinline__ void join_channels(const float (&a)[V], const float (&b)[V], float* lds, const Lanes& L, Put put) {
+    const int t = threadIdx.x, slots = L.active * V;
+    float *sa = lds, *sb = lds + slots;
+    if (t < L.active) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            sa[t * V + j] = a[j];
+            sb[t * V + j] = b[j];
+        }
+    }
+    __syncthreads();
+    for (int c = t; c < L.slab; c += blockDim.x) {
+        float x = 0.0f, y = 0.0f;
+        for (int s = c; s < slots; s += L.slab) {
+            x += sa[s];
+            y += sb[s];
+        }
+        put(c, x, y);
+    }
+}
+
+// ---- statistics of large items: partial results per workgroup --------------------------------------
+// partial[(b * chunks + chunk) * groups + g] = (count, mean, sum of squared deviations). Every batch of kUnroll vectors is
+// reduced around its own mean and joined to the lane's running one (the formula of Chan, Golub and LeVeque), so the sums
+// are as good for a channel with a large mean as for one without.
+template <class T>
+__global__ void __launch_bounds__(1024)
+norm_statistics_kernel(const T* __restrict__ x, float* __restrict__ partial, Lanes L, int64_t chunk_steps, int chunks,
+                       int groups, int per_group) {
+    constexpr int V = Vec<T>::kLen;
+    extern __shared__ float lds[];
+    const int t = threadIdx.x;
+    const int64_t b = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
+    const T* item = x + b * L.total;
+    float mean[V], m2[V], count[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) mean[j] = m2[j] = count[j] = 0.0f;
+    if (t < L.active) {
+        int64_t off = Item<T>::offset(L, t, 0) + chunk * chunk_steps * L.stride;
+        const int64_t end = min(L.total, (chunk + 1) * chunk_steps * L.stride);    // the chunk's elements: a multiple of stride, or the item's end
+        float n = 0.0f;
+        for (; off + (kUnroll - 1) * L.stride + V <= end; off += kUnroll * L.stride) {
+            typename Vec<T>::Type v[kUnroll];
+#pragma unroll
+            for (int k = 0; k < kUnroll; ++k) v[k] = *reinterpret_cast<const typename Vec<T>::Type*>(item + off + k * L.stride);
+            const float inv = 1.0f / (n + kUnroll), share = kUnroll * inv, joint = n * share;
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                float s = 0.0f, d2 = 0.0f;
+#pragma unroll
+                for (int k = 0; k < kUnroll; ++k) s += static_cast<float>(v[k][j]);
+                const float mu = s * (1.0f / kUnroll);
+#pragma unroll
+                for (int k = 0; k < kUnroll; ++k) {
+                    const float d = static_cast<float>(v[k][j]) - mu;
+                    d2 = fmaf(d, d, d2);
+                }
+                const float delta = mu - mean[j];
+                mean[j] = fmaf(delta, share, mean[j]);
+                m2[j] += fmaf(delta * delta, joint, d2);
+            }
+            n += kUnroll;
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) count[j] = n;
+        for (; off < end; off += L.stride) {
+            const auto v = Item<T>::load(item, off, L.total);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                if (off + j >= L.total) continue;
+                const float delta = static_cast<float>(v[j]) - mean[j], share = 1.0f / (count[j] + 1.0f);
+                mean[j] = fmaf(delta, share, mean[j]);
+                m2[j] = fmaf(delta * delta, count[j] * share, m2[j]);
+                count[j] += 1.0f;
+            }
+        }
+    }
+    float* out = partial + blockIdx.x * static_cast<int64_t>(groups) * 3;
+    join_statistics<V>(mean, m2, count, lds, L, per_group, [&](int g, float n, float mu, float dev) {
+        out[3 * g] = n;
+        out[3 * g + 1] = mu;
+        out[3 * g + 2] = dev;
+    });
+}
+
+// One wave per (batch item, group): the partial results of all its workgroups, in their order.
+__global__ void __launch_bounds__(256)
+norm_join_kernel(const float* __restrict__ partial, float* __restrict__ mean, float* __restrict__ rstd, int64_t pairs,
+                 int groups, int chunks, float eps) {
+    const int64_t pair = blockIdx.x * 4ll + threadIdx.x / 64;
+    if (pair >= pairs) return;
+    const int lane = threadIdx.x % 64, g = static_cast<int>(pair % groups);
+    const float* p = partial + (pair / groups * chunks * groups + g) * 3;
+    const int64_t step = static_cast<int64_t>(groups) * 3;
+    float n = 0.0f, sum = 0.0f, dev = 0.0f;
+    for (int i = lane; i < chunks; i += 64) {
+        n += p[i * step];
+        sum = fmaf(p[i * step], p[i * step + 1], sum);
+    }
+    n = sum_over(n, 64);
+    const float mu = sum_over(sum, 64) / n;
+    for (int i = lane; i < chunks; i += 64) {
+        const float d = p[i * step + 1] - mu;
+        dev += p[i * step + 2] + p[i * step] * d * d;
+    }
+    dev = sum_over(dev, 64);
+    if (lane == 0) {
+        mean[pair] = mu;
+        rstd[pair] = 1.0f / sqrtf(dev / n + eps);
+    }
+}
+
+template <class T>
+struct NormArgs {
+    const T *x, *residual;
+    const void *weight, *bias;
+    T* y;
+    bool float_params;
+    int groups, per_group;
+    float eps;
+};
+
+// ---- y from the statistics -------------------------------------------------------------------------
+// (x - mean) is formed first: x * scale + shift would lose what a mean far from zero takes of the digits.
+template <class T, int ACT>
+__global__ void __launch_bounds__(1024)
+norm_apply_kernel(NormArgs<T> a, const float* __restrict__ mean, const float* __restrict__ rstd, Lanes L,
+                  int64_t chunk_steps, int chunks, int total_workgroups) {
+    constexpr int V = Vec<T>::kLen, U = 4;
+    typedef typename Vec<T>::Type Packed;
+    const int t = threadIdx.x;
+    if (t >= L.active) return;
+    // last to first: the end of x is what the statistics left in the memory-side cache
+    const int id = total_workgroups - 1 - blockIdx.x;
+    const int64_t b = id / chunks, chunk = id % chunks;
+    const T *x = a.x + b * L.total, *r = a.residual ? a.residual + b * L.total : nullptr;
+    T* y = a.y + b * L.total;
+    int64_t off = Item<T>::offset(L, t, 0);
+    float mu[V], scale[V], shift[V];
+    int c = static_cast<int>(off % L.channels);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const int64_t pair = b * a.groups + c / a.per_group;
+        mu[j] = mean[pair];
+        scale[j] = rstd[pair] * (a.weight ? load_param<T>(a.weight, a.float_params, c) : 1.0f);
+        shift[j] = a.bias ? load_param<T>(a.bias, a.float_params, c) : 0.0f;
+        if (++c == L.channels) c = 0;
+    }
+    off += chunk * chunk_steps * L.stride;
+    const int64_t end = min(L.total, (chunk + 1) * chunk_steps * L.stride);
+    for (; off + (U - 1) * L.stride + V <= end; off += U * L.stride) {
+        Packed v[U], q[U];
+#pragma unroll
+        for (int k = 0; k < U; ++k) v[k] = *reinterpret_cast<const Packed*>(x + off + k * L.stride);
+        if (r != nullptr) {
+#pragma unroll
+            for (int k = 0; k < U; ++k) q[k] = *reinterpret_cast<const Packed*>(r + off + k * L.stride);
+        } else {
+#pragma unroll
+            for (int k = 0; k < U; ++k) q[k] = Packed{};
+        }
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            Packed o;
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float z = fmaf(static_cast<float>(v[k][j]) - mu[j], scale[j], shift[j]) + static_cast<float>(q[k][j]);
+                o[j] = static_cast<T>(activate<ACT>(z));
+            }
+            *reinterpret_cast<Packed*>(y + off + k * L.stride) = o;
+        }
+    }
+    for (; off < end; off += L.stride) {
+        const Packed v = Item<T>::load(x, off, L.total);
+        Packed q = {}, o;
+        if (r != nullptr) q = Item<T>::load(r, off, L.total);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const float z = fmaf(static_cast<float>(v[j]) - mu[j], scale[j], shift[j]) + static_cast<float>(q[j]);
+            o[j] = static_cast<T>(activate<ACT>(z));
+        }
+        Item<T>::store(y, off, L.total, o);
+    }
+}
+
+// ---- backward, first pass: per-channel sums of dz and dz*u -------------------------------------------
+template <class T>
+struct NormBackwardArgs {
+    const T *x, *residual, *dy;
+    const void *weight, *bias;
+    const float *mean, *rstd;
+    T *dx, *dresidual;
+    void *dweight, *dbias;
+    bool float_params;
+    int groups, per_group;
+};
+
+template <class T, int ACT>
+__global__ void __launch_bounds__(1024)
+norm_sums_kernel(NormBackwardArgs<T> a, float* __restrict__ partial, Lanes L, int64_t chunk_steps, int chunks) {
+    constexpr int V = Vec<T>::kLen, U = 2;
+    typedef typename Vec<T>::Type Packed;
+    extern __shared__ float lds[];
+    const int t = threadIdx.x;
+    const int64_t b = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
+    float sum[V], dot[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) sum[j] = dot[j] = 0.0f;
+    if (t < L.active) {
+        const T *x = a.x + b * L.total, *dy = a.dy + b * L.total;
+        const T* r = ACT != kActNone && a.residual ? a.residual + b * L.total : nullptr;
+        int64_t off = Item<T>::offset(L, t, 0);
+        float mu[V], rs[V], w[V], bias[V];
+        int c = static_cast<int>(off % L.channels);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int64_t pair = b * a.groups + c / a.per_group;
+            mu[j] = a.mean[pair];
+            rs[j] = a.rstd[pair];
+            w[j] = a.weight ? load_param<T>(a.weight, a.float_params, c) : 1.0f;
+            bias[j] = a.bias ? load_param<T>(a.bias, a.float_params, c) : 0.0f;
+            if (++c == L.channels) c = 0;
+        }
+        off += chunk * chunk_steps * L.stride;
+        const int64_t end = min(L.total, (chunk + 1) * chunk_steps * L.stride);
+        auto add = [&](const Packed& v, const Packed& g, const Packed& q) {      // (beyond the end g is zero)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float u = (static_cast<float>(v[j]) - mu[j]) * rs[j];
+                float dz = static_cast<float>(g[j]);
+                if constexpr (ACT != kActNone) dz *= slope<ACT>(fmaf(u, w[j], bias[j]) + static_cast<float>(q[j]));
+                sum[j] += dz;
+                dot[j] = fmaf(dz, u, dot[j]);
+            }
+        };
+        for (; off + (U - 1) * L.stride + V <= end; off += U * L.stride) {
+            Packed v[U], g[U], q[U];
+#pragma unroll
+            for (int k = 0; k < U; ++k) {
+                v[k] = *reinterpret_cast<const Packed*>(x + off + k * L.stride);
+                g[k] = *reinterpret_cast<const Packed*>(dy + off + k * L.stride);
+                q[k] = Packed{};
+            }
+            if (r != nullptr) {
+#pragma unroll
+                for (int k = 0; k < U; ++k) q[k] = *reinterpret_cast<const Packed*>(r + off + k * L.stride);
+            }
+#pragma unroll
+            for (int k = 0; k < U; ++k) add(v[k], g[k], q[k]);
+        }
+        for (; off < end; off += L.stride) {
+            const Packed v = Item<T>::load(x, off, L.total), g = Item<T>::load(dy, off, L.total);
+            Packed q = {};
+            if (r != nullptr) q = Item<T>::load(r, off, L.total);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                if (off + j >= L.total) continue;
+                const float u = (static_cast<float>(v[j]) - mu[j]) * rs[j];
+                float dz = static_cast<float>(g[j]);
+                if constexpr (ACT != kActNone) dz *= slope<ACT>(fmaf(u, w[j], bias[j]) + static_cast<float>(q[j]));
+                sum[j] += dz;
+                dot[j] = fmaf(dz, u, dot[j]);
+            }
+        }
+    }
+    float* out = partial + blockIdx.x * static_cast<int64_t>(L.channels) * 2;
+    join_channels<V>(sum, dot, lds, L, [&](int c, float s, float d) {
+        out[2 * c] = s;
+        out[2 * c + 1] = d;
+    });
+}
+
+// totals[b][c] = the partial sums of all workgroups of an item, 16 channels by 16 rows of threads, always in the same order.
+__global__ void __launch_bounds__(256)
+norm_join_sums_kernel(const float2* __restrict__ partial, float2* __restrict__ totals, int channels, int chunks, int tiles) {
+    __shared__ float2 part[16][17];
+    const int64_t b = blockIdx.x / tiles;
+    const int c = blockIdx.x % tiles * 16 + threadIdx.x % 16, row = threadIdx.x / 16;
+    float2 s = {0.0f, 0.0f};
+    if (c < channels) {
+        const float2* p = partial + b * chunks * channels + c;
+        for (int i = row; i < chunks; i += 16) {
+            const float2 v = p[static_cast<int64_t>(i) * channels];
+            s.x += v.x;
+            s.y += v.y;
+        }
+    }
+    part[row][threadIdx.x % 16] = s;
+    __syncthreads();
+    if (row == 0 && c < channels) {
+        for (int i = 1; i < 16; ++i) {
+            s.x += part[i][threadIdx.x].x;
+            s.y += part[i][threadIdx.x].y;
+        }
+        totals[b * channels + c] = s;
+    }
+}
+
+// s1/m and s2/m of the groups of `slab` channels from c0 on, in LDS, from per-channel totals.
+template <class T, class Total>
+__device__ __forceinline__ void group_terms(float2* terms, Total total, const NormBackwardArgs<T>& a, int c0, int slab, float inv_m) {
+    const int groups = slab / a.per_group, width = lanes_per_group(blockDim.x, groups), t = threadIdx.x;
+    for (int g0 = 0; g0 < groups; g0 += blockDim.x / width) {
+        const int g = g0 + t / width;
+        float s1 = 0.0f, s2 = 0.0f;
+        if (g < groups)
+            for (int i = t % width; i < a.per_group; i += width) {
+                const int c = g * a.per_group + i;
+                const float2 v = total(c);
+                const float w = a.weight ? load_param<T>(a.weight, a.float_params, c0 + c) : 1.0f;
+                s1 = fmaf(w, v.x, s1);
+                s2 = fmaf(w, v.y, s2);
+            }
+        s1 = sum_over(s1, width);
+        s2 = sum_over(s2, width);
+        if (g < groups && t % width == 0) terms[g] = {s1 * inv_m, s2 * inv_m};
+    }
+}
+
+// dweight, dbias: the totals of all batch items, in their order. Threads [first, first + n) of the launch.
+template <class T>
+__device__ __forceinline__ void parameter_sums(const NormBackwardArgs<T>& a, const float2* totals, int64_t batch, int channels, int c) {
+    float s = 0.0f, d = 0.0f;
+    for (int64_t b = 0; b < batch; ++b) {
+        const float2 v = totals[b * channels + c];
+        s += v.x;
+        d += v.y;
+    }
+    if (a.dbias) store_param<T>(a.dbias, a.float_params, c, s);
+    if (a.dweight) store_param<T>(a.dweight, a.float_params, c, d);
+}
+
+// ---- backward, second pass: dx and dresidual -----------------------------------------------------------
+template <class T, int ACT>
+__global__ void __launch_bounds__(1024)
+norm_grad_kernel(NormBackwardArgs<T> a, const float2* __restrict__ totals, Lanes L, int64_t chunk_steps, int chunks,
+                 int64_t batch, float inv_m, int total_workgroups) {
+    constexpr int V = Vec<T>::kLen, U = 2;
+    typedef typename Vec<T>::Type Packed;
+    extern __shared__ float lds[];
+    const int t = threadIdx.x;
+    // the first workgroups add up the parameter gradients on the side
+    for (int64_t c = blockIdx.x * static_cast<int64_t>(blockDim.x) + t; c < L.channels; c += static_cast<int64_t>(total_workgroups) * blockDim.x)
+        parameter_sums(a, totals, batch, L.channels, static_cast<int>(c));
+    if (a.dx == nullptr && a.dresidual == nullptr) return;
+    const int id = total_workgroups - 1 - blockIdx.x;                       // last to first, as in norm_apply_kernel
+    const int64_t b = id / chunks, chunk = id % chunks;
+    float2* terms = reinterpret_cast<float2*>(lds);
+    group_terms(terms, [&](int c) { return totals[b * L.channels + c]; }, a, 0, L.channels, inv_m);
+    __syncthreads();
+    if (t >= L.active) return;
+    const T *x = a.x + b * L.total, *dy = a.dy + b * L.total;
+    const T* r = ACT != kActNone && a.residual ? a.residual + b * L.total : nullptr;
+    T *dx = a.dx ? a.dx + b * L.total : nullptr, *dr = a.dresidual ? a.dresidual + b * L.total : nullptr;
+    int64_t off = Item<T>::offset(L, t, 0);
+    // dx = A dz + B (x - mean) + D,  z = A (x - mean) + bias + r
+    float mu[V], A[V], B[V], D[V], bias[V];
+    int c = static_cast<int>(off % L.channels);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const int g = c / a.per_group;
+        const float rs = a.rstd[b * a.groups + g];
+        mu[j] = a.mean[b * a.groups + g];
+        A[j] = rs * (a.weight ? load_param<T>(a.weight, a.float_params, c) : 1.0f);
+        B[j] = -rs * rs * terms[g].y;
+        D[j] = -rs * terms[g].x;
+        bias[j] = a.bias ? load_param<T>(a.bias, a.float_params, c) : 0.0f;
+        if (++c == L.channels) c = 0;
+    }
+    off += chunk * chunk_steps * L.stride;
+    const int64_t end = min(L.total, (chunk + 1) * chunk_steps * L.stride);
+    auto form = [&](const Packed& v, const Packed& g, const Packed& q, Packed& o, Packed& p) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const float xc = static_cast<float>(v[j]) - mu[j];
+            float dz = static_cast<float>(g[j]);
+            if constexpr (ACT != kActNone) dz *= slope<ACT>(fmaf(xc, A[j], bias[j]) + static_cast<float>(q[j]));
+            o[j] = static_cast<T>(fmaf(A[j], dz, fmaf(B[j], xc, D[j])));
+            p[j] = static_cast<T>(dz);
+        }
+    };
+    for (; off + (U - 1) * L.stride + V <= end; off += U * L.stride) {
+        Packed v[U], g[U], q[U];
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            v[k] = *reinterpret_cast<const Packed*>(x + off + k * L.stride);
+            g[k] = *reinterpret_cast<const Packed*>(dy + off + k * L.stride);
+            q[k] = Packed{};
+        }
+        if (r != nullptr) {
+#pragma unroll
+            for (int k = 0; k < U; ++k) q[k] = *reinterpret_cast<const Packed*>(r + off + k * L.stride);
+        }
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            Packed o, p;
+            form(v[k], g[k], q[k], o, p);
+            if (dx != nullptr) *reinterpret_cast<Packed*>(dx + off + k * L.stride) = o;
+            if (dr != nullptr) *reinterpret_cast<Packed*>(dr + off + k * L.stride) = p;
+        }
+    }
+    for (; off < end; off += L.stride) {
+        const Packed v = Item<T>::load(x, off, L.total), g = Item<T>::load(dy, off, L.total);
+        Packed q = {}, o, p;
+        if (r != nullptr) q = Item<T>::load(r, off, L.total);
+        form(v, g, q, o, p);
+        if (dx != nullptr) Item<T>::store(dx, off, L.total, o);
+        if (dr != nullptr) Item<T>::store(dr, off, L.total, p);
+    }
+}
+
+// ---- items that one workgroup's registers hold: one launch -----------------------------------------------
+template <class T, int ACT, int N>
+__global__ void __launch_bounds__(1024)
+norm_small_kernel(NormArgs<T> a, float* __restrict__ mean_out, float* __restrict__ rstd_out, Lanes L, int slabs) {
+    constexpr int V = Vec<T>::kLen;
+    typedef typename Vec<T>::Type Packed;
+    extern __shared__ float lds[];
+    const int t = threadIdx.x, c0 = blockIdx.x % slabs * L.slab;
+    const int64_t b = blockIdx.x / slabs;
+    const T *x = a.x + b * L.total, *r = a.residual ? a.residual + b * L.total : nullptr;
+    const int64_t off = Item<T>::offset(L, t, c0);
+    const bool live = t < L.active;
+    Packed v[N];
+    if (live) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) v[k] = Item<T>::load(x, off + k * L.stride, L.total);
+    }
+    float mean[V], m2[V], count[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        float n = 0.0f, s = 0.0f, d2 = 0.0f;
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            if (live && off + k * L.stride + j < L.total) {
+                n += 1.0f;
+                s += static_cast<float>(v[k][j]);
+            }
+        const float mu = n > 0.0f ? s / n : 0.0f;
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            if (live && off + k * L.stride + j < L.total) {
+                const float d = static_cast<float>(v[k][j]) - mu;
+                d2 = fmaf(d, d, d2);
+            }
+        mean[j] = mu;
+        m2[j] = d2;
+        count[j] = n;
+    }
+    float2* stats = reinterpret_cast<float2*>(lds + 3 * L.active * V);
+    const int g0 = c0 / a.per_group;
+    join_statistics<V>(mean, m2, count, lds, L, a.per_group, [&](int g, float n, float mu, float dev) {
+        const float rs = 1.0f / sqrtf(dev / n + a.eps);
+        stats[g] = {mu, rs};
+        if (mean_out != nullptr) {
+            mean_out[b * a.groups + g0 + g] = mu;
+            rstd_out[b * a.groups + g0 + g] = rs;
+        }
+    });
+    __syncthreads();
+    if (!live) return;
+    float scale[V], shift[V];
+    int c = static_cast<int>(off % L.channels);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const float2 s = stats[c / a.per_group - g0];
+        mean[j] = s.x;
+        scale[j] = s.y * (a.weight ? load_param<T>(a.weight, a.float_params, c) : 1.0f);
+        shift[j] = a.bias ? load_param<T>(a.bias, a.float_params, c) : 0.0f;
+        if (++c == L.channels) c = 0;
+    }
+    T* y = a.y + b * L.total;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        const int64_t at = off + k * L.stride;
+        if (at >= L.total) break;
+        Packed q = {}, o;
+        if (r != nullptr) q = Item<T>::load(r, at, L.total);
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            o[j] = static_cast<T>(activate<ACT>(fmaf(static_cast<float>(v[k][j]) - mean[j], scale[j], shift[j]) + static_cast<float>(q[j])));
+        Item<T>::store(y, at, L.total, o);
+    }
+}
+
+// The backward reads its tensors twice, the second time from the L2: x and dy would not fit a lane's registers beside the
+// per-channel values of its elements.
+template <class T, int ACT>
+__global__ void __launch_bounds__(1024)
+norm_small_grad_kernel(NormBackwardArgs<T> a, float2* __restrict__ totals, Lanes L, int slabs, float inv_m) {
+    constexpr int V = Vec<T>::kLen;
+    typedef typename Vec<T>::Type Packed;
+    extern __shared__ float lds[];
+    const int t = threadIdx.x, c0 = blockIdx.x % slabs * L.slab, g0 = c0 / a.per_group;
+    const int64_t b = blockIdx.x / slabs;
+    const T *x = a.x + b * L.total, *dy = a.dy + b * L.total;
+    const T* r = ACT != kActNone && a.residual ? a.residual + b * L.total : nullptr;
+    const int64_t off = Item<T>::offset(L, t, c0);
+    const int64_t end = t < L.active ? L.total : 0;
+    float mu[V], rs[V], w[V], bias[V], sum[V], dot[V];
+    int c = static_cast<int>(off % L.channels);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const int64_t pair = b * a.groups + c / a.per_group;
+        sum[j] = dot[j] = 0.0f;
+        mu[j] = a.mean[pair];
+        rs[j] = a.rstd[pair];
+        w[j] = a.weight ? load_param<T>(a.weight, a.float_params, c) : 1.0f;
+        bias[j] = a.bias ? load_param<T>(a.bias, a.float_params, c) : 0.0f;
+        if (++c == L.channels) c = 0;
+    }
+    T* dr = a.dresidual ? a.dresidual + b * L.total : nullptr;
+#pragma unroll 1
+    for (int64_t at = off; at < end; at += L.stride) {
+        const Packed v = Item<T>::load(x, at, L.total), g = Item<T>::load(dy, at, L.total);
+        Packed q = {}, p;
+        if (r != nullptr) q = Item<T>::load(r, at, L.total);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const float u = (static_cast<float>(v[j]) - mu[j]) * rs[j];
+            float dz = static_cast<float>(g[j]);
+            if constexpr (ACT != kActNone) dz *= slope<ACT>(fmaf(u, w[j], bias[j]) + static_cast<float>(q[j]));
+            p[j] = static_cast<T>(dz);
+            if (at + j < L.total) {
+                sum[j] += dz;
+                dot[j] = fmaf(dz, u, dot[j]);
+            }
+        }
+        if (dr != nullptr) Item<T>::store(dr, at, L.total, p);
+    }
+    float2* chan = reinterpret_cast<float2*>(lds + 2 * L.active * V);
+    float2* terms = chan + L.slab;
+    join_channels<V>(sum, dot, lds, L, [&](int ch, float s, float d) {
+        chan[ch] = {s, d};
+        totals[b * L.channels + c0 + ch] = {s, d};
+    });
+    __syncthreads();
+    group_terms(terms, [&](int ch) { return chan[ch]; }, a, c0, L.slab, inv_m);
+    __syncthreads();
+    if (a.dx == nullptr || end == 0) return;
+    T* dx = a.dx + b * L.total;
+    float t1[V], t2[V];
+    c = static_cast<int>(off % L.channels);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const float2 s = terms[c / a.per_group - g0];
+        t1[j] = s.x;
+        t2[j] = s.y;
+        if (++c == L.channels) c = 0;
+    }
+#pragma unroll 1
+    for (int64_t at = off; at < end; at += L.stride) {
+        const Packed v = Item<T>::load(x, at, L.total), g = Item<T>::load(dy, at, L.total);
+        Packed q = {}, o;
+        if (r != nullptr) q = Item<T>::load(r, at, L.total);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const float u = (static_cast<float>(v[j]) - mu[j]) * rs[j];
+            float dz = static_cast<float>(g[j]);
+            if constexpr (ACT != kActNone) dz *= slope<ACT>(fmaf(u, w[j], bias[j]) + static_cast<float>(q[j]));
+            o[j] = static_cast<T>(rs[j] * (fmaf(w[j], dz, -t1[j]) - u * t2[j]));
+        }
+        Item<T>::store(dx, at, L.total, o);
+    }
+}
+
+template <class T>
+__global__ void __launch_bounds__(256) norm_parameter_kernel(NormBackwardArgs<T> a, const float2* __restrict__ totals, int64_t batch, int channels) {
+    const int c = blockIdx.x * 256 + threadIdx.x;
+    if (c < channels) parameter_sums(a, totals, batch, channels, c);
+}
+
+// ---- numbers of channels that no workgroup's lanes can repeat over (odd and above 1024) --------------------
+// One workgroup per (batch item, group), element by element.
+__device__ __forceinline__ float workgroup_sum(float v, float* lds) {
+    v = sum_over(v, 64);
+    __syncthreads();
+    if (threadIdx.x % 64 == 0) lds[threadIdx.x / 64] = v;
+    __syncthreads();
+    v = 0.0f;
+    for (unsigned i = 0; i < blockDim.x / 64; ++i) v += lds[i];
+    return v;
+}
+
+template <class T, int ACT>
+__global__ void __launch_bounds__(256)
+norm_any_kernel(NormArgs<T> a, float* __restrict__ mean_out, float* __restrict__ rstd_out, int64_t pixels, int channels) {
+    __shared__ float lds[4];
+    const int64_t b = blockIdx.x / a.groups, n = pixels * a.per_group;
+    const int g = blockIdx.x % a.groups;
+    const int64_t base = b * pixels * channels + static_cast<int64_t>(g) * a.per_group;
+    float s = 0.0f;
+    for (int64_t i = threadIdx.x; i < n; i += 256) s += static_cast<float>(a.x[base + i / a.per_group * channels + i % a.per_group]);
+    const float mu = workgroup_sum(s, lds) / static_cast<float>(n);
+    s = 0.0f;
+    for (int64_t i = threadIdx.x; i < n; i += 256) {
+        const float d = static_cast<float>(a.x[base + i / a.per_group * channels + i % a.per_group]) - mu;
+        s = fmaf(d, d, s);
+    }
+    const float rs = 1.0f / sqrtf(workgroup_sum(s, lds) / static_cast<float>(n) + a.eps);
+    if (threadIdx.x == 0 && mean_out != nullptr) {
+        mean_out[blockIdx.x] = mu;
+        rstd_out[blockIdx.x] = rs;
+    }
+    for (int64_t i = threadIdx.x; i < n; i += 256) {
+        const int64_t at = base + i / a.per_group * channels + i % a.per_group;
+        const int c = g * a.per_group + static_cast<int>(i % a.per_group);
+        float z = (static_cast<float>(a.x[at]) - mu) * rs;
+        if (a.weight) z *= load_param<T>(a.weight, a.float_params, c);
+        if (a.bias) z += load_param<T>(a.bias, a.float_params, c);
+        if (a.residual) z += static_cast<float>(a.residual[at]);
+        a.y[at] = static_cast<T>(activate<ACT>(z));
+    }
+}
+
+template <class T, int ACT>
+__device__ __forceinline__ float any_dz(const NormBackwardArgs<T>& a, int64_t at, int c, float u) {
+    float dz = static_cast<float>(a.dy[at]);
+    if constexpr (ACT != kActNone) {
+        float z = u;
+        if (a.weight) z *= load_param<T>(a.weight, a.float_params, c);
+        if (a.bias) z += load_param<T>(a.bias, a.float_params, c);
+        if (a.residual) z += static_cast<float>(a.residual[at]);
+        dz *= slope<ACT>(z);
+    }
+    return dz;
+}
+
+// One workgroup per (batch item, channel).
+template <class T, int ACT>
+__global__ void __launch_bounds__(256)
+norm_any_sums_kernel(NormBackwardArgs<T> a, float2* __restrict__ totals, int64_t pixels, int channels) {
+    __shared__ float lds[4];
+    const int64_t b = blockIdx.x / channels;
+    const int c = blockIdx.x % channels;
+    const int64_t pair = b * a.groups + c / a.per_group;
+    const float mu = a.mean[pair], rs = a.rstd[pair];
+    float s = 0.0f, d = 0.0f;
+    for (int64_t i = threadIdx.x; i < pixels; i += 256) {
+        const int64_t at = (b * pixels + i) * channels + c;
+        const float u = (static_cast<float>(a.x[at]) - mu) * rs, dz = any_dz<T, ACT>(a, at, c, u);
+        s += dz;
+        d = fmaf(dz, u, d);
+        if (a.dresidual) a.dresidual[at] = static_cast<T>(dz);
+    }
+    s = workgroup_sum(s, lds);
+    d = workgroup_sum(d, lds);
+    if (threadIdx.x == 0) totals[blockIdx.x] = {s, d};
+}
+
+template <class T, int ACT>
+__global__ void __launch_bounds__(256)
+norm_any_grad_kernel(NormBackwardArgs<T> a, const float2* __restrict__ totals, int64_t pixels, int channels, float inv_m) {
+    __shared__ float lds[4];
+    const int64_t b = blockIdx.x / a.groups, n = pixels * a.per_group;
+    const int g = blockIdx.x % a.groups;
+    float s1 = 0.0f, s2 = 0.0f;
+    for (int i = threadIdx.x; i < a.per_group; i += 256) {
+        const int c = g * a.per_group + i;
+        const float w = a.weight ? load_param<T>(a.weight, a.float_params, c) : 1.0f;
+        const float2 v = totals[b * channels + c];
+        s1 = fmaf(w, v.x, s1);
+        s2 = fmaf(w, v.y, s2);
+    }
+    s1 = workgroup_sum(s1, lds) * inv_m;
+    s2 = workgroup_sum(s2, lds) * inv_m;
+    const float mu = a.mean[blockIdx.x], rs = a.rstd[blockIdx.x];
+    for (int64_t i = threadIdx.x; i < n; i += 256) {
+        const int c = g * a.per_group + static_cast<int>(i % a.per_group);
+        const int64_t at = (b * pixels + i / a.per_group) * channels + c;
+        const float u = (static_cast<float>(a.x[at]) - mu) * rs, dz = any_dz<T, ACT>(a, at, c, u);
+        const float w = a.weight ? load_param<T>(a.weight, a.float_params, c) : 1.0f;
+        a.dx[at] = static_cast<T>(rs * (fmaf(w, dz, -s1) - u * s2));
+    }
+}
+
+// ---- plans -------------------------------------------------------------------------------------------------
+int gcd(int a, int b) { while (b) { const int r = a % b; a = b; b = r; } return a; }
+
+struct NormPlan {
+    bool any;                  // the element-by-element kernels
+    int small;                 // > 0: one launch, so many vectors per lane
+    int threads, slabs, chunks;
+    int64_t chunk_steps;
+    Lanes L;
+};
+
+constexpr int kMostVectors = 8;        // of a lane of the one-launch kernels: what its registers hold of x
+
+NormPlan plan_norm(int64_t batch, int64_t pixels, int channels, int groups, int V) {
+    NormPlan p = {};
+    Lanes& L = p.L;
+    L.channels = L.slab = channels;
+    L.total = pixels * channels;
+    const int per_group = channels / groups;
+    L.phase = channels / gcd(channels, V);
+    p.slabs = 1;
+    if (L.phase > 1024) {
+        p.any = true;
+        return p;
+    }
+    // one launch where a workgroup of at most 1024 lanes can hold an item, or whole groups of it that are at least 64 bytes
+    // wide (narrower pieces of a pixel's channels would fetch the same cache lines from several workgroups)
+    for (int groups_in_slab = groups; groups_in_slab >= 1; --groups_in_slab) {
+        if (groups % groups_in_slab) continue;
+        const int slab = groups_in_slab * per_group;
+        if (groups_in_slab < groups && (channels % V || slab % V || slab < 4 * V)) continue;
+        const int phase = slab == channels ? L.phase : slab / V;
+        const int64_t vectors = slab == channels ? (L.total + V - 1) / V : pixels * phase;
+        if (phase > 1024 || vectors > static_cast<int64_t>(1024 / phase * phase) * kMostVectors) continue;
+        int threads = 64;
+        while (threads < 1024 && (threads < phase || vectors > threads / phase * phase)) threads *= 2;
+        p.threads = threads;
+        p.slabs = groups / groups_in_slab;
+        L.slab = slab;
+        L.phase = phase;
+        L.active = threads / phase * phase;
+        L.stride = slab == channels ? static_cast<int64_t>(L.active) * V : static_cast<int64_t>(L.active / phase) * channels;
+        int n = 1;
+        while (static_cast<int64_t>(L.active) * n < vectors) n *= 2;
+        p.small = n;
+        return p;
+    }
+    p.threads = 256;
+    while (p.threads < L.phase) p.threads *= 2;
+    if (p.threads < 1024 && p.threads / L.phase * L.phase * 4 < p.threads * 3) p.threads *= 2;   // fewer idle lanes
+    L.active = p.threads / L.phase * L.phase;
+    L.stride = static_cast<int64_t>(L.active) * V;
+    const int64_t steps = (L.total + L.stride - 1) / L.stride;
+    const int64_t want = (2048 * 256 / p.threads + batch - 1) / batch;       // workgroups per item: eight waves per SIMD in all
+    p.chunk_steps = (steps + want - 1) / want;
+    if (p.chunk_steps < kUnroll) p.chunk_steps = kUnroll;
+    p.chunks = static_cast<int>((steps + p.chunk_steps - 1) / p.chunk_steps);
+    return p;
+}
+
+template <int ACT> struct ActTag { static constexpr int value = ACT; };
+template <class F>
+hipError_t with_activation(int act, F f) {
+    switch (act) {
+        case kActRelu: return f(ActTag<kActRelu>());
+        case kActSilu: return f(ActTag<kActSilu>());
+        case kActGelu: return f(ActTag<kActGelu>());
+        default: return f(ActTag<kActNone>());
+    }
+}
+template <int N> struct CountTag { static constexpr int value = N; };
+template <class F>
+hipError_t with_count(int n, F f) {
+    switch (n) {
+        case 1: return f(CountTag<1>());
+        case 2: return f(CountTag<2>());
+        case 4: return f(CountTag<4>());
+        default: return f(CountTag<8>());
+    }
+}
+
+template <class T>
+hipError_t forward(const NormCall& n, void* workspace, hipStream_t stream) {
+    constexpr int V = Vec<T>::kLen;
+    NormArgs<T> a;
+    a.x = static_cast<const T*>(n.x);
+    a.residual = static_cast<const T*>(n.residual);
+    a.weight = n.weight;
+    a.bias = n.bias;
+    a.y = static_cast<T*>(n.y);
+    a.float_params = n.float_params;
+    a.groups = n.groups;
+    a.per_group = n.channels / n.groups;
+    a.eps = n.eps;
+    const NormPlan p = plan_norm(n.batch, n.pixels, n.channels, n.groups, V);
+    const Lanes L = p.L;
+    if (p.any)
+        return with_activation(n.activation, [&](auto act) {
+            BOXCONV_LAUNCH("norm_any", (norm_any_kernel<T, decltype(act)::value>), dim3(static_cast<unsigned>(n.batch * n.groups)), dim3(256), 0, stream, a,
+                           n.mean, n.rstd, n.pixels, n.channels);
+            return hipGetLastError();
+        });
+    if (p.small)
+        return with_activation(n.activation, [&](auto act) {
+            return with_count(p.small, [&](auto count) {
+                const size_t lds = static_cast<size_t>(3) * L.active * V * 4 + static_cast<size_t>(L.slab / a.per_group) * 8;
+                BOXCONV_LAUNCH("norm_small", (norm_small_kernel<T, decltype(act)::value, decltype(count)::value>),
+                               dim3(static_cast<unsigned>(n.batch * p.slabs)), dim3(p.threads), lds, stream, a, n.mean, n.rstd, L, p.slabs);
+                return hipGetLastError();
+            });
+        });
+    float* partial = static_cast<float*>(workspace);
+    float *mean = n.mean, *rstd = n.rstd;
+    const int64_t pairs = n.batch * n.groups;
+    if (mean == nullptr) {
+        mean = partial + n.batch * p.chunks * n.groups * 3;
+        rstd = mean + pairs;
+    }
+    const int workgroups = static_cast<int>(n.batch * p.chunks);
+    BOXCONV_LAUNCH("norm_statistics", (norm_statistics_kernel<T>), dim3(workgroups), dim3(p.threads), static_cast<size_t>(3) * L.active * V * 4, stream, a.x,
+                   partial, L, p.chunk_steps, p.chunks, a.groups, a.per_group);
+    BOXCONV_LAUNCH("norm_join", norm_join_kernel, dim3(static_cast<unsigned>((pairs + 3) / 4)), dim3(256), 0, stream, partial, mean, rstd, pairs, a.groups,
+                   p.chunks, a.eps);
+    return with_activation(n.activation, [&](auto act) {
+        BOXCONV_LAUNCH("norm_apply", (norm_apply_kernel<T, decltype(act)::value>), dim3(workgroups), dim3(p.threads), 0, stream, a, mean, rstd, L,
+                       p.chunk_steps, p.chunks, workgroups);
+        return hipGetLastError();
+    });
+}
+
+template <class T>
+hipError_t backward(const NormGradCall& n, void* workspace, hipStream_t stream) {
+    constexpr int V = Vec<T>::kLen;
+    NormBackwardArgs<T> a;
+    a.x = static_cast<const T*>(n.x);
+    a.residual = static_cast<const T*>(n.residual);
+    a.dy = static_cast<const T*>(n.dy);
+    a.weight = n.weight;
+    a.bias = n.bias;
+    a.mean = n.mean;
+    a.rstd = n.rstd;
+    a.dx = static_cast<T*>(n.dx);
+    a.dresidual = static_cast<T*>(n.dresidual);
+    a.dweight = n.dweight;
+    a.dbias = n.dbias;
+    a.float_params = n.float_params;
+    a.groups = n.groups;
+    a.per_group = n.channels / n.groups;
+    const NormPlan p = plan_norm(n.batch, n.pixels, n.channels, n.groups, V);
+    const Lanes L = p.L;
+    const float inv_m = static_cast<float>(1.0 / (static_cast<double>(n.pixels) * a.per_group));
+    float2* totals = static_cast<float2*>(workspace);
+    float2* partial = totals + n.batch * n.channels;
+    const dim3 param_grid(static_cast<unsigned>((n.channels + 255) / 256));
+    const bool params = n.dweight != nullptr || n.dbias != nullptr;
+    if (p.any)
+        return with_activation(n.activation, [&](auto act) {
+            BOXCONV_LAUNCH("norm_any_sums", (norm_any_sums_kernel<T, decltype(act)::value>), dim3(static_cast<unsigned>(n.batch * n.channels)), dim3(256), 0,
+                           stream, a, totals, n.pixels, n.channels);
+            if (params) BOXCONV_LAUNCH("norm_parameter", (norm_parameter_kernel<T>), param_grid, dim3(256), 0, stream, a, totals, n.batch, n.channels);
+            if (a.dx != nullptr)
+                BOXCONV_LAUNCH("norm_any_grad", (norm_any_grad_kernel<T, decltype(act)::value>), dim3(static_cast<unsigned>(n.batch * n.groups)), dim3(256), 0,
+                               stream, a, totals, n.pixels, n.channels, inv_m);
+            return hipGetLastError();
+        });
+    if (p.small)
+        return with_activation(n.activation, [&](auto act) {
+            const size_t lds = static_cast<size_t>(2) * L.active * V * 4 + static_cast<size_t>(L.slab) * 8 + static_cast<size_t>(L.slab / a.per_group) * 8;
+            BOXCONV_LAUNCH("norm_small_grad", (norm_small_grad_kernel<T, decltype(act)::value>), dim3(static_cast<unsigned>(n.batch * p.slabs)),
+                           dim3(p.threads), lds, stream, a, totals, L, p.slabs, inv_m);
+            if (params) BOXCONV_LAUNCH("norm_parameter", (norm_parameter_kernel<T>), param_grid, dim3(256), 0, stream, a, totals, n.batch, n.channels);
+            return hipGetLastError();
+        });
+    const int workgroups = static_cast<int>(n.batch * p.chunks), tiles = (n.channels + 15) / 16;
+    return with_activation(n.activation, [&](auto act) {
+        BOXCONV_LAUNCH("norm_sums", (norm_sums_kernel<T, decltype(act)::value>), dim3(workgroups), dim3(p.threads), static_cast<size_t>(2) * L.active * V * 4,
+                       stream, a, reinterpret_cast<float*>(partial), L, p.chunk_steps, p.chunks);
+        BOXCONV_LAUNCH("norm_join_sums", norm_join_sums_kernel, dim3(static_cast<unsigned>(n.batch * tiles)), dim3(256), 0, stream, partial, totals,
+                       n.channels, p.chunks, tiles);
+        BOXCONV_LAUNCH("norm_grad", (norm_grad_kernel<T, decltype(act)::value>), dim3(workgroups), dim3(p.threads), static_cast<size_t>(a.groups) * 8, stream,
+                       a, totals, L, p.chunk_steps, p.chunks, n.batch, inv_m, workgroups);
+        return hipGetLastError();
+    });
+}
+
+}  // namespace
+
+size_t norm_workspace_bytes(int64_t batch, int64_t pixels, int channels, int groups, int dtype, bool backward_pass) {
+    const NormPlan p = plan_norm(batch, pixels, channels, groups, dtype == kF32 ? 4 : 8);
+    const int64_t chunks = p.any || p.small ? 0 : batch * p.chunks;
+    if (backward_pass) return static_cast<size_t>(batch * channels + chunks * channels) * 8;
+    return chunks ? static_cast<size_t>(chunks * groups * 3 + batch * groups * 2) * 4 : 0;
+}
+
+hipError_t norm_forward_launch(const NormCall& n, void* workspace, hipStream_t stream) {
+    if (n.dtype == kF32) return forward<float>(n, workspace, stream);
+    if (n.dtype == kF16) return forward<_Float16>(n, workspace, stream);
+    return forward<__bf16>(n, workspace, stream);
+}
+
+hipError_t norm_backward_launch(const NormGradCall& n, void* workspace, hipStream_t stream) {
+    if (n.dtype == kF32) return backward<float>(n, workspace, stream);
+    if (n.dtype == kF16) return backward<_Float16>(n, workspace, stream);
+    return backward<__bf16>(n, workspace, stream);
+}
+
+}  // namespace boxconv

@@ -1,0 +1,282 @@
+// The pointwise product y = act(x W^T + bias + residual) and its gradients for one element type (BOXCONV_INST_T: float,
+// _Float16 or __bf16; compiled once for each).
+#include "linear_tile.hpp"
+
+namespace boxconv {
+
+namespace {
+
+// ---- any shape, alignment and size ---------------------------------------------------------------------------
+// A workgroup of four waves (2 x 2) computes a TX x TX tile; operands go through registers into one LDS buffer with every
+// bound checked, the next tile's loads in flight while this one is multiplied. blockIdx.y: the part of k this workgroup sums.
+template <class T, bool A_K, bool B_K, int TX>
+__global__ void __launch_bounds__(256)
+product_kernel(Operand<T> a, Operand<T> b, Tail<T> tail, int64_t k_part, int64_t tiles_m, int64_t tiles_n) {
+    typedef TileShape<T, A_K, TX> SA;
+    typedef TileShape<T, B_K, TX> SB;
+    constexpr int F = TX / 64;                              // 32 x 32 blocks of a wave along each axis
+    __shared__ Chunk lds[SA::kChunks + SB::kChunks];
+    Chunk *ta = lds, *tb = lds + SA::kChunks;
+    const int64_t m0 = blockIdx.x / tiles_n * TX, n0 = blockIdx.x % tiles_n * TX;
+    const int64_t k_begin = blockIdx.y * k_part, k_end = min(a.depth, k_begin + k_part);
+    const int wave = threadIdx.x / 64, wm = wave / 2 * (TX / 2), wn = wave % 2 * (TX / 2);
+    Acc16 acc[F][F] = {};                                   // [n block][m block]
+    Stage<T, A_K, TX, 256, false> sa;
+    Stage<T, B_K, TX, 256, true> sb;
+    if (k_begin < k_end) {
+        sa.load(a, m0, k_begin, k_end);
+        sb.load(b, n0, k_begin, k_end);
+    }
+    for (int64_t k0 = k_begin; k0 < k_end; k0 += SA::KT) {
+        __syncthreads();
+        sa.store(ta);
+        sb.store(tb);
+        __syncthreads();
+        if (k0 + SA::KT < k_end) {
+            sa.load(a, m0, k0 + SA::KT, k_end);
+            sb.load(b, n0, k0 + SA::KT, k_end);
+        }
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+            Chunk fa[F], fb[F];
+#pragma unroll
+            for (int j = 0; j < F; ++j) {
+                fa[j] = fragment<T, A_K, TX, false>(ta, wm + 32 * j, ks);
+                fb[j] = fragment<T, B_K, TX, true>(tb, wn + 32 * j, ks);
+            }
+#pragma unroll
+            for (int i = 0; i < F; ++i)
+#pragma unroll
+                for (int j = 0; j < F; ++j) acc[i][j] = multiply_add<T>(fb[i], fa[j], acc[i][j]);
+        }
+    }
+    const int l = threadIdx.x % 64;
+#pragma unroll
+    for (int i = 0; i < F; ++i)
+#pragma unroll
+        for (int j = 0; j < F; ++j) {
+            const int64_t m = m0 + wm + 32 * j + l % 32, n = n0 + wn + 32 * i + 16 * (l / 32);
+            float z[16];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) z[r] = acc[i][j][r];
+            if (tail.partial != nullptr) {
+                if (m < tail.rows && n < tail.cols)
+                    store_run<float, 16>(tail.partial + (blockIdx.y * tail.rows + m) * tail.cols + n, z, tail.cols - n);
+            } else {
+                apply_tail<T, 16>(tail, z, m, n);
+            }
+        }
+}
+
+// The parts of a split product, added in their order, and the tail. Eight columns per thread.
+template <class T>
+__global__ void __launch_bounds__(256) join_parts_kernel(Tail<T> tail, int splits, int64_t runs_per_row, int64_t runs) {
+    const int64_t id = blockIdx.x * 256ll + threadIdx.x;
+    if (id >= runs) return;
+    const int64_t m = id / runs_per_row, n = id % runs_per_row * 8;
+    float z[8] = {}, v[8];
+    for (int s = 0; s < splits; ++s) {
+        load_run<float, 8>(tail.partial + (s * tail.rows + m) * tail.cols + n, v, tail.cols - n);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) z[i] += v[i];
+    }
+    apply_tail<T, 8>(tail, z, m, n);
+}
+
+// ---- dz = dy * act'(z), and its column sums ---------------------------------------------------------------------
+// A workgroup takes 256 columns (8 per thread, 32 threads) of a band of rows, 8 rows at a time. sums: [bands][cols], null
+// if not wanted; dz: null if not wanted. kept: y for relu, the kept slope for silu and gelu.
+template <class T>
+__global__ void __launch_bounds__(256)
+slope_kernel(const T* __restrict__ dy, const void* __restrict__ kept, T* __restrict__ dz, float* __restrict__ sums, int64_t rows,
+             int64_t cols, int64_t band, int activation) {
+    typedef typename SlopeOf<T>::Type S;
+    __shared__ float part[8][256];
+    const int64_t n = blockIdx.y * 256ll + threadIdx.x % 32 * 8, first = blockIdx.x * band, last = min(rows, first + band);
+    const int64_t valid = cols - n;
+    float sum[8] = {};
+    for (int64_t m = first + threadIdx.x / 32; m < last; m += 8) {
+        if (valid <= 0) break;
+        T g[8];
+        load_run<T, 8>(dy + m * cols + n, g, valid);
+        float d[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) d[i] = static_cast<float>(g[i]);
+        if (activation == kActRelu) {
+            T y[8];
+            load_run<T, 8>(static_cast<const T*>(kept) + m * cols + n, y, valid);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) d[i] *= slope<kActRelu>(static_cast<float>(y[i]));
+        } else if (activation != kActNone) {
+            S s[8];
+            load_run<S, 8>(static_cast<const S*>(kept) + m * cols + n, s, valid);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) d[i] *= kept_slope(s[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            sum[i] += d[i];
+            g[i] = static_cast<T>(d[i]);
+        }
+        if (dz != nullptr) store_run<T, 8>(dz + m * cols + n, g, valid);
+    }
+    if (sums == nullptr) return;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) part[threadIdx.x / 32][threadIdx.x % 32 * 8 + i] = sum[i];
+    __syncthreads();
+    const int64_t col = blockIdx.y * 256ll + threadIdx.x;
+    if (col < cols) {
+        float s = 0.0f;
+        for (int r = 0; r < 8; ++r) s += part[r][threadIdx.x];
+        sums[blockIdx.x * cols + col] = s;
+    }
+}
+
+// dbias: the bands' sums in their order, 32 columns by 8 rows of threads.
+template <class T>
+__global__ void __launch_bounds__(256) join_bias_kernel(const float* __restrict__ sums, T* __restrict__ dbias, int64_t cols, int bands) {
+    __shared__ float part[8][33];
+    const int64_t c = blockIdx.x * 32ll + threadIdx.x % 32;
+    float s = 0.0f;
+    if (c < cols)
+        for (int i = threadIdx.x / 32; i < bands; i += 8) s += sums[i * cols + c];
+    part[threadIdx.x / 32][threadIdx.x % 32] = s;
+    __syncthreads();
+    if (threadIdx.x < 32 && c < cols) {
+        for (int r = 1; r < 8; ++r) s += part[r][threadIdx.x];
+        dbias[c] = static_cast<T>(s);
+    }
+}
+
+// ---- plans ---------------------------------------------------------------------------------------------------------
+struct ProductPlan {
+    int tile, splits;
+    int64_t k_part, tiles_m, tiles_n;
+    size_t partial_bytes;
+};
+
+template <class T>
+ProductPlan plan_product(int64_t m, int64_t n, int64_t k) {
+    constexpr int KT = 8 * Vec<T>::kLen;
+    ProductPlan p;
+    const int64_t big = ((m + 127) / 128) * ((n + 127) / 128);
+    p.tile = m > 64 && n > 64 && big >= 256 ? 128 : 64;
+    p.tiles_m = (m + p.tile - 1) / p.tile;
+    p.tiles_n = (n + p.tile - 1) / p.tile;
+    const int64_t tiles = std::max<int64_t>(p.tiles_m * p.tiles_n, 1), steps = (k + KT - 1) / KT;
+    int64_t splits = 1;
+    if (tiles < 256) splits = std::min<int64_t>({(512 + tiles - 1) / tiles, (steps + 3) / 4, 256});
+    splits = std::max<int64_t>(splits, 1);
+    const int64_t part = (steps + splits - 1) / splits;
+    p.splits = static_cast<int>(steps == 0 ? 1 : (steps + part - 1) / part);
+    p.k_part = std::max<int64_t>(part, 1) * KT;
+    p.partial_bytes = p.splits > 1 ? static_cast<size_t>(p.splits) * m * n * 4 : 0;
+    return p;
+}
+
+template <class T, bool A_K, bool B_K>
+hipError_t product(const char* name, Operand<T> a, Operand<T> b, Tail<T> tail, float* workspace, hipStream_t stream) {
+    const ProductPlan p = plan_product<T>(tail.rows, tail.cols, a.depth);
+    tail.partial = p.splits > 1 ? workspace : nullptr;
+    const dim3 grid(static_cast<unsigned>(p.tiles_m * p.tiles_n), p.splits);
+    if (p.tile == 128) BOXCONV_LAUNCH(name, (product_kernel<T, A_K, B_K, 128>), grid, dim3(256), 0, stream, a, b, tail, p.k_part, p.tiles_m, p.tiles_n);
+    else BOXCONV_LAUNCH(name, (product_kernel<T, A_K, B_K, 64>), grid, dim3(256), 0, stream, a, b, tail, p.k_part, p.tiles_m, p.tiles_n);
+    if (p.splits > 1) {
+        const int64_t per_row = (tail.cols + 7) / 8, runs = per_row * tail.rows;
+        BOXCONV_LAUNCH("join_parts", (join_parts_kernel<T>), dim3(static_cast<unsigned>((runs + 255) / 256)), dim3(256), 0, stream, tail, p.splits, per_row, runs);
+    }
+    return hipGetLastError();
+}
+
+size_t round_up(size_t v) { return (v + 255) / 256 * 256; }
+
+struct BandPlan { int64_t band; int bands; };
+BandPlan plan_bands(int64_t rows, int64_t cols) {
+    const int64_t across = (cols + 255) / 256;
+    int64_t bands = std::max<int64_t>(1, std::min<int64_t>((1024 + across - 1) / across, (rows + 31) / 32));
+    BandPlan p;
+    p.band = (rows + bands - 1) / bands;
+    p.band = std::max<int64_t>(8, (p.band + 7) / 8 * 8);
+    p.bands = static_cast<int>((rows + p.band - 1) / p.band);
+    return p;
+}
+
+}  // namespace
+
+template <class T>
+size_t linear_forward_workspace(int64_t rows, int64_t K, int64_t N) { return plan_product<T>(rows, N, K).partial_bytes; }
+
+// [dz, unless the residual's gradient holds it][column sums per band][parts of a split product]
+template <class T>
+size_t linear_backward_workspace(int64_t rows, int64_t K, int64_t N) {
+    return round_up(static_cast<size_t>(rows) * N * sizeof(T)) + round_up(static_cast<size_t>(plan_bands(rows, N).bands) * N * 4) +
+           std::max(plan_product<T>(rows, K, N).partial_bytes, plan_product<T>(N, K, rows).partial_bytes);
+}
+
+template <class T>
+hipError_t linear_forward(const LinearCall& c, void* workspace, hipStream_t stream) {
+    const Operand<T> a = {static_cast<const T*>(c.x), c.ld_x, c.rows, c.K};
+    const Operand<T> b = {static_cast<const T*>(c.weight), c.K, c.N, c.K};
+    Tail<T> tail = {};
+    tail.out = static_cast<T*>(c.y);
+    tail.rows = c.rows;
+    tail.cols = c.N;
+    tail.bias = static_cast<const T*>(c.bias);
+    tail.residual = static_cast<const T*>(c.residual);
+    tail.ld_residual = c.ld_residual;
+    tail.slope = static_cast<typename SlopeOf<T>::Type*>(c.slope);
+    tail.activation = c.activation;
+    return product<T, true, true>("linear", a, b, tail, static_cast<float*>(workspace), stream);
+}
+
+template <class T>
+hipError_t linear_backward(const LinearGradCall& c, void* workspace, hipStream_t stream) {
+    char* ws = static_cast<char*>(workspace);
+    T* scratch = reinterpret_cast<T*>(ws);
+    ws += round_up(static_cast<size_t>(c.rows) * c.N * sizeof(T));
+    const BandPlan bands = plan_bands(c.rows, c.N);
+    float* sums = reinterpret_cast<float*>(ws);
+    ws += round_up(static_cast<size_t>(bands.bands) * c.N * 4);
+    float* parts = reinterpret_cast<float*>(ws);
+    const T* dy = static_cast<const T*>(c.dy);
+    const T* dz = dy;
+    T* write = static_cast<T*>(c.dresidual);
+    if (c.activation != kActNone) {
+        if (write == nullptr && (c.dx != nullptr || c.dweight != nullptr)) write = scratch;
+        dz = write;
+    }
+    if (write != nullptr || c.dbias != nullptr) {
+        const dim3 grid(bands.bands, static_cast<unsigned>((c.N + 255) / 256));
+        BOXCONV_LAUNCH("linear_slope", (slope_kernel<T>), grid, dim3(256), 0, stream, dy, c.kept, write, c.dbias ? sums : nullptr, c.rows, c.N, bands.band,
+                       c.activation);
+        if (c.dbias != nullptr)
+            BOXCONV_LAUNCH("join_bias", (join_bias_kernel<T>), dim3(static_cast<unsigned>((c.N + 31) / 32)), dim3(256), 0, stream, sums, static_cast<T*>(c.dbias),
+                           c.N, bands.bands);
+        if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    }
+    Tail<T> tail = {};
+    if (c.dx != nullptr) {
+        tail.out = static_cast<T*>(c.dx);
+        tail.rows = c.rows;
+        tail.cols = c.K;
+        const Operand<T> a = {dz, c.N, c.rows, c.N};
+        const Operand<T> b = {static_cast<const T*>(c.weight), c.K, c.K, c.N};
+        if (const hipError_t e = product<T, true, false>("linear_dx", a, b, tail, parts, stream); e != hipSuccess) return e;
+    }
+    if (c.dweight != nullptr) {
+        tail.out = static_cast<T*>(c.dweight);
+        tail.rows = c.N;
+        tail.cols = c.K;
+        const Operand<T> a = {dz, c.N, c.N, c.rows};
+        const Operand<T> b = {static_cast<const T*>(c.x), c.ld_x, c.K, c.rows};
+        if (const hipError_t e = product<T, false, false>("linear_dweight", a, b, tail, parts, stream); e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
+
+template size_t linear_forward_workspace<BOXCONV_INST_T>(int64_t, int64_t, int64_t);
+template size_t linear_backward_workspace<BOXCONV_INST_T>(int64_t, int64_t, int64_t);
+template hipError_t linear_forward<BOXCONV_INST_T>(const LinearCall&, void*, hipStream_t);
+template hipError_t linear_backward<BOXCONV_INST_T>(const LinearGradCall&, void*, hipStream_t);
+
+}  // namespace boxconv

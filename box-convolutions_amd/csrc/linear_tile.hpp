@@ -1,0 +1,239 @@
+// The tile that the pointwise products share: out[m][n] = sum over k of A(m, k) * B(n, k) by matrix instructions, with both
+// operands staged through LDS.
+//
+// Each operand lies in memory either with k contiguous ("K-major": x and weight in the forward) or with k as its slow index
+// (the weight in dx = dz W, both operands in dW = dz^T x). A K-major operand is staged as rows of 128 bytes of k; the other
+// kind as rows of one k, and its fragments are read transposed (ds_read_b64_tr_b16: 16 lanes read a block of 4 k by 16
+// columns and each ends up with the 4 k of one column), so no operand is ever transposed in memory.
+//
+// B is the first operand of the matrix instruction and A the second: of the 32 x 32 block a lane then holds 16 values of
+// one output row m, and with B's rows taken in the order of `column_of` they are 16 consecutive n: epilogue loads and stores
+// are whole vectors without a pass through LDS.
+#pragma once
+
+#include "activation.hpp"
+#include "boxconv_host.hpp"
+#include "operators_host.hpp"
+
+namespace boxconv {
+
+namespace {
+
+typedef float Acc16 __attribute__((ext_vector_type(16)));
+typedef unsigned Chunk __attribute__((ext_vector_type(4)));            // 16 bytes of an operand
+
+// A chunk of `valid` elements (none where it is <= 0, all where it is >= the vector's length); zeros beyond.
+template <class T>
+__device__ __forceinline__ Chunk load_chunk(const T* p, int64_t valid) {
+    constexpr int V = Vec<T>::kLen;
+    if (valid >= V) return __builtin_bit_cast(Chunk, *reinterpret_cast<const typename Vec<T>::Type*>(p));
+    typename Vec<T>::Type v = {};
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+        if (j < valid) v[j] = p[j];
+    return __builtin_bit_cast(Chunk, v);
+}
+
+// Row of a 32-row block of B that row r of the matrix instruction's result stands for: result element i of lane l is row
+// 8 (i/4) + 4 (l/32) + i%4, which this maps to column 16 (l/32) + i.
+__device__ __forceinline__ int column_of(int r) { return 16 * ((r >> 2) & 1) + 4 * (r >> 3) + (r & 3); }
+
+// Shape of one operand's tile in LDS: X rows (m or n) by KT values of k.
+template <class T, bool K_MAJOR, int X>
+struct TileShape {
+    static constexpr int V = Vec<T>::kLen;
+    static constexpr int KT = 8 * V;                                      // 128 bytes of k
+    static constexpr int kRowChunks = K_MAJOR ? 8 : X / V;                // 16-byte chunks in a row of the tile
+    static constexpr int kRows = K_MAJOR ? X : KT;
+    static constexpr int kChunks = kRows * kRowChunks;
+    // Position of chunk c of row r: exclusive-or with a few bits of r, so that the lanes of one LDS access spread over the
+    // 64 banks. PERM: fragments of B take rows in the order of column_of (bits 1, 2 and 4 of the row vary between
+    // neighbouring lanes), those of A in natural order (bits 1 to 3).
+    template <bool PERM>
+    static __device__ __forceinline__ int place(int r, int c) {
+        if constexpr (K_MAJOR) return r * 8 + (c ^ (PERM ? ((r >> 1) & 3) | ((r >> 2) & 4) : (r >> 1) & 7));
+        else if constexpr (sizeof(T) == 2) return r * kRowChunks + (kRowChunks >= 16 ? c ^ (4 * (r & 3)) : kRowChunks == 8 ? c ^ (2 * (r & 2)) : c);
+        else return r * kRowChunks + (kRowChunks >= 16 ? c ^ (2 * (r & 4)) : c);
+    }
+};
+
+// One operand in memory: element (i, k), i counting m or n. `extent` rows i, `depth` values of k.
+template <class T>
+struct Operand {
+    const T* p;
+    int64_t ld;            // elements from one row of memory to the next
+    int64_t extent, depth;
+};
+
+// The chunks of a tile that one thread stages, through registers and with every bound checked.
+template <class T, bool K_MAJOR, int X, int THREADS, bool PERM>
+struct Stage {
+    typedef TileShape<T, K_MAJOR, X> Shape;
+    static constexpr int N = Shape::kChunks / THREADS;
+    Chunk v[N];
+    static_assert(Shape::kChunks % THREADS == 0, "whole chunks per thread");
+    __device__ __forceinline__ void load(const Operand<T>& o, int64_t i0, int64_t k0, int64_t k_end) {
+#pragma unroll
+        for (int s = 0; s < N; ++s) {
+            const int id = threadIdx.x + s * THREADS, r = id / Shape::kRowChunks, c = id % Shape::kRowChunks;
+            if constexpr (K_MAJOR) {
+                const int64_t i = i0 + r, k = k0 + c * Shape::V;
+                v[s] = load_chunk(o.p + i * o.ld + k, i < o.extent ? k_end - k : 0);
+            } else {
+                const int64_t k = k0 + r, i = i0 + c * Shape::V;
+                v[s] = load_chunk(o.p + k * o.ld + i, k < k_end ? o.extent - i : 0);
+            }
+        }
+    }
+    __device__ __forceinline__ void store(Chunk* tile) const {
+#pragma unroll
+        for (int s = 0; s < N; ++s) {
+            const int id = threadIdx.x + s * THREADS, r = id / Shape::kRowChunks, c = id % Shape::kRowChunks;
+            tile[Shape::template place<PERM>(r, c)] = v[s];
+        }
+    }
+};
+
+// The fragment of 32 rows from `i` on and k step ks (0..3, 16 values of k in 16-bit types, 8 in float).
+template <class T, bool K_MAJOR, int X, bool PERM>
+__device__ __forceinline__ Chunk fragment(const Chunk* tile, int i, int ks) {
+    typedef TileShape<T, K_MAJOR, X> Shape;
+    const int l = threadIdx.x % 64;
+    if constexpr (K_MAJOR) {
+        const int r = i + (PERM ? column_of(l % 32) : l % 32);
+        return tile[Shape::template place<PERM>(r, 2 * ks + l / 32)];
+    } else if constexpr (sizeof(T) == 2) {
+        typedef short Four __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) Four* LdsPtr;
+        // lane s of a group of 16 fetches columns 4 (s%4) .. +3 (in the order of the fragment's rows) of k row s/4
+        const int s = l % 16, q = l / 16, four = 4 * (q & 1) + s % 4;
+        const int col = i + (PERM ? 16 * (four & 1) + 4 * (four >> 1) : 4 * four);
+        const int k = 16 * ks + 8 * (q >> 1) + s / 4;
+        const char* base = reinterpret_cast<const char*>(tile);
+        Four lo, hi;
+        lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(base + Shape::template place<PERM>(k, col / 8) * 16 + col % 8 * 2));
+        hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(base + Shape::template place<PERM>(k + 4, col / 8) * 16 + col % 8 * 2));
+        typedef short Eight __attribute__((ext_vector_type(8)));
+        return __builtin_bit_cast(Chunk, Eight(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7)));
+    } else {
+        const int col = i + (PERM ? column_of(l % 32) : l % 32), k = 8 * ks + 4 * (l / 32);
+        const float* base = reinterpret_cast<const float*>(tile);
+        typedef float Four __attribute__((ext_vector_type(4)));
+        Four v;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = base[Shape::template place<PERM>(k + j, col / 4) * 4 + col % 4];
+        return __builtin_bit_cast(Chunk, v);
+    }
+}
+
+template <class T> __device__ __forceinline__ Acc16 multiply_add(Chunk b, Chunk a, Acc16 c);
+template <> __device__ __forceinline__ Acc16 multiply_add<__bf16>(Chunk b, Chunk a, Acc16 c) {
+    typedef __bf16 Eight __attribute__((ext_vector_type(8)));
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(Eight, b), __builtin_bit_cast(Eight, a), c, 0, 0, 0);
+}
+template <> __device__ __forceinline__ Acc16 multiply_add<_Float16>(Chunk b, Chunk a, Acc16 c) {
+    typedef _Float16 Eight __attribute__((ext_vector_type(8)));
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(Eight, b), __builtin_bit_cast(Eight, a), c, 0, 0, 0);
+}
+template <> __device__ __forceinline__ Acc16 multiply_add<float>(Chunk b, Chunk a, Acc16 c) {
+    typedef float Four __attribute__((ext_vector_type(4)));
+    const Four x = __builtin_bit_cast(Four, b), y = __builtin_bit_cast(Four, a);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[j], y[j], c, 0, 0, 0);
+    return c;
+}
+
+// ---- epilogue ------------------------------------------------------------------------------------------------
+// act'(z) kept for the backward: float, or a 16-bit fixed-point number (value + 1/2 in steps of 2^-15; the derivatives of
+// silu and gelu lie in [-0.13, 1.13]): its error of at most 2^-16 is a thirtieth of a bfloat16's, so the gradients it
+// goes into are rounded once, as they would be from float. 65535 stands for NaN.
+template <class T> struct SlopeOf { typedef uint16_t Type; };
+template <> struct SlopeOf<float> { typedef float Type; };
+__device__ __forceinline__ void keep_slope(float d, float& o) { o = d; }
+__device__ __forceinline__ void keep_slope(float d, uint16_t& o) {
+    o = d != d ? 65535 : static_cast<uint16_t>(static_cast<int>(rintf(fmaf(d, 32768.0f, 16384.0f))));
+}
+__device__ __forceinline__ float kept_slope(float v) { return v; }
+__device__ __forceinline__ float kept_slope(uint16_t v) { return v == 65535 ? __builtin_nanf("") : fmaf(static_cast<float>(v), 1.0f / 32768.0f, -0.5f); }
+
+// What becomes of a sum: y = act(sum + bias[n] + residual[m][n]). Null pointers leave their piece out.
+template <class T>
+struct Tail {
+    T* out;
+    int64_t rows, cols;
+    const T *bias, *residual;
+    int64_t ld_residual;
+    typename SlopeOf<T>::Type* slope;
+    int activation;
+    float* partial;            // split products: the sums go here as they are, [split][rows][cols]
+};
+
+template <class T, int ACT, int LEN>
+__device__ __forceinline__ void finish(float (&z)[LEN], T (&y)[LEN], typename SlopeOf<T>::Type (&d)[LEN], bool want_slope) {
+#pragma unroll
+    for (int i = 0; i < LEN; ++i) {
+        y[i] = static_cast<T>(activate<ACT>(z[i]));
+        if (want_slope) keep_slope(slope<ACT>(z[i]), d[i]);
+    }
+}
+
+// LEN consecutive elements of a row to or from memory, `valid` of them.
+template <class E, int LEN>
+__device__ __forceinline__ void load_run(const E* p, E (&v)[LEN], int64_t valid) {
+    if (valid >= LEN) {
+        typedef E Packed __attribute__((ext_vector_type(LEN), aligned(sizeof(E))));
+        const Packed q = *reinterpret_cast<const Packed*>(p);
+#pragma unroll
+        for (int i = 0; i < LEN; ++i) v[i] = q[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < LEN; ++i) v[i] = i < valid ? p[i] : E(0);
+    }
+}
+template <class E, int LEN>
+__device__ __forceinline__ void store_run(E* p, const E (&v)[LEN], int64_t valid) {
+    if (valid >= LEN) {
+        typedef E Packed __attribute__((ext_vector_type(LEN), aligned(sizeof(E))));
+        Packed q;
+#pragma unroll
+        for (int i = 0; i < LEN; ++i) q[i] = v[i];
+        *reinterpret_cast<Packed*>(p) = q;
+    } else {
+#pragma unroll
+        for (int i = 0; i < LEN; ++i)
+            if (i < valid) p[i] = v[i];
+    }
+}
+
+// The tail of LEN consecutive sums of row m from column n on.
+template <class T, int LEN>
+__device__ __forceinline__ void apply_tail(const Tail<T>& t, float (&z)[LEN], int64_t m, int64_t n) {
+    typedef typename SlopeOf<T>::Type S;
+    if (m >= t.rows || n >= t.cols) return;
+    const int64_t valid = t.cols - n;
+    T v[LEN];
+    if (t.bias != nullptr) {
+        load_run<T, LEN>(t.bias + n, v, valid);
+#pragma unroll
+        for (int i = 0; i < LEN; ++i) z[i] += static_cast<float>(v[i]);
+    }
+    if (t.residual != nullptr) {
+        load_run<T, LEN>(t.residual + m * t.ld_residual + n, v, valid);
+#pragma unroll
+        for (int i = 0; i < LEN; ++i) z[i] += static_cast<float>(v[i]);
+    }
+    S d[LEN];
+    const bool keep = t.slope != nullptr;
+    switch (t.activation) {
+        case kActRelu: finish<T, kActRelu, LEN>(z, v, d, false); break;
+        case kActSilu: finish<T, kActSilu, LEN>(z, v, d, keep); break;
+        case kActGelu: finish<T, kActGelu, LEN>(z, v, d, keep); break;
+        default: finish<T, kActNone, LEN>(z, v, d, false);
+    }
+    store_run<T, LEN>(t.out + m * t.cols + n, v, valid);
+    if (keep) store_run<S, LEN>(t.slope + m * t.cols + n, d, valid);
+}
+
+}  // namespace
+
+}  // namespace boxconv

@@ -325,6 +325,65 @@ int boxconv_clip_reparametrize_f64(double* x_min, double* x_max, double* y_min, 
                                    double reparametrization_w, double max_input_h,
                                    double max_input_w, int exact, void* stream);
 
+/* ---- operators around a box convolution ---------------------------------------------------------
+ * No counterpart in the reference's native module: what a network puts before and after a box
+ * convolution (1 x 1 convolution, norm, residual add, activation; BottleneckBoxConv,
+ * examples/Cityscapes/models/ENet.py:282-304), on channels-last data, with gradients. Element types
+ * `dtype`: BOXCONV_F32, BOXCONV_F16, BOXCONV_BF16; sums, statistics and everything in between is
+ * float32. NaN and infinities go through as in the formulas.
+ *
+ * Activations. relu: its derivative is 0 at 0. gelu: z times the normal distribution function. */
+#define BOXCONV_ACT_NONE 0
+#define BOXCONV_ACT_RELU 1
+#define BOXCONV_ACT_SILU 2
+#define BOXCONV_ACT_GELU 3
+
+/* Group norm: input, residual, output [batch][pixels][channels] (channels contiguous). Per batch
+ * item and group of channels / groups channels, over pixels * channels / groups values:
+ *   u = (x - mean) / sqrt(variance + eps),   y = act(u * weight[c] + bias[c] + residual)
+ * weight, bias [channels] of type param_dtype (BOXCONV_F32, or that of the input); null: 1, 0.
+ * residual may be null. mean, rstd [batch][groups] float receive the statistics that the backward
+ * takes (both null where there is none). Any address of a whole element will do. output may be input or residual itself.
+ * The workspace (boxconv_group_norm_workspace_bytes; 0 for small items) is 16-byte aligned. */
+size_t boxconv_group_norm_workspace_bytes(int64_t batch, int64_t pixels, int channels, int groups,
+                                          int dtype, int backward);
+int boxconv_group_norm_forward(const void* input, const void* weight, const void* bias, int param_dtype,
+                               const void* residual, void* output, float* mean, float* rstd, int dtype,
+                               int64_t batch, int64_t pixels, int channels, int groups, float eps,
+                               int activation, void* workspace, size_t workspace_bytes, void* stream);
+/* Its gradients; those whose pointer is null are not formed. grad_weight and grad_bias have
+ * param_dtype. All other arguments as in the forward call. */
+int boxconv_group_norm_backward(const void* input, const void* weight, const void* bias, int param_dtype,
+                                const void* residual, const void* grad_output, const float* mean,
+                                const float* rstd, void* grad_input, void* grad_weight, void* grad_bias,
+                                void* grad_residual, int dtype, int64_t batch, int64_t pixels, int channels,
+                                int groups, int activation, void* workspace, size_t workspace_bytes,
+                                void* stream);
+
+/* Pointwise product (a linear layer; a 1 x 1 convolution with rows = batch * h * w):
+ *   y = act(x W^T + bias + residual)
+ * input [rows][in_features], rows ld_input elements apart; weight [out_features][in_features];
+ * bias [out_features], null: 0; residual [rows][out_features], rows ld_residual apart, null: 0;
+ * output [rows][out_features]. All of type dtype, at any address of a whole element.
+ * slope: null, or for silu and gelu [rows][out_features] elements that receive act' for the backward
+ * (float32 for BOXCONV_F32, else 16 bits each: act' + 1/2 in steps of 2^-15, 65535 for NaN).
+ * The workspace (boxconv_linear_workspace_bytes; may be 0) is 16-byte aligned. */
+size_t boxconv_linear_workspace_bytes(int64_t rows, int64_t in_features, int64_t out_features, int dtype,
+                                      int backward);
+int boxconv_linear_forward(const void* input, int64_t ld_input, const void* weight, const void* bias,
+                           const void* residual, int64_t ld_residual, void* output, void* slope, int dtype,
+                           int64_t rows, int64_t in_features, int64_t out_features, int activation,
+                           void* workspace, size_t workspace_bytes, void* stream);
+/* Its gradients; those whose pointer is null are not formed. With dz = grad_output * act':
+ * grad_input = dz W, grad_weight = dz^T x, grad_bias = column sums of dz, grad_residual = dz.
+ * kept: the forward's output for relu, its slope for silu and gelu, null for none. The products are
+ * taken of dz rounded to dtype. */
+int boxconv_linear_backward(const void* input, int64_t ld_input, const void* weight, const void* grad_output,
+                            const void* kept, void* grad_input, void* grad_weight, void* grad_bias,
+                            void* grad_residual, int dtype, int64_t rows, int64_t in_features,
+                            int64_t out_features, int activation, void* workspace, size_t workspace_bytes,
+                            void* stream);
+
 #ifdef __cplusplus
 }
 #endif

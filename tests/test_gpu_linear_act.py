@@ -1,0 +1,251 @@
+"""``linear_act`` and ``PointwiseConv2d`` against the product in 64 bits (tests/operator_reference.py derives the
+bounds), at sizes, strides, alignments and values where tiles, vectors and splits end."""
+import pytest
+import torch
+
+import operator_reference as ref
+
+pytestmark = pytest.mark.gpu
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+ACTS = [None, "relu", "silu", "gelu"]
+
+
+def make(shape, gen, dtype, scale=1.0):
+    return (torch.randn(shape, generator=gen, dtype=torch.float64) * scale).to(dtype)
+
+
+def run(x, weight, bias, residual, name, grad, like=None):
+    """Host tensors in, {output: device tensor} out; `like` makes the device tensor of a host tensor (default: a copy)."""
+    from box_convolution import linear_act
+    like = like or (lambda t: t.cuda())
+    dev = {k: like(t).detach().requires_grad_(grad is not None) for k, t in
+           (("x", x), ("weight", weight), ("bias", bias), ("residual", residual)) if t is not None}
+    y = linear_act(dev["x"], dev["weight"], dev.get("bias"), residual=dev.get("residual"), activation=name)
+    out = {"y": y}
+    if grad is not None:
+        out.update(zip(dev, torch.autograd.grad(y, list(dev.values()), like(grad))))
+    return out
+
+
+def case(M, K, N, dtype, name, bias=True, residual=False, seed=0, train=True):
+    gen = torch.Generator().manual_seed(seed + 7 * M + 11 * K + 13 * N)
+    x, weight = make((M, K), gen, dtype), make((N, K), gen, dtype, max(K, 1) ** -0.5)
+    b = make((N,), gen, dtype) if bias else None
+    r = make((M, N), gen, dtype) if residual else None
+    g = make((M, N), gen, dtype) if train else None
+    return x, weight, b, r, name, g
+
+
+def expected(x, weight, b, r, name, g, dtype):
+    d = [None if t is None else t.double() for t in (x, weight, b, r)]
+    return ref.linear(*d, name, None if g is None else g.double(), dtype)
+
+
+SIZES = [(1, 1, 1), (1, 64, 64), (2, 8, 200), (3, 5, 7), (16, 128, 32), (17, 1000, 24), (63, 65, 64), (65, 63, 66), (128, 128, 128),
+         (129, 130, 257), (200, 32, 128), (257, 100, 60), (1000, 40, 8), (1, 333, 517), (16, 2048, 256), (300, 8, 16), (4099, 33, 129),
+         (5000, 128, 32), (2048, 16, 16), (700, 520, 264), (33, 24, 1030), (1, 4096, 40), (8, 72, 1024)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("i", range(len(SIZES)))
+def test_sizes(hip, i, dtype):
+    """Every size with one activation (another for each type) and every second with a residual, forward and backward."""
+    M, K, N = SIZES[i]
+    args = case(M, K, N, dtype, ACTS[(i + TYPES.index(dtype)) % 4], bias=i % 3 != 2, residual=i % 2 == 1)
+    ref.check(run(*args), expected(*args, dtype))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("name", ACTS)
+@pytest.mark.parametrize("bias,residual", [(False, False), (True, True)])
+def test_epilogues(hip, name, bias, residual, dtype):
+    for M, K, N in ((130, 72, 136), (7, 72, 136), (3000, 64, 48)):
+        args = case(M, K, N, dtype, name, bias, residual, seed=5)
+        ref.check(run(*args), expected(*args, dtype))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_large_products(hip, dtype):
+    """Tiles of the wide kernels, whole ones and a rest on every side, and a long sum."""
+    for M, K, N in ((640, 512, 768), (1030, 584, 1096), (264, 8200, 256)):
+        args = case(M, K, N, dtype, "silu", residual=True)
+        ref.check(run(*args), expected(*args, dtype))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,K,N", [(70, 40, 72), (3000, 64, 32), (520, 256, 512), (5, 136, 264)])
+def test_rows_apart_and_any_address(hip, M, K, N, dtype):
+    """Inputs inside larger tensors that hold NaN around them: nothing outside is used, at addresses of one element."""
+    args = case(M, K, N, dtype, "gelu", residual=True, seed=3)
+    for shift in (0, 1):
+        def inside(t):
+            if t.dim() == 1:
+                big = torch.full((t.numel() + 2,), float("nan"), dtype=t.dtype, device="cuda")
+                view = big[shift:shift + t.numel()]
+            else:
+                big = torch.full((t.size(0) + 2, t.size(1) + 8), float("nan"), dtype=t.dtype, device="cuda")
+                view = big[1:1 + t.size(0), shift * 3:shift * 3 + t.size(1)]
+            view.copy_(t)
+            return view
+        ref.check(run(*args, like=inside), expected(*args, dtype))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_layouts_that_are_copied_or_broadcast(hip, dtype):
+    from box_convolution import linear_act
+    gen = torch.Generator().manual_seed(1)
+    x, w = make((48, 33), gen, dtype).cuda(), make((33, 20), gen, dtype).cuda()
+    plain = linear_act(x, w.t().contiguous())
+    assert torch.equal(linear_act(x.t().contiguous().t(), w.t()), plain)
+    assert torch.equal(linear_act(x.view(4, 3, 4, 33), w.t()), plain.view(4, 3, 4, 20))
+    row = x[:1].expand(300, 33).detach().requires_grad_(True)          # rows 0 elements apart
+    one = x[:1].repeat(300, 1).requires_grad_(True)
+    g = make((300, 20), gen, dtype).cuda()
+    assert torch.equal(linear_act(row, w.t()), linear_act(one, w.t()))
+    assert torch.equal(torch.autograd.grad(linear_act(row, w.t()), row, g)[0], torch.autograd.grad(linear_act(one, w.t()), one, g)[0])
+    # a broadcast gradient (of a sum) and a single vector as input
+    w2 = w.t().contiguous().requires_grad_(True)
+    a = torch.autograd.grad(linear_act(x, w2, activation="silu").sum(), w2)[0]
+    b = torch.autograd.grad(linear_act(x, w2, activation="silu"), w2, torch.ones(48, 20, dtype=dtype, device="cuda"))[0]
+    assert torch.equal(a, b)
+    assert torch.equal(linear_act(x[0], w2), linear_act(x[:1], w2)[0])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_empty(hip, dtype):
+    for M, K, N in ((0, 5, 7), (4, 0, 6), (4, 5, 0), (0, 0, 0)):
+        args = case(M, K, N, dtype, "gelu", residual=True)
+        ref.check(run(*args), expected(*args, dtype))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,K,N", [(40, 40, 40), (2000, 64, 32), (600, 264, 520), (4, 512, 96)])
+def test_nan_and_infinity_stay_in_their_row_and_column(hip, M, K, N, dtype):
+    x, w, b, _, _, g = case(M, K, N, dtype, None)
+    x[1, 3], x[2, 0], w[5, 1] = float("nan"), float("inf"), float("-inf")
+    with torch.no_grad():
+        out = run(x, w, b, None, None, None)["y"].double().cpu()
+    z = x.double() @ w.double().t() + b.double()
+    assert torch.equal(out.isnan(), z.isnan()) and torch.equal(out.isinf(), z.isinf())
+    # a NaN in the gradient stays in its row of dx and its row of dweight
+    g[2, 4] = float("nan")
+    out = run(*case(M, K, N, dtype, None)[:5], g)
+    assert out["x"].isnan().any(1).nonzero().flatten().tolist() == [2]
+    assert out["weight"].isnan().any(1).nonzero().flatten().tolist() == [4]
+    assert out["bias"].isnan().nonzero().flatten().tolist() == [4]
+    for name in ("relu", "silu", "gelu"):                              # and one in z reaches the gradients
+        x, w, b, _, _, g = case(M, K, N, dtype, name)
+        x[1, 3] = float("nan")
+        out = run(x, w, b, None, name, g)
+        assert out["y"][1].isnan().all() and not out["y"][0].isnan().any()
+        if name != "relu":                                             # (no comparison with NaN is true: relu's derivative is 0 there)
+            assert out["x"][1].isnan().all()
+
+
+@pytest.mark.parametrize("name", [None, "silu", "gelu"])
+def test_gradients_against_differences(hip, name):
+    """Central differences of the operator itself along a random direction. Bounds: the forward's own error over the
+    step, and the change of the 64-bit quotient when the step is doubled (three times a step's truncation error where the
+    function is smooth: relu, whose kinks a step crosses, is held to its formula alone)."""
+    M, K, N, h = 37, 45, 29, 2.0 ** -7
+    x, w, b, r, _, g = case(M, K, N, torch.float32, name, residual=True, seed=9)
+    grads = run(x, w, b, r, name, g)
+    base = {"x": x, "weight": w, "bias": b, "residual": r}
+    gen = torch.Generator().manual_seed(2)
+    for which in base:
+        v = torch.randn(base[which].shape, generator=gen)
+
+        def loss(step, exact):
+            t = dict(base)
+            t[which] = t[which].double() + step * v.double() if exact else (t[which].double() + step * v.double()).float()
+            if exact:
+                y = ref.linear(*[t[k].double() for k in base], name, None, torch.float32)["y"][0]
+            else:
+                y = run(t["x"], t["weight"], t["bias"], t["residual"], name, None)["y"].double().cpu()
+            return (y * g.double()).sum().item()
+        quotient = (loss(h, False) - loss(-h, False)) / (2 * h)
+        exact = [(loss(s, True) - loss(-s, True)) / (2 * s) for s in (h, 2 * h)]
+        bound = (ref.linear(*[t.double() for t in base.values()], name, None, torch.float32)["y"][1] * g.double().abs()).sum().item()
+        rounding = 2.0 ** -24 * (base[which].double().abs() * grads[which].double().cpu().abs()).sum().item()
+        got = (grads[which].double().cpu() * v.double()).sum().item()
+        assert abs(got - quotient) <= 2 * (bound + rounding) / h + 2 * abs(exact[1] - exact[0]) + 1e-6 * abs(got), which
+
+
+def test_only_what_is_needed(hip):
+    from box_convolution import linear_act
+    gen = torch.Generator().manual_seed(4)
+    x, w, b, r, g = (make(s, gen, torch.bfloat16).cuda() for s in ((50, 24), (40, 24), (40,), (50, 40), (50, 40)))
+    for name in ACTS:
+        full = [t.detach().requires_grad_(True) for t in (x, w, b, r)]
+        whole = torch.autograd.grad(linear_act(full[0], full[1], full[2], full[3], name), full, g)
+        for i in range(4):
+            some = [t.detach().requires_grad_(i == k) for k, t in enumerate((x, w, b, r))]
+            assert torch.equal(torch.autograd.grad(linear_act(*some, name), some[i], g)[0], whole[i])
+
+
+def test_another_stream_and_same_bits(hip):
+    """The same call on a stream of its own, twice: the same bits everywhere (no order of additions is left open)."""
+    args = case(3000, 96, 72, torch.bfloat16, "silu", residual=True)
+    first = run(*args)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        second = run(*args)
+    side.synchronize()
+    for k in first:
+        assert torch.equal(first[k], second[k]), k
+
+
+def test_graph_replays(hip):
+    x, w, b, r, _, g = (t.cuda() if torch.is_tensor(t) else t for t in case(600, 72, 40, torch.float16, "gelu", residual=True))
+
+    def step():
+        y, kept = hip.linear_forward(x, w, b, r, "gelu", True)
+        return [y] + hip.linear_backward(x, w, kept, "gelu", g, (True,) * 4)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for k in range(3):
+        x.copy_(x.roll(k + 1, 0))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in captured]
+        for a, e in zip(got, step()):
+            assert torch.equal(a, e)
+
+
+def test_pointwise_conv(hip):
+    """The module is the 1 x 1 convolution of its parameters, on channels-last images and on others."""
+    from box_convolution import PointwiseConv2d
+    torch.manual_seed(3)
+    module = PointwiseConv2d(24, 40, activation="relu").cuda()
+    plain = torch.nn.Conv2d(24, 40, 1)
+    plain.load_state_dict(module.state_dict())
+    x, r = torch.randn(2, 24, 9, 13), torch.randn(2, 40, 9, 13)
+    e = ref.linear(x.double().permute(0, 2, 3, 1).reshape(-1, 24), plain.weight.detach().double().flatten(1), plain.bias.detach().double(),
+                   r.double().permute(0, 2, 3, 1).reshape(-1, 40), "relu", None, torch.float32)
+    for layout in (torch.channels_last, torch.contiguous_format):
+        y = module(x.cuda().to(memory_format=layout), r.cuda().to(memory_format=layout))
+        assert y.shape == r.shape and y.is_contiguous(memory_format=torch.channels_last)
+        ref.check({"y": y.permute(0, 2, 3, 1)}, e)
+
+
+def test_refusals(hip):
+    from box_convolution import PointwiseConv2d, linear_act
+    x, w = torch.zeros(4, 8, device="cuda"), torch.zeros(6, 8, device="cuda")
+    for bad, match in ((lambda: linear_act(x, w[:, :7]), "weight"), (lambda: linear_act(x, w[0]), "weight"),
+                       (lambda: linear_act(x, w.half()), "weight"), (lambda: linear_act(x, w.cpu()), "weight"),
+                       (lambda: linear_act(x, w, torch.zeros(5, device="cuda")), "bias"),
+                       (lambda: linear_act(x, w, torch.zeros(6, device="cuda", dtype=torch.bfloat16)), "bias"),
+                       (lambda: linear_act(x, w, residual=torch.zeros(1, 6, device="cuda")), "residual"),
+                       (lambda: linear_act(x.double(), w.double()), "float32, float16 or bfloat16"),
+                       (lambda: linear_act(x, w, activation="tanh"), "activation"),
+                       (lambda: linear_act(x.cpu(), w), "AMD GPUs only"),
+                       (lambda: PointwiseConv2d(3, 4, activation="tanh"), "activation"),
+                       (lambda: PointwiseConv2d(3, 4).cuda()(torch.zeros(3, 5, 5, device="cuda")), "4 dimensions")):
+        with pytest.raises(RuntimeError, match=match):
+            bad()
