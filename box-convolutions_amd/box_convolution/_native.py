@@ -132,6 +132,9 @@ def glue():
                 "boxconv_backward_f64", "boxconv_training_forward_half_f32", "boxconv_backward_half_f32",
                 "boxconv_integral_image_workspace_bytes", "boxconv_backward_workspace_bytes",
                 "boxconv_last_error")])
+            module.init_operators(*[ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
+                "boxconv_group_norm_workspace_bytes", "boxconv_group_norm_forward", "boxconv_group_norm_backward",
+                "boxconv_linear_workspace_bytes", "boxconv_linear_forward", "boxconv_linear_backward")])
             _glue = module
     return _glue or None
 

@@ -48,9 +48,14 @@ def group_norm_act(input, num_groups, weight=None, bias=None, residual=None, act
     residual:   same shape and type as ``input``, added before the activation.
     activation: ``None``, ``"relu"``, ``"silu"`` or ``"gelu"``.
     """
+    act = _native._activation(activation)
     _native._require_device(input, "group norm input")
+    glue = _native.glue()
+    if glue is not None:
+        # checks, allocations and the autograd node in C++ (csrc/operators_glue.hpp): what follows, with less host time
+        with _native._on_device(input.device):
+            return glue.group_norm_act(input, num_groups, weight, bias, residual, act, eps, _native._stream(input.device) or 0)
     _native._operator_dtype(input, "group norm input")
-    _native._activation(activation)
     if input.dim() < 2:
         raise RuntimeError("box_convolution: group norm input must have >=2 dimensions")
     if num_groups < 1 or input.size(1) < 1 or input.size(1) % num_groups != 0:
@@ -99,9 +104,13 @@ def linear_act(input, weight, bias=None, residual=None, activation=None):
     weight:     ``[N, K]``; bias ``[N]``; residual ``[..., N]``, added before the activation: all of the input's type.
     activation: ``None``, ``"relu"``, ``"silu"`` or ``"gelu"``.
     """
+    act = _native._activation(activation)
     _native._require_device(input, "linear input")
+    glue = _native.glue()
+    if glue is not None:                               # as in group_norm_act
+        with _native._on_device(input.device):
+            return glue.linear_act(input, weight, bias, residual, act, _native._stream(input.device) or 0)
     _native._operator_dtype(input, "linear input")
-    _native._activation(activation)
     if input.dim() < 1 or weight.dim() != 2 or weight.size(1) != input.size(-1):
         raise RuntimeError("box_convolution: linear needs an input [..., K] and a weight [N, K], got %s and %s"
                            % (tuple(input.shape), tuple(weight.shape)))

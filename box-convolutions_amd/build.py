@@ -76,6 +76,7 @@ def _stale(target, deps):
 
 
 GLUE_SRC = os.path.join(CSRC, "torch_glue.cpp")
+GLUE_HEADER = os.path.join(CSRC, "operators_glue.hpp")
 GLUE_PATH = os.path.join(HERE, "box_convolution", "_boxconv_glue.so")
 
 
@@ -83,7 +84,7 @@ def build_glue(force=False, verbose=True):
     """The C++ autograd node of the training step (csrc/torch_glue.cpp): a Python extension module
     compiled with g++ against the installed torch's headers. It holds no kernels and does not link
     to libboxconv_hip.so (it is handed that library's entry points as addresses at start-up)."""
-    if not (force or _stale(GLUE_PATH, [GLUE_SRC, os.path.abspath(__file__)])):
+    if not (force or _stale(GLUE_PATH, [GLUE_SRC, GLUE_HEADER, os.path.abspath(__file__)])):
         return GLUE_PATH
     import sysconfig
     import torch

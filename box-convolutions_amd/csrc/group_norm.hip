@@ -35,6 +35,8 @@ struct Item {
     static __device__ __forceinline__ int64_t offset(const Lanes& L, int t, int c0) {
         return static_cast<int64_t>(t / L.phase) * (L.slab == L.channels ? L.phase * V : L.channels) + c0 + (t % L.phase) * V;
     }
+    // Channel of its first element.
+    static __device__ __forceinline__ int channel(const Lanes& L, int t, int c0) { return (c0 + t % L.phase * V) % L.channels; }
     // Elements [off, off + V) of an item of `total`: V of them, fewer at its end, zeros beyond it.
     static __device__ __forceinline__ Packed load(const T* p, int64_t off, int64_t total) {
         if (off + V <= total) return *reinterpret_cast<const Packed*>(p + off);
@@ -50,6 +52,19 @@ struct Item {
         }
         for (int j = 0; j < V; ++j)
             if (off + j < total) p[off + j] = v[j];
+    }
+};
+
+// The channel and group of a lane's elements one after the other (divisions take dozens of instructions, a step three).
+struct Walk {
+    int c, g, rest;       // channel, its group, its place in the group
+    __device__ __forceinline__ Walk(int channel, int per_group) : c(channel), g(channel / per_group), rest(channel - g * per_group) {}
+    __device__ __forceinline__ void next(int channels, int per_group) {
+        if (++rest == per_group) {
+            rest = 0;
+            ++g;
+        }
+        if (++c == channels) c = g = rest = 0;
     }
 };
 
@@ -83,27 +98,31 @@ __device__ __forceinline__ void join_statistics(const float (&mean)[V], const fl
         }
     }
     __syncthreads();
-    // slots t*V + j with (t % phase)*V + j = c (mod slab) hold channel c: slot c + slab*k for every k
-    const int groups = L.slab / per_group, width = lanes_per_group(blockDim.x, groups), per_channel = slots / L.slab;
+    // slots t*V + j with (t % phase)*V + j = c (mod slab) hold channel c: slot c + slab*k for every k. A group's `width` lanes
+    // share its channels, `across` at a time, and where there are fewer of those the k
+    const int groups = L.slab / per_group, width = lanes_per_group(blockDim.x, groups);
+    int across = width;
+    while (across > per_group) across >>= 1;
+    const int first = t % width % across, row = t % width / across * L.slab, step = width / across * L.slab;
     for (int g0 = 0; g0 < groups; g0 += blockDim.x / width) {
         const int g = g0 + t / width;
         const bool live = g < groups;
         float n = 0.0f, sum = 0.0f;
         if (live)
-            for (int i = t % width; i < per_group * per_channel; i += width) {
-                const int s = g * per_group + i % per_group + L.slab * (i / per_group);
-                n += sn[s];
-                sum = fmaf(sn[s], smean[s], sum);
-            }
+            for (int c = first; c < per_group; c += across)
+                for (int s = g * per_group + c + row; s < slots; s += step) {
+                    n += sn[s];
+                    sum = fmaf(sn[s], smean[s], sum);
+                }
         n = sum_over(n, width);
         const float mu = n > 0.0f ? sum_over(sum, width) / n : 0.0f;
         float dev = 0.0f;
         if (live)
-            for (int i = t % width; i < per_group * per_channel; i += width) {
-                const int s = g * per_group + i % per_group + L.slab * (i / per_group);
-                const float d = smean[s] - mu;
-                dev += sm2[s] + sn[s] * d * d;
-            }
+            for (int c = first; c < per_group; c += across)
+                for (int s = g * per_group + c + row; s < slots; s += step) {
+                    const float d = smean[s] - mu;
+                    dev += sm2[s] + sn[s] * d * d;
+                }
         dev = sum_over(dev, width);
         if (live && t % width == 0) put(g, n, mu, dev);
     }
@@ -133,17 +152,18 @@ __device__ __forceinline__ void join_channels(const float (&a)[V], const float (
 }
 
 // ---- statistics of large items: partial results per workgroup --------------------------------------
-// partial[(b * chunks + chunk) * groups + g] = (count, mean, sum of squared deviations). Every batch of kUnroll vectors is
+// partial[(b * groups + g) * chunks + chunk] = (mean, sum of squared deviations) of a chunk of whole pixels. Every batch of kUnroll vectors is
 // reduced around its own mean and joined to the lane's running one (the formula of Chan, Golub and LeVeque), so the sums
 // are as good for a channel with a large mean as for one without.
 template <class T>
 __global__ void __launch_bounds__(1024)
-norm_statistics_kernel(const T* __restrict__ x, float* __restrict__ partial, Lanes L, int64_t chunk_steps, int chunks,
+norm_statistics_kernel(const T* __restrict__ x, float2* __restrict__ partial, Lanes L, int64_t chunk_steps, int chunks,
                        int groups, int per_group) {
     constexpr int V = Vec<T>::kLen;
     extern __shared__ float lds[];
     const int t = threadIdx.x;
-    const int64_t b = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
+    const unsigned chunk = blockIdx.x % static_cast<unsigned>(chunks);
+    const int64_t b = blockIdx.x / static_cast<unsigned>(chunks);
     const T* item = x + b * L.total;
     float mean[V], m2[V], count[V];
 #pragma unroll
@@ -188,38 +208,49 @@ norm_statistics_kernel(const T* __restrict__ x, float* __restrict__ partial, Lan
             }
         }
     }
-    float* out = partial + blockIdx.x * static_cast<int64_t>(groups) * 3;
-    join_statistics<V>(mean, m2, count, lds, L, per_group, [&](int g, float n, float mu, float dev) {
-        out[3 * g] = n;
-        out[3 * g + 1] = mu;
-        out[3 * g + 2] = dev;
-    });
+    float2* out = partial + b * groups * chunks + chunk;
+    join_statistics<V>(mean, m2, count, lds, L, per_group, [&](int g, float, float mu, float dev) { out[static_cast<int64_t>(g) * chunks] = {mu, dev}; });
 }
 
-// One wave per (batch item, group): the partial results of all its workgroups, in their order.
+// Sum over a workgroup of 256.
+__device__ __forceinline__ float sum_of_workgroup(float v, float* lds) {
+    v = sum_over(v, 64);
+    __syncthreads();
+    if (threadIdx.x % 64 == 0) lds[threadIdx.x / 64] = v;
+    __syncthreads();
+    return lds[0] + lds[1] + lds[2] + lds[3];
+}
+
+// One workgroup per (batch item, group): the results of all its chunks (at most kMostChunks), in their order. A chunk has
+// `in_chunk` values of the group, the last one `in_last`.
+constexpr int kMostChunks = 2048;
 __global__ void __launch_bounds__(256)
-norm_join_kernel(const float* __restrict__ partial, float* __restrict__ mean, float* __restrict__ rstd, int64_t pairs,
-                 int groups, int chunks, float eps) {
-    const int64_t pair = blockIdx.x * 4ll + threadIdx.x / 64;
-    if (pair >= pairs) return;
-    const int lane = threadIdx.x % 64, g = static_cast<int>(pair % groups);
-    const float* p = partial + (pair / groups * chunks * groups + g) * 3;
-    const int64_t step = static_cast<int64_t>(groups) * 3;
-    float n = 0.0f, sum = 0.0f, dev = 0.0f;
-    for (int i = lane; i < chunks; i += 64) {
-        n += p[i * step];
-        sum = fmaf(p[i * step], p[i * step + 1], sum);
+norm_join_kernel(const float2* __restrict__ partial, float* __restrict__ mean, float* __restrict__ rstd, int chunks, float in_chunk,
+                 float in_last, float eps) {
+    __shared__ float lds[4];
+    const int64_t pair = blockIdx.x;
+    float2 v[kMostChunks / 256];
+    float n[kMostChunks / 256], sum = 0.0f, total = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kMostChunks / 256; ++k) {
+        const int i = threadIdx.x + 256 * k;
+        n[k] = i < chunks - 1 ? in_chunk : i == chunks - 1 ? in_last : 0.0f;
+        v[k] = i < chunks ? partial[pair * chunks + i] : float2{0.0f, 0.0f};
+        total += n[k];
+        sum = fmaf(n[k], v[k].x, sum);
     }
-    n = sum_over(n, 64);
-    const float mu = sum_over(sum, 64) / n;
-    for (int i = lane; i < chunks; i += 64) {
-        const float d = p[i * step + 1] - mu;
-        dev += p[i * step + 2] + p[i * step] * d * d;
+    total = sum_of_workgroup(total, lds);
+    const float mu = sum_of_workgroup(sum, lds) / total;
+    float dev = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kMostChunks / 256; ++k) {
+        const float d = v[k].x - mu;
+        dev += n[k] > 0.0f ? fmaf(n[k] * d, d, v[k].y) : 0.0f;
     }
-    dev = sum_over(dev, 64);
-    if (lane == 0) {
+    dev = sum_of_workgroup(dev, lds);
+    if (threadIdx.x == 0) {
         mean[pair] = mu;
-        rstd[pair] = 1.0f / sqrtf(dev / n + eps);
+        rstd[pair] = 1.0f / sqrtf(dev / total + eps);
     }
 }
 
@@ -244,20 +275,21 @@ norm_apply_kernel(NormArgs<T> a, const float* __restrict__ mean, const float* __
     const int t = threadIdx.x;
     if (t >= L.active) return;
     // last to first: the end of x is what the statistics left in the memory-side cache
-    const int id = total_workgroups - 1 - blockIdx.x;
-    const int64_t b = id / chunks, chunk = id % chunks;
+    const unsigned id = total_workgroups - 1 - blockIdx.x, chunk = id % static_cast<unsigned>(chunks);
+    const int64_t b = id / static_cast<unsigned>(chunks);
     const T *x = a.x + b * L.total, *r = a.residual ? a.residual + b * L.total : nullptr;
     T* y = a.y + b * L.total;
     int64_t off = Item<T>::offset(L, t, 0);
     float mu[V], scale[V], shift[V];
-    int c = static_cast<int>(off % L.channels);
+    Walk at(Item<T>::channel(L, t, 0), a.per_group);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        const int64_t pair = b * a.groups + c / a.per_group;
+        const int64_t pair = b * a.groups + at.g;
+        const int c = at.c;
         mu[j] = mean[pair];
         scale[j] = rstd[pair] * (a.weight ? load_param<T>(a.weight, a.float_params, c) : 1.0f);
         shift[j] = a.bias ? load_param<T>(a.bias, a.float_params, c) : 0.0f;
-        if (++c == L.channels) c = 0;
+        at.next(L.channels, a.per_group);
     }
     off += chunk * chunk_steps * L.stride;
     const int64_t end = min(L.total, (chunk + 1) * chunk_steps * L.stride);
@@ -315,7 +347,8 @@ norm_sums_kernel(NormBackwardArgs<T> a, float* __restrict__ partial, Lanes L, in
     typedef typename Vec<T>::Type Packed;
     extern __shared__ float lds[];
     const int t = threadIdx.x;
-    const int64_t b = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
+    const unsigned chunk = blockIdx.x % static_cast<unsigned>(chunks);
+    const int64_t b = blockIdx.x / static_cast<unsigned>(chunks);
     float sum[V], dot[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) sum[j] = dot[j] = 0.0f;
@@ -324,15 +357,16 @@ norm_sums_kernel(NormBackwardArgs<T> a, float* __restrict__ partial, Lanes L, in
         const T* r = ACT != kActNone && a.residual ? a.residual + b * L.total : nullptr;
         int64_t off = Item<T>::offset(L, t, 0);
         float mu[V], rs[V], w[V], bias[V];
-        int c = static_cast<int>(off % L.channels);
+        Walk at(Item<T>::channel(L, t, 0), a.per_group);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const int64_t pair = b * a.groups + c / a.per_group;
+            const int64_t pair = b * a.groups + at.g;
+            const int c = at.c;
             mu[j] = a.mean[pair];
             rs[j] = a.rstd[pair];
             w[j] = a.weight ? load_param<T>(a.weight, a.float_params, c) : 1.0f;
             bias[j] = a.bias ? load_param<T>(a.bias, a.float_params, c) : 0.0f;
-            if (++c == L.channels) c = 0;
+            at.next(L.channels, a.per_group);
         }
         off += chunk * chunk_steps * L.stride;
         const int64_t end = min(L.total, (chunk + 1) * chunk_steps * L.stride);
@@ -383,16 +417,17 @@ norm_sums_kernel(NormBackwardArgs<T> a, float* __restrict__ partial, Lanes L, in
     });
 }
 
-// totals[b][c] = the partial sums of all workgroups of an item, 16 channels by 16 rows of threads, always in the same order.
-__global__ void __launch_bounds__(256)
+// totals[b][c] = the partial sums of all workgroups of an item, 16 channels by 64 rows of threads, always in the same order.
+__global__ void __launch_bounds__(1024)
 norm_join_sums_kernel(const float2* __restrict__ partial, float2* __restrict__ totals, int channels, int chunks, int tiles) {
-    __shared__ float2 part[16][17];
-    const int64_t b = blockIdx.x / tiles;
-    const int c = blockIdx.x % tiles * 16 + threadIdx.x % 16, row = threadIdx.x / 16;
+    __shared__ float2 part[64][17];
+    const int64_t b = blockIdx.x / static_cast<unsigned>(tiles);
+    const int c = blockIdx.x % static_cast<unsigned>(tiles) * 16 + threadIdx.x % 16, row = threadIdx.x / 16;
     float2 s = {0.0f, 0.0f};
     if (c < channels) {
         const float2* p = partial + b * chunks * channels + c;
-        for (int i = row; i < chunks; i += 16) {
+#pragma unroll 4
+        for (int i = row; i < chunks; i += 64) {
             const float2 v = p[static_cast<int64_t>(i) * channels];
             s.x += v.x;
             s.y += v.y;
@@ -400,13 +435,16 @@ norm_join_sums_kernel(const float2* __restrict__ partial, float2* __restrict__ t
     }
     part[row][threadIdx.x % 16] = s;
     __syncthreads();
-    if (row == 0 && c < channels) {
-        for (int i = 1; i < 16; ++i) {
-            s.x += part[i][threadIdx.x].x;
-            s.y += part[i][threadIdx.x].y;
+    for (int half = 32; half > 0; half >>= 1) {
+        if (row < half) {
+            const float2 v = part[row + half][threadIdx.x % 16];
+            s.x += v.x;
+            s.y += v.y;
+            part[row][threadIdx.x % 16] = s;
         }
-        totals[b * channels + c] = s;
+        __syncthreads();
     }
+    if (row == 0 && c < channels) totals[b * channels + c] = s;
 }
 
 // s1/m and s2/m of the groups of `slab` channels from c0 on, in LDS, from per-channel totals.
@@ -456,8 +494,8 @@ norm_grad_kernel(NormBackwardArgs<T> a, const float2* __restrict__ totals, Lanes
     for (int64_t c = blockIdx.x * static_cast<int64_t>(blockDim.x) + t; c < L.channels; c += static_cast<int64_t>(total_workgroups) * blockDim.x)
         parameter_sums(a, totals, batch, L.channels, static_cast<int>(c));
     if (a.dx == nullptr && a.dresidual == nullptr) return;
-    const int id = total_workgroups - 1 - blockIdx.x;                       // last to first, as in norm_apply_kernel
-    const int64_t b = id / chunks, chunk = id % chunks;
+    const unsigned id = total_workgroups - 1 - blockIdx.x, chunk = id % static_cast<unsigned>(chunks);   // last to first, as in norm_apply_kernel
+    const int64_t b = id / static_cast<unsigned>(chunks);
     float2* terms = reinterpret_cast<float2*>(lds);
     group_terms(terms, [&](int c) { return totals[b * L.channels + c]; }, a, 0, L.channels, inv_m);
     __syncthreads();
@@ -468,17 +506,17 @@ norm_grad_kernel(NormBackwardArgs<T> a, const float2* __restrict__ totals, Lanes
     int64_t off = Item<T>::offset(L, t, 0);
     // dx = A dz + B (x - mean) + D,  z = A (x - mean) + bias + r
     float mu[V], A[V], B[V], D[V], bias[V];
-    int c = static_cast<int>(off % L.channels);
+    Walk at(Item<T>::channel(L, t, 0), a.per_group);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        const int g = c / a.per_group;
+        const int g = at.g, c = at.c;
         const float rs = a.rstd[b * a.groups + g];
         mu[j] = a.mean[b * a.groups + g];
         A[j] = rs * (a.weight ? load_param<T>(a.weight, a.float_params, c) : 1.0f);
         B[j] = -rs * rs * terms[g].y;
         D[j] = -rs * terms[g].x;
         bias[j] = a.bias ? load_param<T>(a.bias, a.float_params, c) : 0.0f;
-        if (++c == L.channels) c = 0;
+        at.next(L.channels, a.per_group);
     }
     off += chunk * chunk_steps * L.stride;
     const int64_t end = min(L.total, (chunk + 1) * chunk_steps * L.stride);
@@ -573,14 +611,15 @@ norm_small_kernel(NormArgs<T> a, float* __restrict__ mean_out, float* __restrict
     __syncthreads();
     if (!live) return;
     float scale[V], shift[V];
-    int c = static_cast<int>(off % L.channels);
+    Walk walk(Item<T>::channel(L, t, c0), a.per_group);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        const float2 s = stats[c / a.per_group - g0];
+        const float2 s = stats[walk.g - g0];
+        const int c = walk.c;
         mean[j] = s.x;
         scale[j] = s.y * (a.weight ? load_param<T>(a.weight, a.float_params, c) : 1.0f);
         shift[j] = a.bias ? load_param<T>(a.bias, a.float_params, c) : 0.0f;
-        if (++c == L.channels) c = 0;
+        walk.next(L.channels, a.per_group);
     }
     T* y = a.y + b * L.total;
 #pragma unroll
@@ -611,16 +650,17 @@ norm_small_grad_kernel(NormBackwardArgs<T> a, float2* __restrict__ totals, Lanes
     const int64_t off = Item<T>::offset(L, t, c0);
     const int64_t end = t < L.active ? L.total : 0;
     float mu[V], rs[V], w[V], bias[V], sum[V], dot[V];
-    int c = static_cast<int>(off % L.channels);
+    Walk walk(Item<T>::channel(L, t, c0), a.per_group);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        const int64_t pair = b * a.groups + c / a.per_group;
+        const int64_t pair = b * a.groups + walk.g;
+        const int c = walk.c;
         sum[j] = dot[j] = 0.0f;
         mu[j] = a.mean[pair];
         rs[j] = a.rstd[pair];
         w[j] = a.weight ? load_param<T>(a.weight, a.float_params, c) : 1.0f;
         bias[j] = a.bias ? load_param<T>(a.bias, a.float_params, c) : 0.0f;
-        if (++c == L.channels) c = 0;
+        walk.next(L.channels, a.per_group);
     }
     T* dr = a.dresidual ? a.dresidual + b * L.total : nullptr;
 #pragma unroll 1
@@ -653,13 +693,13 @@ norm_small_grad_kernel(NormBackwardArgs<T> a, float2* __restrict__ totals, Lanes
     if (a.dx == nullptr || end == 0) return;
     T* dx = a.dx + b * L.total;
     float t1[V], t2[V];
-    c = static_cast<int>(off % L.channels);
+    Walk again(Item<T>::channel(L, t, c0), a.per_group);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        const float2 s = terms[c / a.per_group - g0];
+        const float2 s = terms[again.g - g0];
         t1[j] = s.x;
         t2[j] = s.y;
-        if (++c == L.channels) c = 0;
+        again.next(L.channels, a.per_group);
     }
 #pragma unroll 1
     for (int64_t at = off; at < end; at += L.stride) {
@@ -840,7 +880,7 @@ NormPlan plan_norm(int64_t batch, int64_t pixels, int channels, int groups, int 
     L.active = p.threads / L.phase * L.phase;
     L.stride = static_cast<int64_t>(L.active) * V;
     const int64_t steps = (L.total + L.stride - 1) / L.stride;
-    const int64_t want = (2048 * 256 / p.threads + batch - 1) / batch;       // workgroups per item: eight waves per SIMD in all
+    const int64_t want = std::max<int64_t>(1, (2048 * 256 / p.threads + batch - 1) / batch);    // workgroups per item: eight waves per SIMD in all
     p.chunk_steps = (steps + want - 1) / want;
     if (p.chunk_steps < kUnroll) p.chunk_steps = kUnroll;
     p.chunks = static_cast<int>((steps + p.chunk_steps - 1) / p.chunk_steps);
@@ -898,18 +938,19 @@ hipError_t forward(const NormCall& n, void* workspace, hipStream_t stream) {
                 return hipGetLastError();
             });
         });
-    float* partial = static_cast<float*>(workspace);
+    float2* partial = static_cast<float2*>(workspace);
     float *mean = n.mean, *rstd = n.rstd;
     const int64_t pairs = n.batch * n.groups;
     if (mean == nullptr) {
-        mean = partial + n.batch * p.chunks * n.groups * 3;
+        mean = reinterpret_cast<float*>(partial + n.batch * p.chunks * n.groups);
         rstd = mean + pairs;
     }
+    const int64_t chunk_pixels = p.chunk_steps * L.stride / L.channels, last_pixels = n.pixels - (p.chunks - 1) * chunk_pixels;
     const int workgroups = static_cast<int>(n.batch * p.chunks);
     BOXCONV_LAUNCH("norm_statistics", (norm_statistics_kernel<T>), dim3(workgroups), dim3(p.threads), static_cast<size_t>(3) * L.active * V * 4, stream, a.x,
                    partial, L, p.chunk_steps, p.chunks, a.groups, a.per_group);
-    BOXCONV_LAUNCH("norm_join", norm_join_kernel, dim3(static_cast<unsigned>((pairs + 3) / 4)), dim3(256), 0, stream, partial, mean, rstd, pairs, a.groups,
-                   p.chunks, a.eps);
+    BOXCONV_LAUNCH("norm_join", norm_join_kernel, dim3(static_cast<unsigned>(pairs)), dim3(256), 0, stream, partial, mean, rstd, p.chunks,
+                   static_cast<float>(chunk_pixels * a.per_group), static_cast<float>(last_pixels * a.per_group), a.eps);
     return with_activation(n.activation, [&](auto act) {
         BOXCONV_LAUNCH("norm_apply", (norm_apply_kernel<T, decltype(act)::value>), dim3(workgroups), dim3(p.threads), 0, stream, a, mean, rstd, L,
                        p.chunk_steps, p.chunks, workgroups);
@@ -964,7 +1005,7 @@ hipError_t backward(const NormGradCall& n, void* workspace, hipStream_t stream) 
     return with_activation(n.activation, [&](auto act) {
         BOXCONV_LAUNCH("norm_sums", (norm_sums_kernel<T, decltype(act)::value>), dim3(workgroups), dim3(p.threads), static_cast<size_t>(2) * L.active * V * 4,
                        stream, a, reinterpret_cast<float*>(partial), L, p.chunk_steps, p.chunks);
-        BOXCONV_LAUNCH("norm_join_sums", norm_join_sums_kernel, dim3(static_cast<unsigned>(n.batch * tiles)), dim3(256), 0, stream, partial, totals,
+        BOXCONV_LAUNCH("norm_join_sums", norm_join_sums_kernel, dim3(static_cast<unsigned>(n.batch * tiles)), dim3(1024), 0, stream, partial, totals,
                        n.channels, p.chunks, tiles);
         BOXCONV_LAUNCH("norm_grad", (norm_grad_kernel<T, decltype(act)::value>), dim3(workgroups), dim3(p.threads), static_cast<size_t>(a.groups) * 8, stream,
                        a, totals, L, p.chunk_steps, p.chunks, n.batch, inv_m, workgroups);
@@ -978,7 +1019,7 @@ size_t norm_workspace_bytes(int64_t batch, int64_t pixels, int channels, int gro
     const NormPlan p = plan_norm(batch, pixels, channels, groups, dtype == kF32 ? 4 : 8);
     const int64_t chunks = p.any || p.small ? 0 : batch * p.chunks;
     if (backward_pass) return static_cast<size_t>(batch * channels + chunks * channels) * 8;
-    return chunks ? static_cast<size_t>(chunks * groups * 3 + batch * groups * 2) * 4 : 0;
+    return chunks ? static_cast<size_t>(chunks * groups * 2 + batch * groups * 2) * 4 : 0;
 }
 
 hipError_t norm_forward_launch(const NormCall& n, void* workspace, hipStream_t stream) {

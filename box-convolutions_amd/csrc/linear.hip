@@ -68,19 +68,40 @@ product_kernel(Operand<T> a, Operand<T> b, Tail<T> tail, int64_t k_part, int64_t
         }
 }
 
-// The parts of a split product, added in their order, and the tail. Eight columns per thread.
+// The parts of a split product, added in an order that only the shape decides, and the tail. A workgroup takes 256 / `lanes`
+// runs of eight columns; `lanes` (a power of two) threads share the parts of a run.
 template <class T>
-__global__ void __launch_bounds__(256) join_parts_kernel(Tail<T> tail, int splits, int64_t runs_per_row, int64_t runs) {
-    const int64_t id = blockIdx.x * 256ll + threadIdx.x;
-    if (id >= runs) return;
+__global__ void __launch_bounds__(256) join_parts_kernel(Tail<T> tail, int splits, int64_t runs_per_row, int64_t runs, int lanes) {
+    __shared__ float part[256][9];
+    const int per = 256 / lanes, lane = threadIdx.x / per;
+    const int64_t id = blockIdx.x * static_cast<int64_t>(per) + threadIdx.x % per;
     const int64_t m = id / runs_per_row, n = id % runs_per_row * 8;
-    float z[8] = {}, v[8];
-    for (int s = 0; s < splits; ++s) {
-        load_run<float, 8>(tail.partial + (s * tail.rows + m) * tail.cols + n, v, tail.cols - n);
+    float z[8] = {};
+    if (id < runs) {
+        const float* p = tail.partial + m * tail.cols + n;
+#pragma unroll 4
+        for (int s = lane; s < splits; s += lanes) {
+            float v[8];
+            load_run<float, 8>(p + s * tail.rows * tail.cols, v, tail.cols - n);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) z[i] += v[i];
+            for (int i = 0; i < 8; ++i) z[i] += v[i];
+        }
     }
-    apply_tail<T, 8>(tail, z, m, n);
+    if (lanes > 1) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) part[threadIdx.x][i] = z[i];
+        for (int half = lanes / 2; half > 0; half >>= 1) {
+            __syncthreads();
+            if (lane < half) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    z[i] += part[threadIdx.x + half * per][i];
+                    part[threadIdx.x][i] = z[i];
+                }
+            }
+        }
+    }
+    if (lane == 0 && id < runs) apply_tail<T, 8>(tail, z, m, n);
 }
 
 // ---- dz = dy * act'(z), and its column sums ---------------------------------------------------------------------
@@ -132,20 +153,24 @@ slope_kernel(const T* __restrict__ dy, const void* __restrict__ kept, T* __restr
     }
 }
 
-// dbias: the bands' sums in their order, 32 columns by 8 rows of threads.
+// dbias: the bands' sums, 16 columns by 64 rows of threads.
 template <class T>
-__global__ void __launch_bounds__(256) join_bias_kernel(const float* __restrict__ sums, T* __restrict__ dbias, int64_t cols, int bands) {
-    __shared__ float part[8][33];
-    const int64_t c = blockIdx.x * 32ll + threadIdx.x % 32;
+__global__ void __launch_bounds__(1024) join_bias_kernel(const float* __restrict__ sums, T* __restrict__ dbias, int64_t cols, int bands) {
+    __shared__ float part[64][17];
+    const int x = threadIdx.x % 16, row = threadIdx.x / 16;
+    const int64_t c = blockIdx.x * 16ll + x;
     float s = 0.0f;
-    if (c < cols)
-        for (int i = threadIdx.x / 32; i < bands; i += 8) s += sums[i * cols + c];
-    part[threadIdx.x / 32][threadIdx.x % 32] = s;
-    __syncthreads();
-    if (threadIdx.x < 32 && c < cols) {
-        for (int r = 1; r < 8; ++r) s += part[r][threadIdx.x];
-        dbias[c] = static_cast<T>(s);
+    if (c < cols) {
+#pragma unroll 4
+        for (int i = row; i < bands; i += 64) s += sums[i * cols + c];
     }
+    part[row][x] = s;
+    __syncthreads();
+    for (int half = 32; half > 0; half >>= 1) {
+        if (row < half) part[row][x] = s += part[row + half][x];
+        __syncthreads();
+    }
+    if (row == 0 && c < cols) dbias[c] = static_cast<T>(s);
 }
 
 // ---- plans ---------------------------------------------------------------------------------------------------------
@@ -183,7 +208,11 @@ hipError_t product(const char* name, Operand<T> a, Operand<T> b, Tail<T> tail, f
     else BOXCONV_LAUNCH(name, (product_kernel<T, A_K, B_K, 64>), grid, dim3(256), 0, stream, a, b, tail, p.k_part, p.tiles_m, p.tiles_n);
     if (p.splits > 1) {
         const int64_t per_row = (tail.cols + 7) / 8, runs = per_row * tail.rows;
-        BOXCONV_LAUNCH("join_parts", (join_parts_kernel<T>), dim3(static_cast<unsigned>((runs + 255) / 256)), dim3(256), 0, stream, tail, p.splits, per_row, runs);
+        int lanes = 1;                                     // threads for every CU, and at least four parts for each
+        while (lanes < 64 && lanes * 8 <= p.splits && runs * lanes < 65536) lanes *= 2;
+        const int64_t per = 256 / lanes;
+        BOXCONV_LAUNCH("join_parts", (join_parts_kernel<T>), dim3(static_cast<unsigned>((runs + per - 1) / per)), dim3(256), 0, stream, tail, p.splits, per_row,
+                       runs, lanes);
     }
     return hipGetLastError();
 }
@@ -250,7 +279,7 @@ hipError_t linear_backward(const LinearGradCall& c, void* workspace, hipStream_t
         BOXCONV_LAUNCH("linear_slope", (slope_kernel<T>), grid, dim3(256), 0, stream, dy, c.kept, write, c.dbias ? sums : nullptr, c.rows, c.N, bands.band,
                        c.activation);
         if (c.dbias != nullptr)
-            BOXCONV_LAUNCH("join_bias", (join_bias_kernel<T>), dim3(static_cast<unsigned>((c.N + 31) / 32)), dim3(256), 0, stream, sums, static_cast<T*>(c.dbias),
+            BOXCONV_LAUNCH("join_bias", (join_bias_kernel<T>), dim3(static_cast<unsigned>((c.N + 15) / 16)), dim3(1024), 0, stream, sums, static_cast<T*>(c.dbias),
                            c.N, bands.bands);
         if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     }

@@ -308,10 +308,15 @@ void release_workspaces() {
 
 }  // namespace
 
+#include "operators_glue.hpp"
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("init", &init, "hand over the addresses of the C ABI entry points of libboxconv_hip.so");
     m.def("training_step", &training_step,
           "BoxConv2d.forward (training mode: clip = true; eval mode: clip = false) with its backward as a C++ "
           "autograd node");
     m.def("release_workspaces", &release_workspaces);
+    m.def("init_operators", &init_operators, "the same for the operators around a box convolution");
+    m.def("group_norm_act", &group_norm_act, "box_convolution.group_norm_act, autograd node included");
+    m.def("linear_act", &linear_act, "box_convolution.linear_act, autograd node included");
 }
