@@ -47,7 +47,7 @@ for _tag, _t, _tg in (("f32", "float", "float"), ("f64", "double", "double"),
         SOURCES.append(_inst(_tag, _t, _tg, _part, _t == _tg))
 for _tag, _t in (("f32", "float"), ("f16", "_Float16"), ("bf16", "__bf16")):
     SOURCES.append(("linear.hip", "linear_%s.o" % _tag, ["-DBOXCONV_INST_T=" + _t]))
-OPERATOR_HEADERS = ["activation.hpp", "operators_host.hpp", "linear_tile.hpp"]     # only included by the sources below
+OPERATOR_HEADERS = ["activation.hpp", "operators_host.hpp", "linear_tile.hpp", "linear_wide.hpp", "linear_narrow.hpp"]     # only included by the sources below
 OPERATOR_SOURCES = ("operators_c_abi.hip", "group_norm.hip", "linear.hip")
 HEADERS = ["boxconv_device.hpp", "boxconv_host.hpp", "box_sampling_common.hpp", "box_sampling_impl.hpp", "narrow_rows.hpp", "forward_tail.hpp",
            os.path.join("..", "..", "include", "boxconv.h")]

@@ -1,6 +1,6 @@
 // The pointwise product y = act(x W^T + bias + residual) and its gradients for one element type (BOXCONV_INST_T: float,
 // _Float16 or __bf16; compiled once for each).
-#include "linear_tile.hpp"
+#include "linear_wide.hpp"
 
 namespace boxconv {
 
@@ -175,37 +175,77 @@ __global__ void __launch_bounds__(1024) join_bias_kernel(const float* __restrict
 
 // ---- plans ---------------------------------------------------------------------------------------------------------
 struct ProductPlan {
-    int tile, splits;
+    int shape, splits;         // shape: which of the kernels below
     int64_t k_part, tiles_m, tiles_n;
     size_t partial_bytes;
 };
 
-template <class T>
-ProductPlan plan_product(int64_t m, int64_t n, int64_t k) {
+// The kernels' tiles, and what a step of 128 bytes of k takes a compute unit that holds `w` of their workgroups, in us: fixed + each * w,
+// as measured on bfloat16 products of 8192 x 4096 x 2048 and 512 x 512 x 4096.
+struct ProductShape { int tm, tn, resident; double fixed, each; };
+constexpr ProductShape kWide[] = {{256, 256, 1, 0.0, 1.75}, {256, 128, 1, 0.0, 1.05}, {128, 128, 2, 0.35, 0.33}, {64, 64, 4, 0.3, 0.1}};
+constexpr ProductShape kAny[] = {{128, 128, 2, 0.5, 0.55}, {64, 64, 4, 0.4, 0.2}};
+
+// The tile and the number of parts of k that promise the shortest time: rounds of workgroups, each as long as its steps and
+// about four more for its start and its epilogue, and the parts' way through memory at 4 TB/s with one more launch.
+template <class T, int N>
+ProductPlan plan_product(const ProductShape (&shapes)[N], int64_t m, int64_t n, int64_t k) {
     constexpr int KT = 8 * Vec<T>::kLen;
-    ProductPlan p;
-    const int64_t big = ((m + 127) / 128) * ((n + 127) / 128);
-    p.tile = m > 64 && n > 64 && big >= 256 ? 128 : 64;
-    p.tiles_m = (m + p.tile - 1) / p.tile;
-    p.tiles_n = (n + p.tile - 1) / p.tile;
-    const int64_t tiles = std::max<int64_t>(p.tiles_m * p.tiles_n, 1), steps = (k + KT - 1) / KT;
-    int64_t splits = 1;
-    if (tiles < 256) splits = std::min<int64_t>({(512 + tiles - 1) / tiles, (steps + 3) / 4, 256});
-    splits = std::max<int64_t>(splits, 1);
-    const int64_t part = (steps + splits - 1) / splits;
-    p.splits = static_cast<int>(steps == 0 ? 1 : (steps + part - 1) / part);
-    p.k_part = std::max<int64_t>(part, 1) * KT;
-    p.partial_bytes = p.splits > 1 ? static_cast<size_t>(p.splits) * m * n * 4 : 0;
-    return p;
+    ProductPlan best = {};
+    double least = 0.0;
+    const int64_t steps = std::max<int64_t>((k + KT - 1) / KT, 1);
+    for (int i = 0; i < N; ++i) {
+        const ProductShape& s = shapes[i];
+        const int64_t tm = (m + s.tm - 1) / s.tm, tn = (n + s.tn - 1) / s.tn, tiles = std::max<int64_t>(tm * tn, 1);
+        for (int64_t splits = 1; splits <= 256 && splits * 2 <= std::max<int64_t>(steps, 2); splits *= 2) {
+            const int64_t part = (steps + splits - 1) / splits, parts = (steps + part - 1) / part, groups = tiles * parts;
+            const int64_t slots = 256 * s.resident, rounds = (groups + slots - 1) / slots;
+            const double w = groups >= slots ? s.resident : static_cast<double>((groups + 255) / 256);
+            double t = static_cast<double>(rounds) * static_cast<double>(part + 4) * (s.fixed + s.each * w);
+            if (parts > 1) t += 4.0 + static_cast<double>(parts) * static_cast<double>(m) * static_cast<double>(n) * 8.0 / 4e6;
+            if (best.splits == 0 || t < least) {
+                least = t;
+                best = {i, static_cast<int>(parts), part * KT, tm, tn, parts > 1 ? static_cast<size_t>(parts) * m * n * 4 : 0};
+            }
+            if (groups >= 1024) break;
+        }
+    }
+    return best;
+}
+
+// Whether tiles of this operand can come straight into LDS: whole aligned chunks, offsets within a tile in 31 bits.
+template <class T, bool K_MAJOR>
+bool whole_chunks(const Operand<T>& o) {
+    constexpr int V = Vec<T>::kLen;
+    return reinterpret_cast<uintptr_t>(o.p) % 16 == 0 && o.ld % V == 0 && (K_MAJOR ? o.depth : o.extent) % V == 0 && o.depth < (int64_t(1) << 30) &&
+           o.ld < (int64_t(1) << 31) / (256 * static_cast<int64_t>(sizeof(T)));
+}
+
+template <class T, bool A_K, bool B_K, int TM, int TN, int WM, int WN>
+void launch_wide(const char* name, const Operand<T>& a, const Operand<T>& b, const Tail<T>& tail, const ProductPlan& p, hipStream_t stream) {
+    constexpr size_t lds = 2 * sizeof(Chunk) * (TileShape<T, A_K, TM>::kChunks + TileShape<T, B_K, TN>::kChunks);
+    const dim3 grid(static_cast<unsigned>(p.tiles_m * p.tiles_n), p.splits);
+    BOXCONV_LAUNCH(name, (product_wide_kernel<T, A_K, B_K, TM, TN, WM, WN>), grid, dim3(WM * WN * 64), lds, stream, a, b, tail, p.k_part,
+                   static_cast<unsigned>(p.tiles_m), static_cast<unsigned>(p.tiles_n));
 }
 
 template <class T, bool A_K, bool B_K>
 hipError_t product(const char* name, Operand<T> a, Operand<T> b, Tail<T> tail, float* workspace, hipStream_t stream) {
-    const ProductPlan p = plan_product<T>(tail.rows, tail.cols, a.depth);
+    const bool wide = whole_chunks<T, A_K>(a) && whole_chunks<T, B_K>(b);
+    const ProductPlan p = wide ? plan_product<T>(kWide, tail.rows, tail.cols, a.depth) : plan_product<T>(kAny, tail.rows, tail.cols, a.depth);
     tail.partial = p.splits > 1 ? workspace : nullptr;
-    const dim3 grid(static_cast<unsigned>(p.tiles_m * p.tiles_n), p.splits);
-    if (p.tile == 128) BOXCONV_LAUNCH(name, (product_kernel<T, A_K, B_K, 128>), grid, dim3(256), 0, stream, a, b, tail, p.k_part, p.tiles_m, p.tiles_n);
-    else BOXCONV_LAUNCH(name, (product_kernel<T, A_K, B_K, 64>), grid, dim3(256), 0, stream, a, b, tail, p.k_part, p.tiles_m, p.tiles_n);
+    if (wide) {
+        switch (p.shape) {
+            case 0: launch_wide<T, A_K, B_K, 256, 256, 2, 4>(name, a, b, tail, p, stream); break;
+            case 1: launch_wide<T, A_K, B_K, 256, 128, 4, 2>(name, a, b, tail, p, stream); break;
+            case 2: launch_wide<T, A_K, B_K, 128, 128, 2, 2>(name, a, b, tail, p, stream); break;
+            default: launch_wide<T, A_K, B_K, 64, 64, 2, 2>(name, a, b, tail, p, stream);
+        }
+    } else {
+        const dim3 grid(static_cast<unsigned>(p.tiles_m * p.tiles_n), p.splits);
+        if (p.shape == 0) BOXCONV_LAUNCH(name, (product_kernel<T, A_K, B_K, 128>), grid, dim3(256), 0, stream, a, b, tail, p.k_part, p.tiles_m, p.tiles_n);
+        else BOXCONV_LAUNCH(name, (product_kernel<T, A_K, B_K, 64>), grid, dim3(256), 0, stream, a, b, tail, p.k_part, p.tiles_m, p.tiles_n);
+    }
     if (p.splits > 1) {
         const int64_t per_row = (tail.cols + 7) / 8, runs = per_row * tail.rows;
         int lanes = 1;                                     // threads for every CU, and at least four parts for each
@@ -215,6 +255,11 @@ hipError_t product(const char* name, Operand<T> a, Operand<T> b, Tail<T> tail, f
                        runs, lanes);
     }
     return hipGetLastError();
+}
+
+template <class T>
+size_t product_workspace(int64_t m, int64_t n, int64_t k) {
+    return std::max(plan_product<T>(kWide, m, n, k).partial_bytes, plan_product<T>(kAny, m, n, k).partial_bytes);
 }
 
 size_t round_up(size_t v) { return (v + 255) / 256 * 256; }
@@ -233,13 +278,13 @@ BandPlan plan_bands(int64_t rows, int64_t cols) {
 }  // namespace
 
 template <class T>
-size_t linear_forward_workspace(int64_t rows, int64_t K, int64_t N) { return plan_product<T>(rows, N, K).partial_bytes; }
+size_t linear_forward_workspace(int64_t rows, int64_t K, int64_t N) { return product_workspace<T>(rows, N, K); }
 
 // [dz, unless the residual's gradient holds it][column sums per band][parts of a split product]
 template <class T>
 size_t linear_backward_workspace(int64_t rows, int64_t K, int64_t N) {
     return round_up(static_cast<size_t>(rows) * N * sizeof(T)) + round_up(static_cast<size_t>(plan_bands(rows, N).bands) * N * 4) +
-           std::max(plan_product<T>(rows, K, N).partial_bytes, plan_product<T>(N, K, rows).partial_bytes);
+           std::max(product_workspace<T>(rows, K, N), product_workspace<T>(N, K, rows));
 }
 
 template <class T>
