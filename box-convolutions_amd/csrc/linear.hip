@@ -12,8 +12,8 @@ namespace {
 template <class T, bool A_K, bool B_K, int TX>
 __global__ void __launch_bounds__(256)
 product_kernel(Operand<T> a, Operand<T> b, Tail<T> tail, int64_t k_part, int64_t tiles_m, int64_t tiles_n) {
-    typedef TileShape<T, A_K, TX> SA;
-    typedef TileShape<T, B_K, TX> SB;
+    typedef TileShape<T, A_K, TX, 8> SA;
+    typedef TileShape<T, B_K, TX, 8> SB;
     constexpr int F = TX / 64;                              // 32 x 32 blocks of a wave along each axis
     __shared__ Chunk lds[SA::kChunks + SB::kChunks];
     Chunk *ta = lds, *tb = lds + SA::kChunks;
@@ -37,12 +37,12 @@ product_kernel(Operand<T> a, Operand<T> b, Tail<T> tail, int64_t k_part, int64_t
             sb.load(b, n0, k0 + SA::KT, k_end);
         }
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
+        for (int ks = 0; ks < SA::kSteps; ++ks) {
             Chunk fa[F], fb[F];
 #pragma unroll
             for (int j = 0; j < F; ++j) {
-                fa[j] = fragment<T, A_K, TX, false>(ta, wm + 32 * j, ks);
-                fb[j] = fragment<T, B_K, TX, true>(tb, wn + 32 * j, ks);
+                fa[j] = fragment<T, A_K, TX, 8, false>(ta, wm + 32 * j, ks);
+                fb[j] = fragment<T, B_K, TX, 8, true>(tb, wn + 32 * j, ks);
             }
 #pragma unroll
             for (int i = 0; i < F; ++i)
@@ -180,14 +180,16 @@ struct ProductPlan {
     size_t partial_bytes;
 };
 
-// The kernels' tiles, and what a step of 128 bytes of k takes a compute unit that holds `w` of their workgroups, in us: fixed + each * w,
-// as measured on bfloat16 products of 8192 x 4096 x 2048 and 512 x 512 x 4096.
+// The kernels' tiles, and what a step of 128 bytes of k takes a compute unit that holds `w` of their workgroups, in us: fixed + each * w.
+// Measured on bfloat16 products, M x N x K: 8192 x 4096 x 2048 takes 107 us with 256 x 256 tiles, 137 with 128 x 128; 2048 x 2048 x
+// 4096 takes 78, 48 and, with 64 x 64, 52; 512 x 512 x 4096 33 with 128 x 128, 36 with 64 x 64 (none of them split). Tiles of
+// 256 x 128 were no better than 128 x 128 anywhere: their waves read as much from LDS per product.
 struct ProductShape { int tm, tn, resident; double fixed, each; };
-constexpr ProductShape kWide[] = {{256, 256, 1, 0.0, 1.75}, {256, 128, 1, 0.0, 1.05}, {128, 128, 2, 0.35, 0.33}, {64, 64, 4, 0.3, 0.1}};
+constexpr ProductShape kWide[] = {{256, 256, 1, 0.0, 1.38}, {128, 128, 2, 0.46, 0.21}, {64, 64, 4, 0.44, 0.075}};
 constexpr ProductShape kAny[] = {{128, 128, 2, 0.5, 0.55}, {64, 64, 4, 0.4, 0.2}};
 
 // The tile and the number of parts of k that promise the shortest time: rounds of workgroups, each as long as its steps and
-// about four more for its start and its epilogue, and the parts' way through memory at 4 TB/s with one more launch.
+// about seven more for its start and its epilogue, and the parts' way through memory at 4 TB/s with one more launch.
 template <class T, int N>
 ProductPlan plan_product(const ProductShape (&shapes)[N], int64_t m, int64_t n, int64_t k) {
     constexpr int KT = 8 * Vec<T>::kLen;
@@ -201,7 +203,7 @@ ProductPlan plan_product(const ProductShape (&shapes)[N], int64_t m, int64_t n, 
             const int64_t part = (steps + splits - 1) / splits, parts = (steps + part - 1) / part, groups = tiles * parts;
             const int64_t slots = 256 * s.resident, rounds = (groups + slots - 1) / slots;
             const double w = groups >= slots ? s.resident : static_cast<double>((groups + 255) / 256);
-            double t = static_cast<double>(rounds) * static_cast<double>(part + 4) * (s.fixed + s.each * w);
+            double t = static_cast<double>(rounds) * static_cast<double>(part + 7) * (s.fixed + s.each * w);
             if (parts > 1) t += 4.0 + static_cast<double>(parts) * static_cast<double>(m) * static_cast<double>(n) * 8.0 / 4e6;
             if (best.splits == 0 || t < least) {
                 least = t;
@@ -223,7 +225,7 @@ bool whole_chunks(const Operand<T>& o) {
 
 template <class T, bool A_K, bool B_K, int TM, int TN, int WM, int WN>
 void launch_wide(const char* name, const Operand<T>& a, const Operand<T>& b, const Tail<T>& tail, const ProductPlan& p, hipStream_t stream) {
-    constexpr size_t lds = 2 * sizeof(Chunk) * (TileShape<T, A_K, TM>::kChunks + TileShape<T, B_K, TN>::kChunks);
+    constexpr size_t lds = kRing * sizeof(Chunk) * (TileShape<T, A_K, TM, 8>::kChunks + TileShape<T, B_K, TN, 8>::kChunks);
     const dim3 grid(static_cast<unsigned>(p.tiles_m * p.tiles_n), p.splits);
     BOXCONV_LAUNCH(name, (product_wide_kernel<T, A_K, B_K, TM, TN, WM, WN>), grid, dim3(WM * WN * 64), lds, stream, a, b, tail, p.k_part,
                    static_cast<unsigned>(p.tiles_m), static_cast<unsigned>(p.tiles_n));
@@ -236,9 +238,8 @@ hipError_t product(const char* name, Operand<T> a, Operand<T> b, Tail<T> tail, f
     tail.partial = p.splits > 1 ? workspace : nullptr;
     if (wide) {
         switch (p.shape) {
-            case 0: launch_wide<T, A_K, B_K, 256, 256, 2, 4>(name, a, b, tail, p, stream); break;
-            case 1: launch_wide<T, A_K, B_K, 256, 128, 4, 2>(name, a, b, tail, p, stream); break;
-            case 2: launch_wide<T, A_K, B_K, 128, 128, 2, 2>(name, a, b, tail, p, stream); break;
+            case 0: launch_wide<T, A_K, B_K, 256, 256, 4, 2>(name, a, b, tail, p, stream); break;
+            case 1: launch_wide<T, A_K, B_K, 128, 128, 2, 2>(name, a, b, tail, p, stream); break;
             default: launch_wide<T, A_K, B_K, 64, 64, 2, 2>(name, a, b, tail, p, stream);
         }
     } else {

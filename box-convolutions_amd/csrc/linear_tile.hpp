@@ -2,7 +2,7 @@
 // operands staged through LDS.
 //
 // Each operand lies in memory either with k contiguous ("K-major": x and weight in the forward) or with k as its slow index
-// (the weight in dx = dz W, both operands in dW = dz^T x). A K-major operand is staged as rows of 128 bytes of k; the other
+// (the weight in dx = dz W, both operands in dW = dz^T x). A K-major operand is staged as rows of 64 or 128 bytes of k; the other
 // kind as rows of one k, and its fragments are read transposed (ds_read_b64_tr_b16: 16 lanes read a block of 4 k by 16
 // columns and each ends up with the 4 k of one column), so no operand is ever transposed in memory.
 //
@@ -38,20 +38,22 @@ __device__ __forceinline__ Chunk load_chunk(const T* p, int64_t valid) {
 // 8 (i/4) + 4 (l/32) + i%4, which this maps to column 16 (l/32) + i.
 __device__ __forceinline__ int column_of(int r) { return 16 * ((r >> 2) & 1) + 4 * (r >> 3) + (r & 3); }
 
-// Shape of one operand's tile in LDS: X rows (m or n) by KT values of k.
-template <class T, bool K_MAJOR, int X>
+// Shape of one operand's tile in LDS: X rows (m or n) by KT values of k, CH chunks of 16 bytes.
+template <class T, bool K_MAJOR, int X, int CH>
 struct TileShape {
     static constexpr int V = Vec<T>::kLen;
-    static constexpr int KT = 8 * V;                                      // 128 bytes of k
-    static constexpr int kRowChunks = K_MAJOR ? 8 : X / V;                // 16-byte chunks in a row of the tile
+    static constexpr int KT = CH * V;
+    static constexpr int kSteps = CH / 2;                                 // of the matrix instructions: 16 values of k in 16-bit types, 8 in float
+    static constexpr int kRowChunks = K_MAJOR ? CH : X / V;               // 16-byte chunks in a row of the tile
     static constexpr int kRows = K_MAJOR ? X : KT;
     static constexpr int kChunks = kRows * kRowChunks;
     // Position of chunk c of row r: exclusive-or with a few bits of r, so that the lanes of one LDS access spread over the
-    // 64 banks. PERM: fragments of B take rows in the order of column_of (bits 1, 2 and 4 of the row vary between
-    // neighbouring lanes), those of A in natural order (bits 1 to 3).
+    // 64 banks. PERM: fragments of B take rows in the order of column_of (bits 0, 1, 4 and 2 of the row count the lanes of an
+    // access), those of A in natural order (bits 0 to 3).
     template <bool PERM>
     static __device__ __forceinline__ int place(int r, int c) {
-        if constexpr (K_MAJOR) return r * 8 + (c ^ (PERM ? ((r >> 1) & 3) | ((r >> 2) & 4) : (r >> 1) & 7));
+        if constexpr (K_MAJOR && CH == 8) return r * 8 + (c ^ (PERM ? ((r >> 1) & 3) | ((r >> 2) & 4) : (r >> 1) & 7));
+        else if constexpr (K_MAJOR) return r * 4 + (c ^ (PERM ? ((r >> 2) & 1) | ((r >> 3) & 2) : (r >> 2) & 3));
         else if constexpr (sizeof(T) == 2) return r * kRowChunks + (kRowChunks >= 16 ? c ^ (4 * (r & 3)) : kRowChunks == 8 ? c ^ (2 * (r & 2)) : c);
         else return r * kRowChunks + (kRowChunks >= 16 ? c ^ (2 * (r & 4)) : c);
     }
@@ -68,7 +70,7 @@ struct Operand {
 // The chunks of a tile that one thread stages, through registers and with every bound checked.
 template <class T, bool K_MAJOR, int X, int THREADS, bool PERM>
 struct Stage {
-    typedef TileShape<T, K_MAJOR, X> Shape;
+    typedef TileShape<T, K_MAJOR, X, 8> Shape;
     static constexpr int N = Shape::kChunks / THREADS;
     Chunk v[N];
     static_assert(Shape::kChunks % THREADS == 0, "whole chunks per thread");
@@ -94,10 +96,10 @@ struct Stage {
     }
 };
 
-// The fragment of 32 rows from `i` on and k step ks (0..3, 16 values of k in 16-bit types, 8 in float).
-template <class T, bool K_MAJOR, int X, bool PERM>
+// The fragment of 32 rows from `i` on and k step ks.
+template <class T, bool K_MAJOR, int X, int CH, bool PERM>
 __device__ __forceinline__ Chunk fragment(const Chunk* tile, int i, int ks) {
-    typedef TileShape<T, K_MAJOR, X> Shape;
+    typedef TileShape<T, K_MAJOR, X, CH> Shape;
     const int l = threadIdx.x % 64;
     if constexpr (K_MAJOR) {
         const int r = i + (PERM ? column_of(l % 32) : l % 32);

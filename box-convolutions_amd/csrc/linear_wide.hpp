@@ -7,15 +7,20 @@ namespace boxconv {
 
 namespace {
 
-// Loads of up to 64 lanes x 16 bytes from a descriptor's memory into LDS at `to` + 16 * lane. Offsets at or beyond the
-// descriptor's size give zeros; kNowhere is beyond every size.
-constexpr unsigned kNowhere = 0xfffffff0u;
-typedef __attribute__((address_space(3))) void LdsVoid;
+// 16 bytes per lane from `offset` bytes into a descriptor's memory to LDS at `to` + 16 * lane; offsets at or beyond the
+// descriptor's size give zeros. In assembly because the compiler waits for all such loads in front of every transposed LDS
+// read; it writes no register, and settle() does the waiting. (One wait state between the write of M0 and its use.)
+constexpr unsigned kNowhere = 0xfffffff0u;                             // beyond every size
+typedef __attribute__((address_space(3))) const void* LdsVoid;
+typedef int Descriptor __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ void load_to_lds(Descriptor d, unsigned offset, unsigned to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(offset), "s"(d) : "m0");
+}
 
 // One operand's tile as the DMA fills it: where each of a thread's chunks comes from.
 template <class T, bool K_MAJOR, int X, int THREADS, bool PERM>
 struct Feed {
-    typedef TileShape<T, K_MAJOR, X> Shape;
+    typedef TileShape<T, K_MAJOR, X, 8> Shape;
     static constexpr int N = Shape::kChunks / THREADS;
     static_assert(!K_MAJOR || THREADS % 256 == 0, "a thread's chunks of a K-major tile all have the same k");
     unsigned off[N];           // bytes from the tile's corner in memory; kNowhere for rows beyond the operand
@@ -40,18 +45,21 @@ struct Feed {
         size = bytes - corner;
         step = K_MAJOR ? 128 : Shape::KT * ld;
     }
-    // The next tile into `tile`. k_left: values of k from its corner to the end of the sum, none where it is <= 0: a K-major
-    // operand's chunks beyond it would be the next row's. (Rows of k beyond the other kind's end are beyond its descriptor.)
-    __device__ __forceinline__ void fetch(Chunk* tile, int k_left) {
+    // The descriptor of the next tile.
+    __device__ __forceinline__ Descriptor next() {
         const unsigned bytes = size <= 0 ? 0u : size < 0xffffff00ll ? static_cast<unsigned>(size) : 0xffffff00u;
-        const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, static_cast<int>(bytes), 0x00020000);
-        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-        const bool inside = !K_MAJOR || k < k_left;
-#pragma unroll
-        for (int s = 0; s < N; ++s)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (LdsVoid*)(tile + s * THREADS + wave * 64), 16, static_cast<int>(inside ? off[s] : kNowhere), 0, 0, 0);
+        const uint64_t at = reinterpret_cast<uint64_t>(base);
         base += step;
         size -= step;
+        return {static_cast<int>(at), static_cast<int>(at >> 32) & 0xffff, static_cast<int>(bytes), 0x00020000};
+    }
+    // The thread's chunk s of it, with its workgroup's others, into `tile`. k_left: values of k from the tile's corner to the
+    // end of the sum, none where it is <= 0: a K-major operand's chunks beyond it would be the next row's. (Rows of k beyond
+    // the other kind's end are beyond its descriptor.)
+    __device__ __forceinline__ void fetch(Descriptor d, int s, const Chunk* tile, int k_left) const {
+        const unsigned wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+        const unsigned to = static_cast<unsigned>(reinterpret_cast<uintptr_t>((LdsVoid)(tile + s * THREADS))) + wave * 1024;
+        load_to_lds(d, !K_MAJOR || k < k_left ? off[s] : kNowhere, to);
     }
 };
 
@@ -65,12 +73,21 @@ __device__ __forceinline__ void tile_of(unsigned id, unsigned tiles_m, unsigned 
     tn = rest / high;
 }
 
-// TM x TN tile by WM x WN waves, each with (TM/WM) x (TN/WN). Two stages of LDS: while one is multiplied the other fills.
+constexpr int kRing = 2;           // stages of LDS
+
+// At most N of this wave's loads may still be on their way and none of its LDS reads; then wait for every wave to get here.
+template <int N>
+__device__ __forceinline__ void settle() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory"); }
+
+// TM x TN tile by WM x WN waves, each with (TM/WM) x (TN/WN). Two stages of 128 bytes of k. The barrier of a stage stands in front
+// of its last k step, whose fragments are in registers by then: from there on its LDS takes the stage after next, whose loads are
+// issued one at a time between the products of three k steps (eight waves that issue theirs all at once keep the memory pipe,
+// and with it themselves, busy for half a stage), and the next stage's first fragments are read between the last products.
 template <class T, bool A_K, bool B_K, int TM, int TN, int WM, int WN>
 __global__ void __launch_bounds__(WM * WN * 64)
 product_wide_kernel(Operand<T> a, Operand<T> b, Tail<T> tail, int64_t k_part, unsigned tiles_m, unsigned tiles_n) {
-    typedef TileShape<T, A_K, TM> SA;
-    typedef TileShape<T, B_K, TN> SB;
+    typedef TileShape<T, A_K, TM, 8> SA;
+    typedef TileShape<T, B_K, TN, 8> SB;
     constexpr int THREADS = WM * WN * 64, FM = TM / WM / 32, FN = TN / WN / 32;
     constexpr int kStage = SA::kChunks + SB::kChunks;
     extern __shared__ Chunk stages[];
@@ -80,66 +97,61 @@ product_wide_kernel(Operand<T> a, Operand<T> b, Tail<T> tail, int64_t k_part, un
     const int64_t k_begin = blockIdx.y * k_part, k_end = min(a.depth, k_begin + k_part);
     const int wave = threadIdx.x / 64, wm = wave / WN * (TM / WM), wn = wave % WN * (TN / WN);
     Acc16 acc[FN][FM] = {};
-    Feed<T, A_K, TM, THREADS, false> fa;
-    Feed<T, B_K, TN, THREADS, true> fb;
+    typedef Feed<T, A_K, TM, THREADS, false> FeedA;
+    typedef Feed<T, B_K, TN, THREADS, true> FeedB;
+    FeedA fa;
+    FeedB fb;
     fa.start(a, m0, k_begin);
     fb.start(b, n0, k_begin);
-    int left = static_cast<int>(k_end - k_begin);              // of k, from the next tile to fetch on
-    const int steps = (left + SA::KT - 1) / SA::KT;
-    const auto fetch = [&](int stage) {
-        fa.fetch(stages + stage * kStage, left);
-        fb.fetch(stages + stage * kStage + SA::kChunks, left);
-        left -= SA::KT;
+    const int depth = static_cast<int>(k_end - k_begin), steps = (depth + SA::KT - 1) / SA::KT;
+    Descriptor da, db;
+    // piece i of the loads of stage s of the sum (beyond its end: zeros, which nobody uses)
+    const auto load = [&](int s, int i) {
+        const Chunk* tile = stages + s % kRing * kStage;
+        const int k_left = depth - s * SA::KT;
+        if (i == 0) da = fa.next();
+        if (i == FeedA::N) db = fb.next();
+        if (i < FeedA::N) fa.fetch(da, i, tile, k_left);
+        else fb.fetch(db, i - FeedA::N, tile + SA::kChunks, k_left);
     };
     Chunk xa[2][FM], xb[2][FN];
-    const auto read = [&](const Chunk* tile, int ks) {
-#pragma unroll
-        for (int j = 0; j < FM; ++j) xa[ks & 1][j] = fragment<T, A_K, TM, false>(tile, wm + 32 * j, ks);
-#pragma unroll
-        for (int i = 0; i < FN; ++i) xb[ks & 1][i] = fragment<T, B_K, TN, true>(tile + SA::kChunks, wn + 32 * i, ks);
+    // piece i of the fragments of k step ks of stage s
+    const auto read = [&](int s, int ks, int i) {
+        const Chunk* tile = stages + s % kRing * kStage;
+        if (i < FM) xa[ks & 1][i] = fragment<T, A_K, TM, 8, false>(tile, wm + 32 * i, ks);
+        else xb[ks & 1][i - FM] = fragment<T, B_K, TN, 8, true>(tile + SA::kChunks, wn + 32 * (i - FM), ks);
     };
-    const auto multiply = [&](int ks) {
-#pragma unroll
-        for (int i = 0; i < FN; ++i)
-#pragma unroll
-            for (int j = 0; j < FM; ++j) acc[i][j] = multiply_add<T>(xb[ks & 1][i], xa[ks & 1][j], acc[i][j]);
-    };
-    // the fragments of the next k step are requested one at a time between the products of this one
-    const auto interleave = [] {
-        constexpr int kReads = FM * (A_K ? 1 : sizeof(T) == 2 ? 2 : 4) + FN * (B_K ? 1 : sizeof(T) == 2 ? 2 : 4);
-        constexpr int kProducts = FM * FN * (sizeof(T) == 2 ? 1 : 4), kEach = (kReads + kProducts - 1) / kProducts;
-#pragma unroll
-        for (int i = 0; i < kProducts; ++i) {
-            __builtin_amdgcn_sched_group_barrier(0x100, kEach, 0);     // LDS reads
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);         // matrix instructions
-        }
+    constexpr int kLoads = FeedA::N + FeedB::N, kReads = FM + FN, kProducts = FM * FN;     // of a thread: per stage, k step, k step
+    // k step ks: its products, and between them loads [first, last) of stage `to` and the reads of the k step after it, of stage `from`
+    const auto step = [&](int ks, int from, int to, int first, int last) {
         __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int p = 0; p < kProducts; ++p) {
+#pragma unroll
+            for (int i = p * kReads / kProducts; i < (p + 1) * kReads / kProducts; ++i) read(from, (ks + 1) % 4, i);
+#pragma unroll
+            for (int i = p * (last - first) / kProducts; i < (p + 1) * (last - first) / kProducts; ++i) load(to, first + i);
+            acc[p / FM][p % FM] = multiply_add<T>(xb[ks & 1][p / FM], xa[ks & 1][p % FM], acc[p / FM][p % FM]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
     };
-    // this wave's share of the outstanding stage has landed and its own reads are done; then everybody's
-    const auto settle = [] { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+    static_assert(SA::kSteps == 4, "four k steps in a stage");
+    constexpr int kThird = (kLoads + 2) / 3, kThirds = (2 * kLoads + 2) / 3;
     if (steps > 0) {
-        fetch(0);
-        settle();
-        fetch(1);
-        read(stages, 0);
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) load(0, i);
+        settle<0>();
+#pragma unroll
+        for (int i = 0; i < kReads; ++i) read(0, 0, i);
+#pragma unroll
+        for (int i = 0; i < kThird; ++i) load(1, i);
     }
     for (int s = 0; s < steps; ++s) {
-        const Chunk* now = stages + (s & 1) * kStage;
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int ks = 0; ks < 3; ++ks) {
-            read(now, ks + 1);
-            multiply(ks);
-            interleave();
-        }
-        // the last fragments of this stage are on their way: once they are here, its LDS is free for the stage after next, and
-        // the next stage's first fragments can be requested before the last products. (Behind the last stage this fetches
-        // and reads what nobody uses: zeros, or the stage before.)
-        settle();
-        fetch(s & 1);
-        read(stages + (~s & 1) * kStage, 0);
-        multiply(3);
-        interleave();
+        step(0, s, s + 1, kThird, kThirds);
+        step(1, s, s + 1, kThirds, kLoads);
+        step(2, s, 0, 0, 0);
+        settle<0>();                                           // stage s + 1 has landed, and the rest of this one is in registers
+        step(3, s + 1, s + 2, 0, kThird);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");           // nothing may still be on its way into this workgroup's LDS when it ends
     const int l = threadIdx.x % 64;
