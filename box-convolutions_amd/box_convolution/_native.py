@@ -794,7 +794,7 @@ KERNEL_NAMES = ("band_colsum", "band_prefix", "band_scan", "forward_rows", "forw
                 "forward_gather", "grad_input_gather", "grad_params_gather", "int_row_prefix",
                 "int_col_prefix", "norm_statistics", "norm_join", "norm_apply", "norm_small", "norm_any", "norm_sums",
                 "norm_join_sums", "norm_grad", "norm_small_grad", "norm_parameter", "norm_any_sums", "norm_any_grad", "linear",
-                "linear_dx", "linear_dweight", "linear_slope", "join_parts", "join_bias")
+                "linear_dx", "linear_dweight", "linear_narrow_grad", "linear_slope", "join_parts", "join_bias")
 
 
 def reload_switches():

@@ -1,6 +1,6 @@
 // The pointwise product y = act(x W^T + bias + residual) and its gradients for one element type (BOXCONV_INST_T: float,
 // _Float16 or __bf16; compiled once for each).
-#include "linear_wide.hpp"
+#include "linear_narrow.hpp"
 
 namespace boxconv {
 
@@ -174,6 +174,8 @@ __global__ void __launch_bounds__(1024) join_bias_kernel(const float* __restrict
 }
 
 // ---- plans ---------------------------------------------------------------------------------------------------------
+size_t round_up(size_t v) { return (v + 255) / 256 * 256; }
+
 struct ProductPlan {
     int shape, splits;         // shape: which of the kernels below
     int64_t k_part, tiles_m, tiles_n;
@@ -231,6 +233,16 @@ void launch_wide(const char* name, const Operand<T>& a, const Operand<T>& b, con
                    static_cast<unsigned>(p.tiles_m), static_cast<unsigned>(p.tiles_n));
 }
 
+template <class T>
+void join_parts(const Tail<T>& tail, int splits, hipStream_t stream) {
+    const int64_t per_row = (tail.cols + 7) / 8, runs = per_row * tail.rows;
+    int lanes = 1;                                         // threads for every CU, and at least four parts for each
+    while (lanes < 64 && lanes * 8 <= splits && runs * lanes < 65536) lanes *= 2;
+    const int64_t per = 256 / lanes;
+    BOXCONV_LAUNCH("join_parts", (join_parts_kernel<T>), dim3(static_cast<unsigned>((runs + per - 1) / per)), dim3(256), 0, stream, tail, splits, per_row, runs,
+                   lanes);
+}
+
 template <class T, bool A_K, bool B_K>
 hipError_t product(const char* name, Operand<T> a, Operand<T> b, Tail<T> tail, float* workspace, hipStream_t stream) {
     const bool wide = whole_chunks<T, A_K>(a) && whole_chunks<T, B_K>(b);
@@ -247,14 +259,7 @@ hipError_t product(const char* name, Operand<T> a, Operand<T> b, Tail<T> tail, f
         if (p.shape == 0) BOXCONV_LAUNCH(name, (product_kernel<T, A_K, B_K, 128>), grid, dim3(256), 0, stream, a, b, tail, p.k_part, p.tiles_m, p.tiles_n);
         else BOXCONV_LAUNCH(name, (product_kernel<T, A_K, B_K, 64>), grid, dim3(256), 0, stream, a, b, tail, p.k_part, p.tiles_m, p.tiles_n);
     }
-    if (p.splits > 1) {
-        const int64_t per_row = (tail.cols + 7) / 8, runs = per_row * tail.rows;
-        int lanes = 1;                                     // threads for every CU, and at least four parts for each
-        while (lanes < 64 && lanes * 8 <= p.splits && runs * lanes < 65536) lanes *= 2;
-        const int64_t per = 256 / lanes;
-        BOXCONV_LAUNCH("join_parts", (join_parts_kernel<T>), dim3(static_cast<unsigned>((runs + per - 1) / per)), dim3(256), 0, stream, tail, p.splits, per_row,
-                       runs, lanes);
-    }
+    if (p.splits > 1) join_parts(tail, p.splits, stream);
     return hipGetLastError();
 }
 
@@ -263,7 +268,6 @@ size_t product_workspace(int64_t m, int64_t n, int64_t k) {
     return std::max(plan_product<T>(kWide, m, n, k).partial_bytes, plan_product<T>(kAny, m, n, k).partial_bytes);
 }
 
-size_t round_up(size_t v) { return (v + 255) / 256 * 256; }
 
 struct BandPlan { int64_t band; int bands; };
 BandPlan plan_bands(int64_t rows, int64_t cols) {
@@ -276,6 +280,81 @@ BandPlan plan_bands(int64_t rows, int64_t cols) {
     return p;
 }
 
+// ---- few channels --------------------------------------------------------------------------------------------------
+struct NarrowPlan {
+    bool applies;
+    int tm, blocks, workgroups, tiles;
+    size_t lds, bytes;         // of LDS; of the partial sums
+};
+
+// Sizes that narrow_grad_kernel covers, and where it pays: at least four tiles for every workgroup that the chip holds.
+template <class T>
+NarrowPlan plan_narrow(int64_t rows, int64_t K, int64_t N) {
+    constexpr int V = Vec<T>::kLen;
+    NarrowPlan p = {};
+    if (K < V || N < V || K % V || N % V || K > 1024 || N > 128 || rows > (int64_t(1) << 36)) return p;
+    const int blocks = static_cast<int>((K + 31) / 32 * ((N + 31) / 32));
+    p.blocks = 1;
+    while (p.blocks * 8 < blocks) p.blocks *= 2;
+    if (p.blocks > 4) return p;
+    for (p.tm = sizeof(T) == 2 ? 64 : 32; p.tm >= 32; p.tm /= 2) {
+        p.lds = static_cast<size_t>(narrow_lds<T>(static_cast<int>(N), static_cast<int>(K), p.tm).total());
+        if (p.lds <= kMaxDynamicLds && 2 * (512 / static_cast<int>(N / V)) >= p.tm) break;
+    }
+    if (p.tm < 32) return p;
+    const int64_t tiles = (rows + p.tm - 1) / p.tm;
+    const int64_t resident = std::min<int64_t>(2, static_cast<int64_t>(kMaxDynamicLds / p.lds)) * 256;
+    if (tiles < 4 * resident) return p;
+    p.tiles = static_cast<int>(tiles);
+    p.workgroups = static_cast<int>(resident);
+    p.bytes = round_up(static_cast<size_t>(p.workgroups) * N * K * 4) + static_cast<size_t>(p.workgroups) * N * 4;
+    p.applies = true;
+    return p;
+}
+
+template <class T, int TM>
+void launch_narrow(const NarrowArgs<T>& a, const NarrowPlan& p, hipStream_t stream) {
+    const dim3 grid(p.workgroups), block(512);
+    if (p.blocks == 1) BOXCONV_LAUNCH("linear_narrow_grad", (narrow_grad_kernel<T, TM, 1>), grid, block, p.lds, stream, a);
+    else if (p.blocks == 2) BOXCONV_LAUNCH("linear_narrow_grad", (narrow_grad_kernel<T, TM, 2>), grid, block, p.lds, stream, a);
+    else BOXCONV_LAUNCH("linear_narrow_grad", (narrow_grad_kernel<T, TM, 4>), grid, block, p.lds, stream, a);
+}
+
+template <class T>
+hipError_t narrow_backward(const LinearGradCall& c, const NarrowPlan& p, void* workspace, hipStream_t stream) {
+    NarrowArgs<T> a = {};
+    a.x = static_cast<const T*>(c.x);
+    a.weight = static_cast<const T*>(c.weight);
+    a.dy = static_cast<const T*>(c.dy);
+    a.kept = c.kept;
+    a.ld_x = c.ld_x;
+    a.rows = c.rows;
+    a.dx = static_cast<T*>(c.dx);
+    a.dresidual = static_cast<T*>(c.dresidual);
+    a.N = static_cast<int>(c.N);
+    a.K = static_cast<int>(c.K);
+    a.activation = c.activation;
+    a.tiles = p.tiles;
+    float* parts = static_cast<float*>(workspace);
+    float* sums = parts + round_up(static_cast<size_t>(p.workgroups) * c.N * c.K * 4) / 4;
+    a.dweight = c.dweight ? parts : nullptr;
+    a.dbias = c.dbias ? sums : nullptr;
+    if (p.tm == 64) launch_narrow<T, 64>(a, p, stream);
+    else launch_narrow<T, 32>(a, p, stream);
+    if (c.dweight != nullptr) {
+        Tail<T> tail = {};
+        tail.out = static_cast<T*>(c.dweight);
+        tail.rows = c.N;
+        tail.cols = c.K;
+        tail.partial = parts;
+        join_parts(tail, p.workgroups, stream);
+    }
+    if (c.dbias != nullptr)
+        BOXCONV_LAUNCH("join_bias", (join_bias_kernel<T>), dim3(static_cast<unsigned>((c.N + 15) / 16)), dim3(1024), 0, stream, sums, static_cast<T*>(c.dbias), c.N,
+                       p.workgroups);
+    return hipGetLastError();
+}
+
 }  // namespace
 
 template <class T>
@@ -284,8 +363,9 @@ size_t linear_forward_workspace(int64_t rows, int64_t K, int64_t N) { return pro
 // [dz, unless the residual's gradient holds it][column sums per band][parts of a split product]
 template <class T>
 size_t linear_backward_workspace(int64_t rows, int64_t K, int64_t N) {
-    return round_up(static_cast<size_t>(rows) * N * sizeof(T)) + round_up(static_cast<size_t>(plan_bands(rows, N).bands) * N * 4) +
-           std::max(product_workspace<T>(rows, K, N), product_workspace<T>(N, K, rows));
+    return std::max(plan_narrow<T>(rows, K, N).bytes,
+                    round_up(static_cast<size_t>(rows) * N * sizeof(T)) + round_up(static_cast<size_t>(plan_bands(rows, N).bands) * N * 4) +
+                        std::max(product_workspace<T>(rows, K, N), product_workspace<T>(N, K, rows)));
 }
 
 template <class T>
@@ -306,6 +386,11 @@ hipError_t linear_forward(const LinearCall& c, void* workspace, hipStream_t stre
 
 template <class T>
 hipError_t linear_backward(const LinearGradCall& c, void* workspace, hipStream_t stream) {
+    const NarrowPlan narrow = plan_narrow<T>(c.rows, c.K, c.N);
+    const auto aligned = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+    if (narrow.applies && (c.dx != nullptr || c.dweight != nullptr) && c.x != nullptr && c.weight != nullptr && aligned(c.x) && aligned(c.weight) &&
+        aligned(c.dy) && aligned(c.kept) && c.ld_x % Vec<T>::kLen == 0 && c.ld_x >= c.K && c.ld_x < (int64_t(1) << 24))
+        return narrow_backward<T>(c, narrow, workspace, stream);
     char* ws = static_cast<char*>(workspace);
     T* scratch = reinterpret_cast<T*>(ws);
     ws += round_up(static_cast<size_t>(c.rows) * c.N * sizeof(T));

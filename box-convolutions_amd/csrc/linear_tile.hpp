@@ -179,31 +179,48 @@ __device__ __forceinline__ void finish(float (&z)[LEN], T (&y)[LEN], typename Sl
     }
 }
 
-// LEN consecutive elements of a row to or from memory, `valid` of them.
+// f(0), ..., f(N - 1) written out. (A loop over single elements that ends at a number known at run time becomes a copy
+// through the stack, whatever the unrolling.)
+template <int N, int I = 0, class F>
+__device__ __forceinline__ void each(F f) {
+    if constexpr (I < N) {
+        f(I);
+        each<N, I + 1>(f);
+    }
+}
+
+// LEN consecutive elements of a row to or from memory, `valid` of them, 16 bytes at a time.
 template <class E, int LEN>
 __device__ __forceinline__ void load_run(const E* p, E (&v)[LEN], int64_t valid) {
+    constexpr int P = LEN * sizeof(E) < 16 ? LEN : 16 / static_cast<int>(sizeof(E));
+    typedef E Packed __attribute__((ext_vector_type(P), aligned(sizeof(E))));
     if (valid >= LEN) {
-        typedef E Packed __attribute__((ext_vector_type(LEN), aligned(sizeof(E))));
-        const Packed q = *reinterpret_cast<const Packed*>(p);
 #pragma unroll
-        for (int i = 0; i < LEN; ++i) v[i] = q[i];
+        for (int k = 0; k < LEN; k += P) {
+            const Packed q = *reinterpret_cast<const Packed*>(p + k);
+#pragma unroll
+            for (int i = 0; i < P; ++i) v[k + i] = q[i];
+        }
     } else {
-#pragma unroll
-        for (int i = 0; i < LEN; ++i) v[i] = i < valid ? p[i] : E(0);
+        each<LEN>([&](int i) { v[i] = i < valid ? p[i] : E(0); });
     }
 }
 template <class E, int LEN>
 __device__ __forceinline__ void store_run(E* p, const E (&v)[LEN], int64_t valid) {
+    constexpr int P = LEN * sizeof(E) < 16 ? LEN : 16 / static_cast<int>(sizeof(E));
+    typedef E Packed __attribute__((ext_vector_type(P), aligned(sizeof(E))));
     if (valid >= LEN) {
-        typedef E Packed __attribute__((ext_vector_type(LEN), aligned(sizeof(E))));
-        Packed q;
 #pragma unroll
-        for (int i = 0; i < LEN; ++i) q[i] = v[i];
-        *reinterpret_cast<Packed*>(p) = q;
+        for (int k = 0; k < LEN; k += P) {
+            Packed q;
+#pragma unroll
+            for (int i = 0; i < P; ++i) q[i] = v[k + i];
+            *reinterpret_cast<Packed*>(p + k) = q;
+        }
     } else {
-#pragma unroll
-        for (int i = 0; i < LEN; ++i)
+        each<LEN>([&](int i) {
             if (i < valid) p[i] = v[i];
+        });
     }
 }
 
