@@ -81,6 +81,11 @@ __device__ __forceinline__ int lanes_per_group(int threads, int groups) {
     return w;
 }
 
+// Where LDS keeps slot f = V * lane + element: the lanes of one element side by side, so that neither the lanes' writes nor the
+// reads of one channel (every slab-th slot) meet in a bank.
+template <int V>
+__device__ __forceinline__ int kept_at(int f, int active) { return f % V * active + f / V; }
+
 // Per-slot statistics of a workgroup's lanes to per-group ones: count, mean and sum of squared deviations. Means are joined
 // before deviations, so nothing cancels however far the mean is from zero. `put(g, n, mean, m2)` gets the groups that start
 // at channel c0, counted from 0.
@@ -92,9 +97,9 @@ __device__ __forceinline__ void join_statistics(const float (&mean)[V], const fl
     if (t < L.active) {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            smean[t * V + j] = mean[j];
-            sm2[t * V + j] = m2[j];
-            sn[t * V + j] = count[j];
+            smean[j * L.active + t] = mean[j];
+            sm2[j * L.active + t] = m2[j];
+            sn[j * L.active + t] = count[j];
         }
     }
     __syncthreads();
@@ -110,7 +115,8 @@ __device__ __forceinline__ void join_statistics(const float (&mean)[V], const fl
         float n = 0.0f, sum = 0.0f;
         if (live)
             for (int c = first; c < per_group; c += across)
-                for (int s = g * per_group + c + row; s < slots; s += step) {
+                for (int f = g * per_group + c + row; f < slots; f += step) {
+                    const int s = kept_at<V>(f, L.active);
                     n += sn[s];
                     sum = fmaf(sn[s], smean[s], sum);
                 }
@@ -119,7 +125,8 @@ __device__ __forceinline__ void join_statistics(const float (&mean)[V], const fl
         float dev = 0.0f;
         if (live)
             for (int c = first; c < per_group; c += across)
-                for (int s = g * per_group + c + row; s < slots; s += step) {
+                for (int f = g * per_group + c + row; f < slots; f += step) {
+                    const int s = kept_at<V>(f, L.active);
                     const float d = smean[s] - mu;
                     dev += sm2[s] + sn[s] * d * d;
                 }
@@ -136,19 +143,48 @@ __device__ __forceinline__ void join_channels(const float (&a)[V], const float (
     if (t < L.active) {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            sa[t * V + j] = a[j];
-            sb[t * V + j] = b[j];
+            sa[j * L.active + t] = a[j];
+            sb[j * L.active + t] = b[j];
         }
     }
     __syncthreads();
     for (int c = t; c < L.slab; c += blockDim.x) {
         float x = 0.0f, y = 0.0f;
-        for (int s = c; s < slots; s += L.slab) {
+#pragma unroll 4
+        for (int f = c; f < slots; f += L.slab) {
+            const int s = kept_at<V>(f, L.active);
             x += sa[s];
             y += sb[s];
         }
         put(c, x, y);
     }
+}
+
+// Sums per slot to sums per group of the slab, left in `out` by group (and visible to the whole workgroup).
+template <int V>
+__device__ __forceinline__ void join_groups(const float (&v)[V], float* lds, float* out, const Lanes& L, int per_group) {
+    const int t = threadIdx.x, slots = L.active * V;
+    if (t < L.active) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) lds[j * L.active + t] = v[j];
+    }
+    __syncthreads();
+    const int groups = L.slab / per_group, width = lanes_per_group(blockDim.x, groups);
+    int across = width;
+    while (across > per_group) across >>= 1;
+    const int first = t % width % across, row = t % width / across * L.slab, step = width / across * L.slab;
+    for (int g0 = 0; g0 < groups; g0 += blockDim.x / width) {
+        const int g = g0 + t / width;
+        float sum = 0.0f;
+        if (g < groups)
+            for (int c = first; c < per_group; c += across) {
+#pragma unroll 4
+                for (int f = g * per_group + c + row; f < slots; f += step) sum += lds[kept_at<V>(f, L.active)];
+            }
+        sum = sum_over(sum, width);
+        if (g < groups && t % width == 0) out[g] = sum;
+    }
+    __syncthreads();
 }
 
 // ---- statistics of large items: partial results per workgroup --------------------------------------
@@ -563,7 +599,7 @@ norm_grad_kernel(NormBackwardArgs<T> a, const float2* __restrict__ totals, Lanes
 // ---- items that one workgroup's registers hold: one launch -----------------------------------------------
 template <class T, int ACT, int N>
 __global__ void __launch_bounds__(1024)
-norm_small_kernel(NormArgs<T> a, float* __restrict__ mean_out, float* __restrict__ rstd_out, Lanes L, int slabs) {
+norm_small_kernel(NormArgs<T> a, float* __restrict__ mean_out, float* __restrict__ rstd_out, Lanes L, int slabs, float m) {
     constexpr int V = Vec<T>::kLen;
     typedef typename Vec<T>::Type Packed;
     extern __shared__ float lds[];
@@ -577,50 +613,44 @@ norm_small_kernel(NormArgs<T> a, float* __restrict__ mean_out, float* __restrict
 #pragma unroll
         for (int k = 0; k < N; ++k) v[k] = Item<T>::load(x, off + k * L.stride, L.total);
     }
-    float mean[V], m2[V], count[V];
+    // the mean, then the deviations from it: both from registers
+    const int groups = L.slab / a.per_group, g0 = c0 / a.per_group;
+    float *sums = lds + L.active * V, *devs = sums + groups;
+    float v1[V], mean[V], scale[V], shift[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        float n = 0.0f, s = 0.0f, d2 = 0.0f;
+        v1[j] = 0.0f;
 #pragma unroll
         for (int k = 0; k < N; ++k)
-            if (live && off + k * L.stride + j < L.total) {
-                n += 1.0f;
-                s += static_cast<float>(v[k][j]);
-            }
-        const float mu = n > 0.0f ? s / n : 0.0f;
-#pragma unroll
-        for (int k = 0; k < N; ++k)
-            if (live && off + k * L.stride + j < L.total) {
-                const float d = static_cast<float>(v[k][j]) - mu;
-                d2 = fmaf(d, d, d2);
-            }
-        mean[j] = mu;
-        m2[j] = d2;
-        count[j] = n;
+            if (live) v1[j] += static_cast<float>(v[k][j]);    // (zeros beyond the end)
     }
-    float2* stats = reinterpret_cast<float2*>(lds + 3 * L.active * V);
-    const int g0 = c0 / a.per_group;
-    join_statistics<V>(mean, m2, count, lds, L, a.per_group, [&](int g, float n, float mu, float dev) {
-        const float rs = 1.0f / sqrtf(dev / n + a.eps);
-        stats[g] = {mu, rs};
-        if (mean_out != nullptr) {
-            mean_out[b * a.groups + g0 + g] = mu;
-            rstd_out[b * a.groups + g0 + g] = rs;
-        }
-    });
-    __syncthreads();
-    if (!live) return;
-    float scale[V], shift[V];
+    join_groups<V>(v1, lds, sums, L, a.per_group);
     Walk walk(Item<T>::channel(L, t, c0), a.per_group);
+    int group[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        const float2 s = stats[walk.g - g0];
-        const int c = walk.c;
-        mean[j] = s.x;
-        scale[j] = s.y * (a.weight ? load_param<T>(a.weight, a.float_params, c) : 1.0f);
-        shift[j] = a.bias ? load_param<T>(a.bias, a.float_params, c) : 0.0f;
+        group[j] = live ? walk.g - g0 : 0;
+        mean[j] = sums[group[j]] / m;            // (a product with 1/m would be off where all values are the same)
+        scale[j] = live && a.weight ? load_param<T>(a.weight, a.float_params, walk.c) : 1.0f;
+        shift[j] = live && a.bias ? load_param<T>(a.bias, a.float_params, walk.c) : 0.0f;
+        v1[j] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            if (live && off + k * L.stride + j < L.total) {
+                const float d = static_cast<float>(v[k][j]) - mean[j];
+                v1[j] = fmaf(d, d, v1[j]);
+            }
         walk.next(L.channels, a.per_group);
     }
+    join_groups<V>(v1, lds, devs, L, a.per_group);
+    if (mean_out != nullptr)
+        for (int g = t; g < groups; g += blockDim.x) {
+            mean_out[b * a.groups + g0 + g] = sums[g] / m;
+            rstd_out[b * a.groups + g0 + g] = 1.0f / sqrtf(devs[g] / m + a.eps);
+        }
+    if (!live) return;
+#pragma unroll
+    for (int j = 0; j < V; ++j) scale[j] *= 1.0f / sqrtf(devs[group[j]] / m + a.eps);
     T* y = a.y + b * L.total;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
@@ -880,7 +910,7 @@ NormPlan plan_norm(int64_t batch, int64_t pixels, int channels, int groups, int 
     L.active = p.threads / L.phase * L.phase;
     L.stride = static_cast<int64_t>(L.active) * V;
     const int64_t steps = (L.total + L.stride - 1) / L.stride;
-    const int64_t want = std::max<int64_t>(1, (2048 * 256 / p.threads + batch - 1) / batch);    // workgroups per item: eight waves per SIMD in all
+    const int64_t want = std::max<int64_t>(1, (1024 * 256 / p.threads + batch - 1) / batch);    // workgroups per item: four waves per SIMD in all
     p.chunk_steps = (steps + want - 1) / want;
     if (p.chunk_steps < kUnroll) p.chunk_steps = kUnroll;
     p.chunks = static_cast<int>((steps + p.chunk_steps - 1) / p.chunk_steps);
@@ -932,9 +962,10 @@ hipError_t forward(const NormCall& n, void* workspace, hipStream_t stream) {
     if (p.small)
         return with_activation(n.activation, [&](auto act) {
             return with_count(p.small, [&](auto count) {
-                const size_t lds = static_cast<size_t>(3) * L.active * V * 4 + static_cast<size_t>(L.slab / a.per_group) * 8;
+                const size_t lds = static_cast<size_t>(L.active) * V * 4 + static_cast<size_t>(L.slab / a.per_group) * 8;
                 BOXCONV_LAUNCH("norm_small", (norm_small_kernel<T, decltype(act)::value, decltype(count)::value>),
-                               dim3(static_cast<unsigned>(n.batch * p.slabs)), dim3(p.threads), lds, stream, a, n.mean, n.rstd, L, p.slabs);
+                               dim3(static_cast<unsigned>(n.batch * p.slabs)), dim3(p.threads), lds, stream, a, n.mean, n.rstd, L, p.slabs,
+                               static_cast<float>(n.pixels * a.per_group));
                 return hipGetLastError();
             });
         });

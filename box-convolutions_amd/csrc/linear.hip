@@ -68,11 +68,99 @@ product_kernel(Operand<T> a, Operand<T> b, Tail<T> tail, int64_t k_part, int64_t
         }
 }
 
+// ---- few rows ----------------------------------------------------------------------------------------------------
+// y for at most 16 * MT rows: the weight is all there is to read, once. A workgroup takes 16 columns n and its waves share k, each
+// with as many 16-byte loads of the weight in flight as it has; their sums meet in LDS. (16 x 16 matrix instructions: the weight's
+// rows are the first operand, so that a lane ends up with four consecutive n of one row.)
+typedef float Acc4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ Acc4 multiply_add16(Chunk b, Chunk a, Acc4 c, __bf16) {
+    typedef __bf16 Eight __attribute__((ext_vector_type(8)));
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(Eight, b), __builtin_bit_cast(Eight, a), c, 0, 0, 0);
+}
+__device__ __forceinline__ Acc4 multiply_add16(Chunk b, Chunk a, Acc4 c, _Float16) {
+    typedef _Float16 Eight __attribute__((ext_vector_type(8)));
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(Eight, b), __builtin_bit_cast(Eight, a), c, 0, 0, 0);
+}
+__device__ __forceinline__ Acc4 multiply_add16(Chunk b, Chunk a, Acc4 c, float) {
+    const Acc4 x = __builtin_bit_cast(Acc4, b), y = __builtin_bit_cast(Acc4, a);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], y[j], c, 0, 0, 0);
+    return c;
+}
+
+template <class T, int MT>
+__global__ void __launch_bounds__(1024)
+few_rows_kernel(Operand<T> a, Operand<T> b, Tail<T> tail) {
+    constexpr int V = Vec<T>::kLen, STEP = 4 * V, U = MT == 1 ? 8 : 4;     // k of one load of a wave; loads in flight
+    extern __shared__ Acc4 sums[];
+    const int l = threadIdx.x % 64, wave = threadIdx.x / 64, waves = blockDim.x / 64;
+    const int64_t n0 = blockIdx.x * 16ll, n = n0 + l % 16;
+    const int64_t steps = (a.depth + STEP - 1) / STEP, part = (steps + waves - 1) / waves;
+    const int64_t first = wave * part, last = min(steps, first + part);
+    Acc4 acc[MT] = {};
+    for (int64_t s = first; s < last; s += U) {
+        Chunk w[U], x[U][MT];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t k = (s + u) * STEP + l / 16 * V, valid = s + u < last ? a.depth - k : 0;
+            w[u] = load_chunk(b.p + n * b.ld + k, n < b.extent ? valid : 0);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                const int64_t m = 16 * i + l % 16;
+                x[u][i] = load_chunk(a.p + m * a.ld + k, m < a.extent ? valid : 0);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < MT; ++i) acc[i] = multiply_add16(w[u], x[u][i], acc[i], T());
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) sums[(wave * MT + i) * 64 + l] = acc[i];
+    __syncthreads();
+    for (int i = wave; i < MT; i += waves) {
+        float z[4] = {};
+        for (int w = 0; w < waves; ++w) {
+            const Acc4 v = sums[(w * MT + i) * 64 + l];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) z[r] += v[r];
+        }
+        apply_tail<T, 4>(tail, z, 16 * i + l % 16, n0 + 4 * (l / 16));
+    }
+}
+
+// Column sums of `bands` rows of `cols` floats, WIDE columns at a time (all, or `most` from `sums` on), the other threads side by
+// side down the rows: an order that only the shapes decide. part: a float per thread.
+template <class T, int WIDE>
+__device__ __forceinline__ void join_columns(float* part, const float* sums, T* out, int64_t cols, int bands, int64_t most = -1) {
+    const int x = threadIdx.x % WIDE, row = threadIdx.x / WIDE, rows = blockDim.x / WIDE;
+    if (most < 0) most = cols;
+    for (int64_t c0 = 0; c0 < most; c0 += WIDE) {
+        const int64_t c = c0 + x;
+        float s = 0.0f;
+        if (c < most) {
+#pragma unroll 8
+            for (int i = row; i < bands; i += rows) s += sums[i * cols + c];
+        }
+        part[threadIdx.x] = s;
+        __syncthreads();
+        for (int half = rows / 2; half > 0; half >>= 1) {
+            if (row < half) part[threadIdx.x] = s += part[threadIdx.x + half * WIDE];
+            __syncthreads();
+        }
+        if (row == 0 && c < most) out[c] = static_cast<T>(s);
+    }
+}
+
 // The parts of a split product, added in an order that only the shape decides, and the tail. A workgroup takes 256 / `lanes`
 // runs of eight columns; `lanes` (a power of two) threads share the parts of a run.
 template <class T>
-__global__ void __launch_bounds__(256) join_parts_kernel(Tail<T> tail, int splits, int64_t runs_per_row, int64_t runs, int lanes) {
+__global__ void __launch_bounds__(256) join_parts_kernel(Tail<T> tail, int splits, int64_t runs_per_row, int64_t runs, int lanes, const float* sums, T* dbias) {
     __shared__ float part[256][9];
+    if (sums != nullptr && blockIdx.x == gridDim.x - 1) {              // the last workgroup: column sums of the same parts
+        join_columns<T, 32>(&part[0][0], sums, dbias, tail.rows, splits);
+        return;
+    }
     const int per = 256 / lanes, lane = threadIdx.x / per;
     const int64_t id = blockIdx.x * static_cast<int64_t>(per) + threadIdx.x % per;
     const int64_t m = id / runs_per_row, n = id % runs_per_row * 8;
@@ -153,24 +241,10 @@ slope_kernel(const T* __restrict__ dy, const void* __restrict__ kept, T* __restr
     }
 }
 
-// dbias: the bands' sums, 16 columns by 64 rows of threads.
 template <class T>
 __global__ void __launch_bounds__(1024) join_bias_kernel(const float* __restrict__ sums, T* __restrict__ dbias, int64_t cols, int bands) {
-    __shared__ float part[64][17];
-    const int x = threadIdx.x % 16, row = threadIdx.x / 16;
-    const int64_t c = blockIdx.x * 16ll + x;
-    float s = 0.0f;
-    if (c < cols) {
-#pragma unroll 4
-        for (int i = row; i < bands; i += 64) s += sums[i * cols + c];
-    }
-    part[row][x] = s;
-    __syncthreads();
-    for (int half = 32; half > 0; half >>= 1) {
-        if (row < half) part[row][x] = s += part[row + half][x];
-        __syncthreads();
-    }
-    if (row == 0 && c < cols) dbias[c] = static_cast<T>(s);
+    __shared__ float part[1024];
+    join_columns<T, 16>(part, sums + blockIdx.x * 16ll, dbias + blockIdx.x * 16ll, cols, bands, std::min<int64_t>(16, cols - blockIdx.x * 16ll));
 }
 
 // ---- plans ---------------------------------------------------------------------------------------------------------
@@ -234,13 +308,24 @@ void launch_wide(const char* name, const Operand<T>& a, const Operand<T>& b, con
 }
 
 template <class T>
-void join_parts(const Tail<T>& tail, int splits, hipStream_t stream) {
+void join_parts(const Tail<T>& tail, int splits, hipStream_t stream, const float* sums = nullptr, T* dbias = nullptr) {
     const int64_t per_row = (tail.cols + 7) / 8, runs = per_row * tail.rows;
     int lanes = 1;                                         // threads for every CU, and at least four parts for each
     while (lanes < 64 && lanes * 8 <= splits && runs * lanes < 65536) lanes *= 2;
     const int64_t per = 256 / lanes;
-    BOXCONV_LAUNCH("join_parts", (join_parts_kernel<T>), dim3(static_cast<unsigned>((runs + per - 1) / per)), dim3(256), 0, stream, tail, splits, per_row, runs,
-                   lanes);
+    BOXCONV_LAUNCH("join_parts", (join_parts_kernel<T>), dim3(static_cast<unsigned>((runs + per - 1) / per + (sums != nullptr))), dim3(256), 0, stream, tail, splits,
+                   per_row, runs, lanes, sums, dbias);
+}
+
+// Few rows: as many waves (4 to 16) as have 8 loads each.
+template <class T, int MT>
+hipError_t few_rows(const Operand<T>& a, const Operand<T>& b, const Tail<T>& tail, hipStream_t stream) {
+    constexpr int STEP = 4 * Vec<T>::kLen;
+    int waves = 4;
+    while (waves < 16 && waves * 8 * STEP < a.depth) waves *= 2;
+    BOXCONV_LAUNCH("linear_few_rows", (few_rows_kernel<T, MT>), dim3(static_cast<unsigned>((tail.cols + 15) / 16)), dim3(waves * 64),
+                   static_cast<size_t>(waves) * MT * 1024, stream, a, b, tail);
+    return hipGetLastError();
 }
 
 template <class T, bool A_K, bool B_K>
@@ -347,9 +432,8 @@ hipError_t narrow_backward(const LinearGradCall& c, const NarrowPlan& p, void* w
         tail.rows = c.N;
         tail.cols = c.K;
         tail.partial = parts;
-        join_parts(tail, p.workgroups, stream);
-    }
-    if (c.dbias != nullptr)
+        join_parts(tail, p.workgroups, stream, a.dbias, static_cast<T*>(c.dbias));
+    } else if (c.dbias != nullptr)
         BOXCONV_LAUNCH("join_bias", (join_bias_kernel<T>), dim3(static_cast<unsigned>((c.N + 15) / 16)), dim3(1024), 0, stream, sums, static_cast<T*>(c.dbias), c.N,
                        p.workgroups);
     return hipGetLastError();
@@ -381,6 +465,8 @@ hipError_t linear_forward(const LinearCall& c, void* workspace, hipStream_t stre
     tail.ld_residual = c.ld_residual;
     tail.slope = static_cast<typename SlopeOf<T>::Type*>(c.slope);
     tail.activation = c.activation;
+    if (c.rows <= 16) return few_rows<T, 1>(a, b, tail, stream);
+    if (c.rows <= 32) return few_rows<T, 2>(a, b, tail, stream);
     return product<T, true, true>("linear", a, b, tail, static_cast<float*>(workspace), stream);
 }
 
