@@ -68,6 +68,31 @@ struct Walk {
     }
 };
 
+// weight and bias of a lane's V channels from `at` on (1 and 0 where there are none): all requested before any is used.
+template <class T, int V>
+__device__ __forceinline__ void lane_params(const void* weight, const void* bias, bool is_float, Walk at, int channels, int per_group, float (&w)[V], float (&b)[V]) {
+    int c[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        c[j] = at.c;
+        at.next(channels, per_group);
+        w[j] = 1.0f;
+        b[j] = 0.0f;
+    }
+    const auto get = [&](const void* p, float (&v)[V]) {
+        if (p == nullptr) return;
+        if (is_float) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[j] = static_cast<const float*>(p)[c[j]];
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[j] = static_cast<float>(static_cast<const T*>(p)[c[j]]);
+        }
+    };
+    get(weight, w);
+    get(bias, b);
+}
+
 // Sum over `width` (a power of two, at most 64) neighbouring lanes.
 __device__ __forceinline__ float sum_over(float v, int width) {
     for (int d = width >> 1; d > 0; d >>= 1) v += __shfl_xor(v, d);
@@ -160,9 +185,9 @@ __device__ __forceinline__ void join_channels(const float (&a)[V], const float (
     }
 }
 
-// Sums per slot to sums per group of the slab, left in `out` by group (and visible to the whole workgroup).
-template <int V>
-__device__ __forceinline__ void join_groups(const float (&v)[V], float* lds, float* out, const Lanes& L, int per_group) {
+// Sums per slot to sums per group of the slab: out[group] = result(sum), visible to the whole workgroup.
+template <int V, class F>
+__device__ __forceinline__ void join_groups(const float (&v)[V], float* lds, float* out, const Lanes& L, int per_group, F result) {
     const int t = threadIdx.x, slots = L.active * V;
     if (t < L.active) {
 #pragma unroll
@@ -182,7 +207,7 @@ __device__ __forceinline__ void join_groups(const float (&v)[V], float* lds, flo
                 for (int f = g * per_group + c + row; f < slots; f += step) sum += lds[kept_at<V>(f, L.active)];
             }
         sum = sum_over(sum, width);
-        if (g < groups && t % width == 0) out[g] = sum;
+        if (g < groups && t % width == 0) out[g] = result(sum);
     }
     __syncthreads();
 }
@@ -318,13 +343,12 @@ norm_apply_kernel(NormArgs<T> a, const float* __restrict__ mean, const float* __
     int64_t off = Item<T>::offset(L, t, 0);
     float mu[V], scale[V], shift[V];
     Walk at(Item<T>::channel(L, t, 0), a.per_group);
+    lane_params<T, V>(a.weight, a.bias, a.float_params, at, L.channels, a.per_group, scale, shift);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         const int64_t pair = b * a.groups + at.g;
-        const int c = at.c;
         mu[j] = mean[pair];
-        scale[j] = rstd[pair] * (a.weight ? load_param<T>(a.weight, a.float_params, c) : 1.0f);
-        shift[j] = a.bias ? load_param<T>(a.bias, a.float_params, c) : 0.0f;
+        scale[j] *= rstd[pair];
         at.next(L.channels, a.per_group);
     }
     off += chunk * chunk_steps * L.stride;
@@ -394,14 +418,12 @@ norm_sums_kernel(NormBackwardArgs<T> a, float* __restrict__ partial, Lanes L, in
         int64_t off = Item<T>::offset(L, t, 0);
         float mu[V], rs[V], w[V], bias[V];
         Walk at(Item<T>::channel(L, t, 0), a.per_group);
+        lane_params<T, V>(a.weight, a.bias, a.float_params, at, L.channels, a.per_group, w, bias);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const int64_t pair = b * a.groups + at.g;
-            const int c = at.c;
             mu[j] = a.mean[pair];
             rs[j] = a.rstd[pair];
-            w[j] = a.weight ? load_param<T>(a.weight, a.float_params, c) : 1.0f;
-            bias[j] = a.bias ? load_param<T>(a.bias, a.float_params, c) : 0.0f;
             at.next(L.channels, a.per_group);
         }
         off += chunk * chunk_steps * L.stride;
@@ -543,15 +565,15 @@ norm_grad_kernel(NormBackwardArgs<T> a, const float2* __restrict__ totals, Lanes
     // dx = A dz + B (x - mean) + D,  z = A (x - mean) + bias + r
     float mu[V], A[V], B[V], D[V], bias[V];
     Walk at(Item<T>::channel(L, t, 0), a.per_group);
+    lane_params<T, V>(a.weight, a.bias, a.float_params, at, L.channels, a.per_group, A, bias);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        const int g = at.g, c = at.c;
+        const int g = at.g;
         const float rs = a.rstd[b * a.groups + g];
         mu[j] = a.mean[b * a.groups + g];
-        A[j] = rs * (a.weight ? load_param<T>(a.weight, a.float_params, c) : 1.0f);
+        A[j] *= rs;
         B[j] = -rs * rs * terms[g].y;
         D[j] = -rs * terms[g].x;
-        bias[j] = a.bias ? load_param<T>(a.bias, a.float_params, c) : 0.0f;
         at.next(L.channels, a.per_group);
     }
     off += chunk * chunk_steps * L.stride;
@@ -597,71 +619,77 @@ norm_grad_kernel(NormBackwardArgs<T> a, const float2* __restrict__ totals, Lanes
 }
 
 // ---- items that one workgroup's registers hold: one launch -----------------------------------------------
-template <class T, int ACT, int N>
+// One compute unit does all of an item's work, so what counts is instructions: with WHOLE (items of whole vectors) no element
+// is looked at alone, offsets are 32 bits wide, and a group's quotients and root are taken once.
+template <class T, int ACT, int N, bool WHOLE>
 __global__ void __launch_bounds__(1024)
 norm_small_kernel(NormArgs<T> a, float* __restrict__ mean_out, float* __restrict__ rstd_out, Lanes L, int slabs, float m) {
     constexpr int V = Vec<T>::kLen;
     typedef typename Vec<T>::Type Packed;
     extern __shared__ float lds[];
-    const int t = threadIdx.x, c0 = blockIdx.x % slabs * L.slab;
-    const int64_t b = blockIdx.x / slabs;
+    const int t = threadIdx.x, c0 = blockIdx.x % static_cast<unsigned>(slabs) * L.slab, total = static_cast<int>(L.total), stride = static_cast<int>(L.stride);
+    const int64_t b = blockIdx.x / static_cast<unsigned>(slabs);
     const T *x = a.x + b * L.total, *r = a.residual ? a.residual + b * L.total : nullptr;
-    const int64_t off = Item<T>::offset(L, t, c0);
     const bool live = t < L.active;
+    const int off = live ? static_cast<int>(Item<T>::offset(L, t, c0)) : total;
+    // (requested without a branch, so that all are on their way at once; an item has at least one vector)
     Packed v[N];
-    if (live) {
 #pragma unroll
-        for (int k = 0; k < N; ++k) v[k] = Item<T>::load(x, off + k * L.stride, L.total);
-    }
+    for (int k = 0; k < N; ++k) v[k] = *reinterpret_cast<const Packed*>(x + (off + k * stride + V <= total ? off + k * stride : 0));
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+        if (off + k * stride + V > total) v[k] = WHOLE ? Packed{} : Item<T>::load(x, off + k * stride, total);
     // the mean, then the deviations from it: both from registers
     const int groups = L.slab / a.per_group, g0 = c0 / a.per_group;
-    float *sums = lds + L.active * V, *devs = sums + groups;
+    float *means = lds + L.active * V, *rstds = means + groups;
     float v1[V], mean[V], scale[V], shift[V];
+    Walk walk(Item<T>::channel(L, t, c0), a.per_group);
+    lane_params<T, V>(a.weight, a.bias, a.float_params, walk, L.channels, a.per_group, scale, shift);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         v1[j] = 0.0f;
 #pragma unroll
-        for (int k = 0; k < N; ++k)
-            if (live) v1[j] += static_cast<float>(v[k][j]);    // (zeros beyond the end)
+        for (int k = 0; k < N; ++k) v1[j] += static_cast<float>(v[k][j]);    // (zeros beyond the end)
     }
-    join_groups<V>(v1, lds, sums, L, a.per_group);
-    Walk walk(Item<T>::channel(L, t, c0), a.per_group);
+    join_groups<V>(v1, lds, means, L, a.per_group, [&](float sum) { return sum / m; });   // (a product with 1/m would be off where all values are the same)
     int group[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         group[j] = live ? walk.g - g0 : 0;
-        mean[j] = sums[group[j]] / m;            // (a product with 1/m would be off where all values are the same)
-        scale[j] = live && a.weight ? load_param<T>(a.weight, a.float_params, walk.c) : 1.0f;
-        shift[j] = live && a.bias ? load_param<T>(a.bias, a.float_params, walk.c) : 0.0f;
+        mean[j] = means[group[j]];
         v1[j] = 0.0f;
-#pragma unroll
-        for (int k = 0; k < N; ++k)
-            if (live && off + k * L.stride + j < L.total) {
-                const float d = static_cast<float>(v[k][j]) - mean[j];
-                v1[j] = fmaf(d, d, v1[j]);
-            }
         walk.next(L.channels, a.per_group);
     }
-    join_groups<V>(v1, lds, devs, L, a.per_group);
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        if (WHOLE && off + k * stride >= total) continue;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            if (!WHOLE && off + k * stride + j >= total) continue;
+            const float d = static_cast<float>(v[k][j]) - mean[j];
+            v1[j] = fmaf(d, d, v1[j]);
+        }
+    }
+    join_groups<V>(v1, lds, rstds, L, a.per_group, [&](float sum) { return 1.0f / sqrtf(sum / m + a.eps); });
     if (mean_out != nullptr)
         for (int g = t; g < groups; g += blockDim.x) {
-            mean_out[b * a.groups + g0 + g] = sums[g] / m;
-            rstd_out[b * a.groups + g0 + g] = 1.0f / sqrtf(devs[g] / m + a.eps);
+            mean_out[b * a.groups + g0 + g] = means[g];
+            rstd_out[b * a.groups + g0 + g] = rstds[g];
         }
-    if (!live) return;
 #pragma unroll
-    for (int j = 0; j < V; ++j) scale[j] *= 1.0f / sqrtf(devs[group[j]] / m + a.eps);
+    for (int j = 0; j < V; ++j) scale[j] *= rstds[group[j]];
     T* y = a.y + b * L.total;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-        const int64_t at = off + k * L.stride;
-        if (at >= L.total) break;
+        const int at = off + k * stride;
+        if (at >= total) continue;
         Packed q = {}, o;
-        if (r != nullptr) q = Item<T>::load(r, at, L.total);
+        if (r != nullptr) q = WHOLE ? *reinterpret_cast<const Packed*>(r + at) : Item<T>::load(r, at, total);
 #pragma unroll
         for (int j = 0; j < V; ++j)
             o[j] = static_cast<T>(activate<ACT>(fmaf(static_cast<float>(v[k][j]) - mean[j], scale[j], shift[j]) + static_cast<float>(q[j])));
-        Item<T>::store(y, at, L.total, o);
+        if (WHOLE) *reinterpret_cast<Packed*>(y + at) = o;
+        else Item<T>::store(y, at, total, o);
     }
 }
 
@@ -681,15 +709,13 @@ norm_small_grad_kernel(NormBackwardArgs<T> a, float2* __restrict__ totals, Lanes
     const int64_t end = t < L.active ? L.total : 0;
     float mu[V], rs[V], w[V], bias[V], sum[V], dot[V];
     Walk walk(Item<T>::channel(L, t, c0), a.per_group);
+    lane_params<T, V>(a.weight, a.bias, a.float_params, walk, L.channels, a.per_group, w, bias);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         const int64_t pair = b * a.groups + walk.g;
-        const int c = walk.c;
         sum[j] = dot[j] = 0.0f;
         mu[j] = a.mean[pair];
         rs[j] = a.rstd[pair];
-        w[j] = a.weight ? load_param<T>(a.weight, a.float_params, c) : 1.0f;
-        bias[j] = a.bias ? load_param<T>(a.bias, a.float_params, c) : 0.0f;
         walk.next(L.channels, a.per_group);
     }
     T* dr = a.dresidual ? a.dresidual + b * L.total : nullptr;
@@ -870,7 +896,10 @@ struct NormPlan {
 
 constexpr int kMostVectors = 8;        // of a lane of the one-launch kernels: what its registers hold of x
 
-NormPlan plan_norm(int64_t batch, int64_t pixels, int channels, int groups, int V) {
+// per_lane: vectors that a lane of a one-launch kernel should rather take than leave to more lanes. Forward: 8, all on their way at
+// once (one 28 x 28 x 40 item: 1024 lanes with 4 each take 11.8 us, half of it the instructions that every wave repeats). Backward: 1, its
+// loop waits for every vector.
+NormPlan plan_norm(int64_t batch, int64_t pixels, int channels, int groups, int V, int per_lane) {
     NormPlan p = {};
     Lanes& L = p.L;
     L.channels = L.slab = channels;
@@ -878,7 +907,7 @@ NormPlan plan_norm(int64_t batch, int64_t pixels, int channels, int groups, int 
     const int per_group = channels / groups;
     L.phase = channels / gcd(channels, V);
     p.slabs = 1;
-    if (L.phase > 1024) {
+    if (L.phase > 1024 || L.total < V) {
         p.any = true;
         return p;
     }
@@ -892,7 +921,7 @@ NormPlan plan_norm(int64_t batch, int64_t pixels, int channels, int groups, int 
         const int64_t vectors = slab == channels ? (L.total + V - 1) / V : pixels * phase;
         if (phase > 1024 || vectors > static_cast<int64_t>(1024 / phase * phase) * kMostVectors) continue;
         int threads = 64;
-        while (threads < 1024 && (threads < phase || vectors > threads / phase * phase)) threads *= 2;
+        while (threads < 1024 && (threads < phase || vectors > static_cast<int64_t>(threads / phase * phase) * per_lane)) threads *= 2;
         p.threads = threads;
         p.slabs = groups / groups_in_slab;
         L.slab = slab;
@@ -951,7 +980,7 @@ hipError_t forward(const NormCall& n, void* workspace, hipStream_t stream) {
     a.groups = n.groups;
     a.per_group = n.channels / n.groups;
     a.eps = n.eps;
-    const NormPlan p = plan_norm(n.batch, n.pixels, n.channels, n.groups, V);
+    const NormPlan p = plan_norm(n.batch, n.pixels, n.channels, n.groups, V, kMostVectors);
     const Lanes L = p.L;
     if (p.any)
         return with_activation(n.activation, [&](auto act) {
@@ -961,11 +990,17 @@ hipError_t forward(const NormCall& n, void* workspace, hipStream_t stream) {
         });
     if (p.small)
         return with_activation(n.activation, [&](auto act) {
+            const size_t lds = static_cast<size_t>(L.active) * V * 4 + static_cast<size_t>(L.slab / a.per_group) * 8;
+            const dim3 grid(static_cast<unsigned>(n.batch * p.slabs));
+            const float m = static_cast<float>(n.pixels * a.per_group);
+            if (L.total % V != 0) {
+                BOXCONV_LAUNCH("norm_small", (norm_small_kernel<T, decltype(act)::value, kMostVectors, false>), grid, dim3(p.threads), lds, stream, a, n.mean,
+                               n.rstd, L, p.slabs, m);
+                return hipGetLastError();
+            }
             return with_count(p.small, [&](auto count) {
-                const size_t lds = static_cast<size_t>(L.active) * V * 4 + static_cast<size_t>(L.slab / a.per_group) * 8;
-                BOXCONV_LAUNCH("norm_small", (norm_small_kernel<T, decltype(act)::value, decltype(count)::value>),
-                               dim3(static_cast<unsigned>(n.batch * p.slabs)), dim3(p.threads), lds, stream, a, n.mean, n.rstd, L, p.slabs,
-                               static_cast<float>(n.pixels * a.per_group));
+                BOXCONV_LAUNCH("norm_small", (norm_small_kernel<T, decltype(act)::value, decltype(count)::value, true>), grid, dim3(p.threads), lds, stream, a,
+                               n.mean, n.rstd, L, p.slabs, m);
                 return hipGetLastError();
             });
         });
@@ -1007,7 +1042,7 @@ hipError_t backward(const NormGradCall& n, void* workspace, hipStream_t stream) 
     a.float_params = n.float_params;
     a.groups = n.groups;
     a.per_group = n.channels / n.groups;
-    const NormPlan p = plan_norm(n.batch, n.pixels, n.channels, n.groups, V);
+    const NormPlan p = plan_norm(n.batch, n.pixels, n.channels, n.groups, V, 1);
     const Lanes L = p.L;
     const float inv_m = static_cast<float>(1.0 / (static_cast<double>(n.pixels) * a.per_group));
     float2* totals = static_cast<float2*>(workspace);
@@ -1047,7 +1082,7 @@ hipError_t backward(const NormGradCall& n, void* workspace, hipStream_t stream) 
 }  // namespace
 
 size_t norm_workspace_bytes(int64_t batch, int64_t pixels, int channels, int groups, int dtype, bool backward_pass) {
-    const NormPlan p = plan_norm(batch, pixels, channels, groups, dtype == kF32 ? 4 : 8);
+    const NormPlan p = plan_norm(batch, pixels, channels, groups, dtype == kF32 ? 4 : 8, backward_pass ? 1 : kMostVectors);
     const int64_t chunks = p.any || p.small ? 0 : batch * p.chunks;
     if (backward_pass) return static_cast<size_t>(batch * channels + chunks * channels) * 8;
     return chunks ? static_cast<size_t>(chunks * groups * 2 + batch * groups * 2) * 4 : 0;

@@ -21,21 +21,24 @@ product_kernel(Operand<T> a, Operand<T> b, Tail<T> tail, int64_t k_part, int64_t
     const int64_t k_begin = blockIdx.y * k_part, k_end = min(a.depth, k_begin + k_part);
     const int wave = threadIdx.x / 64, wm = wave / 2 * (TX / 2), wn = wave % 2 * (TX / 2);
     Acc16 acc[F][F] = {};                                   // [n block][m block]
-    Stage<T, A_K, TX, 256, false> sa;
-    Stage<T, B_K, TX, 256, true> sb;
-    if (k_begin < k_end) {
-        sa.load(a, m0, k_begin, k_end);
-        sb.load(b, n0, k_begin, k_end);
+    // tiles of 64: two of them on their way while one is multiplied (there is little else to hide memory's latency behind)
+    constexpr int AHEAD = TX == 64 ? 2 : 1;
+    Stage<T, A_K, TX, 256, false> sa[AHEAD];
+    Stage<T, B_K, TX, 256, true> sb[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+        sa[i].request(a, m0, k_begin + i * SA::KT, k_end);
+        sb[i].request(b, n0, k_begin + i * SA::KT, k_end);
     }
-    for (int64_t k0 = k_begin; k0 < k_end; k0 += SA::KT) {
+    const auto turn = [&](int64_t k0, Stage<T, A_K, TX, 256, false>& xa, Stage<T, B_K, TX, 256, true>& xb) {
+        xa.settle(a, m0, k0, k_end);
+        xb.settle(b, n0, k0, k_end);
         __syncthreads();
-        sa.store(ta);
-        sb.store(tb);
+        xa.store(ta);
+        xb.store(tb);
         __syncthreads();
-        if (k0 + SA::KT < k_end) {
-            sa.load(a, m0, k0 + SA::KT, k_end);
-            sb.load(b, n0, k0 + SA::KT, k_end);
-        }
+        xa.request(a, m0, k0 + AHEAD * SA::KT, k_end);         // (all of it beyond the end: one safe vector)
+        xb.request(b, n0, k0 + AHEAD * SA::KT, k_end);
 #pragma unroll
         for (int ks = 0; ks < SA::kSteps; ++ks) {
             Chunk fa[F], fb[F];
@@ -48,6 +51,12 @@ product_kernel(Operand<T> a, Operand<T> b, Tail<T> tail, int64_t k_part, int64_t
             for (int i = 0; i < F; ++i)
 #pragma unroll
                 for (int j = 0; j < F; ++j) acc[i][j] = multiply_add<T>(fb[i], fa[j], acc[i][j]);
+        }
+    };
+    for (int64_t k0 = k_begin; k0 < k_end; k0 += AHEAD * SA::KT) {
+        turn(k0, sa[0], sb[0]);
+        if constexpr (AHEAD == 2) {
+            if (k0 + SA::KT < k_end) turn(k0 + SA::KT, sa[AHEAD - 1], sb[AHEAD - 1]);
         }
     }
     const int l = threadIdx.x % 64;
@@ -98,23 +107,93 @@ few_rows_kernel(Operand<T> a, Operand<T> b, Tail<T> tail) {
     const int64_t steps = (a.depth + STEP - 1) / STEP, part = (steps + waves - 1) / waves;
     const int64_t first = wave * part, last = min(steps, first + part);
     Acc4 acc[MT] = {};
-    for (int64_t s = first; s < last; s += U) {
+    // (rows beyond the end repeat the last one: nobody stores their sums)
+    const T *w_row = b.p + min(n, b.extent - 1) * b.ld + l / 16 * V, *x_row[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) x_row[i] = a.p + min<int64_t>(16 * i + l % 16, a.extent - 1) * a.ld + l / 16 * V;
+    int64_t s = first;
+    for (; s + U <= last && (s + U) * STEP <= a.depth; s += U) {
         Chunk w[U], x[U][MT];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int64_t k = (s + u) * STEP + l / 16 * V, valid = s + u < last ? a.depth - k : 0;
-            w[u] = load_chunk(b.p + n * b.ld + k, n < b.extent ? valid : 0);
+            w[u] = __builtin_bit_cast(Chunk, *reinterpret_cast<const typename Vec<T>::Type*>(w_row + s * STEP + u * STEP));
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                const int64_t m = 16 * i + l % 16;
-                x[u][i] = load_chunk(a.p + m * a.ld + k, m < a.extent ? valid : 0);
-            }
+            for (int i = 0; i < MT; ++i) x[u][i] = __builtin_bit_cast(Chunk, *reinterpret_cast<const typename Vec<T>::Type*>(x_row[i] + s * STEP + u * STEP));
         }
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int i = 0; i < MT; ++i) acc[i] = multiply_add16(w[u], x[u][i], acc[i], T());
     }
+#pragma unroll 1
+    for (; s < last; ++s) {
+        const int64_t valid = a.depth - (s * STEP + l / 16 * V);
+        Chunk w = request_chunk(w_row + s * STEP, valid, b.p), x[MT];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) x[i] = request_chunk(x_row[i] + s * STEP, valid, a.p);
+        settle_chunk(w, w_row + s * STEP, valid);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            settle_chunk(x[i], x_row[i] + s * STEP, valid);
+            acc[i] = multiply_add16(w, x[i], acc[i], T());
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) sums[(wave * MT + i) * 64 + l] = acc[i];
+    __syncthreads();
+    for (int i = wave; i < MT; i += waves) {
+        float z[4] = {};
+        for (int w = 0; w < waves; ++w) {
+            const Acc4 v = sums[(w * MT + i) * 64 + l];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) z[r] += v[r];
+        }
+        apply_tail<T, 4>(tail, z, 16 * i + l % 16, n0 + 4 * (l / 16));
+    }
+}
+
+// The same for operands of whole aligned chunks: fragments read straight from memory touch another cache line with every lane,
+// and the address units take one line a cycle (16 rows of 4096 float16 through 1024 columns: 10.6 us). Here every wave brings
+// 512 bytes of k of its rows to LDS as they lie in memory, then reads its fragments there; chunk c of row r at c ^ r keeps
+// the 16 rows of an access in different banks.
+template <class T, int MT>
+__global__ void __launch_bounds__(512)
+few_whole_rows_kernel(Operand<T> a, Operand<T> b, Tail<T> tail) {
+    constexpr int V = Vec<T>::kLen, BLOCK = 32 * V, kRows = 16 * (MT + 1); // values of k in a block; rows of the weight, then of x
+    extern __shared__ Chunk blocks[];
+    const int l = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), waves = blockDim.x / 64;
+    const int64_t n0 = blockIdx.x * 16ll;
+    const int depth = static_cast<int>(a.depth), count = (depth + BLOCK - 1) / BLOCK, part = (count + waves - 1) / waves;
+    const Chunk* mine = blocks + wave * kRows * 32;
+    const unsigned to = static_cast<unsigned>(reinterpret_cast<uintptr_t>((LdsVoid)mine));
+    const auto describe = [](const T* p, int64_t elements) {
+        const uint64_t at = reinterpret_cast<uint64_t>(p);
+        const int64_t size = elements * static_cast<int64_t>(sizeof(T));
+        return Descriptor{static_cast<int>(at), static_cast<int>(at >> 32) & 0xffff, static_cast<int>(size < 0xffffff00ll ? static_cast<unsigned>(size) : 0xffffff00u), 0x00020000};
+    };
+    const int rows_w = static_cast<int>(min<int64_t>(16, b.extent - n0)), rows_x = static_cast<int>(a.extent);
+    const Descriptor dw = describe(b.p + n0 * b.ld, (rows_w - 1) * b.ld + depth), dx = describe(a.p, (rows_x - 1) * a.ld + depth);
+    Acc4 acc[MT] = {};
+    for (int s = wave * part; s < min(count, (wave + 1) * part); ++s) {
+#pragma unroll
+        for (int i = 0; i < kRows / 2; ++i) {                  // two rows at a time
+            const int r = 2 * i + l / 32, c = l % 32 ^ (r & 15), k = s * BLOCK + c * V, row = i < 8 ? r : r - 16;
+            const bool inside = k < depth && row < (i < 8 ? rows_w : rows_x);
+            const int64_t ld = i < 8 ? b.ld : a.ld;
+            load_to_lds(i < 8 ? dw : dx, inside ? static_cast<unsigned>((row * ld + k) * static_cast<int64_t>(sizeof(T))) : kNowhere, to + i * 1024);
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");       // (a wave's blocks are its own)
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) {
+            const int r = l % 16, c = 4 * ks + l / 16 ^ r;
+            const Chunk w = mine[r * 32 + c];
+#pragma unroll
+            for (int i = 0; i < MT; ++i) acc[i] = multiply_add16(w, mine[(16 + 16 * i + r) * 32 + c], acc[i], T());
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");     // read before the next block overwrites them
+    }
+    __syncthreads();
+    Acc4* sums = reinterpret_cast<Acc4*>(blocks);
 #pragma unroll
     for (int i = 0; i < MT; ++i) sums[(wave * MT + i) * 64 + l] = acc[i];
     __syncthreads();
@@ -317,14 +396,19 @@ void join_parts(const Tail<T>& tail, int splits, hipStream_t stream, const float
                    per_row, runs, lanes, sums, dbias);
 }
 
-// Few rows: as many waves (4 to 16) as have 8 loads each.
 template <class T, int MT>
 hipError_t few_rows(const Operand<T>& a, const Operand<T>& b, const Tail<T>& tail, hipStream_t stream) {
+    const dim3 grid(static_cast<unsigned>((tail.cols + 15) / 16));
+    int waves = 1;
+    if (whole_chunks<T, true>(a) && whole_chunks<T, true>(b) && a.ld >= a.depth && a.depth < (1 << 28)) {
+        constexpr int BLOCK = 32 * Vec<T>::kLen;
+        while (waves < (MT == 1 ? 8 : 4) && waves * BLOCK < a.depth) waves *= 2;
+        BOXCONV_LAUNCH("linear_few_rows", (few_whole_rows_kernel<T, MT>), grid, dim3(waves * 64), static_cast<size_t>(waves) * 16 * (MT + 1) * 512, stream, a, b, tail);
+        return hipGetLastError();
+    }
     constexpr int STEP = 4 * Vec<T>::kLen;
-    int waves = 4;
-    while (waves < 16 && waves * 8 * STEP < a.depth) waves *= 2;
-    BOXCONV_LAUNCH("linear_few_rows", (few_rows_kernel<T, MT>), dim3(static_cast<unsigned>((tail.cols + 15) / 16)), dim3(waves * 64),
-                   static_cast<size_t>(waves) * MT * 1024, stream, a, b, tail);
+    for (waves = 4; waves < 16 && waves * 8 * STEP < a.depth;) waves *= 2;    // waves with 8 loads each
+    BOXCONV_LAUNCH("linear_few_rows", (few_rows_kernel<T, MT>), grid, dim3(waves * 64), static_cast<size_t>(waves) * MT * 1024, stream, a, b, tail);
     return hipGetLastError();
 }
 
@@ -465,8 +549,8 @@ hipError_t linear_forward(const LinearCall& c, void* workspace, hipStream_t stre
     tail.ld_residual = c.ld_residual;
     tail.slope = static_cast<typename SlopeOf<T>::Type*>(c.slope);
     tail.activation = c.activation;
-    if (c.rows <= 16) return few_rows<T, 1>(a, b, tail, stream);
-    if (c.rows <= 32) return few_rows<T, 2>(a, b, tail, stream);
+    if (c.rows <= 16 && c.K >= Vec<T>::kLen) return few_rows<T, 1>(a, b, tail, stream);
+    if (c.rows <= 32 && c.K >= Vec<T>::kLen) return few_rows<T, 2>(a, b, tail, stream);
     return product<T, true, true>("linear", a, b, tail, static_cast<float*>(workspace), stream);
 }
 

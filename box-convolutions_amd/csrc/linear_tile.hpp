@@ -22,16 +22,23 @@ namespace {
 typedef float Acc16 __attribute__((ext_vector_type(16)));
 typedef unsigned Chunk __attribute__((ext_vector_type(4)));            // 16 bytes of an operand
 
-// A chunk of `valid` elements (none where it is <= 0, all where it is >= the vector's length); zeros beyond.
+// A chunk of `valid` elements (none where it is <= 0, all where it is >= the vector's length) and zeros beyond, in two parts:
+// what is requested does not depend on a branch, so that many can be on their way at once. `safe`: any whole vector.
 template <class T>
-__device__ __forceinline__ Chunk load_chunk(const T* p, int64_t valid) {
+__device__ __forceinline__ Chunk request_chunk(const T* p, int64_t valid, const T* safe) {
+    return __builtin_bit_cast(Chunk, *reinterpret_cast<const typename Vec<T>::Type*>(valid >= Vec<T>::kLen ? p : safe));
+}
+template <class T>
+__device__ __forceinline__ void settle_chunk(Chunk& c, const T* p, int64_t valid) {
     constexpr int V = Vec<T>::kLen;
-    if (valid >= V) return __builtin_bit_cast(Chunk, *reinterpret_cast<const typename Vec<T>::Type*>(p));
-    typename Vec<T>::Type v = {};
+    if (valid <= 0) c = Chunk{0, 0, 0, 0};
+    if (valid > 0 && valid < V) {
+        typename Vec<T>::Type v = {};
 #pragma unroll
-    for (int j = 0; j < V; ++j)
-        if (j < valid) v[j] = p[j];
-    return __builtin_bit_cast(Chunk, v);
+        for (int j = 0; j < V; ++j)
+            if (j < valid) v[j] = p[j];
+        c = __builtin_bit_cast(Chunk, v);
+    }
 }
 
 // Row of a 32-row block of B that row r of the matrix instruction's result stands for: result element i of lane l is row
@@ -74,17 +81,39 @@ struct Stage {
     static constexpr int N = Shape::kChunks / THREADS;
     Chunk v[N];
     static_assert(Shape::kChunks % THREADS == 0, "whole chunks per thread");
-    __device__ __forceinline__ void load(const Operand<T>& o, int64_t i0, int64_t k0, int64_t k_end) {
+    // Chunk s of this thread: where it is, and how many elements of it there are.
+    static __device__ __forceinline__ int64_t where(const Operand<T>& o, int s, int64_t i0, int64_t k0, int64_t k_end, const T*& p) {
+        const int id = threadIdx.x + s * THREADS, r = id / Shape::kRowChunks, c = id % Shape::kRowChunks;
+        if constexpr (K_MAJOR) {
+            const int64_t i = i0 + r, k = k0 + c * Shape::V;
+            p = o.p + i * o.ld + k;
+            return i < o.extent ? k_end - k : 0;
+        } else {
+            const int64_t k = k0 + r, i = i0 + c * Shape::V;
+            p = o.p + k * o.ld + i;
+            return k < k_end ? o.extent - i : 0;
+        }
+    }
+    // (an operand whose rows are shorter than a vector has no safe place to read one from)
+    __device__ __forceinline__ void request(const Operand<T>& o, int64_t i0, int64_t k0, int64_t k_end) {
+        const bool roomy = (K_MAJOR ? o.depth : o.extent) >= Shape::V;
+        const T* p;
+#pragma unroll
+        for (int s = 0; s < N; ++s) v[s] = Chunk{0, 0, 0, 0};
+        if (roomy) {
+#pragma unroll
+            for (int s = 0; s < N; ++s) {
+                const int64_t valid = where(o, s, i0, k0, k_end, p);
+                v[s] = request_chunk(p, valid, o.p);
+            }
+        }
+    }
+    __device__ __forceinline__ void settle(const Operand<T>& o, int64_t i0, int64_t k0, int64_t k_end) {
+        const T* p;
 #pragma unroll
         for (int s = 0; s < N; ++s) {
-            const int id = threadIdx.x + s * THREADS, r = id / Shape::kRowChunks, c = id % Shape::kRowChunks;
-            if constexpr (K_MAJOR) {
-                const int64_t i = i0 + r, k = k0 + c * Shape::V;
-                v[s] = load_chunk(o.p + i * o.ld + k, i < o.extent ? k_end - k : 0);
-            } else {
-                const int64_t k = k0 + r, i = i0 + c * Shape::V;
-                v[s] = load_chunk(o.p + k * o.ld + i, k < k_end ? o.extent - i : 0);
-            }
+            const int64_t valid = where(o, s, i0, k0, k_end, p);
+            settle_chunk(v[s], p, valid);
         }
     }
     __device__ __forceinline__ void store(Chunk* tile) const {
