@@ -22,23 +22,35 @@ namespace {
 typedef float Acc16 __attribute__((ext_vector_type(16)));
 typedef unsigned Chunk __attribute__((ext_vector_type(4)));            // 16 bytes of an operand
 
-// A chunk of `valid` elements (none where it is <= 0, all where it is >= the vector's length) and zeros beyond, in two parts:
-// what is requested does not depend on a branch, so that many can be on their way at once. `safe`: any whole vector.
-template <class T>
-__device__ __forceinline__ Chunk request_chunk(const T* p, int64_t valid, const T* safe) {
-    return __builtin_bit_cast(Chunk, *reinterpret_cast<const typename Vec<T>::Type*>(valid >= Vec<T>::kLen ? p : safe));
+// A chunk of `valid` elements (none where it is <= 0, all where it is >= the vector's length) and zeros beyond, in two parts.
+// What is requested does not depend on a branch, so that many can be on their way at once: the end of a row is read as the row's last
+// whole vector (rows have at least one) and shifted down, nothing as `safe`, any whole vector.
+template <class T, class I>
+__device__ __forceinline__ Chunk request_chunk(const T* p, I valid, const T* safe) {
+    constexpr int V = Vec<T>::kLen;
+    const T* from = valid <= 0 ? safe : p - (valid < V ? V - static_cast<int>(valid) : 0);
+    return __builtin_bit_cast(Chunk, *reinterpret_cast<const typename Vec<T>::Type*>(from));
 }
-template <class T>
-__device__ __forceinline__ void settle_chunk(Chunk& c, const T* p, int64_t valid) {
+template <class T, class I>
+__device__ __forceinline__ void settle_chunk(Chunk& c, I valid) {
     constexpr int V = Vec<T>::kLen;
     if (valid <= 0) c = Chunk{0, 0, 0, 0};
     if (valid > 0 && valid < V) {
-        typename Vec<T>::Type v = {};
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-            if (j < valid) v[j] = p[j];
-        c = __builtin_bit_cast(Chunk, v);
+        typedef uint64_t Halves __attribute__((ext_vector_type(2)));
+        Halves h = __builtin_bit_cast(Halves, c);
+        const int bits = (V - static_cast<int>(valid)) * static_cast<int>(sizeof(T)) * 8;        // 16 to 112
+        h = bits >= 64 ? Halves{h.y >> (bits - 64), 0} : Halves{h.x >> bits | h.y << (64 - bits), h.y >> bits};
+        c = __builtin_bit_cast(Chunk, h);
     }
+}
+// The same where rows are shorter than a vector.
+template <class T>
+__device__ __forceinline__ Chunk short_chunk(const T* p, int valid) {
+    typename Vec<T>::Type v = {};
+#pragma unroll
+    for (int j = 0; j < Vec<T>::kLen; ++j)
+        if (j < valid) v[j] = p[j];
+    return __builtin_bit_cast(Chunk, v);
 }
 
 // Row of a 32-row block of B that row r of the matrix instruction's result stands for: result element i of lane l is row
@@ -74,52 +86,62 @@ struct Operand {
     int64_t extent, depth;
 };
 
-// The chunks of a tile that one thread stages, through registers and with every bound checked.
+// The chunks of a tile that one thread of THREADS stages, through registers and with every bound checked.
 template <class T, bool K_MAJOR, int X, int THREADS, bool PERM>
 struct Stage {
     typedef TileShape<T, K_MAJOR, X, 8> Shape;
     static constexpr int N = Shape::kChunks / THREADS;
     Chunk v[N];
     static_assert(Shape::kChunks % THREADS == 0, "whole chunks per thread");
-    // Chunk s of this thread: where it is, and how many elements of it there are.
-    static __device__ __forceinline__ int64_t where(const Operand<T>& o, int s, int64_t i0, int64_t k0, int64_t k_end, const T*& p) {
-        const int id = threadIdx.x + s * THREADS, r = id / Shape::kRowChunks, c = id % Shape::kRowChunks;
-        if constexpr (K_MAJOR) {
-            const int64_t i = i0 + r, k = k0 + c * Shape::V;
-            p = o.p + i * o.ld + k;
-            return i < o.extent ? k_end - k : 0;
-        } else {
-            const int64_t k = k0 + r, i = i0 + c * Shape::V;
-            p = o.p + k * o.ld + i;
-            return k < k_end ? o.extent - i : 0;
-        }
-    }
-    // (an operand whose rows are shorter than a vector has no safe place to read one from)
-    __device__ __forceinline__ void request(const Operand<T>& o, int64_t i0, int64_t k0, int64_t k_end) {
-        const bool roomy = (K_MAJOR ? o.depth : o.extent) >= Shape::V;
-        const T* p;
-#pragma unroll
-        for (int s = 0; s < N; ++s) v[s] = Chunk{0, 0, 0, 0};
-        if (roomy) {
-#pragma unroll
-            for (int s = 0; s < N; ++s) {
-                const int64_t valid = where(o, s, i0, k0, k_end, p);
-                v[s] = request_chunk(p, valid, o.p);
-            }
-        }
-    }
-    __device__ __forceinline__ void settle(const Operand<T>& o, int64_t i0, int64_t k0, int64_t k_end) {
-        const T* p;
+    static_assert(!K_MAJOR || THREADS % Shape::kRowChunks == 0, "a thread's chunks of a K-major tile all have the same k");
+    const T* at[N];            // the thread's chunks in the tile that was last asked for
+    int room[N];               // elements of them inside the operand's extent, at most a vector
+    const T* safe;             // null: the operand's rows are shorter than a vector, and there is no safe place to read one from
+    int64_t step;
+
+    // The tile with rows from i0 and k from k0 on; `step`: k from one tile asked for to the next, in tiles.
+    __device__ __forceinline__ void start(const Operand<T>& o, int64_t i0, int64_t k0, int tiles) {
+        safe = (K_MAJOR ? o.depth : o.extent) >= Shape::V ? o.p : nullptr;
+        step = K_MAJOR ? static_cast<int64_t>(tiles) * Shape::KT : tiles * Shape::KT * o.ld;
 #pragma unroll
         for (int s = 0; s < N; ++s) {
-            const int64_t valid = where(o, s, i0, k0, k_end, p);
-            settle_chunk(v[s], p, valid);
+            const int id = threadIdx.x % THREADS + s * THREADS, r = id / Shape::kRowChunks, c = id % Shape::kRowChunks;
+            const int64_t i = i0 + (K_MAJOR ? r : c * Shape::V), k = k0 + (K_MAJOR ? c * Shape::V : r);
+            at[s] = o.p + (K_MAJOR ? i * o.ld + k : k * o.ld + i);
+            room[s] = static_cast<int>(min<int64_t>(max<int64_t>(o.extent - i, 0), Shape::V));
+            if (K_MAJOR && room[s] > 0) room[s] = Shape::V;
         }
+    }
+    // Elements of chunk s, with k_left values of k from the tile's corner on.
+    __device__ __forceinline__ int valid(int s, int k_left) const {
+        const int id = threadIdx.x % THREADS + s * THREADS, r = id / Shape::kRowChunks, c = id % Shape::kRowChunks;
+        if constexpr (K_MAJOR) return min(room[s], k_left - c * Shape::V);
+        else return r < k_left ? room[s] : 0;
+    }
+    __device__ __forceinline__ void request(int k_left) {
+#pragma unroll
+        for (int s = 0; s < N; ++s) v[s] = Chunk{0, 0, 0, 0};
+        if (safe != nullptr) {
+#pragma unroll
+            for (int s = 0; s < N; ++s) v[s] = request_chunk(at[s], valid(s, k_left), safe);
+        }
+    }
+    __device__ __forceinline__ void settle(int k_left) {
+#pragma unroll
+        for (int s = 0; s < N; ++s) settle_chunk<T>(v[s], valid(s, k_left));
+        if (safe == nullptr) {
+#pragma unroll
+            for (int s = 0; s < N; ++s) v[s] = short_chunk(at[s], valid(s, k_left));
+        }
+    }
+    __device__ __forceinline__ void advance() {
+#pragma unroll
+        for (int s = 0; s < N; ++s) at[s] += step;
     }
     __device__ __forceinline__ void store(Chunk* tile) const {
 #pragma unroll
         for (int s = 0; s < N; ++s) {
-            const int id = threadIdx.x + s * THREADS, r = id / Shape::kRowChunks, c = id % Shape::kRowChunks;
+            const int id = threadIdx.x % THREADS + s * THREADS, r = id / Shape::kRowChunks, c = id % Shape::kRowChunks;
             tile[Shape::template place<PERM>(r, c)] = v[s];
         }
     }
