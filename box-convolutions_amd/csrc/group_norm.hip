@@ -93,6 +93,20 @@ __device__ __forceinline__ void lane_params(const void* weight, const void* bias
     get(bias, b);
 }
 
+// u and z of one element, step by step as the formulas stand, each step rounded: forward and backward kernels form the very same
+// z, so that relu's derivative is 0 exactly where its value is. ((x - mean) comes first: x * scale + shift would lose what a
+// mean far from zero takes of the digits.)
+struct Formed { float u, z; };
+__device__ __forceinline__ Formed form(float x, float mean, float rstd, float w, float b, float r) {
+#pragma clang fp contract(off)
+    const float u = (x - mean) * rstd;
+    const float scaled = u * w;
+    const float shifted = scaled + b;
+    return {u, shifted + r};
+}
+// 1/sqrt(variance + eps), rounded once.
+__device__ __forceinline__ float inverse_deviation(float variance, float eps) { return static_cast<float>(1.0 / sqrt(static_cast<double>(variance + eps))); }
+
 // Sum over `width` (a power of two, at most 64) neighbouring lanes.
 __device__ __forceinline__ float sum_over(float v, int width) {
     for (int d = width >> 1; d > 0; d >>= 1) v += __shfl_xor(v, d);
@@ -311,7 +325,7 @@ norm_join_kernel(const float2* __restrict__ partial, float* __restrict__ mean, f
     dev = sum_of_workgroup(dev, lds);
     if (threadIdx.x == 0) {
         mean[pair] = mu;
-        rstd[pair] = 1.0f / sqrtf(dev / total + eps);
+        rstd[pair] = inverse_deviation(dev / total, eps);
     }
 }
 
@@ -326,7 +340,6 @@ struct NormArgs {
 };
 
 // ---- y from the statistics -------------------------------------------------------------------------
-// (x - mean) is formed first: x * scale + shift would lose what a mean far from zero takes of the digits.
 template <class T, int ACT>
 __global__ void __launch_bounds__(1024)
 norm_apply_kernel(NormArgs<T> a, const float* __restrict__ mean, const float* __restrict__ rstd, Lanes L,
@@ -341,14 +354,14 @@ norm_apply_kernel(NormArgs<T> a, const float* __restrict__ mean, const float* __
     const T *x = a.x + b * L.total, *r = a.residual ? a.residual + b * L.total : nullptr;
     T* y = a.y + b * L.total;
     int64_t off = Item<T>::offset(L, t, 0);
-    float mu[V], scale[V], shift[V];
+    float mu[V], rs[V], w[V], bias[V];
     Walk at(Item<T>::channel(L, t, 0), a.per_group);
-    lane_params<T, V>(a.weight, a.bias, a.float_params, at, L.channels, a.per_group, scale, shift);
+    lane_params<T, V>(a.weight, a.bias, a.float_params, at, L.channels, a.per_group, w, bias);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         const int64_t pair = b * a.groups + at.g;
         mu[j] = mean[pair];
-        scale[j] *= rstd[pair];
+        rs[j] = rstd[pair];
         at.next(L.channels, a.per_group);
     }
     off += chunk * chunk_steps * L.stride;
@@ -369,8 +382,7 @@ norm_apply_kernel(NormArgs<T> a, const float* __restrict__ mean, const float* __
             Packed o;
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const float z = fmaf(static_cast<float>(v[k][j]) - mu[j], scale[j], shift[j]) + static_cast<float>(q[k][j]);
-                o[j] = static_cast<T>(activate<ACT>(z));
+                o[j] = static_cast<T>(activate<ACT>(form(static_cast<float>(v[k][j]), mu[j], rs[j], w[j], bias[j], static_cast<float>(q[k][j])).z));
             }
             *reinterpret_cast<Packed*>(y + off + k * L.stride) = o;
         }
@@ -381,8 +393,7 @@ norm_apply_kernel(NormArgs<T> a, const float* __restrict__ mean, const float* __
         if (r != nullptr) q = Item<T>::load(r, off, L.total);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const float z = fmaf(static_cast<float>(v[j]) - mu[j], scale[j], shift[j]) + static_cast<float>(q[j]);
-            o[j] = static_cast<T>(activate<ACT>(z));
+            o[j] = static_cast<T>(activate<ACT>(form(static_cast<float>(v[j]), mu[j], rs[j], w[j], bias[j], static_cast<float>(q[j])).z));
         }
         Item<T>::store(y, off, L.total, o);
     }
@@ -431,9 +442,9 @@ norm_sums_kernel(NormBackwardArgs<T> a, float* __restrict__ partial, Lanes L, in
         auto add = [&](const Packed& v, const Packed& g, const Packed& q) {      // (beyond the end g is zero)
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const float u = (static_cast<float>(v[j]) - mu[j]) * rs[j];
+                const auto [u, z] = form(static_cast<float>(v[j]), mu[j], rs[j], w[j], bias[j], static_cast<float>(q[j]));
                 float dz = static_cast<float>(g[j]);
-                if constexpr (ACT != kActNone) dz *= slope<ACT>(fmaf(u, w[j], bias[j]) + static_cast<float>(q[j]));
+                if constexpr (ACT != kActNone) dz *= slope<ACT>(z);
                 sum[j] += dz;
                 dot[j] = fmaf(dz, u, dot[j]);
             }
@@ -460,9 +471,9 @@ norm_sums_kernel(NormBackwardArgs<T> a, float* __restrict__ partial, Lanes L, in
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 if (off + j >= L.total) continue;
-                const float u = (static_cast<float>(v[j]) - mu[j]) * rs[j];
+                const auto [u, z] = form(static_cast<float>(v[j]), mu[j], rs[j], w[j], bias[j], static_cast<float>(q[j]));
                 float dz = static_cast<float>(g[j]);
-                if constexpr (ACT != kActNone) dz *= slope<ACT>(fmaf(u, w[j], bias[j]) + static_cast<float>(q[j]));
+                if constexpr (ACT != kActNone) dz *= slope<ACT>(z);
                 sum[j] += dz;
                 dot[j] = fmaf(dz, u, dot[j]);
             }
@@ -562,29 +573,28 @@ norm_grad_kernel(NormBackwardArgs<T> a, const float2* __restrict__ totals, Lanes
     const T* r = ACT != kActNone && a.residual ? a.residual + b * L.total : nullptr;
     T *dx = a.dx ? a.dx + b * L.total : nullptr, *dr = a.dresidual ? a.dresidual + b * L.total : nullptr;
     int64_t off = Item<T>::offset(L, t, 0);
-    // dx = A dz + B (x - mean) + D,  z = A (x - mean) + bias + r
-    float mu[V], A[V], B[V], D[V], bias[V];
+    // dx = rstd w dz + D + E u
+    float mu[V], rs[V], w[V], D[V], E[V], bias[V];
     Walk at(Item<T>::channel(L, t, 0), a.per_group);
-    lane_params<T, V>(a.weight, a.bias, a.float_params, at, L.channels, a.per_group, A, bias);
+    lane_params<T, V>(a.weight, a.bias, a.float_params, at, L.channels, a.per_group, w, bias);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         const int g = at.g;
-        const float rs = a.rstd[b * a.groups + g];
+        rs[j] = a.rstd[b * a.groups + g];
         mu[j] = a.mean[b * a.groups + g];
-        A[j] *= rs;
-        B[j] = -rs * rs * terms[g].y;
-        D[j] = -rs * terms[g].x;
+        D[j] = -rs[j] * terms[g].x;
+        E[j] = -rs[j] * terms[g].y;
         at.next(L.channels, a.per_group);
     }
     off += chunk * chunk_steps * L.stride;
     const int64_t end = min(L.total, (chunk + 1) * chunk_steps * L.stride);
-    auto form = [&](const Packed& v, const Packed& g, const Packed& q, Packed& o, Packed& p) {
+    auto gradients = [&](const Packed& v, const Packed& g, const Packed& q, Packed& o, Packed& p) {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const float xc = static_cast<float>(v[j]) - mu[j];
+            const auto [u, z] = form(static_cast<float>(v[j]), mu[j], rs[j], w[j], bias[j], static_cast<float>(q[j]));
             float dz = static_cast<float>(g[j]);
-            if constexpr (ACT != kActNone) dz *= slope<ACT>(fmaf(xc, A[j], bias[j]) + static_cast<float>(q[j]));
-            o[j] = static_cast<T>(fmaf(A[j], dz, fmaf(B[j], xc, D[j])));
+            if constexpr (ACT != kActNone) dz *= slope<ACT>(z);
+            o[j] = static_cast<T>(fmaf(rs[j] * w[j], dz, fmaf(E[j], u, D[j])));
             p[j] = static_cast<T>(dz);
         }
     };
@@ -603,7 +613,7 @@ norm_grad_kernel(NormBackwardArgs<T> a, const float2* __restrict__ totals, Lanes
 #pragma unroll
         for (int k = 0; k < U; ++k) {
             Packed o, p;
-            form(v[k], g[k], q[k], o, p);
+            gradients(v[k], g[k], q[k], o, p);
             if (dx != nullptr) *reinterpret_cast<Packed*>(dx + off + k * L.stride) = o;
             if (dr != nullptr) *reinterpret_cast<Packed*>(dr + off + k * L.stride) = p;
         }
@@ -612,7 +622,7 @@ norm_grad_kernel(NormBackwardArgs<T> a, const float2* __restrict__ totals, Lanes
         const Packed v = Item<T>::load(x, off, L.total), g = Item<T>::load(dy, off, L.total);
         Packed q = {}, o, p;
         if (r != nullptr) q = Item<T>::load(r, off, L.total);
-        form(v, g, q, o, p);
+        gradients(v, g, q, o, p);
         if (dx != nullptr) Item<T>::store(dx, off, L.total, o);
         if (dr != nullptr) Item<T>::store(dr, off, L.total, p);
     }
@@ -642,9 +652,9 @@ norm_small_kernel(NormArgs<T> a, float* __restrict__ mean_out, float* __restrict
     // the mean, then the deviations from it: both from registers
     const int groups = L.slab / a.per_group, g0 = c0 / a.per_group;
     float *means = lds + L.active * V, *rstds = means + groups;
-    float v1[V], mean[V], scale[V], shift[V];
+    float v1[V], mean[V], rs[V], w[V], bias[V];
     Walk walk(Item<T>::channel(L, t, c0), a.per_group);
-    lane_params<T, V>(a.weight, a.bias, a.float_params, walk, L.channels, a.per_group, scale, shift);
+    lane_params<T, V>(a.weight, a.bias, a.float_params, walk, L.channels, a.per_group, w, bias);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         v1[j] = 0.0f;
@@ -670,14 +680,14 @@ norm_small_kernel(NormArgs<T> a, float* __restrict__ mean_out, float* __restrict
             v1[j] = fmaf(d, d, v1[j]);
         }
     }
-    join_groups<V>(v1, lds, rstds, L, a.per_group, [&](float sum) { return 1.0f / sqrtf(sum / m + a.eps); });
+    join_groups<V>(v1, lds, rstds, L, a.per_group, [&](float sum) { return inverse_deviation(sum / m, a.eps); });
     if (mean_out != nullptr)
         for (int g = t; g < groups; g += blockDim.x) {
             mean_out[b * a.groups + g0 + g] = means[g];
             rstd_out[b * a.groups + g0 + g] = rstds[g];
         }
 #pragma unroll
-    for (int j = 0; j < V; ++j) scale[j] *= rstds[group[j]];
+    for (int j = 0; j < V; ++j) rs[j] = rstds[group[j]];
     T* y = a.y + b * L.total;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
@@ -687,7 +697,7 @@ norm_small_kernel(NormArgs<T> a, float* __restrict__ mean_out, float* __restrict
         if (r != nullptr) q = WHOLE ? *reinterpret_cast<const Packed*>(r + at) : Item<T>::load(r, at, total);
 #pragma unroll
         for (int j = 0; j < V; ++j)
-            o[j] = static_cast<T>(activate<ACT>(fmaf(static_cast<float>(v[k][j]) - mean[j], scale[j], shift[j]) + static_cast<float>(q[j])));
+            o[j] = static_cast<T>(activate<ACT>(form(static_cast<float>(v[k][j]), mean[j], rs[j], w[j], bias[j], static_cast<float>(q[j])).z));
         if (WHOLE) *reinterpret_cast<Packed*>(y + at) = o;
         else Item<T>::store(y, at, total, o);
     }
@@ -726,9 +736,9 @@ norm_small_grad_kernel(NormBackwardArgs<T> a, float2* __restrict__ totals, Lanes
         if (r != nullptr) q = Item<T>::load(r, at, L.total);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const float u = (static_cast<float>(v[j]) - mu[j]) * rs[j];
+            const auto [u, z] = form(static_cast<float>(v[j]), mu[j], rs[j], w[j], bias[j], static_cast<float>(q[j]));
             float dz = static_cast<float>(g[j]);
-            if constexpr (ACT != kActNone) dz *= slope<ACT>(fmaf(u, w[j], bias[j]) + static_cast<float>(q[j]));
+            if constexpr (ACT != kActNone) dz *= slope<ACT>(z);
             p[j] = static_cast<T>(dz);
             if (at + j < L.total) {
                 sum[j] += dz;
@@ -764,9 +774,9 @@ norm_small_grad_kernel(NormBackwardArgs<T> a, float2* __restrict__ totals, Lanes
         if (r != nullptr) q = Item<T>::load(r, at, L.total);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const float u = (static_cast<float>(v[j]) - mu[j]) * rs[j];
+            const auto [u, z] = form(static_cast<float>(v[j]), mu[j], rs[j], w[j], bias[j], static_cast<float>(q[j]));
             float dz = static_cast<float>(g[j]);
-            if constexpr (ACT != kActNone) dz *= slope<ACT>(fmaf(u, w[j], bias[j]) + static_cast<float>(q[j]));
+            if constexpr (ACT != kActNone) dz *= slope<ACT>(z);
             o[j] = static_cast<T>(rs[j] * (fmaf(w[j], dz, -t1[j]) - u * t2[j]));
         }
         Item<T>::store(dx, at, L.total, o);
@@ -806,7 +816,7 @@ norm_any_kernel(NormArgs<T> a, float* __restrict__ mean_out, float* __restrict__
         const float d = static_cast<float>(a.x[base + i / a.per_group * channels + i % a.per_group]) - mu;
         s = fmaf(d, d, s);
     }
-    const float rs = 1.0f / sqrtf(workgroup_sum(s, lds) / static_cast<float>(n) + a.eps);
+    const float rs = inverse_deviation(workgroup_sum(s, lds) / static_cast<float>(n), a.eps);
     if (threadIdx.x == 0 && mean_out != nullptr) {
         mean_out[blockIdx.x] = mu;
         rstd_out[blockIdx.x] = rs;
@@ -814,25 +824,17 @@ norm_any_kernel(NormArgs<T> a, float* __restrict__ mean_out, float* __restrict__
     for (int64_t i = threadIdx.x; i < n; i += 256) {
         const int64_t at = base + i / a.per_group * channels + i % a.per_group;
         const int c = g * a.per_group + static_cast<int>(i % a.per_group);
-        float z = (static_cast<float>(a.x[at]) - mu) * rs;
-        if (a.weight) z *= load_param<T>(a.weight, a.float_params, c);
-        if (a.bias) z += load_param<T>(a.bias, a.float_params, c);
-        if (a.residual) z += static_cast<float>(a.residual[at]);
-        a.y[at] = static_cast<T>(activate<ACT>(z));
+        const float w = a.weight ? load_param<T>(a.weight, a.float_params, c) : 1.0f, shift = a.bias ? load_param<T>(a.bias, a.float_params, c) : 0.0f;
+        a.y[at] = static_cast<T>(activate<ACT>(form(static_cast<float>(a.x[at]), mu, rs, w, shift, a.residual ? static_cast<float>(a.residual[at]) : 0.0f).z));
     }
 }
 
+struct AnyElement { float u, w, dz; };
 template <class T, int ACT>
-__device__ __forceinline__ float any_dz(const NormBackwardArgs<T>& a, int64_t at, int c, float u) {
-    float dz = static_cast<float>(a.dy[at]);
-    if constexpr (ACT != kActNone) {
-        float z = u;
-        if (a.weight) z *= load_param<T>(a.weight, a.float_params, c);
-        if (a.bias) z += load_param<T>(a.bias, a.float_params, c);
-        if (a.residual) z += static_cast<float>(a.residual[at]);
-        dz *= slope<ACT>(z);
-    }
-    return dz;
+__device__ __forceinline__ AnyElement any_element(const NormBackwardArgs<T>& a, int64_t at, int c, float mu, float rs) {
+    const float w = a.weight ? load_param<T>(a.weight, a.float_params, c) : 1.0f, shift = a.bias ? load_param<T>(a.bias, a.float_params, c) : 0.0f;
+    const auto [u, z] = form(static_cast<float>(a.x[at]), mu, rs, w, shift, ACT != kActNone && a.residual ? static_cast<float>(a.residual[at]) : 0.0f);
+    return {u, w, static_cast<float>(a.dy[at]) * slope<ACT>(z)};
 }
 
 // One workgroup per (batch item, channel).
@@ -847,10 +849,10 @@ norm_any_sums_kernel(NormBackwardArgs<T> a, float2* __restrict__ totals, int64_t
     float s = 0.0f, d = 0.0f;
     for (int64_t i = threadIdx.x; i < pixels; i += 256) {
         const int64_t at = (b * pixels + i) * channels + c;
-        const float u = (static_cast<float>(a.x[at]) - mu) * rs, dz = any_dz<T, ACT>(a, at, c, u);
-        s += dz;
-        d = fmaf(dz, u, d);
-        if (a.dresidual) a.dresidual[at] = static_cast<T>(dz);
+        const AnyElement e = any_element<T, ACT>(a, at, c, mu, rs);
+        s += e.dz;
+        d = fmaf(e.dz, e.u, d);
+        if (a.dresidual) a.dresidual[at] = static_cast<T>(e.dz);
     }
     s = workgroup_sum(s, lds);
     d = workgroup_sum(d, lds);
@@ -877,9 +879,8 @@ norm_any_grad_kernel(NormBackwardArgs<T> a, const float2* __restrict__ totals, i
     for (int64_t i = threadIdx.x; i < n; i += 256) {
         const int c = g * a.per_group + static_cast<int>(i % a.per_group);
         const int64_t at = (b * pixels + i / a.per_group) * channels + c;
-        const float u = (static_cast<float>(a.x[at]) - mu) * rs, dz = any_dz<T, ACT>(a, at, c, u);
-        const float w = a.weight ? load_param<T>(a.weight, a.float_params, c) : 1.0f;
-        a.dx[at] = static_cast<T>(rs * (fmaf(w, dz, -s1) - u * s2));
+        const AnyElement e = any_element<T, ACT>(a, at, c, mu, rs);
+        a.dx[at] = static_cast<T>(rs * (fmaf(e.w, e.dz, -s1) - e.u * s2));
     }
 }
 

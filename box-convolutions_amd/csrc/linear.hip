@@ -7,37 +7,36 @@ namespace boxconv {
 namespace {
 
 // ---- any shape, alignment and size ---------------------------------------------------------------------------
-// A TX x TX tile by SHARE groups of four waves (2 x 2), which take the tiles of k in turn and add their sums up at the end; operands
-// go through registers into LDS with every bound checked. A turn is a chain (memory, LDS, barrier, products) of about 1 us,
-// so with few tiles of the result it pays to have four of them side by side: 1501 x 517 -> 333 float16, 9 tiles of k: 19 us
-// with one group. Tiles of 64 have two more on their way while one is multiplied. blockIdx.y: the part of k this workgroup sums.
-template <class T, bool A_K, bool B_K, int TX, int SHARE>
-__global__ void __launch_bounds__(256 * SHARE)
+// A workgroup of four waves (2 x 2) computes a TX x TX tile; operands go through registers into LDS with every bound checked,
+// the next tile's loads (of tiles of 64: the next two tiles') in flight while this one is multiplied. blockIdx.y: the part of k
+// this workgroup sums. (Four groups of waves that take the tiles of k in turn, for products of few tiles, were no better: 1501 x 517
+// -> 333 float16 12.4 against 13.1 us, 517 x 1501 -> 333 17.5 against 14.1 with k split over workgroups.)
+template <class T, bool A_K, bool B_K, int TX>
+__global__ void __launch_bounds__(256)
 product_kernel(Operand<T> a, Operand<T> b, Tail<T> tail, int64_t k_part, int64_t tiles_m, int64_t tiles_n) {
     typedef TileShape<T, A_K, TX, 8> SA;
     typedef TileShape<T, B_K, TX, 8> SB;
     constexpr int F = TX / 64;                              // 32 x 32 blocks of a wave along each axis
-    __shared__ Chunk lds[SHARE * (SA::kChunks + SB::kChunks)];
-    const int group = threadIdx.x / 256;
-    Chunk *ta = lds + group * (SA::kChunks + SB::kChunks), *tb = ta + SA::kChunks;
+    __shared__ Chunk lds[SA::kChunks + SB::kChunks];
+    Chunk *ta = lds, *tb = lds + SA::kChunks;
     const int64_t m0 = blockIdx.x / tiles_n * TX, n0 = blockIdx.x % tiles_n * TX;
     const int64_t k_begin = blockIdx.y * k_part, k_end = min(a.depth, k_begin + k_part);
-    const int wave = threadIdx.x % 256 / 64, wm = wave / 2 * (TX / 2), wn = wave % 2 * (TX / 2);
+    const int wave = threadIdx.x / 64, wm = wave / 2 * (TX / 2), wn = wave % 2 * (TX / 2);
     Acc16 acc[F][F] = {};                                   // [n block][m block]
-    constexpr int AHEAD = TX == 64 ? 2 : 1, EACH = SHARE * SA::KT;
+    constexpr int AHEAD = TX == 64 ? 2 : 1;
     Stage<T, A_K, TX, 256, false> sa[AHEAD];
     Stage<T, B_K, TX, 256, true> sb[AHEAD];
     const auto k_left = [&](int64_t k0) { return static_cast<int>(max<int64_t>(min<int64_t>(k_end - k0, 1 << 20), 0)); };
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
-        const int64_t k0 = k_begin + group * SA::KT + i * EACH;
-        sa[i].start(a, m0, k0, AHEAD * SHARE);
-        sb[i].start(b, n0, k0, AHEAD * SHARE);
+        const int64_t k0 = k_begin + i * SA::KT;
+        sa[i].start(a, m0, k0, AHEAD);
+        sb[i].start(b, n0, k0, AHEAD);
         sa[i].request(k_left(k0));
         sb[i].request(k_left(k0));
     }
     const auto turn = [&](int64_t k0, Stage<T, A_K, TX, 256, false>& xa, Stage<T, B_K, TX, 256, true>& xb) {
-        const int here = k_left(k0), later = k_left(k0 + AHEAD * EACH);
+        const int here = k_left(k0), later = k_left(k0 + AHEAD * SA::KT);
         xa.settle(here);
         xb.settle(here);
         __syncthreads();
@@ -62,23 +61,13 @@ product_kernel(Operand<T> a, Operand<T> b, Tail<T> tail, int64_t k_part, int64_t
                 for (int j = 0; j < F; ++j) acc[i][j] = multiply_add<T>(fb[i], fa[j], acc[i][j]);
         }
     };
-    for (int64_t k0 = k_begin; k0 < k_end; k0 += AHEAD * EACH) {   // (every group takes every turn: behind the end with zeros)
-        turn(k0 + group * SA::KT, sa[0], sb[0]);
+    for (int64_t k0 = k_begin; k0 < k_end; k0 += AHEAD * SA::KT) {
+        turn(k0, sa[0], sb[0]);
         if constexpr (AHEAD == 2) {
-            if (k0 + EACH < k_end) turn(k0 + EACH + group * SA::KT, sa[AHEAD - 1], sb[AHEAD - 1]);
+            if (k0 + SA::KT < k_end) turn(k0 + SA::KT, sa[AHEAD - 1], sb[AHEAD - 1]);
         }
     }
     const int l = threadIdx.x % 64;
-    if constexpr (SHARE > 1) {
-        static_assert(F == 1 && SHARE * (SA::kChunks + SB::kChunks) >= SHARE * 1024, "16 KB of sums per group");
-        Acc16* sums = reinterpret_cast<Acc16*>(lds);
-        __syncthreads();
-        if (group > 0) sums[(group * 4 + wave) * 64 + l] = acc[0][0];
-        __syncthreads();
-        if (group > 0) return;
-#pragma unroll
-        for (int g = 1; g < SHARE; ++g) acc[0][0] += sums[(g * 4 + wave) * 64 + l];
-    }
 #pragma unroll
     for (int i = 0; i < F; ++i)
 #pragma unroll
@@ -358,9 +347,9 @@ struct ProductPlan {
 // Measured on bfloat16 products, M x N x K: 8192 x 4096 x 2048 takes 107 us with 256 x 256 tiles, 137 with 128 x 128; 2048 x 2048 x
 // 4096 takes 78, 48 and, with 64 x 64, 52; 512 x 512 x 4096 33 with 128 x 128, 36 with 64 x 64 (none of them split). Tiles of
 // 256 x 128 were no better than 128 x 128 anywhere: their waves read as much from LDS per product.
-struct ProductShape { int tm, tn, share, resident; double fixed, each; };
-constexpr ProductShape kWide[] = {{256, 256, 1, 1, 0.0, 1.38}, {128, 128, 1, 2, 0.46, 0.21}, {64, 64, 1, 4, 0.44, 0.075}};
-constexpr ProductShape kAny[] = {{128, 128, 1, 2, 0.8, 0.4}, {64, 64, 1, 4, 0.65, 0.15}, {64, 64, 4, 1, 0.7, 0.4}};
+struct ProductShape { int tm, tn, resident; double fixed, each; };
+constexpr ProductShape kWide[] = {{256, 256, 1, 0.0, 1.38}, {128, 128, 2, 0.46, 0.21}, {64, 64, 4, 0.44, 0.075}};
+constexpr ProductShape kAny[] = {{128, 128, 2, 0.8, 0.4}, {64, 64, 4, 0.5, 0.15}};
 
 // The tile and the number of parts of k that promise the shortest time: rounds of workgroups, each as long as its steps and
 // about seven more for its start and its epilogue, and the parts' way through memory at 4 TB/s with one more launch.
@@ -374,10 +363,10 @@ ProductPlan plan_product(const ProductShape (&shapes)[N], int64_t m, int64_t n, 
         const ProductShape& s = shapes[i];
         const int64_t tm = (m + s.tm - 1) / s.tm, tn = (n + s.tn - 1) / s.tn, tiles = std::max<int64_t>(tm * tn, 1);
         for (int64_t splits = 1; splits <= 256 && splits * 2 <= std::max<int64_t>(steps, 2); splits *= 2) {
-            const int64_t part = (steps + splits - 1) / splits, parts = (steps + part - 1) / part, groups = tiles * parts, turns = (part + s.share - 1) / s.share;
+            const int64_t part = (steps + splits - 1) / splits, parts = (steps + part - 1) / part, groups = tiles * parts;
             const int64_t slots = 256 * s.resident, rounds = (groups + slots - 1) / slots;
             const double w = groups >= slots ? s.resident : static_cast<double>((groups + 255) / 256);
-            double t = static_cast<double>(rounds) * static_cast<double>(turns + 7) * (s.fixed + s.each * w);
+            double t = static_cast<double>(rounds) * static_cast<double>(part + 7) * (s.fixed + s.each * w);
             if (parts > 1) t += 4.0 + static_cast<double>(parts) * static_cast<double>(m) * static_cast<double>(n) * 8.0 / 4e6;
             if (best.splits == 0 || t < least) {
                 least = t;
@@ -444,9 +433,8 @@ hipError_t product(const char* name, Operand<T> a, Operand<T> b, Tail<T> tail, f
         }
     } else {
         const dim3 grid(static_cast<unsigned>(p.tiles_m * p.tiles_n), p.splits);
-        if (p.shape == 0) BOXCONV_LAUNCH(name, (product_kernel<T, A_K, B_K, 128, 1>), grid, dim3(256), 0, stream, a, b, tail, p.k_part, p.tiles_m, p.tiles_n);
-        else if (p.shape == 1) BOXCONV_LAUNCH(name, (product_kernel<T, A_K, B_K, 64, 1>), grid, dim3(256), 0, stream, a, b, tail, p.k_part, p.tiles_m, p.tiles_n);
-        else BOXCONV_LAUNCH(name, (product_kernel<T, A_K, B_K, 64, 4>), grid, dim3(1024), 0, stream, a, b, tail, p.k_part, p.tiles_m, p.tiles_n);
+        if (p.shape == 0) BOXCONV_LAUNCH(name, (product_kernel<T, A_K, B_K, 128>), grid, dim3(256), 0, stream, a, b, tail, p.k_part, p.tiles_m, p.tiles_n);
+        else BOXCONV_LAUNCH(name, (product_kernel<T, A_K, B_K, 64>), grid, dim3(256), 0, stream, a, b, tail, p.k_part, p.tiles_m, p.tiles_n);
     }
     if (p.splits > 1) join_parts(tail, p.splits, stream);
     return hipGetLastError();

@@ -259,3 +259,17 @@ def test_refusals(hip):
                        (lambda: GroupNormAct(2, 8, activation=1), "activation")):
         with pytest.raises(RuntimeError, match=match):
             bad()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("size", [(2, 20, 4, (9, 10)), (2, 64, 2, (50, 60)), (2, 32, 8, (130, 131)), (1, 1031, 1, (3, 5))])
+def test_relu_backward_sees_the_forwards_sign(hip, size, dtype):
+    """The residual's gradient is grad_output exactly where the output is positive and 0 elsewhere: the backward forms the
+    value in front of the activation again, to the same bits. (An output that is positive but rounds to 0 in float16
+    has a gradient all the same.)"""
+    c = case(*size, dtype, "relu", True, "float", seed=11)
+    out = {k: t.reshape(-1).cpu() for k, t in run(c).items()}
+    grad, live = c["grad"].reshape(-1), out["y"] > 0
+    assert torch.equal(out["residual"][live], grad[live])
+    rest = out["residual"][~live]
+    assert int((rest != 0).sum()) == 0 or dtype == torch.float16 and int((rest != 0).sum()) < 10
