@@ -384,7 +384,7 @@ norm_apply_kernel(NormArgs<T> a, const float* __restrict__ mean, const float* __
             for (int j = 0; j < V; ++j) {
                 o[j] = static_cast<T>(activate<ACT>(form(static_cast<float>(v[k][j]), mu[j], rs[j], w[j], bias[j], static_cast<float>(q[k][j])).z));
             }
-            *reinterpret_cast<Packed*>(y + off + k * L.stride) = o;
+            __builtin_nontemporal_store(o, reinterpret_cast<Packed*>(y + off + k * L.stride));
         }
     }
     for (; off < end; off += L.stride) {
@@ -614,8 +614,8 @@ norm_grad_kernel(NormBackwardArgs<T> a, const float2* __restrict__ totals, Lanes
         for (int k = 0; k < U; ++k) {
             Packed o, p;
             gradients(v[k], g[k], q[k], o, p);
-            if (dx != nullptr) *reinterpret_cast<Packed*>(dx + off + k * L.stride) = o;
-            if (dr != nullptr) *reinterpret_cast<Packed*>(dr + off + k * L.stride) = p;
+            if (dx != nullptr) __builtin_nontemporal_store(o, reinterpret_cast<Packed*>(dx + off + k * L.stride));
+            if (dr != nullptr) __builtin_nontemporal_store(p, reinterpret_cast<Packed*>(dr + off + k * L.stride));
         }
     }
     for (; off < end; off += L.stride) {
@@ -707,7 +707,7 @@ norm_small_kernel(NormArgs<T> a, float* __restrict__ mean_out, float* __restrict
 // per-channel values of its elements.
 template <class T, int ACT>
 __global__ void __launch_bounds__(1024)
-norm_small_grad_kernel(NormBackwardArgs<T> a, float2* __restrict__ totals, Lanes L, int slabs, float inv_m) {
+norm_small_grad_kernel(NormBackwardArgs<T> a, float2* __restrict__ totals, Lanes L, int slabs, float inv_m, bool only_item) {
     constexpr int V = Vec<T>::kLen;
     typedef typename Vec<T>::Type Packed;
     extern __shared__ float lds[];
@@ -752,6 +752,10 @@ norm_small_grad_kernel(NormBackwardArgs<T> a, float2* __restrict__ totals, Lanes
     join_channels<V>(sum, dot, lds, L, [&](int ch, float s, float d) {
         chan[ch] = {s, d};
         totals[b * L.channels + c0 + ch] = {s, d};
+        if (only_item) {
+            if (a.dbias) store_param<T>(a.dbias, a.float_params, c0 + ch, s);
+            if (a.dweight) store_param<T>(a.dweight, a.float_params, c0 + ch, d);
+        }
     });
     __syncthreads();
     group_terms(terms, [&](int ch) { return chan[ch]; }, a, c0, L.slab, inv_m);
@@ -892,9 +896,12 @@ struct NormPlan {
     int small;                 // > 0: one launch, so many vectors per lane
     int threads, slabs, chunks;
     int64_t chunk_steps;
+    int pieces;                // the same for the passes that write: workgroups per item, steps of each
+    int64_t piece_steps;
     Lanes L;
 };
 
+constexpr int kPieces = 4;             // of a chunk in the passes that write, while they have 16 steps each (537 MB of float32: 201 us with 1024 workgroups, 190 with 4096)
 constexpr int kMostVectors = 8;        // of a lane of the one-launch kernels: what its registers hold of x
 
 // per_lane: vectors that a lane of a one-launch kernel should rather take than leave to more lanes. Forward: 8, all on their way at
@@ -940,10 +947,14 @@ NormPlan plan_norm(int64_t batch, int64_t pixels, int channels, int groups, int 
     L.active = p.threads / L.phase * L.phase;
     L.stride = static_cast<int64_t>(L.active) * V;
     const int64_t steps = (L.total + L.stride - 1) / L.stride;
-    const int64_t want = std::max<int64_t>(1, (1024 * 256 / p.threads + batch - 1) / batch);    // workgroups per item: four waves per SIMD in all
+    const int64_t want = std::max<int64_t>(1, (512 * 256 / p.threads + batch - 1) / batch);    // workgroups per item: two waves per SIMD in all. What a
+    // workgroup does before and after its rows costs as much as 4 to 8 of its steps (33.5 M bfloat16 elements: statistics 20 us with 2048 workgroups, 17
+    // with 1024, 15 with 512; y 30, 26 and 27, and 46 with 4096)
     p.chunk_steps = (steps + want - 1) / want;
     if (p.chunk_steps < kUnroll) p.chunk_steps = kUnroll;
     p.chunks = static_cast<int>((steps + p.chunk_steps - 1) / p.chunk_steps);
+    p.piece_steps = std::min(p.chunk_steps, std::max<int64_t>((steps + kPieces * want - 1) / (kPieces * want), 16));
+    p.pieces = static_cast<int>((steps + p.piece_steps - 1) / p.piece_steps);
     return p;
 }
 
@@ -1013,14 +1024,14 @@ hipError_t forward(const NormCall& n, void* workspace, hipStream_t stream) {
         rstd = mean + pairs;
     }
     const int64_t chunk_pixels = p.chunk_steps * L.stride / L.channels, last_pixels = n.pixels - (p.chunks - 1) * chunk_pixels;
-    const int workgroups = static_cast<int>(n.batch * p.chunks);
-    BOXCONV_LAUNCH("norm_statistics", (norm_statistics_kernel<T>), dim3(workgroups), dim3(p.threads), static_cast<size_t>(3) * L.active * V * 4, stream, a.x,
+    const int workgroups = static_cast<int>(n.batch * p.pieces);
+    BOXCONV_LAUNCH("norm_statistics", (norm_statistics_kernel<T>), dim3(static_cast<unsigned>(n.batch * p.chunks)), dim3(p.threads), static_cast<size_t>(3) * L.active * V * 4, stream, a.x,
                    partial, L, p.chunk_steps, p.chunks, a.groups, a.per_group);
     BOXCONV_LAUNCH("norm_join", norm_join_kernel, dim3(static_cast<unsigned>(pairs)), dim3(256), 0, stream, partial, mean, rstd, p.chunks,
                    static_cast<float>(chunk_pixels * a.per_group), static_cast<float>(last_pixels * a.per_group), a.eps);
     return with_activation(n.activation, [&](auto act) {
         BOXCONV_LAUNCH("norm_apply", (norm_apply_kernel<T, decltype(act)::value>), dim3(workgroups), dim3(p.threads), 0, stream, a, mean, rstd, L,
-                       p.chunk_steps, p.chunks, workgroups);
+                       p.piece_steps, p.pieces, workgroups);
         return hipGetLastError();
     });
 }
@@ -1064,18 +1075,18 @@ hipError_t backward(const NormGradCall& n, void* workspace, hipStream_t stream) 
         return with_activation(n.activation, [&](auto act) {
             const size_t lds = static_cast<size_t>(2) * L.active * V * 4 + static_cast<size_t>(L.slab) * 8 + static_cast<size_t>(L.slab / a.per_group) * 8;
             BOXCONV_LAUNCH("norm_small_grad", (norm_small_grad_kernel<T, decltype(act)::value>), dim3(static_cast<unsigned>(n.batch * p.slabs)),
-                           dim3(p.threads), lds, stream, a, totals, L, p.slabs, inv_m);
-            if (params) BOXCONV_LAUNCH("norm_parameter", (norm_parameter_kernel<T>), param_grid, dim3(256), 0, stream, a, totals, n.batch, n.channels);
+                           dim3(p.threads), lds, stream, a, totals, L, p.slabs, inv_m, n.batch == 1);
+            if (params && n.batch > 1) BOXCONV_LAUNCH("norm_parameter", (norm_parameter_kernel<T>), param_grid, dim3(256), 0, stream, a, totals, n.batch, n.channels);
             return hipGetLastError();
         });
-    const int workgroups = static_cast<int>(n.batch * p.chunks), tiles = (n.channels + 15) / 16;
+    const int workgroups = static_cast<int>(n.batch * p.pieces), tiles = (n.channels + 15) / 16;
     return with_activation(n.activation, [&](auto act) {
-        BOXCONV_LAUNCH("norm_sums", (norm_sums_kernel<T, decltype(act)::value>), dim3(workgroups), dim3(p.threads), static_cast<size_t>(2) * L.active * V * 4,
+        BOXCONV_LAUNCH("norm_sums", (norm_sums_kernel<T, decltype(act)::value>), dim3(static_cast<unsigned>(n.batch * p.chunks)), dim3(p.threads), static_cast<size_t>(2) * L.active * V * 4,
                        stream, a, reinterpret_cast<float*>(partial), L, p.chunk_steps, p.chunks);
         BOXCONV_LAUNCH("norm_join_sums", norm_join_sums_kernel, dim3(static_cast<unsigned>(n.batch * tiles)), dim3(1024), 0, stream, partial, totals,
                        n.channels, p.chunks, tiles);
         BOXCONV_LAUNCH("norm_grad", (norm_grad_kernel<T, decltype(act)::value>), dim3(workgroups), dim3(p.threads), static_cast<size_t>(a.groups) * 8, stream,
-                       a, totals, L, p.chunk_steps, p.chunks, n.batch, inv_m, workgroups);
+                       a, totals, L, p.piece_steps, p.pieces, n.batch, inv_m, workgroups);
         return hipGetLastError();
     });
 }

@@ -284,7 +284,7 @@ __global__ void __launch_bounds__(256) join_parts_kernel(Tail<T> tail, int split
 // if not wanted; dz: null if not wanted. kept: y for relu, the kept slope for silu and gelu.
 template <class T>
 __global__ void __launch_bounds__(256)
-slope_kernel(const T* __restrict__ dy, const void* __restrict__ kept, T* __restrict__ dz, float* __restrict__ sums, int64_t rows,
+slope_kernel(const T* __restrict__ dy, const void* __restrict__ kept, T* __restrict__ dz, float* __restrict__ sums, T* __restrict__ dbias, int64_t rows,
              int64_t cols, int64_t band, int activation) {
     typedef typename SlopeOf<T>::Type S;
     __shared__ float part[8][256];
@@ -324,7 +324,8 @@ slope_kernel(const T* __restrict__ dy, const void* __restrict__ kept, T* __restr
     if (col < cols) {
         float s = 0.0f;
         for (int r = 0; r < 8; ++r) s += part[r][threadIdx.x];
-        sums[blockIdx.x * cols + col] = s;
+        if (gridDim.x == 1) dbias[col] = static_cast<T>(s);            // (one band: nothing to join)
+        else sums[blockIdx.x * cols + col] = s;
     }
 }
 
@@ -449,7 +450,7 @@ size_t product_workspace(int64_t m, int64_t n, int64_t k) {
 struct BandPlan { int64_t band; int bands; };
 BandPlan plan_bands(int64_t rows, int64_t cols) {
     const int64_t across = (cols + 255) / 256;
-    int64_t bands = std::max<int64_t>(1, std::min<int64_t>((1024 + across - 1) / across, (rows + 31) / 32));
+    int64_t bands = std::max<int64_t>(1, std::min<int64_t>((1024 + across - 1) / across, rows <= 256 ? 1 : (rows + 31) / 32));
     BandPlan p;
     p.band = (rows + bands - 1) / bands;
     p.band = std::max<int64_t>(8, (p.band + 7) / 8 * 8);
@@ -464,7 +465,7 @@ struct NarrowPlan {
     size_t lds, bytes;         // of LDS; of the partial sums
 };
 
-// Sizes that narrow_grad_kernel covers, and where it pays: at least four tiles for every workgroup that the chip holds.
+// Sizes that narrow_grad_kernel covers. Two tiles at least for a workgroup, while there are few.
 template <class T>
 NarrowPlan plan_narrow(int64_t rows, int64_t K, int64_t N) {
     constexpr int V = Vec<T>::kLen;
@@ -481,9 +482,9 @@ NarrowPlan plan_narrow(int64_t rows, int64_t K, int64_t N) {
     if (p.tm < 32) return p;
     const int64_t tiles = (rows + p.tm - 1) / p.tm;
     const int64_t resident = std::min<int64_t>(2, static_cast<int64_t>(kMaxDynamicLds / p.lds)) * 256;
-    if (tiles < 4 * resident) return p;
+    if (tiles > (int64_t(1) << 30) || tiles < 1) return p;
     p.tiles = static_cast<int>(tiles);
-    p.workgroups = static_cast<int>(resident);
+    p.workgroups = static_cast<int>(std::min(resident, (tiles + 1) / 2));
     p.bytes = round_up(static_cast<size_t>(p.workgroups) * N * K * 4) + static_cast<size_t>(p.workgroups) * N * 4;
     p.applies = true;
     return p;
@@ -585,9 +586,10 @@ hipError_t linear_backward(const LinearGradCall& c, void* workspace, hipStream_t
     }
     if (write != nullptr || c.dbias != nullptr) {
         const dim3 grid(bands.bands, static_cast<unsigned>((c.N + 255) / 256));
-        BOXCONV_LAUNCH("linear_slope", (slope_kernel<T>), grid, dim3(256), 0, stream, dy, c.kept, write, c.dbias ? sums : nullptr, c.rows, c.N, bands.band,
+        BOXCONV_LAUNCH("linear_slope", (slope_kernel<T>), grid, dim3(256), 0, stream, dy, c.kept, write, c.dbias ? sums : nullptr,
+                       static_cast<T*>(c.dbias), c.rows, c.N, bands.band,
                        c.activation);
-        if (c.dbias != nullptr)
+        if (c.dbias != nullptr && bands.bands > 1)
             BOXCONV_LAUNCH("join_bias", (join_bias_kernel<T>), dim3(static_cast<unsigned>((c.N + 15) / 16)), dim3(1024), 0, stream, sums, static_cast<T*>(c.dbias),
                            c.N, bands.bands);
         if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
