@@ -67,22 +67,7 @@ product_kernel(Operand<T> a, Operand<T> b, Tail<T> tail, int64_t k_part, int64_t
             if (k0 + SA::KT < k_end) turn(k0 + SA::KT, sa[AHEAD - 1], sb[AHEAD - 1]);
         }
     }
-    const int l = threadIdx.x % 64;
-#pragma unroll
-    for (int i = 0; i < F; ++i)
-#pragma unroll
-        for (int j = 0; j < F; ++j) {
-            const int64_t m = m0 + wm + 32 * j + l % 32, n = n0 + wn + 32 * i + 16 * (l / 32);
-            float z[16];
-#pragma unroll
-            for (int r = 0; r < 16; ++r) z[r] = acc[i][j][r];
-            if (tail.partial != nullptr) {
-                if (m < tail.rows && n < tail.cols)
-                    store_run<float, 16>(tail.partial + (blockIdx.y * tail.rows + m) * tail.cols + n, z, tail.cols - n);
-            } else {
-                apply_tail<T, 16>(tail, z, m, n);
-            }
-        }
+    store_blocks<T, F, F>(tail, acc, m0 + wm, n0 + wn, blockIdx.y);
 }
 
 // ---- few rows ----------------------------------------------------------------------------------------------------

@@ -275,10 +275,55 @@ __device__ __forceinline__ void store_run(E* p, const E (&v)[LEN], int64_t valid
     }
 }
 
-// The tail of LEN consecutive sums of row m from column n on.
+// The tail of LEN consecutive sums of row m from column n on, in two parts: what it reads is requested a block ahead, so that the
+// blocks of a tile do not wait for memory one after the other (256 x 256 tiles of 8192 x 2048 -> 4096 bfloat16: 3.5 us for the bias and
+// 13 for the residual when they did).
+template <class T, int LEN>
+struct TailInputs {
+    static constexpr int V = Vec<T>::kLen, CHUNKS = LEN / V;
+    Chunk bias[CHUNKS > 0 ? CHUNKS : 1], residual[CHUNKS > 0 ? CHUNKS : 1];
+    bool whole;                // all LEN values are there: requested; else the tail reads them one by one
+
+    __device__ __forceinline__ void request(const Tail<T>& t, int64_t m, int64_t n) {
+        whole = LEN % V == 0 && m < t.rows && n + LEN <= t.cols;
+        if (!whole) return;
+        if (t.bias != nullptr) {
+#pragma unroll
+            for (int k = 0; k < CHUNKS; ++k) bias[k] = __builtin_bit_cast(Chunk, *reinterpret_cast<const typename Vec<T>::Type*>(t.bias + n + k * V));
+        }
+        if (t.residual != nullptr) {
+#pragma unroll
+            for (int k = 0; k < CHUNKS; ++k)
+                residual[k] = __builtin_bit_cast(Chunk, *reinterpret_cast<const typename Vec<T>::Type*>(t.residual + m * t.ld_residual + n + k * V));
+        }
+    }
+    // z + what was requested
+    static __device__ __forceinline__ void add(float (&z)[LEN], const Chunk* from) {
+#pragma unroll
+        for (int i = 0; i < LEN; ++i) z[i] += static_cast<float>(__builtin_bit_cast(typename Vec<T>::Type, from[i / V])[i % V]);
+    }
+};
+
+template <class T, int LEN>
+__device__ __forceinline__ void finish_tail(const Tail<T>& t, float (&z)[LEN], int64_t m, int64_t n) {
+    typedef typename SlopeOf<T>::Type S;
+    const int64_t valid = t.cols - n;
+    T v[LEN];
+    S d[LEN];
+    const bool keep = t.slope != nullptr;
+    switch (t.activation) {
+        case kActRelu: finish<T, kActRelu, LEN>(z, v, d, false); break;
+        case kActSilu: finish<T, kActSilu, LEN>(z, v, d, keep); break;
+        case kActGelu: finish<T, kActGelu, LEN>(z, v, d, keep); break;
+        default: finish<T, kActNone, LEN>(z, v, d, false);
+    }
+    store_run<T, LEN>(t.out + m * t.cols + n, v, valid);
+    if (keep) store_run<S, LEN>(t.slope + m * t.cols + n, d, valid);
+}
+
+// All of it at once, at the ends of rows too.
 template <class T, int LEN>
 __device__ __forceinline__ void apply_tail(const Tail<T>& t, float (&z)[LEN], int64_t m, int64_t n) {
-    typedef typename SlopeOf<T>::Type S;
     if (m >= t.rows || n >= t.cols) return;
     const int64_t valid = t.cols - n;
     T v[LEN];
@@ -292,16 +337,42 @@ __device__ __forceinline__ void apply_tail(const Tail<T>& t, float (&z)[LEN], in
 #pragma unroll
         for (int i = 0; i < LEN; ++i) z[i] += static_cast<float>(v[i]);
     }
-    S d[LEN];
-    const bool keep = t.slope != nullptr;
-    switch (t.activation) {
-        case kActRelu: finish<T, kActRelu, LEN>(z, v, d, false); break;
-        case kActSilu: finish<T, kActSilu, LEN>(z, v, d, keep); break;
-        case kActGelu: finish<T, kActGelu, LEN>(z, v, d, keep); break;
-        default: finish<T, kActNone, LEN>(z, v, d, false);
+    finish_tail<T, LEN>(t, z, m, n);
+}
+
+// The blocks of a wave's part of a tile, from row m0 and column n0 on, to memory: sums as they are, or through the tail.
+template <class T, int FN, int FM>
+__device__ __forceinline__ void store_blocks(const Tail<T>& t, const Acc16 (&acc)[FN][FM], int64_t m0, int64_t n0, int64_t part) {
+    const int l = threadIdx.x % 64;
+    const auto row = [&](int b) { return m0 + 32 * (b % FM) + l % 32; };
+    const auto column = [&](int b) { return n0 + 32 * (b / FM) + 16 * (l / 32); };
+    if (t.partial != nullptr) {
+#pragma unroll
+        for (int b = 0; b < FN * FM; ++b) {
+            float z[16];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) z[r] = acc[b / FM][b % FM][r];
+            if (row(b) < t.rows && column(b) < t.cols)
+                store_run<float, 16>(t.partial + (part * t.rows + row(b)) * t.cols + column(b), z, t.cols - column(b));
+        }
+        return;
     }
-    store_run<T, LEN>(t.out + m * t.cols + n, v, valid);
-    if (keep) store_run<S, LEN>(t.slope + m * t.cols + n, d, valid);
+    TailInputs<T, 16> in[2];
+    in[0].request(t, row(0), column(0));
+#pragma unroll
+    for (int b = 0; b < FN * FM; ++b) {
+        if (b + 1 < FN * FM) in[(b + 1) & 1].request(t, row(b + 1), column(b + 1));
+        float z[16];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) z[r] = acc[b / FM][b % FM][r];
+        if (in[b & 1].whole) {
+            if (t.bias != nullptr) TailInputs<T, 16>::add(z, in[b & 1].bias);
+            if (t.residual != nullptr) TailInputs<T, 16>::add(z, in[b & 1].residual);
+            finish_tail<T, 16>(t, z, row(b), column(b));
+        } else {
+            apply_tail<T, 16>(t, z, row(b), column(b));
+        }
+    }
 }
 
 }  // namespace

@@ -154,22 +154,7 @@ product_wide_kernel(Operand<T> a, Operand<T> b, Tail<T> tail, int64_t k_part, un
         step(3, s + 1, s + 2, 0, kThird);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");           // nothing may still be on its way into this workgroup's LDS when it ends
-    const int l = threadIdx.x % 64;
-#pragma unroll
-    for (int i = 0; i < FN; ++i)
-#pragma unroll
-        for (int j = 0; j < FM; ++j) {
-            const int64_t m = m0 + wm + 32 * j + l % 32, n = n0 + wn + 32 * i + 16 * (l / 32);
-            float z[16];
-#pragma unroll
-            for (int r = 0; r < 16; ++r) z[r] = acc[i][j][r];
-            if (tail.partial != nullptr) {
-                if (m < tail.rows && n < tail.cols)
-                    store_run<float, 16>(tail.partial + (blockIdx.y * tail.rows + m) * tail.cols + n, z, tail.cols - n);
-            } else {
-                apply_tail<T, 16>(tail, z, m, n);
-            }
-        }
+    store_blocks<T, FN, FM>(tail, acc, m0 + wm, n0 + wn, blockIdx.y);
 }
 
 }  // namespace
