@@ -927,9 +927,11 @@ NormPlan plan_norm(int64_t batch, int64_t pixels, int channels, int groups, int 
         if (groups_in_slab < groups && (channels % V || slab % V || slab < 4 * V)) continue;
         const int phase = slab == channels ? L.phase : slab / V;
         const int64_t vectors = slab == channels ? (L.total + V - 1) / V : pixels * phase;
-        if (phase > 1024 || vectors > static_cast<int64_t>(1024 / phase * phase) * kMostVectors) continue;
+        if (phase > 1024 || vectors > static_cast<int64_t>(1024 / phase * phase) * kMostVectors || L.total > 0x7fffffff) continue;
         int threads = 64;
         while (threads < 1024 && (threads < phase || vectors > static_cast<int64_t>(threads / phase * phase) * per_lane)) threads *= 2;
+        const int active = threads / phase * phase;
+        if (static_cast<size_t>(2) * active * V * 4 + static_cast<size_t>(slab + groups_in_slab) * 8 > kMaxDynamicLds) continue;   // (the backward's)
         p.threads = threads;
         p.slabs = groups / groups_in_slab;
         L.slab = slab;

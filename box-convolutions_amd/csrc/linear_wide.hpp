@@ -136,7 +136,7 @@ product_wide_kernel(Operand<T> a, Operand<T> b, Tail<T> tail, int64_t k_part, un
         }
     };
     static_assert(SA::kSteps == 4, "four k steps in a stage");
-    constexpr int kThird = (kLoads + 2) / 3, kThirds = (2 * kLoads + 2) / 3;
+    constexpr int kThird = (kLoads + 1) / 2, kThirds = kLoads;
     if (steps > 0) {
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) load(0, i);

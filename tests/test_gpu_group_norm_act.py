@@ -53,7 +53,7 @@ def expected(c):
 SIZES = [(1, 1, 1, (1, 1)), (3, 4, 2, ()), (2, 6, 3, (5, 7)), (1, 40, 8, (28, 28)), (32, 40, 8, (7, 9)), (3, 48, 6, (33, 17)), (2, 5, 5, (9,)),
          (2, 128, 32, (64, 64)), (1, 320, 32, (40, 41)), (2, 1031, 1, (3, 5)), (1, 1100, 275, (2, 3)), (1, 2048, 32, (3, 3)), (1, 7, 1, (300, 301)),
          (2, 64, 1, (100, 99)), (1, 256, 8, (96, 20)), (5, 333, 3, (11, 13)), (1, 24, 24, (200, 211)), (1, 8192, 64, (3, 7)), (2, 16, 4, (1, 1)),
-         (1, 12, 2, (2, 3, 5)), (70, 32, 8, (65, 33))]
+         (1, 12, 2, (2, 3, 5)), (70, 32, 8, (65, 33)), (1, 8192, 8192, (5, 1)), (2, 4096, 4096, (7,))]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -245,7 +245,27 @@ def test_module_is_group_norm(hip):
     assert (got.double().cpu() - e).abs().max() <= 2.0 ** -18 * 8       # (two dozen roundings of values up to 8)
 
 
-def test_refusals(hip):
+@pytest.fixture(params=["C++", "Python"])
+def host_side(request, hip, monkeypatch):
+    """Both host sides of the operators (the second one is what runs where the C++ extension was not built)."""
+    if request.param == "Python":
+        monkeypatch.setattr(hip, "_glue", False)
+        assert hip.glue() is None
+    elif hip.glue() is None:
+        pytest.skip("the C++ extension was not built")
+    return request.param
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_both_host_sides(host_side, dtype):
+    for name in ACTS:
+        c = case(2, 12, 3, (9, 7), dtype, name, name != "relu", "float" if name else "none")
+        ref.check(run(c), expected(c))
+        other = run(c, layout=lambda t: t.movedim(-1, 1).contiguous())
+        assert all(torch.equal(t, other[k]) for k, t in run(c).items())
+
+
+def test_refusals(host_side):
     from box_convolution import GroupNormAct, group_norm_act
     x = torch.zeros(2, 8, 3, 3, device="cuda")
     one = torch.ones(8, device="cuda")

@@ -234,7 +234,27 @@ def test_pointwise_conv(hip):
         ref.check({"y": y.permute(0, 2, 3, 1)}, e)
 
 
-def test_refusals(hip):
+@pytest.fixture(params=["C++", "Python"])
+def host_side(request, hip, monkeypatch):
+    """Both host sides of the operators (the second one is what runs where the C++ extension was not built)."""
+    if request.param == "Python":
+        monkeypatch.setattr(hip, "_glue", False)
+        assert hip.glue() is None
+    elif hip.glue() is None:
+        pytest.skip("the C++ extension was not built")
+    return request.param
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_both_host_sides(host_side, dtype):
+    for name in ACTS:
+        args = case(70, 40, 24, dtype, name, bias=name != "relu", residual=name != "silu")
+        ref.check(run(*args), expected(*args, dtype))
+        args = case(0, 40, 24, dtype, name, residual=True)
+        ref.check(run(*args), expected(*args, dtype))
+
+
+def test_refusals(host_side):
     from box_convolution import PointwiseConv2d, linear_act
     x, w = torch.zeros(4, 8, device="cuda"), torch.zeros(6, 8, device="cuda")
     for bad, match in ((lambda: linear_act(x, w[:, :7]), "weight"), (lambda: linear_act(x, w[0]), "weight"),
