@@ -293,3 +293,25 @@ def test_relu_backward_sees_the_forwards_sign(hip, size, dtype):
     assert torch.equal(out["residual"][live], grad[live])
     rest = out["residual"][~live]
     assert int((rest != 0).sum()) == 0 or dtype == torch.float16 and int((rest != 0).sum()) < 10
+
+
+def test_more_than_2_31_elements(hip):
+    """An item of more than 2^31 elements: the result is the one of the same values in a smaller item (every row repeated:
+    the statistics are the same up to their rounding), at its far end too."""
+    from box_convolution import group_norm_act
+    C, repeats, small = 32, 1040, 64 * 1024
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    base = torch.randn(small, C, generator=gen, device="cuda")
+    x = base.to(torch.bfloat16).repeat(repeats, 1)[None].movedim(-1, 1).requires_grad_(True)
+    assert x.numel() > 1 << 31
+    y = group_norm_act(x, 8, activation="silu")
+    xs = base.to(torch.bfloat16)[None].movedim(-1, 1).requires_grad_(True)
+    ys = group_norm_act(xs, 8, activation="silu")
+    for k in (0, repeats // 2, repeats - 1):
+        part = y[:, :, k * small:(k + 1) * small]
+        assert (part.float() - ys.float()).abs().max() <= 2.0 ** -8 * ys.float().abs().max()          # one bfloat16 rounding either way
+    g = torch.randn(small, C, generator=gen, device="cuda").to(torch.bfloat16)
+    dxs = torch.autograd.grad(ys, xs, g[None].movedim(-1, 1))[0].float()
+    dx = torch.autograd.grad(y, x, g.repeat(repeats, 1)[None].movedim(-1, 1))[0]
+    for k in (0, repeats - 1):
+        assert (dx[:, :, k * small:(k + 1) * small].float() - dxs).abs().max() <= 2.0 ** -8 * dxs.abs().max()

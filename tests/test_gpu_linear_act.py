@@ -269,3 +269,32 @@ def test_refusals(host_side):
                        (lambda: PointwiseConv2d(3, 4).cuda()(torch.zeros(3, 5, 5, device="cuda")), "4 dimensions")):
         with pytest.raises(RuntimeError, match=match):
             bad()
+
+
+@pytest.mark.parametrize("K,N", [(64, 64), (33, 64)])
+def test_more_than_2_31_elements(hip, K, N):
+    """Rows whose elements lie beyond 2^31 of each tensor, through few channels (whole chunks, and any alignment): the first and
+    the last rows against the product of those rows alone, and the weight's gradient against the sum over halves."""
+    from box_convolution import linear_act
+    rows = (1 << 31) // 33 + 1000
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    x = torch.randn(rows, K, generator=gen, device="cuda", dtype=torch.bfloat16)
+    w = torch.randn(N, K, generator=gen, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    g = torch.randn(rows, N, generator=gen, device="cuda", dtype=torch.bfloat16)
+    assert x.numel() > 1 << 31 and g.numel() > 1 << 31
+    x.requires_grad_(True)
+    y = linear_act(x, w, activation="relu")
+    dx, dw = torch.autograd.grad(y, (x, w), g)
+    for part in (slice(0, 700), slice(rows - 700, rows)):
+        xs = x.detach()[part].clone().requires_grad_(True)
+        ys = linear_act(xs, w, activation="relu")
+        assert torch.equal(ys, y[part])
+        # (another kernel may take so few rows: one more rounding of dx)
+        ds = torch.autograd.grad(ys, xs, g[part])[0]
+        assert (ds.double() - dx[part].double()).abs().max() <= 2.0 ** -7 * ds.double().abs().max()
+    half = rows // 2
+    sums = torch.zeros(N, K, dtype=torch.float64, device="cuda")
+    for part in (slice(0, half), slice(half, rows)):
+        xs, ws = x.detach()[part], w.detach().clone().requires_grad_(True)
+        sums += torch.autograd.grad(linear_act(xs, ws, activation="relu"), ws, g[part])[0].double()
+    assert (sums - dw.double()).abs().max() <= 3 * 2.0 ** -8 * dw.double().abs().max()      # three bfloat16 roundings
