@@ -18,6 +18,27 @@ def _channels_last(t):
     return t if t.is_contiguous() else t.contiguous()
 
 
+class _OnceFunction(torch.autograd.Function):
+    """``apply(grad, *of)``: ``grad``, with a node that refuses to be differentiated."""
+
+    @staticmethod
+    def forward(ctx, grad, *of):
+        return grad.detach()
+
+    @staticmethod
+    def backward(ctx, grad_output):
+        raise RuntimeError("box_convolution: group_norm_act and linear_act can be differentiated once, not twice")
+
+
+def _once(grads, x, grad_output):
+    """The gradients of a backward pass. They come from kernels that leave no graph: where one is asked for, they must
+    not count as constants."""
+    if not torch.is_grad_enabled():
+        return grads
+    needs_grad = torch.empty(0, device=x.device, requires_grad=True)
+    return tuple(g if g is None else _OnceFunction.apply(g, x, grad_output, needs_grad) for g in grads)
+
+
 class GroupNormActFunction(torch.autograd.Function):
     """``apply(input, weight, bias, residual, num_groups, activation, eps)``, tensors ``[B, ..., C]``, contiguous."""
 
@@ -30,13 +51,12 @@ class GroupNormActFunction(torch.autograd.Function):
         return output
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad_output):
         input, weight, bias, residual, mean, rstd = ctx.saved_tensors
         grads = _native.group_norm_backward(
             input, ctx.num_groups, weight, bias, residual, ctx.activation, mean, rstd, grad_output.contiguous(),
             ctx.needs_input_grad[:4])
-        return (*grads, None, None, None)
+        return (*_once(grads, input, grad_output), None, None, None)
 
 
 def group_norm_act(input, num_groups, weight=None, bias=None, residual=None, activation=None, eps=1e-5):
@@ -90,11 +110,10 @@ class LinearActFunction(torch.autograd.Function):
         return output
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad_output):
         input, weight, kept = ctx.saved_tensors
         grads = _native.linear_backward(input, weight, kept, ctx.activation, grad_output.contiguous(), ctx.needs_input_grad[:4])
-        return (*grads, None)
+        return (*_once(grads, input, grad_output), None)
 
 
 def linear_act(input, weight, bias=None, residual=None, activation=None):

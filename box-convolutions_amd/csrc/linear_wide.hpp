@@ -81,7 +81,7 @@ __device__ __forceinline__ void settle() { asm volatile("s_waitcnt vmcnt(%0) lgk
 
 // TM x TN tile by WM x WN waves, each with (TM/WM) x (TN/WN). Two stages of 128 bytes of k. The barrier of a stage stands in front
 // of its last k step, whose fragments are in registers by then: from there on its LDS takes the stage after next, whose loads are
-// issued one at a time between the products of three k steps (eight waves that issue theirs all at once keep the memory pipe,
+// issued one at a time between the products of two k steps (eight waves that issue theirs all at once keep the memory pipe,
 // and with it themselves, busy for half a stage), and the next stage's first fragments are read between the last products.
 template <class T, bool A_K, bool B_K, int TM, int TN, int WM, int WN>
 __global__ void __launch_bounds__(WM * WN * 64)
@@ -136,7 +136,7 @@ product_wide_kernel(Operand<T> a, Operand<T> b, Tail<T> tail, int64_t k_part, un
         }
     };
     static_assert(SA::kSteps == 4, "four k steps in a stage");
-    constexpr int kThird = (kLoads + 1) / 2, kThirds = kLoads;
+    constexpr int kHalf = (kLoads + 1) / 2;
     if (steps > 0) {
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) load(0, i);
@@ -144,14 +144,14 @@ product_wide_kernel(Operand<T> a, Operand<T> b, Tail<T> tail, int64_t k_part, un
 #pragma unroll
         for (int i = 0; i < kReads; ++i) read(0, 0, i);
 #pragma unroll
-        for (int i = 0; i < kThird; ++i) load(1, i);
+        for (int i = 0; i < kHalf; ++i) load(1, i);
     }
     for (int s = 0; s < steps; ++s) {
-        step(0, s, s + 1, kThird, kThirds);
-        step(1, s, s + 1, kThirds, kLoads);
+        step(0, s, s + 1, kHalf, kLoads);
+        step(1, s, 0, 0, 0);
         step(2, s, 0, 0, 0);
         settle<0>();                                           // stage s + 1 has landed, and the rest of this one is in registers
-        step(3, s + 1, s + 2, 0, kThird);
+        step(3, s + 1, s + 2, 0, kHalf);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");           // nothing may still be on its way into this workgroup's LDS when it ends
     store_blocks<T, FN, FM>(tail, acc, m0 + wm, n0 + wn, blockIdx.y);

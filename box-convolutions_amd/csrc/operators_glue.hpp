@@ -64,6 +64,26 @@ std::vector<bool> needed(torch::autograd::AutogradContext* ctx, const std::vecto
     return out;
 }
 
+// The gradients are formed by kernels that leave no graph. Where a graph of the backward is asked for, every gradient gets a
+// node that refuses to be differentiated, in place of none, which would count as a constant.
+struct Once : public torch::autograd::Function<Once> {
+    static at::Tensor forward(torch::autograd::AutogradContext*, const at::Tensor& grad, const at::Tensor& /*x*/, const at::Tensor& /*grad_output*/,
+                              const at::Tensor& /*needs_grad: that there always is a node*/) {
+        return grad.detach();
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext*, torch::autograd::variable_list) {
+        TORCH_CHECK(false, "box_convolution: group_norm_act and linear_act can be differentiated once, not twice");
+    }
+};
+
+torch::autograd::variable_list once(torch::autograd::variable_list grads, const at::Tensor& x, const at::Tensor& grad_output) {
+    if (!at::GradMode::is_enabled()) return grads;
+    const at::Tensor needs_grad = at::empty({0}, x.options()).requires_grad_();
+    for (at::Tensor& g : grads)
+        if (g.defined()) g = Once::apply(g, x, grad_output, needs_grad);
+    return grads;
+}
+
 Optional saved_or_none(const at::Tensor& t) { return t.defined() ? Optional(t) : std::nullopt; }
 
 // ---- group norm ------------------------------------------------------------------------------------------
@@ -140,7 +160,7 @@ struct GroupNormAct : public torch::autograd::Function<GroupNormAct> {
         for (int k = 1; k <= 2; ++k)
             if (need[k]) grads[k] = x.numel() ? at::empty({n.channels}, param_options) : at::zeros({n.channels}, param_options);
         if (need[3]) grads[3] = empty_channels_last(x);
-        if (x.numel() == 0) return grads;
+        if (x.numel() == 0) return once(grads, x, g);
         const int code = type_code(x.scalar_type());
         const size_t nbytes = g_operators.norm_bytes(n.batch, n.pixels, n.channels, groups, code, 1);
         const at::Tensor ws = scratch(nbytes, x);
@@ -150,7 +170,7 @@ struct GroupNormAct : public torch::autograd::Function<GroupNormAct> {
                                            n.batch, n.pixels, n.channels, groups, act, address(ws), nbytes,
                                            reinterpret_cast<void*>(ctx->saved_data["stream"].toInt())),
                  "group_norm backward");
-        return grads;
+        return once(grads, x, g);
     }
 };
 
@@ -250,7 +270,7 @@ struct LinearAct : public torch::autograd::Function<LinearAct> {
         if (need[1]) grads[1] = fresh({N, K});
         if (need[2]) grads[2] = fresh({N});
         if (need[3]) grads[3] = act ? at::empty_like(g) : g;   // without an activation the residual's gradient is grad_output itself
-        if (none) return grads;
+        if (none) return once(grads, x, g);
         const int code = type_code(x.scalar_type());
         const size_t nbytes = g_operators.linear_bytes(rows, K, N, code, 1);
         const at::Tensor ws = scratch(nbytes, x);
@@ -258,7 +278,7 @@ struct LinearAct : public torch::autograd::Function<LinearAct> {
                                              address(grads[2]), act ? address(grads[3]) : nullptr, code, rows, K, N, act, address(ws), nbytes,
                                              reinterpret_cast<void*>(ctx->saved_data["stream"].toInt())),
                  "linear backward");
-        return grads;
+        return once(grads, x, g);
     }
 };
 

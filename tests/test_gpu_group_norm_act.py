@@ -281,6 +281,18 @@ def test_refusals(host_side):
             bad()
 
 
+def test_not_twice(host_side):
+    """Gradients of gradients are refused, not taken for zero; asking for a graph alone changes no gradient."""
+    from box_convolution import group_norm_act
+    x, w = torch.randn(2, 8, 3, 3, device="cuda", requires_grad=True), torch.ones(8, device="cuda", requires_grad=True)
+    once = torch.autograd.grad(group_norm_act(x, 4, w, activation="silu").sum(), [x, w])
+    again = torch.autograd.grad(group_norm_act(x, 4, w, activation="silu").sum(), [x, w], create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(once, again))
+    for g in again:
+        with pytest.raises(RuntimeError, match="not twice"):
+            g.square().sum().backward()
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("size", [(2, 20, 4, (9, 10)), (2, 64, 2, (50, 60)), (2, 32, 8, (130, 131)), (1, 1031, 1, (3, 5))])
 def test_relu_backward_sees_the_forwards_sign(hip, size, dtype):

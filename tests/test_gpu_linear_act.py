@@ -271,6 +271,19 @@ def test_refusals(host_side):
             bad()
 
 
+def test_not_twice(host_side):
+    """Gradients of gradients are refused, not taken for zero; asking for a graph alone changes no gradient."""
+    from box_convolution import linear_act
+    x, w = torch.randn(5, 8, device="cuda"), torch.randn(6, 8, device="cuda", requires_grad=True)
+    r = torch.randn(5, 6, device="cuda", requires_grad=True)
+    once = torch.autograd.grad(linear_act(x, w, residual=r, activation="silu").sum(), [w, r])
+    again = torch.autograd.grad(linear_act(x, w, residual=r, activation="silu").sum(), [w, r], create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(once, again))
+    for g in again:
+        with pytest.raises(RuntimeError, match="not twice"):
+            g.square().sum().backward()
+
+
 @pytest.mark.parametrize("K,N", [(64, 64), (33, 64)])
 def test_more_than_2_31_elements(hip, K, N):
     """Rows whose elements lie beyond 2^31 of each tensor, through few channels (whole chunks, and any alignment): the first and
