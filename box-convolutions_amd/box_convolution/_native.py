@@ -792,7 +792,7 @@ def linear_backward(input, weight, kept, activation, grad_output, needs):
 KERNEL_NAMES = ("band_colsum", "band_prefix", "band_scan", "forward_rows", "forward_quads", "forward_narrow", "forward_narrow_unaligned",
                 "grad_output_stream", "grad_input_cols", "grad_input_taps", "param_grad_finalize", "fill_zero", "fill_marker", "clip",
                 "forward_gather", "grad_input_gather", "grad_params_gather", "int_row_prefix",
-                "int_col_prefix", "norm_statistics", "norm_join", "norm_apply", "norm_small", "norm_any", "norm_sums",
+                "int_col_prefix", "norm_statistics", "norm_join", "norm_apply", "norm_small", "norm_any_statistics", "norm_any_apply", "norm_sums",
                 "norm_join_sums", "norm_grad", "norm_small_grad", "norm_parameter", "norm_any_sums", "norm_any_grad", "linear", "linear_few_rows",
                 "linear_dx", "linear_dweight", "linear_narrow_grad", "linear_slope", "join_parts", "join_bias")
 

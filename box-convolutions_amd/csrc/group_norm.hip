@@ -793,8 +793,26 @@ __global__ void __launch_bounds__(256) norm_parameter_kernel(NormBackwardArgs<T>
     if (c < channels) parameter_sums(a, totals, batch, channels, c);
 }
 
-// ---- numbers of channels that no workgroup's lanes can repeat over (odd and above 1024) --------------------
-// One workgroup per (batch item, group), element by element.
+// ---- numbers of channels that no workgroup's lanes can repeat over (odd and above 1024), items of a few elements --------------
+// A workgroup takes a chunk of whole pixels of one (batch item, group), element by element. Bound by the index arithmetic and the
+// loads of two or four bytes: @ANY@
+struct AnyChunk { int64_t base; int g; unsigned elements; };     // of the group: its first element, and how many there are
+__device__ __forceinline__ AnyChunk any_chunk(int64_t pixels, int channels, int groups, int per_group, int64_t chunk_pixels, int chunks) {
+    const unsigned chunk = blockIdx.x % static_cast<unsigned>(chunks), pair = blockIdx.x / static_cast<unsigned>(chunks);
+    const int64_t b = pair / static_cast<unsigned>(groups), first = chunk * chunk_pixels;
+    const int g = static_cast<int>(pair % static_cast<unsigned>(groups));
+    return {(b * pixels + first) * channels + static_cast<int64_t>(g) * per_group, g, static_cast<unsigned>(min(chunk_pixels, pixels - first)) * per_group};
+}
+// f(place in memory, channel) of this thread's elements of the chunk
+template <class F>
+__device__ __forceinline__ void any_elements(const AnyChunk& c, int channels, int per_group, F f) {
+    const unsigned width = static_cast<unsigned>(per_group);
+    for (unsigned i = threadIdx.x; i < c.elements; i += 256) {
+        const unsigned pixel = i / width, channel = i - pixel * width;
+        f(c.base + static_cast<int64_t>(pixel) * channels + channel, static_cast<int>(c.g * width + channel));
+    }
+}
+
 __device__ __forceinline__ float workgroup_sum(float v, float* lds) {
     v = sum_over(v, 64);
     __syncthreads();
@@ -805,32 +823,35 @@ __device__ __forceinline__ float workgroup_sum(float v, float* lds) {
     return v;
 }
 
+template <class T>
+__global__ void __launch_bounds__(256)
+norm_any_statistics_kernel(const T* __restrict__ x, float2* __restrict__ partial, int64_t pixels, int channels, int groups, int per_group,
+                           int64_t chunk_pixels, int chunks) {
+    __shared__ float lds[4];
+    const AnyChunk chunk = any_chunk(pixels, channels, groups, per_group, chunk_pixels, chunks);
+    float s = 0.0f;
+    any_elements(chunk, channels, per_group, [&](int64_t at, int) { s += static_cast<float>(x[at]); });
+    const float mu = workgroup_sum(s, lds) / static_cast<float>(chunk.elements);
+    s = 0.0f;
+    any_elements(chunk, channels, per_group, [&](int64_t at, int) {
+        const float d = static_cast<float>(x[at]) - mu;
+        s = fmaf(d, d, s);
+    });
+    s = workgroup_sum(s, lds);
+    if (threadIdx.x == 0) partial[blockIdx.x] = {mu, s};
+}
+
 template <class T, int ACT>
 __global__ void __launch_bounds__(256)
-norm_any_kernel(NormArgs<T> a, float* __restrict__ mean_out, float* __restrict__ rstd_out, int64_t pixels, int channels) {
-    __shared__ float lds[4];
-    const int64_t b = blockIdx.x / a.groups, n = pixels * a.per_group;
-    const int g = blockIdx.x % a.groups;
-    const int64_t base = b * pixels * channels + static_cast<int64_t>(g) * a.per_group;
-    float s = 0.0f;
-    for (int64_t i = threadIdx.x; i < n; i += 256) s += static_cast<float>(a.x[base + i / a.per_group * channels + i % a.per_group]);
-    const float mu = workgroup_sum(s, lds) / static_cast<float>(n);
-    s = 0.0f;
-    for (int64_t i = threadIdx.x; i < n; i += 256) {
-        const float d = static_cast<float>(a.x[base + i / a.per_group * channels + i % a.per_group]) - mu;
-        s = fmaf(d, d, s);
-    }
-    const float rs = inverse_deviation(workgroup_sum(s, lds) / static_cast<float>(n), a.eps);
-    if (threadIdx.x == 0 && mean_out != nullptr) {
-        mean_out[blockIdx.x] = mu;
-        rstd_out[blockIdx.x] = rs;
-    }
-    for (int64_t i = threadIdx.x; i < n; i += 256) {
-        const int64_t at = base + i / a.per_group * channels + i % a.per_group;
-        const int c = g * a.per_group + static_cast<int>(i % a.per_group);
+norm_any_apply_kernel(NormArgs<T> a, const float* __restrict__ mean, const float* __restrict__ rstd, int64_t pixels, int channels, int64_t chunk_pixels,
+                      int chunks) {
+    const AnyChunk chunk = any_chunk(pixels, channels, a.groups, a.per_group, chunk_pixels, chunks);
+    const unsigned pair = blockIdx.x / static_cast<unsigned>(chunks);
+    const float mu = mean[pair], rs = rstd[pair];
+    any_elements(chunk, channels, a.per_group, [&](int64_t at, int c) {
         const float w = a.weight ? load_param<T>(a.weight, a.float_params, c) : 1.0f, shift = a.bias ? load_param<T>(a.bias, a.float_params, c) : 0.0f;
         a.y[at] = static_cast<T>(activate<ACT>(form(static_cast<float>(a.x[at]), mu, rs, w, shift, a.residual ? static_cast<float>(a.residual[at]) : 0.0f).z));
-    }
+    });
 }
 
 struct AnyElement { float u, w, dz; };
@@ -865,27 +886,24 @@ norm_any_sums_kernel(NormBackwardArgs<T> a, float2* __restrict__ totals, int64_t
 
 template <class T, int ACT>
 __global__ void __launch_bounds__(256)
-norm_any_grad_kernel(NormBackwardArgs<T> a, const float2* __restrict__ totals, int64_t pixels, int channels, float inv_m) {
+norm_any_grad_kernel(NormBackwardArgs<T> a, const float2* __restrict__ totals, int64_t pixels, int channels, int64_t chunk_pixels, int chunks, float inv_m) {
     __shared__ float lds[4];
-    const int64_t b = blockIdx.x / a.groups, n = pixels * a.per_group;
-    const int g = blockIdx.x % a.groups;
+    const AnyChunk chunk = any_chunk(pixels, channels, a.groups, a.per_group, chunk_pixels, chunks);
+    const unsigned pair = blockIdx.x / static_cast<unsigned>(chunks);
+    const float2* of_group = totals + static_cast<int64_t>(pair) * a.per_group;             // (batch item by batch item, group by group)
     float s1 = 0.0f, s2 = 0.0f;
     for (int i = threadIdx.x; i < a.per_group; i += 256) {
-        const int c = g * a.per_group + i;
-        const float w = a.weight ? load_param<T>(a.weight, a.float_params, c) : 1.0f;
-        const float2 v = totals[b * channels + c];
-        s1 = fmaf(w, v.x, s1);
-        s2 = fmaf(w, v.y, s2);
+        const float w = a.weight ? load_param<T>(a.weight, a.float_params, chunk.g * a.per_group + i) : 1.0f;
+        s1 = fmaf(w, of_group[i].x, s1);
+        s2 = fmaf(w, of_group[i].y, s2);
     }
     s1 = workgroup_sum(s1, lds) * inv_m;
     s2 = workgroup_sum(s2, lds) * inv_m;
-    const float mu = a.mean[blockIdx.x], rs = a.rstd[blockIdx.x];
-    for (int64_t i = threadIdx.x; i < n; i += 256) {
-        const int c = g * a.per_group + static_cast<int>(i % a.per_group);
-        const int64_t at = (b * pixels + i / a.per_group) * channels + c;
+    const float mu = a.mean[pair], rs = a.rstd[pair];
+    any_elements(chunk, channels, a.per_group, [&](int64_t at, int c) {
         const AnyElement e = any_element<T, ACT>(a, at, c, mu, rs);
         a.dx[at] = static_cast<T>(rs * (fmaf(e.w, e.dz, -s1) - e.u * s2));
-    }
+    });
 }
 
 // ---- plans -------------------------------------------------------------------------------------------------
@@ -916,7 +934,10 @@ NormPlan plan_norm(int64_t batch, int64_t pixels, int channels, int groups, int 
     L.phase = channels / gcd(channels, V);
     p.slabs = 1;
     if (L.phase > 1024 || L.total < V) {
-        p.any = true;
+        p.any = true;                                      // chunks of whole pixels of a group, chunk_steps of them
+        const int64_t want = std::min<int64_t>(kMostChunks, std::max<int64_t>(1, 2048 / std::max<int64_t>(1, batch * groups)));
+        p.chunk_steps = std::max<int64_t>((pixels + want - 1) / want, (2047 + per_group) / per_group);
+        p.chunks = static_cast<int>((pixels + p.chunk_steps - 1) / p.chunk_steps);
         return p;
     }
     // one launch where a workgroup of at most 1024 lanes can hold an item, or whole groups of it that are at least 64 bytes
@@ -996,12 +1017,6 @@ hipError_t forward(const NormCall& n, void* workspace, hipStream_t stream) {
     a.eps = n.eps;
     const NormPlan p = plan_norm(n.batch, n.pixels, n.channels, n.groups, V, kMostVectors);
     const Lanes L = p.L;
-    if (p.any)
-        return with_activation(n.activation, [&](auto act) {
-            BOXCONV_LAUNCH("norm_any", (norm_any_kernel<T, decltype(act)::value>), dim3(static_cast<unsigned>(n.batch * n.groups)), dim3(256), 0, stream, a,
-                           n.mean, n.rstd, n.pixels, n.channels);
-            return hipGetLastError();
-        });
     if (p.small)
         return with_activation(n.activation, [&](auto act) {
             const size_t lds = static_cast<size_t>(L.active) * V * 4 + static_cast<size_t>(L.slab / a.per_group) * 8;
@@ -1025,15 +1040,24 @@ hipError_t forward(const NormCall& n, void* workspace, hipStream_t stream) {
         mean = reinterpret_cast<float*>(partial + n.batch * p.chunks * n.groups);
         rstd = mean + pairs;
     }
-    const int64_t chunk_pixels = p.chunk_steps * L.stride / L.channels, last_pixels = n.pixels - (p.chunks - 1) * chunk_pixels;
+    const int64_t chunk_pixels = p.any ? p.chunk_steps : p.chunk_steps * L.stride / L.channels, last_pixels = n.pixels - (p.chunks - 1) * chunk_pixels;
+    const dim3 any_grid(static_cast<unsigned>(pairs * p.chunks));
     const int workgroups = static_cast<int>(n.batch * p.pieces);
-    BOXCONV_LAUNCH("norm_statistics", (norm_statistics_kernel<T>), dim3(static_cast<unsigned>(n.batch * p.chunks)), dim3(p.threads), static_cast<size_t>(3) * L.active * V * 4, stream, a.x,
-                   partial, L, p.chunk_steps, p.chunks, a.groups, a.per_group);
+    if (p.any)
+        BOXCONV_LAUNCH("norm_any_statistics", (norm_any_statistics_kernel<T>), any_grid, dim3(256), 0, stream, a.x, partial, n.pixels, n.channels, a.groups,
+                       a.per_group, chunk_pixels, p.chunks);
+    else
+        BOXCONV_LAUNCH("norm_statistics", (norm_statistics_kernel<T>), dim3(static_cast<unsigned>(n.batch * p.chunks)), dim3(p.threads),
+                       static_cast<size_t>(3) * L.active * V * 4, stream, a.x, partial, L, p.chunk_steps, p.chunks, a.groups, a.per_group);
     BOXCONV_LAUNCH("norm_join", norm_join_kernel, dim3(static_cast<unsigned>(pairs)), dim3(256), 0, stream, partial, mean, rstd, p.chunks,
                    static_cast<float>(chunk_pixels * a.per_group), static_cast<float>(last_pixels * a.per_group), a.eps);
     return with_activation(n.activation, [&](auto act) {
-        BOXCONV_LAUNCH("norm_apply", (norm_apply_kernel<T, decltype(act)::value>), dim3(workgroups), dim3(p.threads), 0, stream, a, mean, rstd, L,
-                       p.piece_steps, p.pieces, workgroups);
+        if (p.any)
+            BOXCONV_LAUNCH("norm_any_apply", (norm_any_apply_kernel<T, decltype(act)::value>), any_grid, dim3(256), 0, stream, a, mean, rstd, n.pixels,
+                           n.channels, chunk_pixels, p.chunks);
+        else
+            BOXCONV_LAUNCH("norm_apply", (norm_apply_kernel<T, decltype(act)::value>), dim3(workgroups), dim3(p.threads), 0, stream, a, mean, rstd, L,
+                           p.piece_steps, p.pieces, workgroups);
         return hipGetLastError();
     });
 }
@@ -1069,8 +1093,8 @@ hipError_t backward(const NormGradCall& n, void* workspace, hipStream_t stream) 
                            stream, a, totals, n.pixels, n.channels);
             if (params) BOXCONV_LAUNCH("norm_parameter", (norm_parameter_kernel<T>), param_grid, dim3(256), 0, stream, a, totals, n.batch, n.channels);
             if (a.dx != nullptr)
-                BOXCONV_LAUNCH("norm_any_grad", (norm_any_grad_kernel<T, decltype(act)::value>), dim3(static_cast<unsigned>(n.batch * n.groups)), dim3(256), 0,
-                               stream, a, totals, n.pixels, n.channels, inv_m);
+                BOXCONV_LAUNCH("norm_any_grad", (norm_any_grad_kernel<T, decltype(act)::value>), dim3(static_cast<unsigned>(n.batch * n.groups * p.chunks)),
+                               dim3(256), 0, stream, a, totals, n.pixels, n.channels, p.chunk_steps, p.chunks, inv_m);
             return hipGetLastError();
         });
     if (p.small)
@@ -1097,7 +1121,7 @@ hipError_t backward(const NormGradCall& n, void* workspace, hipStream_t stream) 
 
 size_t norm_workspace_bytes(int64_t batch, int64_t pixels, int channels, int groups, int dtype, bool backward_pass) {
     const NormPlan p = plan_norm(batch, pixels, channels, groups, dtype == kF32 ? 4 : 8, backward_pass ? 1 : kMostVectors);
-    const int64_t chunks = p.any || p.small ? 0 : batch * p.chunks;
+    const int64_t chunks = p.small || (p.any && backward_pass) ? 0 : batch * p.chunks;
     if (backward_pass) return static_cast<size_t>(batch * channels + chunks * channels) * 8;
     return chunks ? static_cast<size_t>(chunks * groups * 2 + batch * groups * 2) * 4 : 0;
 }

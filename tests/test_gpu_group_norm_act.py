@@ -281,6 +281,15 @@ def test_refusals(host_side):
             bad()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("size", [(2, 1031, 1, (41, 67)), (1, 2053, 2053, (7, 50)), (3, 3077, 17, (10, 11)), (1, 1, 1, (1, 1)), (2, 3, 1, (1, 2))])
+def test_channels_that_no_lanes_repeat_over(hip, size, dtype):
+    """Element by element, the pixels cut into chunks: one group, a group per channel, a last chunk that is shorter."""
+    for name, residual, params in (("silu", True, "float"), (None, False, "none")):
+        c = case(*size, dtype, name, residual, params)
+        ref.check(run(c), expected(c))
+
+
 def test_not_twice(host_side):
     """Gradients of gradients are refused, not taken for zero; asking for a graph alone changes no gradient."""
     from box_convolution import group_norm_act
