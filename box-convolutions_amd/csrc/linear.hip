@@ -67,7 +67,9 @@ product_kernel(Operand<T> a, Operand<T> b, Tail<T> tail, int64_t k_part, int64_t
             if (k0 + SA::KT < k_end) turn(k0 + SA::KT, sa[AHEAD - 1], sb[AHEAD - 1]);
         }
     }
-    store_blocks<T, F, F>(tail, acc, m0 + wm, n0 + wn, blockIdx.y);
+    __syncthreads();
+    static_assert(4 * 256 * F <= SA::kChunks + SB::kChunks, "each wave turns its sums in a part of the tiles");
+    store_blocks<T, F, F>(tail, acc, m0 + wm, n0 + wn, blockIdx.y, lds + wave * 256 * F);
 }
 
 // ---- few rows ----------------------------------------------------------------------------------------------------

@@ -153,8 +153,9 @@ product_wide_kernel(Operand<T> a, Operand<T> b, Tail<T> tail, int64_t k_part, un
         settle<0>();                                           // stage s + 1 has landed, and the rest of this one is in registers
         step(3, s + 1, s + 2, 0, kHalf);
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");           // nothing may still be on its way into this workgroup's LDS when it ends
-    store_blocks<T, FN, FM>(tail, acc, m0 + wm, n0 + wn, blockIdx.y);
+    settle<0>();                                               // every wave's loads have landed and its fragments are read: the LDS is free
+    static_assert(WM * WN * 256 * FN <= kRing * kStage, "each wave turns its sums in a part of the stages");
+    store_blocks<T, FN, FM>(tail, acc, m0 + wm, n0 + wn, blockIdx.y, stages + wave * 256 * FN);
 }
 
 }  // namespace
