@@ -161,11 +161,12 @@ __device__ __forceinline__ Chunk fragment(const Chunk* tile, int i, int ks) {
         // lane s of a group of 16 fetches columns 4 (s%4) .. +3 (in the order of the fragment's rows) of k row s/4
         const int s = l % 16, q = l / 16, four = 4 * (q & 1) + s % 4;
         const int col = i + (PERM ? 16 * (four & 1) + 4 * (four >> 1) : 4 * four);
-        const int k = 16 * ks + 8 * (q >> 1) + s / 4;
-        const char* base = reinterpret_cast<const char*>(tile);
+        // (`place` looks at two bits of the row: the rows of a later k step and of the second half are as far on for every lane)
+        const char* base = reinterpret_cast<const char*>(tile) + (Shape::template place<PERM>(8 * (q >> 1) + s / 4, col / 8) * 16 + col % 8 * 2);
+        constexpr int kRow = Shape::kRowChunks * 16;
         Four lo, hi;
-        lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(base + Shape::template place<PERM>(k, col / 8) * 16 + col % 8 * 2));
-        hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(base + Shape::template place<PERM>(k + 4, col / 8) * 16 + col % 8 * 2));
+        lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(base + 16 * ks * kRow));
+        hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(base + (16 * ks + 4) * kRow));
         typedef short Eight __attribute__((ext_vector_type(8)));
         return __builtin_bit_cast(Chunk, Eight(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7)));
     } else {
