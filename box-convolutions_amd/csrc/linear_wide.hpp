@@ -63,11 +63,15 @@ struct Feed {
     }
 };
 
-// Tile m0, n0 of workgroup `id`: neighbours in id share an XCD's L2 (the hardware deals workgroups to the eight XCDs in
-// turn) and walk down 8 tiles of m before the next n.
-__device__ __forceinline__ void tile_of(unsigned id, unsigned tiles_m, unsigned tiles_n, unsigned& tm, unsigned& tn) {
-    const unsigned total = tiles_m * tiles_n, whole = total / 8 * 8;
+// Tile and part of k of this workgroup: neighbours share an XCD's L2 (the hardware deals workgroups to the eight XCDs in turn), the
+// tiles of one part among them, which read the same rows (200000 rows, 256 x 256 weight gradient in parts of four tiles: 66 us with the tiles on four XCDs, 53 on one), and
+// walk down 8 tiles of m before the next n.
+__device__ __forceinline__ void tile_of(unsigned tiles_m, unsigned tiles_n, unsigned& tm, unsigned& tn, unsigned& part) {
+    const unsigned tiles = tiles_m * tiles_n, total = tiles * gridDim.y, whole = total / 8 * 8;
+    unsigned id = blockIdx.y * tiles + blockIdx.x;
     if (id < whole) id = id % 8 * (whole / 8) + id / 8;
+    part = id / tiles;
+    id -= part * tiles;
     const unsigned group = id / (8 * tiles_n), first = group * 8, high = min(8u, tiles_m - first), rest = id - group * 8 * tiles_n;
     tm = first + rest % high;
     tn = rest / high;
@@ -91,10 +95,10 @@ product_wide_kernel(Operand<T> a, Operand<T> b, Tail<T> tail, int64_t k_part, un
     constexpr int THREADS = WM * WN * 64, FM = TM / WM / 32, FN = TN / WN / 32;
     constexpr int kStage = SA::kChunks + SB::kChunks;
     extern __shared__ Chunk stages[];
-    unsigned tm, tn;
-    tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn);
+    unsigned tm, tn, part;
+    tile_of(tiles_m, tiles_n, tm, tn, part);
     const int64_t m0 = static_cast<int64_t>(tm) * TM, n0 = static_cast<int64_t>(tn) * TN;
-    const int64_t k_begin = blockIdx.y * k_part, k_end = min(a.depth, k_begin + k_part);
+    const int64_t k_begin = part * k_part, k_end = min(a.depth, k_begin + k_part);
     const int wave = threadIdx.x / 64, wm = wave / WN * (TM / WM), wn = wave % WN * (TN / WN);
     Acc16 acc[FN][FM] = {};
     typedef Feed<T, A_K, TM, THREADS, false> FeedA;
@@ -155,7 +159,7 @@ product_wide_kernel(Operand<T> a, Operand<T> b, Tail<T> tail, int64_t k_part, un
     }
     settle<0>();                                               // every wave's loads have landed and its fragments are read: the LDS is free
     static_assert(WM * WN * 256 * FN <= kRing * kStage, "each wave turns its sums in a part of the stages");
-    store_blocks<T, FN, FM>(tail, acc, m0 + wm, n0 + wn, blockIdx.y, stages + wave * 256 * FN);
+    store_blocks<T, FN, FM>(tail, acc, m0 + wm, n0 + wn, part, stages + wave * 256 * FN);
 }
 
 }  // namespace
