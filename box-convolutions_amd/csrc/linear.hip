@@ -331,18 +331,20 @@ struct ProductPlan {
     size_t partial_bytes;
 };
 
-// The kernels' tiles, and what a step of 128 bytes of k takes a compute unit that holds `w` of their workgroups, in us: fixed + each * w.
+// The kernels' tiles, and what they take a compute unit that holds `w` of their workgroups, in us: a step of 128 bytes of k fixed + each * w
+// (float: each_float), a workgroup's start and epilogue as long as `ends` steps, and `slope` for an epilogue that keeps act' on a full unit.
 // Measured on bfloat16 products, M x N x K: 8192 x 4096 x 2048 takes 107 us with 256 x 256 tiles, 137 with 128 x 128; 2048 x 2048 x
-// 4096 takes 78, 48 and, with 64 x 64, 52; 512 x 512 x 4096 33 with 128 x 128, 36 with 64 x 64 (none of them split). Tiles of
-// 256 x 128 were no better than 128 x 128 anywhere: their waves read as much from LDS per product.
-struct ProductShape { int tm, tn, resident; double fixed, each; };
-constexpr ProductShape kWide[] = {{256, 256, 1, 0.0, 1.38}, {128, 128, 2, 0.46, 0.21}, {64, 64, 4, 0.44, 0.075}};
-constexpr ProductShape kAny[] = {{128, 128, 2, 0.8, 0.4}, {64, 64, 4, 0.5, 0.15}};
+// 4096 takes 78, 48 and, with 64 x 64, 52; 512 x 512 x 4096 33 with 128 x 128, 36 with 64 x 64 (none of them split). Short k, the same
+// three: 300000 x 256 x 64 68, 76 and 86 us; 380192 x 160 x 32 with a kept slope 137, 149 and 109; float, 48552 x 456 x 208 with one 185, 158
+// and 145. Tiles of 256 x 128 were no better than 128 x 128 anywhere: their waves read as much from LDS per product.
+struct ProductShape { int tm, tn, resident; double fixed, each, each_float, ends, slope; };
+constexpr ProductShape kWide[] = {{256, 256, 1, 0.0, 1.38, 7.2, 8.7, 10.0}, {128, 128, 2, 0.46, 0.21, 1.8, 7.6, 5.0}, {64, 64, 4, 0.44, 0.075, 0.44, 5.0, 1.6}};
+constexpr ProductShape kAny[] = {{128, 128, 2, 0.8, 0.4, 2.0, 7.0, 5.0}, {64, 64, 4, 0.5, 0.15, 0.5, 7.0, 1.6}};
 
-// The tile and the number of parts of k that promise the shortest time: rounds of workgroups, each as long as its steps and
-// about seven more for its start and its epilogue, and the parts' way through memory at 4 TB/s with one more launch.
+// The tile and the number of parts of k that promise the shortest time: rounds of workgroups, and the parts' way through memory at 4 TB/s
+// with one more launch.
 template <class T, int N>
-ProductPlan plan_product(const ProductShape (&shapes)[N], int64_t m, int64_t n, int64_t k) {
+ProductPlan plan_product(const ProductShape (&shapes)[N], int64_t m, int64_t n, int64_t k, bool keeps_slope) {
     constexpr int KT = 8 * Vec<T>::kLen;
     ProductPlan best = {};
     double least = 0.0;
@@ -354,7 +356,9 @@ ProductPlan plan_product(const ProductShape (&shapes)[N], int64_t m, int64_t n, 
             const int64_t part = (steps + splits - 1) / splits, parts = (steps + part - 1) / part, groups = tiles * parts;
             const int64_t slots = 256 * s.resident, rounds = (groups + slots - 1) / slots;
             const double w = groups >= slots ? s.resident : static_cast<double>((groups + 255) / 256);
-            double t = static_cast<double>(rounds) * static_cast<double>(part + 7) * (s.fixed + s.each * w);
+            double t = static_cast<double>(part) * (s.fixed + (sizeof(T) == 4 ? s.each_float : s.each) * w) + s.ends * (s.fixed + s.each * w);
+            if (keeps_slope && parts == 1) t += s.slope * w / s.resident;
+            t *= static_cast<double>(rounds);
             if (parts > 1) t += 4.0 + static_cast<double>(parts) * static_cast<double>(m) * static_cast<double>(n) * 8.0 / 4e6;
             if (best.splits == 0 || t < least) {
                 least = t;
@@ -411,7 +415,8 @@ hipError_t few_rows(const Operand<T>& a, const Operand<T>& b, const Tail<T>& tai
 template <class T, bool A_K, bool B_K>
 hipError_t product(const char* name, Operand<T> a, Operand<T> b, Tail<T> tail, float* workspace, hipStream_t stream) {
     const bool wide = whole_chunks<T, A_K>(a) && whole_chunks<T, B_K>(b);
-    const ProductPlan p = wide ? plan_product<T>(kWide, tail.rows, tail.cols, a.depth) : plan_product<T>(kAny, tail.rows, tail.cols, a.depth);
+    const bool keeps = tail.slope != nullptr;
+    const ProductPlan p = wide ? plan_product<T>(kWide, tail.rows, tail.cols, a.depth, keeps) : plan_product<T>(kAny, tail.rows, tail.cols, a.depth, keeps);
     tail.partial = p.splits > 1 ? workspace : nullptr;
     if (wide) {
         switch (p.shape) {
@@ -430,7 +435,10 @@ hipError_t product(const char* name, Operand<T> a, Operand<T> b, Tail<T> tail, f
 
 template <class T>
 size_t product_workspace(int64_t m, int64_t n, int64_t k) {
-    return std::max(plan_product<T>(kWide, m, n, k).partial_bytes, plan_product<T>(kAny, m, n, k).partial_bytes);
+    size_t most = 0;
+    for (const bool keeps : {false, true})
+        most = std::max({most, plan_product<T>(kWide, m, n, k, keeps).partial_bytes, plan_product<T>(kAny, m, n, k, keeps).partial_bytes});
+    return most;
 }
 
 
