@@ -78,6 +78,10 @@ __device__ __forceinline__ Chunk transposed(const char* tile, int pitch, int i, 
 }
 
 // BLOCKS: 32 x 32 blocks of dW that a wave sums.
+// 131072 rows, 128 -> 32 bfloat16 21 us (84 MB, 3.9 TB/s), 64 -> 64 float16 20 us; 65536 rows, 256 -> 64 float 71 us, of which the matrix
+// instructions take 33: one workgroup of 512 threads fills a compute unit, and its phases (loads, dz to LDS, products, stores) follow each
+// other. Without dx it takes 42 us, without dW 56, without either 24. Fragments of the weight held in registers, or of x used twice, gained
+// nothing in float and cost 7 us in bfloat16.
 template <class T, int TM, int BLOCKS>
 __global__ void __launch_bounds__(512)
 narrow_grad_kernel(NarrowArgs<T> a) {
