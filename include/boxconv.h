@@ -57,7 +57,11 @@ void boxconv_reload_env(void);
  * "band_scan", "forward_rows", "forward_quads", "grad_output_stream", "grad_input_cols",
  * "grad_input_taps", "param_grad_finalize", "fill_zero", "fill_marker", "clip", "forward_gather", "grad_input_gather",
  * "int_row_prefix", "int_col_prefix", "probe_copy_bands", "probe_grad_input_pattern",
- * "grad_params_gather".
+ * "grad_params_gather"; of the operators around a box convolution "norm_statistics", "norm_join",
+ * "norm_apply", "norm_small", "norm_any_statistics", "norm_any_apply", "norm_sums", "norm_join_sums",
+ * "norm_grad", "norm_small_grad", "norm_any_sums", "norm_any_grad", "norm_parameter", "linear",
+ * "linear_few_rows", "linear_dx", "linear_dweight", "linear_narrow_grad", "linear_slope", "join_parts",
+ * "join_bias".
  * NULL or "" disarms. Arming discards earlier measurements.
  * boxconv_profile_arm_every(name, n): the same, but only every n-th launch of that kernel (the
  * first, the (n+1)-th, ...) is bracketed; an event pair costs a few microseconds of GPU time, which
