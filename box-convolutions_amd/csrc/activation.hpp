@@ -20,13 +20,13 @@ __device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf
 // remains for z far below zero is a product and no difference: no cancellation there.
 struct Normal { float below, density; };
 __device__ __forceinline__ Normal normal(float z) {
-    const float e = __expf(-0.5f * z * z);
+    const float e = __builtin_amdgcn_exp2f(z * z * (-0.5f * 1.44269504089f));
     const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678118f, fabsf(z), 1.0f));
-    float q = fmaf(1.061405429f, t, -1.453152027f);
-    q = fmaf(q, t, 1.421413741f);
-    q = fmaf(q, t, -0.284496736f);
-    q = fmaf(q, t, 0.254829592f);
-    const float tail = 0.5f * q * t * e;
+    float q = fmaf(0.5f * 1.061405429f, t, 0.5f * -1.453152027f);
+    q = fmaf(q, t, 0.5f * 1.421413741f);
+    q = fmaf(q, t, 0.5f * -0.284496736f);
+    q = fmaf(q, t, 0.5f * 0.254829592f);
+    const float tail = q * t * e;
     return {z > 0.0f ? 1.0f - tail : tail, 0.39894228040f * e};
 }
 
@@ -45,7 +45,7 @@ __device__ __forceinline__ float slope(float z) {
     if constexpr (ACT == kActRelu) return z > 0.0f ? 1.0f : 0.0f;
     if constexpr (ACT == kActSilu) {
         const float s = sigmoid(z);
-        return s * fmaf(z, 1.0f - s, 1.0f);
+        return fmaf(z * s, 1.0f - s, s);
     }
     if constexpr (ACT == kActGelu) {
         const Normal n = normal(z);
