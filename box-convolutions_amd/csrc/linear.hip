@@ -11,8 +11,8 @@ namespace {
 // the next tile's loads (of tiles of 64: the next two tiles') in flight while this one is multiplied. blockIdx.y: the part of k
 // this workgroup sums. (Four groups of waves that take the tiles of k in turn, for products of few tiles, were no better: 1501 x 517
 // -> 333 float16 12.4 against 13.1 us, 517 x 1501 -> 333 17.5 against 14.1 with k split over workgroups.) Bound by issue: request, shift, mask
-// and store of every chunk, then the products. 1501 rows, 333 -> 517 float16 with gelu and a residual 12.6 us, dx 13.8, dW 9.8; 90022 rows,
-// 431 -> 149 bfloat16 71 us.
+// and store of every chunk, then the products. 1501 rows, 333 -> 517 float16 with gelu and a residual 13 us, dx 14, dW 10; 90022 rows, 431 ->
+// 149 bfloat16 63 us.
 template <class T, bool A_K, bool B_K, int TX>
 __global__ void __launch_bounds__(256)
 product_kernel(Operand<T> a, Operand<T> b, Tail<T> tail, int64_t k_part, int64_t tiles_m, int64_t tiles_n) {

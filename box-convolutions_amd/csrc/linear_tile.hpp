@@ -97,11 +97,15 @@ struct Stage {
     const T* at[N];            // the thread's chunks in the tile that was last asked for
     int room[N];               // elements of them inside the operand's extent, at most a vector
     const T* safe;             // null: the operand's rows are shorter than a vector, and there is no safe place to read one from
+    bool inner;                // no chunk ends inside the extent: with KT values of k left, all that is read is used as it lies in memory.
+                               // (Rows beyond the extent of a K-major operand hold anything then: sums that nobody stores. 90022 rows, 431 -> 149
+                               // bfloat16 68 us with every chunk masked, 63 so; 8000 rows, 1001 -> 999 47 and 43.)
     int64_t step;
 
     // The tile with rows from i0 and k from k0 on; `step`: k from one tile asked for to the next, in tiles.
     __device__ __forceinline__ void start(const Operand<T>& o, int64_t i0, int64_t k0, int tiles) {
         safe = (K_MAJOR ? o.depth : o.extent) >= Shape::V ? o.p : nullptr;
+        inner = safe != nullptr && (K_MAJOR || i0 + X <= o.extent);
         step = K_MAJOR ? static_cast<int64_t>(tiles) * Shape::KT : tiles * Shape::KT * o.ld;
 #pragma unroll
         for (int s = 0; s < N; ++s) {
@@ -119,6 +123,11 @@ struct Stage {
         else return r < k_left ? room[s] : 0;
     }
     __device__ __forceinline__ void request(int k_left) {
+        if (inner && k_left >= Shape::KT) {
+#pragma unroll
+            for (int s = 0; s < N; ++s) v[s] = __builtin_bit_cast(Chunk, *reinterpret_cast<const typename Vec<T>::Type*>(room[s] > 0 ? at[s] : safe));
+            return;
+        }
 #pragma unroll
         for (int s = 0; s < N; ++s) v[s] = Chunk{0, 0, 0, 0};
         if (safe != nullptr) {
@@ -127,6 +136,7 @@ struct Stage {
         }
     }
     __device__ __forceinline__ void settle(int k_left) {
+        if (inner && k_left >= Shape::KT) return;
 #pragma unroll
         for (int s = 0; s < N; ++s) settle_chunk<T>(v[s], valid(s, k_left));
         if (safe == nullptr) {
