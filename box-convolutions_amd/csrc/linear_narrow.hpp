@@ -31,12 +31,12 @@ struct NarrowArgs {
 struct NarrowLds {
     int px, pa, pb;              // rows of x and the weight; rows of dz for 16-byte reads; for transposed ones
     int x_bytes, a_bytes, b_bytes, w_bytes;
-    __host__ __device__ int total() const { return 2 * (x_bytes + a_bytes + b_bytes) + w_bytes + 128; }   // (a fragment may reach 96 bytes past the last row)
+    __host__ __device__ constexpr int total() const { return 2 * (x_bytes + a_bytes + b_bytes) + w_bytes + 128; }   // (a fragment may reach 96 bytes past the last row)
 };
 template <class T>
-__host__ __device__ inline NarrowLds narrow_lds(int N, int K, int TM) {
+__host__ __device__ constexpr NarrowLds narrow_lds(int N, int K, int TM) {
     constexpr int V = Vec<T>::kLen;
-    NarrowLds s;
+    NarrowLds s = {};
     const int cx = K / V, cn = (N / V + 1) / 2 * 2;                       // (whole k steps of n)
     if (sizeof(T) == 2) {
         s.px = cx + (12 - cx % 8) % 8;
@@ -52,6 +52,22 @@ __host__ __device__ inline NarrowLds narrow_lds(int N, int K, int TM) {
     s.w_bytes = (cn * V * s.px + 63) / 64 * 1024;
     return s;
 }
+// Rows of column sums that the workgroup's threads hold at the end, N floats each: those of one pass over a tile, as far as the tile reaches.
+template <class T>
+__host__ __device__ constexpr int narrow_sum_rows(int N, int TM) {
+    const int per_pass = 512 / (N / Vec<T>::kLen);
+    return per_pass < TM ? per_pass : TM;
+}
+// The column sums take the place of the tiles and have to fit there, for every K and N the kernel may be asked for.
+template <class T>
+constexpr bool sums_fit() {
+    for (int N = Vec<T>::kLen; N <= 128; N += Vec<T>::kLen)
+        for (int K = Vec<T>::kLen; K <= 1024; K += Vec<T>::kLen)
+            for (int TM = 32; TM <= 64; TM *= 2)
+                if (narrow_sum_rows<T>(N, TM) * N * 4 > narrow_lds<T>(N, K, TM).total()) return false;
+    return true;
+}
+static_assert(sums_fit<BOXCONV_INST_T>(), "column sums beyond the LDS of the tiles");
 
 // A transposed fragment (32 columns from `i` on, k step ks of the rows) of a tile of `pitch` chunks per row.
 template <class T, bool PERM>
@@ -228,13 +244,14 @@ narrow_grad_kernel(NarrowArgs<T> a) {
     if (a.dbias != nullptr) {
         __syncthreads();                                       // (the tiles are done with: their LDS takes the sums)
         float* part = reinterpret_cast<float*>(lds);
-        if (row < per_pass)
+        const int rows = narrow_sum_rows<T>(a.N, TM);          // (threads of the rows from there on hold zeros, and there is no room for them)
+        if (row < rows)
 #pragma unroll
             for (int j = 0; j < V; ++j) part[row * a.N + col + j] = sums[j];
         __syncthreads();
         for (int n = t; n < a.N; n += 512) {
             float f = 0.0f;
-            for (int r = 0; r < min(per_pass, TM); ++r) f += part[r * a.N + n];
+            for (int r = 0; r < rows; ++r) f += part[r * a.N + n];
             a.dbias[static_cast<int64_t>(blockIdx.x) * a.N + n] = f;
         }
     }

@@ -311,3 +311,12 @@ def test_more_than_2_31_elements(hip, K, N):
         xs, ws = x.detach()[part], w.detach().clone().requires_grad_(True)
         sums += torch.autograd.grad(linear_act(xs, ws, activation="relu"), ws, g[part])[0].double()
     assert (sums - dw.double()).abs().max() <= 3 * 2.0 ** -8 * dw.double().abs().max()      # three bfloat16 roundings
+
+
+@pytest.mark.parametrize("K", [4, 8, 12])
+@pytest.mark.parametrize("N", [4, 8, 12])
+def test_few_channels_on_both_sides(hip, K, N):
+    """float32 layers whose tiles take less LDS than the bias sums of all 512 threads would: only the rows of a tile are kept there."""
+    for M in (33, 70, 5000):
+        args = case(M, K, N, torch.float32, "relu", residual=K == N)
+        ref.check(run(*args), expected(*args, torch.float32))
