@@ -39,6 +39,11 @@ def _once(grads, x, grad_output):
     return tuple(g if g is None else _OnceFunction.apply(g, x, grad_output, needs_grad) for g in grads)
 
 
+def _contiguous(*tensors):
+    """What was saved, as the kernels take it: hooks on saved tensors may hand the values back in any memory order."""
+    return [None if t is None else t.contiguous() for t in tensors]
+
+
 class GroupNormActFunction(torch.autograd.Function):
     """``apply(input, weight, bias, residual, num_groups, activation, eps)``, tensors ``[B, ..., C]``, contiguous."""
 
@@ -52,7 +57,7 @@ class GroupNormActFunction(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad_output):
-        input, weight, bias, residual, mean, rstd = ctx.saved_tensors
+        input, weight, bias, residual, mean, rstd = _contiguous(*ctx.saved_tensors)
         grads = _native.group_norm_backward(
             input, ctx.num_groups, weight, bias, residual, ctx.activation, mean, rstd, grad_output.contiguous(),
             ctx.needs_input_grad[:4])
@@ -112,6 +117,7 @@ class LinearActFunction(torch.autograd.Function):
     @staticmethod
     def backward(ctx, grad_output):
         input, weight, kept = ctx.saved_tensors
+        input, (weight, kept) = _rows(input, *input.shape), _contiguous(weight, kept)
         grads = _native.linear_backward(input, weight, kept, ctx.activation, grad_output.contiguous(), ctx.needs_input_grad[:4])
         return (*_once(grads, input, grad_output), None)
 

@@ -84,7 +84,8 @@ torch::autograd::variable_list once(torch::autograd::variable_list grads, const 
     return grads;
 }
 
-Optional saved_or_none(const at::Tensor& t) { return t.defined() ? Optional(t) : std::nullopt; }
+// What was saved, as the kernels take it: hooks on saved tensors may hand the values back in any memory order.
+Optional saved_or_none(const at::Tensor& t) { return t.defined() ? Optional(t.contiguous()) : std::nullopt; }
 
 // ---- group norm ------------------------------------------------------------------------------------------
 // A new tensor of x's shape [B, C, ...] in channels-last memory.
@@ -148,7 +149,8 @@ struct GroupNormAct : public torch::autograd::Function<GroupNormAct> {
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grad_outputs) {
         const auto saved = ctx->get_saved_variables();
-        const at::Tensor &x = saved[0], &statistics = saved[4];
+        const at::Tensor x = channels_last(saved[0]), residual = saved[3].defined() ? channels_last(saved[3]) : at::Tensor();
+        const at::Tensor statistics = saved[4].contiguous();
         const Optional w = saved_or_none(saved[1]), b = saved_or_none(saved[2]);
         const int groups = static_cast<int>(ctx->saved_data["groups"].toInt()), act = static_cast<int>(ctx->saved_data["act"].toInt());
         const std::vector<bool> need = needed(ctx, ctx->saved_data["present"].toBoolList().vec());
@@ -165,7 +167,7 @@ struct GroupNormAct : public torch::autograd::Function<GroupNormAct> {
         const size_t nbytes = g_operators.norm_bytes(n.batch, n.pixels, n.channels, groups, code, 1);
         const at::Tensor ws = scratch(nbytes, x);
         const float* mean = statistics.data_ptr<float>();
-        check_rc(g_operators.norm_backward(x.data_ptr(), address(w), address(b), param_code(w, b), address(saved[3]), g.data_ptr(), mean,
+        check_rc(g_operators.norm_backward(x.data_ptr(), address(w), address(b), param_code(w, b), address(residual), g.data_ptr(), mean,
                                            mean + n.batch * groups, address(grads[0]), address(grads[1]), address(grads[2]), address(grads[3]), code,
                                            n.batch, n.pixels, n.channels, groups, act, address(ws), nbytes,
                                            reinterpret_cast<void*>(ctx->saved_data["stream"].toInt())),
@@ -258,11 +260,13 @@ struct LinearAct : public torch::autograd::Function<LinearAct> {
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grad_outputs) {
         const auto saved = ctx->get_saved_variables();
-        const at::Tensor &x = saved[0], &w = saved[1], &kept = saved[2];
+        const at::Tensor w = saved[1].contiguous(), kept = saved[2].defined() ? saved[2].contiguous() : at::Tensor();
         const int act = static_cast<int>(ctx->saved_data["act"].toInt());
         const std::vector<bool> need = needed(ctx, ctx->saved_data["present"].toBoolList().vec());
         const at::Tensor g = grad_outputs[0].contiguous();
-        const int64_t rows = x.size(0), N = w.size(0), K = w.size(1);
+        const int64_t rows = saved[0].size(0), N = w.size(0), K = w.size(1);
+        const Rows held(saved[0], rows, K);
+        const at::Tensor& x = held.hold;
         const bool none = rows == 0 || N == 0;
         const auto fresh = [&](at::IntArrayRef shape) { return none || K == 0 ? at::zeros(shape, x.options()) : at::empty(shape, x.options()); };
         torch::autograd::variable_list grads(6);               // one per argument of forward
@@ -274,7 +278,7 @@ struct LinearAct : public torch::autograd::Function<LinearAct> {
         const int code = type_code(x.scalar_type());
         const size_t nbytes = g_operators.linear_bytes(rows, K, N, code, 1);
         const at::Tensor ws = scratch(nbytes, x);
-        check_rc(g_operators.linear_backward(x.data_ptr(), x.stride(0), w.data_ptr(), g.data_ptr(), address(kept), address(grads[0]), address(grads[1]),
+        check_rc(g_operators.linear_backward(x.data_ptr(), held.ld, w.data_ptr(), g.data_ptr(), address(kept), address(grads[0]), address(grads[1]),
                                              address(grads[2]), act ? address(grads[3]) : nullptr, code, rows, K, N, act, address(ws), nbytes,
                                              reinterpret_cast<void*>(ctx->saved_data["stream"].toInt())),
                  "linear backward");

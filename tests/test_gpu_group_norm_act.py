@@ -336,3 +336,25 @@ def test_more_than_2_31_elements(hip):
     dx = torch.autograd.grad(y, x, g.repeat(repeats, 1)[None].movedim(-1, 1))[0]
     for k in (0, repeats - 1):
         assert (dx[:, :, k * small:(k + 1) * small].float() - dxs).abs().max() <= 2.0 ** -8 * dxs.abs().max()
+
+
+def _as_rows(t):
+    """What saving to the CPU and back makes of a tensor: the same values in torch's default memory order."""
+    return torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t)
+
+
+def _turned(t):
+    return t.transpose(0, -1).contiguous().transpose(0, -1) if t.dim() > 1 else torch.stack((t, t), 1)[:, 0]
+
+
+@pytest.mark.parametrize("unpack", [_as_rows, _turned])
+def test_saved_tensors_of_another_layout(host_side, unpack):
+    """Hooks on saved tensors may give the values back in any memory order."""
+    for size in ((2, 12, 3, (9, 7)), (1, 24, 4, (130, 140)), (3, 8, 4, ())):
+        for name in (None, "gelu"):
+            c = case(*size, torch.float32, name, True, "float")
+            plain = run(c)
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+                hooked = run(c)
+            for k in plain:
+                assert torch.equal(plain[k], hooked[k]), (k, size, name)

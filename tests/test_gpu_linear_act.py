@@ -320,3 +320,17 @@ def test_few_channels_on_both_sides(hip, K, N):
     for M in (33, 70, 5000):
         args = case(M, K, N, torch.float32, "relu", residual=K == N)
         ref.check(run(*args), expected(*args, torch.float32))
+
+
+@pytest.mark.parametrize("unpack", [lambda t: torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t),
+                                    lambda t: t.t().contiguous().t()])
+def test_saved_tensors_of_another_layout(host_side, unpack):
+    """Hooks on saved tensors may give the values back in any memory order."""
+    for M, K, N in ((70, 40, 24), (600, 264, 520)):
+        for name in ACTS:
+            args = case(M, K, N, torch.float16, name, residual=True)
+            plain = run(*args)
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+                hooked = run(*args)
+            for k in plain:
+                assert torch.equal(plain[k], hooked[k]), (k, name)
