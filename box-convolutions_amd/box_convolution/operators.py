@@ -39,6 +39,14 @@ def _once(grads, x, grad_output):
     return tuple(g if g is None else _OnceFunction.apply(g, x, grad_output, needs_grad) for g in grads)
 
 
+def _refuse_tangents(*tensors):
+    """Neither the kernels nor the autograd functions know forward-mode derivatives: a tangent is refused, since dropping
+    it would make it zero."""
+    for t in tensors:
+        if t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError("box_convolution: group_norm_act and linear_act have no forward-mode derivative")
+
+
 def _contiguous(*tensors):
     """What was saved, as the kernels take it: hooks on saved tensors may hand the values back in any memory order."""
     return [None if t is None else t.contiguous() for t in tensors]
@@ -57,6 +65,7 @@ class GroupNormActFunction(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad_output):
+        _refuse_tangents(grad_output)
         input, weight, bias, residual, mean, rstd = _contiguous(*ctx.saved_tensors)
         grads = _native.group_norm_backward(
             input, ctx.num_groups, weight, bias, residual, ctx.activation, mean, rstd, grad_output.contiguous(),
@@ -81,6 +90,7 @@ def group_norm_act(input, num_groups, weight=None, bias=None, residual=None, act
         with _native._on_device(input.device):
             return glue.group_norm_act(input, num_groups, weight, bias, residual, act, eps, _native._stream(input.device) or 0)
     _native._operator_dtype(input, "group norm input")
+    _refuse_tangents(input, weight, bias, residual)
     if input.dim() < 2:
         raise RuntimeError("box_convolution: group norm input must have >=2 dimensions")
     if num_groups < 1 or input.size(1) < 1 or input.size(1) % num_groups != 0:
@@ -116,6 +126,7 @@ class LinearActFunction(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad_output):
+        _refuse_tangents(grad_output)
         input, weight, kept = ctx.saved_tensors
         input, (weight, kept) = _rows(input, *input.shape), _contiguous(weight, kept)
         grads = _native.linear_backward(input, weight, kept, ctx.activation, grad_output.contiguous(), ctx.needs_input_grad[:4])
@@ -136,6 +147,7 @@ def linear_act(input, weight, bias=None, residual=None, activation=None):
         with _native._on_device(input.device):
             return glue.linear_act(input, weight, bias, residual, act, _native._stream(input.device) or 0)
     _native._operator_dtype(input, "linear input")
+    _refuse_tangents(input, weight, bias, residual)
     if input.dim() < 1 or weight.dim() != 2 or weight.size(1) != input.size(-1):
         raise RuntimeError("box_convolution: linear needs an input [..., K] and a weight [N, K], got %s and %s"
                            % (tuple(input.shape), tuple(weight.shape)))

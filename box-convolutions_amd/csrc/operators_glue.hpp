@@ -56,6 +56,16 @@ bool wants_grad(const at::Tensor& a, std::initializer_list<const Optional*> more
     return false;
 }
 
+// Neither the kernels nor the nodes know forward-mode derivatives: a tangent is refused, since dropping it would make it zero.
+void refuse_tangents(std::initializer_list<const at::Tensor*> tensors) {
+    for (const at::Tensor* t : tensors)
+        TORCH_CHECK(!t->defined() || !t->_fw_grad(/*level=*/0).defined(), "box_convolution: group_norm_act and linear_act have no forward-mode derivative");
+}
+const at::Tensor& or_undefined(const Optional& t) {
+    static const at::Tensor none;
+    return t ? *t : none;
+}
+
 // Which of the arguments of a node, in their order, have a gradient to form (absent ones have no edge).
 std::vector<bool> needed(torch::autograd::AutogradContext* ctx, const std::vector<bool>& present) {
     std::vector<bool> out;
@@ -148,6 +158,7 @@ struct GroupNormAct : public torch::autograd::Function<GroupNormAct> {
         return y;
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grad_outputs) {
+        refuse_tangents({&grad_outputs[0]});
         const auto saved = ctx->get_saved_variables();
         const at::Tensor x = channels_last(saved[0]), residual = saved[3].defined() ? channels_last(saved[3]) : at::Tensor();
         const at::Tensor statistics = saved[4].contiguous();
@@ -192,6 +203,7 @@ void check_same(const Optional& t, at::IntArrayRef shape, const at::Tensor& like
 at::Tensor group_norm_act(const at::Tensor& input, int64_t groups, const Optional& weight, const Optional& bias, const Optional& residual, int64_t act,
                           double eps, int64_t stream) {
     check_operator_input(input, "group norm input");
+    refuse_tangents({&input, &or_undefined(weight), &or_undefined(bias), &or_undefined(residual)});
     TORCH_CHECK(input.dim() >= 2, "box_convolution: group norm input must have >=2 dimensions");
     const int64_t channels = input.size(1);
     TORCH_CHECK(groups >= 1 && channels >= 1 && channels % groups == 0 && channels <= INT32_MAX, "box_convolution: ", channels,
@@ -259,6 +271,7 @@ struct LinearAct : public torch::autograd::Function<LinearAct> {
         return y;
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grad_outputs) {
+        refuse_tangents({&grad_outputs[0]});
         const auto saved = ctx->get_saved_variables();
         const at::Tensor w = saved[1].contiguous(), kept = saved[2].defined() ? saved[2].contiguous() : at::Tensor();
         const int act = static_cast<int>(ctx->saved_data["act"].toInt());
@@ -288,6 +301,7 @@ struct LinearAct : public torch::autograd::Function<LinearAct> {
 
 at::Tensor linear_act(const at::Tensor& input, const at::Tensor& weight, const Optional& bias, const Optional& residual, int64_t act, int64_t stream) {
     check_operator_input(input, "linear input");
+    refuse_tangents({&input, &weight, &or_undefined(bias), &or_undefined(residual)});
     TORCH_CHECK(input.dim() >= 1 && weight.dim() == 2 && weight.size(1) == input.size(-1),
                 "box_convolution: linear needs an input [..., K] and a weight [N, K], got ", input.sizes(), " and ", weight.sizes());
     std::vector<int64_t> shape(input.sizes().begin(), input.sizes().end());

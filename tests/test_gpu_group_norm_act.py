@@ -358,3 +358,22 @@ def test_saved_tensors_of_another_layout(host_side, unpack):
                 hooked = run(c)
             for k in plain:
                 assert torch.equal(plain[k], hooked[k]), (k, size, name)
+
+
+def test_forward_mode_is_refused(host_side):
+    """A tangent on any input, or on the gradient, is refused and not dropped, whether or not gradients are recorded."""
+    import torch.autograd.forward_ad as forward_ad
+    from box_convolution import group_norm_act
+    x, r = torch.randn(2, 8, 3, 3, device="cuda"), torch.randn(2, 8, 3, 3, device="cuda")
+    w, b = torch.randn(8, device="cuda"), torch.randn(8, device="cuda")
+    with forward_ad.dual_level():
+        for i in range(4):
+            args = [forward_ad.make_dual(t, torch.ones_like(t)) if i == k else t for k, t in enumerate((x, w, b, r))]
+            for recorded in (False, True):
+                with torch.set_grad_enabled(recorded), pytest.raises(RuntimeError, match="forward-mode"):
+                    group_norm_act(args[0], 4, *args[1:], activation="silu")
+        leaf = x.clone().requires_grad_(True)
+        y = group_norm_act(leaf, 4, w, b, r, "silu")
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.autograd.grad(y, leaf, forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y)))
+        assert torch.equal(group_norm_act(x, 4, w, b, r, "silu"), y)

@@ -334,3 +334,21 @@ def test_saved_tensors_of_another_layout(host_side, unpack):
                 hooked = run(*args)
             for k in plain:
                 assert torch.equal(plain[k], hooked[k]), (k, name)
+
+
+def test_forward_mode_is_refused(host_side):
+    """A tangent on any input, or on the gradient, is refused and not dropped, whether or not gradients are recorded."""
+    import torch.autograd.forward_ad as forward_ad
+    from box_convolution import linear_act
+    plain = [torch.randn(s, device="cuda") for s in ((5, 8), (6, 8), (6,), (5, 6))]
+    with forward_ad.dual_level():
+        for i in range(4):
+            args = [forward_ad.make_dual(t, torch.ones_like(t)) if i == k else t for k, t in enumerate(plain)]
+            for recorded in (False, True):
+                with torch.set_grad_enabled(recorded), pytest.raises(RuntimeError, match="forward-mode"):
+                    linear_act(*args, "silu")
+        leaf = plain[0].clone().requires_grad_(True)
+        y = linear_act(leaf, *plain[1:], "silu")
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.autograd.grad(y, leaf, forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y)))
+        assert torch.equal(linear_act(*plain, "silu"), y)
