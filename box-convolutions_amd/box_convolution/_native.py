@@ -665,6 +665,12 @@ def _operator_workspace_bytes(fn, *key):
     return n
 
 
+def _scratch(nbytes, device):
+    """Scratch of one call, back with the allocator when the call returns. Not the buffer that `_workspace` keeps for a stream:
+    these calls launch several kernels without the interpreter's lock, and two threads' launches on one stream may alternate."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
 def _norm_parameters(input, channels, weight, bias):
     """(weight, bias, their dtype code): contiguous vectors of `channels` values, both float32 or both
     of the input's type."""
@@ -704,7 +710,7 @@ def group_norm_forward(input, num_groups, weight, bias, residual, activation, ep
     with _on_device(input.device):
         nbytes = _operator_workspace_bytes("boxconv_group_norm_workspace_bytes", B, pixels, C, num_groups, dtype, 0)
         stream = _stream(input.device)
-        ws = _workspace(nbytes, input.device, stream)
+        ws = _scratch(nbytes, input.device)
         rc = load().boxconv_group_norm_forward(
             _ptr(input), _ptr(weight), _ptr(bias), param_dtype, _ptr(residual), _ptr(output), _ptr(mean), _ptr(rstd),
             dtype, B, pixels, C, num_groups, eps, act, _ptr(ws), nbytes, stream)
@@ -730,7 +736,7 @@ def group_norm_backward(input, num_groups, weight, bias, residual, activation, m
     with _on_device(input.device):
         nbytes = _operator_workspace_bytes("boxconv_group_norm_workspace_bytes", B, pixels, C, num_groups, dtype, 1)
         stream = _stream(input.device)
-        ws = _workspace(nbytes, input.device, stream)
+        ws = _scratch(nbytes, input.device)
         rc = load().boxconv_group_norm_backward(
             _ptr(input), _ptr(weight), _ptr(bias), param_dtype, _ptr(residual), _ptr(grad_output), _ptr(mean), _ptr(rstd),
             *[_ptr(g) for g in grads], dtype, B, pixels, C, num_groups, act, _ptr(ws), nbytes, stream)
@@ -753,7 +759,7 @@ def linear_forward(input, weight, bias, residual, activation, keep_slope):
         with _on_device(input.device):
             nbytes = _operator_workspace_bytes("boxconv_linear_workspace_bytes", rows, K, N, dtype, 0)
             stream = _stream(input.device)
-            ws = _workspace(nbytes, input.device, stream)
+            ws = _scratch(nbytes, input.device)
             rc = load().boxconv_linear_forward(
                 _ptr(input), input.stride(0), _ptr(weight), _ptr(bias), _ptr(residual),
                 0 if residual is None else residual.stride(0), _ptr(output), _ptr(slope), dtype, rows, K, N, act,
@@ -780,7 +786,7 @@ def linear_backward(input, weight, kept, activation, grad_output, needs):
         with _on_device(input.device):
             nbytes = _operator_workspace_bytes("boxconv_linear_workspace_bytes", rows, K, N, dtype, 1)
             stream = _stream(input.device)
-            ws = _workspace(nbytes, input.device, stream)
+            ws = _scratch(nbytes, input.device)
             rc = load().boxconv_linear_backward(
                 _ptr(input), input.stride(0), _ptr(weight), _ptr(grad_output), _ptr(kept),
                 *[_ptr(g) for g in grads[:3]], _ptr(grads[3]) if act else None, dtype, rows, K, N, act, _ptr(ws), nbytes,

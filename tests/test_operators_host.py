@@ -96,3 +96,43 @@ def test_reference_against_torch():
         e = dict(zip(("x", "weight", "bias", "residual"), torch.autograd.grad(y, leaves, g)), y=y)
         got = ref.group_norm(*[x.detach(), 3] + [t.detach() for t in leaves[1:]], name, 1e-5, g, torch.float32, torch.float32)
         assert all(torch.allclose(got[k][0], e[k]) for k in e) and set(got) == set(e)
+
+
+@pytest.mark.parametrize("call", ["norm", "norm_backward", "linear", "linear_backward"])
+def test_scratch_of_calls_that_overlap(monkeypatch, call):
+    """Two threads may launch on one stream in turn: while one call's kernels are being launched, another's must not get the same scratch
+    memory. (The native library is replaced by one that starts the other call from within the first.)"""
+    import contextlib
+    import threading
+    from box_convolution import _native
+    x, w, g = torch.zeros(6, 8), torch.zeros(8, 8), torch.zeros(6, 8)
+    stat = torch.zeros(6, 2)
+    calls = {"norm": lambda: _native.group_norm_forward(x, 2, None, None, None, None, 1e-5, False),
+             "norm_backward": lambda: _native.group_norm_backward(x, 2, None, None, None, None, stat, stat, g, (True, False, False, False)),
+             "linear": lambda: _native.linear_forward(x, w, None, None, None, False),
+             "linear_backward": lambda: _native.linear_backward(x, w, None, None, g, (True, True, False, False))}
+    seen = []
+
+    class Library:
+        def __getattr__(self, name):
+            return self.workspace_bytes if name.endswith("workspace_bytes") else self.entry
+
+        def workspace_bytes(self, *args):
+            return 256
+
+        def entry(self, *args):
+            seen.append(args[-3])
+            if len(seen) == 1:
+                other = threading.Thread(target=calls[call])
+                other.start()
+                other.join()
+            return 0
+    library = Library()
+    monkeypatch.setattr(_native, "load", lambda: library)
+    monkeypatch.setattr(_native, "_on_device", lambda device: contextlib.nullcontext())
+    monkeypatch.setattr(_native, "_stream", lambda device: 0)
+    monkeypatch.setattr(_native, "_workspace_bytes", {})
+    monkeypatch.setattr(_native, "_workspaces", {})
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    calls[call]()
+    assert len(seen) == 2 and None not in seen and seen[0] != seen[1]
