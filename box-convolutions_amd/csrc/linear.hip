@@ -375,12 +375,14 @@ ProductPlan plan_product(const ProductShape (&shapes)[N], int64_t m, int64_t n, 
     return best;
 }
 
-// Whether tiles of this operand can come straight into LDS: whole aligned chunks, offsets within a tile in 31 bits.
+// Whether tiles of this operand can come straight into LDS: whole aligned chunks, offsets within a tile in 31 bits. With k as the slow index
+// rows must not overlap either (an expanded input's lie on top of each other): rows beyond the last one are zeros only because they lie beyond the
+// operand's end, and others' values there would be multiplied by the other operand's zeros, which gives NaN where they are infinite.
 template <class T, bool K_MAJOR>
 bool whole_chunks(const Operand<T>& o) {
     constexpr int V = Vec<T>::kLen;
     return reinterpret_cast<uintptr_t>(o.p) % 16 == 0 && o.ld % V == 0 && (K_MAJOR ? o.depth : o.extent) % V == 0 && o.depth < (int64_t(1) << 30) &&
-           o.ld < (int64_t(1) << 31) / (256 * static_cast<int64_t>(sizeof(T)));
+           o.ld < (int64_t(1) << 31) / (256 * static_cast<int64_t>(sizeof(T))) && (K_MAJOR || o.ld >= o.extent);
 }
 
 template <class T, bool A_K, bool B_K, int TM, int TN, int WM, int WN>

@@ -352,3 +352,17 @@ def test_forward_mode_is_refused(host_side):
         with pytest.raises(RuntimeError, match="forward-mode"):
             torch.autograd.grad(y, leaf, forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y)))
         assert torch.equal(linear_act(*plain, "silu"), y)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_infinity_in_a_broadcast_row(hip, dtype):
+    """Rows that lie on top of each other: beyond the last one the weight's gradient takes none of their values (0 times infinity is NaN)."""
+    gen = torch.Generator().manual_seed(1)
+    row, w, g = make((1, 64), gen, dtype), make((72, 64), gen, dtype), make((301, 72), gen, dtype).abs() + 1
+    row[0, 3] = float("inf")
+    w.requires_grad_(True)
+    from box_convolution import linear_act
+    wd = w.detach().cuda().requires_grad_(True)
+    for x in (row.cuda().expand(301, 64), row.cuda().repeat(301, 1)):
+        dw = torch.autograd.grad(linear_act(x, wd), wd, g.cuda())[0]
+        assert not dw.isnan().any() and bool((dw[:, 3] == float("inf")).all()) and int(dw.isinf().sum()) == 72
