@@ -15,17 +15,21 @@ namespace {
 // 1 / (1 + exp(-z)). exp overflows to infinity from z = -88.7 on, where the quotient is 0 as it should be.
 __device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + __expf(-z)); }
 
-// The normal distribution's probability below z, and its density: with t = 1/(1 + p|z|/sqrt 2) and q the polynomial of
-// Abramowitz and Stegun 7.1.26, erfc(|z|/sqrt 2) = q(t) exp(-z*z/2) within 1.5e-7. One exponential serves both, and what
-// remains for z far below zero is a product and no difference: no cancellation there.
+// The normal distribution's probability below z, and its density. With t = 1/(1 + 0.3039 |z|) the probability beyond |z| is q(t) exp(-z*z/2),
+// q the polynomial of eight terms that fits it best relatively (weighted least squares, the weights raised where the error is largest): within
+// 8.3e-8 from z = 0 to 13.3, where the exponential leaves float32. In float32 it is within 4e-7, and the exponential adds its argument's
+// rounding, z*z * 1e-7: digits are kept as far as the value is a normal number. One exponential serves both.
 struct Normal { float below, density; };
 __device__ __forceinline__ Normal normal(float z) {
     const float e = __builtin_amdgcn_exp2f(z * z * (-0.5f * 1.44269504089f));
-    const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678118f, fabsf(z), 1.0f));
-    float q = fmaf(0.5f * 1.061405429f, t, 0.5f * -1.453152027f);
-    q = fmaf(q, t, 0.5f * 1.421413741f);
-    q = fmaf(q, t, 0.5f * -0.284496736f);
-    q = fmaf(q, t, 0.5f * 0.254829592f);
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.3039f, fabsf(z), 1.0f));
+    float q = fmaf(0.036879742f, t, -0.155553320f);
+    q = fmaf(q, t, 0.192881254f);
+    q = fmaf(q, t, -0.043691076f);
+    q = fmaf(q, t, 0.123832448f);
+    q = fmaf(q, t, 0.102314367f);
+    q = fmaf(q, t, 0.122142549f);
+    q = fmaf(q, t, 0.121194078f);
     const float tail = q * t * e;
     return {z > 0.0f ? 1.0f - tail : tail, 0.39894228040f * e};
 }

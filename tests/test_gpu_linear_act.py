@@ -366,3 +366,18 @@ def test_infinity_in_a_broadcast_row(hip, dtype):
     for x in (row.cuda().expand(301, 64), row.cuda().repeat(301, 1)):
         dw = torch.autograd.grad(linear_act(x, wd), wd, g.cuda())[0]
         assert not dw.isnan().any() and bool((dw[:, 3] == float("inf")).all()) and int(dw.isinf().sum()) == 72
+
+
+@pytest.mark.parametrize("name", ["silu", "gelu"])
+def test_small_values_keep_their_digits(hip, name):
+    """float32 values and derivatives far below zero against 64 bits, relatively: the exponential's argument a is a product rounded twice
+    (3 * 2^-24 |a| with its constant), everything else a dozen roundings, and gelu's fit of the error function 2e-7."""
+    lowest = {"silu": -80.0, "gelu": -12.0}[name]
+    z = torch.linspace(lowest, -2.0, 4001, dtype=torch.float64).float().reshape(-1, 1)
+    out = run(z, torch.ones(1, 1), None, torch.zeros_like(z), name, torch.ones_like(z))
+    zd = z.double()
+    a = zd.abs() if name == "silu" else 0.5 * zd.square()
+    allowed = 3 * 2.0 ** -24 * a + 12 * 2.0 ** -23 + 2e-7
+    for got, want, extra in ((out["y"], ref.act(zd, name), 1), (out["residual"], ref.slope(zd, name), 4)):
+        off = ((got.double().cpu() - want) / want).abs() / (extra * allowed)
+        assert off.max() <= 1, (off.max().item(), z[off.argmax()].item())
