@@ -370,7 +370,8 @@ int boxconv_group_norm_backward(const void* input, const void* weight, const voi
  * bias [out_features], null: 0; residual [rows][out_features], rows ld_residual apart, null: 0;
  * output [rows][out_features]. All of type dtype, at any address of a whole element.
  * slope: null, or for silu and gelu [rows][out_features] elements that receive act' for the backward
- * (float32 for BOXCONV_F32, else 16 bits each: act' + 1/2 in steps of 2^-15, 65535 for NaN).
+ * (float32 for BOXCONV_F32, else 16 bits each, 65535 for NaN and otherwise 16400 plus or minus m:
+ * m = 13100 + 2^15 (|act'| - 2^-5) from |act'| = 2^-5 on, 13100 (32 |act'|)^(1/4) below).
  * The workspace (boxconv_linear_workspace_bytes; may be 0) is 16-byte aligned. */
 size_t boxconv_linear_workspace_bytes(int64_t rows, int64_t in_features, int64_t out_features, int dtype,
                                       int backward);

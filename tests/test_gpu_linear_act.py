@@ -381,3 +381,28 @@ def test_small_values_keep_their_digits(hip, name):
     for got, want, extra in ((out["y"], ref.act(zd, name), 1), (out["residual"], ref.slope(zd, name), 4)):
         off = ((got.double().cpu() - want) / want).abs() / (extra * allowed)
         assert off.max() <= 1, (off.max().item(), z[off.argmax()].item())
+
+
+def _tail_values(name, dtype):
+    """z from where the derivative of silu or gelu is some 1e-10 to where it is 1."""
+    lowest = {"silu": -27.0, "gelu": -7.0}[name]
+    z = torch.linspace(lowest, 8.0, 4001, dtype=torch.float64).to(dtype)
+    return z.reshape(-1, 1)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("name", ["silu", "gelu"])
+def test_small_slopes_keep_their_digits(hip, name, dtype):
+    """dz = act'(z) for a gradient of 1 and z = x: the kept 16-bit act' is off by at most 2^-16, and below 2^-5 by 2^-13.9 |act'|^(3/4) (a code of
+    its fourth root in steps of 1/13100: 4 * 0.5 / 13100 * 2^(-5/4) |act'|^(3/4)), the float32 derivative by 4e-7 near its zero and, in
+    the tail, by the exponential's argument's rounding, and the result is rounded once."""
+    z = _tail_values(name, dtype)
+    ones = torch.ones(z.size(0), 1, dtype=dtype)
+    got = run(z, torch.ones(1, 1, dtype=dtype), None, torch.zeros_like(ones), name, ones)["residual"].double().cpu()
+    d = ref.slope(z.double(), name)
+    error = torch.where(d.abs() < 2.0 ** -5, 2.0 ** -13.9 * d.abs() ** 0.75, 2.0 ** -16) + 1e-6 * d.abs() * (1 + z.double().square()) + 4e-7 * (z.double().abs() < 3)
+    assert bool(((got - d).abs() <= ref.rounded(d, error, dtype)).all())
+    # and what that is: two roundings of float16 (little more than one of bfloat16) at most, wherever |act'| is at least 2^-12
+    tail = (d.abs() >= 2.0 ** -12) & (z.double().abs() > 2)
+    assert bool(((got - d).abs()[tail] <= 2.1 * ref.UNIT[dtype] * d.abs()[tail]).all())
+    assert name == "silu" or bool((got[z.double() == 8] == 1).all())
