@@ -498,19 +498,15 @@ norm_sums_kernel(NormBackwardArgs<T> a, float* __restrict__ partial, Lanes L, in
     });
 }
 
-// totals[b][c] = the partial sums of all workgroups of an item, 16 channels by 64 rows of threads, always in the same order. 5 us, most
-// of it the launch and the chain of sums.
-__global__ void __launch_bounds__(1024)
-norm_join_sums_kernel(const float2* __restrict__ partial, float2* __restrict__ totals, int channels, int chunks, int tiles) {
-    __shared__ float2 part[64][17];
-    const int64_t b = blockIdx.x / static_cast<unsigned>(tiles);
-    const int c = blockIdx.x % static_cast<unsigned>(tiles) * 16 + threadIdx.x % 16, row = threadIdx.x / 16;
+// The sums of rows [first, last) of [..][channels] pairs, channel c of 16 side by side (threadIdx.x % 16): a workgroup's 64 rows of threads
+// walk down, then a tree, always in the same order. The result is in the first row of threads.
+__device__ __forceinline__ float2 sum_rows(const float2* __restrict__ rows, int64_t first, int64_t last, int channels, int c, float2 (*part)[17]) {
+    const int row = threadIdx.x / 16;
     float2 s = {0.0f, 0.0f};
     if (c < channels) {
-        const float2* p = partial + b * chunks * channels + c;
 #pragma unroll 4
-        for (int i = row; i < chunks; i += 64) {
-            const float2 v = p[static_cast<int64_t>(i) * channels];
+        for (int64_t i = first + row; i < last; i += 64) {
+            const float2 v = rows[i * channels + c];
             s.x += v.x;
             s.y += v.y;
         }
@@ -526,7 +522,18 @@ norm_join_sums_kernel(const float2* __restrict__ partial, float2* __restrict__ t
         }
         __syncthreads();
     }
-    if (row == 0 && c < channels) totals[b * channels + c] = s;
+    return s;
+}
+
+// totals[p][c] = the sums of rows [p * per, (p + 1) * per) of `rows`: of an item's workgroups, or of some of the batch items. 5 us, most of
+// it the launch and the chain of sums.
+__global__ void __launch_bounds__(1024)
+norm_join_sums_kernel(const float2* __restrict__ partial, float2* __restrict__ totals, int channels, int64_t per, int64_t rows, int tiles) {
+    __shared__ float2 part[64][17];
+    const int64_t p = blockIdx.x / static_cast<unsigned>(tiles);
+    const int c = blockIdx.x % static_cast<unsigned>(tiles) * 16 + threadIdx.x % 16;
+    const float2 s = sum_rows(partial, p * per, min(rows, (p + 1) * per), channels, c, part);
+    if (threadIdx.x < 16 && c < channels) totals[p * channels + c] = s;
 }
 
 // s1/m and s2/m of the groups of `slab` channels from c0 on, in LDS, from per-channel totals.
@@ -550,7 +557,8 @@ __device__ __forceinline__ void group_terms(float2* terms, Total total, const No
     }
 }
 
-// dweight, dbias: the totals of all batch items, in their order. Threads [first, first + n) of the launch.
+// dweight, dbias: the totals of a few batch items, one after the other.
+constexpr int64_t kFewItems = 64;
 template <class T>
 __device__ __forceinline__ void parameter_sums(const NormBackwardArgs<T>& a, const float2* totals, int64_t batch, int channels, int c) {
     float s = 0.0f, d = 0.0f;
@@ -561,6 +569,17 @@ __device__ __forceinline__ void parameter_sums(const NormBackwardArgs<T>& a, con
     }
     if (a.dbias) store_param<T>(a.dbias, a.float_params, c, s);
     if (a.dweight) store_param<T>(a.dweight, a.float_params, c, d);
+}
+
+// The same of many items (or of sums over some of them each).
+template <class T>
+__global__ void __launch_bounds__(1024) norm_parameter_kernel(NormBackwardArgs<T> a, const float2* __restrict__ totals, int64_t rows, int channels) {
+    __shared__ float2 part[64][17];
+    const int c = blockIdx.x * 16 + threadIdx.x % 16;
+    const float2 s = sum_rows(totals, 0, rows, channels, c, part);
+    if (threadIdx.x >= 16 || c >= channels) return;
+    if (a.dbias) store_param<T>(a.dbias, a.float_params, c, s.x);
+    if (a.dweight) store_param<T>(a.dweight, a.float_params, c, s.y);
 }
 
 // ---- backward, second pass: dx and dresidual -----------------------------------------------------------
@@ -574,9 +593,10 @@ norm_grad_kernel(NormBackwardArgs<T> a, const float2* __restrict__ totals, Lanes
     typedef typename Vec<T>::Type Packed;
     extern __shared__ float lds[];
     const int t = threadIdx.x;
-    // the first workgroups add up the parameter gradients on the side
-    for (int64_t c = blockIdx.x * static_cast<int64_t>(blockDim.x) + t; c < L.channels; c += static_cast<int64_t>(total_workgroups) * blockDim.x)
-        parameter_sums(a, totals, batch, L.channels, static_cast<int>(c));
+    // the first workgroups add up the parameter gradients of a small batch on the side
+    if (batch <= kFewItems)
+        for (int64_t c = blockIdx.x * static_cast<int64_t>(blockDim.x) + t; c < L.channels; c += static_cast<int64_t>(total_workgroups) * blockDim.x)
+            parameter_sums(a, totals, batch, L.channels, static_cast<int>(c));
     if (a.dx == nullptr && a.dresidual == nullptr) return;
     const unsigned id = total_workgroups - 1 - blockIdx.x, chunk = id % static_cast<unsigned>(chunks);   // last to first, as in norm_apply_kernel
     const int64_t b = id / static_cast<unsigned>(chunks);
@@ -804,12 +824,6 @@ norm_small_grad_kernel(NormBackwardArgs<T> a, float2* __restrict__ totals, Lanes
     }
 }
 
-template <class T>
-__global__ void __launch_bounds__(256) norm_parameter_kernel(NormBackwardArgs<T> a, const float2* __restrict__ totals, int64_t batch, int channels) {
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    if (c < channels) parameter_sums(a, totals, batch, channels, c);
-}
-
 // ---- numbers of channels that no workgroup's lanes can repeat over (odd and above 1024), items of a few elements --------------
 // A workgroup takes a chunk of whole pixels of one (batch item, group), element by element. Bound by the index arithmetic and loads of
 // two or four bytes: 2 x 64 x 64 x
@@ -1000,6 +1014,15 @@ NormPlan plan_norm(int64_t batch, int64_t pixels, int channels, int groups, int 
     return p;
 }
 
+// How the parameters' gradients are summed over the batch: in pieces of `per` items, whose sums are added by another launch. A thread adds 64
+// to 512 values one after the other up to half a billion items, and a tree joins the threads' sums. (One chain over all items loses digits
+// with their number: 100000 times the same gradient 1.1 was off by 9e-4 of the sum.) One piece up to 4096 items.
+struct ItemsPlan { int64_t pieces, per; };
+ItemsPlan plan_items(int64_t batch) {
+    const int64_t per = std::max<int64_t>(4096, (batch + 16383) / 16384);
+    return {(batch + per - 1) / per, per};
+}
+
 template <int ACT> struct ActTag { static constexpr int value = ACT; };
 template <class F>
 hipError_t with_activation(int act, F f) {
@@ -1081,6 +1104,19 @@ hipError_t forward(const NormCall& n, void* workspace, hipStream_t stream) {
     });
 }
 
+// dweight and dbias from the items' totals; `spare`: room for the sums of several pieces.
+template <class T>
+void parameter_gradients(const NormBackwardArgs<T>& a, const float2* totals, float2* spare, int64_t batch, int channels, hipStream_t stream) {
+    if (a.dweight == nullptr && a.dbias == nullptr) return;
+    const ItemsPlan p = plan_items(batch);
+    const int tiles = (channels + 15) / 16;
+    if (p.pieces > 1)
+        BOXCONV_LAUNCH("norm_join_sums", norm_join_sums_kernel, dim3(static_cast<unsigned>(p.pieces * tiles)), dim3(1024), 0, stream, totals, spare, channels,
+                       p.per, batch, tiles);
+    BOXCONV_LAUNCH("norm_parameter", (norm_parameter_kernel<T>), dim3(static_cast<unsigned>(tiles)), dim3(1024), 0, stream, a, p.pieces > 1 ? spare : totals,
+                   p.pieces > 1 ? p.pieces : batch, channels);
+}
+
 template <class T>
 hipError_t backward(const NormGradCall& n, void* workspace, hipStream_t stream) {
     constexpr int V = Vec<T>::kLen;
@@ -1103,14 +1139,12 @@ hipError_t backward(const NormGradCall& n, void* workspace, hipStream_t stream) 
     const Lanes L = p.L;
     const float inv_m = static_cast<float>(1.0 / (static_cast<double>(n.pixels) * a.per_group));
     float2* totals = static_cast<float2*>(workspace);
-    float2* partial = totals + n.batch * n.channels;
-    const dim3 param_grid(static_cast<unsigned>((n.channels + 255) / 256));
-    const bool params = n.dweight != nullptr || n.dbias != nullptr;
+    float2 *partial = totals + n.batch * n.channels, *spare = partial + (p.any || p.small ? 0 : n.batch * p.chunks * n.channels);
     if (p.any)
         return with_activation(n.activation, [&](auto act) {
             BOXCONV_LAUNCH("norm_any_sums", (norm_any_sums_kernel<T, decltype(act)::value>), dim3(static_cast<unsigned>(n.batch * n.channels)), dim3(256), 0,
                            stream, a, totals, n.pixels, n.channels);
-            if (params) BOXCONV_LAUNCH("norm_parameter", (norm_parameter_kernel<T>), param_grid, dim3(256), 0, stream, a, totals, n.batch, n.channels);
+            parameter_gradients(a, totals, spare, n.batch, n.channels, stream);
             if (a.dx != nullptr)
                 BOXCONV_LAUNCH("norm_any_grad", (norm_any_grad_kernel<T, decltype(act)::value>), dim3(static_cast<unsigned>(n.batch * n.groups * p.chunks)),
                                dim3(256), 0, stream, a, totals, n.pixels, n.channels, p.chunk_steps, p.chunks, inv_m);
@@ -1121,7 +1155,7 @@ hipError_t backward(const NormGradCall& n, void* workspace, hipStream_t stream) 
             const size_t lds = static_cast<size_t>(2) * kept_words(L.active, V) * 4 + static_cast<size_t>(L.slab) * 8 + static_cast<size_t>(L.slab / a.per_group) * 8;
             BOXCONV_LAUNCH("norm_small_grad", (norm_small_grad_kernel<T, decltype(act)::value>), dim3(static_cast<unsigned>(n.batch * p.slabs)),
                            dim3(p.threads), lds, stream, a, totals, L, p.slabs, inv_m, n.batch == 1);
-            if (params && n.batch > 1) BOXCONV_LAUNCH("norm_parameter", (norm_parameter_kernel<T>), param_grid, dim3(256), 0, stream, a, totals, n.batch, n.channels);
+            if (n.batch > 1) parameter_gradients(a, totals, spare, n.batch, n.channels, stream);
             return hipGetLastError();
         });
     const int workgroups = static_cast<int>(n.batch * p.pieces), tiles = (n.channels + 15) / 16;
@@ -1129,7 +1163,8 @@ hipError_t backward(const NormGradCall& n, void* workspace, hipStream_t stream) 
         BOXCONV_LAUNCH("norm_sums", (norm_sums_kernel<T, decltype(act)::value>), dim3(static_cast<unsigned>(n.batch * p.chunks)), dim3(p.threads), static_cast<size_t>(2) * kept_words(L.active, V) * 4,
                        stream, a, reinterpret_cast<float*>(partial), L, p.chunk_steps, p.chunks);
         BOXCONV_LAUNCH("norm_join_sums", norm_join_sums_kernel, dim3(static_cast<unsigned>(n.batch * tiles)), dim3(1024), 0, stream, partial, totals,
-                       n.channels, p.chunks, tiles);
+                       n.channels, p.chunks, n.batch * p.chunks, tiles);
+        if (n.batch > kFewItems) parameter_gradients(a, totals, spare, n.batch, n.channels, stream);
         BOXCONV_LAUNCH("norm_grad", (norm_grad_kernel<T, decltype(act)::value>), dim3(workgroups), dim3(p.threads), static_cast<size_t>(a.groups) * 8, stream,
                        a, totals, L, p.piece_steps, p.pieces, n.batch, inv_m, workgroups);
         return hipGetLastError();
@@ -1141,7 +1176,8 @@ hipError_t backward(const NormGradCall& n, void* workspace, hipStream_t stream) 
 size_t norm_workspace_bytes(int64_t batch, int64_t pixels, int channels, int groups, int dtype, bool backward_pass) {
     const NormPlan p = plan_norm(batch, pixels, channels, groups, dtype == kF32 ? 4 : 8, backward_pass ? 1 : kMostVectors);
     const int64_t chunks = p.small || (p.any && backward_pass) ? 0 : batch * p.chunks;
-    if (backward_pass) return static_cast<size_t>(batch * channels + chunks * channels) * 8;
+    const ItemsPlan items = plan_items(batch);
+    if (backward_pass) return static_cast<size_t>(batch + chunks + (items.pieces > 1 ? items.pieces : 0)) * channels * 8;
     return chunks ? static_cast<size_t>(chunks * groups * 2 + batch * groups * 2) * 4 : 0;
 }
 

@@ -377,3 +377,12 @@ def test_forward_mode_is_refused(host_side):
         with pytest.raises(RuntimeError, match="forward-mode"):
             torch.autograd.grad(y, leaf, forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y)))
         assert torch.equal(group_norm_act(x, 4, w, b, r, "silu"), y)
+
+
+@pytest.mark.parametrize("size", [(100001, 64, 8, ()), (30001, 8, 2, (2, 2)), (4097, 1031, 1, ()), (70003, 3, 1, ()), (257, 4, 2, (92, 91)), (4095, 16, 4, ())])
+def test_parameter_gradients_over_many_items(hip, size):
+    """The sums over the batch are joined as the others are: as many float32 additions in a row as the bound allows, whatever the batch.
+    The same gradient everywhere, as a mean has it: in one chain of additions its roundings would add up."""
+    c = case(*size, torch.float32, None, False, "float")
+    c["grad"] = torch.full_like(c["grad"], 1.1)
+    ref.check(run(c), expected(c))
