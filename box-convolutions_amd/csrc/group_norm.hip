@@ -573,13 +573,14 @@ __device__ __forceinline__ void parameter_sums(const NormBackwardArgs<T>& a, con
 
 // The same of many items (or of sums over some of them each).
 template <class T>
-__global__ void __launch_bounds__(1024) norm_parameter_kernel(NormBackwardArgs<T> a, const float2* __restrict__ totals, int64_t rows, int channels) {
+__global__ void __launch_bounds__(1024) norm_parameter_kernel(const float2* __restrict__ totals, int64_t rows, int channels, void* dweight,
+                                                                    void* dbias, bool float_params) {
     __shared__ float2 part[64][17];
     const int c = blockIdx.x * 16 + threadIdx.x % 16;
     const float2 s = sum_rows(totals, 0, rows, channels, c, part);
     if (threadIdx.x >= 16 || c >= channels) return;
-    if (a.dbias) store_param<T>(a.dbias, a.float_params, c, s.x);
-    if (a.dweight) store_param<T>(a.dweight, a.float_params, c, s.y);
+    if (dbias) store_param<T>(dbias, float_params, c, s.x);
+    if (dweight) store_param<T>(dweight, float_params, c, s.y);
 }
 
 // ---- backward, second pass: dx and dresidual -----------------------------------------------------------
@@ -1044,8 +1045,18 @@ hipError_t with_count(int n, F f) {
     }
 }
 
+// Items that one launch takes: a grid has fewer than 2^32 threads. (What a workgroup does depends on the plan for all items, not on the launch.)
+int64_t items_per_launch(const NormPlan& p, int64_t channels, int64_t groups) {
+    const int64_t widest = p.any     ? std::max(channels, groups * p.chunks) * 256
+                           : p.small ? static_cast<int64_t>(p.slabs) * p.threads
+                                     : std::max({static_cast<int64_t>(std::max(p.chunks, p.pieces)) * p.threads, groups * 256, (channels + 15) / 16 * 1024});
+    return std::max<int64_t>(1, kMostThreads / widest);
+}
+template <class T, class P>
+P* from_item(P* p, int64_t elements) { return p == nullptr ? nullptr : reinterpret_cast<P*>(reinterpret_cast<uintptr_t>(p) + elements * sizeof(T)); }
+
 template <class T>
-hipError_t forward(const NormCall& n, void* workspace, hipStream_t stream) {
+hipError_t forward_items(const NormCall& n, const NormPlan& p, void* workspace, hipStream_t stream) {
     constexpr int V = Vec<T>::kLen;
     NormArgs<T> a;
     a.x = static_cast<const T*>(n.x);
@@ -1057,7 +1068,6 @@ hipError_t forward(const NormCall& n, void* workspace, hipStream_t stream) {
     a.groups = n.groups;
     a.per_group = n.channels / n.groups;
     a.eps = n.eps;
-    const NormPlan p = plan_norm(n.batch, n.pixels, n.channels, n.groups, V, kMostVectors);
     const Lanes L = p.L;
     if (p.small)
         return with_activation(n.activation, [&](auto act) {
@@ -1106,19 +1116,37 @@ hipError_t forward(const NormCall& n, void* workspace, hipStream_t stream) {
 
 // dweight and dbias from the items' totals; `spare`: room for the sums of several pieces.
 template <class T>
-void parameter_gradients(const NormBackwardArgs<T>& a, const float2* totals, float2* spare, int64_t batch, int channels, hipStream_t stream) {
-    if (a.dweight == nullptr && a.dbias == nullptr) return;
+void parameter_gradients(const NormGradCall& n, const float2* totals, float2* spare, int64_t batch, hipStream_t stream) {
+    if (n.dweight == nullptr && n.dbias == nullptr) return;
     const ItemsPlan p = plan_items(batch);
-    const int tiles = (channels + 15) / 16;
+    const int tiles = (n.channels + 15) / 16;
     if (p.pieces > 1)
-        BOXCONV_LAUNCH("norm_join_sums", norm_join_sums_kernel, dim3(static_cast<unsigned>(p.pieces * tiles)), dim3(1024), 0, stream, totals, spare, channels,
+        BOXCONV_LAUNCH("norm_join_sums", norm_join_sums_kernel, dim3(static_cast<unsigned>(p.pieces * tiles)), dim3(1024), 0, stream, totals, spare, n.channels,
                        p.per, batch, tiles);
-    BOXCONV_LAUNCH("norm_parameter", (norm_parameter_kernel<T>), dim3(static_cast<unsigned>(tiles)), dim3(1024), 0, stream, a, p.pieces > 1 ? spare : totals,
-                   p.pieces > 1 ? p.pieces : batch, channels);
+    BOXCONV_LAUNCH("norm_parameter", (norm_parameter_kernel<T>), dim3(static_cast<unsigned>(tiles)), dim3(1024), 0, stream, p.pieces > 1 ? spare : totals,
+                   p.pieces > 1 ? p.pieces : batch, n.channels, n.dweight, n.dbias, n.float_params);
 }
 
 template <class T>
-hipError_t backward(const NormGradCall& n, void* workspace, hipStream_t stream) {
+hipError_t forward(NormCall n, void* workspace, hipStream_t stream) {
+    const NormPlan p = plan_norm(n.batch, n.pixels, n.channels, n.groups, Vec<T>::kLen, kMostVectors);
+    const int64_t most = items_per_launch(p, n.channels, n.groups);
+    for (int64_t left = n.batch; left > 0; left -= n.batch) {
+        n.batch = std::min(left, most);
+        if (const hipError_t e = forward_items<T>(n, p, workspace, stream); e != hipSuccess) return e;
+        const int64_t elements = n.batch * p.L.total, pairs = n.batch * n.groups;
+        n.x = from_item<T>(n.x, elements);
+        n.residual = from_item<T>(n.residual, elements);
+        n.y = from_item<T>(n.y, elements);
+        n.mean = from_item<float>(n.mean, pairs);
+        n.rstd = from_item<float>(n.rstd, pairs);
+    }
+    return hipSuccess;
+}
+
+// dx, dresidual and the items' totals; of `all_items` up to kFewItems dweight and dbias too (then this is all of them).
+template <class T>
+hipError_t backward_items(const NormGradCall& n, const NormPlan& p, int64_t all_items, float2* totals, float2* partial, hipStream_t stream) {
     constexpr int V = Vec<T>::kLen;
     NormBackwardArgs<T> a;
     a.x = static_cast<const T*>(n.x);
@@ -1135,16 +1163,12 @@ hipError_t backward(const NormGradCall& n, void* workspace, hipStream_t stream) 
     a.float_params = n.float_params;
     a.groups = n.groups;
     a.per_group = n.channels / n.groups;
-    const NormPlan p = plan_norm(n.batch, n.pixels, n.channels, n.groups, V, 1);
     const Lanes L = p.L;
     const float inv_m = static_cast<float>(1.0 / (static_cast<double>(n.pixels) * a.per_group));
-    float2* totals = static_cast<float2*>(workspace);
-    float2 *partial = totals + n.batch * n.channels, *spare = partial + (p.any || p.small ? 0 : n.batch * p.chunks * n.channels);
     if (p.any)
         return with_activation(n.activation, [&](auto act) {
             BOXCONV_LAUNCH("norm_any_sums", (norm_any_sums_kernel<T, decltype(act)::value>), dim3(static_cast<unsigned>(n.batch * n.channels)), dim3(256), 0,
                            stream, a, totals, n.pixels, n.channels);
-            parameter_gradients(a, totals, spare, n.batch, n.channels, stream);
             if (a.dx != nullptr)
                 BOXCONV_LAUNCH("norm_any_grad", (norm_any_grad_kernel<T, decltype(act)::value>), dim3(static_cast<unsigned>(n.batch * n.groups * p.chunks)),
                                dim3(256), 0, stream, a, totals, n.pixels, n.channels, p.chunk_steps, p.chunks, inv_m);
@@ -1154,8 +1178,7 @@ hipError_t backward(const NormGradCall& n, void* workspace, hipStream_t stream) 
         return with_activation(n.activation, [&](auto act) {
             const size_t lds = static_cast<size_t>(2) * kept_words(L.active, V) * 4 + static_cast<size_t>(L.slab) * 8 + static_cast<size_t>(L.slab / a.per_group) * 8;
             BOXCONV_LAUNCH("norm_small_grad", (norm_small_grad_kernel<T, decltype(act)::value>), dim3(static_cast<unsigned>(n.batch * p.slabs)),
-                           dim3(p.threads), lds, stream, a, totals, L, p.slabs, inv_m, n.batch == 1);
-            if (n.batch > 1) parameter_gradients(a, totals, spare, n.batch, n.channels, stream);
+                           dim3(p.threads), lds, stream, a, totals, L, p.slabs, inv_m, all_items == 1);
             return hipGetLastError();
         });
     const int workgroups = static_cast<int>(n.batch * p.pieces), tiles = (n.channels + 15) / 16;
@@ -1164,11 +1187,35 @@ hipError_t backward(const NormGradCall& n, void* workspace, hipStream_t stream) 
                        stream, a, reinterpret_cast<float*>(partial), L, p.chunk_steps, p.chunks);
         BOXCONV_LAUNCH("norm_join_sums", norm_join_sums_kernel, dim3(static_cast<unsigned>(n.batch * tiles)), dim3(1024), 0, stream, partial, totals,
                        n.channels, p.chunks, n.batch * p.chunks, tiles);
-        if (n.batch > kFewItems) parameter_gradients(a, totals, spare, n.batch, n.channels, stream);
         BOXCONV_LAUNCH("norm_grad", (norm_grad_kernel<T, decltype(act)::value>), dim3(workgroups), dim3(p.threads), static_cast<size_t>(a.groups) * 8, stream,
-                       a, totals, L, p.piece_steps, p.pieces, n.batch, inv_m, workgroups);
+                       a, totals, L, p.piece_steps, p.pieces, all_items, inv_m, workgroups);
         return hipGetLastError();
     });
+}
+
+template <class T>
+hipError_t backward(NormGradCall n, void* workspace, hipStream_t stream) {
+    const NormPlan p = plan_norm(n.batch, n.pixels, n.channels, n.groups, Vec<T>::kLen, 1);
+    const int64_t batch = n.batch, most = items_per_launch(p, n.channels, n.groups);
+    float2* totals = static_cast<float2*>(workspace);
+    float2 *partial = totals + batch * n.channels, *spare = partial + (p.any || p.small ? 0 : batch * p.chunks * n.channels);
+    float2* of_items = totals;
+    for (int64_t left = batch; left > 0; left -= n.batch) {
+        n.batch = std::min(left, most);
+        if (const hipError_t e = backward_items<T>(n, p, batch, of_items, partial, stream); e != hipSuccess) return e;
+        const int64_t elements = n.batch * p.L.total, pairs = n.batch * n.groups;
+        n.x = from_item<T>(n.x, elements);
+        n.residual = from_item<T>(n.residual, elements);
+        n.dy = from_item<T>(n.dy, elements);
+        n.dx = from_item<T>(n.dx, elements);
+        n.dresidual = from_item<T>(n.dresidual, elements);
+        n.mean = from_item<float>(n.mean, pairs);
+        n.rstd = from_item<float>(n.rstd, pairs);
+        of_items += n.batch * n.channels;
+    }
+    const bool done = p.small ? batch == 1 : !p.any && batch <= kFewItems;     // by the launches above
+    if (!done) parameter_gradients<T>(n, totals, spare, batch, stream);
+    return hipGetLastError();
 }
 
 }  // namespace

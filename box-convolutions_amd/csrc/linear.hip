@@ -420,22 +420,38 @@ hipError_t few_rows(const Operand<T>& a, const Operand<T>& b, const Tail<T>& tai
 }
 
 template <class T, bool A_K, bool B_K>
+void launch_product(const char* name, Operand<T> a, const Operand<T>& b, Tail<T> tail, ProductPlan p, bool wide, hipStream_t stream) {
+    // a grid has fewer than 2^32 threads: with more tiles (never in several parts of k) some rows of the output after the others
+    const int64_t threads = wide && p.shape == 0 ? 512 : 256, tile = wide ? kWide[p.shape].tm : kAny[p.shape].tm;
+    const int64_t rows = tail.rows, most = std::max<int64_t>(1, kMostThreads / threads / p.tiles_n) * tile;
+    for (int64_t m = 0; m < rows; m += most) {
+        tail.rows = a.extent = std::min(most, rows - m);
+        p.tiles_m = (tail.rows + tile - 1) / tile;
+        if (wide) {
+            switch (p.shape) {
+                case 0: launch_wide<T, A_K, B_K, 256, 256, 4, 2>(name, a, b, tail, p, stream); break;
+                case 1: launch_wide<T, A_K, B_K, 128, 128, 2, 2>(name, a, b, tail, p, stream); break;
+                default: launch_wide<T, A_K, B_K, 64, 64, 2, 2>(name, a, b, tail, p, stream);
+            }
+        } else {
+            const dim3 grid(static_cast<unsigned>(p.tiles_m * p.tiles_n), p.splits);
+            if (p.shape == 0) BOXCONV_LAUNCH(name, (product_kernel<T, A_K, B_K, 128>), grid, dim3(256), 0, stream, a, b, tail, p.k_part, p.tiles_m, p.tiles_n);
+            else BOXCONV_LAUNCH(name, (product_kernel<T, A_K, B_K, 64>), grid, dim3(256), 0, stream, a, b, tail, p.k_part, p.tiles_m, p.tiles_n);
+        }
+        a.p += most * (A_K ? a.ld : 1);
+        tail.out += most * tail.cols;
+        if (tail.residual != nullptr) tail.residual += most * tail.ld_residual;
+        if (tail.slope != nullptr) tail.slope += most * tail.cols;
+    }
+}
+
+template <class T, bool A_K, bool B_K>
 hipError_t product(const char* name, Operand<T> a, Operand<T> b, Tail<T> tail, float* workspace, hipStream_t stream) {
     const bool wide = whole_chunks<T, A_K>(a) && whole_chunks<T, B_K>(b);
     const bool keeps = tail.slope != nullptr;
     const ProductPlan p = wide ? plan_product<T>(kWide, tail.rows, tail.cols, a.depth, keeps) : plan_product<T>(kAny, tail.rows, tail.cols, a.depth, keeps);
     tail.partial = p.splits > 1 ? workspace : nullptr;
-    if (wide) {
-        switch (p.shape) {
-            case 0: launch_wide<T, A_K, B_K, 256, 256, 4, 2>(name, a, b, tail, p, stream); break;
-            case 1: launch_wide<T, A_K, B_K, 128, 128, 2, 2>(name, a, b, tail, p, stream); break;
-            default: launch_wide<T, A_K, B_K, 64, 64, 2, 2>(name, a, b, tail, p, stream);
-        }
-    } else {
-        const dim3 grid(static_cast<unsigned>(p.tiles_m * p.tiles_n), p.splits);
-        if (p.shape == 0) BOXCONV_LAUNCH(name, (product_kernel<T, A_K, B_K, 128>), grid, dim3(256), 0, stream, a, b, tail, p.k_part, p.tiles_m, p.tiles_n);
-        else BOXCONV_LAUNCH(name, (product_kernel<T, A_K, B_K, 64>), grid, dim3(256), 0, stream, a, b, tail, p.k_part, p.tiles_m, p.tiles_n);
-    }
+    launch_product<T, A_K, B_K>(name, a, b, tail, p, wide, stream);
     if (p.splits > 1) join_parts(tail, p.splits, stream);
     return hipGetLastError();
 }

@@ -21,8 +21,8 @@ int check_norm(int dtype, int param_dtype, int64_t batch, int64_t pixels, int ch
                     static_cast<long long>(pixels), channels, groups);
     if (activation < BOXCONV_ACT_NONE || activation > BOXCONV_ACT_GELU)
         return fail(BOXCONV_E_INVALID_ARGUMENT, "group norm: unknown activation %d", activation);
-    // workgroups of one launch: at most 2048 + batch of an item's parts, or one per batch item and channel
-    if (batch > kMaxExtent / channels || pixels > (int64_t(1) << 46) / channels)
+    // batch items are split over launches where a grid would have 2^32 threads or more; one item has at most a workgroup of 256 per channel
+    if (channels > kMostThreads / 256 || batch > kMaxExtent / channels || pixels > (int64_t(1) << 46) / channels)
         return fail(BOXCONV_E_TOO_LARGE, "group norm: batch=%lld items of pixels=%lld x channels=%d are too many", static_cast<long long>(batch),
                     static_cast<long long>(pixels), channels);
     return 0;
@@ -126,6 +126,9 @@ int boxconv_linear_backward(const void* input, int64_t ld_input, const void* wei
     if (grad_output == nullptr || (activation != BOXCONV_ACT_NONE && kept == nullptr) || (grad_input != nullptr && weight == nullptr) ||
         (grad_weight != nullptr && input == nullptr))
         return fail(BOXCONV_E_INVALID_ARGUMENT, "linear: null input, weight, grad_output or kept pointer");
+    // (rows of tiles are split over launches where a grid would have 2^32 threads or more; one row of them has to fit)
+    if ((grad_input != nullptr || grad_weight != nullptr) && (in_features + 63) / 64 > kMostThreads / 256)
+        return fail(BOXCONV_E_TOO_LARGE, "linear: gradients of in_features=%lld are too large", static_cast<long long>(in_features));
     const size_t need = boxconv_linear_workspace_bytes(rows, in_features, out_features, dtype, 1);
     if (const int rc = check_workspace("linear", workspace, workspace_bytes, need)) return rc;
     const LinearGradCall call = {input, weight, grad_output, kept, ld_input, grad_input, grad_weight, grad_bias, grad_residual, rows, in_features, out_features,

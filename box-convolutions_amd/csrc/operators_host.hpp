@@ -10,6 +10,8 @@ namespace boxconv {
 // element type codes, BOXCONV_F32 / F16 / BF16 of include/boxconv.h
 constexpr int kF32 = 0, kF16 = 1, kBF16 = 2;
 
+constexpr int64_t kMostThreads = (int64_t(1) << 32) - 1;     // of a grid along x
+
 // Arguments as in boxconv_group_norm_forward / _backward (include/boxconv.h), checked by the caller.
 struct NormCall {
     const void *x, *weight, *bias, *residual;

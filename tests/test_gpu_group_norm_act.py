@@ -386,3 +386,30 @@ def test_parameter_gradients_over_many_items(hip, size):
     c = case(*size, torch.float32, None, False, "float")
     c["grad"] = torch.full_like(c["grad"], 1.1)
     ref.check(run(c), expected(c))
+
+
+@pytest.mark.parametrize("B,C,G", [(5000003, 4, 4), ((1 << 26) + 3, 8, 2)])
+def test_more_workgroups_than_a_grid_takes(hip, B, C, G):
+    """Items whose workgroups have 2^32 threads and more together (a workgroup per item and channel, and one per item): the first, the last
+    and those around every 2^22nd are those of the same items alone, and the parameters' gradients the sums over parts."""
+    from box_convolution import group_norm_act
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    x, g = (torch.randn(B, C, generator=gen, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    w, b = (torch.randn(C, generator=gen, device="cuda").requires_grad_(True) for _ in range(2))
+
+    def both(part):
+        xs = x[part].detach().requires_grad_(True)
+        y = group_norm_act(xs, G, w, b, activation="silu")
+        return (y.detach(), *torch.autograd.grad(y, (xs, w, b), g[part]))
+    y, dx, dw, db = both(slice(0, B))
+    for at in [0, B - 500] + list(range((1 << 22) - 250, B - 500, 1 << 22)):
+        part = slice(at, at + 500)
+        some = both(part)
+        assert torch.equal(some[0], y[part]) and torch.equal(some[1], dx[part]), at
+    step, sums = B // 4 + 1, [0.0, 0.0]
+    for at in range(0, B, step):
+        some = both(slice(at, at + step))
+        sums = [s + t.double() for s, t in zip(sums, some[2:])]
+    # (512 additions in a row, of B values of the size 1 to 4 that mostly cancel: both ways)
+    for got, want in zip((dw, db), sums):
+        assert (got.double() - want).abs().max() <= 2 * ref.DEPTH * ref.U32 * 4 * B

@@ -406,3 +406,21 @@ def test_small_slopes_keep_their_digits(hip, name, dtype):
     tail = (d.abs() >= 2.0 ** -12) & (z.double().abs() > 2)
     assert bool(((got - d).abs()[tail] <= 2.1 * ref.UNIT[dtype] * d.abs()[tail]).all())
     assert name == "silu" or bool((got[z.double() == 8] == 1).all())
+
+
+def test_more_tiles_than_a_grid_takes(hip):
+    """Rows in so many tiles that their workgroups have 2^32 threads together: the rows around the place where the second launch starts, the
+    first and the last are those of the same rows alone."""
+    from box_convolution import linear_act
+    rows, base = (1 << 30) + 777, 1 << 20
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    x = torch.randn(base, 8, generator=gen, device="cuda", dtype=torch.bfloat16).repeat(rows // base + 1, 1)[:rows].requires_grad_(True)
+    w = torch.randn(1, 8, generator=gen, device="cuda", dtype=torch.bfloat16)
+    y = linear_act(x, w, activation="silu")
+    g = torch.randn(base, 1, generator=gen, device="cuda", dtype=torch.bfloat16).repeat(rows // base + 1, 1)[:rows]
+    dx = torch.autograd.grad(y, x, g)[0]
+    for at in (0, (1 << 30) - 64 - 500, (1 << 30) - 500, rows - 1000):
+        part = slice(at, at + 1000)
+        xs = x.detach()[part].requires_grad_(True)
+        ys = linear_act(xs, w, activation="silu")
+        assert torch.equal(ys, y[part]) and torch.equal(torch.autograd.grad(ys, xs, g[part])[0], dx[part]), at

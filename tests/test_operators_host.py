@@ -136,3 +136,14 @@ def test_scratch_of_calls_that_overlap(monkeypatch, call):
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
     calls[call]()
     assert len(seen) == 2 and None not in seen and seen[0] != seen[1]
+
+
+def test_sizes_that_no_launch_takes(lib):
+    """A grid has fewer than 2^32 threads: one item's or one row of tiles' workgroups have to fit, and are refused where they do not."""
+    most = (1 << 24) - 1
+    assert norm(lib, batch=1, pixels=1, channels=most + 1, groups=1) == -3 and b"too many" in lib.boxconv_last_error()
+    assert norm(lib, batch=1, pixels=1, channels=most, groups=1) == -2               # (a workspace is all that is missing)
+    back = lib.boxconv_linear_backward
+    for K, code in ((64 * most, -2), (64 * most + 1, -3)):
+        assert back(P, K, P, P, None, P, None, None, None, 1, 100, K, 1, 0, None, 0, None) == code, K
+    assert b"too large" in lib.boxconv_last_error()
