@@ -50,6 +50,18 @@ int check_workspace(const char* what, const void* workspace, size_t have, size_t
     return 0;
 }
 
+__global__ void __launch_bounds__(256) zero_kernel(uint16_t* __restrict__ p, int64_t n) {
+    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) p[i] = 0;
+}
+
+// Sums of nothing: zeros in a gradient of `elements` of type `dtype`, unless it is not wanted.
+int write_zeros(void* p, int64_t elements, int dtype, const char* what, hipStream_t stream) {
+    if (p == nullptr || elements == 0) return 0;
+    const int64_t n = elements * (dtype == BOXCONV_F32 ? 2 : 1), groups = std::min<int64_t>((n + 255) / 256, 4096);
+    BOXCONV_LAUNCH("fill_zero", zero_kernel, dim3(static_cast<unsigned>(groups)), dim3(256), 0, stream, static_cast<uint16_t*>(p), n);
+    return hip_result(hipGetLastError(), what);
+}
+
 template <class F>
 auto with_type(int dtype, F f) {
     if (dtype == BOXCONV_F32) return f(float());
@@ -83,7 +95,10 @@ int boxconv_group_norm_backward(const void* input, const void* weight, const voi
                                 void* grad_residual, int dtype, int64_t batch, int64_t pixels, int channels, int groups, int activation, void* workspace,
                                 size_t workspace_bytes, void* stream) {
     if (const int rc = check_norm(dtype, param_dtype, batch, pixels, channels, groups, activation)) return rc;
-    if (batch == 0 || pixels == 0) return 0;
+    if (batch == 0 || pixels == 0) {
+        if (const int rc = write_zeros(grad_weight, channels, param_dtype, "group norm", static_cast<hipStream_t>(stream))) return rc;
+        return write_zeros(grad_bias, channels, param_dtype, "group norm", static_cast<hipStream_t>(stream));
+    }
     if (grad_input == nullptr && grad_weight == nullptr && grad_bias == nullptr && grad_residual == nullptr) return 0;
     if (input == nullptr || grad_output == nullptr || mean == nullptr || rstd == nullptr)
         return fail(BOXCONV_E_INVALID_ARGUMENT, "group norm: null input, grad_output, mean or rstd pointer");
@@ -120,7 +135,12 @@ int boxconv_linear_backward(const void* input, int64_t ld_input, const void* wei
                             void* grad_weight, void* grad_bias, void* grad_residual, int dtype, int64_t rows, int64_t in_features,
                             int64_t out_features, int activation, void* workspace, size_t workspace_bytes, void* stream) {
     if (const int rc = check_linear(dtype, rows, in_features, out_features, ld_input, activation)) return rc;
-    if (rows == 0 || out_features == 0) return 0;
+    if (rows == 0 || out_features == 0) {
+        const auto zeros = [&](void* p, int64_t elements) { return write_zeros(p, elements, dtype, "linear", static_cast<hipStream_t>(stream)); };
+        if (const int rc = zeros(grad_input, rows * in_features)) return rc;
+        if (const int rc = zeros(grad_weight, out_features * in_features)) return rc;
+        return zeros(grad_bias, out_features);
+    }
     if (in_features == 0) grad_input = grad_weight = nullptr;
     if (grad_input == nullptr && grad_weight == nullptr && grad_bias == nullptr && grad_residual == nullptr) return 0;
     if (grad_output == nullptr || (activation != BOXCONV_ACT_NONE && kept == nullptr) || (grad_input != nullptr && weight == nullptr) ||

@@ -356,7 +356,7 @@ int boxconv_group_norm_forward(const void* input, const void* weight, const void
                                int64_t batch, int64_t pixels, int channels, int groups, float eps,
                                int activation, void* workspace, size_t workspace_bytes, void* stream);
 /* Its gradients; those whose pointer is null are not formed. grad_weight and grad_bias have
- * param_dtype. All other arguments as in the forward call. */
+ * param_dtype; without batch items or pixels they are 0. All other arguments as in the forward call. */
 int boxconv_group_norm_backward(const void* input, const void* weight, const void* bias, int param_dtype,
                                 const void* residual, const void* grad_output, const float* mean,
                                 const float* rstd, void* grad_input, void* grad_weight, void* grad_bias,
@@ -382,7 +382,7 @@ int boxconv_linear_forward(const void* input, int64_t ld_input, const void* weig
 /* Its gradients; those whose pointer is null are not formed. With dz = grad_output * act':
  * grad_input = dz W, grad_weight = dz^T x, grad_bias = column sums of dz, grad_residual = dz.
  * kept: the forward's output for relu, its slope for silu and gelu, null for none. The products are
- * taken of dz rounded to dtype. */
+ * taken of dz rounded to dtype. Sums over no rows or no out_features are 0. */
 int boxconv_linear_backward(const void* input, int64_t ld_input, const void* weight, const void* grad_output,
                             const void* kept, void* grad_input, void* grad_weight, void* grad_bias,
                             void* grad_residual, int dtype, int64_t rows, int64_t in_features,

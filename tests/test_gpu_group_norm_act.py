@@ -413,3 +413,14 @@ def test_more_workgroups_than_a_grid_takes(hip, B, C, G):
     # (512 additions in a row, of B values of the size 1 to 4 that mostly cancel: both ways)
     for got, want in zip((dw, db), sums):
         assert (got.double() - want).abs().max() <= 2 * ref.DEPTH * ref.U32 * 4 * B
+
+
+def test_nothing_to_sum_at_the_c_entry(hip):
+    """Without rows the parameters' gradients are sums of nothing: 0, written by the call."""
+    lib, stream = hip.load(), torch.cuda.current_stream().cuda_stream
+    gw, gb = torch.full((8,), float("nan"), device="cuda"), torch.full((8,), float("nan"), device="cuda", dtype=torch.float32)
+    for batch, pixels in ((0, 9), (2, 0)):
+        gw.fill_(float("nan")), gb.fill_(float("nan"))
+        assert lib.boxconv_group_norm_backward(None, None, None, 0, None, None, None, None, None, gw.data_ptr(), gb.data_ptr(), None, 1, batch, pixels, 8, 2,
+                                               0, None, 0, stream) == 0
+        assert not gw.any() and not gb.any()

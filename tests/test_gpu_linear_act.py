@@ -424,3 +424,13 @@ def test_more_tiles_than_a_grid_takes(hip):
         xs = x.detach()[part].requires_grad_(True)
         ys = linear_act(xs, w, activation="silu")
         assert torch.equal(ys, y[part]) and torch.equal(torch.autograd.grad(ys, xs, g[part])[0], dx[part]), at
+
+
+def test_nothing_to_sum_at_the_c_entry(hip):
+    """Without rows the parameters' gradients are sums of nothing, without output features the input's: 0, written by the call."""
+    lib, stream = hip.load(), torch.cuda.current_stream().cuda_stream
+    for dtype, code in zip(TYPES, (0, 1, 2)):
+        dx, dw, db = (torch.full(s, float("nan"), device="cuda", dtype=dtype) for s in ((5, 8), (6, 8), (6,)))
+        assert lib.boxconv_linear_backward(None, 8, None, None, None, None, dw.data_ptr(), db.data_ptr(), None, code, 0, 8, 6, 0, None, 0, stream) == 0
+        assert lib.boxconv_linear_backward(None, 8, None, None, None, dx.data_ptr(), None, None, None, code, 5, 8, 0, 0, None, 0, stream) == 0
+        assert not dw.any() and not db.any() and not dx.any()
