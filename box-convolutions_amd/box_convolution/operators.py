@@ -77,7 +77,8 @@ def group_norm_act(input, num_groups, weight=None, bias=None, residual=None, act
     """``act(group_norm(input) * weight + bias + residual)`` with gradients.
 
     input:      ``[B, C, ...]``; channels-last memory (``torch.channels_last`` for images) is used as it
-                is, anything else is copied once. The result has channels-last memory.
+                is, anything else is copied once (planes, as ``BoxConv2d`` returns them: the copy takes two to three times
+                the norm's own time). The result has channels-last memory, and so has the gradient.
     weight, bias: ``[C]``, both float32 or both of the input's type; ``None`` is 1 and 0.
     residual:   same shape and type as ``input``, added before the activation.
     activation: ``None``, ``"relu"``, ``"silu"`` or ``"gelu"``.
@@ -139,6 +140,9 @@ def linear_act(input, weight, bias=None, residual=None, activation=None):
     input:      ``[..., K]``; rows may lie apart (a slice of wider rows is not copied).
     weight:     ``[N, K]``; bias ``[N]``; residual ``[..., N]``, added before the activation: all of the input's type.
     activation: ``None``, ``"relu"``, ``"silu"`` or ``"gelu"``.
+
+    Sums are float32. For float16 and bfloat16 the gradient in front of the activation is rounded to the input's type before it is
+    multiplied by weight and input, as it would be between two layers.
     """
     act = _native._activation(activation)
     _native._require_device(input, "linear input")
@@ -188,7 +192,7 @@ class GroupNormAct(torch.nn.GroupNorm):
 class PointwiseConv2d(torch.nn.Conv2d):
     """A 1 x 1 ``torch.nn.Conv2d`` (same parameters, so state dicts interchange) with a residual add and an activation in
     the same kernel: ``module(x, residual=None)``. The output has channels-last memory; so should the input (see
-    ``linear_act``; other layouts are copied)."""
+    ``linear_act``; other layouts are copied). Parameters have the input's type, under ``torch.autocast`` too: nothing is cast."""
 
     def __init__(self, in_channels, out_channels, bias=True, activation=None, device=None, dtype=None):
         super().__init__(in_channels, out_channels, 1, bias=bias, device=device, dtype=dtype)

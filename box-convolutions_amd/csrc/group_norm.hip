@@ -825,11 +825,11 @@ norm_small_grad_kernel(NormBackwardArgs<T> a, float2* __restrict__ totals, Lanes
     }
 }
 
-// ---- numbers of channels that no workgroup's lanes can repeat over (odd and above 1024), items of a few elements --------------
-// A workgroup takes a chunk of whole pixels of one (batch item, group), element by element. Bound by the index arithmetic and loads of
-// two or four bytes: 2 x 64 x 64 x
-// 1031 float16 in one group (17 MB) statistics 16 us, y 17, input gradient 21; the channel sums of the backward, which walk down single channels,
-// 88 us.
+// ---- channels that no workgroup's lanes can repeat over --------------------------------------------------------
+// (odd numbers of them above 1024, multiples of 8 above 8192 in 16-bit types and of 4 above 4096 in float, the like between), and items of fewer
+// elements than a vector. A workgroup takes a chunk of whole pixels of one (batch item, group), element by element. Bound by the index arithmetic
+// and loads of two or four bytes: 2 x 64 x 64 x 1031 float16 in one group (17 MB) statistics 16 us, y 17, input gradient 21; the channel sums of the
+// backward, which walk down single channels, 88 us.
 struct AnyChunk { int64_t base; int g; unsigned elements; };     // of the group: its first element, and how many there are
 __device__ __forceinline__ AnyChunk any_chunk(int64_t pixels, int channels, int groups, int per_group, int64_t chunk_pixels, int chunks) {
     const unsigned chunk = blockIdx.x % static_cast<unsigned>(chunks), pair = blockIdx.x / static_cast<unsigned>(chunks);

@@ -273,7 +273,9 @@ __global__ void __launch_bounds__(256) join_parts_kernel(Tail<T> tail, int split
 // ---- dz = dy * act'(z), and its column sums ---------------------------------------------------------------------
 // A workgroup takes 256 columns (8 per thread, 32 threads) of a band of rows, 8 rows at a time. sums: [bands][cols], null
 // if not wanted; dz: null if not wanted. kept: y for relu, the kept slope for silu and gelu. Bound by memory: 8192 x 2048 bfloat16 (101 MB)
-// 20.6 us, 4.9 TB/s.
+// 22 us, 4.5 TB/s. dz is rounded to T here, once, for both products: with 16-bit types these are the matrix instructions' operands, and dz in two
+// parts would double the backward's matrix work. dx and dW of silu and gelu are then 1.4 times as far from 64 bits as with dz in float: 0.0024 of
+// their norm instead of 0.0017 in bfloat16 (8192 x 4096 -> 2048), 0.00029 instead of 0.00021 in float16 (1501 x 333 -> 517). The column sums take it unrounded.
 template <class T>
 __global__ void __launch_bounds__(256)
 slope_kernel(const T* __restrict__ dy, const void* __restrict__ kept, T* __restrict__ dz, float* __restrict__ sums, T* __restrict__ dbias, int64_t rows,
@@ -341,7 +343,9 @@ struct ProductPlan {
 // Measured on bfloat16 products, M x N x K: 8192 x 4096 x 2048 takes 107 us with 256 x 256 tiles, 137 with 128 x 128; 2048 x 2048 x
 // 4096 takes 78, 48 and, with 64 x 64, 52; 512 x 512 x 4096 33 with 128 x 128, 36 with 64 x 64 (none of them split). Short k, the same
 // three: 300000 x 256 x 64 68, 76 and 86 us; 380192 x 160 x 32 with a kept slope 137, 149 and 109; float, 48552 x 456 x 208 with one 185, 158
-// and 145. Tiles of 256 x 128 were no better than 128 x 128 anywhere: their waves read as much from LDS per product.
+// and 145. Tiles of 256 x 128 were no better than 128 x 128 anywhere: their waves read as much from LDS per product. All of these have k contiguous
+// in both operands. For the weight gradient, where it is the slow index of both, the costs promise too little: 8192 x 4096 -> 2048 with 128 x 128 tiles 119
+// us, and it takes 136 alone and 164 in a training step; other tiles and splits have not been measured there.
 struct ProductShape { int tm, tn, resident; double fixed, each, each_float, ends, slope; };
 constexpr ProductShape kWide[] = {{256, 256, 1, 0.0, 1.38, 7.2, 8.7, 10.0}, {128, 128, 2, 0.46, 0.21, 1.8, 7.6, 5.0}, {64, 64, 4, 0.44, 0.075, 0.44, 5.0, 1.6}};
 constexpr ProductShape kAny[] = {{128, 128, 2, 0.8, 0.4, 2.0, 7.0, 5.0}, {64, 64, 4, 0.5, 0.15, 0.5, 7.0, 1.6}};

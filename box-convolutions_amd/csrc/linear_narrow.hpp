@@ -170,7 +170,7 @@ narrow_grad_kernel(NarrowArgs<T> a) {
                 else if (a.activation != kActNone) f *= kept_slope(static_cast<S>(d[j]));
                 if (m0 + r < a.rows) sums[j] += f;
                 else f = 0.0f;
-                z[j] = static_cast<T>(f);
+                z[j] = static_cast<T>(f);                      // (the products' operands: rounded once; the column sums are not)
             }
             const Chunk c = __builtin_bit_cast(Chunk, z);
             *reinterpret_cast<Chunk*>(das + buffer * s.a_bytes + (r * s.pa) * 16 + col / V * 16) = c;

@@ -7,8 +7,8 @@
 // columns and each ends up with the 4 k of one column), so no operand is ever transposed in memory.
 //
 // B is the first operand of the matrix instruction and A the second: of the 32 x 32 block a lane then holds 16 values of
-// one output row m, and with B's rows taken in the order of `column_of` they are 16 consecutive n: epilogue loads and stores
-// are whole vectors without a pass through LDS.
+// one output row m, and with B's rows taken in the order of `column_of` they are 16 consecutive n. They leave as whole runs of a row, turned
+// through LDS (store_blocks); the narrow backward stores a lane's 16 values as they are.
 #pragma once
 
 #include "activation.hpp"
@@ -303,7 +303,8 @@ __device__ __forceinline__ void finish_tail(const Tail<T>& t, float (&z)[LEN], i
     S d[LEN];
     const bool keep = t.slope != nullptr;
     // (asked here and not element by element: those branches kept the elements' instructions from overlapping:
-    // 895560 x 32 -> 88 with gelu and a kept slope 190 us, 172 without them; 48552 x 208 -> 456 float 158 and 144)
+    // 895560 x 32 -> 88 with gelu and a kept slope 190 us, 172 without them, 175 with gelu's tail and small slopes kept; 48552 x 208 -> 456
+    // float 158 and 144)
     if (keep) {
         if (t.activation == kActSilu) finish<T, kActSilu, true>(z, v, d);
         else finish<T, kActGelu, true>(z, v, d);

@@ -87,9 +87,10 @@ __device__ __forceinline__ void settle() { asm volatile("s_waitcnt vmcnt(%0) lgk
 // of its last k step, whose fragments are in registers by then: from there on its LDS takes the stage after next, whose loads are
 // issued one at a time between the products of two k steps (eight waves that issue theirs all at once keep the memory pipe,
 // and with it themselves, busy for half a stage), and the next stage's first fragments are read between the last products.
-// Bound by the matrix instructions and the power they draw: 8192 x 2048 -> 4096 bfloat16 115 to 120 us, 1.17 PFLOP/s, where a library
-// product takes 95 to 100 (both 20 % faster on zeros), 131 with gelu and bias; 8192 x 4096 -> 2048 108 us, dx 111 to 122 against 102 to 115,
-// dW 129 to 136 against 126 to 133. No better: four stages of 64 bytes of k, waves of 128 x 128 (they spill), wave priorities.
+// Bound by the matrix instructions and the power they draw. Each repeated alone, bfloat16: 8192 x 2048 -> 4096 119 us (1.16 PFLOP/s), 133 with gelu and
+// bias, where a library product takes 98 to 112; 8192 x 4096 -> 2048 109 us, dx 118, dW 136 against 90 to 100, 113 to 129 and 128 to 147. One after
+// the other in a training step the clock is lower: y with silu, a residual and a kept slope 146 us, dx 133, dW 164. (On zeros everything is
+// 20 % faster.) No better: four stages of 64 bytes of k, waves of 128 x 128 (they spill), wave priorities.
 template <class T, bool A_K, bool B_K, int TM, int TN, int WM, int WN>
 __global__ void __launch_bounds__(WM * WN * 64)
 product_wide_kernel(Operand<T> a, Operand<T> b, Tail<T> tail, int64_t k_part, unsigned tiles_m, unsigned tiles_n) {
