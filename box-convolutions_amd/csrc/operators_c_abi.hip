@@ -12,7 +12,7 @@ constexpr int64_t kMaxExtent = (int64_t(1) << 31) - 1;
 
 bool known_dtype(int dtype) { return dtype == BOXCONV_F32 || dtype == BOXCONV_F16 || dtype == BOXCONV_BF16; }
 
-int check_norm(int dtype, int param_dtype, int64_t batch, int64_t pixels, int channels, int groups, int activation) {
+int check_norm(int dtype, int param_dtype, int64_t batch, int64_t pixels, int channels, int groups, int activation, bool backward) {
     if (!known_dtype(dtype)) return fail(BOXCONV_E_INVALID_ARGUMENT, "group norm: dtype must be BOXCONV_F32, BOXCONV_F16 or BOXCONV_BF16, got %d", dtype);
     if (param_dtype != BOXCONV_F32 && param_dtype != dtype)
         return fail(BOXCONV_E_INVALID_ARGUMENT, "group norm: param_dtype must be BOXCONV_F32 or that of the input, got %d", param_dtype);
@@ -21,8 +21,9 @@ int check_norm(int dtype, int param_dtype, int64_t batch, int64_t pixels, int ch
                     static_cast<long long>(pixels), channels, groups);
     if (activation < BOXCONV_ACT_NONE || activation > BOXCONV_ACT_GELU)
         return fail(BOXCONV_E_INVALID_ARGUMENT, "group norm: unknown activation %d", activation);
-    // batch items are split over launches where a grid would have 2^32 threads or more; one item has at most a workgroup of 256 per channel
-    if (channels > kMostThreads / 256 || batch > kMaxExtent / channels || pixels > (int64_t(1) << 46) / channels)
+    // batch items are split over launches where a grid would have 2^32 threads or more; one item has at most a workgroup of 256 per group, in the
+    // backward per channel
+    if ((backward ? channels : groups) > kMostThreads / 256 || batch > kMaxExtent / channels || pixels > (int64_t(1) << 46) / channels)
         return fail(BOXCONV_E_TOO_LARGE, "group norm: batch=%lld items of pixels=%lld x channels=%d are too many", static_cast<long long>(batch),
                     static_cast<long long>(pixels), channels);
     return 0;
@@ -74,14 +75,14 @@ auto with_type(int dtype, F f) {
 extern "C" {
 
 size_t boxconv_group_norm_workspace_bytes(int64_t batch, int64_t pixels, int channels, int groups, int dtype, int backward) {
-    if (check_norm(dtype, BOXCONV_F32, batch, pixels, channels, groups, 0) != 0 || batch == 0 || pixels == 0) return 0;
+    if (check_norm(dtype, BOXCONV_F32, batch, pixels, channels, groups, 0, backward != 0) != 0 || batch == 0 || pixels == 0) return 0;
     return norm_workspace_bytes(batch, pixels, channels, groups, dtype, backward != 0);
 }
 
 int boxconv_group_norm_forward(const void* input, const void* weight, const void* bias, int param_dtype, const void* residual, void* output,
                                float* mean, float* rstd, int dtype, int64_t batch, int64_t pixels, int channels, int groups, float eps,
                                int activation, void* workspace, size_t workspace_bytes, void* stream) {
-    if (const int rc = check_norm(dtype, param_dtype, batch, pixels, channels, groups, activation)) return rc;
+    if (const int rc = check_norm(dtype, param_dtype, batch, pixels, channels, groups, activation, false)) return rc;
     if ((mean == nullptr) != (rstd == nullptr)) return fail(BOXCONV_E_INVALID_ARGUMENT, "group norm: mean and rstd go together");
     if (batch == 0 || pixels == 0) return 0;
     if (input == nullptr || output == nullptr) return fail(BOXCONV_E_INVALID_ARGUMENT, "group norm: null input or output pointer");
@@ -94,7 +95,7 @@ int boxconv_group_norm_backward(const void* input, const void* weight, const voi
                                 const void* grad_output, const float* mean, const float* rstd, void* grad_input, void* grad_weight, void* grad_bias,
                                 void* grad_residual, int dtype, int64_t batch, int64_t pixels, int channels, int groups, int activation, void* workspace,
                                 size_t workspace_bytes, void* stream) {
-    if (const int rc = check_norm(dtype, param_dtype, batch, pixels, channels, groups, activation)) return rc;
+    if (const int rc = check_norm(dtype, param_dtype, batch, pixels, channels, groups, activation, true)) return rc;
     if (batch == 0 || pixels == 0) {
         if (const int rc = write_zeros(grad_weight, channels, param_dtype, "group norm", static_cast<hipStream_t>(stream))) return rc;
         return write_zeros(grad_bias, channels, param_dtype, "group norm", static_cast<hipStream_t>(stream));

@@ -424,3 +424,15 @@ def test_nothing_to_sum_at_the_c_entry(hip):
         assert lib.boxconv_group_norm_backward(None, None, None, 0, None, None, None, None, None, gw.data_ptr(), gb.data_ptr(), None, 1, batch, pixels, 8, 2,
                                                0, None, 0, stream) == 0
         assert not gw.any() and not gb.any()
+
+
+def test_most_channels(hip):
+    """More channels than the backward takes, in the forward: one item of 2^24 + 3 channels in one group."""
+    from box_convolution import group_norm_act
+    x = torch.randn(2, (1 << 24) + 3, generator=torch.Generator(device="cuda").manual_seed(0), device="cuda")
+    y = group_norm_act(x, 1)
+    d = x.double()
+    d = (d - d.mean(1, keepdim=True)) / (d.var(1, unbiased=False, keepdim=True) + EPS).sqrt()
+    assert (y - d).abs().max() <= ref.DEPTH * ref.U32 * x.abs().max()
+    with pytest.raises(RuntimeError, match="too many"):
+        group_norm_act(x.requires_grad_(True), 1).sum().backward()

@@ -141,8 +141,10 @@ def test_scratch_of_calls_that_overlap(monkeypatch, call):
 def test_sizes_that_no_launch_takes(lib):
     """A grid has fewer than 2^32 threads: one item's or one row of tiles' workgroups have to fit, and are refused where they do not."""
     most = (1 << 24) - 1
-    assert norm(lib, batch=1, pixels=1, channels=most + 1, groups=1) == -3 and b"too many" in lib.boxconv_last_error()
-    assert norm(lib, batch=1, pixels=1, channels=most, groups=1) == -2               # (a workspace is all that is missing)
+    assert norm(lib, batch=1, pixels=1, channels=most + 1, groups=most + 1) == -3 and b"too many" in lib.boxconv_last_error()
+    assert norm(lib, batch=1, pixels=1, channels=most + 1, groups=1) == -2           # (a workspace is all that is missing)
+    for channels, code in ((most, -2), (most + 1, -3)):
+        assert lib.boxconv_group_norm_backward(P, P, P, 0, None, P, P, P, P, None, None, None, 0, 1, 1, channels, 1, 0, None, 0, None) == code
     back = lib.boxconv_linear_backward
     for K, code in ((64 * most, -2), (64 * most + 1, -3)):
         assert back(P, K, P, P, None, P, None, None, None, 1, 100, K, 1, 0, None, 0, None) == code, K
