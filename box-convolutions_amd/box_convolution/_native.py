@@ -16,7 +16,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_NAME = "libboxconv_hip.so"
 LIB_PATH = os.path.join(_HERE, LIB_NAME)
 
-ABI_VERSION = 4
+ABI_VERSION = 5
 
 _lib = None
 
@@ -62,11 +62,19 @@ _SIGNATURES["boxconv_group_norm_forward"] = (
     _i, [_vp] * 3 + [_i] + [_vp] * 4 + [_i, _i64, _i64, _i, _i, _f, _i, _vp, _sz, _vp])
 _SIGNATURES["boxconv_group_norm_backward"] = (
     _i, [_vp] * 3 + [_i] + [_vp] * 8 + [_i, _i64, _i64, _i, _i, _i, _vp, _sz, _vp])
+_RESIDUAL_NORM = [_vp] * 3 + [_i, _i, _f, _i] + [_vp] * 4 + [_i, _f]
+_SIGNATURES["boxconv_residual_norm_forward"] = (_i, _RESIDUAL_NORM + [_vp] * 3 + [_i, _i64, _i64, _i, _vp])
+_SIGNATURES["boxconv_residual_norm_workspace_bytes"] = (_sz, [_i64, _i64, _i, _i, _i])
+_SIGNATURES["boxconv_residual_norm_backward"] = (_i, _RESIDUAL_NORM + [_vp] * 9 + [_i, _i64, _i64, _i, _vp, _sz, _vp])
 _SIGNATURES["boxconv_linear_workspace_bytes"] = (_sz, [_i64, _i64, _i64, _i, _i])
 _SIGNATURES["boxconv_linear_forward"] = (
     _i, [_vp, _i64, _vp, _vp, _vp, _i64, _vp, _vp, _i, _i64, _i64, _i64, _i, _vp, _sz, _vp])
 _SIGNATURES["boxconv_linear_backward"] = (
     _i, [_vp, _i64] + [_vp] * 7 + [_i, _i64, _i64, _i64, _i, _vp, _sz, _vp])
+_SIGNATURES["boxconv_quantize_blocks"] = (_i, [_vp, _i64, _i, _i64, _i64, _vp, _vp, _vp])
+_SIGNATURES["boxconv_linear_float8_workspace_bytes"] = (_sz, [_i64, _i64, _i64, _i, _i])
+_SIGNATURES["boxconv_linear_float8_forward"] = (
+    _i, [_vp, _i64, _i, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _i, _i64, _i64, _i64, _i, _vp, _sz, _vp])
 
 EXPORTED_SYMBOLS = tuple(sorted(_SIGNATURES))
 
@@ -744,6 +752,53 @@ def group_norm_backward(input, num_groups, weight, bias, residual, activation, m
     return grads
 
 
+# flags BOXCONV_NORM_* and gate kinds BOXCONV_GATE_* (include/boxconv.h)
+NORM_AFTER, NORM_BEFORE, NORM_CENTRE = 1, 2, 4
+GATE_NONE, GATE_CHANNEL, GATE_ITEM, GATE_FULL = 0, 1, 2, 3
+
+
+def _residual_norm_arguments(input, residual, gate, gate_kind, scale, norms, params, eps):
+    """The arguments that boxconv_residual_norm_forward and _backward begin with, and (dtype, batch, pixels, channels)."""
+    dtype = _FUSED_OUTPUT[input.dtype]
+    kind = next((p.dtype for p in params if p is not None), torch.float32)
+    begin = [_ptr(input), _ptr(residual), _ptr(gate), gate_kind, dtype if gate is None else _FUSED_OUTPUT[gate.dtype], scale, norms,
+             *[_ptr(p) for p in params], _FUSED_OUTPUT[kind], eps]
+    B, C = input.size(0), input.size(-1)
+    return begin, (dtype, B, input.numel() // (B * C) if B * C else 0, C)
+
+
+def residual_norm_forward(input, residual, gate, gate_kind, scale, norms, params, eps, want_stream, blocks=None):
+    """What lies between two residual blocks, of contiguous ``[B, ..., C]`` tensors (include/boxconv.h,
+    boxconv_residual_norm_forward). ``params``: weight and bias of the norm after and of the norm before. ``blocks``: (codes, exponents)
+    that receive the normed rows in 8 bits. Returns ``(stream, normed)``, ``None`` for what is not formed."""
+    stream = torch.empty_like(input) if want_stream else None
+    normed = torch.empty_like(input) if norms & NORM_BEFORE and blocks is None else None
+    if input.numel() > 0:
+        begin, sizes = _residual_norm_arguments(input, residual, gate, gate_kind, scale, norms, params, eps)
+        to = (_ptr(normed), None) if blocks is None else (_ptr(blocks[0]), _ptr(blocks[1]))
+        with _on_device(input.device):
+            rc = load().boxconv_residual_norm_forward(*begin, _ptr(stream), *to, *sizes, _stream(input.device))
+        _check(rc, "residual_norm")
+    return stream, normed
+
+
+def residual_norm_backward(input, residual, gate, gate_kind, scale, norms, params, eps, grad_stream, grad_normed, needs):
+    """Gradients of ``residual_norm_forward``, all tensors contiguous ``[B, ..., C]``. ``needs``: whether input, residual, gate and the four
+    parameters need theirs; returns the seven, ``None`` where not."""
+    grads = [torch.empty_like(t) if need else None for t, need in zip((input, residual, gate, *params), needs)]
+    if input.numel() == 0:
+        return [None if g is None else g.zero_() for g in grads]
+    begin, sizes = _residual_norm_arguments(input, residual, gate, gate_kind, scale, norms, params, eps)
+    with _on_device(input.device):
+        nbytes = _operator_workspace_bytes("boxconv_residual_norm_workspace_bytes", *sizes[1:], gate_kind, sizes[0])
+        stream = _stream(input.device)
+        ws = _scratch(nbytes, input.device)
+        rc = load().boxconv_residual_norm_backward(*begin, _ptr(grad_stream), _ptr(grad_normed), *[_ptr(g) for g in grads], *sizes,
+                                                   _ptr(ws), nbytes, stream)
+    _check(rc, "residual_norm backward")
+    return grads
+
+
 def linear_forward(input, weight, bias, residual, activation, keep_slope):
     """``act(input @ weight.T + bias + residual)`` of a ``[rows, K]`` tensor with contiguous rows
     (include/boxconv.h, boxconv_linear_forward). Returns ``(output, kept)``: what the backward
@@ -766,6 +821,49 @@ def linear_forward(input, weight, bias, residual, activation, keep_slope):
                 _ptr(ws), nbytes, stream)
         _check(rc, "linear")
     return output, slope if act >= 2 else output if keep_slope and act == 1 else None
+
+
+BLOCK = 128           # columns that share a power of two
+_E4M3 = 8             # BOXCONV_E4M3
+
+
+def block_sizes(columns):
+    """(codes, exponents) of a row of `columns` values in 8 bits (include/boxconv.h, boxconv_quantize_blocks)."""
+    blocks = -(-columns // BLOCK)
+    return blocks * BLOCK, -(-blocks // 4) * 4
+
+
+def quantize_blocks(input):
+    """(codes, exponents) of a ``[rows, K]`` tensor with contiguous rows."""
+    rows, K = input.shape
+    codes, exponents = block_sizes(K)
+    codes = torch.empty((rows, codes), dtype=torch.float8_e4m3fn, device=input.device)
+    exponents = torch.empty((rows, exponents), dtype=torch.uint8, device=input.device)
+    if codes.numel() > 0:
+        with _on_device(input.device):
+            rc = load().boxconv_quantize_blocks(_ptr(input), input.stride(0), _FUSED_OUTPUT[input.dtype], rows, K, _ptr(codes),
+                                                _ptr(exponents), _stream(input.device))
+        _check(rc, "quantize_blocks")
+    return codes, exponents
+
+
+def linear_float8_forward(input, exponents, weight, weight_exponents, K, bias, residual, activation, dtype):
+    """``act(input @ weight.T + bias + residual)`` of 8-bit rows (include/boxconv.h, boxconv_linear_float8_forward). ``input``:
+    ``[rows, K]`` values with contiguous rows (``exponents`` ``None``), or codes."""
+    rows, N = input.size(0), weight.size(0)
+    output = torch.empty((rows, N), dtype=dtype, device=input.device)
+    if output.numel() > 0:
+        code, act = _FUSED_OUTPUT[dtype], ACTIVATIONS[activation]
+        given = code if exponents is None else _E4M3
+        with _on_device(input.device):
+            nbytes = _operator_workspace_bytes("boxconv_linear_float8_workspace_bytes", rows, K, N, given, code)
+            stream = _stream(input.device)
+            ws = _scratch(nbytes, input.device)
+            rc = load().boxconv_linear_float8_forward(
+                _ptr(input), input.stride(0), given, _ptr(exponents), _ptr(weight), _ptr(weight_exponents), _ptr(bias), _ptr(residual),
+                0 if residual is None else residual.stride(0), _ptr(output), code, rows, K, N, act, _ptr(ws), nbytes, stream)
+        _check(rc, "linear_float8")
+    return output
 
 
 def linear_backward(input, weight, kept, activation, grad_output, needs):
@@ -800,7 +898,8 @@ KERNEL_NAMES = ("band_colsum", "band_prefix", "band_scan", "forward_rows", "forw
                 "forward_gather", "grad_input_gather", "grad_params_gather", "int_row_prefix",
                 "int_col_prefix", "norm_statistics", "norm_join", "norm_apply", "norm_small", "norm_any_statistics", "norm_any_apply", "norm_sums",
                 "norm_join_sums", "norm_grad", "norm_small_grad", "norm_parameter", "norm_any_sums", "norm_any_grad", "linear", "linear_few_rows",
-                "linear_dx", "linear_dweight", "linear_narrow_grad", "linear_slope", "join_parts", "join_bias")
+                "linear_dx", "linear_dweight", "linear_narrow_grad", "linear_slope", "join_parts", "join_bias", "norm_rows", "norm_rows_grad", "join_rows",
+                "quantize", "linear_float8")
 
 
 def reload_switches():

@@ -1,6 +1,8 @@
 """What a network puts around a box convolution: the pointwise product (1 x 1 convolution, linear layer) with bias,
-residual and activation in its epilogue, and group norm with a residual and an activation. Both work on channels-last
-data in float32, float16 or bfloat16, with gradients; sums and statistics are float32.
+residual and activation in its epilogue, group norm with a residual and an activation, and what lies between two residual
+blocks (a norm after the one, gate, residual add, a norm before the other). All work on channels-last data in float32, float16
+or bfloat16, with gradients; sums and statistics are float32. For inference the product also comes in 8-bit floating point,
+in blocks of 128 with a power of two each.
 
 (The reference builds such a block from torch's own layers: BottleneckBoxConv,
 examples/Cityscapes/models/ENet.py:282-304.)
@@ -27,7 +29,7 @@ class _OnceFunction(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad_output):
-        raise RuntimeError("box_convolution: group_norm_act and linear_act can be differentiated once, not twice")
+        raise RuntimeError("box_convolution: group_norm_act, linear_act and residual_norm can be differentiated once, not twice")
 
 
 def _once(grads, x, grad_output):
@@ -44,7 +46,7 @@ def _refuse_tangents(*tensors):
     it would make it zero."""
     for t in tensors:
         if t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
-            raise RuntimeError("box_convolution: group_norm_act and linear_act have no forward-mode derivative")
+            raise RuntimeError("box_convolution: group_norm_act, linear_act and residual_norm have no forward-mode derivative")
 
 
 def _contiguous(*tensors):
@@ -173,6 +175,225 @@ def linear_act(input, weight, bias=None, residual=None, activation=None):
     return y.view(out_shape)
 
 
+class ResidualNormFunction(torch.autograd.Function):
+    """``apply(input, residual, gate, after_weight, after_bias, before_weight, before_bias, gate_kind, scale, norms, eps, want_stream)``,
+    tensors ``[B, ..., C]`` and parameters contiguous. Returns the stream (unless it is the input itself) and, with a norm
+    before, the normed rows."""
+
+    @staticmethod
+    def forward(ctx, input, residual, gate, after_weight, after_bias, before_weight, before_bias, gate_kind, scale, norms, eps, want_stream):
+        params = (after_weight, after_bias, before_weight, before_bias)
+        outputs = _native.residual_norm_forward(input, residual, gate, gate_kind, scale, norms, params, eps, want_stream)
+        ctx.save_for_backward(input, residual, gate, *params)
+        ctx.rest = gate_kind, scale, norms
+        ctx.eps, ctx.want_stream = eps, want_stream
+        ctx.set_materialize_grads(False)
+        outputs = tuple(t for t in outputs if t is not None)
+        return outputs if len(outputs) > 1 else outputs[0]
+
+    @staticmethod
+    def backward(ctx, *grad_outputs):
+        given = [None if g is None else g.contiguous() for g in grad_outputs]
+        _refuse_tangents(*grad_outputs)
+        grad_stream = given.pop(0) if ctx.want_stream else None
+        grad_normed = given.pop(0) if given else None
+        input, residual, gate, *params = _contiguous(*ctx.saved_tensors)
+        gate_kind, scale, norms = ctx.rest
+        needs = [n and t is not None for n, t in zip(ctx.needs_input_grad, (input, residual, gate, *params))]
+        grads = _native.residual_norm_backward(input, residual, gate, gate_kind, scale, norms, params, ctx.eps, grad_stream, grad_normed, needs)
+        like = next((g for g in grad_outputs if g is not None), input)
+        return (*_once(grads, input, like), None, None, None, None, None)
+
+
+def _gate_kind(gate, input):
+    if gate is None:
+        return _native.GATE_NONE
+    B, C = input.size(0), input.size(1)
+    for kind, shape in ((_native.GATE_FULL, tuple(input.shape)), (_native.GATE_CHANNEL, (C,)), (_native.GATE_ITEM, (B, C))):
+        if tuple(gate.shape) == shape:
+            if gate.device != input.device or gate.dtype not in ((input.dtype,) if kind == _native.GATE_FULL else (input.dtype, torch.float32)):
+                raise RuntimeError("box_convolution: gate must be on %s, of the input's type or, where it has one value per channel, float32" % input.device)
+            return kind
+    raise RuntimeError("box_convolution: gate must have the shape [C], [B, C] or that of the input, got %s for an input of %s"
+                       % (tuple(gate.shape), tuple(input.shape)))
+
+
+def _norm_pairs(input, after, before):
+    """The four parameters, contiguous, of norms given as None or (weight, bias)."""
+    out, kind = [], None
+    for name, pair in (("after", after), ("before", before)):
+        if pair is not None and (not isinstance(pair, (tuple, list)) or len(pair) != 2):
+            raise RuntimeError("box_convolution: %s must be None or a pair (weight, bias), either of which may be None" % name)
+        for p in pair or (None, None):
+            if p is not None:
+                if p.device != input.device or p.dim() != 1 or p.size(0) != input.size(1):
+                    raise RuntimeError("box_convolution: the parameters of a norm must hold %d values on %s" % (input.size(1), input.device))
+                if p.dtype not in (torch.float32, input.dtype) or kind not in (None, p.dtype):
+                    raise RuntimeError("box_convolution: the norms' parameters must all be float32 or all of the input's type")
+                kind = p.dtype
+                p = p.contiguous()
+            out.append(p)
+    return out
+
+
+def residual_norm(input, residual=None, gate=None, scale=1.0, after=None, before=None, kind="rms", eps=1e-6, quantize=False):
+    """What lies between two blocks of a residual network, with gradients: ``input`` is what a block gives, ``residual`` the stream it
+    is added to:
+
+        ``stream = residual + scale * gate * norm(input; after)``,  ``normed = norm(stream; before)``.
+
+    Returns ``(stream, normed)``, or the stream alone where there is no norm before the next block.
+
+    input:    ``[B, C, ...]``; channels-last memory is used as it is, anything else is copied once. The results have channels-last memory.
+    residual: same shape and type, or ``None`` for 0.
+    gate:     ``None`` for 1, ``[C]`` (a layer scale), ``[B, C]`` (a gate per batch item) or of the input's shape; of the input's type, or
+              float32 where it has one value per channel.
+    after, before: the norms behind this block and before the next one: ``None`` where there is none, or ``(weight, bias)``,
+              each ``[C]`` or ``None`` for 1 and 0, all float32 or all of the input's type.
+    kind:     ``"rms"``: ``v / sqrt(mean(v * v) + eps)`` over a row's channels; ``"layer"``: the same of ``v - mean(v)``.
+    quantize: the normed rows as ``Float8Blocks``, for ``linear_act_float8`` (inference only: nothing here may require a gradient).
+
+    Where nothing is done to the input (no residual, gate or norm behind the block, scale 1), the stream is the input itself.
+    Statistics and sums are float32; ``normed`` is formed from the stream before it is rounded to the input's type.
+    """
+    _native._require_device(input, "residual norm input")
+    _native._operator_dtype(input, "residual norm input")
+    if kind not in ("rms", "layer"):
+        raise RuntimeError("box_convolution: kind must be 'rms' or 'layer', got %r" % (kind,))
+    if input.dim() < 2 or input.size(1) < 1:
+        raise RuntimeError("box_convolution: residual norm input must have >=2 dimensions and a channel")
+    gate_kind = _gate_kind(gate, input)
+    params = _norm_pairs(input, after, before)
+    if residual is not None:
+        _native._same_as(residual, input, "residual")
+    tensors = (input, residual, gate, *params)
+    _refuse_tangents(*tensors)
+    norms = (_native.NORM_AFTER * (after is not None) | _native.NORM_BEFORE * (before is not None) | _native.NORM_CENTRE * (kind == "layer"))
+    scale, eps = float(scale), float(eps)
+    same = residual is None and gate is None and after is None and scale == 1.0
+    recorded = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if quantize and (before is None or recorded):
+        raise RuntimeError("box_convolution: quantize needs a norm before the next block, and is for inference only")
+    if same and before is None:
+        return input
+    x = _channels_last(input)
+    r = None if residual is None else _channels_last(residual)
+    g = None if gate is None else _channels_last(gate) if gate_kind == _native.GATE_FULL else gate.contiguous()
+    if recorded:
+        outputs = ResidualNormFunction.apply(x, r, g, *params, gate_kind, scale, norms, eps, not same)
+        outputs = list(outputs) if isinstance(outputs, tuple) else [outputs]
+        stream, normed = None if same else outputs.pop(0), outputs.pop(0) if outputs else None
+    else:
+        blocks = None
+        if quantize:
+            codes, exponents = _native.block_sizes(x.size(-1))
+            blocks = (torch.empty((*x.shape[:-1], codes), dtype=torch.float8_e4m3fn, device=x.device),
+                      torch.empty((*x.shape[:-1], exponents), dtype=torch.uint8, device=x.device))
+        stream, normed = _native.residual_norm_forward(x, r, g, gate_kind, scale, norms, params, eps, not same, blocks)
+        if quantize:
+            normed = Float8Blocks(*blocks, x.size(-1))
+    stream = input if same else stream.movedim(-1, 1)
+    if before is None:
+        return stream
+    return stream, normed if quantize else normed.movedim(-1, 1)
+
+
+class Float8Blocks:
+    """Rows ``[..., columns]`` in 8-bit floating point (e4m3), a power of two for each block of 128 columns: value =
+    ``codes * 2**(exponents - 127)``. ``codes``: ``[..., columns rounded up to 128]`` float8_e4m3fn, zeros beyond the columns;
+    ``exponents``: ``[..., blocks rounded up to 4]`` uint8, from 1 to 254, 127 beyond the blocks. Both contiguous, on one device."""
+
+    __slots__ = ("codes", "exponents", "columns")
+
+    def __init__(self, codes, exponents, columns):
+        width, words = _native.block_sizes(columns)
+        if (codes.dtype != torch.float8_e4m3fn or exponents.dtype != torch.uint8 or codes.device != exponents.device or columns < 1
+                or codes.dim() < 1 or codes.size(-1) != width or tuple(exponents.shape) != (*codes.shape[:-1], words)):
+            raise RuntimeError("box_convolution: Float8Blocks needs float8_e4m3fn codes [..., %d] and uint8 exponents [..., %d] on one device for %d "
+                               "columns, got %s %s and %s %s" % (width, words, columns, codes.dtype, tuple(codes.shape), exponents.dtype, tuple(exponents.shape)))
+        if not codes.is_contiguous() or not exponents.is_contiguous() or codes.data_ptr() % 16 or exponents.data_ptr() % 4:
+            raise RuntimeError("box_convolution: the codes and exponents of Float8Blocks must be contiguous, at addresses of whole 16 and 4 bytes")
+        self.codes, self.exponents, self.columns = codes, exponents, columns
+
+    @property
+    def shape(self):
+        return torch.Size((*self.codes.shape[:-1], self.columns))
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    def to(self, device):
+        return Float8Blocks(self.codes.to(device), self.exponents.to(device), self.columns)
+
+    def dequantize(self, dtype=torch.float32):
+        """The values, ``[..., columns]`` (elementary torch operations: to look at, not for a fast path)."""
+        blocks = self.codes.float().unflatten(-1, (-1, _native.BLOCK))
+        # 2**(exponent - 127), put together from its bits
+        power = (self.exponents[..., :blocks.size(-2)].int() << 23).view(torch.float32)
+        return (blocks * power[..., None]).flatten(-2)[..., :self.columns].to(dtype)
+
+
+def quantize_blocks(input):
+    """``[..., K]`` values in float32, float16 or bfloat16 as ``Float8Blocks``: per block of 128 the least power of two (from 2**-126 on) that
+    keeps its largest finite magnitude at or below 448 times it; values rounded to nearest, ties to even, once. NaN and infinities
+    become NaN and leave the rest of their block alone. Not differentiable: an input that requires a gradient is refused while
+    gradients are recorded."""
+    _native._require_device(input, "quantize input")
+    _native._operator_dtype(input, "quantize input")
+    if input.dim() < 1 or input.size(-1) < 1:
+        raise RuntimeError("box_convolution: quantize_blocks needs an input [..., K] with at least one column")
+    _refuse_gradients("quantize_blocks", input)
+    codes, exponents = _native.quantize_blocks(_rows(input, math.prod(input.shape[:-1]), input.size(-1)))
+    return Float8Blocks(codes.view(*input.shape[:-1], codes.size(-1)), exponents.view(*input.shape[:-1], exponents.size(-1)), input.size(-1))
+
+
+def _refuse_gradients(what, *tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError("box_convolution: %s is for inference only: it has no gradient (call it under torch.no_grad())" % what)
+    _refuse_tangents(*tensors)
+
+
+def linear_act_float8(input, weight, bias=None, residual=None, activation=None, dtype=None):
+    """``act(input @ weight.T + bias + residual)`` of 8-bit rows, for inference: see ``linear_act`` for training.
+
+    input:    ``Float8Blocks`` ``[..., K]``, or values ``[..., K]``, which are quantized on the way as by ``quantize_blocks``.
+    weight:   ``Float8Blocks`` ``[N, K]`` (``quantize_blocks(weight)``, once).
+    bias:     ``[N]``; residual ``[..., N]``, added before the activation: both of the result's type.
+    activation: ``None``, ``"relu"``, ``"silu"`` or ``"gelu"``.
+    dtype:    the result's type: that of the values; for ``Float8Blocks`` float32, float16 or bfloat16 (default).
+
+    Products of codes and powers of two are exact, sums are float32.
+    """
+    _native._activation(activation)
+    coded = isinstance(input, Float8Blocks)
+    rows_of = input.codes if coded else input
+    _native._require_device(rows_of, "linear float8 input")
+    if not coded:
+        _native._operator_dtype(input, "linear float8 input")
+    dtype = dtype or (torch.bfloat16 if coded else input.dtype)
+    if dtype not in _native._FUSED_OUTPUT or (not coded and dtype != input.dtype):
+        raise RuntimeError("box_convolution: the result's type must be that of the values, or float32, float16 or bfloat16 for Float8Blocks, got %s" % dtype)
+    if not isinstance(weight, Float8Blocks):
+        raise RuntimeError("box_convolution: weight must be Float8Blocks (quantize_blocks(weight)), got %s" % type(weight).__name__)
+    if len(input.shape) < 1 or len(weight.shape) != 2 or weight.columns != input.shape[-1] or weight.device != rows_of.device:
+        raise RuntimeError("box_convolution: linear float8 needs an input [..., K] and a weight [N, K] on one device, got %s and %s"
+                           % (tuple(input.shape), tuple(weight.shape)))
+    N, K = weight.shape
+    out_shape = (*input.shape[:-1], N)
+    for name, t, shape in (("bias", bias, (N,)), ("residual", residual, out_shape)):
+        if t is not None and (t.device != rows_of.device or t.dtype != dtype or tuple(t.shape) != shape):
+            raise RuntimeError("box_convolution: %s must have the shape %s, type %s and device %s, got %s, %s, %s"
+                               % (name, shape, dtype, rows_of.device, tuple(t.shape), t.dtype, t.device))
+    _refuse_gradients("linear_act_float8", None if coded else input, bias, residual)
+    rows = math.prod(out_shape[:-1])
+    x = input.codes.view(rows, weight.codes.size(-1)) if coded else _rows(input, rows, K)
+    exponents = input.exponents.view(rows, weight.exponents.size(-1)) if coded else None
+    y = _native.linear_float8_forward(x, exponents, weight.codes, weight.exponents, K,
+                                      None if bias is None else bias.contiguous(), None if residual is None else _rows(residual, rows, N), activation, dtype)
+    return y.view(out_shape)
+
+
 class GroupNormAct(torch.nn.GroupNorm):
     """``torch.nn.GroupNorm`` (same arguments and parameters, so state dicts interchange) followed by a residual add
     and an activation in the same kernels: ``module(x, residual=None)``. See ``group_norm_act``."""
@@ -208,3 +429,67 @@ class PointwiseConv2d(torch.nn.Conv2d):
 
     def extra_repr(self):
         return super().extra_repr() + ", activation=%r" % (self.activation,)
+
+
+class ResidualNorm(torch.nn.Module):
+    """``residual_norm`` with its parameters: ``module(x, residual=None, gate=None)`` for ``[B, channels, ...]``.
+
+    after, before: whether there is a norm behind the block and one before the next; ``kind`` "rms" (weights) or "layer" (weights and
+    biases). layer_scale: the initial value of a learned gate per channel, ``None`` for none; it excludes a gate in the call.
+    Parameters may be float32 beside inputs in half precision."""
+
+    def __init__(self, channels, after=True, before=True, kind="rms", scale=1.0, layer_scale=None, eps=1e-6, device=None, dtype=None):
+        super().__init__()
+        if kind not in ("rms", "layer"):
+            raise RuntimeError("box_convolution: kind must be 'rms' or 'layer', got %r" % (kind,))
+        self.channels, self.kind, self.scale, self.eps = channels, kind, scale, eps
+
+        def parameter(value):
+            return torch.nn.Parameter(torch.full((channels,), float(value), device=device, dtype=dtype))
+        for name, there in (("after", after), ("before", before)):
+            setattr(self, name, there)
+            self.register_parameter(name + "_weight", parameter(1) if there else None)
+            self.register_parameter(name + "_bias", parameter(0) if there and kind == "layer" else None)
+        self.register_parameter("layer_scale", None if layer_scale is None else parameter(layer_scale))
+
+    def forward(self, input, residual=None, gate=None, quantize=False):
+        if gate is not None and self.layer_scale is not None:
+            raise RuntimeError("ResidualNorm: a gate and a layer scale exclude each other")
+        return residual_norm(input, residual, self.layer_scale if gate is None else gate, self.scale,
+                             (self.after_weight, self.after_bias) if self.after else None,
+                             (self.before_weight, self.before_bias) if self.before else None, self.kind, self.eps, quantize)
+
+    def extra_repr(self):
+        return "%d, after=%r, before=%r, kind=%r, scale=%r, eps=%r" % (self.channels, self.after, self.before, self.kind, self.scale, self.eps)
+
+
+class PointwiseConv2dFloat8(torch.nn.Module):
+    """The inference form of a ``PointwiseConv2d`` (or 1 x 1 ``torch.nn.Conv2d``) in 8 bits: ``PointwiseConv2dFloat8(conv)`` quantizes its
+    weight once; ``module(x, residual=None)`` takes ``[B, C, h, w]`` values of the bias's type, or the ``Float8Blocks`` ``[B, h, w, C]``
+    of a quantizing ``ResidualNorm``, and returns ``[B, out_channels, h, w]`` in channels-last memory. Codes, exponents and bias
+    are buffers."""
+
+    def __init__(self, conv, activation=None):
+        super().__init__()
+        if (not isinstance(conv, torch.nn.Conv2d) or conv.kernel_size != (1, 1) or conv.stride != (1, 1) or conv.padding not in ((0, 0), "valid")
+                or conv.groups != 1):
+            raise RuntimeError("PointwiseConv2dFloat8: needs a 1 x 1 convolution without stride, padding and groups")
+        _native._activation(activation)
+        self.activation = activation or getattr(conv, "activation", None)
+        self.in_channels, self.out_channels, self.dtype = conv.in_channels, conv.out_channels, conv.weight.dtype
+        with torch.no_grad():
+            weight = quantize_blocks(conv.weight.flatten(1))
+        self.register_buffer("codes", weight.codes)
+        self.register_buffer("exponents", weight.exponents)
+        self.register_buffer("bias", None if conv.bias is None else conv.bias.detach().clone())
+
+    def forward(self, input, residual=None):
+        coded = isinstance(input, Float8Blocks)
+        if len(input.shape) != 4:
+            raise RuntimeError("PointwiseConv2dFloat8: input must have 4 dimensions")
+        y = linear_act_float8(input if coded else input.permute(0, 2, 3, 1), Float8Blocks(self.codes, self.exponents, self.in_channels), self.bias,
+                              None if residual is None else residual.permute(0, 2, 3, 1), self.activation, self.dtype if coded else None)
+        return y.permute(0, 3, 1, 2)
+
+    def extra_repr(self):
+        return "%d, %d, bias=%r, activation=%r" % (self.in_channels, self.out_channels, self.bias is not None, self.activation)

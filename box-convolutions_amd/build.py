@@ -40,15 +40,17 @@ def _inst(tag, t, tg, part, same):
 
 SOURCES = [(s, s.replace(".hip", ".o"), []) for s in
            ("box_sampling.hip", "integral_image.hip", "integral_image_int.hip", "box_misc.hip",
-            "boxconv_c_abi.hip", "operators_c_abi.hip", "group_norm.hip")]
+            "boxconv_c_abi.hip", "operators_c_abi.hip", "group_norm.hip", "float8_quantize.hip")]
 for _tag, _t, _tg in (("f32", "float", "float"), ("f64", "double", "double"),
                       ("f16", "float", "f16_t"), ("bf16", "float", "bf16_t")):
     for _part in (1, 2, 9) + ((3, 4, 5, 6, 7, 8) if _t == "float" else ()):
         SOURCES.append(_inst(_tag, _t, _tg, _part, _t == _tg))
 for _tag, _t in (("f32", "float"), ("f16", "_Float16"), ("bf16", "__bf16")):
     SOURCES.append(("linear.hip", "linear_%s.o" % _tag, ["-DBOXCONV_INST_T=" + _t]))
-OPERATOR_HEADERS = ["activation.hpp", "operators_host.hpp", "linear_tile.hpp", "linear_wide.hpp", "linear_narrow.hpp"]     # only included by the sources below
-OPERATOR_SOURCES = ("operators_c_abi.hip", "group_norm.hip", "linear.hip")
+    SOURCES.append(("residual_norm.hip", "residual_norm_%s.o" % _tag, ["-DBOXCONV_INST_T=" + _t]))
+OPERATOR_HEADERS = ["activation.hpp", "operators_host.hpp", "linear_tile.hpp", "linear_wide.hpp", "linear_narrow.hpp", "float8_blocks.hpp",
+                    "linear_float8.hpp", "residual_norm.hpp"]     # only included by the sources below
+OPERATOR_SOURCES = ("operators_c_abi.hip", "group_norm.hip", "linear.hip", "residual_norm.hip", "float8_quantize.hip")
 HEADERS = ["boxconv_device.hpp", "boxconv_host.hpp", "box_sampling_common.hpp", "box_sampling_impl.hpp", "narrow_rows.hpp", "forward_tail.hpp",
            os.path.join("..", "..", "include", "boxconv.h")]
 

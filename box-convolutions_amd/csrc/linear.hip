@@ -1,5 +1,6 @@
 // The pointwise product y = act(x W^T + bias + residual) and its gradients for one element type (BOXCONV_INST_T: float,
 // _Float16 or __bf16; compiled once for each).
+#include "linear_float8.hpp"
 #include "linear_narrow.hpp"
 
 namespace boxconv {
@@ -640,5 +641,7 @@ template size_t linear_forward_workspace<BOXCONV_INST_T>(int64_t, int64_t, int64
 template size_t linear_backward_workspace<BOXCONV_INST_T>(int64_t, int64_t, int64_t);
 template hipError_t linear_forward<BOXCONV_INST_T>(const LinearCall&, void*, hipStream_t);
 template hipError_t linear_backward<BOXCONV_INST_T>(const LinearGradCall&, void*, hipStream_t);
+template size_t linear_float8_workspace<BOXCONV_INST_T>(int64_t, int64_t, int64_t, bool);
+template hipError_t linear_float8_forward<BOXCONV_INST_T>(const LinearFloat8Call&, void*, hipStream_t);
 
 }  // namespace boxconv

@@ -1,4 +1,4 @@
-// extern "C" entry points of group norm and the pointwise product (declared in include/boxconv.h): argument checks on the
+// extern "C" entry points of group norm, the norms between residual blocks and the pointwise product (declared in include/boxconv.h): argument checks on the
 // host, then the launches. No torch types, no allocation, no synchronisation.
 #include "../../include/boxconv.h"
 #include "boxconv_host.hpp"
@@ -41,6 +41,37 @@ int check_linear(int dtype, int64_t rows, int64_t in_features, int64_t out_featu
         tk * tn > kMaxExtent || out_features > int64_t(256) * 65535)
         return fail(BOXCONV_E_TOO_LARGE, "linear: rows=%lld in_features=%lld out_features=%lld are too large", static_cast<long long>(rows),
                     static_cast<long long>(in_features), static_cast<long long>(out_features));
+    return 0;
+}
+
+// Sizes as the 16-bit product's; in_features of 0 (no blocks) are refused.
+int check_linear_float8(int dtype, int input_dtype, int64_t rows, int64_t in_features, int64_t out_features, int64_t ld_input, int activation) {
+    if (const int rc = check_linear(dtype, rows, in_features, out_features, ld_input, activation)) return rc;
+    if (input_dtype != BOXCONV_E4M3 && input_dtype != dtype)
+        return fail(BOXCONV_E_INVALID_ARGUMENT, "linear float8: input_dtype must be BOXCONV_E4M3 or that of the output, got %d", input_dtype);
+    if (in_features == 0) return fail(BOXCONV_E_INVALID_ARGUMENT, "linear float8: invalid sizes: in_features=0");
+    // a workgroup's tile is addressed in 31 bits: 256 rows of codes
+    if (in_features > (int64_t(1) << 22)) return fail(BOXCONV_E_TOO_LARGE, "linear float8: in_features=%lld are too large", static_cast<long long>(in_features));
+    return 0;
+}
+
+int check_residual_norm(int dtype, int param_dtype, int gate_dtype, int gate_kind, bool gate, int norms, int64_t batch, int64_t pixels, int channels) {
+    if (!known_dtype(dtype)) return fail(BOXCONV_E_INVALID_ARGUMENT, "residual norm: dtype must be BOXCONV_F32, BOXCONV_F16 or BOXCONV_BF16, got %d", dtype);
+    if (param_dtype != BOXCONV_F32 && param_dtype != dtype)
+        return fail(BOXCONV_E_INVALID_ARGUMENT, "residual norm: param_dtype must be BOXCONV_F32 or that of the input, got %d", param_dtype);
+    if (gate_kind < BOXCONV_GATE_NONE || gate_kind > BOXCONV_GATE_FULL) return fail(BOXCONV_E_INVALID_ARGUMENT, "residual norm: unknown gate_kind %d", gate_kind);
+    if (gate != (gate_kind != BOXCONV_GATE_NONE)) return fail(BOXCONV_E_INVALID_ARGUMENT, "residual norm: gate and gate_kind do not agree");
+    if (gate && gate_dtype != dtype && (gate_dtype != BOXCONV_F32 || gate_kind == BOXCONV_GATE_FULL))
+        return fail(BOXCONV_E_INVALID_ARGUMENT, "residual norm: gate_dtype must be that of the input, or BOXCONV_F32 where the gate is no whole tensor, got %d", gate_dtype);
+    if (norms < 0 || norms > (BOXCONV_NORM_AFTER | BOXCONV_NORM_BEFORE | BOXCONV_NORM_CENTRE))
+        return fail(BOXCONV_E_INVALID_ARGUMENT, "residual norm: unknown norms %d", norms);
+    if (batch < 0 || pixels < 0 || channels < 1)
+        return fail(BOXCONV_E_INVALID_ARGUMENT, "residual norm: invalid sizes: batch=%lld pixels=%lld channels=%d", static_cast<long long>(batch),
+                    static_cast<long long>(pixels), channels);
+    // (no tensor's bytes overflow 63 bits; the joining launch has a workgroup of 1024 threads for every 32 channels)
+    if (batch > kMaxExtent || pixels > (int64_t(1) << 46) / channels / std::max<int64_t>(batch, 1) || channels / 32 >= kMostThreads / 1024)
+        return fail(BOXCONV_E_TOO_LARGE, "residual norm: batch=%lld items of pixels=%lld x channels=%d are too many", static_cast<long long>(batch),
+                    static_cast<long long>(pixels), channels);
     return 0;
 }
 
@@ -109,6 +140,65 @@ int boxconv_group_norm_backward(const void* input, const void* weight, const voi
     return hip_result(norm_backward_launch(call, workspace, static_cast<hipStream_t>(stream)), "group norm");
 }
 
+int boxconv_residual_norm_forward(const void* input, const void* residual, const void* gate, int gate_kind, int gate_dtype, float scale, int norms,
+                                  const void* after_weight, const void* after_bias, const void* before_weight, const void* before_bias, int param_dtype,
+                                  float eps, void* stream_output, void* normed, void* normed_exponents, int dtype, int64_t batch, int64_t pixels,
+                                  int channels, void* stream) {
+    if (const int rc = check_residual_norm(dtype, param_dtype, gate_dtype, gate_kind, gate != nullptr, norms, batch, pixels, channels)) return rc;
+    if (normed != nullptr && !(norms & BOXCONV_NORM_BEFORE)) return fail(BOXCONV_E_INVALID_ARGUMENT, "residual norm: normed without BOXCONV_NORM_BEFORE");
+    if (normed == nullptr && normed_exponents != nullptr) return fail(BOXCONV_E_INVALID_ARGUMENT, "residual norm: normed_exponents without normed");
+    if (normed_exponents != nullptr && (reinterpret_cast<uintptr_t>(normed) % 16 != 0 || reinterpret_cast<uintptr_t>(normed_exponents) % 4 != 0))
+        return fail(BOXCONV_E_INVALID_ARGUMENT, "residual norm: codes must be 16-byte aligned, exponents 4-byte aligned");
+    if (batch == 0 || pixels == 0 || (stream_output == nullptr && normed == nullptr)) return 0;
+    if (input == nullptr) return fail(BOXCONV_E_INVALID_ARGUMENT, "residual norm: null input pointer");
+    const ResidualNormCall call = {input, residual, gate, after_weight, after_bias, before_weight, before_bias, gate_kind, (norms & BOXCONV_NORM_AFTER) != 0,
+                                   normed != nullptr, (norms & BOXCONV_NORM_CENTRE) != 0, param_dtype == BOXCONV_F32, gate_dtype == BOXCONV_F32, batch,
+                                   pixels, channels, scale, eps};
+    const ResidualNormOut out = {stream_output, normed, static_cast<uint8_t*>(normed_exponents)};
+    return hip_result(with_type(dtype, [&](auto t) { return residual_norm_forward<decltype(t)>(call, out, static_cast<hipStream_t>(stream)); }), "residual norm");
+}
+
+size_t boxconv_residual_norm_workspace_bytes(int64_t batch, int64_t pixels, int channels, int gate_kind, int dtype) {
+    if (check_residual_norm(dtype, BOXCONV_F32, dtype, gate_kind, gate_kind != BOXCONV_GATE_NONE, 0, batch, pixels, channels) != 0 || batch == 0 || pixels == 0) return 0;
+    ResidualNormCall call = {};
+    call.gate_kind = gate_kind;
+    call.batch = batch;
+    call.pixels = pixels;
+    call.channels = channels;
+    return with_type(dtype, [&](auto t) { return residual_norm_workspace<decltype(t)>(call); });
+}
+
+int boxconv_residual_norm_backward(const void* input, const void* residual, const void* gate, int gate_kind, int gate_dtype, float scale, int norms,
+                                   const void* after_weight, const void* after_bias, const void* before_weight, const void* before_bias, int param_dtype,
+                                   float eps, const void* grad_stream, const void* grad_normed, void* grad_input, void* grad_residual, void* grad_gate,
+                                   void* grad_after_weight, void* grad_after_bias, void* grad_before_weight, void* grad_before_bias, int dtype,
+                                   int64_t batch, int64_t pixels, int channels, void* workspace, size_t workspace_bytes, void* stream) {
+    if (const int rc = check_residual_norm(dtype, param_dtype, gate_dtype, gate_kind, gate != nullptr, norms, batch, pixels, channels)) return rc;
+    if (gate == nullptr && grad_gate != nullptr) return fail(BOXCONV_E_INVALID_ARGUMENT, "residual norm: grad_gate without a gate");
+    if ((!(norms & BOXCONV_NORM_AFTER) && (grad_after_weight != nullptr || grad_after_bias != nullptr)) ||
+        (!(norms & BOXCONV_NORM_BEFORE) && (grad_normed != nullptr || grad_before_weight != nullptr || grad_before_bias != nullptr)))
+        return fail(BOXCONV_E_INVALID_ARGUMENT, "residual norm: gradients of a norm that norms does not have");
+    if (batch == 0 || pixels == 0) {
+        for (void* p : {grad_after_weight, grad_after_bias, grad_before_weight, grad_before_bias})
+            if (const int rc = write_zeros(p, channels, param_dtype, "residual norm", static_cast<hipStream_t>(stream))) return rc;
+        const int64_t gates = gate_kind == BOXCONV_GATE_CHANNEL ? channels : gate_kind == BOXCONV_GATE_ITEM ? batch * channels : 0;
+        return write_zeros(grad_gate, gates, gate_dtype, "residual norm", static_cast<hipStream_t>(stream));
+    }
+    const bool sums = grad_after_weight != nullptr || grad_after_bias != nullptr || grad_before_weight != nullptr || grad_before_bias != nullptr ||
+                      (grad_gate != nullptr && gate_kind != BOXCONV_GATE_FULL);
+    if (!sums && grad_input == nullptr && grad_residual == nullptr && grad_gate == nullptr) return 0;
+    if (input == nullptr) return fail(BOXCONV_E_INVALID_ARGUMENT, "residual norm: null input pointer");
+    if (sums)
+        if (const int rc = check_workspace("residual norm", workspace, workspace_bytes, boxconv_residual_norm_workspace_bytes(batch, pixels, channels, gate_kind, dtype)))
+            return rc;
+    const ResidualNormCall call = {input, residual, gate, after_weight, after_bias, before_weight, before_bias, gate_kind, (norms & BOXCONV_NORM_AFTER) != 0,
+                                   (norms & BOXCONV_NORM_BEFORE) != 0, (norms & BOXCONV_NORM_CENTRE) != 0, param_dtype == BOXCONV_F32,
+                                   gate_dtype == BOXCONV_F32, batch, pixels, channels, scale, eps};
+    const ResidualNormGrads grads = {grad_stream, grad_normed, grad_input, grad_residual, grad_gate, grad_after_weight, grad_after_bias, grad_before_weight, grad_before_bias};
+    return hip_result(with_type(dtype, [&](auto t) { return residual_norm_backward<decltype(t)>(call, grads, workspace, static_cast<hipStream_t>(stream)); }),
+                      "residual norm");
+}
+
 size_t boxconv_linear_workspace_bytes(int64_t rows, int64_t in_features, int64_t out_features, int dtype, int backward) {
     if (check_linear(dtype, rows, in_features, out_features, 0, 0) != 0 || rows == 0 || out_features == 0) return 0;
     return with_type(dtype, [&](auto t) {
@@ -155,6 +245,47 @@ int boxconv_linear_backward(const void* input, int64_t ld_input, const void* wei
     const LinearGradCall call = {input, weight, grad_output, kept, ld_input, grad_input, grad_weight, grad_bias, grad_residual, rows, in_features, out_features,
                                  activation};
     return hip_result(with_type(dtype, [&](auto t) { return linear_backward<decltype(t)>(call, workspace, static_cast<hipStream_t>(stream)); }), "linear");
+}
+
+int boxconv_quantize_blocks(const void* input, int64_t ld_input, int dtype, int64_t rows, int64_t columns, void* codes, void* exponents, void* stream) {
+    if (!known_dtype(dtype)) return fail(BOXCONV_E_INVALID_ARGUMENT, "quantize: dtype must be BOXCONV_F32, BOXCONV_F16 or BOXCONV_BF16, got %d", dtype);
+    if (rows < 0 || columns < 0 || ld_input < 0)
+        return fail(BOXCONV_E_INVALID_ARGUMENT, "quantize: invalid sizes: rows=%lld columns=%lld ld_input=%lld", static_cast<long long>(rows),
+                    static_cast<long long>(columns), static_cast<long long>(ld_input));
+    if (rows > (int64_t(1) << 40) || columns > kMaxExtent - 512 || rows > (int64_t(1) << 46) / std::max<int64_t>({columns, ld_input, 1}))
+        return fail(BOXCONV_E_TOO_LARGE, "quantize: rows=%lld columns=%lld are too large", static_cast<long long>(rows), static_cast<long long>(columns));
+    if (rows == 0 || columns == 0) return 0;
+    if (input == nullptr || codes == nullptr || exponents == nullptr) return fail(BOXCONV_E_INVALID_ARGUMENT, "quantize: null input, codes or exponents pointer");
+    if (reinterpret_cast<uintptr_t>(codes) % 16 != 0 || reinterpret_cast<uintptr_t>(exponents) % 4 != 0)
+        return fail(BOXCONV_E_INVALID_ARGUMENT, "quantize: codes must be 16-byte aligned, exponents 4-byte aligned");
+    const QuantizeCall call = {input, ld_input, dtype, rows, columns, static_cast<uint8_t*>(codes), static_cast<uint8_t*>(exponents)};
+    return hip_result(quantize_launch(call, static_cast<hipStream_t>(stream)), "quantize");
+}
+
+size_t boxconv_linear_float8_workspace_bytes(int64_t rows, int64_t in_features, int64_t out_features, int input_dtype, int dtype) {
+    if (check_linear_float8(dtype, input_dtype, rows, in_features, out_features, 0, 0) != 0 || rows == 0 || in_features == 0 || out_features == 0) return 0;
+    return with_type(dtype, [&](auto t) { return linear_float8_workspace<decltype(t)>(rows, in_features, out_features, input_dtype != BOXCONV_E4M3); });
+}
+
+int boxconv_linear_float8_forward(const void* input, int64_t ld_input, int input_dtype, const void* input_exponents, const void* weight,
+                                  const void* weight_exponents, const void* bias, const void* residual, int64_t ld_residual, void* output, int dtype,
+                                  int64_t rows, int64_t in_features, int64_t out_features, int activation, void* workspace, size_t workspace_bytes,
+                                  void* stream) {
+    if (const int rc = check_linear_float8(dtype, input_dtype, rows, in_features, out_features, ld_input, activation)) return rc;
+    if (ld_residual < 0) return fail(BOXCONV_E_INVALID_ARGUMENT, "linear float8: negative ld_residual");
+    if (rows == 0 || out_features == 0) return 0;
+    const bool coded = input_dtype == BOXCONV_E4M3;
+    if (output == nullptr || input == nullptr || weight == nullptr || weight_exponents == nullptr || coded != (input_exponents != nullptr))
+        return fail(BOXCONV_E_INVALID_ARGUMENT, "linear float8: null input, weight, exponents or output pointer, or exponents of values");
+    for (const void* p : {coded ? input : nullptr, weight})
+        if (reinterpret_cast<uintptr_t>(p) % 16 != 0) return fail(BOXCONV_E_INVALID_ARGUMENT, "linear float8: codes must be 16-byte aligned");
+    for (const void* p : {input_exponents, weight_exponents})
+        if (reinterpret_cast<uintptr_t>(p) % 4 != 0) return fail(BOXCONV_E_INVALID_ARGUMENT, "linear float8: exponents must be 4-byte aligned");
+    const size_t need = boxconv_linear_float8_workspace_bytes(rows, in_features, out_features, input_dtype, dtype);
+    if (const int rc = check_workspace("linear float8", workspace, workspace_bytes, need)) return rc;
+    const LinearFloat8Call call = {input, ld_input, input_dtype, static_cast<const uint8_t*>(input_exponents), static_cast<const uint8_t*>(weight),
+                                   static_cast<const uint8_t*>(weight_exponents), bias, residual, ld_residual, output, rows, in_features, out_features, activation};
+    return hip_result(with_type(dtype, [&](auto t) { return linear_float8_forward<decltype(t)>(call, workspace, static_cast<hipStream_t>(stream)); }), "linear float8");
 }
 
 }  // extern "C"

@@ -58,4 +58,50 @@ template <class T> size_t linear_backward_workspace(int64_t rows, int64_t K, int
 template <class T> hipError_t linear_forward(const LinearCall& c, void* workspace, hipStream_t stream);
 template <class T> hipError_t linear_backward(const LinearGradCall& c, void* workspace, hipStream_t stream);
 
+// Arguments as in boxconv_quantize_blocks and boxconv_linear_float8_forward (include/boxconv.h), checked by the caller.
+constexpr int kE4M3 = 8;           // BOXCONV_E4M3
+struct QuantizeCall {
+    const void* x;
+    int64_t ld;
+    int dtype;
+    int64_t rows, columns;
+    uint8_t *codes, *exponents;
+};
+hipError_t quantize_launch(const QuantizeCall& q, hipStream_t stream);
+struct LinearFloat8Call {
+    const void* x;
+    int64_t ld_x;
+    int input_dtype;
+    const uint8_t *x_exponents, *weight, *weight_exponents;
+    const void *bias, *residual;
+    int64_t ld_residual;
+    void* y;
+    int64_t rows, K, N;
+    int activation;
+};
+template <class T> size_t linear_float8_workspace(int64_t rows, int64_t K, int64_t N, bool values);
+template <class T> hipError_t linear_float8_forward(const LinearFloat8Call& c, void* workspace, hipStream_t stream);
+
+// Arguments as in boxconv_residual_norm_forward / _backward (include/boxconv.h), checked by the caller.
+constexpr int kGateNone = 0, kGateChannel = 1, kGateItem = 2, kGateFull = 3;
+struct ResidualNormCall {
+    const void *x, *residual, *gate, *after_weight, *after_bias, *before_weight, *before_bias;
+    int gate_kind;
+    bool after, before, centre, float_params, float_gate;
+    int64_t batch, pixels;
+    int channels;
+    float scale, eps;
+};
+struct ResidualNormOut {
+    void *stream, *normed;
+    uint8_t* exponents;          // not null: `normed` is codes
+};
+struct ResidualNormGrads {
+    const void *dstream, *dnormed;
+    void *dx, *dresidual, *dgate, *dafter_weight, *dafter_bias, *dbefore_weight, *dbefore_bias;
+};
+template <class T> hipError_t residual_norm_forward(const ResidualNormCall& c, const ResidualNormOut& out, hipStream_t stream);
+template <class T> size_t residual_norm_workspace(const ResidualNormCall& c);
+template <class T> hipError_t residual_norm_backward(const ResidualNormCall& c, const ResidualNormGrads& g, void* workspace, hipStream_t stream);
+
 }  // namespace boxconv

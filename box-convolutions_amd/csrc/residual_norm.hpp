@@ -1,0 +1,45 @@
+// How residual_norm.hip deals rows to workgroups.
+#pragma once
+
+#include <algorithm>
+
+#include "activation.hpp"
+#include "boxconv_host.hpp"
+#include "operators_host.hpp"
+
+namespace boxconv {
+
+namespace {
+
+// The sums over rows that a workgroup of the backward keeps per channel, and where their totals go.
+constexpr int kSums = 5, kSumGate = 4;
+struct RowGrads { void* p[kSums]; };       // after_weight, after_bias, before_weight, before_bias, gate
+
+// Items (what shares a gate: a batch item, or everything) over workgroups: `parts` workgroups an item with `rows` rows each, or `items` whole
+// items a workgroup.
+struct RowPlan { int64_t batch, parts, items, rows, groups; };
+
+// About `target` workgroups, of at least `least` rows each where an item is cut.
+RowPlan plan_rows(const ResidualNormCall& c, int64_t target, int64_t least) {
+    RowPlan p = {1, 1, 1, 0, 0};
+    int64_t pixels = c.batch * c.pixels;
+    if (c.gate_kind == kGateItem) {
+        p.batch = c.batch;
+        pixels = c.pixels;
+    }
+    if (p.batch >= target) {
+        p.items = (p.batch + target - 1) / target;
+        p.rows = pixels;
+        p.groups = (p.batch + p.items - 1) / p.items;
+    } else {
+        p.parts = std::max<int64_t>(1, std::min(target / p.batch, (pixels + least - 1) / least));
+        p.rows = (pixels + p.parts - 1) / p.parts;
+        p.parts = (pixels + p.rows - 1) / p.rows;
+        p.groups = p.batch * p.parts;
+    }
+    return p;
+}
+
+}  // namespace
+
+}  // namespace boxconv

@@ -31,7 +31,7 @@
 extern "C" {
 #endif
 
-#define BOXCONV_ABI_VERSION 4
+#define BOXCONV_ABI_VERSION 5
 
 #define BOXCONV_E_INVALID_ARGUMENT (-1) /* null pointer, non-positive size, ... */
 #define BOXCONV_E_WORKSPACE        (-2) /* workspace missing or smaller than *_workspace_bytes() */
@@ -388,6 +388,60 @@ int boxconv_linear_backward(const void* input, int64_t ld_input, const void* wei
                             void* grad_residual, int dtype, int64_t rows, int64_t in_features,
                             int64_t out_features, int activation, void* workspace, size_t workspace_bytes,
                             void* stream);
+
+/* What lies between two blocks of a residual network, on rows of `channels` values (input, residual, outputs
+ * [batch][pixels][channels], all of type dtype, at any address of a whole element). With
+ *   n(v; w, b) = (v - mean) / sqrt(variance + eps) * w + b   over a row; without BOXCONV_NORM_CENTRE the mean counts as 0,
+ *   u = n(input; after_weight, after_bias) with BOXCONV_NORM_AFTER, else the input,
+ *   s = residual + scale * gate * u   (null residual: 0; gate_kind BOXCONV_GATE_NONE: 1),
+ *   h = n(s; before_weight, before_bias) with BOXCONV_NORM_BEFORE:
+ * stream_output receives s, normed receives h, formed from s before it is rounded. Either may be null. norms is the sum of the
+ * flags. Weights and biases [channels] have param_dtype (BOXCONV_F32 or dtype); null: 1, 0. The gate has gate_dtype (the same
+ * choice) and as many values as its kind says: one per channel, [batch][channels], or, of type dtype, as the input has.
+ * normed_exponents: null, or h is written in 8 bits: normed then holds codes and this their exponents, as
+ * boxconv_quantize_blocks lays them out (normed 16-byte aligned, normed_exponents 4-byte aligned). */
+#define BOXCONV_NORM_AFTER 1
+#define BOXCONV_NORM_BEFORE 2
+#define BOXCONV_NORM_CENTRE 4
+#define BOXCONV_GATE_NONE 0
+#define BOXCONV_GATE_CHANNEL 1
+#define BOXCONV_GATE_ITEM 2
+#define BOXCONV_GATE_FULL 3
+int boxconv_residual_norm_forward(const void* input, const void* residual, const void* gate, int gate_kind, int gate_dtype,
+                                  float scale, int norms, const void* after_weight, const void* after_bias,
+                                  const void* before_weight, const void* before_bias, int param_dtype, float eps,
+                                  void* stream_output, void* normed, void* normed_exponents, int dtype, int64_t batch,
+                                  int64_t pixels, int channels, void* stream);
+/* Its gradients; those whose pointer is null are not formed. grad_stream, grad_normed: the gradients of s and h, null: 0.
+ * grad_gate has the gate's type and shape, the parameters' gradients param_dtype. Sums over no rows are 0. All other arguments as
+ * in the forward call; the workspace (boxconv_residual_norm_workspace_bytes) is 16-byte aligned. */
+size_t boxconv_residual_norm_workspace_bytes(int64_t batch, int64_t pixels, int channels, int gate_kind, int dtype);
+int boxconv_residual_norm_backward(const void* input, const void* residual, const void* gate, int gate_kind, int gate_dtype,
+                                   float scale, int norms, const void* after_weight, const void* after_bias,
+                                   const void* before_weight, const void* before_bias, int param_dtype, float eps,
+                                   const void* grad_stream, const void* grad_normed, void* grad_input, void* grad_residual,
+                                   void* grad_gate, void* grad_after_weight, void* grad_after_bias, void* grad_before_weight,
+                                   void* grad_before_bias, int dtype, int64_t batch, int64_t pixels, int channels,
+                                   void* workspace, size_t workspace_bytes, void* stream);
+
+/* Rows of values in 8-bit floating point (e4m3: largest value 448, no infinities), a power of two for each block of 128 columns:
+ * value = code * 2^(exponent - 127), exponent the least from 1 on that keeps the block's largest finite magnitude at or below 448 times
+ * its power (127 for a block of zeros), code rounded to nearest, ties to even; NaN and infinities become NaN. input [rows][columns], rows
+ * ld_input elements apart, at any address of a whole element. codes [rows][columns rounded up to 128], the rest zeros, 16-byte aligned;
+ * exponents [rows][blocks rounded up to 4], the rest 127, 4-byte aligned. */
+#define BOXCONV_E4M3 8
+int boxconv_quantize_blocks(const void* input, int64_t ld_input, int dtype, int64_t rows, int64_t columns, void* codes,
+                            void* exponents, void* stream);
+/* The pointwise product of such rows (inference): y = act(x W^T + bias + residual), the product exact but for float32 sums. weight and
+ * weight_exponents: [out_features] rows of in_features columns as boxconv_quantize_blocks lays them out. input: the same with input_dtype
+ * BOXCONV_E4M3 (ld_input is not looked at); or values of type dtype, rows ld_input apart, which are quantized on the way
+ * (input_exponents null). bias, residual and output as in boxconv_linear_forward, of type dtype. The workspace
+ * (boxconv_linear_float8_workspace_bytes; may be 0) is 16-byte aligned. */
+size_t boxconv_linear_float8_workspace_bytes(int64_t rows, int64_t in_features, int64_t out_features, int input_dtype, int dtype);
+int boxconv_linear_float8_forward(const void* input, int64_t ld_input, int input_dtype, const void* input_exponents,
+                                  const void* weight, const void* weight_exponents, const void* bias, const void* residual,
+                                  int64_t ld_residual, void* output, int dtype, int64_t rows, int64_t in_features,
+                                  int64_t out_features, int activation, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
