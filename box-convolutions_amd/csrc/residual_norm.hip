@@ -11,7 +11,10 @@
 //   dw_before = sum dh q, db_before = sum dh, dw_after = sum du p, db_after = sum du
 //
 // s is formed in float32 and h and the backward take it unrounded: the backward forms it again from x, the residual and the gate.
+#include <type_traits>
+
 #include "float8_blocks.hpp"
+#include "linear_tile.hpp"
 #include "residual_norm.hpp"
 
 namespace boxconv {
@@ -35,6 +38,7 @@ struct Rows {
     T *dx, *dresidual, *dgate_full;
     void* dgate;                       // of an item, where a workgroup has all its rows
     float* sums;                       // [workgroup][kSums][channels]
+    int wanted;                        // bit k: sum k, over all the workgroup's rows
 };
 
 // The rows [first, last) of item i of the workgroup's, counted over the whole tensor; none from `items` on.
@@ -212,6 +216,410 @@ __global__ void __launch_bounds__(kAnyThreads) norm_rows_any_grad_kernel(Rows<T>
     }
 }
 
+// ---- rows in registers ----------------------------------------------------------------------------------------------
+// A team of lanes holds a row, kPerLane neighbouring elements a lane: `lanes` (a power of two) of a
+// wave, or, WIDE, a whole workgroup. Every tensor is read once and written once; means and deviations are taken from registers. A team
+// keeps its columns from row to row, so parameters stay in registers too, and so do the backward's sums over rows.
+constexpr int kPerLane = 8, kNarrowThreads = 256;
+constexpr int kMostRegisterChannels = 1024 * kPerLane;
+
+template <class T, bool WIDE, bool RAGGED>
+struct Team {
+    static constexpr int V = Vec<T>::kLen, NV = kPerLane / V, E = kPerLane;
+    int lanes, lane, channels;
+    float inverse;                     // 1 / channels
+    float (*exchange)[16][2];          // WIDE: [2][wave][2] in LDS, the two halves in turn
+    int turn = 0;
+
+    __device__ __forceinline__ int column(int v) const { return lane * E + v * V; }
+    // whether element j of vector v lies in the row
+    __device__ __forceinline__ bool inside(int v, int j) const { return column(v) + (RAGGED ? j : 0) < channels; }
+
+    __device__ __forceinline__ void request(const T* tensor, int64_t row, Chunk (&raw)[NV]) const {
+        if (tensor == nullptr) return;
+        const T* p = tensor + row * channels;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const int c = column(v), n = channels - c;
+            if constexpr (RAGGED) raw[v] = channels < V ? short_chunk(p + c, n) : request_chunk(p + c, n, tensor);
+            else raw[v] = n > 0 ? __builtin_bit_cast(Chunk, *reinterpret_cast<const typename Vec<T>::Type*>(p + c)) : Chunk{0, 0, 0, 0};
+        }
+    }
+    // What was requested, as floats; 0 beyond the row.
+    __device__ __forceinline__ void settle(Chunk (&raw)[NV], float (&out)[E]) const {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            if constexpr (RAGGED) {
+                if (channels >= V) settle_chunk<T>(raw[v], channels - column(v));
+            }
+            const auto x = __builtin_bit_cast(typename Vec<T>::Type, raw[v]);
+#pragma unroll
+            for (int j = 0; j < V; ++j) out[v * V + j] = static_cast<float>(x[j]);
+        }
+    }
+    __device__ __forceinline__ void store(T* tensor, int64_t row, const float (&value)[E]) const {
+        T* p = tensor + row * channels;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            T out[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) out[j] = static_cast<T>(value[v * V + j]);
+            const int n = channels - column(v);
+            if constexpr (RAGGED) store_run<T, V>(p + column(v), out, n);
+            else if (n > 0) store_run<T, V>(p + column(v), out, V);
+        }
+    }
+    // Values per column, of the parameters' type or float; `none` beyond the row and without a vector.
+    __device__ __forceinline__ void params(const void* p, bool is_float, float none, float (&out)[E]) const {
+#pragma unroll
+        for (int i = 0; i < E; ++i) out[i] = none;
+        if (p == nullptr) return;
+        if (is_float) {
+#pragma unroll
+            for (int i = 0; i < E; ++i)
+                if (inside(i / V, i % V)) out[i] = static_cast<const float*>(p)[column(i / V) + i % V];
+        } else {
+#pragma unroll
+            for (int i = 0; i < E; ++i)
+                if (inside(i / V, i % V)) out[i] = static_cast<float>(static_cast<const T*>(p)[column(i / V) + i % V]);
+        }
+    }
+    // Over the row: the sums of a and b, the same in all its lanes.
+    __device__ __forceinline__ void pair_sum(float& a, float& b) {
+        if constexpr (!WIDE) {
+            a = sum_of_lanes(a, lanes);
+            b = sum_of_lanes(b, lanes);
+        } else {
+            a = sum_of_lanes(a, 64);
+            b = sum_of_lanes(b, 64);
+            swap(a, b);
+            a = b = 0.0f;
+            for (int w = 0; w < static_cast<int>(blockDim.x) / 64; ++w) {
+                a += exchange[turn ^ 1][w][0];
+                b += exchange[turn ^ 1][w][1];
+            }
+        }
+    }
+    // WIDE: a and b of every wave to the half of `exchange` that is now turn ^ 1. (One barrier: a wave that is a call ahead writes the
+    // other half, and none gets two ahead.)
+    __device__ __forceinline__ void swap(float a, float b) {
+        if (threadIdx.x % 64 == 0) {
+            exchange[turn][threadIdx.x / 64][0] = a;
+            exchange[turn][threadIdx.x / 64][1] = b;
+        }
+        __syncthreads();
+        turn ^= 1;
+    }
+    // Mean (0 unless centred) and 1/sqrt(variance + eps) of the row.
+    __device__ __forceinline__ Moments moments(const float (&value)[E], bool centre, float eps) {
+        Moments m = {0.0f, 0.0f};
+        float sum = 0.0f, square = 0.0f;
+        if (!centre) {
+#pragma unroll
+            for (int i = 0; i < E; ++i) square += value[i] * value[i];
+            pair_sum(square, sum);
+        } else {
+            // within a wave first the mean, then the deviations from it
+#pragma unroll
+            for (int i = 0; i < E; ++i) sum += value[i];
+            sum = sum_of_lanes(sum, WIDE ? 64 : lanes);
+            float part = inverse;
+            int count = channels;
+            if constexpr (WIDE) {
+                count = in_wave(threadIdx.x / 64);
+                part = 1.0f / static_cast<float>(max(count, 1));
+            }
+            m.mean = sum * part;
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                const float d = inside(i / V, i % V) ? value[i] - m.mean : 0.0f;
+                square += d * d;
+            }
+            square = sum_of_lanes(square, WIDE ? 64 : lanes);
+            if constexpr (WIDE) {
+                // the waves' means before their deviations: nothing cancels however far the mean is from zero
+                const int waves = blockDim.x / 64;
+                swap(m.mean, square);
+                float mean = 0.0f;
+                for (int w = 0; w < waves; ++w) mean += static_cast<float>(in_wave(w)) * exchange[turn ^ 1][w][0];
+                m.mean = mean * inverse;
+                square = 0.0f;
+                for (int w = 0; w < waves; ++w) {
+                    const float d = exchange[turn ^ 1][w][0] - m.mean;
+                    square += exchange[turn ^ 1][w][1] + static_cast<float>(in_wave(w)) * d * d;
+                }
+            }
+        }
+        m.rstd = rsqrtf(square * inverse + eps);
+        return m;
+    }
+    // Elements of the row in wave w.
+    __device__ __forceinline__ int in_wave(int w) const { return min(max(channels - w * 64 * E, 0), 64 * E); }
+};
+
+// The team of this thread, the first row of its wave's next ones (from 0 on), its own place among them, and how far apart they are.
+template <class T, bool WIDE, bool RAGGED>
+struct Place {
+    Team<T, WIDE, RAGGED> team;
+    int first, own, step;
+    __device__ __forceinline__ Place(const Rows<T>& a, int lanes, float (*exchange)[16][2]) {
+        team.lanes = lanes;
+        team.lane = WIDE ? threadIdx.x : threadIdx.x & (lanes - 1);
+        team.channels = a.channels;
+        team.inverse = 1.0f / static_cast<float>(a.channels);
+        team.exchange = exchange;
+        const int teams = WIDE ? 1 : 64 / lanes;                       // in a wave
+        first = WIDE ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / 64) * teams;
+        own = WIDE ? 0 : threadIdx.x % 64 / lanes;
+        step = WIDE ? 1 : kNarrowThreads / 64 * teams;
+    }
+};
+
+template <class T, bool WIDE, bool RAGGED>
+__device__ __forceinline__ void item_gate(const Team<T, WIDE, RAGGED>& team, const Rows<T>& a, int64_t item, float (&g)[kPerLane]) {
+    const int64_t at = a.gate_kind == kGateItem ? item * a.channels : 0;
+    if (a.gate_kind == kGateChannel || a.gate_kind == kGateItem)
+        team.params(a.float_gate ? static_cast<const void*>(static_cast<const float*>(a.gate) + at) : static_cast<const void*>(static_cast<const T*>(a.gate) + at),
+                    a.float_gate, 1.0f, g);
+}
+
+// CODES: the normed rows leave in 8 bits. A block of 128 lies in 128 / kPerLane neighbouring lanes.
+template <class T, bool WIDE, bool RAGGED, bool CODES>
+__global__ void __launch_bounds__(WIDE ? 1024 : kNarrowThreads) norm_rows_kernel(Rows<T> a, int lanes) {
+    typedef Team<T, WIDE, RAGGED> Row;
+    constexpr int E = Row::E, V = Row::V, NV = Row::NV;
+    __shared__ float exchange[2][16][2];
+    Place<T, WIDE, RAGGED> place(a, lanes, exchange);
+    Row& team = place.team;
+    float wa[E], ba[E], wb[E], bb[E], g[E];
+    const T* const full = a.gate_kind == kGateFull ? static_cast<const T*>(a.gate) : nullptr;
+#pragma unroll
+    for (int i = 0; i < E; ++i) g[i] = 1.0f;
+    bool loaded = false;
+    for (int64_t i = 0; i < a.plan.items; ++i) {
+        const Span span = span_of(a.plan, a.pixels, i);
+        Chunk xs[NV] = {}, rs[NV] = {}, gs[NV] = {};
+        const auto request = [&](int64_t base) {
+            const int64_t row = min(base + place.own, span.last - 1);
+            team.request(a.x, row, xs);
+            team.request(a.residual, row, rs);
+            team.request(full, row, gs);
+        };
+        int64_t base = span.first + place.first;
+        if (base < span.last) request(base);
+        if (!loaded) {
+            team.params(a.after_weight, a.float_params, 1.0f, wa);
+            team.params(a.after_bias, a.float_params, 0.0f, ba);
+            team.params(a.before_weight, a.float_params, 1.0f, wb);
+            team.params(a.before_bias, a.float_params, 0.0f, bb);
+            loaded = true;
+        }
+        item_gate(team, a, span.item, g);
+        for (; base < span.last; base += place.step) {
+            const int64_t row = base + place.own;
+            const bool live = row < span.last;
+            float x[E], r[E];
+            team.settle(xs, x);
+            team.settle(rs, r);
+            if (full != nullptr) team.settle(gs, g);
+            if (base + place.step < span.last) request(base + place.step);
+            if (a.after) {
+                const Moments m = team.moments(x, a.centre, a.eps);
+#pragma unroll
+                for (int k = 0; k < E; ++k) x[k] = (x[k] - m.mean) * m.rstd * wa[k] + ba[k];
+            }
+#pragma unroll
+            for (int k = 0; k < E; ++k) x[k] = r[k] + x[k] * g[k] * a.scale;
+            if constexpr (RAGGED) {
+#pragma unroll
+                for (int k = 0; k < E; ++k)
+                    if (!team.inside(k / V, k % V)) x[k] = 0.0f;
+            } else {
+#pragma unroll
+                for (int k = 0; k < E; ++k)
+                    if (!team.inside(k / V, 0)) x[k] = 0.0f;
+            }
+            if (a.stream != nullptr && live) team.store(a.stream, row, x);
+            if (!a.before) continue;
+            const Moments m = team.moments(x, a.centre, a.eps);
+#pragma unroll
+            for (int k = 0; k < E; ++k) x[k] = (x[k] - m.mean) * m.rstd * wb[k] + bb[k];
+            if constexpr (!CODES) {
+                if (live) team.store(a.normed, row, x);
+            } else {
+                const int blocks = blocks_of(a.channels), words = exponents_of(a.channels), c = team.column(0), b = c / kBlock;
+#pragma unroll
+                for (int k = 0; k < E; ++k) x[k] = team.inside(k / V, k % V) ? x[k] : 0.0f;
+                const int e = block_exponent(most_of_lanes(largest(x), kBlock / E));
+                const Codes<E> codes = to_codes(x, e);
+                if (live && b < blocks) {
+                    typedef unsigned Words __attribute__((ext_vector_type(E / 4)));
+                    *reinterpret_cast<Words*>(a.codes + row * blocks * kBlock + c) = __builtin_bit_cast(Words, codes);
+                    if (c % kBlock == 0) {
+                        a.exponents[row * words + b] = static_cast<uint8_t>(e);
+                        if (b == blocks - 1)
+                            for (int w = blocks; w < words; ++w) a.exponents[row * words + w] = 127;
+                    }
+                }
+            }
+        }
+    }
+}
+
+// BIG: rows of more than 512 lanes, 128 registers each: parameters come from the caches again for every row, and no row is requested ahead.
+template <class T, bool WIDE, bool RAGGED, bool BIG>
+__global__ void __launch_bounds__(WIDE ? (BIG ? 1024 : 512) : kNarrowThreads) norm_rows_grad_kernel(Rows<T> a, int lanes) {
+    typedef Team<T, WIDE, RAGGED> Row;
+    constexpr int E = Row::E, V = Row::V, NV = Row::NV;
+    __shared__ float exchange[2][16][2];
+    __shared__ float gather[WIDE ? 1 : kNarrowThreads / 64][WIDE ? 1 : 64 * kPerLane];
+    Place<T, WIDE, RAGGED> place(a, lanes, exchange);
+    Row& team = place.team;
+    float wa[E], ba[E], wb[E], g[E], sum[kSums][E];
+    const T* const full = a.gate_kind == kGateFull ? static_cast<const T*>(a.gate) : nullptr;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        g[i] = 1.0f;
+#pragma unroll
+        for (int k = 0; k < kSums; ++k) sum[k][i] = 0.0f;
+    }
+    const auto parameters = [&] {
+        team.params(a.after_weight, a.float_params, 1.0f, wa);
+        team.params(a.after_bias, a.float_params, 0.0f, ba);
+        team.params(a.before_weight, a.float_params, 1.0f, wb);
+    };
+    if constexpr (!BIG) parameters();
+    const bool has_dh = a.before && a.dnormed != nullptr;
+    // sum k of the workgroup's teams to memory
+    const auto put = [&](const float (&v)[E], void* to, int64_t at, bool is_float) {
+        const auto write = [&](int c, float s) {
+            if (is_float) static_cast<float*>(to)[at + c] = s;
+            else static_cast<T*>(to)[at + c] = static_cast<T>(s);
+        };
+        if constexpr (WIDE) {
+#pragma unroll
+            for (int k = 0; k < E; ++k)
+                if (team.inside(k / V, k % V)) write(team.column(k / V) + k % V, v[k]);
+        } else {
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < E; ++k) {
+                float s = v[k];
+                for (int d = lanes; d < 64; d <<= 1) s += __shfl_xor(s, d);
+                if (static_cast<int>(threadIdx.x) % 64 < lanes) gather[threadIdx.x / 64][team.column(k / V) + k % V] = s;
+            }
+            __syncthreads();
+            for (int c = threadIdx.x; c < a.channels; c += kNarrowThreads) {
+                float s = 0.0f;
+#pragma unroll
+                for (int w = 0; w < kNarrowThreads / 64; ++w) s += gather[w][c];
+                write(c, s);
+            }
+        }
+    };
+    for (int64_t i = 0; i < a.plan.items; ++i) {
+        const Span span = span_of(a.plan, a.pixels, i);
+        Chunk xs[NV] = {}, rs[NV] = {}, gs[NV] = {}, ds[NV] = {}, hs[NV] = {};
+        const auto request = [&](int64_t base) {
+            const int64_t row = min(base + place.own, span.last - 1);
+            team.request(a.x, row, xs);
+            if (a.before) team.request(a.residual, row, rs);
+            team.request(full, row, gs);
+            team.request(a.dstream, row, ds);
+            if (a.before) team.request(a.dnormed, row, hs);
+        };
+        int64_t base = span.first + place.first;
+        if constexpr (!BIG) {
+            if (base < span.last) request(base);
+            item_gate(team, a, span.item, g);
+        }
+        for (; base < span.last; base += place.step) {
+            const int64_t row = base + place.own;
+            const bool live = row < span.last;
+            if constexpr (BIG) {
+                request(base);
+                parameters();
+                item_gate(team, a, span.item, g);
+            }
+            float p[E], q[E], d[E], h[E];                              // normalised x, normalised s, gradients of s and h
+            team.settle(xs, p);
+            team.settle(rs, q);
+            team.settle(ds, d);
+            team.settle(hs, h);
+            if (full != nullptr) team.settle(gs, g);
+            if constexpr (!BIG) {
+                if (base + place.step < span.last) request(base + place.step);
+            }
+            Moments mx = {0.0f, 1.0f};
+            if (a.after) {
+                mx = team.moments(p, a.centre, a.eps);
+#pragma unroll
+                for (int k = 0; k < E; ++k) p[k] = (p[k] - mx.mean) * mx.rstd;
+            }
+            if (has_dh) {
+#pragma unroll
+                for (int k = 0; k < E; ++k) {
+                    const float u = a.after ? p[k] * wa[k] + ba[k] : p[k];
+                    q[k] = team.inside(k / V, k % V) ? q[k] + u * g[k] * a.scale : 0.0f;
+                }
+                const Moments ms = team.moments(q, a.centre, a.eps);
+                float e1 = 0.0f, e2 = 0.0f;
+#pragma unroll
+                for (int k = 0; k < E; ++k) {
+                    q[k] = (q[k] - ms.mean) * ms.rstd;
+                    const float e = h[k] * wb[k];                      // (0 beyond the row)
+                    e1 += e;
+                    e2 += e * q[k];
+                    sum[2][k] += live ? h[k] * q[k] : 0.0f;
+                    sum[3][k] += live ? h[k] : 0.0f;
+                }
+                team.pair_sum(e1, e2);
+                e1 = a.centre ? e1 * team.inverse : 0.0f;
+                e2 *= team.inverse;
+#pragma unroll
+                for (int k = 0; k < E; ++k) d[k] += ms.rstd * (h[k] * wb[k] - e1 - q[k] * e2);
+            }
+            if (a.dresidual != nullptr && live) team.store(a.dresidual, row, d);
+            float f1 = 0.0f, f2 = 0.0f;
+#pragma unroll
+            for (int k = 0; k < E; ++k) {
+                const float u = a.after ? p[k] * wa[k] + ba[k] : p[k], t = a.scale * d[k];
+                q[k] = u * t;                                          // of the gate
+                d[k] = t * g[k];                                       // of u
+                sum[kSumGate][k] += live ? q[k] : 0.0f;
+            }
+            if (a.dgate_full != nullptr && live) team.store(a.dgate_full, row, q);
+            if (a.after) {
+#pragma unroll
+                for (int k = 0; k < E; ++k) {
+                    const bool in = team.inside(k / V, k % V);
+                    const float du = in ? d[k] : 0.0f;
+                    sum[0][k] += live ? du * p[k] : 0.0f;
+                    sum[1][k] += live ? du : 0.0f;
+                    d[k] = du * wa[k];
+                    f1 += d[k];
+                    f2 += in ? d[k] * p[k] : 0.0f;
+                }
+                team.pair_sum(f1, f2);
+                f1 = a.centre ? f1 * team.inverse : 0.0f;
+                f2 *= team.inverse;
+#pragma unroll
+                for (int k = 0; k < E; ++k) d[k] = mx.rstd * (d[k] - f1 - p[k] * f2);
+            }
+            if (a.dx != nullptr && live) team.store(a.dx, row, d);
+        }
+        if (a.gate_kind == kGateItem && (a.dgate != nullptr || a.sums != nullptr) && span.last > span.first) {
+            if (a.dgate != nullptr) put(sum[kSumGate], a.dgate, span.item * a.channels, a.float_gate);
+            else put(sum[kSumGate], a.sums, (static_cast<int64_t>(blockIdx.x) * kSums + kSumGate) * a.channels, true);
+#pragma unroll
+            for (int k = 0; k < E; ++k) sum[kSumGate][k] = 0.0f;
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < kSums; ++k)
+        if (a.wanted >> k & 1) put(sum[k], a.sums, (static_cast<int64_t>(blockIdx.x) * kSums + k) * a.channels, true);
+}
+
 // ---- sums over workgroups -----------------------------------------------------------------------------------------
 // Column sums of [workgroup][kSums][channels] in an order that only the sizes decide. blockIdx.y: which sum; from kSums on the gate's of item
 // blockIdx.y - kSums, over its own workgroups. A workgroup takes 32 columns, 32 threads side by side down the workgroups.
@@ -265,22 +673,59 @@ Rows<T> rows_of(const ResidualNormCall& c) {
     return a;
 }
 
+// How the rows of a call are dealt out: lanes of a team, its workgroup's threads, and rows that a workgroup takes at once. No lanes: rows of more
+// channels than the registers of a workgroup hold.
+struct Shape { bool wide; int lanes, threads, rows; };
+template <class T>
+Shape shape_of(int channels, bool codes) {
+    if (channels > kMostRegisterChannels) return {true, 0, kAnyThreads, 1};
+    const int columns = codes ? blocks_of(channels) * kBlock : channels;           // (codes are written to the end of the last block)
+    int lanes = codes ? kBlock / kPerLane : 1;        // (more lanes without a share add zeros: the sums are the same to the bit)
+    while (lanes < 64 && lanes * kPerLane < columns) lanes *= 2;
+    if (lanes * kPerLane >= columns) return {false, lanes, kNarrowThreads, kNarrowThreads / lanes};
+    lanes = (columns + 64 * kPerLane - 1) / (64 * kPerLane) * 64;
+    return {true, lanes, lanes, 1};
+}
+
+// f(true) or f(false), with the value known to the compiler.
+template <class F>
+void known(bool value, F f) {
+    if (value) f(std::true_type());
+    else f(std::false_type());
+}
+
+RowPlan forward_plan(const ResidualNormCall& c, const Shape& s) { return plan_rows(c, 2048, s.rows); }
+RowPlan backward_plan(const ResidualNormCall& c, const Shape& s) { return plan_rows(c, s.wide ? 512 : 1024, s.rows); }
+
 }  // namespace
 
 template <class T>
 hipError_t residual_norm_forward(const ResidualNormCall& c, const ResidualNormOut& out, hipStream_t stream) {
     Rows<T> a = rows_of<T>(c);
     a.stream = static_cast<T*>(out.stream);
-    (out.exponents != nullptr ? reinterpret_cast<void*&>(a.codes) : reinterpret_cast<void*&>(a.normed)) = out.normed;
     a.exponents = out.exponents;
-    a.plan = plan_rows(c, 2048, 1);
-    BOXCONV_LAUNCH("norm_rows", (norm_rows_any_kernel<T>), dim3(static_cast<unsigned>(a.plan.groups)), dim3(kAnyThreads), 0, stream, a);
+    const bool coded = out.exponents != nullptr;
+    if (coded) a.codes = static_cast<uint8_t*>(out.normed);
+    else a.normed = static_cast<T*>(out.normed);
+    const Shape s = shape_of<T>(c.channels, coded);
+    a.plan = forward_plan(c, s);
+    const dim3 grid(static_cast<unsigned>(a.plan.groups)), block(s.threads);
+    if (s.lanes == 0) BOXCONV_LAUNCH("norm_rows", (norm_rows_any_kernel<T>), grid, block, 0, stream, a);
+    else
+        known(s.wide, [&](auto wide) {
+            known(c.channels % Vec<T>::kLen != 0, [&](auto ragged) {
+                known(coded, [&](auto codes) {
+                    BOXCONV_LAUNCH("norm_rows", (norm_rows_kernel<T, decltype(wide)::value, decltype(ragged)::value, decltype(codes)::value>), grid, block, 0, stream, a,
+                                   s.lanes);
+                });
+            });
+        });
     return hipGetLastError();
 }
 
 template <class T>
 size_t residual_norm_workspace(const ResidualNormCall& c) {
-    return static_cast<size_t>(plan_rows(c, 512, 1).groups) * kSums * c.channels * sizeof(float);
+    return static_cast<size_t>(backward_plan(c, shape_of<T>(c.channels, false)).groups) * kSums * c.channels * sizeof(float);
 }
 
 template <class T>
@@ -290,18 +735,29 @@ hipError_t residual_norm_backward(const ResidualNormCall& c, const ResidualNormG
     a.dnormed = static_cast<const T*>(g.dnormed);
     a.dx = static_cast<T*>(g.dx);
     a.dresidual = static_cast<T*>(g.dresidual);
-    a.plan = plan_rows(c, 512, 1);
+    const Shape s = shape_of<T>(c.channels, false);
+    a.plan = backward_plan(c, s);
     RowGrads to = {{g.dafter_weight, g.dafter_bias, g.dbefore_weight, g.dbefore_bias, c.gate_kind == kGateFull ? nullptr : g.dgate}};
     if (c.gate_kind == kGateFull) a.dgate_full = static_cast<T*>(g.dgate);
-    bool any = false;
-    for (void* p : to.p) any = any || p != nullptr;
-    if (any) a.sums = static_cast<float*>(workspace);
+    for (int k = 0; k < kSums; ++k) {
+        if (to.p[k] == nullptr) continue;
+        a.sums = static_cast<float*>(workspace);
+        if (k != kSumGate || c.gate_kind != kGateItem) a.wanted |= 1 << k;
+    }
     if (c.gate_kind == kGateItem && a.plan.parts == 1) {
         a.dgate = g.dgate;
         to.p[kSumGate] = nullptr;
     }
-    BOXCONV_LAUNCH("norm_rows_grad", (norm_rows_any_grad_kernel<T>), dim3(static_cast<unsigned>(a.plan.groups)), dim3(kAnyThreads), 0, stream, a);
-    any = false;
+    const dim3 grid(static_cast<unsigned>(a.plan.groups)), block(s.threads);
+    if (s.lanes == 0) BOXCONV_LAUNCH("norm_rows_grad", (norm_rows_any_grad_kernel<T>), grid, block, 0, stream, a);
+    else
+        known(c.channels % Vec<T>::kLen != 0, [&](auto ragged) {
+            constexpr bool R = decltype(ragged)::value;
+            if (!s.wide) BOXCONV_LAUNCH("norm_rows_grad", (norm_rows_grad_kernel<T, false, R, false>), grid, block, 0, stream, a, s.lanes);
+            else if (s.threads <= 512) BOXCONV_LAUNCH("norm_rows_grad", (norm_rows_grad_kernel<T, true, R, false>), grid, block, 0, stream, a, s.lanes);
+            else BOXCONV_LAUNCH("norm_rows_grad", (norm_rows_grad_kernel<T, true, R, true>), grid, block, 0, stream, a, s.lanes);
+        });
+    bool any = false;
     for (void* p : to.p) any = any || p != nullptr;
     if (any) {
         const unsigned kinds = to.p[kSumGate] != nullptr && c.gate_kind == kGateItem ? kSumGate + static_cast<unsigned>(c.batch) : kSums;
