@@ -142,7 +142,9 @@ def glue():
                 "boxconv_last_error")])
             module.init_operators(*[ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
                 "boxconv_group_norm_workspace_bytes", "boxconv_group_norm_forward", "boxconv_group_norm_backward",
-                "boxconv_linear_workspace_bytes", "boxconv_linear_forward", "boxconv_linear_backward")])
+                "boxconv_linear_workspace_bytes", "boxconv_linear_forward", "boxconv_linear_backward",
+                "boxconv_residual_norm_workspace_bytes", "boxconv_residual_norm_forward", "boxconv_residual_norm_backward",
+                "boxconv_quantize_blocks", "boxconv_linear_float8_workspace_bytes", "boxconv_linear_float8_forward")])
             _glue = module
     return _glue or None
 

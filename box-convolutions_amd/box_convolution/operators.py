@@ -221,9 +221,7 @@ def _gate_kind(gate, input):
 def _norm_pairs(input, after, before):
     """The four parameters, contiguous, of norms given as None or (weight, bias)."""
     out, kind = [], None
-    for name, pair in (("after", after), ("before", before)):
-        if pair is not None and (not isinstance(pair, (tuple, list)) or len(pair) != 2):
-            raise RuntimeError("box_convolution: %s must be None or a pair (weight, bias), either of which may be None" % name)
+    for pair in (after, before):
         for p in pair or (None, None):
             if p is not None:
                 if p.device != input.device or p.dim() != 1 or p.size(0) != input.size(1):
@@ -257,9 +255,20 @@ def residual_norm(input, residual=None, gate=None, scale=1.0, after=None, before
     Statistics and sums are float32; ``normed`` is formed from the stream before it is rounded to the input's type.
     """
     _native._require_device(input, "residual norm input")
-    _native._operator_dtype(input, "residual norm input")
     if kind not in ("rms", "layer"):
         raise RuntimeError("box_convolution: kind must be 'rms' or 'layer', got %r" % (kind,))
+    for name, pair in (("after", after), ("before", before)):
+        if pair is not None and (not isinstance(pair, (tuple, list)) or len(pair) != 2):
+            raise RuntimeError("box_convolution: %s must be None or a pair (weight, bias), either of which may be None" % name)
+    glue = _native.glue()
+    if glue is not None:                               # as in group_norm_act
+        with _native._on_device(input.device):
+            out = glue.residual_norm(input, residual, gate, scale, after is not None, *(after or (None, None)), before is not None,
+                                     *(before or (None, None)), kind == "layer", eps, quantize, _native._stream(input.device) or 0)
+        if before is None:
+            return out[0]
+        return out[0], Float8Blocks._of(out[1], out[2], input.size(1)) if quantize else out[1]
+    _native._operator_dtype(input, "residual norm input")
     if input.dim() < 2 or input.size(1) < 1:
         raise RuntimeError("box_convolution: residual norm input must have >=2 dimensions and a channel")
     gate_kind = _gate_kind(gate, input)
@@ -291,7 +300,7 @@ def residual_norm(input, residual=None, gate=None, scale=1.0, after=None, before
                       torch.empty((*x.shape[:-1], exponents), dtype=torch.uint8, device=x.device))
         stream, normed = _native.residual_norm_forward(x, r, g, gate_kind, scale, norms, params, eps, not same, blocks)
         if quantize:
-            normed = Float8Blocks(*blocks, x.size(-1))
+            normed = Float8Blocks._of(*blocks, x.size(-1))
     stream = input if same else stream.movedim(-1, 1)
     if before is None:
         return stream
@@ -314,6 +323,13 @@ class Float8Blocks:
         if not codes.is_contiguous() or not exponents.is_contiguous() or codes.data_ptr() % 16 or exponents.data_ptr() % 4:
             raise RuntimeError("box_convolution: the codes and exponents of Float8Blocks must be contiguous, at addresses of whole 16 and 4 bytes")
         self.codes, self.exponents, self.columns = codes, exponents, columns
+
+    @classmethod
+    def _of(cls, codes, exponents, columns):
+        """Of tensors that an operator made: nothing to check."""
+        self = object.__new__(cls)
+        self.codes, self.exponents, self.columns = codes, exponents, columns
+        return self
 
     @property
     def shape(self):
@@ -340,12 +356,16 @@ def quantize_blocks(input):
     become NaN and leave the rest of their block alone. Not differentiable: an input that requires a gradient is refused while
     gradients are recorded."""
     _native._require_device(input, "quantize input")
+    glue = _native.glue()
+    if glue is not None:                               # as in group_norm_act
+        with _native._on_device(input.device):
+            return Float8Blocks._of(*glue.quantize_blocks(input, _native._stream(input.device) or 0), input.size(-1))
     _native._operator_dtype(input, "quantize input")
     if input.dim() < 1 or input.size(-1) < 1:
         raise RuntimeError("box_convolution: quantize_blocks needs an input [..., K] with at least one column")
     _refuse_gradients("quantize_blocks", input)
     codes, exponents = _native.quantize_blocks(_rows(input, math.prod(input.shape[:-1]), input.size(-1)))
-    return Float8Blocks(codes.view(*input.shape[:-1], codes.size(-1)), exponents.view(*input.shape[:-1], exponents.size(-1)), input.size(-1))
+    return Float8Blocks._of(codes.view(*input.shape[:-1], codes.size(-1)), exponents.view(*input.shape[:-1], exponents.size(-1)), input.size(-1))
 
 
 def _refuse_gradients(what, *tensors):
@@ -365,17 +385,22 @@ def linear_act_float8(input, weight, bias=None, residual=None, activation=None, 
 
     Products of codes and powers of two are exact, sums are float32.
     """
-    _native._activation(activation)
+    act = _native._activation(activation)
     coded = isinstance(input, Float8Blocks)
     rows_of = input.codes if coded else input
     _native._require_device(rows_of, "linear float8 input")
+    if not isinstance(weight, Float8Blocks):
+        raise RuntimeError("box_convolution: weight must be Float8Blocks (quantize_blocks(weight)), got %s" % type(weight).__name__)
+    glue = _native.glue()
+    if glue is not None:                               # as in group_norm_act
+        with _native._on_device(rows_of.device):
+            return glue.linear_act_float8(rows_of, input.exponents if coded else None, input.columns if coded else input.shape[-1] if input.dim() else 0,
+                                          weight.codes, weight.exponents, weight.columns, bias, residual, act, dtype, _native._stream(rows_of.device) or 0)
     if not coded:
         _native._operator_dtype(input, "linear float8 input")
     dtype = dtype or (torch.bfloat16 if coded else input.dtype)
     if dtype not in _native._FUSED_OUTPUT or (not coded and dtype != input.dtype):
         raise RuntimeError("box_convolution: the result's type must be that of the values, or float32, float16 or bfloat16 for Float8Blocks, got %s" % dtype)
-    if not isinstance(weight, Float8Blocks):
-        raise RuntimeError("box_convolution: weight must be Float8Blocks (quantize_blocks(weight)), got %s" % type(weight).__name__)
     if len(input.shape) < 1 or len(weight.shape) != 2 or weight.columns != input.shape[-1] or weight.device != rows_of.device:
         raise RuntimeError("box_convolution: linear float8 needs an input [..., K] and a weight [N, K] on one device, got %s and %s"
                            % (tuple(input.shape), tuple(weight.shape)))

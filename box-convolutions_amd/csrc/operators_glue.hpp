@@ -1,4 +1,4 @@
-// Host side of group_norm_act and linear_act in C++ (part of torch_glue.cpp): checks, allocations and autograd nodes around
+// Host side of group_norm_act, linear_act, residual_norm and the 8-bit product in C++ (part of torch_glue.cpp): checks, allocations and autograd nodes around
 // the C ABI's calls, as box_convolution/operators.py has them in Python. A training step of a small layer costs the Python
 // version 130 to 200 us of host time.
 #pragma once
@@ -8,6 +8,8 @@
 #include <algorithm>
 #include <cstdint>
 #include <optional>
+#include <tuple>
+#include <utility>
 
 namespace {
 
@@ -24,10 +26,26 @@ struct OperatorAbi {
                           void*, size_t, void*) = nullptr;
     int (*linear_backward)(const void*, int64_t, const void*, const void*, const void*, void*, void*, void*, void*, int, int64_t, int64_t, int64_t, int,
                            void*, size_t, void*) = nullptr;
+    size_t (*residual_bytes)(int64_t, int64_t, int, int, int) = nullptr;
+    int (*residual_forward)(const void*, const void*, const void*, int, int, float, int, const void*, const void*, const void*, const void*, int, float, void*,
+                            void*, void*, int, int64_t, int64_t, int, void*) = nullptr;
+    int (*residual_backward)(const void*, const void*, const void*, int, int, float, int, const void*, const void*, const void*, const void*, int, float,
+                             const void*, const void*, void*, void*, void*, void*, void*, void*, void*, int, int64_t, int64_t, int, void*, size_t, void*) = nullptr;
+    int (*quantize)(const void*, int64_t, int, int64_t, int64_t, void*, void*, void*) = nullptr;
+    size_t (*float8_bytes)(int64_t, int64_t, int64_t, int, int) = nullptr;
+    int (*float8_forward)(const void*, int64_t, int, const void*, const void*, const void*, const void*, const void*, int64_t, void*, int, int64_t, int64_t,
+                          int64_t, int, void*, size_t, void*) = nullptr;
 } g_operators;
 
 void init_operators(uint64_t norm_bytes, uint64_t norm_forward, uint64_t norm_backward, uint64_t linear_bytes, uint64_t linear_forward,
-                    uint64_t linear_backward) {
+                    uint64_t linear_backward, uint64_t residual_bytes, uint64_t residual_forward, uint64_t residual_backward, uint64_t quantize,
+                    uint64_t float8_bytes, uint64_t float8_forward) {
+    g_operators.residual_bytes = reinterpret_cast<decltype(g_operators.residual_bytes)>(residual_bytes);
+    g_operators.residual_forward = reinterpret_cast<decltype(g_operators.residual_forward)>(residual_forward);
+    g_operators.residual_backward = reinterpret_cast<decltype(g_operators.residual_backward)>(residual_backward);
+    g_operators.quantize = reinterpret_cast<decltype(g_operators.quantize)>(quantize);
+    g_operators.float8_bytes = reinterpret_cast<decltype(g_operators.float8_bytes)>(float8_bytes);
+    g_operators.float8_forward = reinterpret_cast<decltype(g_operators.float8_forward)>(float8_forward);
     g_operators.norm_bytes = reinterpret_cast<decltype(g_operators.norm_bytes)>(norm_bytes);
     g_operators.norm_forward = reinterpret_cast<decltype(g_operators.norm_forward)>(norm_forward);
     g_operators.norm_backward = reinterpret_cast<decltype(g_operators.norm_backward)>(norm_backward);
@@ -59,7 +77,7 @@ bool wants_grad(const at::Tensor& a, std::initializer_list<const Optional*> more
 // Neither the kernels nor the nodes know forward-mode derivatives: a tangent is refused, since dropping it would make it zero.
 void refuse_tangents(std::initializer_list<const at::Tensor*> tensors) {
     for (const at::Tensor* t : tensors)
-        TORCH_CHECK(!t->defined() || !t->_fw_grad(/*level=*/0).defined(), "box_convolution: group_norm_act and linear_act have no forward-mode derivative");
+        TORCH_CHECK(!t->defined() || !t->_fw_grad(/*level=*/0).defined(), "box_convolution: group_norm_act, linear_act and residual_norm have no forward-mode derivative");
 }
 const at::Tensor& or_undefined(const Optional& t) {
     static const at::Tensor none;
@@ -82,7 +100,7 @@ struct Once : public torch::autograd::Function<Once> {
         return grad.detach();
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext*, torch::autograd::variable_list) {
-        TORCH_CHECK(false, "box_convolution: group_norm_act and linear_act can be differentiated once, not twice");
+        TORCH_CHECK(false, "box_convolution: group_norm_act, linear_act and residual_norm can be differentiated once, not twice");
     }
 };
 
@@ -312,6 +330,236 @@ at::Tensor linear_act(const at::Tensor& input, const at::Tensor& weight, const O
     if (wants_grad(input, {&bias, &residual}) || (at::GradMode::is_enabled() && weight.requires_grad()))
         return LinearAct::apply(input, weight, bias, residual, act, stream);
     return LinearAct::call(input, weight.contiguous(), contiguous(bias), residual, static_cast<int>(act), stream, nullptr, nullptr);
+}
+
+// ---- between residual blocks ------------------------------------------------------------------------------------
+enum { kAfter = 1, kBefore = 2, kCentre = 4 };                 // BOXCONV_NORM_*
+enum { kNoGate = 0, kGateOfChannel = 1, kGateOfItem = 2, kGateOfElement = 3 };         // BOXCONV_GATE_*
+
+// What a call has besides its tensors.
+struct Between {
+    int gate_kind, norms;
+    double scale, eps;
+    int64_t stream;
+};
+
+struct ResidualNorm : public torch::autograd::Function<ResidualNorm> {
+    static int param_code(std::initializer_list<const Optional*> params) {
+        for (const Optional* p : params)
+            if (*p) return type_code((*p)->scalar_type());
+        return 0;
+    }
+    // Images in channels-last memory. `s` and `h` (values or codes, the latter with exponents) may be undefined.
+    static void call(const at::Tensor& x, const Optional& residual, const Optional& gate, const Optional& aw, const Optional& ab, const Optional& bw,
+                     const Optional& bb, const Between& b, const at::Tensor& s, const at::Tensor& h, const at::Tensor& exponents) {
+        if (x.numel() == 0) return;
+        const GroupNormAct::Sizes n = GroupNormAct::sizes(x);
+        const int code = type_code(x.scalar_type());
+        check_rc(g_operators.residual_forward(x.data_ptr(), address(residual), address(gate), b.gate_kind, gate ? type_code(gate->scalar_type()) : code,
+                                              static_cast<float>(b.scale), b.norms, address(aw), address(ab), address(bw), address(bb),
+                                              param_code({&aw, &ab, &bw, &bb}), static_cast<float>(b.eps), address(s), address(h), address(exponents), code, n.batch,
+                                              n.pixels, n.channels, reinterpret_cast<void*>(b.stream)),
+                 "residual_norm");
+    }
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& input, const Optional& residual, const Optional& gate,
+                                                  const Optional& after_weight, const Optional& after_bias, const Optional& before_weight,
+                                                  const Optional& before_bias, int64_t gate_kind, int64_t norms, double scale, double eps, bool want_stream,
+                                                  int64_t stream) {
+        const at::Tensor x = channels_last(input);
+        const Optional r = residual ? Optional(channels_last(*residual)) : std::nullopt;
+        const Optional g = !gate ? std::nullopt : Optional(gate_kind == kGateOfElement ? channels_last(*gate) : gate->contiguous());
+        const Optional aw = contiguous(after_weight), ab = contiguous(after_bias), bw = contiguous(before_weight), bb = contiguous(before_bias);
+        const at::Tensor s = want_stream ? empty_channels_last(x) : at::Tensor(), h = norms & kBefore ? empty_channels_last(x) : at::Tensor();
+        call(x, r, g, aw, ab, bw, bb, {static_cast<int>(gate_kind), static_cast<int>(norms), scale, eps, stream}, s, h, at::Tensor());
+        const auto or_none = [](const Optional& t) { return t.value_or(at::Tensor()); };
+        ctx->save_for_backward({x, or_none(r), or_none(g), or_none(aw), or_none(ab), or_none(bw), or_none(bb)});
+        ctx->set_materialize_grads(false);
+        ctx->saved_data["present"] = c10::List<bool>({true, residual.has_value(), gate.has_value(), after_weight.has_value(), after_bias.has_value(),
+                                                      before_weight.has_value(), before_bias.has_value()});
+        ctx->saved_data["gate_kind"] = gate_kind;
+        ctx->saved_data["norms"] = norms;
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["eps"] = eps;
+        ctx->saved_data["want_stream"] = want_stream;
+        ctx->saved_data["stream"] = stream;
+        torch::autograd::variable_list out;
+        if (s.defined()) out.push_back(s);
+        if (h.defined()) out.push_back(h);
+        return out;
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grad_outputs) {
+        for (const at::Tensor& g : grad_outputs) refuse_tangents({&g});
+        const auto saved = ctx->get_saved_variables();
+        const int gate_kind = static_cast<int>(ctx->saved_data["gate_kind"].toInt()), norms = static_cast<int>(ctx->saved_data["norms"].toInt());
+        const auto image = [](const at::Tensor& t) { return t.defined() ? channels_last(t) : at::Tensor(); };
+        const at::Tensor x = channels_last(saved[0]), residual = image(saved[1]);
+        const Optional gate = !saved[2].defined() ? std::nullopt : Optional(gate_kind == kGateOfElement ? channels_last(saved[2]) : saved[2].contiguous());
+        const Optional aw = saved_or_none(saved[3]), ab = saved_or_none(saved[4]), bw = saved_or_none(saved[5]), bb = saved_or_none(saved[6]);
+        const bool want_stream = ctx->saved_data["want_stream"].toBool();
+        const at::Tensor ds = want_stream ? image(grad_outputs[0]) : at::Tensor();
+        const at::Tensor dh = norms & kBefore ? image(grad_outputs[want_stream ? 1 : 0]) : at::Tensor();
+        const std::vector<bool> need = needed(ctx, ctx->saved_data["present"].toBoolList().vec());
+        torch::autograd::variable_list grads(13);              // one per argument of forward
+        const Optional* const vectors[] = {&gate, &aw, &ab, &bw, &bb};
+        for (int k = 0; k < 2; ++k)
+            if (need[k]) grads[k] = empty_channels_last(x);
+        for (int k = 0; k < 5; ++k)
+            if (need[k + 2]) grads[k + 2] = k == 0 && gate_kind == kGateOfElement ? empty_channels_last(x) : at::empty_like(**vectors[k]);
+        const at::Tensor& like = ds.defined() ? ds : dh.defined() ? dh : x;
+        if (x.numel() == 0) {
+            for (at::Tensor& g : grads)
+                if (g.defined()) g.zero_();
+            return once(grads, x, like);
+        }
+        const GroupNormAct::Sizes n = GroupNormAct::sizes(x);
+        const int code = type_code(x.scalar_type());
+        const size_t nbytes = g_operators.residual_bytes(n.batch, n.pixels, n.channels, gate_kind, code);
+        const at::Tensor ws = scratch(nbytes, x);
+        check_rc(g_operators.residual_backward(x.data_ptr(), address(residual), address(gate), gate_kind, gate ? type_code(gate->scalar_type()) : code,
+                                               static_cast<float>(ctx->saved_data["scale"].toDouble()), norms, address(aw), address(ab), address(bw), address(bb),
+                                               param_code({&aw, &ab, &bw, &bb}), static_cast<float>(ctx->saved_data["eps"].toDouble()), address(ds), address(dh),
+                                               address(grads[0]), address(grads[1]), address(grads[2]), address(grads[3]), address(grads[4]), address(grads[5]),
+                                               address(grads[6]), code, n.batch, n.pixels, n.channels, address(ws), nbytes,
+                                               reinterpret_cast<void*>(ctx->saved_data["stream"].toInt())),
+                 "residual_norm backward");
+        return once(grads, x, like);
+    }
+};
+
+// Codes (float8_e4m3fn) and exponents of rows of `columns` values, `shape` without its last entry in front.
+std::pair<at::Tensor, at::Tensor> empty_blocks(at::IntArrayRef shape, int64_t columns, const at::TensorOptions& options) {
+    const int64_t blocks = (columns + 127) / 128;
+    std::vector<int64_t> codes(shape.begin(), shape.end()), exponents = codes;
+    codes.back() = blocks * 128;
+    exponents.back() = (blocks + 3) / 4 * 4;
+    return {at::empty(codes, options.dtype(at::kFloat8_e4m3fn)), at::empty(exponents, options.dtype(at::kByte))};
+}
+
+// (stream, normed) as they are defined; with `quantize` (stream, codes, exponents). `after`, `before`: whether there are these norms.
+std::vector<at::Tensor> residual_norm(const at::Tensor& input, const Optional& residual, const Optional& gate, double scale, bool after,
+                                      const Optional& after_weight, const Optional& after_bias, bool before, const Optional& before_weight,
+                                      const Optional& before_bias, bool centre, double eps, bool quantize, int64_t stream) {
+    check_operator_input(input, "residual norm input");
+    refuse_tangents({&input, &or_undefined(residual), &or_undefined(gate), &or_undefined(after_weight), &or_undefined(after_bias), &or_undefined(before_weight),
+                     &or_undefined(before_bias)});
+    TORCH_CHECK(input.dim() >= 2 && input.size(1) >= 1, "box_convolution: residual norm input must have >=2 dimensions and a channel");
+    const int64_t B = input.size(0), C = input.size(1);
+    TORCH_CHECK(C <= INT32_MAX, "box_convolution: residual norm of ", C, " channels");
+    int gate_kind = kNoGate;
+    if (gate) {
+        gate_kind = gate->sizes() == input.sizes() ? kGateOfElement : gate->sizes() == at::IntArrayRef({C}) ? kGateOfChannel : gate->sizes() == at::IntArrayRef({B, C}) ? kGateOfItem : -1;
+        TORCH_CHECK(gate_kind >= 0, "box_convolution: gate must have the shape [C], [B, C] or that of the input, got ", gate->sizes(), " for an input of ", input.sizes());
+        TORCH_CHECK(gate->device() == input.device() && (gate->scalar_type() == input.scalar_type() || (gate->scalar_type() == at::kFloat && gate_kind != kGateOfElement)),
+                    "box_convolution: gate must be on ", input.device(), ", of the input's type or, where it has one value per channel, float32");
+    }
+    std::optional<at::ScalarType> kind;
+    for (const Optional* p : {&after_weight, &after_bias, &before_weight, &before_bias}) {
+        if (!*p) continue;
+        TORCH_CHECK((*p)->device() == input.device() && (*p)->dim() == 1 && (*p)->size(0) == C, "box_convolution: the parameters of a norm must hold ", C, " values on ",
+                    input.device());
+        const at::ScalarType t = (*p)->scalar_type();
+        TORCH_CHECK((t == at::kFloat || t == input.scalar_type()) && (!kind || *kind == t), "box_convolution: the norms' parameters must all be float32 or all of the input's type");
+        kind = t;
+    }
+    check_same(residual, input.sizes(), input, "residual");
+    const bool same = !residual && !gate && !after && scale == 1.0;
+    const bool recorded = wants_grad(input, {&residual, &gate, &after_weight, &after_bias, &before_weight, &before_bias});
+    TORCH_CHECK(!quantize || (before && !recorded), "box_convolution: quantize needs a norm before the next block, and is for inference only");
+    if (same && !before) return {input};
+    const int norms = kAfter * after | kBefore * before | kCentre * centre;
+    std::vector<at::Tensor> out;
+    if (same) out.push_back(input);
+    if (recorded) {
+        for (at::Tensor& t : ResidualNorm::apply(input, residual, gate, after_weight, after_bias, before_weight, before_bias, static_cast<int64_t>(gate_kind),
+                                                 static_cast<int64_t>(norms), scale, eps, !same, stream))
+            out.push_back(t);
+        return out;
+    }
+    const at::Tensor x = channels_last(input);
+    const at::Tensor s = same ? at::Tensor() : empty_channels_last(x);
+    if (!same) out.push_back(s);
+    at::Tensor h, exponents;
+    if (quantize) {
+        std::vector<int64_t> shape(1, B);
+        for (int64_t d = 2; d < x.dim(); ++d) shape.push_back(x.size(d));
+        shape.push_back(C);
+        std::tie(h, exponents) = empty_blocks(shape, C, x.options());
+        out.push_back(h);
+        out.push_back(exponents);
+    } else if (before) {
+        h = empty_channels_last(x);
+        out.push_back(h);
+    }
+    const Optional g = !gate ? std::nullopt : Optional(gate_kind == kGateOfElement ? channels_last(*gate) : gate->contiguous());
+    ResidualNorm::call(x, residual ? Optional(channels_last(*residual)) : std::nullopt, g, contiguous(after_weight), contiguous(after_bias), contiguous(before_weight),
+                       contiguous(before_bias), {gate_kind, norms, scale, eps, stream}, s, h, exponents);
+    return out;
+}
+
+// ---- 8 bits -------------------------------------------------------------------------------------------------------
+void refuse_gradients(const char* what, std::initializer_list<const Optional*> tensors) {
+    for (const Optional* t : tensors) {
+        TORCH_CHECK(!*t || !at::GradMode::is_enabled() || !(*t)->requires_grad(), "box_convolution: ", what,
+                    " is for inference only: it has no gradient (call it under torch.no_grad())");
+        refuse_tangents({&or_undefined(*t)});
+    }
+}
+
+int64_t rows_of(const at::Tensor& t) {
+    int64_t rows = 1;
+    for (int64_t d = 0; d + 1 < t.dim(); ++d) rows *= t.size(d);
+    return rows;
+}
+
+std::vector<at::Tensor> quantize_blocks(const at::Tensor& input, int64_t stream) {
+    check_operator_input(input, "quantize input");
+    TORCH_CHECK(input.dim() >= 1 && input.size(-1) >= 1, "box_convolution: quantize_blocks needs an input [..., K] with at least one column");
+    const Optional given(input);
+    refuse_gradients("quantize_blocks", {&given});
+    const int64_t rows = rows_of(input), K = input.size(-1);
+    auto [codes, exponents] = empty_blocks(input.sizes(), K, input.options());
+    if (rows > 0) {
+        const Rows x(input, rows, K);
+        check_rc(g_operators.quantize(x.hold.data_ptr(), x.ld, type_code(input.scalar_type()), rows, K, codes.data_ptr(), exponents.data_ptr(),
+                                      reinterpret_cast<void*>(stream)),
+                 "quantize_blocks");
+    }
+    return {codes, exponents};
+}
+
+// `input`: values, or codes with `exponents`. The shapes of blocks were looked at when they were made.
+at::Tensor linear_act_float8(const at::Tensor& input, const Optional& exponents, int64_t columns, const at::Tensor& weight, const at::Tensor& weight_exponents,
+                             int64_t weight_columns, const Optional& bias, const Optional& residual, int64_t act, std::optional<at::ScalarType> dtype, int64_t stream) {
+    if (!exponents) check_operator_input(input, "linear float8 input");
+    const at::ScalarType to = dtype ? *dtype : exponents ? at::kBFloat16 : input.scalar_type();
+    TORCH_CHECK((to == at::kFloat || to == at::kHalf || to == at::kBFloat16) && (exponents || to == input.scalar_type()),
+                "box_convolution: the result's type must be that of the values, or float32, float16 or bfloat16 for Float8Blocks, got ", to);
+    std::vector<int64_t> shape(input.sizes().begin(), input.sizes().end());
+    TORCH_CHECK(shape.size() >= 1 && weight.dim() == 2 && weight_columns == columns && weight.device() == input.device(),
+                "box_convolution: linear float8 needs an input [..., K] and a weight [N, K] on one device, got ", input.sizes(), " and ", weight.sizes());
+    const int64_t rows = rows_of(input), N = weight.size(0), K = columns;
+    shape.back() = N;
+    const auto options = input.options().dtype(to);
+    const auto check = [&](const Optional& t, at::IntArrayRef like, const char* name) {
+        TORCH_CHECK(!t || (t->sizes() == like && t->scalar_type() == to && t->device() == input.device()), "box_convolution: ", name, " must have the shape ", like,
+                    ", type ", to, " and device ", input.device(), ", got ", t ? t->sizes() : like, ", ", t ? t->scalar_type() : to, ", ", t ? t->device() : input.device());
+    };
+    check(bias, {N}, "bias");
+    check(residual, shape, "residual");
+    const Optional given = exponents ? std::nullopt : Optional(input);
+    refuse_gradients("linear_act_float8", {&given, &bias, &residual});
+    at::Tensor y = at::empty(shape, options);
+    if (y.numel() == 0) return y;
+    const std::optional<Rows> x = exponents ? std::nullopt : std::optional<Rows>(Rows(input, rows, K)), r = residual ? std::optional<Rows>(Rows(*residual, rows, N)) : std::nullopt;
+    const Optional b = contiguous(bias);
+    const int code = type_code(to), kind = exponents ? 8 : code;           // BOXCONV_E4M3
+    const size_t nbytes = g_operators.float8_bytes(rows, K, N, kind, code);
+    const at::Tensor ws = scratch(nbytes, input);
+    check_rc(g_operators.float8_forward(x ? x->hold.data_ptr() : input.data_ptr(), x ? x->ld : 0, kind, address(exponents), weight.data_ptr(),
+                                        weight_exponents.data_ptr(), address(b), r ? r->hold.data_ptr() : nullptr, r ? r->ld : 0, y.data_ptr(), code, rows, K, N,
+                                        static_cast<int>(act), address(ws), nbytes, reinterpret_cast<void*>(stream)),
+             "linear_float8");
+    return y;
 }
 
 }  // namespace

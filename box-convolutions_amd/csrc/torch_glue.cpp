@@ -319,4 +319,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("init_operators", &init_operators, "the same for the operators around a box convolution");
     m.def("group_norm_act", &group_norm_act, "box_convolution.group_norm_act, autograd node included");
     m.def("linear_act", &linear_act, "box_convolution.linear_act, autograd node included");
+    m.def("residual_norm", &residual_norm, "box_convolution.residual_norm, autograd node included");
+    m.def("quantize_blocks", &quantize_blocks, "the codes and exponents of box_convolution.quantize_blocks");
+    m.def("linear_act_float8", &linear_act_float8, "box_convolution.linear_act_float8");
 }
