@@ -637,6 +637,73 @@ hipError_t linear_backward(const LinearGradCall& c, void* workspace, hipStream_t
     return hipSuccess;
 }
 
+// ---- 8-bit rows ------------------------------------------------------------------------------------------------------
+namespace {
+
+template <class T, int TM, int TN, int WM, int WN>
+void launch_float8(const Coded& a, const Coded& b, const Tail<T>& tail, const ProductPlan& p, hipStream_t stream) {
+    constexpr size_t lds = kRing * sizeof(Chunk) * (TileShape<Code, true, TM, 8>::kChunks + TileShape<Code, true, TN, 8>::kChunks) + 2 * (TM + TN) * sizeof(unsigned);
+    BOXCONV_LAUNCH("linear_float8", (product_float8_kernel<T, TM, TN, WM, WN>), dim3(static_cast<unsigned>(p.tiles_m * p.tiles_n), p.splits), dim3(WM * WN * 64), lds, stream,
+                   a, b, tail, static_cast<int>(p.k_part / kBlock), static_cast<unsigned>(p.tiles_m), static_cast<unsigned>(p.tiles_n));
+}
+
+// The plan of 16-bit products, a stage of 128 bytes being a block here; parts of k are whole words of exponents. (Results in float32: no tiles of
+// 256 x 256, whose fragments do not fit the registers as bfloat16.)
+template <class T>
+ProductPlan plan_float8(int64_t rows, int64_t K, int64_t N) {
+    constexpr ProductShape kSmall[] = {kWide[1], kWide[2]};
+    ProductPlan p = sizeof(T) == 2 ? plan_product<Code>(kWide, rows, N, K, false) : plan_product<Code>(kSmall, rows, N, K, false);
+    if (sizeof(T) == 4) ++p.shape;
+    if (p.splits > 1) {
+        p.k_part = (p.k_part + 4 * kBlock - 1) / (4 * kBlock) * (4 * kBlock);
+        p.splits = static_cast<int>((K + p.k_part - 1) / p.k_part);
+        p.partial_bytes = p.splits > 1 ? static_cast<size_t>(p.splits) * rows * N * 4 : 0;
+    }
+    return p;
+}
+
+}  // namespace
+
+// [parts of a split product][the input's codes][their exponents]
+template <class T>
+size_t linear_float8_workspace(int64_t rows, int64_t K, int64_t N, bool values) {
+    return round_up(plan_float8<T>(rows, K, N).partial_bytes) + (values ? static_cast<size_t>(rows) * (blocks_of(K) * kBlock + exponents_of(K)) : 0);
+}
+
+template <class T>
+hipError_t linear_float8_forward(const LinearFloat8Call& c, void* workspace, hipStream_t stream) {
+    const ProductPlan p = plan_float8<T>(c.rows, c.K, c.N);
+    Coded a = {static_cast<const uint8_t*>(c.x), c.x_exponents, c.rows, static_cast<int>(blocks_of(c.K)), static_cast<int>(exponents_of(c.K))}, b = a;
+    if (c.input_dtype != kE4M3) {
+        QuantizeCall q = {c.x, c.ld_x, c.input_dtype, c.rows, c.K, static_cast<uint8_t*>(workspace) + round_up(p.partial_bytes), nullptr};
+        q.exponents = q.codes + c.rows * a.blocks * kBlock;
+        a.codes = q.codes;
+        a.exponents = q.exponents;
+        if (const hipError_t e = quantize_launch(q, stream); e != hipSuccess) return e;
+    }
+    b.codes = c.weight;
+    b.exponents = c.weight_exponents;
+    b.extent = c.N;
+    Tail<T> tail = {};
+    tail.out = static_cast<T*>(c.y);
+    tail.rows = c.rows;
+    tail.cols = c.N;
+    tail.bias = static_cast<const T*>(c.bias);
+    tail.residual = static_cast<const T*>(c.residual);
+    tail.ld_residual = c.ld_residual;
+    tail.activation = c.activation;
+    if (p.splits > 1) tail.partial = static_cast<float*>(workspace);
+    switch (p.shape) {
+        case 0:
+            if constexpr (sizeof(T) == 2) launch_float8<T, 256, 256, 4, 2>(a, b, tail, p, stream);
+            break;
+        case 1: launch_float8<T, 128, 128, 2, 2>(a, b, tail, p, stream); break;
+        default: launch_float8<T, 64, 64, 2, 2>(a, b, tail, p, stream);
+    }
+    if (p.splits > 1) join_parts(tail, p.splits, stream);
+    return hipGetLastError();
+}
+
 template size_t linear_forward_workspace<BOXCONV_INST_T>(int64_t, int64_t, int64_t);
 template size_t linear_backward_workspace<BOXCONV_INST_T>(int64_t, int64_t, int64_t);
 template hipError_t linear_forward<BOXCONV_INST_T>(const LinearCall&, void*, hipStream_t);
