@@ -8,29 +8,75 @@ namespace boxconv {
 
 namespace {
 
-// A wave takes a block, a lane two of its values.
-template <class T>
-__global__ void __launch_bounds__(256) quantize_kernel(QuantizeCall q, int64_t blocks, int64_t padded) {
-    const int l = threadIdx.x % 64;
-    for (int64_t id = blockIdx.x * 4ll + threadIdx.x / 64; id < q.rows * blocks; id += gridDim.x * 4ll) {
-        const int64_t row = id / blocks, b = id % blocks, c = b * kBlock + 2 * l;
-        const T* p = static_cast<const T*>(q.x) + row * q.ld;
-        const float v[2] = {c < q.columns ? static_cast<float>(p[c]) : 0.0f, c + 1 < q.columns ? static_cast<float>(p[c + 1]) : 0.0f};
-        const int e = block_exponent(most_of_lanes(largest(v), 64));
-        *reinterpret_cast<uint16_t*>(q.codes + id * kBlock + 2 * l) = static_cast<uint16_t>(to_codes(v, e)[0]);
-        if (l == 0) q.exponents[row * padded + b] = static_cast<uint8_t>(e);
-        if (b == blocks - 1 && l > 0 && b + l < padded) q.exponents[row * padded + b + l] = 127;
+// Eight lanes take a block, a lane 16 neighbouring values: whole 16-byte vectors in and out, the largest magnitude over the eight by moves within the
+// vector unit. kAhead blocks of a lane are requested before the first is used. I: a type that counts all blocks (64-bit divisions take dozens of
+// instructions).
+template <class T, class I>
+__global__ void __launch_bounds__(256) quantize_kernel(QuantizeCall q, I blocks, I padded, I total) {
+    constexpr int V = Vec<T>::kLen, PER = 16, NV = PER / V, kAhead = NV == 2 ? 4 : 2;
+    typedef typename Vec<T>::Type Packed;
+    const int sub = threadIdx.x % 8;
+    const I step = static_cast<I>(gridDim.x) * 32;
+    for (I first = blockIdx.x * static_cast<I>(32) + threadIdx.x / 8; first < total; first += kAhead * step) {
+        Packed raw[kAhead][NV];
+        int64_t row[kAhead];
+        I block[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const I id = min(static_cast<I>(first + i * step), static_cast<I>(total - 1));
+            row[i] = id / blocks;
+            block[i] = id - static_cast<I>(row[i]) * blocks;
+            const int64_t c = static_cast<int64_t>(block[i]) * kBlock + sub * PER, left = q.columns - c;
+            const T* p = static_cast<const T*>(q.x) + row[i] * q.ld + c;
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                if (left >= (v + 1) * V) raw[i][v] = *reinterpret_cast<const Packed*>(p + v * V);
+                else {
+                    Packed part = {};
+#pragma unroll
+                    for (int j = 0; j < V; ++j)
+                        if (v * V + j < left) part[j] = p[v * V + j];
+                    raw[i][v] = part;
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            float x[PER];
+#pragma unroll
+            for (int j = 0; j < PER; ++j) x[j] = static_cast<float>(raw[i][j / V][j % V]);
+            const int e = block_exponent(most_of_lanes(largest(x), 8));
+            if (first + i * step >= total) break;                  // (the same for all eight)
+            typedef unsigned Four __attribute__((ext_vector_type(4)));
+            const Codes<PER> codes = to_codes(x, e);
+            *reinterpret_cast<Four*>(q.codes + (row[i] * blocks + block[i]) * kBlock + sub * PER) = __builtin_bit_cast(Four, codes);
+            uint8_t* to = q.exponents + row[i] * padded + block[i];
+            if (sub == 0) to[0] = static_cast<uint8_t>(e);
+            else if (block[i] == blocks - 1 && block[i] + sub < padded) to[sub] = 127;
+        }
     }
 }
 
 }  // namespace
 
+namespace {
+
+template <class T>
+void quantize(const QuantizeCall& q, hipStream_t stream) {
+    const int64_t blocks = blocks_of(q.columns), padded = exponents_of(q.columns), total = q.rows * blocks;
+    const dim3 grid(static_cast<unsigned>(std::min<int64_t>((total + 31) / 32, 4096)));
+    if (total < (int64_t(1) << 30))
+        BOXCONV_LAUNCH("quantize", (quantize_kernel<T, unsigned>), grid, dim3(256), 0, stream, q, static_cast<unsigned>(blocks), static_cast<unsigned>(padded),
+                       static_cast<unsigned>(total));
+    else BOXCONV_LAUNCH("quantize", (quantize_kernel<T, int64_t>), grid, dim3(256), 0, stream, q, blocks, padded, total);
+}
+
+}  // namespace
+
 hipError_t quantize_launch(const QuantizeCall& q, hipStream_t stream) {
-    const int64_t blocks = blocks_of(q.columns), padded = exponents_of(q.columns), groups = std::min<int64_t>((q.rows * blocks + 3) / 4, 8192);
-    const dim3 grid(static_cast<unsigned>(groups));
-    if (q.dtype == kF32) BOXCONV_LAUNCH("quantize", (quantize_kernel<float>), grid, dim3(256), 0, stream, q, blocks, padded);
-    else if (q.dtype == kF16) BOXCONV_LAUNCH("quantize", (quantize_kernel<_Float16>), grid, dim3(256), 0, stream, q, blocks, padded);
-    else BOXCONV_LAUNCH("quantize", (quantize_kernel<__bf16>), grid, dim3(256), 0, stream, q, blocks, padded);
+    if (q.dtype == kF32) quantize<float>(q, stream);
+    else if (q.dtype == kF16) quantize<_Float16>(q, stream);
+    else quantize<__bf16>(q, stream);
     return hipGetLastError();
 }
 

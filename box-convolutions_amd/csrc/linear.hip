@@ -79,7 +79,6 @@ product_kernel(Operand<T> a, Operand<T> b, Tail<T> tail, int64_t k_part, int64_t
 // y for at most 16 * MT rows: the weight is all there is to read, once. A workgroup takes 16 columns n and its waves share k, each
 // with as many 16-byte loads of the weight in flight as it has; their sums meet in LDS. (16 x 16 matrix instructions: the weight's
 // rows are the first operand, so that a lane ends up with four consecutive n of one row.)
-typedef float Acc4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ Acc4 multiply_add16(Chunk b, Chunk a, Acc4 c, __bf16) {
     typedef __bf16 Eight __attribute__((ext_vector_type(8)));
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(Eight, b), __builtin_bit_cast(Eight, a), c, 0, 0, 0);
@@ -662,28 +661,32 @@ ProductPlan plan_float8(int64_t rows, int64_t K, int64_t N) {
     return p;
 }
 
+constexpr int64_t kFewRows = 32;           // whose product takes one launch, values or codes
+
+template <class T, int MT, bool CODED>
+hipError_t few_rows_float8(const LinearFloat8Call& c, const Coded& a, const Coded& b, const Tail<T>& tail, hipStream_t stream) {
+    int waves = 1, ahead = 1;              // all waves with a block at least, then up to four blocks on their way for each
+    while (waves < (MT == 1 ? 8 : 4) && waves < a.blocks) waves *= 2;
+    while (ahead < 4 && ahead * waves < a.blocks) ahead *= 2;
+    const size_t lds = std::max<size_t>(static_cast<size_t>(waves) * 16 * (CODED ? MT + 1 : 1) * ahead * kBlock, static_cast<size_t>(waves) * MT * 1024);
+    BOXCONV_LAUNCH("linear_float8_few_rows", (few_rows_float8_kernel<T, MT, CODED>), dim3(static_cast<unsigned>((c.N + 15) / 16)), dim3(waves * 64), lds, stream, a,
+                   static_cast<const T*>(c.x), c.ld_x, c.K, b, tail, ahead);
+    return hipGetLastError();
+}
+
 }  // namespace
 
 // [parts of a split product][the input's codes][their exponents]
 template <class T>
 size_t linear_float8_workspace(int64_t rows, int64_t K, int64_t N, bool values) {
+    if (rows <= kFewRows) return 0;
     return round_up(plan_float8<T>(rows, K, N).partial_bytes) + (values ? static_cast<size_t>(rows) * (blocks_of(K) * kBlock + exponents_of(K)) : 0);
 }
 
 template <class T>
 hipError_t linear_float8_forward(const LinearFloat8Call& c, void* workspace, hipStream_t stream) {
-    const ProductPlan p = plan_float8<T>(c.rows, c.K, c.N);
-    Coded a = {static_cast<const uint8_t*>(c.x), c.x_exponents, c.rows, static_cast<int>(blocks_of(c.K)), static_cast<int>(exponents_of(c.K))}, b = a;
-    if (c.input_dtype != kE4M3) {
-        QuantizeCall q = {c.x, c.ld_x, c.input_dtype, c.rows, c.K, static_cast<uint8_t*>(workspace) + round_up(p.partial_bytes), nullptr};
-        q.exponents = q.codes + c.rows * a.blocks * kBlock;
-        a.codes = q.codes;
-        a.exponents = q.exponents;
-        if (const hipError_t e = quantize_launch(q, stream); e != hipSuccess) return e;
-    }
-    b.codes = c.weight;
-    b.exponents = c.weight_exponents;
-    b.extent = c.N;
+    Coded a = {static_cast<const uint8_t*>(c.x), c.x_exponents, c.rows, static_cast<int>(blocks_of(c.K)), static_cast<int>(exponents_of(c.K))};
+    const Coded b = {c.weight, c.weight_exponents, c.N, a.blocks, a.padded};
     Tail<T> tail = {};
     tail.out = static_cast<T*>(c.y);
     tail.rows = c.rows;
@@ -692,6 +695,19 @@ hipError_t linear_float8_forward(const LinearFloat8Call& c, void* workspace, hip
     tail.residual = static_cast<const T*>(c.residual);
     tail.ld_residual = c.ld_residual;
     tail.activation = c.activation;
+    const bool coded = c.input_dtype == kE4M3;
+    if (c.rows <= kFewRows) {
+        if (c.rows <= 16) return coded ? few_rows_float8<T, 1, true>(c, a, b, tail, stream) : few_rows_float8<T, 1, false>(c, a, b, tail, stream);
+        return coded ? few_rows_float8<T, 2, true>(c, a, b, tail, stream) : few_rows_float8<T, 2, false>(c, a, b, tail, stream);
+    }
+    const ProductPlan p = plan_float8<T>(c.rows, c.K, c.N);
+    if (!coded) {
+        QuantizeCall q = {c.x, c.ld_x, c.input_dtype, c.rows, c.K, static_cast<uint8_t*>(workspace) + round_up(p.partial_bytes), nullptr};
+        q.exponents = q.codes + c.rows * a.blocks * kBlock;
+        a.codes = q.codes;
+        a.exponents = q.exponents;
+        if (const hipError_t e = quantize_launch(q, stream); e != hipSuccess) return e;
+    }
     if (p.splits > 1) tail.partial = static_cast<float*>(workspace);
     switch (p.shape) {
         case 0:

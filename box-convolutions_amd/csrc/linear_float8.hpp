@@ -25,31 +25,39 @@ struct Codes32 { Chunk lo, hi; };
 // is). That is 1e-5 to 4e-5 of a sum of random signs, far below half a step of the 16-bit types. Results in float32 take the bfloat16
 // instructions instead, at half the rate: codes and powers of two fit that type, and its products add up in float32.
 typedef int Eight __attribute__((ext_vector_type(8)));
+typedef __bf16 Run __attribute__((ext_vector_type(8)));
+typedef float Acc4 __attribute__((ext_vector_type(4)));
+
+// Codes 8 i to 8 i + 7 times their block's power.
+__device__ __forceinline__ Run as_bfloat16(const Codes32& v, int exponent, int i) {
+    typedef __bf16 Pair __attribute__((ext_vector_type(2)));
+    const float power = __builtin_bit_cast(float, (static_cast<unsigned>(exponent) & 255) << 23);
+    const Chunk from = i < 2 ? v.lo : v.hi;
+    Run out;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const unsigned word = from[i % 2 * 2 + j / 2];
+        const Pair two = j % 2 == 0 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(word, power, false) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(word, power, true);
+        out[2 * j] = two[0];
+        out[2 * j + 1] = two[1];
+    }
+    return out;
+}
+
+// 32 x 32 results, 64 values of k; 16 x 16, 128. The low byte of an exponent counts.
 template <class T>
 __device__ __forceinline__ Acc16 multiply_add8(const Codes32& b, int eb, const Codes32& a, int ea, Acc16 c) {
-    typedef __bf16 Pair __attribute__((ext_vector_type(2)));
-    typedef __bf16 Run __attribute__((ext_vector_type(8)));
-    if constexpr (sizeof(T) == 2) {
-        const auto join = [](const Codes32& v) { return __builtin_bit_cast(Eight, v); };
-        return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(join(b), join(a), c, 0, 0, 0, eb, 0, ea);
-    } else {
-        const auto wide = [](const Codes32& v, int e, int i) {             // eight codes as bfloat16
-            const float power = __builtin_bit_cast(float, (static_cast<unsigned>(e) & 255) << 23);
-            const Chunk from = i < 2 ? v.lo : v.hi;
-            Run out;
+    if constexpr (sizeof(T) == 2) return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(__builtin_bit_cast(Eight, b), __builtin_bit_cast(Eight, a), c, 0, 0, 0, eb, 0, ea);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const unsigned word = from[i % 2 * 2 + j / 2];
-                const Pair two = j % 2 == 0 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(word, power, false) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(word, power, true);
-                out[2 * j] = two[0];
-                out[2 * j + 1] = two[1];
-            }
-            return out;
-        };
+    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bfloat16(b, eb, i), as_bfloat16(a, ea, i), c, 0, 0, 0);
+    return c;
+}
+template <class T>
+__device__ __forceinline__ Acc4 multiply_add8(const Codes32& b, int eb, const Codes32& a, int ea, Acc4 c) {
+    if constexpr (sizeof(T) == 2) return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(__builtin_bit_cast(Eight, b), __builtin_bit_cast(Eight, a), c, 0, 0, 0, eb, 0, ea);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wide(b, eb, i), wide(a, ea, i), c, 0, 0, 0);
-        return c;
-    }
+    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bfloat16(b, eb, i), as_bfloat16(a, ea, i), c, 0, 0, 0);
+    return c;
 }
 
 // A byte as an operand's element, for the tiles and the feed of the wide kernels.
@@ -171,6 +179,96 @@ product_float8_kernel(Coded a, Coded b, Tail<T> tail, int part_blocks, unsigned 
     settle<0>();                                               // every wave's loads have landed and its fragments are read: the LDS is free
     static_assert(WM * WN * 256 * FN <= kRing * kStage, "each wave turns its sums in a part of the stages");
     store_blocks<T, FN, FM>(tail, acc, m0 + wm, n0 + wn, part, stages + wave * 256 * FN);
+}
+
+// ---- few rows --------------------------------------------------------------------------------------------------------
+// y for at most 16 * MT rows: the weight's codes are all there is to read, once. A workgroup takes 16 columns n and its waves share k. A wave
+// brings `ahead` blocks of its 16 rows of the weight to LDS at a time (fragments read straight from memory would touch four times as many cache
+// lines per load), and reads its fragments there. CODED: x is codes, which come the same way; else values, quantized on the way in registers: the
+// four lanes that hold a row's share of a block agree on its exponent. That saves a launch, and the few rows come from the caches.
+template <class T>
+__device__ __forceinline__ void quantize_share(const T* p, int64_t left, Codes32& codes, int& exponent) {
+    float v[32];
+    constexpr int V = Vec<T>::kLen;
+#pragma unroll
+    for (int i = 0; i < 32; i += V) {
+        T part[V];
+        load_run<T, V>(p + i, part, left - i);
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[i + j] = static_cast<float>(part[j]);
+    }
+    float most = largest(v);
+    most = fmaxf(most, partner<16>(most));
+    most = fmaxf(most, partner<32>(most));
+    exponent = block_exponent(most);
+    const Codes<32> c = to_codes(v, exponent);
+    codes = __builtin_bit_cast(Codes32, c);
+}
+
+template <class T, int MT, bool CODED>
+__global__ void __launch_bounds__(512)
+few_rows_float8_kernel(Coded a, const T* x, int64_t ld_x, int64_t columns, Coded b, Tail<T> tail, int ahead) {
+    extern __shared__ Chunk blocks[];
+    const int l = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), waves = blockDim.x / 64;
+    const int64_t n0 = blockIdx.x * 16ll;
+    const int count = a.blocks, part = (count + waves - 1) / waves, last = min(count, (wave + 1) * part);
+    constexpr int kRows = 16 * (CODED ? MT + 1 : 1);           // rows of the weight, then of x
+    Chunk* const mine = blocks + wave * kRows * 8 * ahead;
+    const unsigned to = static_cast<unsigned>(reinterpret_cast<uintptr_t>((LdsVoid)mine));
+    const int ld = count * kBlock, rows_w = static_cast<int>(min<int64_t>(16, b.extent - n0)), rows_x = static_cast<int>(a.extent);
+    const auto describe = [](const uint8_t* p, int64_t size) {
+        const uint64_t at = reinterpret_cast<uint64_t>(p);
+        return Descriptor{__builtin_amdgcn_readfirstlane(static_cast<int>(at)), __builtin_amdgcn_readfirstlane(static_cast<int>(at >> 32) & 0xffff),
+                          __builtin_amdgcn_readfirstlane(static_cast<int>(size)), 0x00020000};
+    };
+    const Descriptor dw = describe(b.codes + n0 * ld, static_cast<int64_t>(rows_w) * ld), dx = describe(a.codes, CODED ? static_cast<int64_t>(rows_x) * ld : 0);
+    const uint8_t* w_exponents = b.exponents + min(n0 + l % 16, b.extent - 1) * b.padded;
+    Acc4 acc[MT] = {};
+    for (int s = wave * part; s < last; s += ahead) {
+        // chunk c of row r lies at c ^ r, whose low bits keep neighbouring rows in different banks
+        const int chunks = 8 * ahead, mask = chunks - 1;
+        for (int i = 0; i < kRows * ahead / 8; ++i) {
+            const int q = i * 64 + l, r = q / chunks, c = (q & mask) ^ (r & mask), k = s * kBlock + c * 16, row = r < 16 ? r : r - 16;
+            const bool inside = k < ld && row < (r < 16 ? rows_w : rows_x);
+            load_to_lds(i * 64 / chunks < 16 ? dw : dx, inside ? static_cast<unsigned>(row * ld + k) : kNowhere, __builtin_amdgcn_readfirstlane(to + i * 1024));
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");       // (a wave's blocks are its own)
+        for (int j = 0; j < ahead && s + j < last; ++j) {
+            const int r = l % 16, c = 8 * j + l / 16 * 2;
+            const auto from_lds = [&](int row) { return Codes32{mine[row * chunks + (c ^ (row & mask))], mine[row * chunks + ((c + 1) ^ (row & mask))]}; };
+            const Codes32 w = from_lds(r);
+            const int ew = w_exponents[s + j];
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                Codes32 v;
+                int e;
+                if constexpr (CODED) {
+                    v = from_lds(16 + 16 * i + r);
+                    e = a.exponents[min(16 * i + r, rows_x - 1) * a.padded + s + j];
+                } else {
+                    const int64_t k = static_cast<int64_t>(s + j) * kBlock + l / 16 * 32;
+                    // (rows beyond the end repeat the last one: nobody stores their sums)
+                    quantize_share(x + min(16 * i + r, rows_x - 1) * ld_x + k, columns - k, v, e);
+                }
+                acc[i] = multiply_add8<T>(w, ew, v, e, acc[i]);
+            }
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");     // read before the next blocks overwrite them
+    }
+    __syncthreads();
+    Acc4* sums = reinterpret_cast<Acc4*>(blocks);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) sums[(wave * MT + i) * 64 + l] = acc[i];
+    __syncthreads();
+    for (int i = wave; i < MT; i += waves) {
+        float z[4] = {};
+        for (int w = 0; w < waves; ++w) {
+            const Acc4 v = sums[(w * MT + i) * 64 + l];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) z[r] += v[r];
+        }
+        apply_tail<T, 4>(tail, z, 16 * i + l % 16, n0 + 4 * (l / 16));
+    }
 }
 
 }  // namespace
