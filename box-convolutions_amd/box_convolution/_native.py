@@ -901,7 +901,7 @@ KERNEL_NAMES = ("band_colsum", "band_prefix", "band_scan", "forward_rows", "forw
                 "int_col_prefix", "norm_statistics", "norm_join", "norm_apply", "norm_small", "norm_any_statistics", "norm_any_apply", "norm_sums",
                 "norm_join_sums", "norm_grad", "norm_small_grad", "norm_parameter", "norm_any_sums", "norm_any_grad", "linear", "linear_few_rows",
                 "linear_dx", "linear_dweight", "linear_narrow_grad", "linear_slope", "join_parts", "join_bias", "norm_rows", "norm_rows_grad", "join_rows",
-                "quantize", "linear_float8", "linear_float8_few_rows")
+                "quantize", "linear_float8", "linear_float8_few_rows", "linear_float8_narrow")
 
 
 def reload_switches():

@@ -674,12 +674,43 @@ hipError_t few_rows_float8(const LinearFloat8Call& c, const Coded& a, const Code
     return hipGetLastError();
 }
 
+// Sizes of narrow_float8_kernel.
+template <class T>
+bool narrow_float8(int64_t rows, int64_t K, int64_t N, bool coded) {
+    return rows >= 65536 && blocks_of(K) <= (coded ? kNarrowBlocks : K % kBlock == 0 ? 2 : 1) && K >= Vec<T>::kLen &&
+           N * blocks_of(K) * kBlock <= static_cast<int64_t>(kNarrowWeight);
+}
+
+template <class T, int KB, bool CODED, bool WHOLE>
+void launch_narrow_float8(const LinearFloat8Call& c, const Coded& a, const Coded& b, const Tail<T>& tail, hipStream_t stream) {
+    const size_t lds = narrow_float8_lds(c.N, KB);
+    const int64_t groups = (c.rows + kNarrowWaves * 32 - 1) / (kNarrowWaves * 32), resident = std::min<int64_t>(4, static_cast<int64_t>(kMaxDynamicLds / lds)) * 256;
+    BOXCONV_LAUNCH("linear_float8_narrow", (narrow_float8_kernel<T, KB, CODED, WHOLE>), dim3(static_cast<unsigned>(std::min(groups, resident))), dim3(kNarrowWaves * 64), lds,
+                   stream, a, static_cast<const T*>(c.x), c.ld_x, c.K, b, tail);
+}
+template <class T, bool CODED>
+hipError_t run_narrow_float8(const LinearFloat8Call& c, const Coded& a, const Coded& b, const Tail<T>& tail, hipStream_t stream) {
+    if constexpr (CODED) {
+        switch (a.blocks) {
+            case 1: launch_narrow_float8<T, 1, true, true>(c, a, b, tail, stream); break;
+            case 2: launch_narrow_float8<T, 2, true, true>(c, a, b, tail, stream); break;
+            case 3: launch_narrow_float8<T, 3, true, true>(c, a, b, tail, stream); break;
+            default: launch_narrow_float8<T, 4, true, true>(c, a, b, tail, stream);
+        }
+    } else {
+        if (c.K % kBlock != 0) launch_narrow_float8<T, 1, false, false>(c, a, b, tail, stream);
+        else if (a.blocks == 1) launch_narrow_float8<T, 1, false, true>(c, a, b, tail, stream);
+        else launch_narrow_float8<T, 2, false, true>(c, a, b, tail, stream);
+    }
+    return hipGetLastError();
+}
+
 }  // namespace
 
 // [parts of a split product][the input's codes][their exponents]
 template <class T>
 size_t linear_float8_workspace(int64_t rows, int64_t K, int64_t N, bool values) {
-    if (rows <= kFewRows) return 0;
+    if (rows <= kFewRows || narrow_float8<T>(rows, K, N, !values)) return 0;
     return round_up(plan_float8<T>(rows, K, N).partial_bytes) + (values ? static_cast<size_t>(rows) * (blocks_of(K) * kBlock + exponents_of(K)) : 0);
 }
 
@@ -700,6 +731,7 @@ hipError_t linear_float8_forward(const LinearFloat8Call& c, void* workspace, hip
         if (c.rows <= 16) return coded ? few_rows_float8<T, 1, true>(c, a, b, tail, stream) : few_rows_float8<T, 1, false>(c, a, b, tail, stream);
         return coded ? few_rows_float8<T, 2, true>(c, a, b, tail, stream) : few_rows_float8<T, 2, false>(c, a, b, tail, stream);
     }
+    if (narrow_float8<T>(c.rows, c.K, c.N, coded)) return coded ? run_narrow_float8<T, true>(c, a, b, tail, stream) : run_narrow_float8<T, false>(c, a, b, tail, stream);
     const ProductPlan p = plan_float8<T>(c.rows, c.K, c.N);
     if (!coded) {
         QuantizeCall q = {c.x, c.ld_x, c.input_dtype, c.rows, c.K, static_cast<uint8_t*>(workspace) + round_up(p.partial_bytes), nullptr};

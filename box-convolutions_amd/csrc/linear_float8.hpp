@@ -80,7 +80,7 @@ product_float8_kernel(Coded a, Coded b, Tail<T> tail, int part_blocks, unsigned 
     typedef TileShape<Code, true, TN, 8> SB;
     constexpr int THREADS = WM * WN * 64, FM = TM / WM / 32, FN = TN / WN / 32;
     constexpr int kStage = SA::kChunks + SB::kChunks;
-    static_assert(THREADS >= TM + TN && TM % 64 == 0 && SA::KT == kBlock, "a thread per row of exponents, whole waves of them; a block a stage");
+    static_assert(TM % 64 == 0 && TN % 64 == 0 && SA::KT == kBlock, "whole waves of rows; a block a stage");
     extern __shared__ Chunk stages[];
     unsigned* const words = reinterpret_cast<unsigned*>(stages + kRing * kStage);          // [2][TM + TN]
     unsigned tm, tn, part;
@@ -96,17 +96,25 @@ product_float8_kernel(Coded a, Coded b, Tail<T> tail, int part_blocks, unsigned 
     const int64_t row_bytes = static_cast<int64_t>(a.blocks) * kBlock;
     fa.start({reinterpret_cast<const Code*>(a.codes), row_bytes, a.extent, row_bytes}, m0, static_cast<int64_t>(first) * kBlock);
     fb.start({reinterpret_cast<const Code*>(b.codes), row_bytes, b.extent, row_bytes}, n0, static_cast<int64_t>(first) * kBlock);
-    // the exponents of this wave's 64 rows of the tile
-    const bool of_a = wave * 64 < TM;
-    const int64_t row0 = of_a ? m0 + wave * 64 : n0 + wave * 64 - TM, rows = (of_a ? a.extent : b.extent) - row0;
-    const uint64_t at = reinterpret_cast<uint64_t>((of_a ? a.exponents : b.exponents) + row0 * a.padded);
+    // exponents: 64 rows of the tile at a time, one or two times a wave
+    constexpr int kWaves = WM * WN, kPieces = (TM + TN) / 64, kOwn = (kPieces + kWaves - 1) / kWaves;
     const auto scalar = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
-    const Descriptor dw = {scalar(static_cast<int>(at)), scalar(static_cast<int>(at >> 32) & 0xffff),
-                           scalar(rows <= 0 ? 0 : static_cast<int>(min<int64_t>(rows, 64)) * a.padded), 0x00020000};
+    Descriptor dw[kOwn];
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+        const int piece = wave + i * kWaves;
+        const bool of_a = piece * 64 < TM;
+        const int64_t row0 = of_a ? m0 + piece * 64 : n0 + piece * 64 - TM, rows = (of_a ? a.extent : b.extent) - row0;
+        const uint64_t at = reinterpret_cast<uint64_t>((of_a ? a.exponents : b.exponents) + row0 * a.padded);
+        dw[i] = {scalar(static_cast<int>(at)), scalar(static_cast<int>(at >> 32) & 0xffff), scalar(rows <= 0 ? 0 : static_cast<int>(min<int64_t>(rows, 64)) * a.padded),
+                 0x00020000};
+    }
     const auto load_words = [&](int group) {                   // (beyond the end: zeros, which nobody uses)
-        if (wave * 64 < TM + TN)
-            word_to_lds(dw, 4 * group < a.padded ? static_cast<unsigned>(l * a.padded + 4 * group) : kNowhere,
-                        scalar(static_cast<int>(reinterpret_cast<uintptr_t>((LdsVoid)(words + (group & 1) * (TM + TN)))) + wave * 256));
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i)
+            if (wave + i * kWaves < kPieces)
+                word_to_lds(dw[i], 4 * group < a.padded ? static_cast<unsigned>(l * a.padded + 4 * group) : kNowhere,
+                            scalar(static_cast<int>(reinterpret_cast<uintptr_t>((LdsVoid)(words + (group & 1) * (TM + TN)))) + (wave + i * kWaves) * 256));
     };
     Descriptor da, db;
     const auto load = [&](int s, int i) {
@@ -142,7 +150,9 @@ product_float8_kernel(Coded a, Coded b, Tail<T> tail, int part_blocks, unsigned 
                 for (int i = p * kLoads / kProducts; i < (p + 1) * kLoads / kProducts; ++i) load(to, i);
             }
             acc[p / FM][p % FM] = multiply_add8<T>(xb[slot(h, p / FM)], eb[p / FM], xa[h][p % FM], ea[p % FM], acc[p / FM][p % FM]);
-            asm volatile("" : "+v"(acc[p / FM][p % FM]));      // (keeps the product here: it would be moved behind all loads and reads of the stage, and spill)
+            // (keeps the product here: it would be moved behind all loads and reads of the stage, and spill)
+            if constexpr (kProducts > 8) asm volatile("" : "+a"(acc[p / FM][p % FM]));
+            else asm volatile("" : "+v"(acc[p / FM][p % FM]));
             __builtin_amdgcn_sched_barrier(0);
         }
     };
@@ -268,6 +278,96 @@ few_rows_float8_kernel(Coded a, const T* x, int64_t ld_x, int64_t columns, Coded
             for (int r = 0; r < 4; ++r) z[r] += v[r];
         }
         apply_tail<T, 4>(tail, z, 16 * i + l % 16, n0 + 4 * (l / 16));
+    }
+}
+
+// ---- few channels ----------------------------------------------------------------------------------------------------
+// y of many rows through a weight of at most KB blocks a row that LDS holds whole. A wave takes 32 rows at a time with all their columns: its
+// lanes read the row's values (or, CODED, its codes) once, two lanes a row, and quantize them in registers; the codes never go through memory.
+// Then 32 columns at a time: products, epilogue. Workgroups of eight waves go round over the rows. WHOLE: rows of values end with a block.
+constexpr int kNarrowBlocks = 4, kNarrowWaves = 8;         // (a row's exponents are one word)
+constexpr size_t kNarrowWeight = 64 * 1024;
+constexpr size_t narrow_float8_lds(int64_t columns, int blocks) { return static_cast<size_t>((columns + 31) / 32 * 32) * (blocks * kBlock + 4) + kNarrowWaves * 4096; }
+
+template <class T, int KB, bool CODED, bool WHOLE>
+__global__ void __launch_bounds__(kNarrowWaves * 64, KB == 1 && WHOLE && sizeof(T) == 2 ? 4 : 2)
+narrow_float8_kernel(Coded a, const T* x, int64_t ld_x, int64_t columns, Coded b, Tail<T> tail) {
+    typedef TileShape<Code, true, 32, 8> Tile;
+    extern __shared__ Chunk lds[];
+    const int l = threadIdx.x % 64, wave = threadIdx.x / 64, rows_w = static_cast<int>(b.extent + 31) / 32 * 32;
+    Chunk* const turn = lds + wave * 256;                      // where a wave turns its sums
+    Chunk* const weight = lds + kNarrowWaves * 256;            // [KB][rows_w][8]
+    unsigned* const words = reinterpret_cast<unsigned*>(weight + KB * rows_w * 8);
+    for (int i = threadIdx.x; i < KB * rows_w * 8; i += kNarrowWaves * 64) {
+        const int row = i / (KB * 8), c = i % (KB * 8);
+        const Chunk v = row < b.extent ? *reinterpret_cast<const Chunk*>(b.codes + (row * KB * 8 + c) * 16ll) : Chunk{0, 0, 0, 0};
+        weight[c / 8 * rows_w * 8 + Tile::place<true>(row, c % 8)] = v;
+    }
+    for (int i = threadIdx.x; i < rows_w; i += kNarrowWaves * 64) words[i] = i < b.extent ? *reinterpret_cast<const unsigned*>(b.exponents + i * 4ll) : 0x7f7f7f7fu;
+    __syncthreads();
+    for (int64_t m0 = (blockIdx.x * static_cast<int64_t>(kNarrowWaves) + wave) * 32; m0 < a.extent; m0 += gridDim.x * static_cast<int64_t>(kNarrowWaves * 32)) {
+        // (rows beyond the end repeat the last one: nobody stores their sums)
+        const int64_t m = min(m0 + l % 32, a.extent - 1);
+        Codes32 codes[KB][2];
+        int ea[KB];
+        if constexpr (CODED) {
+            const unsigned word = *reinterpret_cast<const unsigned*>(a.exponents + m * 4);
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) {
+                ea[kb] = static_cast<int>(word >> 8 * kb);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const Chunk* p = reinterpret_cast<const Chunk*>(a.codes + m * (KB * kBlock) + kb * kBlock) + 4 * h + l / 32;
+                    codes[kb][h] = {p[0], p[2]};
+                }
+            }
+        } else {
+            const T* p = x + m * ld_x;
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) {
+                // chunks l / 32 and l / 32 + 2 of each half, as the weight's fragments have them
+                float v[64];
+                constexpr int V = Vec<T>::kLen;
+                typename Vec<T>::Type raw[64 / V] = {};
+                const auto k_of = [&](int i) { return kb * kBlock + i * V / 16 * 32 + l / 32 * 16 + i * V % 16; };
+                if constexpr (WHOLE) {
+#pragma unroll
+                    for (int i = 0; i < 64 / V; ++i) raw[i] = *reinterpret_cast<const typename Vec<T>::Type*>(p + k_of(i));
+                } else {                                       // (rows hold a vector at least)
+                    Chunk part[64 / V];
+#pragma unroll
+                    for (int i = 0; i < 64 / V; ++i) part[i] = request_chunk(p + k_of(i), static_cast<int>(columns) - k_of(i), x);
+#pragma unroll
+                    for (int i = 0; i < 64 / V; ++i) {
+                        settle_chunk<T>(part[i], static_cast<int>(columns) - k_of(i));
+                        raw[i] = __builtin_bit_cast(typename Vec<T>::Type, part[i]);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 64; ++i) v[i] = static_cast<float>(raw[i / V][i % V]);
+                float most = largest(v);
+                most = fmaxf(most, partner<32>(most));
+                ea[kb] = block_exponent(most);
+                const Codes<64> c = to_codes(v, ea[kb]);
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    codes[kb][h] = {Chunk{c[8 * h], c[8 * h + 1], c[8 * h + 2], c[8 * h + 3]}, Chunk{c[8 * h + 4], c[8 * h + 5], c[8 * h + 6], c[8 * h + 7]}};
+            }
+        }
+        for (int n0 = 0; n0 < b.extent; n0 += 32) {
+            Acc16 acc[1][1] = {};
+            const unsigned word = words[n0 + column_of(l % 32)];
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) {
+                const Chunk* tile = weight + kb * rows_w * 8;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const Codes32 w = {fragment<Code, true, 32, 8, true>(tile, n0, 2 * h), fragment<Code, true, 32, 8, true>(tile, n0, 2 * h + 1)};
+                    acc[0][0] = multiply_add8<T>(w, static_cast<int>(word >> 8 * kb), codes[kb][h], ea[kb], acc[0][0]);
+                }
+            }
+            store_blocks<T, 1, 1>(tail, acc, m0, n0, 0, turn);
+        }
     }
 }
 

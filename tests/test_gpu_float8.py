@@ -156,6 +156,20 @@ def test_large_products(hip, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,K,N", [(65536, 128, 32), (65600, 100, 40), (70001, 256, 33), (65543, 8, 5), (66000, 300, 72), (65536, 512, 24), (65537, 130, 8)])
+def test_many_rows_through_few_channels(hip, M, K, N, dtype):
+    args = case(M, K, N, dtype, ACTS[(M + K) % 4], residual=K % 3 == 0)
+    want = expected(*args)
+    for coded in (False, True):
+        check(run(*args, coded), want)
+    x, w = args[:2]
+    x[M - 1, 3], x[5, K - 1], w[N - 1, 0] = float("nan"), float("inf"), float("nan")
+    bad = run(x, w, None, None, None, False)["y"].isnan().cpu()
+    rows_, columns = bad.all(1).nonzero().flatten().tolist(), bad.all(0).nonzero().flatten().tolist()
+    assert rows_ == [5, M - 1] and columns == [N - 1] and int(bad.sum()) == 2 * N + M - 2
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("M,K,N", [(1, 256, 40), (20, 200, 72), (70, 40, 72), (520, 256, 512)])
 def test_powers_of_all_sizes(hip, M, K, N, dtype):
     """Blocks whose powers differ by many orders within a row: each is multiplied by its own."""
