@@ -217,23 +217,24 @@ __global__ void __launch_bounds__(kAnyThreads) norm_rows_any_grad_kernel(Rows<T>
 }
 
 // ---- rows in registers ----------------------------------------------------------------------------------------------
-// A team of lanes holds a row, kPerLane neighbouring elements a lane: `lanes` (a power of two) of a
-// wave, or, WIDE, a whole workgroup. Every tensor is read once and written once; means and deviations are taken from registers. A team
+// A team of lanes holds a row, kPerLane neighbouring elements a lane: LANES (a power of two) of a
+// wave, or, LANES = 0 (WIDE), a whole workgroup. (With a number of lanes known at run time only, every step of a sum over them is a branch.) Every tensor is read once and written once; means and deviations are taken from registers. A team
 // keeps its columns from row to row, so parameters stay in registers too, and so do the backward's sums over rows.
 constexpr int kPerLane = 8, kNarrowThreads = 256;
 constexpr int kMostRegisterChannels = 1024 * kPerLane;
 
-template <class T, bool WIDE, bool RAGGED>
+template <class T, int LANES, bool RAGGED>
 struct Team {
+    static constexpr bool WIDE = LANES == 0;
     static constexpr int V = Vec<T>::kLen, NV = kPerLane / V, E = kPerLane;
-    int lanes, lane, channels;
+    int lane, channels;
     float inverse;                     // 1 / channels
     float (*exchange)[16][2];          // WIDE: [2][wave][2] in LDS, the two halves in turn
     int turn = 0;
 
     __device__ __forceinline__ int column(int v) const { return lane * E + v * V; }
-    // whether element j of vector v lies in the row
-    __device__ __forceinline__ bool inside(int v, int j) const { return column(v) + (RAGGED ? j : 0) < channels; }
+    // whether element k of the lane's lies in the row (without RAGGED a lane's lie there all or none)
+    __device__ __forceinline__ bool inside(int k) const { return lane * E + (RAGGED ? k : 0) < channels; }
 
     __device__ __forceinline__ void request(const T* tensor, int64_t row, Chunk (&raw)[NV]) const {
         if (tensor == nullptr) return;
@@ -277,18 +278,18 @@ struct Team {
         if (is_float) {
 #pragma unroll
             for (int i = 0; i < E; ++i)
-                if (inside(i / V, i % V)) out[i] = static_cast<const float*>(p)[column(i / V) + i % V];
+                if (inside(i)) out[i] = static_cast<const float*>(p)[column(0) + i];
         } else {
 #pragma unroll
             for (int i = 0; i < E; ++i)
-                if (inside(i / V, i % V)) out[i] = static_cast<float>(static_cast<const T*>(p)[column(i / V) + i % V]);
+                if (inside(i)) out[i] = static_cast<float>(static_cast<const T*>(p)[column(0) + i]);
         }
     }
     // Over the row: the sums of a and b, the same in all its lanes.
     __device__ __forceinline__ void pair_sum(float& a, float& b) {
         if constexpr (!WIDE) {
-            a = sum_of_lanes(a, lanes);
-            b = sum_of_lanes(b, lanes);
+            a = sum_of_lanes(a, LANES);
+            b = sum_of_lanes(b, LANES);
         } else {
             a = sum_of_lanes(a, 64);
             b = sum_of_lanes(b, 64);
@@ -322,7 +323,7 @@ struct Team {
             // within a wave first the mean, then the deviations from it
 #pragma unroll
             for (int i = 0; i < E; ++i) sum += value[i];
-            sum = sum_of_lanes(sum, WIDE ? 64 : lanes);
+            sum = sum_of_lanes(sum, WIDE ? 64 : LANES);
             float part = inverse;
             int count = channels;
             if constexpr (WIDE) {
@@ -330,12 +331,13 @@ struct Team {
                 part = 1.0f / static_cast<float>(max(count, 1));
             }
             m.mean = sum * part;
+            const float from = RAGGED || inside(0) ? m.mean : 0.0f;
 #pragma unroll
             for (int i = 0; i < E; ++i) {
-                const float d = inside(i / V, i % V) ? value[i] - m.mean : 0.0f;
+                const float d = RAGGED && !inside(i) ? 0.0f : value[i] - from;
                 square += d * d;
             }
-            square = sum_of_lanes(square, WIDE ? 64 : lanes);
+            square = sum_of_lanes(square, WIDE ? 64 : LANES);
             if constexpr (WIDE) {
                 // the waves' means before their deviations: nothing cancels however far the mean is from zero
                 const int waves = blockDim.x / 64;
@@ -353,18 +355,26 @@ struct Team {
         m.rstd = rsqrtf(square * inverse + eps);
         return m;
     }
+    // (value - mean) * rstd, 0 beyond the row (whose values are 0).
+    __device__ __forceinline__ void normalise(float (&value)[E], const Moments& m) const {
+        const bool in = RAGGED || inside(0);
+        const float mean = in ? m.mean : 0.0f, rstd = in ? m.rstd : 0.0f;
+#pragma unroll
+        for (int i = 0; i < E; ++i) value[i] = RAGGED && !inside(i) ? 0.0f : (value[i] - mean) * rstd;
+    }
     // Elements of the row in wave w.
     __device__ __forceinline__ int in_wave(int w) const { return min(max(channels - w * 64 * E, 0), 64 * E); }
 };
 
 // The team of this thread, the first row of its wave's next ones (from 0 on), its own place among them, and how far apart they are.
-template <class T, bool WIDE, bool RAGGED>
+template <class T, int LANES, bool RAGGED>
 struct Place {
-    Team<T, WIDE, RAGGED> team;
+    static constexpr bool WIDE = LANES == 0;
+    Team<T, LANES, RAGGED> team;
     int first, own, step;
-    __device__ __forceinline__ Place(const Rows<T>& a, int lanes, float (*exchange)[16][2]) {
-        team.lanes = lanes;
-        team.lane = WIDE ? threadIdx.x : threadIdx.x & (lanes - 1);
+    __device__ __forceinline__ Place(const Rows<T>& a, float (*exchange)[16][2]) {
+        constexpr int lanes = WIDE ? 64 : LANES;
+        team.lane = WIDE ? threadIdx.x : threadIdx.x % lanes;
         team.channels = a.channels;
         team.inverse = 1.0f / static_cast<float>(a.channels);
         team.exchange = exchange;
@@ -375,8 +385,8 @@ struct Place {
     }
 };
 
-template <class T, bool WIDE, bool RAGGED>
-__device__ __forceinline__ void item_gate(const Team<T, WIDE, RAGGED>& team, const Rows<T>& a, int64_t item, float (&g)[kPerLane]) {
+template <class T, int LANES, bool RAGGED>
+__device__ __forceinline__ void item_gate(const Team<T, LANES, RAGGED>& team, const Rows<T>& a, int64_t item, float (&g)[kPerLane]) {
     const int64_t at = a.gate_kind == kGateItem ? item * a.channels : 0;
     if (a.gate_kind == kGateChannel || a.gate_kind == kGateItem)
         team.params(a.float_gate ? static_cast<const void*>(static_cast<const float*>(a.gate) + at) : static_cast<const void*>(static_cast<const T*>(a.gate) + at),
@@ -384,12 +394,12 @@ __device__ __forceinline__ void item_gate(const Team<T, WIDE, RAGGED>& team, con
 }
 
 // CODES: the normed rows leave in 8 bits. A block of 128 lies in 128 / kPerLane neighbouring lanes.
-template <class T, bool WIDE, bool RAGGED, bool CODES>
-__global__ void __launch_bounds__(WIDE ? 1024 : kNarrowThreads) norm_rows_kernel(Rows<T> a, int lanes) {
-    typedef Team<T, WIDE, RAGGED> Row;
-    constexpr int E = Row::E, V = Row::V, NV = Row::NV;
+template <class T, int LANES, bool RAGGED, bool CODES>
+__global__ void __launch_bounds__(LANES == 0 ? 1024 : kNarrowThreads) norm_rows_kernel(Rows<T> a) {
+    typedef Team<T, LANES, RAGGED> Row;
+    constexpr int E = Row::E, NV = Row::NV;
     __shared__ float exchange[2][16][2];
-    Place<T, WIDE, RAGGED> place(a, lanes, exchange);
+    Place<T, LANES, RAGGED> place(a, exchange);
     Row& team = place.team;
     float wa[E], ba[E], wb[E], bb[E], g[E];
     const T* const full = a.gate_kind == kGateFull ? static_cast<const T*>(a.gate) : nullptr;
@@ -424,32 +434,22 @@ __global__ void __launch_bounds__(WIDE ? 1024 : kNarrowThreads) norm_rows_kernel
             if (full != nullptr) team.settle(gs, g);
             if (base + place.step < span.last) request(base + place.step);
             if (a.after) {
-                const Moments m = team.moments(x, a.centre, a.eps);
+                team.normalise(x, team.moments(x, a.centre, a.eps));
 #pragma unroll
-                for (int k = 0; k < E; ++k) x[k] = (x[k] - m.mean) * m.rstd * wa[k] + ba[k];
+                for (int k = 0; k < E; ++k) x[k] = x[k] * wa[k] + ba[k];
             }
+            // (0 beyond the row, where x, the residual and the bias are)
 #pragma unroll
             for (int k = 0; k < E; ++k) x[k] = r[k] + x[k] * g[k] * a.scale;
-            if constexpr (RAGGED) {
-#pragma unroll
-                for (int k = 0; k < E; ++k)
-                    if (!team.inside(k / V, k % V)) x[k] = 0.0f;
-            } else {
-#pragma unroll
-                for (int k = 0; k < E; ++k)
-                    if (!team.inside(k / V, 0)) x[k] = 0.0f;
-            }
             if (a.stream != nullptr && live) team.store(a.stream, row, x);
             if (!a.before) continue;
-            const Moments m = team.moments(x, a.centre, a.eps);
+            team.normalise(x, team.moments(x, a.centre, a.eps));
 #pragma unroll
-            for (int k = 0; k < E; ++k) x[k] = (x[k] - m.mean) * m.rstd * wb[k] + bb[k];
+            for (int k = 0; k < E; ++k) x[k] = x[k] * wb[k] + bb[k];
             if constexpr (!CODES) {
                 if (live) team.store(a.normed, row, x);
             } else {
                 const int blocks = blocks_of(a.channels), words = exponents_of(a.channels), c = team.column(0), b = c / kBlock;
-#pragma unroll
-                for (int k = 0; k < E; ++k) x[k] = team.inside(k / V, k % V) ? x[k] : 0.0f;
                 const int e = block_exponent(most_of_lanes(largest(x), kBlock / E));
                 const Codes<E> codes = to_codes(x, e);
                 if (live && b < blocks) {
@@ -466,23 +466,21 @@ __global__ void __launch_bounds__(WIDE ? 1024 : kNarrowThreads) norm_rows_kernel
     }
 }
 
-// BIG: rows of more than 512 lanes, 128 registers each: parameters come from the caches again for every row, and no row is requested ahead.
-template <class T, bool WIDE, bool RAGGED, bool BIG>
-__global__ void __launch_bounds__(WIDE ? (BIG ? 1024 : 512) : kNarrowThreads) norm_rows_grad_kernel(Rows<T> a, int lanes) {
-    typedef Team<T, WIDE, RAGGED> Row;
-    constexpr int E = Row::E, V = Row::V, NV = Row::NV;
+// BIG: rows of more than 512 lanes, 128 registers each: parameters come from the caches again for every row.
+template <class T, int LANES, bool RAGGED, bool BIG>
+__global__ void __launch_bounds__(LANES == 0 ? (BIG ? 1024 : 512) : kNarrowThreads) norm_rows_grad_kernel(Rows<T> a) {
+    typedef Team<T, LANES, RAGGED> Row;
+    constexpr bool WIDE = LANES == 0;
+    constexpr int E = Row::E, NV = Row::NV;
     __shared__ float exchange[2][16][2];
     __shared__ float gather[WIDE ? 1 : kNarrowThreads / 64][WIDE ? 1 : 64 * kPerLane];
-    Place<T, WIDE, RAGGED> place(a, lanes, exchange);
+    Place<T, LANES, RAGGED> place(a, exchange);
     Row& team = place.team;
-    float wa[E], ba[E], wb[E], g[E], sum[kSums][E];
+    float sum[kSums][E] = {};
     const T* const full = a.gate_kind == kGateFull ? static_cast<const T*>(a.gate) : nullptr;
+    float wa[E], ba[E], wb[E], g[E];
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-        g[i] = 1.0f;
-#pragma unroll
-        for (int k = 0; k < kSums; ++k) sum[k][i] = 0.0f;
-    }
+    for (int i = 0; i < E; ++i) g[i] = 1.0f;
     const auto parameters = [&] {
         team.params(a.after_weight, a.float_params, 1.0f, wa);
         team.params(a.after_bias, a.float_params, 0.0f, ba);
@@ -499,14 +497,14 @@ __global__ void __launch_bounds__(WIDE ? (BIG ? 1024 : 512) : kNarrowThreads) no
         if constexpr (WIDE) {
 #pragma unroll
             for (int k = 0; k < E; ++k)
-                if (team.inside(k / V, k % V)) write(team.column(k / V) + k % V, v[k]);
+                if (team.inside(k)) write(team.column(0) + k, v[k]);
         } else {
             __syncthreads();
 #pragma unroll
             for (int k = 0; k < E; ++k) {
                 float s = v[k];
-                for (int d = lanes; d < 64; d <<= 1) s += __shfl_xor(s, d);
-                if (static_cast<int>(threadIdx.x) % 64 < lanes) gather[threadIdx.x / 64][team.column(k / V) + k % V] = s;
+                for (int d = LANES; d < 64; d <<= 1) s += __shfl_xor(s, d);
+                if (static_cast<int>(threadIdx.x) % 64 < LANES) gather[threadIdx.x / 64][team.column(0) + k] = s;
             }
             __syncthreads();
             for (int c = threadIdx.x; c < a.channels; c += kNarrowThreads) {
@@ -541,7 +539,7 @@ __global__ void __launch_bounds__(WIDE ? (BIG ? 1024 : 512) : kNarrowThreads) no
                 parameters();
                 item_gate(team, a, span.item, g);
             }
-            float p[E], q[E], d[E], h[E];                              // normalised x, normalised s, gradients of s and h
+            float p[E], q[E], d[E], h[E];                              // normalised x, normalised s, gradients of s and h; later what they become
             team.settle(xs, p);
             team.settle(rs, q);
             team.settle(ds, d);
@@ -553,52 +551,64 @@ __global__ void __launch_bounds__(WIDE ? (BIG ? 1024 : 512) : kNarrowThreads) no
             Moments mx = {0.0f, 1.0f};
             if (a.after) {
                 mx = team.moments(p, a.centre, a.eps);
-#pragma unroll
-                for (int k = 0; k < E; ++k) p[k] = (p[k] - mx.mean) * mx.rstd;
+                team.normalise(p, mx);
             }
             if (has_dh) {
 #pragma unroll
                 for (int k = 0; k < E; ++k) {
                     const float u = a.after ? p[k] * wa[k] + ba[k] : p[k];
-                    q[k] = team.inside(k / V, k % V) ? q[k] + u * g[k] * a.scale : 0.0f;
+                    q[k] += u * g[k] * a.scale;
                 }
                 const Moments ms = team.moments(q, a.centre, a.eps);
+                team.normalise(q, ms);
+                if (live) {
+#pragma unroll
+                    for (int k = 0; k < E; ++k) {
+                        sum[2][k] += h[k] * q[k];
+                        sum[3][k] += h[k];
+                    }
+                }
                 float e1 = 0.0f, e2 = 0.0f;
 #pragma unroll
                 for (int k = 0; k < E; ++k) {
-                    q[k] = (q[k] - ms.mean) * ms.rstd;
-                    const float e = h[k] * wb[k];                      // (0 beyond the row)
-                    e1 += e;
-                    e2 += e * q[k];
-                    sum[2][k] += live ? h[k] * q[k] : 0.0f;
-                    sum[3][k] += live ? h[k] : 0.0f;
+                    h[k] *= wb[k];                                      // (0 beyond the row)
+                    e1 += h[k];
+                    e2 += h[k] * q[k];
                 }
                 team.pair_sum(e1, e2);
                 e1 = a.centre ? e1 * team.inverse : 0.0f;
                 e2 *= team.inverse;
-#pragma unroll
-                for (int k = 0; k < E; ++k) d[k] += ms.rstd * (h[k] * wb[k] - e1 - q[k] * e2);
-            }
-            if (a.dresidual != nullptr && live) team.store(a.dresidual, row, d);
-            float f1 = 0.0f, f2 = 0.0f;
-#pragma unroll
-            for (int k = 0; k < E; ++k) {
-                const float u = a.after ? p[k] * wa[k] + ba[k] : p[k], t = a.scale * d[k];
-                q[k] = u * t;                                          // of the gate
-                d[k] = t * g[k];                                       // of u
-                sum[kSumGate][k] += live ? q[k] : 0.0f;
-            }
-            if (a.dgate_full != nullptr && live) team.store(a.dgate_full, row, q);
-            if (a.after) {
+                const float rstd = RAGGED || team.inside(0) ? ms.rstd : 0.0f;
 #pragma unroll
                 for (int k = 0; k < E; ++k) {
-                    const bool in = team.inside(k / V, k % V);
-                    const float du = in ? d[k] : 0.0f;
-                    sum[0][k] += live ? du * p[k] : 0.0f;
-                    sum[1][k] += live ? du : 0.0f;
-                    d[k] = du * wa[k];
+                    const float through = rstd * (h[k] - e1 - q[k] * e2);
+                    d[k] += RAGGED && !team.inside(k) ? 0.0f : through;
+                }
+            }
+            if (a.dresidual != nullptr && live) team.store(a.dresidual, row, d);
+            // d: gradient of s, then of u; h: of the gate
+#pragma unroll
+            for (int k = 0; k < E; ++k) {
+                d[k] *= a.scale;
+                h[k] = (a.after ? p[k] * wa[k] + ba[k] : p[k]) * d[k];
+                d[k] *= g[k];
+            }
+            if (a.dgate_full != nullptr && live) team.store(a.dgate_full, row, h);
+            if (live) {
+#pragma unroll
+                for (int k = 0; k < E; ++k) {
+                    sum[kSumGate][k] += h[k];
+                    sum[0][k] += d[k] * p[k];
+                    sum[1][k] += d[k];
+                }
+            }
+            if (a.after) {
+                float f1 = 0.0f, f2 = 0.0f;
+#pragma unroll
+                for (int k = 0; k < E; ++k) {
+                    d[k] *= wa[k];
                     f1 += d[k];
-                    f2 += in ? d[k] * p[k] : 0.0f;
+                    f2 += d[k] * p[k];
                 }
                 team.pair_sum(f1, f2);
                 f1 = a.centre ? f1 * team.inverse : 0.0f;
@@ -687,11 +697,19 @@ Shape shape_of(int channels, bool codes) {
     return {true, lanes, lanes, 1};
 }
 
-// f(true) or f(false), with the value known to the compiler.
+// f(value) with the value known to the compiler: true or false; LANES from `least` on, 0 for a workgroup.
 template <class F>
 void known(bool value, F f) {
     if (value) f(std::true_type());
     else f(std::false_type());
+}
+template <int LEAST, class F>
+void known_lanes(const Shape& s, F f) {
+    if (s.wide) return f(std::integral_constant<int, 0>());
+    if constexpr (LEAST < 64) {
+        if (s.lanes > LEAST) return known_lanes<LEAST * 2>(s, f);
+    }
+    f(std::integral_constant<int, LEAST>());
 }
 
 RowPlan forward_plan(const ResidualNormCall& c, const Shape& s) { return plan_rows(c, 2048, s.rows); }
@@ -712,13 +730,11 @@ hipError_t residual_norm_forward(const ResidualNormCall& c, const ResidualNormOu
     const dim3 grid(static_cast<unsigned>(a.plan.groups)), block(s.threads);
     if (s.lanes == 0) BOXCONV_LAUNCH("norm_rows", (norm_rows_any_kernel<T>), grid, block, 0, stream, a);
     else
-        known(s.wide, [&](auto wide) {
-            known(c.channels % Vec<T>::kLen != 0, [&](auto ragged) {
-                known(coded, [&](auto codes) {
-                    BOXCONV_LAUNCH("norm_rows", (norm_rows_kernel<T, decltype(wide)::value, decltype(ragged)::value, decltype(codes)::value>), grid, block, 0, stream, a,
-                                   s.lanes);
-                });
-            });
+        known(c.channels % kPerLane != 0, [&](auto ragged) {
+            constexpr bool R = decltype(ragged)::value;
+            if (coded)
+                known_lanes<kBlock / kPerLane>(s, [&](auto lanes) { BOXCONV_LAUNCH("norm_rows", (norm_rows_kernel<T, decltype(lanes)::value, R, true>), grid, block, 0, stream, a); });
+            else known_lanes<1>(s, [&](auto lanes) { BOXCONV_LAUNCH("norm_rows", (norm_rows_kernel<T, decltype(lanes)::value, R, false>), grid, block, 0, stream, a); });
         });
     return hipGetLastError();
 }
@@ -751,11 +767,10 @@ hipError_t residual_norm_backward(const ResidualNormCall& c, const ResidualNormG
     const dim3 grid(static_cast<unsigned>(a.plan.groups)), block(s.threads);
     if (s.lanes == 0) BOXCONV_LAUNCH("norm_rows_grad", (norm_rows_any_grad_kernel<T>), grid, block, 0, stream, a);
     else
-        known(c.channels % Vec<T>::kLen != 0, [&](auto ragged) {
+        known(c.channels % kPerLane != 0, [&](auto ragged) {
             constexpr bool R = decltype(ragged)::value;
-            if (!s.wide) BOXCONV_LAUNCH("norm_rows_grad", (norm_rows_grad_kernel<T, false, R, false>), grid, block, 0, stream, a, s.lanes);
-            else if (s.threads <= 512) BOXCONV_LAUNCH("norm_rows_grad", (norm_rows_grad_kernel<T, true, R, false>), grid, block, 0, stream, a, s.lanes);
-            else BOXCONV_LAUNCH("norm_rows_grad", (norm_rows_grad_kernel<T, true, R, true>), grid, block, 0, stream, a, s.lanes);
+            if (s.wide && s.threads > 512) BOXCONV_LAUNCH("norm_rows_grad", (norm_rows_grad_kernel<T, 0, R, true>), grid, block, 0, stream, a);
+            else known_lanes<1>(s, [&](auto lanes) { BOXCONV_LAUNCH("norm_rows_grad", (norm_rows_grad_kernel<T, decltype(lanes)::value, R, false>), grid, block, 0, stream, a); });
         });
     bool any = false;
     for (void* p : to.p) any = any || p != nullptr;
