@@ -220,13 +220,13 @@ __global__ void __launch_bounds__(kAnyThreads) norm_rows_any_grad_kernel(Rows<T>
 // A team of lanes holds a row, kPerLane neighbouring elements a lane: LANES (a power of two) of a
 // wave, or, LANES = 0 (WIDE), a whole workgroup. (With a number of lanes known at run time only, every step of a sum over them is a branch.) Every tensor is read once and written once; means and deviations are taken from registers. A team
 // keeps its columns from row to row, so parameters stay in registers too, and so do the backward's sums over rows.
-constexpr int kPerLane = 8, kNarrowThreads = 256;
-constexpr int kMostRegisterChannels = 1024 * kPerLane;
+constexpr int kPerLane = 8, kNarrowThreads = 256, kWideThreads = 512;
+constexpr int kMostRegisterChannels = kWideThreads * 2 * kPerLane;
 
-template <class T, int LANES, bool RAGGED>
+template <class T, int LANES, int E, bool RAGGED>
 struct Team {
     static constexpr bool WIDE = LANES == 0;
-    static constexpr int V = Vec<T>::kLen, NV = kPerLane / V, E = kPerLane;
+    static constexpr int V = Vec<T>::kLen, NV = E / V;
     int lane, channels;
     float inverse;                     // 1 / channels
     float (*exchange)[16][2];          // WIDE: [2][wave][2] in LDS, the two halves in turn
@@ -367,10 +367,10 @@ struct Team {
 };
 
 // The team of this thread, the first row of its wave's next ones (from 0 on), its own place among them, and how far apart they are.
-template <class T, int LANES, bool RAGGED>
+template <class T, int LANES, int E, bool RAGGED>
 struct Place {
     static constexpr bool WIDE = LANES == 0;
-    Team<T, LANES, RAGGED> team;
+    Team<T, LANES, E, RAGGED> team;
     int first, own, step;
     __device__ __forceinline__ Place(const Rows<T>& a, float (*exchange)[16][2]) {
         constexpr int lanes = WIDE ? 64 : LANES;
@@ -385,8 +385,8 @@ struct Place {
     }
 };
 
-template <class T, int LANES, bool RAGGED>
-__device__ __forceinline__ void item_gate(const Team<T, LANES, RAGGED>& team, const Rows<T>& a, int64_t item, float (&g)[kPerLane]) {
+template <class T, int LANES, int E, bool RAGGED>
+__device__ __forceinline__ void item_gate(const Team<T, LANES, E, RAGGED>& team, const Rows<T>& a, int64_t item, float (&g)[E]) {
     const int64_t at = a.gate_kind == kGateItem ? item * a.channels : 0;
     if (a.gate_kind == kGateChannel || a.gate_kind == kGateItem)
         team.params(a.float_gate ? static_cast<const void*>(static_cast<const float*>(a.gate) + at) : static_cast<const void*>(static_cast<const T*>(a.gate) + at),
@@ -394,12 +394,12 @@ __device__ __forceinline__ void item_gate(const Team<T, LANES, RAGGED>& team, co
 }
 
 // CODES: the normed rows leave in 8 bits. A block of 128 lies in 128 / kPerLane neighbouring lanes.
-template <class T, int LANES, bool RAGGED, bool CODES>
-__global__ void __launch_bounds__(LANES == 0 ? 1024 : kNarrowThreads) norm_rows_kernel(Rows<T> a) {
-    typedef Team<T, LANES, RAGGED> Row;
-    constexpr int E = Row::E, NV = Row::NV;
+template <class T, int LANES, int E, bool RAGGED, bool CODES>
+__global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads) norm_rows_kernel(Rows<T> a) {
+    typedef Team<T, LANES, E, RAGGED> Row;
+    constexpr int NV = Row::NV;
     __shared__ float exchange[2][16][2];
-    Place<T, LANES, RAGGED> place(a, exchange);
+    Place<T, LANES, E, RAGGED> place(a, exchange);
     Row& team = place.team;
     float wa[E], ba[E], wb[E], bb[E], g[E];
     const T* const full = a.gate_kind == kGateFull ? static_cast<const T*>(a.gate) : nullptr;
@@ -466,15 +466,16 @@ __global__ void __launch_bounds__(LANES == 0 ? 1024 : kNarrowThreads) norm_rows_
     }
 }
 
-// BIG: rows of more than 512 lanes, 128 registers each: parameters come from the caches again for every row.
-template <class T, int LANES, bool RAGGED, bool BIG>
-__global__ void __launch_bounds__(LANES == 0 ? (BIG ? 1024 : 512) : kNarrowThreads) norm_rows_grad_kernel(Rows<T> a) {
-    typedef Team<T, LANES, RAGGED> Row;
-    constexpr bool WIDE = LANES == 0;
-    constexpr int E = Row::E, NV = Row::NV;
+// Two rows ahead are on their way while one is worked on. With twice the elements a lane (BIG) there are no registers for that, nor for the
+// parameters, which come from the caches again for every row.
+template <class T, int LANES, int E, bool RAGGED>
+__global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads) norm_rows_grad_kernel(Rows<T> a) {
+    typedef Team<T, LANES, E, RAGGED> Row;
+    constexpr bool WIDE = LANES == 0, BIG = E > kPerLane;
+    constexpr int NV = Row::NV;
     __shared__ float exchange[2][16][2];
     __shared__ float gather[WIDE ? 1 : kNarrowThreads / 64][WIDE ? 1 : 64 * kPerLane];
-    Place<T, LANES, RAGGED> place(a, exchange);
+    Place<T, LANES, E, RAGGED> place(a, exchange);
     Row& team = place.team;
     float sum[kSums][E] = {};
     const T* const full = a.gate_kind == kGateFull ? static_cast<const T*>(a.gate) : nullptr;
@@ -517,36 +518,31 @@ __global__ void __launch_bounds__(LANES == 0 ? (BIG ? 1024 : 512) : kNarrowThrea
     };
     for (int64_t i = 0; i < a.plan.items; ++i) {
         const Span span = span_of(a.plan, a.pixels, i);
-        Chunk xs[NV] = {}, rs[NV] = {}, gs[NV] = {}, ds[NV] = {}, hs[NV] = {};
-        const auto request = [&](int64_t base) {
+        struct Raw { Chunk x[NV], r[NV], g[NV], d[NV], h[NV]; } ahead[BIG ? 1 : 2] = {};
+        const auto request = [&](int64_t base, Raw& raw) {
             const int64_t row = min(base + place.own, span.last - 1);
-            team.request(a.x, row, xs);
-            if (a.before) team.request(a.residual, row, rs);
-            team.request(full, row, gs);
-            team.request(a.dstream, row, ds);
-            if (a.before) team.request(a.dnormed, row, hs);
+            team.request(a.x, row, raw.x);
+            if (a.before) team.request(a.residual, row, raw.r);
+            team.request(full, row, raw.g);
+            team.request(a.dstream, row, raw.d);
+            if (a.before) team.request(a.dnormed, row, raw.h);
         };
-        int64_t base = span.first + place.first;
-        if constexpr (!BIG) {
-            if (base < span.last) request(base);
-            item_gate(team, a, span.item, g);
-        }
-        for (; base < span.last; base += place.step) {
+        const auto work = [&](int64_t base, Raw& raw) {
             const int64_t row = base + place.own;
             const bool live = row < span.last;
             if constexpr (BIG) {
-                request(base);
+                request(base, raw);
                 parameters();
                 item_gate(team, a, span.item, g);
             }
             float p[E], q[E], d[E], h[E];                              // normalised x, normalised s, gradients of s and h; later what they become
-            team.settle(xs, p);
-            team.settle(rs, q);
-            team.settle(ds, d);
-            team.settle(hs, h);
-            if (full != nullptr) team.settle(gs, g);
+            team.settle(raw.x, p);
+            team.settle(raw.r, q);
+            team.settle(raw.d, d);
+            team.settle(raw.h, h);
+            if (full != nullptr) team.settle(raw.g, g);
             if constexpr (!BIG) {
-                if (base + place.step < span.last) request(base + place.step);
+                if (base + 2 * place.step < span.last) request(base + 2 * place.step, raw);
             }
             Moments mx = {0.0f, 1.0f};
             if (a.after) {
@@ -617,6 +613,18 @@ __global__ void __launch_bounds__(LANES == 0 ? (BIG ? 1024 : 512) : kNarrowThrea
                 for (int k = 0; k < E; ++k) d[k] = mx.rstd * (d[k] - f1 - p[k] * f2);
             }
             if (a.dx != nullptr && live) team.store(a.dx, row, d);
+        };
+        int64_t base = span.first + place.first;
+        if constexpr (BIG) {
+            for (; base < span.last; base += place.step) work(base, ahead[0]);
+        } else {
+            if (base < span.last) request(base, ahead[0]);
+            if (base + place.step < span.last) request(base + place.step, ahead[1]);
+            item_gate(team, a, span.item, g);
+            for (; base < span.last; base += 2 * place.step) {
+                work(base, ahead[0]);
+                if (base + place.step < span.last) work(base + place.step, ahead[1]);
+            }
         }
         if (a.gate_kind == kGateItem && (a.dgate != nullptr || a.sums != nullptr) && span.last > span.first) {
             if (a.dgate != nullptr) put(sum[kSumGate], a.dgate, span.item * a.channels, a.float_gate);
@@ -683,18 +691,19 @@ Rows<T> rows_of(const ResidualNormCall& c) {
     return a;
 }
 
-// How the rows of a call are dealt out: lanes of a team, its workgroup's threads, and rows that a workgroup takes at once. No lanes: rows of more
-// channels than the registers of a workgroup hold.
-struct Shape { bool wide; int lanes, threads, rows; };
+// How the rows of a call are dealt out: lanes of a team, its workgroup's threads, and rows that a workgroup takes at once. big: twice
+// kPerLane elements a lane. No lanes: rows of more channels than the registers of a workgroup hold.
+struct Shape { bool wide; int lanes, threads, rows; bool big; };
 template <class T>
 Shape shape_of(int channels, bool codes) {
-    if (channels > kMostRegisterChannels) return {true, 0, kAnyThreads, 1};
+    if (channels > kMostRegisterChannels) return {true, 0, kAnyThreads, 1, false};
     const int columns = codes ? blocks_of(channels) * kBlock : channels;           // (codes are written to the end of the last block)
     int lanes = codes ? kBlock / kPerLane : 1;        // (more lanes without a share add zeros: the sums are the same to the bit)
     while (lanes < 64 && lanes * kPerLane < columns) lanes *= 2;
-    if (lanes * kPerLane >= columns) return {false, lanes, kNarrowThreads, kNarrowThreads / lanes};
-    lanes = (columns + 64 * kPerLane - 1) / (64 * kPerLane) * 64;
-    return {true, lanes, lanes, 1};
+    if (lanes * kPerLane >= columns) return {false, lanes, kNarrowThreads, kNarrowThreads / lanes, false};
+    const int each = columns > kWideThreads * kPerLane ? 2 * kPerLane : kPerLane;
+    lanes = (columns + 64 * each - 1) / (64 * each) * 64;
+    return {true, lanes, lanes, 1, each > kPerLane};
 }
 
 // f(value) with the value known to the compiler: true or false; LANES from `least` on, 0 for a workgroup.
@@ -705,15 +714,18 @@ void known(bool value, F f) {
 }
 template <int LEAST, class F>
 void known_lanes(const Shape& s, F f) {
-    if (s.wide) return f(std::integral_constant<int, 0>());
+    typedef std::integral_constant<int, kPerLane> Each;
+    if (s.wide && s.big) return f(std::integral_constant<int, 0>(), std::integral_constant<int, 2 * kPerLane>());
+    if (s.wide) return f(std::integral_constant<int, 0>(), Each());
     if constexpr (LEAST < 64) {
         if (s.lanes > LEAST) return known_lanes<LEAST * 2>(s, f);
     }
-    f(std::integral_constant<int, LEAST>());
+    f(std::integral_constant<int, LEAST>(), Each());
 }
 
-RowPlan forward_plan(const ResidualNormCall& c, const Shape& s) { return plan_rows(c, 2048, s.rows); }
-RowPlan backward_plan(const ResidualNormCall& c, const Shape& s) { return plan_rows(c, s.wide ? 512 : 1024, s.rows); }
+// As many workgroups as the chip holds at once: the forward's kernels leave room for four waves a SIMD, the backward's for two.
+RowPlan forward_plan(const ResidualNormCall& c, const Shape& s) { return plan_rows(c, 256 * 16 * 64 / s.threads, s.rows); }
+RowPlan backward_plan(const ResidualNormCall& c, const Shape& s) { return plan_rows(c, 256 * 8 * 64 / std::min(s.threads, 512), s.rows); }
 
 }  // namespace
 
@@ -730,11 +742,11 @@ hipError_t residual_norm_forward(const ResidualNormCall& c, const ResidualNormOu
     const dim3 grid(static_cast<unsigned>(a.plan.groups)), block(s.threads);
     if (s.lanes == 0) BOXCONV_LAUNCH("norm_rows", (norm_rows_any_kernel<T>), grid, block, 0, stream, a);
     else
-        known(c.channels % kPerLane != 0, [&](auto ragged) {
+        known(c.channels % (s.big ? 2 * kPerLane : kPerLane) != 0, [&](auto ragged) {
             constexpr bool R = decltype(ragged)::value;
             if (coded)
-                known_lanes<kBlock / kPerLane>(s, [&](auto lanes) { BOXCONV_LAUNCH("norm_rows", (norm_rows_kernel<T, decltype(lanes)::value, R, true>), grid, block, 0, stream, a); });
-            else known_lanes<1>(s, [&](auto lanes) { BOXCONV_LAUNCH("norm_rows", (norm_rows_kernel<T, decltype(lanes)::value, R, false>), grid, block, 0, stream, a); });
+                known_lanes<kBlock / kPerLane>(s, [&](auto lanes, auto each) { BOXCONV_LAUNCH("norm_rows", (norm_rows_kernel<T, decltype(lanes)::value, decltype(each)::value, R, true>), grid, block, 0, stream, a); });
+            else known_lanes<1>(s, [&](auto lanes, auto each) { BOXCONV_LAUNCH("norm_rows", (norm_rows_kernel<T, decltype(lanes)::value, decltype(each)::value, R, false>), grid, block, 0, stream, a); });
         });
     return hipGetLastError();
 }
@@ -767,10 +779,9 @@ hipError_t residual_norm_backward(const ResidualNormCall& c, const ResidualNormG
     const dim3 grid(static_cast<unsigned>(a.plan.groups)), block(s.threads);
     if (s.lanes == 0) BOXCONV_LAUNCH("norm_rows_grad", (norm_rows_any_grad_kernel<T>), grid, block, 0, stream, a);
     else
-        known(c.channels % kPerLane != 0, [&](auto ragged) {
+        known(c.channels % (s.big ? 2 * kPerLane : kPerLane) != 0, [&](auto ragged) {
             constexpr bool R = decltype(ragged)::value;
-            if (s.wide && s.threads > 512) BOXCONV_LAUNCH("norm_rows_grad", (norm_rows_grad_kernel<T, 0, R, true>), grid, block, 0, stream, a);
-            else known_lanes<1>(s, [&](auto lanes) { BOXCONV_LAUNCH("norm_rows_grad", (norm_rows_grad_kernel<T, decltype(lanes)::value, R, false>), grid, block, 0, stream, a); });
+            known_lanes<1>(s, [&](auto lanes, auto each) { BOXCONV_LAUNCH("norm_rows_grad", (norm_rows_grad_kernel<T, decltype(lanes)::value, decltype(each)::value, R>), grid, block, 0, stream, a); });
         });
     bool any = false;
     for (void* p : to.p) any = any || p != nullptr;
