@@ -63,9 +63,10 @@ _SIGNATURES["boxconv_group_norm_forward"] = (
 _SIGNATURES["boxconv_group_norm_backward"] = (
     _i, [_vp] * 3 + [_i] + [_vp] * 8 + [_i, _i64, _i64, _i, _i, _i, _vp, _sz, _vp])
 _RESIDUAL_NORM = [_vp] * 3 + [_i, _i, _f, _i] + [_vp] * 4 + [_i, _f]
-_SIGNATURES["boxconv_residual_norm_forward"] = (_i, _RESIDUAL_NORM + [_vp] * 3 + [_i, _i64, _i64, _i, _vp])
+_SIGNATURES["boxconv_residual_norm_statistics_bytes"] = (_sz, [_i64, _i64, _i])
+_SIGNATURES["boxconv_residual_norm_forward"] = (_i, _RESIDUAL_NORM + [_vp] * 4 + [_i, _i64, _i64, _i, _vp])
 _SIGNATURES["boxconv_residual_norm_workspace_bytes"] = (_sz, [_i64, _i64, _i, _i, _i])
-_SIGNATURES["boxconv_residual_norm_backward"] = (_i, _RESIDUAL_NORM + [_vp] * 9 + [_i, _i64, _i64, _i, _vp, _sz, _vp])
+_SIGNATURES["boxconv_residual_norm_backward"] = (_i, _RESIDUAL_NORM + [_vp] * 10 + [_i, _i64, _i64, _i, _vp, _sz, _vp])
 _SIGNATURES["boxconv_linear_workspace_bytes"] = (_sz, [_i64, _i64, _i64, _i, _i])
 _SIGNATURES["boxconv_linear_forward"] = (
     _i, [_vp, _i64, _vp, _vp, _vp, _i64, _vp, _vp, _i, _i64, _i64, _i64, _i, _vp, _sz, _vp])
@@ -143,8 +144,8 @@ def glue():
             module.init_operators(*[ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
                 "boxconv_group_norm_workspace_bytes", "boxconv_group_norm_forward", "boxconv_group_norm_backward",
                 "boxconv_linear_workspace_bytes", "boxconv_linear_forward", "boxconv_linear_backward",
-                "boxconv_residual_norm_workspace_bytes", "boxconv_residual_norm_forward", "boxconv_residual_norm_backward",
-                "boxconv_quantize_blocks", "boxconv_linear_float8_workspace_bytes", "boxconv_linear_float8_forward")])
+                "boxconv_residual_norm_workspace_bytes", "boxconv_residual_norm_statistics_bytes", "boxconv_residual_norm_forward",
+                "boxconv_residual_norm_backward", "boxconv_quantize_blocks", "boxconv_linear_float8_workspace_bytes", "boxconv_linear_float8_forward")])
             _glue = module
     return _glue or None
 
@@ -769,23 +770,28 @@ def _residual_norm_arguments(input, residual, gate, gate_kind, scale, norms, par
     return begin, (dtype, B, input.numel() // (B * C) if B * C else 0, C)
 
 
-def residual_norm_forward(input, residual, gate, gate_kind, scale, norms, params, eps, want_stream, blocks=None):
+def residual_norm_forward(input, residual, gate, gate_kind, scale, norms, params, eps, want_stream, blocks=None, keep_statistics=False):
     """What lies between two residual blocks, of contiguous ``[B, ..., C]`` tensors (include/boxconv.h,
     boxconv_residual_norm_forward). ``params``: weight and bias of the norm after and of the norm before. ``blocks``: (codes, exponents)
-    that receive the normed rows in 8 bits. Returns ``(stream, normed)``, ``None`` for what is not formed."""
+    that receive the normed rows in 8 bits. Returns ``(stream, normed, statistics)``, ``None`` for what is not formed; the last, for the backward,
+    only where it is asked for and rows are long enough to keep any."""
     stream = torch.empty_like(input) if want_stream else None
     normed = torch.empty_like(input) if norms & NORM_BEFORE and blocks is None else None
+    statistics = None
     if input.numel() > 0:
         begin, sizes = _residual_norm_arguments(input, residual, gate, gate_kind, scale, norms, params, eps)
         to = (_ptr(normed), None) if blocks is None else (_ptr(blocks[0]), _ptr(blocks[1]))
+        nbytes = _operator_workspace_bytes("boxconv_residual_norm_statistics_bytes", *sizes[1:]) if keep_statistics else 0
+        if nbytes:
+            statistics = torch.empty(nbytes // 4, dtype=torch.float32, device=input.device)
         with _on_device(input.device):
-            rc = load().boxconv_residual_norm_forward(*begin, _ptr(stream), *to, *sizes, _stream(input.device))
+            rc = load().boxconv_residual_norm_forward(*begin, _ptr(stream), *to, _ptr(statistics), *sizes, _stream(input.device))
         _check(rc, "residual_norm")
-    return stream, normed
+    return stream, normed, statistics
 
 
-def residual_norm_backward(input, residual, gate, gate_kind, scale, norms, params, eps, grad_stream, grad_normed, needs):
-    """Gradients of ``residual_norm_forward``, all tensors contiguous ``[B, ..., C]``. ``needs``: whether input, residual, gate and the four
+def residual_norm_backward(input, residual, gate, gate_kind, scale, norms, params, eps, statistics, grad_stream, grad_normed, needs):
+    """Gradients of ``residual_norm_forward``, all tensors contiguous ``[B, ..., C]``. ``statistics``: the forward's, or ``None``. ``needs``: whether input, residual, gate and the four
     parameters need theirs; returns the seven, ``None`` where not."""
     grads = [torch.empty_like(t) if need else None for t, need in zip((input, residual, gate, *params), needs)]
     if input.numel() == 0:
@@ -795,7 +801,7 @@ def residual_norm_backward(input, residual, gate, gate_kind, scale, norms, param
         nbytes = _operator_workspace_bytes("boxconv_residual_norm_workspace_bytes", *sizes[1:], gate_kind, sizes[0])
         stream = _stream(input.device)
         ws = _scratch(nbytes, input.device)
-        rc = load().boxconv_residual_norm_backward(*begin, _ptr(grad_stream), _ptr(grad_normed), *[_ptr(g) for g in grads], *sizes,
+        rc = load().boxconv_residual_norm_backward(*begin, _ptr(statistics), _ptr(grad_stream), _ptr(grad_normed), *[_ptr(g) for g in grads], *sizes,
                                                    _ptr(ws), nbytes, stream)
     _check(rc, "residual_norm backward")
     return grads

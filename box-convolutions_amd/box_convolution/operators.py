@@ -183,8 +183,8 @@ class ResidualNormFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, input, residual, gate, after_weight, after_bias, before_weight, before_bias, gate_kind, scale, norms, eps, want_stream):
         params = (after_weight, after_bias, before_weight, before_bias)
-        outputs = _native.residual_norm_forward(input, residual, gate, gate_kind, scale, norms, params, eps, want_stream)
-        ctx.save_for_backward(input, residual, gate, *params)
+        *outputs, statistics = _native.residual_norm_forward(input, residual, gate, gate_kind, scale, norms, params, eps, want_stream, None, True)
+        ctx.save_for_backward(input, residual, gate, *params, statistics)
         ctx.rest = gate_kind, scale, norms
         ctx.eps, ctx.want_stream = eps, want_stream
         ctx.set_materialize_grads(False)
@@ -197,10 +197,11 @@ class ResidualNormFunction(torch.autograd.Function):
         _refuse_tangents(*grad_outputs)
         grad_stream = given.pop(0) if ctx.want_stream else None
         grad_normed = given.pop(0) if given else None
-        input, residual, gate, *params = _contiguous(*ctx.saved_tensors)
+        input, residual, gate, *params, statistics = _contiguous(*ctx.saved_tensors)
         gate_kind, scale, norms = ctx.rest
         needs = [n and t is not None for n, t in zip(ctx.needs_input_grad, (input, residual, gate, *params))]
-        grads = _native.residual_norm_backward(input, residual, gate, gate_kind, scale, norms, params, ctx.eps, grad_stream, grad_normed, needs)
+        grads = _native.residual_norm_backward(input, residual, gate, gate_kind, scale, norms, params, ctx.eps, statistics, grad_stream,
+                                               grad_normed, needs)
         like = next((g for g in grad_outputs if g is not None), input)
         return (*_once(grads, input, like), None, None, None, None, None)
 
@@ -298,7 +299,7 @@ def residual_norm(input, residual=None, gate=None, scale=1.0, after=None, before
             codes, exponents = _native.block_sizes(x.size(-1))
             blocks = (torch.empty((*x.shape[:-1], codes), dtype=torch.float8_e4m3fn, device=x.device),
                       torch.empty((*x.shape[:-1], exponents), dtype=torch.uint8, device=x.device))
-        stream, normed = _native.residual_norm_forward(x, r, g, gate_kind, scale, norms, params, eps, not same, blocks)
+        stream, normed, _ = _native.residual_norm_forward(x, r, g, gate_kind, scale, norms, params, eps, not same, blocks)
         if quantize:
             normed = Float8Blocks._of(*blocks, x.size(-1))
     stream = input if same else stream.movedim(-1, 1)

@@ -75,6 +75,14 @@ int check_residual_norm(int dtype, int param_dtype, int gate_dtype, int gate_kin
     return 0;
 }
 
+int check_statistics(const void* statistics, int64_t batch, int64_t pixels, int channels) {
+    if (statistics == nullptr) return 0;
+    if (boxconv_residual_norm_statistics_bytes(batch, pixels, channels) == 0)
+        return fail(BOXCONV_E_INVALID_ARGUMENT, "residual norm: statistics of rows that do without");
+    if (reinterpret_cast<uintptr_t>(statistics) % 16 != 0) return fail(BOXCONV_E_INVALID_ARGUMENT, "residual norm: statistics must be 16-byte aligned");
+    return 0;
+}
+
 int check_workspace(const char* what, const void* workspace, size_t have, size_t need) {
     if (need == 0) return 0;
     if (workspace == nullptr || have < need)
@@ -142,20 +150,26 @@ int boxconv_group_norm_backward(const void* input, const void* weight, const voi
 
 int boxconv_residual_norm_forward(const void* input, const void* residual, const void* gate, int gate_kind, int gate_dtype, float scale, int norms,
                                   const void* after_weight, const void* after_bias, const void* before_weight, const void* before_bias, int param_dtype,
-                                  float eps, void* stream_output, void* normed, void* normed_exponents, int dtype, int64_t batch, int64_t pixels,
-                                  int channels, void* stream) {
+                                  float eps, void* stream_output, void* normed, void* normed_exponents, void* statistics, int dtype, int64_t batch,
+                                  int64_t pixels, int channels, void* stream) {
     if (const int rc = check_residual_norm(dtype, param_dtype, gate_dtype, gate_kind, gate != nullptr, norms, batch, pixels, channels)) return rc;
     if (normed != nullptr && !(norms & BOXCONV_NORM_BEFORE)) return fail(BOXCONV_E_INVALID_ARGUMENT, "residual norm: normed without BOXCONV_NORM_BEFORE");
     if (normed == nullptr && normed_exponents != nullptr) return fail(BOXCONV_E_INVALID_ARGUMENT, "residual norm: normed_exponents without normed");
     if (normed_exponents != nullptr && (reinterpret_cast<uintptr_t>(normed) % 16 != 0 || reinterpret_cast<uintptr_t>(normed_exponents) % 4 != 0))
         return fail(BOXCONV_E_INVALID_ARGUMENT, "residual norm: codes must be 16-byte aligned, exponents 4-byte aligned");
-    if (batch == 0 || pixels == 0 || (stream_output == nullptr && normed == nullptr)) return 0;
+    if (const int rc = check_statistics(statistics, batch, pixels, channels)) return rc;
+    if (batch == 0 || pixels == 0 || (stream_output == nullptr && normed == nullptr && statistics == nullptr)) return 0;
     if (input == nullptr) return fail(BOXCONV_E_INVALID_ARGUMENT, "residual norm: null input pointer");
     const ResidualNormCall call = {input, residual, gate, after_weight, after_bias, before_weight, before_bias, gate_kind, (norms & BOXCONV_NORM_AFTER) != 0,
-                                   normed != nullptr, (norms & BOXCONV_NORM_CENTRE) != 0, param_dtype == BOXCONV_F32, gate_dtype == BOXCONV_F32, batch,
+                                   normed != nullptr || (statistics != nullptr && (norms & BOXCONV_NORM_BEFORE)), (norms & BOXCONV_NORM_CENTRE) != 0, param_dtype == BOXCONV_F32, gate_dtype == BOXCONV_F32, batch,
                                    pixels, channels, scale, eps};
-    const ResidualNormOut out = {stream_output, normed, static_cast<uint8_t*>(normed_exponents)};
+    const ResidualNormOut out = {stream_output, normed, static_cast<uint8_t*>(normed_exponents), static_cast<float*>(statistics)};
     return hip_result(with_type(dtype, [&](auto t) { return residual_norm_forward<decltype(t)>(call, out, static_cast<hipStream_t>(stream)); }), "residual norm");
+}
+
+size_t boxconv_residual_norm_statistics_bytes(int64_t batch, int64_t pixels, int channels) {
+    if (check_residual_norm(BOXCONV_F32, BOXCONV_F32, BOXCONV_F32, BOXCONV_GATE_NONE, false, 0, batch, pixels, channels) != 0) return 0;
+    return channels > kMostChannelsWithoutStatistics ? static_cast<size_t>(batch) * pixels * 4 * sizeof(float) : 0;
 }
 
 size_t boxconv_residual_norm_workspace_bytes(int64_t batch, int64_t pixels, int channels, int gate_kind, int dtype) {
@@ -170,7 +184,7 @@ size_t boxconv_residual_norm_workspace_bytes(int64_t batch, int64_t pixels, int 
 
 int boxconv_residual_norm_backward(const void* input, const void* residual, const void* gate, int gate_kind, int gate_dtype, float scale, int norms,
                                    const void* after_weight, const void* after_bias, const void* before_weight, const void* before_bias, int param_dtype,
-                                   float eps, const void* grad_stream, const void* grad_normed, void* grad_input, void* grad_residual, void* grad_gate,
+                                   float eps, const void* statistics, const void* grad_stream, const void* grad_normed, void* grad_input, void* grad_residual, void* grad_gate,
                                    void* grad_after_weight, void* grad_after_bias, void* grad_before_weight, void* grad_before_bias, int dtype,
                                    int64_t batch, int64_t pixels, int channels, void* workspace, size_t workspace_bytes, void* stream) {
     if (const int rc = check_residual_norm(dtype, param_dtype, gate_dtype, gate_kind, gate != nullptr, norms, batch, pixels, channels)) return rc;
@@ -184,6 +198,7 @@ int boxconv_residual_norm_backward(const void* input, const void* residual, cons
         const int64_t gates = gate_kind == BOXCONV_GATE_CHANNEL ? channels : gate_kind == BOXCONV_GATE_ITEM ? batch * channels : 0;
         return write_zeros(grad_gate, gates, gate_dtype, "residual norm", static_cast<hipStream_t>(stream));
     }
+    if (const int rc = check_statistics(statistics, batch, pixels, channels)) return rc;
     const bool sums = grad_after_weight != nullptr || grad_after_bias != nullptr || grad_before_weight != nullptr || grad_before_bias != nullptr ||
                       (grad_gate != nullptr && gate_kind != BOXCONV_GATE_FULL);
     if (!sums && grad_input == nullptr && grad_residual == nullptr && grad_gate == nullptr) return 0;
@@ -194,7 +209,7 @@ int boxconv_residual_norm_backward(const void* input, const void* residual, cons
     const ResidualNormCall call = {input, residual, gate, after_weight, after_bias, before_weight, before_bias, gate_kind, (norms & BOXCONV_NORM_AFTER) != 0,
                                    (norms & BOXCONV_NORM_BEFORE) != 0, (norms & BOXCONV_NORM_CENTRE) != 0, param_dtype == BOXCONV_F32,
                                    gate_dtype == BOXCONV_F32, batch, pixels, channels, scale, eps};
-    const ResidualNormGrads grads = {grad_stream, grad_normed, grad_input, grad_residual, grad_gate, grad_after_weight, grad_after_bias, grad_before_weight, grad_before_bias};
+    const ResidualNormGrads grads = {static_cast<const float*>(statistics), grad_stream, grad_normed, grad_input, grad_residual, grad_gate, grad_after_weight, grad_after_bias, grad_before_weight, grad_before_bias};
     return hip_result(with_type(dtype, [&](auto t) { return residual_norm_backward<decltype(t)>(call, grads, workspace, static_cast<hipStream_t>(stream)); }),
                       "residual norm");
 }

@@ -27,10 +27,12 @@ struct OperatorAbi {
     int (*linear_backward)(const void*, int64_t, const void*, const void*, const void*, void*, void*, void*, void*, int, int64_t, int64_t, int64_t, int,
                            void*, size_t, void*) = nullptr;
     size_t (*residual_bytes)(int64_t, int64_t, int, int, int) = nullptr;
+    size_t (*statistics_bytes)(int64_t, int64_t, int) = nullptr;
     int (*residual_forward)(const void*, const void*, const void*, int, int, float, int, const void*, const void*, const void*, const void*, int, float, void*,
-                            void*, void*, int, int64_t, int64_t, int, void*) = nullptr;
+                            void*, void*, void*, int, int64_t, int64_t, int, void*) = nullptr;
     int (*residual_backward)(const void*, const void*, const void*, int, int, float, int, const void*, const void*, const void*, const void*, int, float,
-                             const void*, const void*, void*, void*, void*, void*, void*, void*, void*, int, int64_t, int64_t, int, void*, size_t, void*) = nullptr;
+                             const void*, const void*, const void*, void*, void*, void*, void*, void*, void*, void*, int, int64_t, int64_t, int, void*, size_t,
+                             void*) = nullptr;
     int (*quantize)(const void*, int64_t, int, int64_t, int64_t, void*, void*, void*) = nullptr;
     size_t (*float8_bytes)(int64_t, int64_t, int64_t, int, int) = nullptr;
     int (*float8_forward)(const void*, int64_t, int, const void*, const void*, const void*, const void*, const void*, int64_t, void*, int, int64_t, int64_t,
@@ -38,9 +40,10 @@ struct OperatorAbi {
 } g_operators;
 
 void init_operators(uint64_t norm_bytes, uint64_t norm_forward, uint64_t norm_backward, uint64_t linear_bytes, uint64_t linear_forward,
-                    uint64_t linear_backward, uint64_t residual_bytes, uint64_t residual_forward, uint64_t residual_backward, uint64_t quantize,
+                    uint64_t linear_backward, uint64_t residual_bytes, uint64_t statistics_bytes, uint64_t residual_forward, uint64_t residual_backward, uint64_t quantize,
                     uint64_t float8_bytes, uint64_t float8_forward) {
     g_operators.residual_bytes = reinterpret_cast<decltype(g_operators.residual_bytes)>(residual_bytes);
+    g_operators.statistics_bytes = reinterpret_cast<decltype(g_operators.statistics_bytes)>(statistics_bytes);
     g_operators.residual_forward = reinterpret_cast<decltype(g_operators.residual_forward)>(residual_forward);
     g_operators.residual_backward = reinterpret_cast<decltype(g_operators.residual_backward)>(residual_backward);
     g_operators.quantize = reinterpret_cast<decltype(g_operators.quantize)>(quantize);
@@ -349,15 +352,15 @@ struct ResidualNorm : public torch::autograd::Function<ResidualNorm> {
             if (*p) return type_code((*p)->scalar_type());
         return 0;
     }
-    // Images in channels-last memory. `s` and `h` (values or codes, the latter with exponents) may be undefined.
+    // Images in channels-last memory. `s`, `h` (values or codes, the latter with exponents) and `statistics` may be undefined.
     static void call(const at::Tensor& x, const Optional& residual, const Optional& gate, const Optional& aw, const Optional& ab, const Optional& bw,
-                     const Optional& bb, const Between& b, const at::Tensor& s, const at::Tensor& h, const at::Tensor& exponents) {
+                     const Optional& bb, const Between& b, const at::Tensor& s, const at::Tensor& h, const at::Tensor& exponents, const at::Tensor& statistics) {
         if (x.numel() == 0) return;
         const GroupNormAct::Sizes n = GroupNormAct::sizes(x);
         const int code = type_code(x.scalar_type());
         check_rc(g_operators.residual_forward(x.data_ptr(), address(residual), address(gate), b.gate_kind, gate ? type_code(gate->scalar_type()) : code,
                                               static_cast<float>(b.scale), b.norms, address(aw), address(ab), address(bw), address(bb),
-                                              param_code({&aw, &ab, &bw, &bb}), static_cast<float>(b.eps), address(s), address(h), address(exponents), code, n.batch,
+                                              param_code({&aw, &ab, &bw, &bb}), static_cast<float>(b.eps), address(s), address(h), address(exponents), address(statistics), code, n.batch,
                                               n.pixels, n.channels, reinterpret_cast<void*>(b.stream)),
                  "residual_norm");
     }
@@ -370,9 +373,12 @@ struct ResidualNorm : public torch::autograd::Function<ResidualNorm> {
         const Optional g = !gate ? std::nullopt : Optional(gate_kind == kGateOfElement ? channels_last(*gate) : gate->contiguous());
         const Optional aw = contiguous(after_weight), ab = contiguous(after_bias), bw = contiguous(before_weight), bb = contiguous(before_bias);
         const at::Tensor s = want_stream ? empty_channels_last(x) : at::Tensor(), h = norms & kBefore ? empty_channels_last(x) : at::Tensor();
-        call(x, r, g, aw, ab, bw, bb, {static_cast<int>(gate_kind), static_cast<int>(norms), scale, eps, stream}, s, h, at::Tensor());
+        const GroupNormAct::Sizes n = GroupNormAct::sizes(x);
+        const size_t kept = x.numel() ? g_operators.statistics_bytes(n.batch, n.pixels, n.channels) : 0;
+        const at::Tensor statistics = kept ? at::empty({static_cast<int64_t>(kept / sizeof(float))}, x.options().dtype(at::kFloat)) : at::Tensor();
+        call(x, r, g, aw, ab, bw, bb, {static_cast<int>(gate_kind), static_cast<int>(norms), scale, eps, stream}, s, h, at::Tensor(), statistics);
         const auto or_none = [](const Optional& t) { return t.value_or(at::Tensor()); };
-        ctx->save_for_backward({x, or_none(r), or_none(g), or_none(aw), or_none(ab), or_none(bw), or_none(bb)});
+        ctx->save_for_backward({x, or_none(r), or_none(g), or_none(aw), or_none(ab), or_none(bw), or_none(bb), statistics});
         ctx->set_materialize_grads(false);
         ctx->saved_data["present"] = c10::List<bool>({true, residual.has_value(), gate.has_value(), after_weight.has_value(), after_bias.has_value(),
                                                       before_weight.has_value(), before_bias.has_value()});
@@ -395,6 +401,7 @@ struct ResidualNorm : public torch::autograd::Function<ResidualNorm> {
         const at::Tensor x = channels_last(saved[0]), residual = image(saved[1]);
         const Optional gate = !saved[2].defined() ? std::nullopt : Optional(gate_kind == kGateOfElement ? channels_last(saved[2]) : saved[2].contiguous());
         const Optional aw = saved_or_none(saved[3]), ab = saved_or_none(saved[4]), bw = saved_or_none(saved[5]), bb = saved_or_none(saved[6]);
+        const Optional statistics = saved_or_none(saved[7]);
         const bool want_stream = ctx->saved_data["want_stream"].toBool();
         const at::Tensor ds = want_stream ? image(grad_outputs[0]) : at::Tensor();
         const at::Tensor dh = norms & kBefore ? image(grad_outputs[want_stream ? 1 : 0]) : at::Tensor();
@@ -417,7 +424,7 @@ struct ResidualNorm : public torch::autograd::Function<ResidualNorm> {
         const at::Tensor ws = scratch(nbytes, x);
         check_rc(g_operators.residual_backward(x.data_ptr(), address(residual), address(gate), gate_kind, gate ? type_code(gate->scalar_type()) : code,
                                                static_cast<float>(ctx->saved_data["scale"].toDouble()), norms, address(aw), address(ab), address(bw), address(bb),
-                                               param_code({&aw, &ab, &bw, &bb}), static_cast<float>(ctx->saved_data["eps"].toDouble()), address(ds), address(dh),
+                                               param_code({&aw, &ab, &bw, &bb}), static_cast<float>(ctx->saved_data["eps"].toDouble()), address(statistics), address(ds), address(dh),
                                                address(grads[0]), address(grads[1]), address(grads[2]), address(grads[3]), address(grads[4]), address(grads[5]),
                                                address(grads[6]), code, n.batch, n.pixels, n.channels, address(ws), nbytes,
                                                reinterpret_cast<void*>(ctx->saved_data["stream"].toInt())),
@@ -492,7 +499,7 @@ std::vector<at::Tensor> residual_norm(const at::Tensor& input, const Optional& r
     }
     const Optional g = !gate ? std::nullopt : Optional(gate_kind == kGateOfElement ? channels_last(*gate) : gate->contiguous());
     ResidualNorm::call(x, residual ? Optional(channels_last(*residual)) : std::nullopt, g, contiguous(after_weight), contiguous(after_bias), contiguous(before_weight),
-                       contiguous(before_bias), {gate_kind, norms, scale, eps, stream}, s, h, exponents);
+                       contiguous(before_bias), {gate_kind, norms, scale, eps, stream}, s, h, exponents, at::Tensor());
     return out;
 }
 

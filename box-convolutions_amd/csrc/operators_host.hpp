@@ -95,13 +95,19 @@ struct ResidualNormCall {
 struct ResidualNormOut {
     void *stream, *normed;
     uint8_t* exponents;          // not null: `normed` is codes
+    float* statistics;           // [row][mean and rstd of x, of the stream], or null
 };
 struct ResidualNormGrads {
+    const float* statistics;     // null: formed again
     const void *dstream, *dnormed;
     void *dx, *dresidual, *dgate, *dafter_weight, *dafter_bias, *dbefore_weight, *dbefore_bias;
 };
 template <class T> hipError_t residual_norm_forward(const ResidualNormCall& c, const ResidualNormOut& out, hipStream_t stream);
 template <class T> size_t residual_norm_workspace(const ResidualNormCall& c);
+// Rows of more channels keep their statistics for the backward: a workgroup works on them, and forming them again takes it two of four
+// barriers a row (8192 rows of 4096 bfloat16 128 us, kept 96). Within a wave they cost next to nothing (131072 rows of 128 48 and 45 us), and
+// short rows would have as much to read instead.
+constexpr int kMostChannelsWithoutStatistics = 512;
 template <class T> hipError_t residual_norm_backward(const ResidualNormCall& c, const ResidualNormGrads& g, void* workspace, hipStream_t stream);
 
 }  // namespace boxconv

@@ -28,6 +28,7 @@ struct Rows {
     const void *gate, *after_weight, *after_bias, *before_weight, *before_bias;
     T *stream, *normed;
     uint8_t *codes, *exponents;        // the normed rows in 8 bits, in place of `normed`
+    float* statistics;                 // written by the forward, read by the backward: a row's four
     int channels, gate_kind;
     bool after, before, centre, float_params, float_gate;
     float scale, eps;
@@ -72,6 +73,7 @@ __device__ __forceinline__ void sum_of_workgroup(float (&v)[N], float* lds) {
 }
 
 struct Moments { float mean, rstd; };
+typedef float Four __attribute__((ext_vector_type(4)));
 
 template <class F>
 __device__ __forceinline__ Moments moments_any(F value, int channels, bool centre, float eps, float* lds) {
@@ -117,7 +119,13 @@ struct AnyRow {
         const float t = u(c) * gate(c) * a.scale;
         return a.residual != nullptr ? static_cast<float>(a.residual[at + c]) + t : t;
     }
-    __device__ __forceinline__ void measure(float* lds) {
+    // `kept`: the row's statistics, or null: formed here.
+    __device__ __forceinline__ void measure(float* lds, const float* kept) {
+        if (kept != nullptr) {
+            x = {kept[0], kept[1]};
+            s = {kept[2], kept[3]};
+            return;
+        }
         if (a.after) x = moments_any([&](int c) { return input(c); }, a.channels, a.centre, a.eps, lds);
         if (a.before) s = moments_any([&](int c) { return stream(c); }, a.channels, a.centre, a.eps, lds);
     }
@@ -131,7 +139,8 @@ __global__ void __launch_bounds__(kAnyThreads) norm_rows_any_kernel(Rows<T> a) {
         const Span span = span_of(a.plan, a.pixels, i);
         for (int64_t row = span.first; row < span.last; ++row) {
             AnyRow<T> r = {a, row * a.channels, span.item};
-            r.measure(lds);
+            r.measure(lds, nullptr);
+            if (a.statistics != nullptr && threadIdx.x == 0) *reinterpret_cast<Four*>(a.statistics + 4 * row) = Four{r.x.mean, r.x.rstd, r.s.mean, r.s.rstd};
             if (a.stream != nullptr)
                 for (int c = threadIdx.x; c < a.channels; c += kAnyThreads) a.stream[r.at + c] = static_cast<T>(r.stream(c));
             if (a.normed != nullptr)
@@ -163,7 +172,7 @@ __global__ void __launch_bounds__(kAnyThreads) norm_rows_any_grad_kernel(Rows<T>
         const Span span = span_of(a.plan, a.pixels, i);
         for (int64_t row = span.first; row < span.last; ++row) {
             AnyRow<T> r = {a, row * a.channels, span.item};
-            r.measure(lds);
+            r.measure(lds, a.statistics == nullptr ? nullptr : a.statistics + 4 * row);
             const auto dh = [&](int c) { return a.before && a.dnormed != nullptr ? static_cast<float>(a.dnormed[r.at + c]) : 0.0f; };
             const auto q = [&](int c) { return (r.stream(c) - r.s.mean) * r.s.rstd; };
             const auto e = [&](int c) { return dh(c) * r.param(a.before_weight, c, 1.0f); };
@@ -433,8 +442,11 @@ __global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads) no
             team.settle(rs, r);
             if (full != nullptr) team.settle(gs, g);
             if (base + place.step < span.last) request(base + place.step);
+            Four kept = {0.0f, 1.0f, 0.0f, 1.0f};
             if (a.after) {
-                team.normalise(x, team.moments(x, a.centre, a.eps));
+                const Moments m = team.moments(x, a.centre, a.eps);
+                team.normalise(x, m);
+                if (LANES == 0) kept = Four{m.mean, m.rstd, 0.0f, 1.0f};
 #pragma unroll
                 for (int k = 0; k < E; ++k) x[k] = x[k] * wa[k] + ba[k];
             }
@@ -442,8 +454,13 @@ __global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads) no
 #pragma unroll
             for (int k = 0; k < E; ++k) x[k] = r[k] + x[k] * g[k] * a.scale;
             if (a.stream != nullptr && live) team.store(a.stream, row, x);
-            if (!a.before) continue;
-            team.normalise(x, team.moments(x, a.centre, a.eps));
+            Moments m = {0.0f, 1.0f};
+            if (a.before) m = team.moments(x, a.centre, a.eps);
+            if constexpr (LANES == 0) {
+                if (a.statistics != nullptr && threadIdx.x == 0) *reinterpret_cast<Four*>(a.statistics + 4 * row) = Four{kept[0], kept[1], m.mean, m.rstd};
+            }
+            if (a.normed == nullptr && !CODES) continue;
+            team.normalise(x, m);
 #pragma unroll
             for (int k = 0; k < E; ++k) x[k] = x[k] * wb[k] + bb[k];
             if constexpr (!CODES) {
@@ -469,7 +486,7 @@ __global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads) no
 // Two rows ahead are on their way while one is worked on. With twice the elements a lane (BIG) there are no registers for that, nor for the
 // parameters, which come from the caches again for every row.
 template <class T, int LANES, int E, bool RAGGED>
-__global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads) norm_rows_grad_kernel(Rows<T> a) {
+__global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads, 2) norm_rows_grad_kernel(Rows<T> a) {
     typedef Team<T, LANES, E, RAGGED> Row;
     constexpr bool WIDE = LANES == 0, BIG = E > kPerLane;
     constexpr int NV = Row::NV;
@@ -518,7 +535,7 @@ __global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads) no
     };
     for (int64_t i = 0; i < a.plan.items; ++i) {
         const Span span = span_of(a.plan, a.pixels, i);
-        struct Raw { Chunk x[NV], r[NV], g[NV], d[NV], h[NV]; } ahead[BIG ? 1 : 2] = {};
+        struct Raw { Chunk x[NV], r[NV], g[NV], d[NV], h[NV]; Four kept; } ahead[BIG ? 1 : 2] = {};
         const auto request = [&](int64_t base, Raw& raw) {
             const int64_t row = min(base + place.own, span.last - 1);
             team.request(a.x, row, raw.x);
@@ -526,6 +543,9 @@ __global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads) no
             team.request(full, row, raw.g);
             team.request(a.dstream, row, raw.d);
             if (a.before) team.request(a.dnormed, row, raw.h);
+            if constexpr (WIDE) {
+                if (a.statistics != nullptr) raw.kept = *reinterpret_cast<const Four*>(a.statistics + 4 * row);
+            }
         };
         const auto work = [&](int64_t base, Raw& raw) {
             const int64_t row = base + place.own;
@@ -541,12 +561,14 @@ __global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads) no
             team.settle(raw.d, d);
             team.settle(raw.h, h);
             if (full != nullptr) team.settle(raw.g, g);
+            const Four kept = raw.kept;
+            const bool again = !WIDE || a.statistics == nullptr;
             if constexpr (!BIG) {
                 if (base + 2 * place.step < span.last) request(base + 2 * place.step, raw);
             }
             Moments mx = {0.0f, 1.0f};
             if (a.after) {
-                mx = team.moments(p, a.centre, a.eps);
+                mx = again ? team.moments(p, a.centre, a.eps) : Moments{kept[0], kept[1]};
                 team.normalise(p, mx);
             }
             if (has_dh) {
@@ -555,7 +577,7 @@ __global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads) no
                     const float u = a.after ? p[k] * wa[k] + ba[k] : p[k];
                     q[k] += u * g[k] * a.scale;
                 }
-                const Moments ms = team.moments(q, a.centre, a.eps);
+                const Moments ms = again ? team.moments(q, a.centre, a.eps) : Moments{kept[2], kept[3]};
                 team.normalise(q, ms);
                 if (live) {
 #pragma unroll
@@ -734,6 +756,7 @@ hipError_t residual_norm_forward(const ResidualNormCall& c, const ResidualNormOu
     Rows<T> a = rows_of<T>(c);
     a.stream = static_cast<T*>(out.stream);
     a.exponents = out.exponents;
+    a.statistics = out.statistics;
     const bool coded = out.exponents != nullptr;
     if (coded) a.codes = static_cast<uint8_t*>(out.normed);
     else a.normed = static_cast<T*>(out.normed);
@@ -759,6 +782,7 @@ size_t residual_norm_workspace(const ResidualNormCall& c) {
 template <class T>
 hipError_t residual_norm_backward(const ResidualNormCall& c, const ResidualNormGrads& g, void* workspace, hipStream_t stream) {
     Rows<T> a = rows_of<T>(c);
+    a.statistics = const_cast<float*>(g.statistics);
     a.dstream = static_cast<const T*>(g.dstream);
     a.dnormed = static_cast<const T*>(g.dnormed);
     a.dx = static_cast<T*>(g.dx);

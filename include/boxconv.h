@@ -398,6 +398,8 @@ int boxconv_linear_backward(const void* input, int64_t ld_input, const void* wei
  * stream_output receives s, normed receives h, formed from s before it is rounded. Either may be null. norms is the sum of the
  * flags. Weights and biases [channels] have param_dtype (BOXCONV_F32 or dtype); null: 1, 0. The gate has gate_dtype (the same
  * choice) and as many values as its kind says: one per channel, [batch][channels], or, of type dtype, as the input has.
+ * statistics: null, or boxconv_residual_norm_statistics_bytes (0 for rows that do without, to be given as null) that receive what the
+ * backward would have to form again: per row the mean and 1/sqrt(variance + eps) of input and s (floats, 16-byte aligned).
  * normed_exponents: null, or h is written in 8 bits: normed then holds codes and this their exponents, as
  * boxconv_quantize_blocks lays them out (normed 16-byte aligned, normed_exponents 4-byte aligned). */
 #define BOXCONV_NORM_AFTER 1
@@ -410,17 +412,19 @@ int boxconv_linear_backward(const void* input, int64_t ld_input, const void* wei
 int boxconv_residual_norm_forward(const void* input, const void* residual, const void* gate, int gate_kind, int gate_dtype,
                                   float scale, int norms, const void* after_weight, const void* after_bias,
                                   const void* before_weight, const void* before_bias, int param_dtype, float eps,
-                                  void* stream_output, void* normed, void* normed_exponents, int dtype, int64_t batch,
-                                  int64_t pixels, int channels, void* stream);
+                                  void* stream_output, void* normed, void* normed_exponents, void* statistics, int dtype,
+                                  int64_t batch, int64_t pixels, int channels, void* stream);
+size_t boxconv_residual_norm_statistics_bytes(int64_t batch, int64_t pixels, int channels);
 /* Its gradients; those whose pointer is null are not formed. grad_stream, grad_normed: the gradients of s and h, null: 0.
+ * statistics: the forward call's with the same input, residual, gate and after-norm, or null: formed again.
  * grad_gate has the gate's type and shape, the parameters' gradients param_dtype. Sums over no rows are 0. All other arguments as
  * in the forward call; the workspace (boxconv_residual_norm_workspace_bytes) is 16-byte aligned. */
 size_t boxconv_residual_norm_workspace_bytes(int64_t batch, int64_t pixels, int channels, int gate_kind, int dtype);
 int boxconv_residual_norm_backward(const void* input, const void* residual, const void* gate, int gate_kind, int gate_dtype,
                                    float scale, int norms, const void* after_weight, const void* after_bias,
                                    const void* before_weight, const void* before_bias, int param_dtype, float eps,
-                                   const void* grad_stream, const void* grad_normed, void* grad_input, void* grad_residual,
-                                   void* grad_gate, void* grad_after_weight, void* grad_after_bias, void* grad_before_weight,
+                                   const void* statistics, const void* grad_stream, const void* grad_normed,
+                                   void* grad_input, void* grad_residual, void* grad_gate, void* grad_after_weight, void* grad_after_bias, void* grad_before_weight,
                                    void* grad_before_bias, int dtype, int64_t batch, int64_t pixels, int channels,
                                    void* workspace, size_t workspace_bytes, void* stream);
 

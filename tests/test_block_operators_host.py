@@ -14,13 +14,13 @@ def lib():
     return _native.load()
 
 
-def forward(lib, x=P, residual=None, gate=None, kind=0, gate_dtype=0, norms=3, param=0, stream=P, normed=P, exponents=None, dtype=0, batch=2, pixels=9, channels=8):
-    return lib.boxconv_residual_norm_forward(x, residual, gate, kind, gate_dtype, 1.0, norms, P, P, P, P, param, 1e-6, stream, normed, exponents, dtype, batch,
+def forward(lib, x=P, residual=None, gate=None, kind=0, gate_dtype=0, norms=3, param=0, stream=P, normed=P, exponents=None, statistics=None, dtype=0, batch=2, pixels=9, channels=8):
+    return lib.boxconv_residual_norm_forward(x, residual, gate, kind, gate_dtype, 1.0, norms, P, P, P, P, param, 1e-6, stream, normed, exponents, statistics, dtype, batch,
                                              pixels, channels, None)
 
 
-def backward(lib, gate=None, kind=0, norms=3, grads=(None,) * 7, stream=P, normed=P, x=P, batch=2, pixels=9, channels=8, ws=None, n=0):
-    return lib.boxconv_residual_norm_backward(x, None, gate, kind, 0, 1.0, norms, P, P, P, P, 0, 1e-6, stream, normed, *grads, 0, batch, pixels, channels, ws, n, None)
+def backward(lib, gate=None, kind=0, norms=3, grads=(None,) * 7, statistics=None, stream=P, normed=P, x=P, batch=2, pixels=9, channels=8, ws=None, n=0):
+    return lib.boxconv_residual_norm_backward(x, None, gate, kind, 0, 1.0, norms, P, P, P, P, 0, 1e-6, statistics, stream, normed, *grads, 0, batch, pixels, channels, ws, n, None)
 
 
 def test_residual_norm_argument_errors(lib):
@@ -29,7 +29,7 @@ def test_residual_norm_argument_errors(lib):
                            ({"kind": 1}, -1, b"do not agree"), ({"gate": P}, -1, b"do not agree"), ({"gate": P, "kind": 1, "gate_dtype": 2}, -1, b"gate_dtype"),
                            ({"gate": P, "kind": 3, "gate_dtype": 0, "dtype": 1, "param": 1}, -1, b"gate_dtype"), ({"norms": 8}, -1, b"norms"),
                            ({"channels": 0}, -1, b"sizes"), ({"batch": -1}, -1, b"sizes"), ({"pixels": -1}, -1, b"sizes"), ({"x": None}, -1, b"null"),
-                           ({"norms": 1}, -1, b"BEFORE"), ({"normed": None, "exponents": P}, -1, b"without normed"), ({"normed": odd, "exponents": P}, -1, b"aligned"),
+                           ({"norms": 1}, -1, b"BEFORE"), ({"normed": None, "exponents": P}, -1, b"without normed"), ({"normed": odd, "exponents": P}, -1, b"aligned"), ({"statistics": P}, -1, b"do without"), ({"statistics": odd, "channels": 1000}, -1, b"aligned"),
                            ({"batch": 1 << 31}, -3, b"too many"), ({"pixels": 1 << 46}, -3, b"too many"), ({"channels": (1 << 31) - 1}, -3, b"too many")):
         assert forward(lib, **kw) == code, kw
         assert text in lib.boxconv_last_error(), (kw, lib.boxconv_last_error())
@@ -37,7 +37,7 @@ def test_residual_norm_argument_errors(lib):
     assert backward(lib) == 0                                                        # nothing wanted
     for kw, code, text in (({"grads": (None, None, P, None, None, None, None)}, -1, b"grad_gate"), ({"norms": 2, "grads": (None, None, None, P, None, None, None)}, -1, b"norms"),
                            ({"norms": 1}, -1, b"norms"), ({"norms": 1, "normed": None, "grads": (None,) * 5 + (P, None)}, -1, b"norms"),
-                           ({"x": None, "grads": (P,) + (None,) * 6}, -1, b"null"), ({"grads": (None,) * 3 + (P,) + (None,) * 3}, -2, b"workspace")):
+                           ({"x": None, "grads": (P,) + (None,) * 6}, -1, b"null"), ({"statistics": P, "grads": (P,) + (None,) * 6}, -1, b"do without"), ({"grads": (None,) * 3 + (P,) + (None,) * 3}, -2, b"workspace")):
         assert backward(lib, **kw) == code, kw
         assert text in lib.boxconv_last_error(), (kw, lib.boxconv_last_error())
 
@@ -66,6 +66,8 @@ def test_float8_argument_errors(lib):
 
 
 def test_workspace_sizes(lib):
+    assert lib.boxconv_residual_norm_statistics_bytes(4, 100, 512) == 0 and lib.boxconv_residual_norm_statistics_bytes(4, 100, 513) == 4 * 100 * 16
+    assert lib.boxconv_residual_norm_statistics_bytes(4, 0, 1000) == 0 and lib.boxconv_residual_norm_statistics_bytes(4, 100, 0) == 0
     assert lib.boxconv_residual_norm_workspace_bytes(4, 100, 40, 1, 2) >= 5 * 40 * 4
     assert lib.boxconv_residual_norm_workspace_bytes(0, 100, 40, 0, 2) == 0 and lib.boxconv_residual_norm_workspace_bytes(4, 100, 0, 0, 2) == 0
     assert lib.boxconv_linear_float8_workspace_bytes(4000, 130, 64, 2, 2) >= 4000 * (256 + 4)      # the input's codes and exponents

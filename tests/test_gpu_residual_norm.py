@@ -268,7 +268,8 @@ def test_graph_replays(hip, size):
 
     def step():
         begin = (dev["x"], dev["residual"], dev["gate"], hip.GATE_ITEM, 0.5, norms, params, 1e-6)
-        return list(hip.residual_norm_forward(*begin, True)) + hip.residual_norm_backward(*begin, *grads, (True,) * 7)
+        *out, statistics = hip.residual_norm_forward(*begin, True, None, True)
+        return out + hip.residual_norm_backward(*begin, statistics, *grads, (True,) * 7)
     side = torch.cuda.Stream()
     with torch.cuda.stream(side):
         step()
