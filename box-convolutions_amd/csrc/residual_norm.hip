@@ -240,43 +240,85 @@ struct Team {
     float inverse;                     // 1 / channels
     float (*exchange)[16][2];          // WIDE: [2][wave][2] in LDS, the two halves in turn
     int turn = 0;
+    Chunk keep[RAGGED ? NV : 1];
 
     __device__ __forceinline__ int column(int v) const { return lane * E + v * V; }
     // whether element k of the lane's lies in the row (without RAGGED a lane's lie there all or none)
     __device__ __forceinline__ bool inside(int k) const { return lane * E + (RAGGED ? k : 0) < channels; }
 
-    __device__ __forceinline__ void request(const T* tensor, int64_t row, Chunk (&raw)[NV]) const {
+    // Vectors of a row, as they lie in memory. RAGGED: the last one runs into the next row, whose elements settle() takes away; `clear` says that
+    // no row of the wave's ends within a vector of the tensor's end, where that would be out of bounds: there it is read as the row's last
+    // whole vector and shifted at once.
+    __device__ __forceinline__ void request(const T* tensor, int64_t row, bool clear, Chunk (&raw)[NV]) const {
         if (tensor == nullptr) return;
         const T* p = tensor + row * channels;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
             const int c = column(v), n = channels - c;
-            if constexpr (RAGGED) raw[v] = channels < V ? short_chunk(p + c, n) : request_chunk(p + c, n, tensor);
-            else raw[v] = n > 0 ? __builtin_bit_cast(Chunk, *reinterpret_cast<const typename Vec<T>::Type*>(p + c)) : Chunk{0, 0, 0, 0};
+            if (!RAGGED || clear) raw[v] = n > 0 ? __builtin_bit_cast(Chunk, *reinterpret_cast<const typename Vec<T>::Type*>(p + c)) : Chunk{0, 0, 0, 0};
+            else if (channels < V) raw[v] = short_chunk(p + c, n);
+            else {
+                raw[v] = request_chunk(p + c, n, tensor);
+                settle_chunk<T>(raw[v], n);
+            }
         }
     }
+    __device__ __forceinline__ bool clear_of_end(int64_t last_row, int64_t rows) const { return (rows - 1 - last_row) * channels >= V; }
     // What was requested, as floats; 0 beyond the row.
-    __device__ __forceinline__ void settle(Chunk (&raw)[NV], float (&out)[E]) const {
+    __device__ __forceinline__ void settle(const Chunk (&raw)[NV], float (&out)[E]) const {
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            if constexpr (RAGGED) {
-                if (channels >= V) settle_chunk<T>(raw[v], channels - column(v));
-            }
-            const auto x = __builtin_bit_cast(typename Vec<T>::Type, raw[v]);
+            Chunk c = raw[v];
+            if constexpr (RAGGED) c &= keep[v];
+            const auto x = __builtin_bit_cast(typename Vec<T>::Type, c);
 #pragma unroll
             for (int j = 0; j < V; ++j) out[v * V + j] = static_cast<float>(x[j]);
         }
     }
+    // RAGGED: the bits of each vector that lie in the row.
+    __device__ __forceinline__ void start() {
+        if constexpr (RAGGED) {
+#pragma unroll
+            for (int v = 0; v < NV; ++v)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const int n = (channels - column(v)) * static_cast<int>(sizeof(T)) - 4 * w;        // bytes from here to the row's end
+                    keep[v][w] = n >= 4 ? 0xffffffffu : n <= 0 ? 0u : (1u << 8 * n) - 1;
+                }
+        }
+    }
     __device__ __forceinline__ void store(T* tensor, int64_t row, const float (&value)[E]) const {
+        typedef typename Vec<T>::Type Packed;
         T* p = tensor + row * channels;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            T out[V];
+            Packed out;
 #pragma unroll
             for (int j = 0; j < V; ++j) out[j] = static_cast<T>(value[v * V + j]);
+            T* to = p + column(v);
             const int n = channels - column(v);
-            if constexpr (RAGGED) store_run<T, V>(p + column(v), out, n);
-            else if (n > 0) store_run<T, V>(p + column(v), out, V);
+            if (n >= V || (!RAGGED && n > 0)) *reinterpret_cast<Packed*>(to) = out;
+            else if (RAGGED && n > 0) {
+                // the row's last elements: as many as for every row, in pieces of 4, 2 and 1
+                constexpr int B = sizeof(T);
+                typedef T Two __attribute__((ext_vector_type(2), aligned(B)));
+                typedef T Several __attribute__((ext_vector_type(4), aligned(B)));
+                if constexpr (V == 8) {
+                    if (channels & 4) {
+                        *reinterpret_cast<Several*>(to) = Several{out[0], out[1], out[2], out[3]};
+                        to += 4;
+                        out[0] = out[4];
+                        out[1] = out[5];
+                        out[2] = out[6];
+                    }
+                }
+                if (channels & 2) {
+                    *reinterpret_cast<Two*>(to) = Two{out[0], out[1]};
+                    to += 2;
+                    out[0] = out[2];
+                }
+                if (channels & 1) *to = out[0];
+            }
         }
     }
     // Values per column, of the parameters' type or float; `none` beyond the row and without a vector.
@@ -380,14 +422,15 @@ template <class T, int LANES, int E, bool RAGGED>
 struct Place {
     static constexpr bool WIDE = LANES == 0;
     Team<T, LANES, E, RAGGED> team;
-    int first, own, step;
+    int first, own, step, teams;       // teams: of a wave
     __device__ __forceinline__ Place(const Rows<T>& a, float (*exchange)[16][2]) {
         constexpr int lanes = WIDE ? 64 : LANES;
         team.lane = WIDE ? threadIdx.x : threadIdx.x % lanes;
         team.channels = a.channels;
         team.inverse = 1.0f / static_cast<float>(a.channels);
         team.exchange = exchange;
-        const int teams = WIDE ? 1 : 64 / lanes;                       // in a wave
+        team.start();
+        teams = WIDE ? 1 : 64 / lanes;
         first = WIDE ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / 64) * teams;
         own = WIDE ? 0 : threadIdx.x % 64 / lanes;
         step = WIDE ? 1 : kNarrowThreads / 64 * teams;
@@ -420,9 +463,10 @@ __global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads) no
         Chunk xs[NV] = {}, rs[NV] = {}, gs[NV] = {};
         const auto request = [&](int64_t base) {
             const int64_t row = min(base + place.own, span.last - 1);
-            team.request(a.x, row, xs);
-            team.request(a.residual, row, rs);
-            team.request(full, row, gs);
+            const bool clear = team.clear_of_end(min(base + place.teams, span.last) - 1, a.plan.batch * a.pixels);
+            team.request(a.x, row, clear, xs);
+            team.request(a.residual, row, clear, rs);
+            team.request(full, row, clear, gs);
         };
         int64_t base = span.first + place.first;
         if (base < span.last) request(base);
@@ -538,11 +582,12 @@ __global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads, 2)
         struct Raw { Chunk x[NV], r[NV], g[NV], d[NV], h[NV]; Four kept; } ahead[BIG ? 1 : 2] = {};
         const auto request = [&](int64_t base, Raw& raw) {
             const int64_t row = min(base + place.own, span.last - 1);
-            team.request(a.x, row, raw.x);
-            if (a.before) team.request(a.residual, row, raw.r);
-            team.request(full, row, raw.g);
-            team.request(a.dstream, row, raw.d);
-            if (a.before) team.request(a.dnormed, row, raw.h);
+            const bool clear = team.clear_of_end(min(base + place.teams, span.last) - 1, a.plan.batch * a.pixels);
+            team.request(a.x, row, clear, raw.x);
+            if (a.before) team.request(a.residual, row, clear, raw.r);
+            team.request(full, row, clear, raw.g);
+            team.request(a.dstream, row, clear, raw.d);
+            if (a.before) team.request(a.dnormed, row, clear, raw.h);
             if constexpr (WIDE) {
                 if (a.statistics != nullptr) raw.kept = *reinterpret_cast<const Four*>(a.statistics + 4 * row);
             }
