@@ -192,6 +192,8 @@ int boxconv_residual_norm_backward(const void* input, const void* residual, cons
     if ((!(norms & BOXCONV_NORM_AFTER) && (grad_after_weight != nullptr || grad_after_bias != nullptr)) ||
         (!(norms & BOXCONV_NORM_BEFORE) && (grad_normed != nullptr || grad_before_weight != nullptr || grad_before_bias != nullptr)))
         return fail(BOXCONV_E_INVALID_ARGUMENT, "residual norm: gradients of a norm that norms does not have");
+    if ((grad_after_bias != nullptr && after_bias == nullptr) || (grad_before_bias != nullptr && before_bias == nullptr))
+        return fail(BOXCONV_E_INVALID_ARGUMENT, "residual norm: a bias' gradient without the bias");
     if (batch == 0 || pixels == 0) {
         for (void* p : {grad_after_weight, grad_after_bias, grad_before_weight, grad_before_bias})
             if (const int rc = write_zeros(p, channels, param_dtype, "residual norm", static_cast<hipStream_t>(stream))) return rc;

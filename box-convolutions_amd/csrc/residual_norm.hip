@@ -527,9 +527,10 @@ __global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads) no
     }
 }
 
+// BIAS: whether either norm has one (sums and values that root-mean-square norms seldom need).
 // Two rows ahead are on their way while one is worked on. With twice the elements a lane (BIG) there are no registers for that, nor for the
 // parameters, which come from the caches again for every row.
-template <class T, int LANES, int E, bool RAGGED>
+template <class T, int LANES, int E, bool RAGGED, bool BIAS>
 __global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads, 2) norm_rows_grad_kernel(Rows<T> a) {
     typedef Team<T, LANES, E, RAGGED> Row;
     constexpr bool WIDE = LANES == 0, BIG = E > kPerLane;
@@ -540,12 +541,12 @@ __global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads, 2)
     Row& team = place.team;
     float sum[kSums][E] = {};
     const T* const full = a.gate_kind == kGateFull ? static_cast<const T*>(a.gate) : nullptr;
-    float wa[E], ba[E], wb[E], g[E];
+    float wa[E], ba[E] = {}, wb[E], g[E];
 #pragma unroll
     for (int i = 0; i < E; ++i) g[i] = 1.0f;
     const auto parameters = [&] {
         team.params(a.after_weight, a.float_params, 1.0f, wa);
-        team.params(a.after_bias, a.float_params, 0.0f, ba);
+        if constexpr (BIAS) team.params(a.after_bias, a.float_params, 0.0f, ba);
         team.params(a.before_weight, a.float_params, 1.0f, wb);
     };
     if constexpr (!BIG) parameters();
@@ -619,7 +620,7 @@ __global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads, 2)
             if (has_dh) {
 #pragma unroll
                 for (int k = 0; k < E; ++k) {
-                    const float u = a.after ? p[k] * wa[k] + ba[k] : p[k];
+                    const float u = a.after ? BIAS ? p[k] * wa[k] + ba[k] : p[k] * wa[k] : p[k];
                     q[k] += u * g[k] * a.scale;
                 }
                 const Moments ms = again ? team.moments(q, a.centre, a.eps) : Moments{kept[2], kept[3]};
@@ -628,7 +629,7 @@ __global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads, 2)
 #pragma unroll
                     for (int k = 0; k < E; ++k) {
                         sum[2][k] += h[k] * q[k];
-                        sum[3][k] += h[k];
+                        if constexpr (BIAS) sum[3][k] += h[k];
                     }
                 }
                 float e1 = 0.0f, e2 = 0.0f;
@@ -653,7 +654,7 @@ __global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads, 2)
 #pragma unroll
             for (int k = 0; k < E; ++k) {
                 d[k] *= a.scale;
-                h[k] = (a.after ? p[k] * wa[k] + ba[k] : p[k]) * d[k];
+                h[k] = (a.after ? BIAS ? p[k] * wa[k] + ba[k] : p[k] * wa[k] : p[k]) * d[k];
                 d[k] *= g[k];
             }
             if (a.dgate_full != nullptr && live) team.store(a.dgate_full, row, h);
@@ -662,7 +663,7 @@ __global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads, 2)
                 for (int k = 0; k < E; ++k) {
                     sum[kSumGate][k] += h[k];
                     sum[0][k] += d[k] * p[k];
-                    sum[1][k] += d[k];
+                    if constexpr (BIAS) sum[1][k] += d[k];
                 }
             }
             if (a.after) {
@@ -702,7 +703,7 @@ __global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads, 2)
     }
 #pragma unroll
     for (int k = 0; k < kSums; ++k)
-        if (a.wanted >> k & 1) put(sum[k], a.sums, (static_cast<int64_t>(blockIdx.x) * kSums + k) * a.channels, true);
+        if ((BIAS || k % 2 == 0) && (a.wanted >> k & 1)) put(sum[k], a.sums, (static_cast<int64_t>(blockIdx.x) * kSums + k) * a.channels, true);
 }
 
 // ---- sums over workgroups -----------------------------------------------------------------------------------------
@@ -850,7 +851,12 @@ hipError_t residual_norm_backward(const ResidualNormCall& c, const ResidualNormG
     else
         known(c.channels % (s.big ? 2 * kPerLane : kPerLane) != 0, [&](auto ragged) {
             constexpr bool R = decltype(ragged)::value;
-            known_lanes<1>(s, [&](auto lanes, auto each) { BOXCONV_LAUNCH("norm_rows_grad", (norm_rows_grad_kernel<T, decltype(lanes)::value, decltype(each)::value, R>), grid, block, 0, stream, a); });
+            known(c.after_bias != nullptr || c.before_bias != nullptr, [&](auto bias) {
+                known_lanes<1>(s, [&](auto lanes, auto each) {
+                    BOXCONV_LAUNCH("norm_rows_grad", (norm_rows_grad_kernel<T, decltype(lanes)::value, decltype(each)::value, R, decltype(bias)::value>), grid, block, 0,
+                                   stream, a);
+                });
+            });
         });
     bool any = false;
     for (void* p : to.p) any = any || p != nullptr;

@@ -417,7 +417,7 @@ int boxconv_residual_norm_forward(const void* input, const void* residual, const
 size_t boxconv_residual_norm_statistics_bytes(int64_t batch, int64_t pixels, int channels);
 /* Its gradients; those whose pointer is null are not formed. grad_stream, grad_normed: the gradients of s and h, null: 0.
  * statistics: the forward call's with the same input, residual, gate and after-norm, or null: formed again.
- * grad_gate has the gate's type and shape, the parameters' gradients param_dtype. Sums over no rows are 0. All other arguments as
+ * grad_gate has the gate's type and shape, the parameters' gradients param_dtype (a bias' only where there is that bias). Sums over no rows are 0. All other arguments as
  * in the forward call; the workspace (boxconv_residual_norm_workspace_bytes) is 16-byte aligned. */
 size_t boxconv_residual_norm_workspace_bytes(int64_t batch, int64_t pixels, int channels, int gate_kind, int dtype);
 int boxconv_residual_norm_backward(const void* input, const void* residual, const void* gate, int gate_kind, int gate_dtype,
