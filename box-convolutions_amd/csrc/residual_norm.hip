@@ -242,13 +242,14 @@ struct Team {
     int turn = 0;
     Chunk keep[RAGGED ? NV : 1];
 
-    __device__ __forceinline__ int column(int v) const { return lane * E + v * V; }
-    // whether element k of the lane's lies in the row (without RAGGED a lane's lie there all or none)
-    __device__ __forceinline__ bool inside(int k) const { return lane * E + (RAGGED ? k : 0) < channels; }
+    // columns of element k and of vector v: kPerLane neighbouring ones, and as many again behind those of all lanes
+    __device__ __forceinline__ int column_at(int k) const { return k / kPerLane * static_cast<int>(blockDim.x) * kPerLane + lane * kPerLane + k % kPerLane; }
+    __device__ __forceinline__ int column(int v) const { return column_at(v * V); }
+    // whether element k of the lane's lies in the row (without RAGGED kPerLane of them lie there or none)
+    __device__ __forceinline__ bool inside(int k) const { return column_at(RAGGED ? k : k / kPerLane * kPerLane) < channels; }
 
     // Vectors of a row, as they lie in memory. RAGGED: the last one runs into the next row, whose elements settle() takes away; `clear` says that
-    // no row of the wave's ends within a vector of the tensor's end, where that would be out of bounds: there it is read as the row's last
-    // whole vector and shifted at once.
+    // no row of the wave's ends within a vector of the tensor's end, where that would be out of bounds: there it is read element by element.
     __device__ __forceinline__ void request(const T* tensor, int64_t row, bool clear, Chunk (&raw)[NV]) const {
         if (tensor == nullptr) return;
         const T* p = tensor + row * channels;
@@ -256,11 +257,7 @@ struct Team {
         for (int v = 0; v < NV; ++v) {
             const int c = column(v), n = channels - c;
             if (!RAGGED || clear) raw[v] = n > 0 ? __builtin_bit_cast(Chunk, *reinterpret_cast<const typename Vec<T>::Type*>(p + c)) : Chunk{0, 0, 0, 0};
-            else if (channels < V) raw[v] = short_chunk(p + c, n);
-            else {
-                raw[v] = request_chunk(p + c, n, tensor);
-                settle_chunk<T>(raw[v], n);
-            }
+            else raw[v] = short_chunk(p + c, n);
         }
     }
     __device__ __forceinline__ bool clear_of_end(int64_t last_row, int64_t rows) const { return (rows - 1 - last_row) * channels >= V; }
@@ -329,11 +326,11 @@ struct Team {
         if (is_float) {
 #pragma unroll
             for (int i = 0; i < E; ++i)
-                if (inside(i)) out[i] = static_cast<const float*>(p)[column(0) + i];
+                if (inside(i)) out[i] = static_cast<const float*>(p)[column_at(i)];
         } else {
 #pragma unroll
             for (int i = 0; i < E; ++i)
-                if (inside(i)) out[i] = static_cast<float>(static_cast<const T*>(p)[column(0) + i]);
+                if (inside(i)) out[i] = static_cast<float>(static_cast<const T*>(p)[column_at(i)]);
         }
     }
     // Over the row: the sums of a and b, the same in all its lanes.
@@ -382,10 +379,9 @@ struct Team {
                 part = 1.0f / static_cast<float>(max(count, 1));
             }
             m.mean = sum * part;
-            const float from = RAGGED || inside(0) ? m.mean : 0.0f;
 #pragma unroll
             for (int i = 0; i < E; ++i) {
-                const float d = RAGGED && !inside(i) ? 0.0f : value[i] - from;
+                const float d = RAGGED ? inside(i) ? value[i] - m.mean : 0.0f : value[i] - (inside(i) ? m.mean : 0.0f);
                 square += d * d;
             }
             square = sum_of_lanes(square, WIDE ? 64 : LANES);
@@ -408,13 +404,20 @@ struct Team {
     }
     // (value - mean) * rstd, 0 beyond the row (whose values are 0).
     __device__ __forceinline__ void normalise(float (&value)[E], const Moments& m) const {
-        const bool in = RAGGED || inside(0);
-        const float mean = in ? m.mean : 0.0f, rstd = in ? m.rstd : 0.0f;
 #pragma unroll
-        for (int i = 0; i < E; ++i) value[i] = RAGGED && !inside(i) ? 0.0f : (value[i] - mean) * rstd;
+        for (int i = 0; i < E; ++i) {
+            const bool in = inside(i);
+            value[i] = RAGGED ? in ? (value[i] - m.mean) * m.rstd : 0.0f : (value[i] - (in ? m.mean : 0.0f)) * (in ? m.rstd : 0.0f);
+        }
     }
     // Elements of the row in wave w.
-    __device__ __forceinline__ int in_wave(int w) const { return min(max(channels - w * 64 * E, 0), 64 * E); }
+    __device__ __forceinline__ int in_wave(int w) const {
+        constexpr int kWave = 64 * kPerLane;
+        int n = 0;
+#pragma unroll
+        for (int k = 0; k < E; k += kPerLane) n += min(max(channels - k * static_cast<int>(blockDim.x) - w * kWave, 0), kWave);
+        return n;
+    }
 };
 
 // The team of this thread, the first row of its wave's next ones (from 0 on), its own place among them, and how far apart they are.
@@ -510,16 +513,22 @@ __global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads) no
             if constexpr (!CODES) {
                 if (live) team.store(a.normed, row, x);
             } else {
-                const int blocks = blocks_of(a.channels), words = exponents_of(a.channels), c = team.column(0), b = c / kBlock;
-                const int e = block_exponent(most_of_lanes(largest(x), kBlock / E));
-                const Codes<E> codes = to_codes(x, e);
-                if (live && b < blocks) {
-                    typedef unsigned Words __attribute__((ext_vector_type(E / 4)));
-                    *reinterpret_cast<Words*>(a.codes + row * blocks * kBlock + c) = __builtin_bit_cast(Words, codes);
-                    if (c % kBlock == 0) {
-                        a.exponents[row * words + b] = static_cast<uint8_t>(e);
-                        if (b == blocks - 1)
-                            for (int w = blocks; w < words; ++w) a.exponents[row * words + w] = 127;
+                const int blocks = blocks_of(a.channels), words = exponents_of(a.channels);
+#pragma unroll
+                for (int k = 0; k < E; k += kPerLane) {
+                    float part[kPerLane];
+#pragma unroll
+                    for (int j = 0; j < kPerLane; ++j) part[j] = x[k + j];
+                    const int e = block_exponent(most_of_lanes(largest(part), kBlock / kPerLane)), c = team.column_at(k), b = c / kBlock;
+                    const Codes<kPerLane> codes = to_codes(part, e);
+                    if (live && b < blocks) {
+                        typedef unsigned Words __attribute__((ext_vector_type(kPerLane / 4)));
+                        *reinterpret_cast<Words*>(a.codes + row * blocks * kBlock + c) = __builtin_bit_cast(Words, codes);
+                        if (c % kBlock == 0) {
+                            a.exponents[row * words + b] = static_cast<uint8_t>(e);
+                            if (b == blocks - 1)
+                                for (int w = blocks; w < words; ++w) a.exponents[row * words + w] = 127;
+                        }
                     }
                 }
             }
@@ -560,7 +569,7 @@ __global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads, 2)
         if constexpr (WIDE) {
 #pragma unroll
             for (int k = 0; k < E; ++k)
-                if (team.inside(k)) write(team.column(0) + k, v[k]);
+                if (team.inside(k)) write(team.column_at(k), v[k]);
         } else {
             __syncthreads();
 #pragma unroll
@@ -642,11 +651,10 @@ __global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads, 2)
                 team.pair_sum(e1, e2);
                 e1 = a.centre ? e1 * team.inverse : 0.0f;
                 e2 *= team.inverse;
-                const float rstd = RAGGED || team.inside(0) ? ms.rstd : 0.0f;
 #pragma unroll
                 for (int k = 0; k < E; ++k) {
-                    const float through = rstd * (h[k] - e1 - q[k] * e2);
-                    d[k] += RAGGED && !team.inside(k) ? 0.0f : through;
+                    const float through = h[k] - e1 - q[k] * e2;
+                    d[k] += RAGGED ? team.inside(k) ? ms.rstd * through : 0.0f : (team.inside(k) ? ms.rstd : 0.0f) * through;
                 }
             }
             if (a.dresidual != nullptr && live) team.store(a.dresidual, row, d);
@@ -811,7 +819,7 @@ hipError_t residual_norm_forward(const ResidualNormCall& c, const ResidualNormOu
     const dim3 grid(static_cast<unsigned>(a.plan.groups)), block(s.threads);
     if (s.lanes == 0) BOXCONV_LAUNCH("norm_rows", (norm_rows_any_kernel<T>), grid, block, 0, stream, a);
     else
-        known(c.channels % (s.big ? 2 * kPerLane : kPerLane) != 0, [&](auto ragged) {
+        known(c.channels % kPerLane != 0, [&](auto ragged) {
             constexpr bool R = decltype(ragged)::value;
             if (coded)
                 known_lanes<kBlock / kPerLane>(s, [&](auto lanes, auto each) { BOXCONV_LAUNCH("norm_rows", (norm_rows_kernel<T, decltype(lanes)::value, decltype(each)::value, R, true>), grid, block, 0, stream, a); });
@@ -849,7 +857,7 @@ hipError_t residual_norm_backward(const ResidualNormCall& c, const ResidualNormG
     const dim3 grid(static_cast<unsigned>(a.plan.groups)), block(s.threads);
     if (s.lanes == 0) BOXCONV_LAUNCH("norm_rows_grad", (norm_rows_any_grad_kernel<T>), grid, block, 0, stream, a);
     else
-        known(c.channels % (s.big ? 2 * kPerLane : kPerLane) != 0, [&](auto ragged) {
+        known(c.channels % kPerLane != 0, [&](auto ragged) {
             constexpr bool R = decltype(ragged)::value;
             known(c.after_bias != nullptr || c.before_bias != nullptr, [&](auto bias) {
                 known_lanes<1>(s, [&](auto lanes, auto each) {
