@@ -323,14 +323,24 @@ struct Team {
 #pragma unroll
         for (int i = 0; i < E; ++i) out[i] = none;
         if (p == nullptr) return;
-        if (is_float) {
+        if (is_float) run(static_cast<const float*>(p), out);
+        else run(static_cast<const T*>(p), out);
+    }
+    template <class P>
+    __device__ __forceinline__ void run(const P* p, float (&out)[E]) const {
+        typedef P Run __attribute__((ext_vector_type(kPerLane), aligned(sizeof(P))));
 #pragma unroll
-            for (int i = 0; i < E; ++i)
-                if (inside(i)) out[i] = static_cast<const float*>(p)[column_at(i)];
-        } else {
+        for (int k = 0; k < E; k += kPerLane) {
+            const int c = column_at(k);
+            if (c + kPerLane <= channels) {
+                const Run v = *reinterpret_cast<const Run*>(p + c);
 #pragma unroll
-            for (int i = 0; i < E; ++i)
-                if (inside(i)) out[i] = static_cast<float>(static_cast<const T*>(p)[column_at(i)]);
+                for (int j = 0; j < kPerLane; ++j) out[k + j] = static_cast<float>(v[j]);
+            } else if (RAGGED) {
+#pragma unroll
+                for (int j = 0; j < kPerLane; ++j)
+                    if (c + j < channels) out[k + j] = static_cast<float>(p[c + j]);
+            }
         }
     }
     // Over the row: the sums of a and b, the same in all its lanes.
@@ -553,12 +563,15 @@ __global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads, 2)
     float wa[E], ba[E] = {}, wb[E], g[E];
 #pragma unroll
     for (int i = 0; i < E; ++i) g[i] = 1.0f;
-    const auto parameters = [&] {
+    const auto after_parameters = [&] {
         team.params(a.after_weight, a.float_params, 1.0f, wa);
         if constexpr (BIAS) team.params(a.after_bias, a.float_params, 0.0f, ba);
-        team.params(a.before_weight, a.float_params, 1.0f, wb);
     };
-    if constexpr (!BIG) parameters();
+    const auto before_parameters = [&] { team.params(a.before_weight, a.float_params, 1.0f, wb); };
+    if constexpr (!BIG) {
+        after_parameters();
+        before_parameters();
+    }
     const bool has_dh = a.before && a.dnormed != nullptr;
     // sum k of the workgroup's teams to memory
     const auto put = [&](const float (&v)[E], void* to, int64_t at, bool is_float) {
@@ -607,7 +620,7 @@ __global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads, 2)
             const bool live = row < span.last;
             if constexpr (BIG) {
                 request(base, raw);
-                parameters();
+                after_parameters();
                 item_gate(team, a, span.item, g);
             }
             float p[E], q[E], d[E], h[E];                              // normalised x, normalised s, gradients of s and h; later what they become
@@ -641,6 +654,7 @@ __global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads, 2)
                         if constexpr (BIAS) sum[3][k] += h[k];
                     }
                 }
+                if constexpr (BIG) before_parameters();
                 float e1 = 0.0f, e2 = 0.0f;
 #pragma unroll
                 for (int k = 0; k < E; ++k) {
@@ -658,6 +672,11 @@ __global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads, 2)
                 }
             }
             if (a.dresidual != nullptr && live) team.store(a.dresidual, row, d);
+            if constexpr (BIG) {                                       // (again: they would wait in registers, or in memory)
+                asm volatile("" ::: "memory");
+                after_parameters();
+                item_gate(team, a, span.item, g);
+            }
             // d: gradient of s, then of u; h: of the gate
 #pragma unroll
             for (int k = 0; k < E; ++k) {
