@@ -492,8 +492,8 @@ class ResidualNorm(torch.nn.Module):
 class PointwiseConv2dFloat8(torch.nn.Module):
     """The inference form of a ``PointwiseConv2d`` (or 1 x 1 ``torch.nn.Conv2d``) in 8 bits: ``PointwiseConv2dFloat8(conv)`` quantizes its
     weight once; ``module(x, residual=None)`` takes ``[B, C, h, w]`` values of the bias's type, or the ``Float8Blocks`` ``[B, h, w, C]``
-    of a quantizing ``ResidualNorm``, and returns ``[B, out_channels, h, w]`` in channels-last memory. Codes, exponents and bias
-    are buffers."""
+    of a quantizing ``ResidualNorm``, and returns ``[B, out_channels, h, w]`` in channels-last memory, of the values' type, or the bias's
+    (without a bias, the convolution's) for blocks. Codes (as bytes), exponents and bias are buffers."""
 
     def __init__(self, conv, activation=None):
         super().__init__()
@@ -505,7 +505,7 @@ class PointwiseConv2dFloat8(torch.nn.Module):
         self.in_channels, self.out_channels, self.dtype = conv.in_channels, conv.out_channels, conv.weight.dtype
         with torch.no_grad():
             weight = quantize_blocks(conv.weight.flatten(1))
-        self.register_buffer("codes", weight.codes)
+        self.register_buffer("codes", weight.codes.view(torch.uint8))        # (as bytes: module.to(dtype) converts floating-point buffers)
         self.register_buffer("exponents", weight.exponents)
         self.register_buffer("bias", None if conv.bias is None else conv.bias.detach().clone())
 
@@ -513,8 +513,10 @@ class PointwiseConv2dFloat8(torch.nn.Module):
         coded = isinstance(input, Float8Blocks)
         if len(input.shape) != 4:
             raise RuntimeError("PointwiseConv2dFloat8: input must have 4 dimensions")
-        y = linear_act_float8(input if coded else input.permute(0, 2, 3, 1), Float8Blocks(self.codes, self.exponents, self.in_channels), self.bias,
-                              None if residual is None else residual.permute(0, 2, 3, 1), self.activation, self.dtype if coded else None)
+        weight = Float8Blocks(self.codes.view(torch.float8_e4m3fn), self.exponents, self.in_channels)
+        dtype = None if not coded else self.dtype if self.bias is None else self.bias.dtype
+        y = linear_act_float8(input if coded else input.permute(0, 2, 3, 1), weight, self.bias, None if residual is None else residual.permute(0, 2, 3, 1),
+                              self.activation, dtype)
         return y.permute(0, 3, 1, 2)
 
     def extra_repr(self):

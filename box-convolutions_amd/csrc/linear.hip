@@ -639,11 +639,21 @@ hipError_t linear_backward(const LinearGradCall& c, void* workspace, hipStream_t
 // ---- 8-bit rows ------------------------------------------------------------------------------------------------------
 namespace {
 
+// (Rows of tiles go over launches where a grid would have 2^32 threads or more, as launch_product has them.)
 template <class T, int TM, int TN, int WM, int WN>
-void launch_float8(const Coded& a, const Coded& b, const Tail<T>& tail, const ProductPlan& p, hipStream_t stream) {
+void launch_float8(Coded a, const Coded& b, Tail<T> tail, const ProductPlan& p, hipStream_t stream) {
     constexpr size_t lds = kRing * sizeof(Chunk) * (TileShape<Code, true, TM, 8>::kChunks + TileShape<Code, true, TN, 8>::kChunks) + 2 * (TM + TN) * sizeof(unsigned);
-    BOXCONV_LAUNCH("linear_float8", (product_float8_kernel<T, TM, TN, WM, WN>), dim3(static_cast<unsigned>(p.tiles_m * p.tiles_n), p.splits), dim3(WM * WN * 64), lds, stream,
-                   a, b, tail, static_cast<int>(p.k_part / kBlock), static_cast<unsigned>(p.tiles_m), static_cast<unsigned>(p.tiles_n));
+    const int64_t rows = a.extent, most = std::max<int64_t>(1, kMostThreads / (WM * WN * 64) / p.tiles_n) * TM;
+    for (int64_t m = 0; m < rows; m += most) {
+        tail.rows = a.extent = std::min(most, rows - m);
+        const int64_t tiles_m = (a.extent + TM - 1) / TM;
+        BOXCONV_LAUNCH("linear_float8", (product_float8_kernel<T, TM, TN, WM, WN>), dim3(static_cast<unsigned>(tiles_m * p.tiles_n), p.splits), dim3(WM * WN * 64), lds,
+                       stream, a, b, tail, static_cast<int>(p.k_part / kBlock), static_cast<unsigned>(tiles_m), static_cast<unsigned>(p.tiles_n));
+        a.codes += most * a.blocks * kBlock;
+        a.exponents += most * a.padded;
+        tail.out += most * tail.cols;
+        if (tail.residual != nullptr) tail.residual += most * tail.ld_residual;
+    }
 }
 
 // The plan of 16-bit products, a stage of 128 bytes being a block here; parts of k are whole words of exponents. (Results in float32: no tiles of

@@ -818,9 +818,10 @@ void known_lanes(const Shape& s, F f) {
     f(std::integral_constant<int, LEAST>(), Each());
 }
 
-// As many workgroups as the chip holds at once: the forward's kernels leave room for four waves a SIMD, the backward's for two.
+// As many workgroups as the chip holds at once: the forward's kernels leave room for four waves a SIMD, the backward's for two. (Fewer where the
+// backward's sums are long and in memory.)
 RowPlan forward_plan(const ResidualNormCall& c, const Shape& s) { return plan_rows(c, 256 * 16 * 64 / s.threads, s.rows); }
-RowPlan backward_plan(const ResidualNormCall& c, const Shape& s) { return plan_rows(c, 256 * 8 * 64 / std::min(s.threads, 512), s.rows); }
+RowPlan backward_plan(const ResidualNormCall& c, const Shape& s) { return plan_rows(c, s.lanes == 0 ? 128 : 256 * 8 * 64 / s.threads, s.rows); }
 
 }  // namespace
 

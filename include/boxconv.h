@@ -395,7 +395,7 @@ int boxconv_linear_backward(const void* input, int64_t ld_input, const void* wei
  *   u = n(input; after_weight, after_bias) with BOXCONV_NORM_AFTER, else the input,
  *   s = residual + scale * gate * u   (null residual: 0; gate_kind BOXCONV_GATE_NONE: 1),
  *   h = n(s; before_weight, before_bias) with BOXCONV_NORM_BEFORE:
- * stream_output receives s, normed receives h, formed from s before it is rounded. Either may be null. norms is the sum of the
+ * stream_output receives s, normed receives h, formed from s before it is rounded. Either may be null; they overlap no input. norms is the sum of the
  * flags. Weights and biases [channels] have param_dtype (BOXCONV_F32 or dtype); null: 1, 0. The gate has gate_dtype (the same
  * choice) and as many values as its kind says: one per channel, [batch][channels], or, of type dtype, as the input has.
  * statistics: null, or boxconv_residual_norm_statistics_bytes (0 for rows that do without, to be given as null) that receive what the

@@ -130,3 +130,40 @@ def test_modules_hold_what_they_say():
     m = ResidualNorm(8, kind="layer", layer_scale=1e-4)
     assert sorted(n for n, _ in m.named_parameters()) == ["after_bias", "after_weight", "before_bias", "before_weight", "layer_scale"]
     assert sorted(n for n, _ in ResidualNorm(8, before=False).named_parameters()) == ["after_weight"] and "rms" in repr(ResidualNorm(8))
+
+
+@pytest.mark.parametrize("call", ["residual_norm_backward", "linear_float8"])
+def test_scratch_of_calls_that_overlap(monkeypatch, call):
+    """While one call's kernels are being launched, another thread's must not get the same scratch memory. (The native library is replaced by one
+    that starts the other call from within the first.)"""
+    import contextlib
+    import threading
+    from box_convolution import _native
+    x, w, g = torch.zeros(6, 8), torch.zeros(8, 128).to(torch.float8_e4m3fn), torch.zeros(6, 8)
+    e, one = torch.zeros(8, 4, dtype=torch.uint8), torch.ones(8)
+    calls = {"residual_norm_backward": lambda: _native.residual_norm_backward(x, None, None, 0, 1.0, 1, [one, None, None, None], 1e-6, None, g, None,
+                                                                              (True, False, False, True, False, False, False)),
+             "linear_float8": lambda: _native.linear_float8_forward(x, None, w, e, 8, None, None, None, torch.float32)}
+    seen = []
+
+    class Library:
+        def __getattr__(self, name):
+            return self.workspace_bytes if name.endswith("workspace_bytes") else self.entry
+
+        def workspace_bytes(self, *args):
+            return 256
+
+        def entry(self, *args):
+            seen.append(args[-3])
+            if len(seen) == 1:
+                other = threading.Thread(target=calls[call])
+                other.start()
+                other.join()
+            return 0
+    library = Library()
+    monkeypatch.setattr(_native, "load", lambda: library)
+    monkeypatch.setattr(_native, "_on_device", lambda device: contextlib.nullcontext())
+    monkeypatch.setattr(_native, "_stream", lambda device: 0)
+    monkeypatch.setattr(_native, "_workspace_bytes", {})
+    calls[call]()
+    assert len(seen) == 2 and None not in seen and seen[0] != seen[1]

@@ -425,6 +425,21 @@ def test_more_than_2_31_elements(hip):
             assert torch.equal(a[k * small:(k + 1) * small], b)
 
 
+@pytest.mark.parametrize("C", [520, 4097, 6000, 9001])
+def test_kept_statistics_are_those_formed_again(hip, C):
+    """The backward with the forward's statistics and without them: the same bits."""
+    c = case(2, C, (5,), torch.bfloat16, "layer", "item")
+    dev = {k: t.detach() for k, t in placed(c)[0].items()}
+    dev = {k: t.movedim(1, -1) if k in ("x", "residual") else t for k, t in dev.items()}
+    norms = hip.NORM_AFTER | hip.NORM_BEFORE | hip.NORM_CENTRE
+    begin = (dev["x"], dev["residual"], dev["gate"], hip.GATE_ITEM, 0.5, norms, [dev[k] for k in LEAVES[3:]], 1e-6)
+    statistics = hip.residual_norm_forward(*begin, True, None, True)[2]
+    assert statistics.numel() == 2 * 5 * 4 and hip.residual_norm_forward(*begin, True)[2] is None
+    grads = [c[k].cuda() for k in ("grad_stream", "grad_normed")]
+    kept, again = (hip.residual_norm_backward(*begin, s, *grads, (True,) * 7) for s in (statistics, None))
+    assert all(torch.equal(a, b) for a, b in zip(kept, again))
+
+
 def test_random_sizes(hip):
     """Forty draws of everything at once."""
     rng = random.Random(5)
