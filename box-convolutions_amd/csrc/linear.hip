@@ -640,14 +640,14 @@ hipError_t linear_backward(const LinearGradCall& c, void* workspace, hipStream_t
 namespace {
 
 // (Rows of tiles go over launches where a grid would have 2^32 threads or more, as launch_product has them.)
-template <class T, int TM, int TN, int WM, int WN>
+template <class T, int TM, int TN, int WM, int WN, int RING>
 void launch_float8(Coded a, const Coded& b, Tail<T> tail, const ProductPlan& p, hipStream_t stream) {
-    constexpr size_t lds = kRing * sizeof(Chunk) * (TileShape<Code, true, TM, 8>::kChunks + TileShape<Code, true, TN, 8>::kChunks) + 2 * (TM + TN) * sizeof(unsigned);
+    constexpr size_t lds = RING * sizeof(Chunk) * (TileShape<Code, true, TM, 8>::kChunks + TileShape<Code, true, TN, 8>::kChunks) + 2 * (TM + TN) * sizeof(unsigned);
     const int64_t rows = a.extent, most = std::max<int64_t>(1, kMostThreads / (WM * WN * 64) / p.tiles_n) * TM;
     for (int64_t m = 0; m < rows; m += most) {
         tail.rows = a.extent = std::min(most, rows - m);
         const int64_t tiles_m = (a.extent + TM - 1) / TM;
-        BOXCONV_LAUNCH("linear_float8", (product_float8_kernel<T, TM, TN, WM, WN>), dim3(static_cast<unsigned>(tiles_m * p.tiles_n), p.splits), dim3(WM * WN * 64), lds,
+        BOXCONV_LAUNCH("linear_float8", (product_float8_kernel<T, TM, TN, WM, WN, RING>), dim3(static_cast<unsigned>(tiles_m * p.tiles_n), p.splits), dim3(WM * WN * 64), lds,
                        stream, a, b, tail, static_cast<int>(p.k_part / kBlock), static_cast<unsigned>(tiles_m), static_cast<unsigned>(p.tiles_n));
         a.codes += most * a.blocks * kBlock;
         a.exponents += most * a.padded;
@@ -751,12 +751,20 @@ hipError_t linear_float8_forward(const LinearFloat8Call& c, void* workspace, hip
         if (const hipError_t e = quantize_launch(q, stream); e != hipSuccess) return e;
     }
     if (p.splits > 1) tail.partial = static_cast<float*>(workspace);
+    // few workgroups for a compute unit: what hides a load's way is more stages, not more workgroups
+    const int64_t groups = p.tiles_m * p.tiles_n * p.splits;
+    const bool few = groups <= (p.shape == 1 ? 256 : 512);
     switch (p.shape) {
         case 0:
-            if constexpr (sizeof(T) == 2) launch_float8<T, 256, 256, 4, 2>(a, b, tail, p, stream);
+            if constexpr (sizeof(T) == 2) launch_float8<T, 256, 256, 4, 2, 2>(a, b, tail, p, stream);
             break;
-        case 1: launch_float8<T, 128, 128, 2, 2>(a, b, tail, p, stream); break;
-        default: launch_float8<T, 64, 64, 2, 2>(a, b, tail, p, stream);
+        case 1:
+            if (few) launch_float8<T, 128, 128, 2, 2, 4>(a, b, tail, p, stream);
+            else launch_float8<T, 128, 128, 2, 2, 2>(a, b, tail, p, stream);
+            break;
+        default:
+            if (few) launch_float8<T, 64, 64, 2, 2, 4>(a, b, tail, p, stream);
+            else launch_float8<T, 64, 64, 2, 2, 2>(a, b, tail, p, stream);
     }
     if (p.splits > 1) join_parts(tail, p.splits, stream);
     return hipGetLastError();

@@ -69,11 +69,11 @@ __device__ __forceinline__ void word_to_lds(Descriptor d, unsigned offset, unsig
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(to), "v"(offset), "s"(d) : "m0");
 }
 
-// TM x TN tile by WM x WN waves, each with (TM/WM) x (TN/WN), as in product_wide_kernel: two stages of LDS, each a block of 128 codes of every
-// row. A block is two steps of 64 values of k. The barrier stands between them: the second step's fragments are in registers by then, so the
-// stage takes the block after next, whose loads go out one at a time between the second step's products. Exponents come four blocks at a time, a
+// TM x TN tile by WM x WN waves, each with (TM/WM) x (TN/WN), as in product_wide_kernel: RING stages of LDS (a power of two), each a block of 128
+// codes of every row. A block is two steps of 64 values of k. The barrier stands between them: the second step's fragments are in registers by then, so the
+// stage takes a block RING further on, whose loads go out one at a time between the second step's products. Exponents come four blocks at a time, a
 // word of every row, into a ring of their own; a lane keeps the words of its rows and shifts them by a byte from block to block.
-template <class T, int TM, int TN, int WM, int WN>
+template <class T, int TM, int TN, int WM, int WN, int RING>
 __global__ void __launch_bounds__(WM * WN * 64)
 product_float8_kernel(Coded a, Coded b, Tail<T> tail, int part_blocks, unsigned tiles_m, unsigned tiles_n) {
     typedef TileShape<Code, true, TM, 8> SA;
@@ -82,7 +82,7 @@ product_float8_kernel(Coded a, Coded b, Tail<T> tail, int part_blocks, unsigned 
     constexpr int kStage = SA::kChunks + SB::kChunks;
     static_assert(TM % 64 == 0 && TN % 64 == 0 && SA::KT == kBlock, "whole waves of rows; a block a stage");
     extern __shared__ Chunk stages[];
-    unsigned* const words = reinterpret_cast<unsigned*>(stages + kRing * kStage);          // [2][TM + TN]
+    unsigned* const words = reinterpret_cast<unsigned*>(stages + RING * kStage);           // [2][TM + TN]
     unsigned tm, tn, part;
     tile_of(tiles_m, tiles_n, tm, tn, part);
     const int64_t m0 = static_cast<int64_t>(tm) * TM, n0 = static_cast<int64_t>(tn) * TN;
@@ -118,7 +118,7 @@ product_float8_kernel(Coded a, Coded b, Tail<T> tail, int part_blocks, unsigned 
     };
     Descriptor da, db;
     const auto load = [&](int s, int i) {
-        const Chunk* tile = stages + s % kRing * kStage;
+        const Chunk* tile = stages + s % RING * kStage;
         const int k_left = (steps - s) * kBlock;
         if (i == 0) da = fa.next();
         if (i == FeedA::N) db = fb.next();
@@ -129,7 +129,7 @@ product_float8_kernel(Coded a, Coded b, Tail<T> tail, int part_blocks, unsigned 
     // every other replaces its own (two sets of B as well do not fit the registers of 256 x 256 tiles).
     Codes32 xa[2][FM], xb[FN + 1];
     const auto take = [&](int s, int h, int f) {
-        const Chunk* tile = stages + s % kRing * kStage;
+        const Chunk* tile = stages + s % RING * kStage;
         return f < FM ? Codes32{fragment<Code, true, TM, 8, false>(tile, wm + 32 * f, 2 * h), fragment<Code, true, TM, 8, false>(tile, wm + 32 * f, 2 * h + 1)}
                       : Codes32{fragment<Code, true, TN, 8, true>(tile + SA::kChunks, wn + 32 * (f - FM), 2 * h),
                                 fragment<Code, true, TN, 8, true>(tile + SA::kChunks, wn + 32 * (f - FM), 2 * h + 1)};
@@ -157,16 +157,20 @@ product_float8_kernel(Coded a, Coded b, Tail<T> tail, int part_blocks, unsigned 
         }
     };
     if (steps > 0) {
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) load(0, i);
         load_words(first / 4);
-        settle<0>();
+#pragma unroll
+        for (int s = 0; s < RING - (RING == 2); ++s)
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) load(s, i);
+        settle<RING == 2 ? 0 : (RING - 1) * kLoads>();         // stage 0 and the words have landed
 #pragma unroll
         for (int i = 0; i < FM; ++i) xa[0][i] = take(0, 0, i);
 #pragma unroll
         for (int i = 0; i < FN; ++i) xb[slot(0, i)] = take(0, 0, FM + i);
+        if constexpr (RING == 2) {
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) load(1, i);
+            for (int i = 0; i < kLoads; ++i) load(1, i);
+        }
     }
     for (int s = 0; s < steps; ++s) {
         if (s % 4 == 0) {
@@ -179,15 +183,18 @@ product_float8_kernel(Coded a, Coded b, Tail<T> tail, int part_blocks, unsigned 
             load_words(group + 1);
         }
         step(0, s, -1);
-        settle<0>();                                           // stage s + 1 has landed, and the rest of this one is in registers
-        step(1, s + 1, s + 2);
+        // stage s + 1 has landed, and the rest of this one is in registers. (Words are older than the loads of the three stages behind them by the
+        // time that they are used.)
+        static_assert(RING <= 4, "words land in time");
+        settle<(RING - 2) * kLoads>();
+        step(1, s + 1, s + RING);
 #pragma unroll
         for (int i = 0; i < FM; ++i) ea[i] >>= 8;
 #pragma unroll
         for (int i = 0; i < FN; ++i) eb[i] >>= 8;
     }
     settle<0>();                                               // every wave's loads have landed and its fragments are read: the LDS is free
-    static_assert(WM * WN * 256 * FN <= kRing * kStage, "each wave turns its sums in a part of the stages");
+    static_assert(WM * WN * 256 * FN <= RING * kStage, "each wave turns its sums in a part of the stages");
     store_blocks<T, FN, FM>(tail, acc, m0 + wm, n0 + wn, part, stages + wave * 256 * FN);
 }
 
