@@ -28,10 +28,21 @@ __global__ void __launch_bounds__(256) quantize_kernel(QuantizeCall q, I blocks,
             block[i] = id - static_cast<I>(row[i]) * blocks;
             const int64_t c = static_cast<int64_t>(block[i]) * kBlock + sub * PER, left = q.columns - c;
             const T* p = static_cast<const T*>(q.x) + row[i] * q.ld + c;
+            // the last values of a row: whole vectors that run into what follows, while that is inside the tensor, and a mask (element by element every
+            // wave waits for them in turn: 10000 x 1001 float32 20.4 us, 11.5 this way)
+            const bool clear = (q.rows - 1 - row[i]) * q.ld + q.columns >= static_cast<int64_t>(blocks) * kBlock;
+            if (left >= PER || (clear && left > 0)) {
 #pragma unroll
-            for (int v = 0; v < NV; ++v) {
-                if (left >= (v + 1) * V) raw[i][v] = *reinterpret_cast<const Packed*>(p + v * V);
-                else {
+                for (int v = 0; v < NV; ++v) raw[i][v] = *reinterpret_cast<const Packed*>(p + v * V);
+                if (left < PER) {
+#pragma unroll
+                    for (int v = 0; v < NV; ++v)
+#pragma unroll
+                        for (int j = 0; j < V; ++j) raw[i][v][j] = v * V + j < left ? raw[i][v][j] : static_cast<T>(0.0f);
+                }
+            } else {
+#pragma unroll
+                for (int v = 0; v < NV; ++v) {
                     Packed part = {};
 #pragma unroll
                     for (int j = 0; j < V; ++j)

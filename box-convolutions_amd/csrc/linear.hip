@@ -671,14 +671,22 @@ ProductPlan plan_float8(int64_t rows, int64_t K, int64_t N) {
     return p;
 }
 
-constexpr int64_t kFewRows = 32;           // whose product takes one launch, values or codes
+// Few rows take one launch, values too while quantizing them in every workgroup again costs less than another launch: 16 rows of 1024 -> 4096
+// bfloat16 5.5 us as values or codes, of 4096 12.2 and 7.4, of 8192 -> 2048 20.6 and 11.9, where quantizing takes 3 to 4; 32 rows of 2048 -> 4096 11.0 and 7.7.
+// (64 rows this way were no better than tiles: 1024 -> 4096 7.4 and 7.8, 4096 -> 4096 20 and 12.)
+constexpr int64_t kFewRows = 32, kFewRowsValues = 2048;
+
+// The bytes of rows in 8 bits, codes and then exponents.
+size_t blocks_bytes(int64_t rows, int64_t K) { return static_cast<size_t>(rows) * (blocks_of(K) * kBlock + exponents_of(K)); }
 
 template <class T, int MT, bool CODED>
 hipError_t few_rows_float8(const LinearFloat8Call& c, const Coded& a, const Coded& b, const Tail<T>& tail, hipStream_t stream) {
-    int waves = 1, ahead = 1;              // all waves with a block at least, then up to four blocks on their way for each
-    while (waves < (MT == 1 ? 8 : 4) && waves < a.blocks) waves *= 2;
-    while (ahead < 4 && ahead * waves < a.blocks) ahead *= 2;
-    const size_t lds = std::max<size_t>(static_cast<size_t>(waves) * 16 * (CODED ? MT + 1 : 1) * ahead * kBlock, static_cast<size_t>(waves) * MT * 1024);
+    // all waves with a block at least, then up to four blocks on their way for each, while two workgroups fit the LDS or one just does
+    int waves = 1, ahead = 1;
+    while (waves < (CODED && MT > 1 ? 4 : 8) && waves < a.blocks) waves *= 2;
+    const auto bytes = [&](int blocks) { return static_cast<size_t>(waves) * 16 * (CODED ? MT + 1 : 1) * blocks * kBlock; };
+    while (ahead < 4 && ahead * waves < a.blocks && bytes(2 * ahead) <= 100 * 1024) ahead *= 2;
+    const size_t lds = std::max<size_t>(bytes(ahead), static_cast<size_t>(waves) * MT * 1024);
     BOXCONV_LAUNCH("linear_float8_few_rows", (few_rows_float8_kernel<T, MT, CODED>), dim3(static_cast<unsigned>((c.N + 15) / 16)), dim3(waves * 64), lds, stream, a,
                    static_cast<const T*>(c.x), c.ld_x, c.K, b, tail, ahead);
     return hipGetLastError();
@@ -720,8 +728,8 @@ hipError_t run_narrow_float8(const LinearFloat8Call& c, const Coded& a, const Co
 // [parts of a split product][the input's codes][their exponents]
 template <class T>
 size_t linear_float8_workspace(int64_t rows, int64_t K, int64_t N, bool values) {
-    if (rows <= kFewRows || narrow_float8<T>(rows, K, N, !values)) return 0;
-    return round_up(plan_float8<T>(rows, K, N).partial_bytes) + (values ? static_cast<size_t>(rows) * (blocks_of(K) * kBlock + exponents_of(K)) : 0);
+    if (narrow_float8<T>(rows, K, N, !values) || (rows <= kFewRows && (!values || K <= kFewRowsValues))) return 0;
+    return (rows <= kFewRows ? 0 : round_up(plan_float8<T>(rows, K, N).partial_bytes)) + (values ? blocks_bytes(rows, K) : 0);
 }
 
 template <class T>
@@ -736,20 +744,25 @@ hipError_t linear_float8_forward(const LinearFloat8Call& c, void* workspace, hip
     tail.residual = static_cast<const T*>(c.residual);
     tail.ld_residual = c.ld_residual;
     tail.activation = c.activation;
-    const bool coded = c.input_dtype == kE4M3;
+    bool coded = c.input_dtype == kE4M3;
+    const ProductPlan p = plan_float8<T>(c.rows, c.K, c.N);
+    const auto quantize = [&](size_t at) {
+        QuantizeCall q = {c.x, c.ld_x, c.input_dtype, c.rows, c.K, static_cast<uint8_t*>(workspace) + at, nullptr};
+        q.exponents = q.codes + c.rows * a.blocks * kBlock;
+        a.codes = q.codes;
+        a.exponents = q.exponents;
+        coded = true;
+        return quantize_launch(q, stream);
+    };
     if (c.rows <= kFewRows) {
+        if (!coded && c.K > kFewRowsValues)
+            if (const hipError_t e = quantize(0); e != hipSuccess) return e;
         if (c.rows <= 16) return coded ? few_rows_float8<T, 1, true>(c, a, b, tail, stream) : few_rows_float8<T, 1, false>(c, a, b, tail, stream);
         return coded ? few_rows_float8<T, 2, true>(c, a, b, tail, stream) : few_rows_float8<T, 2, false>(c, a, b, tail, stream);
     }
     if (narrow_float8<T>(c.rows, c.K, c.N, coded)) return coded ? run_narrow_float8<T, true>(c, a, b, tail, stream) : run_narrow_float8<T, false>(c, a, b, tail, stream);
-    const ProductPlan p = plan_float8<T>(c.rows, c.K, c.N);
-    if (!coded) {
-        QuantizeCall q = {c.x, c.ld_x, c.input_dtype, c.rows, c.K, static_cast<uint8_t*>(workspace) + round_up(p.partial_bytes), nullptr};
-        q.exponents = q.codes + c.rows * a.blocks * kBlock;
-        a.codes = q.codes;
-        a.exponents = q.exponents;
-        if (const hipError_t e = quantize_launch(q, stream); e != hipSuccess) return e;
-    }
+    if (!coded)
+        if (const hipError_t e = quantize(round_up(p.partial_bytes)); e != hipSuccess) return e;
     if (p.splits > 1) tail.partial = static_cast<float*>(workspace);
     // few workgroups for a compute unit: what hides a load's way is more stages, not more workgroups
     const int64_t groups = p.tiles_m * p.tiles_n * p.splits;
