@@ -656,8 +656,8 @@ void launch_float8(Coded a, const Coded& b, Tail<T> tail, const ProductPlan& p, 
     }
 }
 
-// The plan of 16-bit products, a stage of 128 bytes being a block here; parts of k are whole words of exponents. (Results in float32: no tiles of
-// 256 x 256, whose fragments do not fit the registers as bfloat16.)
+// The plan of 16-bit products by the same estimate, a stage of 128 bytes being a block here; parts of k are whole words of exponents. (Results in
+// float32: no tiles of 256 x 256, whose fragments do not fit the registers as bfloat16.)
 template <class T>
 ProductPlan plan_float8(int64_t rows, int64_t K, int64_t N) {
     constexpr ProductShape kSmall[] = {kWide[1], kWide[2]};
@@ -692,7 +692,9 @@ hipError_t few_rows_float8(const LinearFloat8Call& c, const Coded& a, const Code
     return hipGetLastError();
 }
 
-// Sizes of narrow_float8_kernel.
+// Sizes of narrow_float8_kernel: a weight that fits its LDS, rows that fit a lane's registers (values take twice those of codes, a part of a block
+// more yet), and enough of them to go round every wave: 131072 x 128 -> 32 bfloat16 11.4 us and 24.2 quantized first and through tiles; of 8192 to 32768 rows
+// tiles were no worse.
 template <class T>
 bool narrow_float8(int64_t rows, int64_t K, int64_t N, bool coded) {
     return rows >= 65536 && blocks_of(K) <= (coded ? kNarrowBlocks : K % kBlock == 0 ? 2 : 1) && K >= Vec<T>::kLen &&
@@ -764,7 +766,8 @@ hipError_t linear_float8_forward(const LinearFloat8Call& c, void* workspace, hip
     if (!coded)
         if (const hipError_t e = quantize(round_up(p.partial_bytes)); e != hipSuccess) return e;
     if (p.splits > 1) tail.partial = static_cast<float*>(workspace);
-    // few workgroups for a compute unit: what hides a load's way is more stages, not more workgroups
+    // few workgroups for a compute unit: what hides a load's way is more stages, not more workgroups (bfloat16, two stages and four: 7223 x 3704 -> 80
+    // 21 and 17 us, 1024 x 4096 -> 1024 20.7 and 19.1; with more workgroups the LDS of four stages keeps the next one out)
     const int64_t groups = p.tiles_m * p.tiles_n * p.splits;
     const bool few = groups <= (p.shape == 1 ? 256 : 512);
     switch (p.shape) {

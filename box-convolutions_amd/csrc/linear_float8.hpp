@@ -73,6 +73,10 @@ __device__ __forceinline__ void word_to_lds(Descriptor d, unsigned offset, unsig
 // codes of every row. A block is two steps of 64 values of k. The barrier stands between them: the second step's fragments are in registers by then, so the
 // stage takes a block RING further on, whose loads go out one at a time between the second step's products. Exponents come four blocks at a time, a
 // word of every row, into a ring of their own; a lane keeps the words of its rows and shifts them by a byte from block to block.
+// Bound by the matrix instructions while tiles go round: 8192 x 8192 -> 8192 bfloat16 2.5 PFLOP/s, where a library's product with one scale a tensor
+// reaches 2.6. With one tile a compute unit its first loads and its epilogue are not hidden: 8192 x 4096 -> 2048 62 us (2.2 PFLOP/s), with silu, bias and a
+// residual 70 to 76, a library's without them 50; 8192 x 2048 -> 4096 69, with gelu 87, a library's 65. Float32 results: at most half of that.
+// No better: parts of k that start at another block in every tile, four waves for a tile of 256 x 256.
 template <class T, int TM, int TN, int WM, int WN, int RING>
 __global__ void __launch_bounds__(WM * WN * 64)
 product_float8_kernel(Coded a, Coded b, Tail<T> tail, int part_blocks, unsigned tiles_m, unsigned tiles_n) {
@@ -203,6 +207,7 @@ product_float8_kernel(Coded a, Coded b, Tail<T> tail, int part_blocks, unsigned 
 // brings `ahead` blocks of its 16 rows of the weight to LDS at a time (fragments read straight from memory would touch four times as many cache
 // lines per load), and reads its fragments there. CODED: x is codes, which come the same way; else values, quantized on the way in registers: the
 // four lanes that hold a row's share of a block agree on its exponent. That saves a launch, and the few rows come from the caches.
+// Bound by the launch and one way to memory and back: one row of 1024 -> 4096 bfloat16 5.2 us (with two launches the call took 11.4 us, 8.4 this way).
 template <class T>
 __device__ __forceinline__ void quantize_share(const T* p, int64_t left, Codes32& codes, int& exponent) {
     float v[32];
@@ -292,6 +297,7 @@ few_rows_float8_kernel(Coded a, const T* x, int64_t ld_x, int64_t columns, Coded
 // y of many rows through a weight of at most KB blocks a row that LDS holds whole. A wave takes 32 rows at a time with all their columns: its
 // lanes read the row's values (or, CODED, its codes) once, two lanes a row, and quantize them in registers; the codes never go through memory.
 // Then 32 columns at a time: products, epilogue. Workgroups of eight waves go round over the rows. WHOLE: rows of values end with a block.
+// Bound by memory: 131072 x 128 -> 32 bfloat16 with relu 11.4 us, 3.7 TB/s of values in and results out (quantized first and through tiles 24.2).
 constexpr int kNarrowBlocks = 4, kNarrowWaves = 8;         // (a row's exponents are one word)
 constexpr size_t kNarrowWeight = 64 * 1024;
 constexpr size_t narrow_float8_lds(int64_t columns, int blocks) { return static_cast<size_t>((columns + 31) / 32 * 32) * (blocks * kBlock + 4) + kNarrowWaves * 4096; }

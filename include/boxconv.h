@@ -61,7 +61,8 @@ void boxconv_reload_env(void);
  * "norm_apply", "norm_small", "norm_any_statistics", "norm_any_apply", "norm_sums", "norm_join_sums",
  * "norm_grad", "norm_small_grad", "norm_any_sums", "norm_any_grad", "norm_parameter", "linear",
  * "linear_few_rows", "linear_dx", "linear_dweight", "linear_narrow_grad", "linear_slope", "join_parts",
- * "join_bias".
+ * "join_bias", "norm_rows", "norm_rows_grad", "join_rows", "quantize", "linear_float8",
+ * "linear_float8_few_rows", "linear_float8_narrow".
  * NULL or "" disarms. Arming discards earlier measurements.
  * boxconv_profile_arm_every(name, n): the same, but only every n-th launch of that kernel (the
  * first, the (n+1)-th, ...) is bracketed; an event pair costs a few microseconds of GPU time, which
