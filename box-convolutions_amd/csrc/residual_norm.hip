@@ -16,8 +16,9 @@
 // Bound by memory: forward 20, backward 40 operations for each of 4 and 6 elements moved. Where a copy of 1 GiB reaches 5.2 TB/s:
 //   forward   4 x 128 x 256 x 128 bfloat16, layer, gate per item   28 us 4.8 TB/s    8192 x 4096 bfloat16, rms   48 to 54 us 5.0 to 5.6 TB/s
 //   backward                                                        41 us 4.9 TB/s                                 86 to 95 us 4.2 to 4.7 TB/s
-//   2 x 301 x 767 x 52 float16, layer, gate per element             forward 68 to 72 us 3.3 to 3.5 TB/s, backward 100 to 105 us 3.7 to 3.8 TB/s
-// and its sums' join 4 to 5 us. One row of 4096 without gradients 4.4 us. Rows of an odd number of 16-bit elements stay at 2.8 TB/s.
+//   2 x 301 x 767 x 52 float16, layer, gate per element             forward 55 to 58 us 4.2 to 4.3 TB/s, backward 89 to 92 us 4.2 to 4.3 TB/s
+// and its sums' join 4 to 5 us. One row of 4096 without gradients 4.4 us. 16384 x 1000 bfloat16 26 and 42 us, x 1001 30 and 52.
+// Still far from it: the backward of more than 4096 channels, whose sums leave the registers (4096 x 8190 bfloat16 205 us, 2 TB/s).
 #include <type_traits>
 
 #include "float8_blocks.hpp"
@@ -256,16 +257,40 @@ struct Team {
     // whether element k of the lane's lies in the row (without RAGGED kPerLane of them lie there or none)
     __device__ __forceinline__ bool inside(int k) const { return column_at(RAGGED ? k : k / kPerLane * kPerLane) < channels; }
 
-    // Vectors of a row, as they lie in memory. RAGGED: the last one runs into the next row, whose elements settle() takes away; `clear` says that
-    // no row of the wave's ends within a vector of the tensor's end, where that would be out of bounds: there it is read element by element.
-    __device__ __forceinline__ void request(const T* tensor, int64_t row, bool clear, Chunk (&raw)[NV]) const {
+    // value of element k, 0 beyond the row
+    __device__ __forceinline__ float within(float value, int k) const {
+        if constexpr (!RAGGED) return inside(k) ? value : 0.0f;
+        else {
+            unsigned bits = keep[k / V][k % V * static_cast<int>(sizeof(T)) / 4];
+            if constexpr (sizeof(T) == 2) bits = static_cast<unsigned>(static_cast<int>(k % 2 ? bits : bits << 16) >> 16);
+            return __builtin_bit_cast(float, __builtin_bit_cast(unsigned, value) & bits);
+        }
+    }
+
+    // Vectors of a row, as they lie in memory. RAGGED: the last one runs into the next row, whose elements settle() takes away; at the tensor's end,
+    // where that would be out of bounds, it starts so much earlier, and mend() moves it. (Element by element such reads took a third of the
+    // kernel's instructions, and their conditions drove the others out of the scalar registers: 16384 x 1001 bfloat16 forward 43 us, backward 57.)
+    __device__ __forceinline__ int limit(int64_t row, int64_t elements) const {        // the last column that a vector of the row may start at
+        return static_cast<int>(min<int64_t>(elements - V - row * channels, INT32_MAX));
+    }
+    __device__ __forceinline__ void request(const T* tensor, int64_t row, int last, Chunk (&raw)[NV]) const {
         if (tensor == nullptr) return;
         const T* p = tensor + row * channels;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            const int c = column(v), n = channels - c;
-            if (!RAGGED || clear) raw[v] = n > 0 ? __builtin_bit_cast(Chunk, *reinterpret_cast<const typename Vec<T>::Type*>(p + c)) : Chunk{0, 0, 0, 0};
-            else raw[v] = short_chunk(p + c, n);
+            const int c = column(v);
+            if constexpr (RAGGED) raw[v] = __builtin_bit_cast(Chunk, *reinterpret_cast<const typename Vec<T>::Type*>(p + min(c < channels ? c : 0, last)));
+            else raw[v] = c < channels ? __builtin_bit_cast(Chunk, *reinterpret_cast<const typename Vec<T>::Type*>(p + c)) : Chunk{0, 0, 0, 0};
+        }
+    }
+    __device__ __forceinline__ void mend(int last, Chunk (&raw)[NV]) const {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            Chunk& w = raw[v];
+            const int c = column(v) < channels ? column(v) : 0, k = c - min(c, last);      // elements too early
+            if (k * static_cast<int>(sizeof(T)) & 8) w = Chunk{w[2], w[3], 0, 0};
+            if (k * static_cast<int>(sizeof(T)) & 4) w = Chunk{w[1], w[2], w[3], 0};
+            if (sizeof(T) == 2 && (k & 1)) w = Chunk{w[0] >> 16 | w[1] << 16, w[1] >> 16 | w[2] << 16, w[2] >> 16 | w[3] << 16, w[3] >> 16};
         }
     }
     __device__ __forceinline__ bool clear_of_end(int64_t last_row, int64_t rows) const { return (rows - 1 - last_row) * channels >= V; }
@@ -326,10 +351,11 @@ struct Team {
             }
         }
     }
-    // Values per column, of the parameters' type or float; `none` beyond the row and without a vector.
+    // Values per column, of the parameters' type or float; `none` without a vector. RAGGED: 0 beyond the row (so that products with weight and gate
+    // are 0 there, whatever was normalised).
     __device__ __forceinline__ void params(const void* p, bool is_float, float none, float (&out)[E]) const {
 #pragma unroll
-        for (int i = 0; i < E; ++i) out[i] = none;
+        for (int i = 0; i < E; ++i) out[i] = !RAGGED ? none : p == nullptr ? within(none, i) : 0.0f;
         if (p == nullptr) return;
         if (is_float) run(static_cast<const float*>(p), out);
         else run(static_cast<const T*>(p), out);
@@ -399,7 +425,7 @@ struct Team {
             m.mean = sum * part;
 #pragma unroll
             for (int i = 0; i < E; ++i) {
-                const float d = RAGGED ? inside(i) ? value[i] - m.mean : 0.0f : value[i] - (inside(i) ? m.mean : 0.0f);
+                const float d = RAGGED ? within(value[i] - m.mean, i) : value[i] - (inside(i) ? m.mean : 0.0f);
                 square += d * d;
             }
             square = sum_of_lanes(square, WIDE ? 64 : LANES);
@@ -420,12 +446,12 @@ struct Team {
         m.rstd = rsqrtf(square * inverse + eps);
         return m;
     }
-    // (value - mean) * rstd, 0 beyond the row (whose values are 0).
+    // (value - mean) * rstd; 0 beyond the row (whose values are 0), but for RAGGED.
     __device__ __forceinline__ void normalise(float (&value)[E], const Moments& m) const {
 #pragma unroll
         for (int i = 0; i < E; ++i) {
             const bool in = inside(i);
-            value[i] = RAGGED ? in ? (value[i] - m.mean) * m.rstd : 0.0f : (value[i] - (in ? m.mean : 0.0f)) * (in ? m.rstd : 0.0f);
+            value[i] = RAGGED ? (value[i] - m.mean) * m.rstd : (value[i] - (in ? m.mean : 0.0f)) * (in ? m.rstd : 0.0f);
         }
     }
     // Elements of the row in wave w.
@@ -467,8 +493,9 @@ __device__ __forceinline__ void item_gate(const Team<T, LANES, E, RAGGED>& team,
 }
 
 // CODES: the normed rows leave in 8 bits. A block of 128 lies in 128 / kPerLane neighbouring lanes.
+// (Four waves a SIMD, as forward_plan counts on: rows of odd length would take 133 registers otherwise, and leave three.)
 template <class T, int LANES, int E, bool RAGGED, bool CODES>
-__global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads) norm_rows_kernel(Rows<T> a) {
+__global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads, E > kPerLane ? 2 : 4) norm_rows_kernel(Rows<T> a) {
     typedef Team<T, LANES, E, RAGGED> Row;
     constexpr int NV = Row::NV;
     __shared__ float exchange[2][16][2];
@@ -477,17 +504,25 @@ __global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads) no
     float wa[E], ba[E], wb[E], bb[E], g[E];
     const T* const full = a.gate_kind == kGateFull ? static_cast<const T*>(a.gate) : nullptr;
 #pragma unroll
-    for (int i = 0; i < E; ++i) g[i] = 1.0f;
+    for (int i = 0; i < E; ++i) g[i] = RAGGED ? team.within(1.0f, i) : 1.0f;
+    const int64_t rows = a.plan.batch * a.pixels, elements = rows * a.channels;
     bool loaded = false;
     for (int64_t i = 0; i < a.plan.items; ++i) {
         const Span span = span_of(a.plan, a.pixels, i);
         Chunk xs[NV] = {}, rs[NV] = {}, gs[NV] = {};
         const auto request = [&](int64_t base) {
             const int64_t row = min(base + place.own, span.last - 1);
-            const bool clear = team.clear_of_end(min(base + place.teams, span.last) - 1, a.plan.batch * a.pixels);
-            team.request(a.x, row, clear, xs);
-            team.request(a.residual, row, clear, rs);
-            team.request(full, row, clear, gs);
+            const int last = RAGGED ? team.limit(row, elements) : 0;
+            team.request(a.x, row, last, xs);
+            team.request(a.residual, row, last, rs);
+            team.request(full, row, last, gs);
+        };
+        const auto mend = [&](int64_t base) {
+            if (!RAGGED || team.clear_of_end(min(base + place.teams, span.last) - 1, rows)) return;
+            const int last = team.limit(min(base + place.own, span.last - 1), elements);
+            team.mend(last, xs);
+            team.mend(last, rs);
+            team.mend(last, gs);
         };
         int64_t base = span.first + place.first;
         if (base < span.last) request(base);
@@ -503,6 +538,7 @@ __global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads) no
             const int64_t row = base + place.own;
             const bool live = row < span.last;
             float x[E], r[E];
+            mend(base);
             team.settle(xs, x);
             team.settle(rs, r);
             if (full != nullptr) team.settle(gs, g);
@@ -536,7 +572,7 @@ __global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads) no
                 for (int k = 0; k < E; k += kPerLane) {
                     float part[kPerLane];
 #pragma unroll
-                    for (int j = 0; j < kPerLane; ++j) part[j] = x[k + j];
+                    for (int j = 0; j < kPerLane; ++j) part[j] = RAGGED ? team.within(x[k + j], k + j) : x[k + j];
                     const int e = block_exponent(most_of_lanes(largest(part), kBlock / kPerLane)), c = team.column_at(k), b = c / kBlock;
                     const Codes<kPerLane> codes = to_codes(part, e);
                     if (live && b < blocks) {
@@ -571,7 +607,7 @@ __global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads, 2)
     const T* const full = a.gate_kind == kGateFull ? static_cast<const T*>(a.gate) : nullptr;
     float wa[E], ba[E] = {}, wb[E], g[E];
 #pragma unroll
-    for (int i = 0; i < E; ++i) g[i] = 1.0f;
+    for (int i = 0; i < E; ++i) g[i] = RAGGED ? team.within(1.0f, i) : 1.0f;
     const auto after_parameters = [&] {
         team.params(a.after_weight, a.float_params, 1.0f, wa);
         if constexpr (BIAS) team.params(a.after_bias, a.float_params, 0.0f, ba);
@@ -582,6 +618,7 @@ __global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads, 2)
         before_parameters();
     }
     const bool has_dh = a.before && a.dnormed != nullptr;
+    const int64_t rows = a.plan.batch * a.pixels, elements = rows * a.channels;
     // sum k of the workgroup's teams to memory
     const auto put = [&](const float (&v)[E], void* to, int64_t at, bool is_float) {
         const auto write = [&](int c, float s) {
@@ -614,15 +651,24 @@ __global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads, 2)
         struct Raw { Chunk x[NV], r[NV], g[NV], d[NV], h[NV]; Four kept; } ahead[BIG ? 1 : 2] = {};
         const auto request = [&](int64_t base, Raw& raw) {
             const int64_t row = min(base + place.own, span.last - 1);
-            const bool clear = team.clear_of_end(min(base + place.teams, span.last) - 1, a.plan.batch * a.pixels);
-            team.request(a.x, row, clear, raw.x);
-            if (a.before) team.request(a.residual, row, clear, raw.r);
-            team.request(full, row, clear, raw.g);
-            team.request(a.dstream, row, clear, raw.d);
-            if (a.before) team.request(a.dnormed, row, clear, raw.h);
+            const int last = RAGGED ? team.limit(row, elements) : 0;
+            team.request(a.x, row, last, raw.x);
+            if (a.before) team.request(a.residual, row, last, raw.r);
+            team.request(full, row, last, raw.g);
+            team.request(a.dstream, row, last, raw.d);
+            if (a.before) team.request(a.dnormed, row, last, raw.h);
             if constexpr (WIDE) {
                 if (a.statistics != nullptr) raw.kept = *reinterpret_cast<const Four*>(a.statistics + 4 * row);
             }
+        };
+        const auto mend = [&](int64_t base, Raw& raw) {
+            if (!RAGGED || team.clear_of_end(min(base + place.teams, span.last) - 1, rows)) return;
+            const int last = team.limit(min(base + place.own, span.last - 1), elements);
+            team.mend(last, raw.x);
+            team.mend(last, raw.r);
+            team.mend(last, raw.g);
+            team.mend(last, raw.d);
+            team.mend(last, raw.h);
         };
         const auto work = [&](int64_t base, Raw& raw) {
             const int64_t row = base + place.own;
@@ -633,6 +679,7 @@ __global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads, 2)
                 item_gate(team, a, span.item, g);
             }
             float p[E], q[E], d[E], h[E];                              // normalised x, normalised s, gradients of s and h; later what they become
+            mend(base, raw);
             team.settle(raw.x, p);
             team.settle(raw.r, q);
             team.settle(raw.d, d);
@@ -677,7 +724,7 @@ __global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads, 2)
 #pragma unroll
                 for (int k = 0; k < E; ++k) {
                     const float through = h[k] - e1 - q[k] * e2;
-                    d[k] += RAGGED ? team.inside(k) ? ms.rstd * through : 0.0f : (team.inside(k) ? ms.rstd : 0.0f) * through;
+                    d[k] += RAGGED ? ms.rstd * through : (team.inside(k) ? ms.rstd : 0.0f) * through;
                 }
             }
             if (a.dresidual != nullptr && live) team.store(a.dresidual, row, d);
@@ -796,11 +843,12 @@ Rows<T> rows_of(const ResidualNormCall& c) {
 }
 
 // How the rows of a call are dealt out: lanes of a team, its workgroup's threads, and rows that a workgroup takes at once. big: twice
-// kPerLane elements a lane. No lanes: rows of more channels than the registers of a workgroup hold.
+// kPerLane elements a lane. No lanes: rows of more channels than the registers of a workgroup hold, and tensors smaller than a vector.
 struct Shape { bool wide; int lanes, threads, rows; bool big; };
 template <class T>
-Shape shape_of(int channels, bool codes) {
-    if (channels > kMostRegisterChannels) return {true, 0, kAnyThreads, 1, false};
+Shape shape_of(const ResidualNormCall& c, bool codes) {
+    const int channels = c.channels;
+    if (channels > kMostRegisterChannels || c.batch * c.pixels * channels < kPerLane) return {true, 0, kAnyThreads, 1, false};
     const int columns = codes ? blocks_of(channels) * kBlock : channels;           // (codes are written to the end of the last block)
     int lanes = codes ? kBlock / kPerLane : 1;        // (more lanes without a share add zeros: the sums are the same to the bit)
     while (lanes < 64 && lanes * kPerLane < columns) lanes *= 2;
@@ -843,7 +891,7 @@ hipError_t residual_norm_forward(const ResidualNormCall& c, const ResidualNormOu
     const bool coded = out.exponents != nullptr;
     if (coded) a.codes = static_cast<uint8_t*>(out.normed);
     else a.normed = static_cast<T*>(out.normed);
-    const Shape s = shape_of<T>(c.channels, coded);
+    const Shape s = shape_of<T>(c, coded);
     a.plan = forward_plan(c, s);
     const dim3 grid(static_cast<unsigned>(a.plan.groups)), block(s.threads);
     if (s.lanes == 0) BOXCONV_LAUNCH("norm_rows", (norm_rows_any_kernel<T>), grid, block, 0, stream, a);
@@ -859,7 +907,7 @@ hipError_t residual_norm_forward(const ResidualNormCall& c, const ResidualNormOu
 
 template <class T>
 size_t residual_norm_workspace(const ResidualNormCall& c) {
-    return static_cast<size_t>(backward_plan(c, shape_of<T>(c.channels, false)).groups) * kSums * c.channels * sizeof(float);
+    return static_cast<size_t>(backward_plan(c, shape_of<T>(c, false)).groups) * kSums * c.channels * sizeof(float);
 }
 
 template <class T>
@@ -870,7 +918,7 @@ hipError_t residual_norm_backward(const ResidualNormCall& c, const ResidualNormG
     a.dnormed = static_cast<const T*>(g.dnormed);
     a.dx = static_cast<T*>(g.dx);
     a.dresidual = static_cast<T*>(g.dresidual);
-    const Shape s = shape_of<T>(c.channels, false);
+    const Shape s = shape_of<T>(c, false);
     a.plan = backward_plan(c, s);
     RowGrads to = {{g.dafter_weight, g.dafter_bias, g.dbefore_weight, g.dbefore_bias, c.gate_kind == kGateFull ? nullptr : g.dgate}};
     if (c.gate_kind == kGateFull) a.dgate_full = static_cast<T*>(g.dgate);

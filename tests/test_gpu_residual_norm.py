@@ -99,6 +99,16 @@ def test_sizes(hip, i, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("C", [*range(1, 18), 519, 1023, 4099, 4101])
+def test_last_rows_of_the_tensor(hip, C, dtype):
+    """A row's last vector may not read beyond the tensor: every number of elements by which one would, in the last rows and in a tensor of less
+    than a vector. A gate per element is read the same way."""
+    for size in ((1, C, (1,)), (2, C, (2,)), (3, C, (1, 5))):
+        c = case(*size, dtype, ("rms", "layer")[C % 2], "full" if C % 3 else "item", params=("same", "none")[C % 5 == 0])
+        check(run(c), expected(c))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("after,before", [(True, True), (True, False), (False, True), (False, False)])
 @pytest.mark.parametrize("gate", GATES)
 def test_pieces(hip, after, before, gate, dtype):
