@@ -15,10 +15,10 @@
 //
 // Bound by memory: forward 20, backward 40 operations for each of 4 and 6 elements moved. Where a copy of 1 GiB reaches 5.2 TB/s:
 //   forward   4 x 128 x 256 x 128 bfloat16, layer, gate per item   28 us 4.8 TB/s    8192 x 4096 bfloat16, rms   48 to 54 us 5.0 to 5.6 TB/s
-//   backward                                                        41 us 4.9 TB/s                                 86 to 95 us 4.2 to 4.7 TB/s
+//   backward                                                        41 us 4.9 TB/s                                 83 to 88 us 4.6 to 4.9 TB/s
 //   2 x 301 x 767 x 52 float16, layer, gate per element             forward 55 to 58 us 4.2 to 4.3 TB/s, backward 89 to 92 us 4.2 to 4.3 TB/s
-// and its sums' join 4 to 5 us. One row of 4096 without gradients 4.4 us. 16384 x 1000 bfloat16 26 and 42 us, x 1001 30 and 52.
-// Still far from it: the backward of more than 4096 channels, whose sums leave the registers (4096 x 8190 bfloat16 205 us, 2 TB/s).
+// and its sums' join 4 to 5 us. One row of 4096 without gradients 4.4 us. 16384 x 1000 bfloat16 26 and 40 us, x 1001 31 and 52.
+// Still far from it: the backward of more than 4096 channels, whose sums leave the registers (4096 x 8190 bfloat16 145 us, 2.8 TB/s).
 #include <type_traits>
 
 #include "float8_blocks.hpp"
@@ -378,12 +378,13 @@ struct Team {
         }
     }
     // Over the row: the sums of a and b, the same in all its lanes.
-    __device__ __forceinline__ void pair_sum(float& a, float& b) {
+    template <bool BOTH = true>
+    __device__ __forceinline__ void pair_sum(float& a, float& b) {         // (without BOTH only b's)
         if constexpr (!WIDE) {
-            a = sum_of_lanes(a, LANES);
+            if constexpr (BOTH) a = sum_of_lanes(a, LANES);
             b = sum_of_lanes(b, LANES);
         } else {
-            a = sum_of_lanes(a, 64);
+            if constexpr (BOTH) a = sum_of_lanes(a, 64);
             b = sum_of_lanes(b, 64);
             swap(a, b);
             a = b = 0.0f;
@@ -484,12 +485,20 @@ struct Place {
     }
 };
 
+// g: the gate times the scale, the scale alone without one; of a gate per element whenever it is settled.
+template <class T, int E>
+__device__ __forceinline__ void scaled(const Rows<T>& a, float (&g)[E]) {
+#pragma unroll
+    for (int i = 0; i < E; ++i) g[i] *= a.scale;
+}
 template <class T, int LANES, int E, bool RAGGED>
 __device__ __forceinline__ void item_gate(const Team<T, LANES, E, RAGGED>& team, const Rows<T>& a, int64_t item, float (&g)[E]) {
+    if (a.gate_kind == kGateFull) return;
     const int64_t at = a.gate_kind == kGateItem ? item * a.channels : 0;
-    if (a.gate_kind == kGateChannel || a.gate_kind == kGateItem)
-        team.params(a.float_gate ? static_cast<const void*>(static_cast<const float*>(a.gate) + at) : static_cast<const void*>(static_cast<const T*>(a.gate) + at),
-                    a.float_gate, 1.0f, g);
+    const void* const gate = a.gate_kind != kGateChannel && a.gate_kind != kGateItem ? nullptr :
+                             a.float_gate ? static_cast<const void*>(static_cast<const float*>(a.gate) + at) : static_cast<const void*>(static_cast<const T*>(a.gate) + at);
+    team.params(gate, a.float_gate, 1.0f, g);
+    scaled(a, g);
 }
 
 // CODES: the normed rows leave in 8 bits. A block of 128 lies in 128 / kPerLane neighbouring lanes.
@@ -503,8 +512,6 @@ __global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads, E 
     Row& team = place.team;
     float wa[E], ba[E], wb[E], bb[E], g[E];
     const T* const full = a.gate_kind == kGateFull ? static_cast<const T*>(a.gate) : nullptr;
-#pragma unroll
-    for (int i = 0; i < E; ++i) g[i] = RAGGED ? team.within(1.0f, i) : 1.0f;
     const int64_t rows = a.plan.batch * a.pixels, elements = rows * a.channels;
     bool loaded = false;
     for (int64_t i = 0; i < a.plan.items; ++i) {
@@ -541,7 +548,10 @@ __global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads, E 
             mend(base);
             team.settle(xs, x);
             team.settle(rs, r);
-            if (full != nullptr) team.settle(gs, g);
+            if (full != nullptr) {
+                team.settle(gs, g);
+                scaled(a, g);
+            }
             if (base + place.step < span.last) request(base + place.step);
             Four kept = {0.0f, 1.0f, 0.0f, 1.0f};
             if (a.after) {
@@ -553,7 +563,7 @@ __global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads, E 
             }
             // (0 beyond the row, where x, the residual and the bias are)
 #pragma unroll
-            for (int k = 0; k < E; ++k) x[k] = r[k] + x[k] * g[k] * a.scale;
+            for (int k = 0; k < E; ++k) x[k] = r[k] + x[k] * g[k];
             if (a.stream != nullptr && live) team.store(a.stream, row, x);
             Moments m = {0.0f, 1.0f};
             if (a.before) m = team.moments(x, a.centre, a.eps);
@@ -590,11 +600,12 @@ __global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads, E 
     }
 }
 
-// BIAS: whether either norm has one (sums and values that root-mean-square norms seldom need).
+// LAYER: whether the norms centre or have biases: sums, means and values that root-mean-square norms do without (8192 x 4096 bfloat16
+// 95 us with them, 88 without; 4096 x 4096 46 and 42, 4096 x 8190 205 and 145).
 // Two rows ahead are on their way while one is worked on (4 x 128 x 256 x 128 bfloat16 56 us with one, 48 with two; 16384 x 1024 92 and 62). With twice the
 // elements a lane (BIG) there are no registers for that, nor for the parameters, which come from the caches again for every row. Workgroups that
 // hold a row (WIDE) take its means from the forward: each would cost two barriers a row (8192 x 4096 bfloat16 128 us, 95 this way).
-template <class T, int LANES, int E, bool RAGGED, bool BIAS>
+template <class T, int LANES, int E, bool RAGGED, bool LAYER>
 __global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads, 2) norm_rows_grad_kernel(Rows<T> a) {
     typedef Team<T, LANES, E, RAGGED> Row;
     constexpr bool WIDE = LANES == 0, BIG = E > kPerLane;
@@ -606,11 +617,10 @@ __global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads, 2)
     float sum[kSums][E] = {};
     const T* const full = a.gate_kind == kGateFull ? static_cast<const T*>(a.gate) : nullptr;
     float wa[E], ba[E] = {}, wb[E], g[E];
-#pragma unroll
-    for (int i = 0; i < E; ++i) g[i] = RAGGED ? team.within(1.0f, i) : 1.0f;
+    const bool centre = LAYER && a.centre;
     const auto after_parameters = [&] {
         team.params(a.after_weight, a.float_params, 1.0f, wa);
-        if constexpr (BIAS) team.params(a.after_bias, a.float_params, 0.0f, ba);
+        if constexpr (LAYER) team.params(a.after_bias, a.float_params, 0.0f, ba);
     };
     const auto before_parameters = [&] { team.params(a.before_weight, a.float_params, 1.0f, wb); };
     if constexpr (!BIG) {
@@ -684,7 +694,10 @@ __global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads, 2)
             team.settle(raw.r, q);
             team.settle(raw.d, d);
             team.settle(raw.h, h);
-            if (full != nullptr) team.settle(raw.g, g);
+            if (full != nullptr) {
+                team.settle(raw.g, g);
+                scaled(a, g);
+            }
             const Four kept = raw.kept;
             const bool again = !WIDE || a.statistics == nullptr;
             if constexpr (!BIG) {
@@ -692,22 +705,22 @@ __global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads, 2)
             }
             Moments mx = {0.0f, 1.0f};
             if (a.after) {
-                mx = again ? team.moments(p, a.centre, a.eps) : Moments{kept[0], kept[1]};
+                mx = again ? team.moments(p, centre, a.eps) : Moments{centre ? kept[0] : 0.0f, kept[1]};
                 team.normalise(p, mx);
             }
             if (has_dh) {
 #pragma unroll
                 for (int k = 0; k < E; ++k) {
-                    const float u = a.after ? BIAS ? p[k] * wa[k] + ba[k] : p[k] * wa[k] : p[k];
-                    q[k] += u * g[k] * a.scale;
+                    const float u = a.after ? LAYER ? p[k] * wa[k] + ba[k] : p[k] * wa[k] : p[k];
+                    q[k] += u * g[k];
                 }
-                const Moments ms = again ? team.moments(q, a.centre, a.eps) : Moments{kept[2], kept[3]};
+                const Moments ms = again ? team.moments(q, centre, a.eps) : Moments{centre ? kept[2] : 0.0f, kept[3]};
                 team.normalise(q, ms);
                 if (live) {
 #pragma unroll
                     for (int k = 0; k < E; ++k) {
                         sum[2][k] += h[k] * q[k];
-                        if constexpr (BIAS) sum[3][k] += h[k];
+                        if constexpr (LAYER) sum[3][k] += h[k];
                     }
                 }
                 if constexpr (BIG) before_parameters();
@@ -715,11 +728,11 @@ __global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads, 2)
 #pragma unroll
                 for (int k = 0; k < E; ++k) {
                     h[k] *= wb[k];                                      // (0 beyond the row)
-                    e1 += h[k];
+                    if constexpr (LAYER) e1 += h[k];
                     e2 += h[k] * q[k];
                 }
-                team.pair_sum(e1, e2);
-                e1 = a.centre ? e1 * team.inverse : 0.0f;
+                team.template pair_sum<LAYER>(e1, e2);
+                e1 = centre ? e1 * team.inverse : 0.0f;
                 e2 *= team.inverse;
 #pragma unroll
                 for (int k = 0; k < E; ++k) {
@@ -733,20 +746,24 @@ __global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads, 2)
                 after_parameters();
                 item_gate(team, a, span.item, g);
             }
-            // d: gradient of s, then of u; h: of the gate
+            // d: gradient of s, then of u; h: of the gate, over the scale
 #pragma unroll
             for (int k = 0; k < E; ++k) {
-                d[k] *= a.scale;
-                h[k] = (a.after ? BIAS ? p[k] * wa[k] + ba[k] : p[k] * wa[k] : p[k]) * d[k];
+                h[k] = (a.after ? LAYER ? p[k] * wa[k] + ba[k] : p[k] * wa[k] : p[k]) * d[k];
                 d[k] *= g[k];
             }
-            if (a.dgate_full != nullptr && live) team.store(a.dgate_full, row, h);
+            if (a.dgate_full != nullptr && live) {
+                float out[E];
+#pragma unroll
+                for (int k = 0; k < E; ++k) out[k] = h[k] * a.scale;
+                team.store(a.dgate_full, row, out);
+            }
             if (live) {
 #pragma unroll
                 for (int k = 0; k < E; ++k) {
                     sum[kSumGate][k] += h[k];
                     sum[0][k] += d[k] * p[k];
-                    if constexpr (BIAS) sum[1][k] += d[k];
+                    if constexpr (LAYER) sum[1][k] += d[k];
                 }
             }
             if (a.after) {
@@ -754,11 +771,11 @@ __global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads, 2)
 #pragma unroll
                 for (int k = 0; k < E; ++k) {
                     d[k] *= wa[k];
-                    f1 += d[k];
+                    if constexpr (LAYER) f1 += d[k];
                     f2 += d[k] * p[k];
                 }
-                team.pair_sum(f1, f2);
-                f1 = a.centre ? f1 * team.inverse : 0.0f;
+                team.template pair_sum<LAYER>(f1, f2);
+                f1 = centre ? f1 * team.inverse : 0.0f;
                 f2 *= team.inverse;
 #pragma unroll
                 for (int k = 0; k < E; ++k) d[k] = mx.rstd * (d[k] - f1 - p[k] * f2);
@@ -778,15 +795,17 @@ __global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads, 2)
             }
         }
         if (a.gate_kind == kGateItem && (a.dgate != nullptr || a.sums != nullptr) && span.last > span.first) {
+            scaled(a, sum[kSumGate]);
             if (a.dgate != nullptr) put(sum[kSumGate], a.dgate, span.item * a.channels, a.float_gate);
             else put(sum[kSumGate], a.sums, (static_cast<int64_t>(blockIdx.x) * kSums + kSumGate) * a.channels, true);
 #pragma unroll
             for (int k = 0; k < E; ++k) sum[kSumGate][k] = 0.0f;
         }
     }
+    if (a.wanted >> kSumGate & 1) scaled(a, sum[kSumGate]);
 #pragma unroll
     for (int k = 0; k < kSums; ++k)
-        if ((BIAS || k % 2 == 0) && (a.wanted >> k & 1)) put(sum[k], a.sums, (static_cast<int64_t>(blockIdx.x) * kSums + k) * a.channels, true);
+        if ((LAYER || k % 2 == 0) && (a.wanted >> k & 1)) put(sum[k], a.sums, (static_cast<int64_t>(blockIdx.x) * kSums + k) * a.channels, true);
 }
 
 // ---- sums over workgroups -----------------------------------------------------------------------------------------
@@ -936,9 +955,9 @@ hipError_t residual_norm_backward(const ResidualNormCall& c, const ResidualNormG
     else
         known(c.channels % kPerLane != 0, [&](auto ragged) {
             constexpr bool R = decltype(ragged)::value;
-            known(c.after_bias != nullptr || c.before_bias != nullptr, [&](auto bias) {
+            known(c.centre || c.after_bias != nullptr || c.before_bias != nullptr, [&](auto layer) {
                 known_lanes<1>(s, [&](auto lanes, auto each) {
-                    BOXCONV_LAUNCH("norm_rows_grad", (norm_rows_grad_kernel<T, decltype(lanes)::value, decltype(each)::value, R, decltype(bias)::value>), grid, block, 0,
+                    BOXCONV_LAUNCH("norm_rows_grad", (norm_rows_grad_kernel<T, decltype(lanes)::value, decltype(each)::value, R, decltype(layer)::value>), grid, block, 0,
                                    stream, a);
                 });
             });
