@@ -502,7 +502,8 @@ __device__ __forceinline__ void item_gate(const Team<T, LANES, E, RAGGED>& team,
 }
 
 // CODES: the normed rows leave in 8 bits. A block of 128 lies in 128 / kPerLane neighbouring lanes.
-// (Four waves a SIMD, as forward_plan counts on: rows of odd length would take 133 registers otherwise, and leave three.)
+// Four waves a SIMD, as forward_plan counts on: rows of odd length would take 133 registers otherwise, and leave three (4096 x 4095 bfloat16 43 us, 32 with
+// four, a few values in scratch among the cost; 16384 x 1001 36 and 30; float32 the same within 5 %).
 template <class T, int LANES, int E, bool RAGGED, bool CODES>
 __global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads, E > kPerLane ? 2 : 4) norm_rows_kernel(Rows<T> a) {
     typedef Team<T, LANES, E, RAGGED> Row;
