@@ -108,6 +108,25 @@ def test_last_rows_of_the_tensor(hip, C, dtype):
         check(run(c), expected(c))
 
 
+@pytest.mark.parametrize("C", [1, 2, 3, 5, 7, 9, 13, 130, 1021, 4103])
+def test_last_rows_in_8_bits(hip, C):
+    """The same reads where the normed rows leave in 8 bits: float32 rows are stored as they are quantized, so the codes are theirs; zeros behind a row, with a
+    row of NaN among them too."""
+    from box_convolution import quantize_blocks, residual_norm
+    for rows in (1, 2, 5):
+        torch.manual_seed(C * 8 + rows)
+        x, r = (torch.randn(1, rows, C, device="cuda").movedim(-1, 1) for _ in range(2))
+        w = torch.rand(C, device="cuda") + 0.5
+        for k in range(2):
+            stream, blocks = residual_norm(x, r, w, 0.5, (w, None), (w, w), "layer", quantize=True)
+            same, normed = residual_norm(x, r, w, 0.5, (w, None), (w, w), "layer")
+            want = quantize_blocks(normed.movedim(1, -1))
+            assert torch.equal(stream.nan_to_num(7.0), same.nan_to_num(7.0))
+            assert torch.equal(blocks.codes.view(torch.uint8), want.codes.view(torch.uint8)) and torch.equal(blocks.exponents, want.exponents)
+            assert not blocks.codes[..., C:].float().any()
+            x[0, 0, rows - 1] = float("nan")
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("after,before", [(True, True), (True, False), (False, True), (False, False)])
 @pytest.mark.parametrize("gate", GATES)
