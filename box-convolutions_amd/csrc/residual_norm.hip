@@ -895,10 +895,12 @@ void known_lanes(const Shape& s, F f) {
     f(std::integral_constant<int, LEAST>(), Each());
 }
 
-// As many workgroups as the chip holds at once: the forward's kernels leave room for four waves a SIMD, the backward's for two. (Fewer where the
-// backward's sums are long and in memory.)
-RowPlan forward_plan(const ResidualNormCall& c, const Shape& s) { return plan_rows(c, 256 * 16 * 64 / s.threads, s.rows); }
-RowPlan backward_plan(const ResidualNormCall& c, const Shape& s) { return plan_rows(c, s.lanes == 0 ? 128 : 256 * 8 * 64 / s.threads, s.rows); }
+// As many workgroups as the chip holds at once: the forward's kernels leave room for four waves a SIMD, the backward's for two, and a workgroup is on one
+// compute unit whole: counted in waves, workgroups of 3, 5, 6 or 7 came in two rounds (8192 x 3500 bfloat16 forward 71 us, backward 139; 53 and 82 this way;
+// 4096 x 6400 backward 162 and 101; with 4 or 8 waves the count is the same). (Fewer where the backward's sums are long and in memory.)
+int64_t resident(const Shape& s, int waves) { return 256 * std::max(1, waves * 64 / s.threads); }
+RowPlan forward_plan(const ResidualNormCall& c, const Shape& s) { return plan_rows(c, resident(s, s.big ? 8 : 16), s.rows); }
+RowPlan backward_plan(const ResidualNormCall& c, const Shape& s) { return plan_rows(c, s.lanes == 0 ? 128 : resident(s, 8), s.rows); }
 
 }  // namespace
 
