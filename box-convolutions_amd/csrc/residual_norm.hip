@@ -50,15 +50,6 @@ struct Rows {
     int wanted;                        // bit k: sum k, over all the workgroup's rows
 };
 
-// The rows [first, last) of item i of the workgroup's, counted over the whole tensor; none from `items` on.
-struct Span { int64_t item, first, last; };
-__device__ __forceinline__ Span span_of(const RowPlan& p, int64_t pixels, int64_t i) {
-    const int64_t item = p.parts > 1 ? blockIdx.x / p.parts : blockIdx.x * p.items + i;
-    if (i >= p.items || item >= p.batch) return {item, 0, 0};
-    const int64_t part = p.parts > 1 ? blockIdx.x % p.parts : 0, begin = part * p.rows;
-    return {item, item * pixels + begin, item * pixels + min(pixels, begin + p.rows)};
-}
-
 // ---- any number of channels -------------------------------------------------------------------------------------
 // A workgroup takes a row at a time and reads it again for every mean; the rows it does so with come from the caches.
 constexpr int kAnyThreads = 1024;
@@ -143,8 +134,8 @@ struct AnyRow {
 template <class T>
 __global__ void __launch_bounds__(kAnyThreads) norm_rows_any_kernel(Rows<T> a) {
     __shared__ float lds[kAnyThreads / 64];
-    for (int64_t i = 0; i < a.plan.items; ++i) {
-        const Span span = span_of(a.plan, a.pixels, i);
+    for (int64_t i = 0; i < items_of(a.plan, blockIdx.x); ++i) {
+        const Span span = span_of(a.plan, a.pixels, blockIdx.x, i);
         for (int64_t row = span.first; row < span.last; ++row) {
             AnyRow<T> r = {a, row * a.channels, span.item};
             r.measure(lds, nullptr);
@@ -176,8 +167,8 @@ __global__ void __launch_bounds__(kAnyThreads) norm_rows_any_grad_kernel(Rows<T>
     float* const sums = a.sums == nullptr ? nullptr : a.sums + static_cast<int64_t>(blockIdx.x) * kSums * a.channels;
     // (each thread adds to sums of its own channels only; the first row's are stored)
     bool first = true;
-    for (int64_t i = 0; i < a.plan.items; ++i) {
-        const Span span = span_of(a.plan, a.pixels, i);
+    for (int64_t i = 0; i < items_of(a.plan, blockIdx.x); ++i) {
+        const Span span = span_of(a.plan, a.pixels, blockIdx.x, i);
         for (int64_t row = span.first; row < span.last; ++row) {
             AnyRow<T> r = {a, row * a.channels, span.item};
             r.measure(lds, a.statistics == nullptr ? nullptr : a.statistics + 4 * row);
@@ -515,8 +506,8 @@ __global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads, E 
     const T* const full = a.gate_kind == kGateFull ? static_cast<const T*>(a.gate) : nullptr;
     const int64_t rows = a.plan.batch * a.pixels, elements = rows * a.channels;
     bool loaded = false;
-    for (int64_t i = 0; i < a.plan.items; ++i) {
-        const Span span = span_of(a.plan, a.pixels, i);
+    for (int64_t i = 0; i < items_of(a.plan, blockIdx.x); ++i) {
+        const Span span = span_of(a.plan, a.pixels, blockIdx.x, i);
         Chunk xs[NV] = {}, rs[NV] = {}, gs[NV] = {};
         const auto request = [&](int64_t base) {
             const int64_t row = min(base + place.own, span.last - 1);
@@ -657,8 +648,8 @@ __global__ void __launch_bounds__(LANES == 0 ? kWideThreads : kNarrowThreads, 2)
             }
         }
     };
-    for (int64_t i = 0; i < a.plan.items; ++i) {
-        const Span span = span_of(a.plan, a.pixels, i);
+    for (int64_t i = 0; i < items_of(a.plan, blockIdx.x); ++i) {
+        const Span span = span_of(a.plan, a.pixels, blockIdx.x, i);
         struct Raw { Chunk x[NV], r[NV], g[NV], d[NV], h[NV]; Four kept; } ahead[BIG ? 1 : 2] = {};
         const auto request = [&](int64_t base, Raw& raw) {
             const int64_t row = min(base + place.own, span.last - 1);

@@ -3,8 +3,6 @@
 
 #include <algorithm>
 
-#include "activation.hpp"
-#include "boxconv_host.hpp"
 #include "operators_host.hpp"
 
 namespace boxconv {
@@ -38,6 +36,20 @@ RowPlan plan_rows(const ResidualNormCall& c, int64_t target, int64_t least) {
         p.groups = p.batch * p.parts;
     }
     return p;
+}
+
+// Items of a workgroup. (The last ones have fewer, where they do not divide: what is read by an item's number has to stop with them.)
+__host__ __device__ inline int64_t items_of(const RowPlan& p, int64_t group) {
+    const int64_t left = p.batch - group * p.items;
+    return p.parts > 1 ? 1 : left < p.items ? left : p.items;
+}
+
+// The rows [first, last) of item i of the workgroup's items_of, counted over the whole tensor.
+struct Span { int64_t item, first, last; };
+__host__ __device__ inline Span span_of(const RowPlan& p, int64_t pixels, int64_t group, int64_t i) {
+    const int64_t item = p.parts > 1 ? group / p.parts : group * p.items + i, begin = p.parts > 1 ? group % p.parts * p.rows : 0;
+    const int64_t end = begin + p.rows < pixels ? begin + p.rows : pixels;
+    return {item, item * pixels + begin, item * pixels + end};
 }
 
 }  // namespace

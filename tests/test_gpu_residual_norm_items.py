@@ -1,0 +1,29 @@
+"""``residual_norm`` with a gate per batch item, at numbers of items that the workgroups do not divide: the last workgroup has fewer than the others,
+and reads no gate behind the last item's (tests/test_row_plan_host.py walks the plan itself)."""
+import pytest
+import torch
+
+from operator_reference import check
+from test_gpu_residual_norm import TYPES, case, expected, run
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B,C,spatial", [(1025, 24, (1,)), (1300, 20, (3,)), (4099, 8, (1,)), (1025, 40, (1,)), (257, 700, (1,)), (1023, 513, (1,)), (2049, 700, (1,)), (257, 4096, (1,)),
+                                         (513, 4095, (1,)), (257, 6000, (1,)), (130, 8200, (1,)), (257, 8200, (1,))])
+def test_items_that_workgroups_do_not_divide(hip, B, C, spatial, dtype):
+    c = case(B, C, spatial, dtype, ("layer", "rms")[C % 2], "item", params=("same", "float")[B % 2], float_gate=C % 16 == 0)
+    check(run(c), expected(c))
+
+
+def test_blocks_of_items_that_workgroups_do_not_divide(hip):
+    from box_convolution import quantize_blocks, residual_norm
+    for B, C in ((1025, 24), (2049, 700), (513, 4096), (257, 6000)):
+        torch.manual_seed(B)
+        x, gate, w = torch.randn(B, C, 2, device="cuda"), torch.randn(B, C, device="cuda"), torch.rand(C, device="cuda") + 0.5
+        stream, blocks = residual_norm(x, None, gate, 0.5, (w, None), (w, None), quantize=True)
+        same, normed = residual_norm(x, None, gate, 0.5, (w, None), (w, None))
+        want = quantize_blocks(normed.movedim(1, -1))
+        assert torch.equal(stream, same) and torch.equal(blocks.exponents, want.exponents)
+        assert torch.equal(blocks.codes.view(torch.uint8), want.codes.view(torch.uint8))
