@@ -3,6 +3,8 @@
 // of a row.
 #pragma once
 
+#include <type_traits>
+
 #include "float8_blocks.hpp"
 #include "linear_wide.hpp"
 
@@ -45,19 +47,55 @@ __device__ __forceinline__ Run as_bfloat16(const Codes32& v, int exponent, int i
 }
 
 // 32 x 32 results, 64 values of k; 16 x 16, 128. The low byte of an exponent counts.
-template <class T>
-__device__ __forceinline__ Acc16 multiply_add8(const Codes32& b, int eb, const Codes32& a, int ea, Acc16 c) {
-    if constexpr (sizeof(T) == 2) return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(__builtin_bit_cast(Eight, b), __builtin_bit_cast(Eight, a), c, 0, 0, 0, eb, 0, ea);
+__device__ __forceinline__ Acc16 multiply_add_scaled(const Codes32& b, int eb, const Codes32& a, int ea, Acc16 c) {
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(__builtin_bit_cast(Eight, b), __builtin_bit_cast(Eight, a), c, 0, 0, 0, eb, 0, ea);
+}
+__device__ __forceinline__ Acc4 multiply_add_scaled(const Codes32& b, int eb, const Codes32& a, int ea, Acc4 c) {
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(__builtin_bit_cast(Eight, b), __builtin_bit_cast(Eight, a), c, 0, 0, 0, eb, 0, ea);
+}
+__device__ __forceinline__ Acc16 multiply_add_decoded(const Codes32& b, int eb, const Codes32& a, int ea, Acc16 c) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bfloat16(b, eb, i), as_bfloat16(a, ea, i), c, 0, 0, 0);
     return c;
 }
-template <class T>
-__device__ __forceinline__ Acc4 multiply_add8(const Codes32& b, int eb, const Codes32& a, int ea, Acc4 c) {
-    if constexpr (sizeof(T) == 2) return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(__builtin_bit_cast(Eight, b), __builtin_bit_cast(Eight, a), c, 0, 0, 0, eb, 0, ea);
+__device__ __forceinline__ Acc4 multiply_add_decoded(const Codes32& b, int eb, const Codes32& a, int ea, Acc4 c) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bfloat16(b, eb, i), as_bfloat16(a, ea, i), c, 0, 0, 0);
     return c;
+}
+// The row of the first operand that result i of a lane belongs to (its row of the second is the lane's own).
+__device__ __forceinline__ int first_row(const Acc16&, int i) { return 8 * (i / 4) + threadIdx.x % 64 / 32 * 4 + i % 4; }
+__device__ __forceinline__ int first_row(const Acc4&, int i) { return threadIdx.x % 64 / 16 * 4 + i; }
+
+// bfloat16 holds every code as a normal number under the exponents 10 to 246 (2^-9 * 2^-117 to 448 * 2^119). Under others (a block with a value next to
+// the type's largest has 247; 0 is no block's but that of rows beyond the operand, which are zeros) a sum is formed with the nearest of these, and multiplied
+// by what is left over, a power of two. Asked once a block, and not in front of every product: 8192 x 4096 -> 2048 float32 167 to 172 us without, 172 to 176
+// this way, 191 to 196 that way.
+__device__ __forceinline__ int held_exponent(int e) { return min(max(e & 255, 10), 246); }
+__device__ __forceinline__ bool beyond_bfloat16(int e) { return (e & 255) != 0 && held_exponent(e) != (e & 255); }
+
+// BEYOND (results in float32): exponents beyond those of bfloat16 too.
+template <class T, bool BEYOND, class Acc>
+__device__ __forceinline__ Acc multiply_add8(const Codes32& b, int eb, const Codes32& a, int ea, Acc c) {
+    if constexpr (sizeof(T) == 2) return multiply_add_scaled(b, eb, a, ea, c);
+    else if constexpr (!BEYOND) return multiply_add_decoded(b, eb, a, ea, c);
+    else {
+        int xa = held_exponent(ea), xb = held_exponent(eb);
+        const int of_a = (ea & 255) - xa, of_b = (eb & 255) - xb;
+        asm volatile("" : "+v"(xa), "+v"(xb));                 // (or operands would be decoded ahead of the branch that leads here)
+        const Acc sum = multiply_add_decoded(b, xb, a, xa, Acc{});
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(Acc) / sizeof(float)); ++i) c[i] += ldexpf(sum[i], of_a + __shfl(of_b, first_row(c, i)));
+        return c;
+    }
+}
+// f(std::true_type()) where the wave has an exponent beyond those of bfloat16 and that matters, else f(std::false_type()).
+template <class T, class F>
+__device__ __forceinline__ void with_exponents(bool beyond, F f) {
+    if constexpr (sizeof(T) == 4) {
+        if (__builtin_expect(__any(beyond), 0)) return f(std::true_type());
+    }
+    f(std::false_type());
 }
 
 // A byte as an operand's element, for the tiles and the feed of the wide kernels.
@@ -140,6 +178,21 @@ product_float8_kernel(Coded a, Coded b, Tail<T> tail, int part_blocks, unsigned 
     };
     const auto slot = [](int h, int j) { return j < FN - 1 ? j : FN - 1 + h; };
     unsigned ea[FM], eb[FN];
+    // Float32 results of a block with exponents beyond those of bfloat16: the sums so far wait in scratch memory, where they take no registers.
+    volatile float aside[sizeof(T) == 4 ? FN * FM * 16 : 1];
+    const auto by_a = [&](int i) { return sizeof(T) == 4 ? held_exponent(static_cast<int>(ea[i])) : static_cast<int>(ea[i]); };
+    const auto by_b = [&](int i) { return sizeof(T) == 4 ? held_exponent(static_cast<int>(eb[i])) : static_cast<int>(eb[i]); };
+    const auto block_beyond = [&] {
+        bool any = false;
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < FM; ++i) any |= beyond_bfloat16(static_cast<int>(ea[i]));
+#pragma unroll
+            for (int i = 0; i < FN; ++i) any |= beyond_bfloat16(static_cast<int>(eb[i]));
+            any = __any(any);
+        }
+        return any;
+    };
     constexpr int kLoads = FeedA::N + FeedB::N, kProducts = FM * FN;
     // step h: its products, and between them the loads of stage `to` (none: -1) and the reads of the other step, of stage `from`
     const auto step = [&](int h, int from, int to) {
@@ -153,7 +206,7 @@ product_float8_kernel(Coded a, Coded b, Tail<T> tail, int part_blocks, unsigned 
 #pragma unroll
                 for (int i = p * kLoads / kProducts; i < (p + 1) * kLoads / kProducts; ++i) load(to, i);
             }
-            acc[p / FM][p % FM] = multiply_add8<T>(xb[slot(h, p / FM)], eb[p / FM], xa[h][p % FM], ea[p % FM], acc[p / FM][p % FM]);
+            acc[p / FM][p % FM] = multiply_add8<T, false>(xb[slot(h, p / FM)], by_b(p / FM), xa[h][p % FM], by_a(p % FM), acc[p / FM][p % FM]);
             // (keeps the product here: it would be moved behind all loads and reads of the stage, and spill)
             if constexpr (kProducts > 8) asm volatile("" : "+a"(acc[p / FM][p % FM]));
             else asm volatile("" : "+v"(acc[p / FM][p % FM]));
@@ -186,12 +239,25 @@ product_float8_kernel(Coded a, Coded b, Tail<T> tail, int part_blocks, unsigned 
             for (int i = 0; i < FN; ++i) eb[i] = from[TM + wn + 32 * i + column_of(l % 32)];
             load_words(group + 1);
         }
+        const bool beyond = block_beyond();
+        if (beyond) {
+            each<FN * FM * 16>([&](int i) {
+                aside[i] = acc[i / 16 / FM][i / 16 % FM][i % 16];
+                acc[i / 16 / FM][i / 16 % FM][i % 16] = 0.0f;
+            });
+        }
         step(0, s, -1);
         // stage s + 1 has landed, and the rest of this one is in registers. (Words are older than the loads of the three stages behind them by the
         // time that they are used.)
         static_assert(RING <= 4, "words land in time");
         settle<(RING - 2) * kLoads>();
         step(1, s + 1, s + RING);
+        if (beyond) {
+            each<FN * FM * 16>([&](int i) {
+                const int f = i / 16 / FM, g = i / 16 % FM, of_b = static_cast<int>(eb[f] & 255) - by_b(f), of_a = static_cast<int>(ea[g] & 255) - by_a(g);
+                acc[f][g][i % 16] = aside[i] + ldexpf(acc[f][g][i % 16], of_a + __shfl(of_b, first_row(acc[f][g], i % 16)));
+            });
+        }
 #pragma unroll
         for (int i = 0; i < FM; ++i) ea[i] >>= 8;
 #pragma unroll
@@ -272,7 +338,7 @@ few_rows_float8_kernel(Coded a, const T* x, int64_t ld_x, int64_t columns, Coded
                     // (rows beyond the end repeat the last one: nobody stores their sums)
                     quantize_share(x + min(16 * i + r, rows_x - 1) * ld_x + k, columns - k, v, e);
                 }
-                acc[i] = multiply_add8<T>(w, ew, v, e, acc[i]);
+                with_exponents<T>(beyond_bfloat16(e) || beyond_bfloat16(ew), [&](auto far) { acc[i] = multiply_add8<T, decltype(far)::value>(w, ew, v, e, acc[i]); });
             }
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");     // read before the next blocks overwrite them
@@ -318,6 +384,13 @@ narrow_float8_kernel(Coded a, const T* x, int64_t ld_x, int64_t columns, Coded b
     }
     for (int i = threadIdx.x; i < rows_w; i += kNarrowWaves * 64) words[i] = i < b.extent ? *reinterpret_cast<const unsigned*>(b.exponents + i * 4ll) : 0x7f7f7f7fu;
     __syncthreads();
+    bool weight_beyond = false;
+    if constexpr (sizeof(T) == 4) {
+        for (int i = l; i < rows_w; i += 64) {
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) weight_beyond |= beyond_bfloat16(static_cast<int>(words[i] >> 8 * kb));
+        }
+    }
     for (int64_t m0 = (blockIdx.x * static_cast<int64_t>(kNarrowWaves) + wave) * 32; m0 < a.extent; m0 += gridDim.x * static_cast<int64_t>(kNarrowWaves * 32)) {
         // (rows beyond the end repeat the last one: nobody stores their sums)
         const int64_t m = min(m0 + l % 32, a.extent - 1);
@@ -367,20 +440,27 @@ narrow_float8_kernel(Coded a, const T* x, int64_t ld_x, int64_t columns, Coded b
                     codes[kb][h] = {Chunk{c[8 * h], c[8 * h + 1], c[8 * h + 2], c[8 * h + 3]}, Chunk{c[8 * h + 4], c[8 * h + 5], c[8 * h + 6], c[8 * h + 7]}};
             }
         }
-        for (int n0 = 0; n0 < b.extent; n0 += 32) {
-            Acc16 acc[1][1] = {};
-            const unsigned word = words[n0 + column_of(l % 32)];
+        bool beyond = weight_beyond;
+        if constexpr (sizeof(T) == 4) {
 #pragma unroll
-            for (int kb = 0; kb < KB; ++kb) {
-                const Chunk* tile = weight + kb * rows_w * 8;
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const Codes32 w = {fragment<Code, true, 32, 8, true>(tile, n0, 2 * h), fragment<Code, true, 32, 8, true>(tile, n0, 2 * h + 1)};
-                    acc[0][0] = multiply_add8<T>(w, static_cast<int>(word >> 8 * kb), codes[kb][h], ea[kb], acc[0][0]);
-                }
-            }
-            store_blocks<T, 1, 1>(tail, acc, m0, n0, 0, turn);
+            for (int kb = 0; kb < KB; ++kb) beyond |= beyond_bfloat16(ea[kb]);
         }
+        with_exponents<T>(beyond, [&](auto far) {
+            for (int n0 = 0; n0 < b.extent; n0 += 32) {
+                Acc16 acc[1][1] = {};
+                const unsigned word = words[n0 + column_of(l % 32)];
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb) {
+                    const Chunk* tile = weight + kb * rows_w * 8;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const Codes32 w = {fragment<Code, true, 32, 8, true>(tile, n0, 2 * h), fragment<Code, true, 32, 8, true>(tile, n0, 2 * h + 1)};
+                        acc[0][0] = multiply_add8<T, decltype(far)::value>(w, static_cast<int>(word >> 8 * kb), codes[kb][h], ea[kb], acc[0][0]);
+                    }
+                }
+                store_blocks<T, 1, 1>(tail, acc, m0, n0, 0, turn);
+            }
+        });
     }
 }
 
