@@ -22,10 +22,12 @@ struct Coded {
 // 32 codes of a row: a lane's share of 64 values of k.
 struct Codes32 { Chunk lo, hi; };
 
-// The 8-bit instructions cut every product of 8 neighbouring k down to a multiple of 2^-13 of the largest of them before they add (found
-// with products of one large and one small pair: one 2^13 times smaller is kept, one 2^14 times smaller is lost, from the ninth k on nothing
-// is). That is 1e-5 to 4e-5 of a sum of random signs, far below half a step of the 16-bit types. Results in float32 take the bfloat16
-// instructions instead, at half the rate: codes and powers of two fit that type, and its products add up in float32.
+// The 8-bit instructions cut every product of 8 neighbouring k down, towards zero, to a multiple of 2^-13 of the largest of them before they add (found
+// with products of one large and one small pair: one 2^13 times smaller is kept, one 2^14 times smaller is lost, of either sign, from the ninth k on nothing
+// is). Measured against 64 bits: 1.5e-5 to 4e-5 of a sum of random signs, -3e-6 of a sum of one sign (normal values, K 64 to 4096); at worst 7 * 2^-13 of each
+// group's largest product. Half a step of the 16-bit types is 2^-9 to 2^-8 and 2^-12 to 2^-11 of a result, but of the result: where large products cancel, what is
+// left of small ones beside them can be lost. 16-bit results take these instructions all the same: their operands were rounded to 2^-4. Results in float32 take
+// the bfloat16 instructions instead, at half the rate or less: codes and powers of two fit that type, and its products add up in float32.
 typedef int Eight __attribute__((ext_vector_type(8)));
 typedef __bf16 Run __attribute__((ext_vector_type(8)));
 typedef float Acc4 __attribute__((ext_vector_type(4)));

@@ -1,6 +1,6 @@
 """How far the sums of ``linear_act_float8`` may be off: float32 results have float32's sums of exact products; for 16-bit results the matrix instructions
-cut every product down (towards zero) to a multiple of 2^-13 of the largest among 8 neighbouring ones. Powers over
-their whole range."""
+cut every product down (towards zero) to a multiple of 2^-13 of the largest among 8 neighbouring ones. Data of one sign, whose cuts add up, products that
+cancel, and powers over their whole range."""
 import pytest
 import torch
 
@@ -41,6 +41,43 @@ def within(y, x, w, dtype):
     off[y.isinf() & (y.sign() == z.sign()) & (z.abs() + bound >= most)] = 0.0          # (rounds to an infinity, or may)
     worst = (off / bound).max().item()
     assert worst <= 1.0, "%.3g times the bound" % worst
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,K,N", SHAPES)
+def test_values_of_one_sign(hip, M, K, N, dtype):
+    """Rows behind a relu through weights of one sign, with channels of very different size: nothing cancels, every cut is a loss."""
+    from box_convolution import linear_act_float8, quantize_blocks
+    gen = torch.Generator().manual_seed(M + K)
+    rows = min(M, 300)
+    x = (torch.randn(rows, K, generator=gen).clamp_min(0) * torch.exp(torch.randn(K, generator=gen))).to(dtype)
+    w = torch.randn(N, K, generator=gen).abs() * K ** -0.5
+    w8, repeat = quantize_blocks(w.cuda()), -(-M // rows)
+    x8, xs = ref.dequantize(x.double()), x.cuda().repeat(repeat, 1)[:M]
+    for given in (xs, quantize_blocks(xs)):
+        y = linear_act_float8(given, w8, dtype=dtype)
+        within(y[:rows], x8, ref.dequantize(w.double()), dtype)
+        assert torch.equal(y[M - M % rows:], y[:M % rows])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,K,N", SHAPES)
+def test_products_that_cancel(hip, M, K, N, dtype):
+    """Two large products of opposite sign in a group of 8 and six small ones: float32 results are what the small ones add up to, exactly."""
+    from box_convolution import Float8Blocks, linear_act_float8, quantize_blocks
+    gen = torch.Generator().manual_seed(M + K)
+    x, w = (torch.randint(-8, 9, (n, K), generator=gen).float() / 8 for n in (min(M, 300), N))
+    x[:, 0::8], x[:, 7::8], w[:, 0::8], w[:, 7::8] = 256.0, 256.0, 256.0, -256.0
+    if K % 8:
+        x[:, K // 8 * 8:] = 0.0
+    w8, xs = quantize_blocks(w.cuda()), x.repeat(-(-M // x.size(0)), 1)[:M].cuda().to(dtype)
+    assert torch.equal(w8.dequantize().cpu(), w)
+    given = quantize_blocks(xs)
+    assert isinstance(given, Float8Blocks) and torch.equal(given.dequantize()[:x.size(0)].cpu(), x)
+    y = linear_act_float8(given, w8, dtype=dtype)[:x.size(0)]
+    within(y, x.double(), w.double(), dtype)
+    if dtype == torch.float32:
+        assert torch.equal(y.cpu().double(), x.double() @ w.double().t())
 
 
 @pytest.mark.parametrize("dtype", TYPES)
