@@ -211,9 +211,11 @@ def _gate_kind(gate, input):
         return _native.GATE_NONE
     B, C = input.size(0), input.size(1)
     for kind, shape in ((_native.GATE_FULL, tuple(input.shape)), (_native.GATE_CHANNEL, (C,)), (_native.GATE_ITEM, (B, C))):
+        if kind == _native.GATE_FULL and input.dim() == 2 and gate.dtype != input.dtype:
+            continue                                   # (an input [B, C] has one value per item and channel itself)
         if tuple(gate.shape) == shape:
             if gate.device != input.device or gate.dtype not in ((input.dtype,) if kind == _native.GATE_FULL else (input.dtype, torch.float32)):
-                raise RuntimeError("box_convolution: gate must be on %s, of the input's type or, where it has one value per channel, float32" % input.device)
+                raise RuntimeError("box_convolution: gate must be on %s, of the input's type or, where it is [C] or [B, C], float32" % input.device)
             return kind
     raise RuntimeError("box_convolution: gate must have the shape [C], [B, C] or that of the input, got %s for an input of %s"
                        % (tuple(gate.shape), tuple(input.shape)))
@@ -246,7 +248,7 @@ def residual_norm(input, residual=None, gate=None, scale=1.0, after=None, before
     input:    ``[B, C, ...]``; channels-last memory is used as it is, anything else is copied once. The results have channels-last memory.
     residual: same shape and type, or ``None`` for 0.
     gate:     ``None`` for 1, ``[C]`` (a layer scale), ``[B, C]`` (a gate per batch item) or of the input's shape; of the input's type, or
-              float32 where it has one value per channel.
+              float32 where it is ``[C]`` or ``[B, C]``.
     after, before: the norms behind this block and before the next one: ``None`` where there is none, or ``(weight, bias)``,
               each ``[C]`` or ``None`` for 1 and 0, all float32 or all of the input's type.
     kind:     ``"rms"``: ``v / sqrt(mean(v * v) + eps)`` over a row's channels; ``"layer"``: the same of ``v - mean(v)``.

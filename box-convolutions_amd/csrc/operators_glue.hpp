@@ -454,10 +454,12 @@ std::vector<at::Tensor> residual_norm(const at::Tensor& input, const Optional& r
     TORCH_CHECK(C <= INT32_MAX, "box_convolution: residual norm of ", C, " channels");
     int gate_kind = kNoGate;
     if (gate) {
-        gate_kind = gate->sizes() == input.sizes() ? kGateOfElement : gate->sizes() == at::IntArrayRef({C}) ? kGateOfChannel : gate->sizes() == at::IntArrayRef({B, C}) ? kGateOfItem : -1;
+        // (an input [B, C] has one value per item and channel itself: a gate of another type is then one per item)
+        const bool whole = gate->sizes() == input.sizes() && (input.dim() > 2 || gate->scalar_type() == input.scalar_type());
+        gate_kind = whole ? kGateOfElement : gate->sizes() == at::IntArrayRef({C}) ? kGateOfChannel : gate->sizes() == at::IntArrayRef({B, C}) ? kGateOfItem : -1;
         TORCH_CHECK(gate_kind >= 0, "box_convolution: gate must have the shape [C], [B, C] or that of the input, got ", gate->sizes(), " for an input of ", input.sizes());
         TORCH_CHECK(gate->device() == input.device() && (gate->scalar_type() == input.scalar_type() || (gate->scalar_type() == at::kFloat && gate_kind != kGateOfElement)),
-                    "box_convolution: gate must be on ", input.device(), ", of the input's type or, where it has one value per channel, float32");
+                    "box_convolution: gate must be on ", input.device(), ", of the input's type or, where it is [C] or [B, C], float32");
     }
     std::optional<at::ScalarType> kind;
     for (const Optional* p : {&after_weight, &after_bias, &before_weight, &before_bias}) {

@@ -27,3 +27,16 @@ def test_blocks_of_items_that_workgroups_do_not_divide(hip):
         want = quantize_blocks(normed.movedim(1, -1))
         assert torch.equal(stream, same) and torch.equal(blocks.exponents, want.exponents)
         assert torch.equal(blocks.codes.view(torch.uint8), want.codes.view(torch.uint8))
+
+
+@pytest.mark.parametrize("side", ["C++", "Python"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("B,C", [(1, 40), (5, 52), (1025, 24), (257, 700), (513, 4096), (9, 8200)])
+def test_float32_gate_per_item_of_rows(hip, monkeypatch, B, C, dtype, side):
+    """An input [B, C] has a row per item: a float32 gate [B, C] beside 16-bit rows is a gate per item like any other, with a float32 gradient."""
+    if side == "Python":
+        monkeypatch.setattr(hip, "_glue", False)
+    c = case(B, C, (), dtype, ("layer", "rms")[C % 3 == 0], "item", params="float", float_gate=True)
+    out = run(c)
+    assert out["gate"].dtype == torch.float32
+    check(out, expected(c))
