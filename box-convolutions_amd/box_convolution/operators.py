@@ -313,11 +313,25 @@ def residual_norm(input, residual=None, gate=None, scale=1.0, after=None, before
 class Float8Blocks:
     """Rows ``[..., columns]`` in 8-bit floating point (e4m3), a power of two for each block of 128 columns: value =
     ``codes * 2**(exponents - 127)``. ``codes``: ``[..., columns rounded up to 128]`` float8_e4m3fn, zeros beyond the columns;
-    ``exponents``: ``[..., blocks rounded up to 4]`` uint8, from 1 to 254, 127 beyond the blocks. Both contiguous, on one device."""
+    ``exponents``: ``[..., blocks rounded up to 4]`` uint8, from 1 to 254, 127 beyond the blocks. Both contiguous, on one device. What belongs together stays
+    together: none of the three can be assigned (their values can be written in place)."""
 
-    __slots__ = ("codes", "exponents", "columns")
+    __slots__ = ("_codes", "_exponents", "_columns")           # read-only: kernels address codes and exponents by what was checked
 
     def __init__(self, codes, exponents, columns):
+        self._codes, self._exponents, self._columns = codes, exponents, columns
+        self._check()
+
+    @classmethod
+    def _of(cls, codes, exponents, columns):
+        """Of tensors that an operator made: nothing to check."""
+        self = object.__new__(cls)
+        self._codes, self._exponents, self._columns = codes, exponents, columns
+        return self
+
+    def _check(self):
+        """Raises unless the tensors are what the columns need. (Again in every call: tensors can be resized, and point to other memory later.)"""
+        codes, exponents, columns = self._codes, self._exponents, self._columns
         width, words = _native.block_sizes(columns)
         if (codes.dtype != torch.float8_e4m3fn or exponents.dtype != torch.uint8 or codes.device != exponents.device or columns < 1
                 or codes.dim() < 1 or codes.size(-1) != width or tuple(exponents.shape) != (*codes.shape[:-1], words)):
@@ -325,14 +339,10 @@ class Float8Blocks:
                                "columns, got %s %s and %s %s" % (width, words, columns, codes.dtype, tuple(codes.shape), exponents.dtype, tuple(exponents.shape)))
         if not codes.is_contiguous() or not exponents.is_contiguous() or codes.data_ptr() % 16 or exponents.data_ptr() % 4:
             raise RuntimeError("box_convolution: the codes and exponents of Float8Blocks must be contiguous, at addresses of whole 16 and 4 bytes")
-        self.codes, self.exponents, self.columns = codes, exponents, columns
 
-    @classmethod
-    def _of(cls, codes, exponents, columns):
-        """Of tensors that an operator made: nothing to check."""
-        self = object.__new__(cls)
-        self.codes, self.exponents, self.columns = codes, exponents, columns
-        return self
+    codes = property(lambda self: self._codes)
+    exponents = property(lambda self: self._exponents)
+    columns = property(lambda self: self._columns)
 
     @property
     def shape(self):
@@ -404,6 +414,8 @@ def linear_act_float8(input, weight, bias=None, residual=None, activation=None, 
                                           weight.codes, weight.exponents, weight.columns, bias, residual, act, dtype, _native._stream(rows_of.device) or 0)
     if not coded:
         _native._operator_dtype(input, "linear float8 input")
+    for blocks in (input, weight) if coded else (weight,):
+        blocks._check()
     dtype = dtype or (torch.bfloat16 if coded else input.dtype)
     if dtype not in _native._FUSED_OUTPUT or (not coded and dtype != input.dtype):
         raise RuntimeError("box_convolution: the result's type must be that of the values, or float32, float16 or bfloat16 for Float8Blocks, got %s" % dtype)

@@ -536,10 +536,23 @@ std::vector<at::Tensor> quantize_blocks(const at::Tensor& input, int64_t stream)
     return {codes, exponents};
 }
 
-// `input`: values, or codes with `exponents`. The shapes of blocks were looked at when they were made.
+// The kernels address blocks by their columns alone. (What Float8Blocks looked at when it was made may have been resized since, or point to other memory.)
+void check_blocks(const at::Tensor& codes, const at::Tensor& exponents, int64_t columns) {
+    const int64_t blocks = (columns + 127) / 128, words = (blocks + 3) / 4 * 4;
+    bool fits = columns >= 1 && codes.scalar_type() == at::kFloat8_e4m3fn && exponents.scalar_type() == at::kByte && codes.device() == exponents.device() &&
+                codes.dim() >= 1 && codes.dim() == exponents.dim() && codes.size(-1) == blocks * 128 && exponents.size(-1) == words;
+    for (int64_t d = 0; fits && d + 1 < codes.dim(); ++d) fits = codes.size(d) == exponents.size(d);
+    TORCH_CHECK(fits, "box_convolution: Float8Blocks needs float8_e4m3fn codes [..., ", blocks * 128, "] and uint8 exponents [..., ", words, "] on one device for ", columns,
+                " columns, got ", codes.scalar_type(), " ", codes.sizes(), " and ", exponents.scalar_type(), " ", exponents.sizes());
+    TORCH_CHECK(codes.is_contiguous() && exponents.is_contiguous(), "box_convolution: the codes and exponents of Float8Blocks must be contiguous");
+}
+
+// `input`: values, or codes with `exponents`.
 at::Tensor linear_act_float8(const at::Tensor& input, const Optional& exponents, int64_t columns, const at::Tensor& weight, const at::Tensor& weight_exponents,
                              int64_t weight_columns, const Optional& bias, const Optional& residual, int64_t act, std::optional<at::ScalarType> dtype, int64_t stream) {
-    if (!exponents) check_operator_input(input, "linear float8 input");
+    if (exponents) check_blocks(input, *exponents, columns);
+    else check_operator_input(input, "linear float8 input");
+    check_blocks(weight, weight_exponents, weight_columns);
     const at::ScalarType to = dtype ? *dtype : exponents ? at::kBFloat16 : input.scalar_type();
     TORCH_CHECK((to == at::kFloat || to == at::kHalf || to == at::kBFloat16) && (exponents || to == input.scalar_type()),
                 "box_convolution: the result's type must be that of the values, or float32, float16 or bfloat16 for Float8Blocks, got ", to);
