@@ -356,10 +356,12 @@ class Float8Blocks:
         return Float8Blocks(self.codes.to(device), self.exponents.to(device), self.columns)
 
     def dequantize(self, dtype=torch.float32):
-        """The values, ``[..., columns]`` (elementary torch operations: to look at, not for a fast path)."""
-        blocks = self.codes.float().unflatten(-1, (-1, _native.BLOCK))
+        """The values, ``[..., columns]`` (elementary torch operations: to look at, not for a fast path). Of float32 and narrower types those above the type's
+        largest are infinite: a value next to float32's own largest may be rounded up to 2**128."""
+        wide = torch.float64 if dtype == torch.float64 else torch.float32
+        blocks = self.codes.to(wide).unflatten(-1, (-1, _native.BLOCK))
         # 2**(exponent - 127), put together from its bits
-        power = (self.exponents[..., :blocks.size(-2)].int() << 23).view(torch.float32)
+        power = (self.exponents[..., :blocks.size(-2)].int() << 23).view(torch.float32).to(wide)
         return (blocks * power[..., None]).flatten(-2)[..., :self.columns].to(dtype)
 
 

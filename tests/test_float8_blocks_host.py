@@ -46,3 +46,14 @@ def test_calls_look_again(how, monkeypatch):
                 continue                                                    # (values on the CPU are refused first there)
             with pytest.raises(RuntimeError, match="Float8Blocks"):
                 linear_act_float8(x, w)
+
+
+def test_values_of_every_exponent():
+    """In 64 bits every code times every power is a number; in float32 those from 2^128 on are infinite."""
+    import block_reference as ref
+    units = torch.cat([ref.CODE_VALUES, -ref.CODE_VALUES[1:]])
+    b = Float8Blocks(torch.zeros(254, 256).to(torch.float8_e4m3fn), torch.full((254, 4), 127, dtype=torch.uint8), units.numel())
+    b.codes[:, :units.numel()] = units.to(torch.float8_e4m3fn)
+    b.exponents[:, :2] = torch.arange(1, 255, dtype=torch.uint8)[:, None]
+    want = units * ref.two_to(torch.arange(1, 255) - 127)[:, None]
+    assert torch.equal(b.dequantize(torch.float64), want) and torch.equal(b.dequantize(), want.float())
