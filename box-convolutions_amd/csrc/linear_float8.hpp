@@ -447,22 +447,27 @@ narrow_float8_kernel(Coded a, const T* x, int64_t ld_x, int64_t columns, Coded b
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) beyond |= beyond_bfloat16(ea[kb]);
         }
-        with_exponents<T>(beyond, [&](auto far) {
-            for (int n0 = 0; n0 < b.extent; n0 += 32) {
-                Acc16 acc[1][1] = {};
-                const unsigned word = words[n0 + column_of(l % 32)];
+        const auto columns_from = [&](auto far, int n0) {
+            Acc16 acc[1][1] = {};
+            const unsigned word = words[n0 + column_of(l % 32)];
 #pragma unroll
-                for (int kb = 0; kb < KB; ++kb) {
-                    const Chunk* tile = weight + kb * rows_w * 8;
+            for (int kb = 0; kb < KB; ++kb) {
+                const Chunk* tile = weight + kb * rows_w * 8;
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const Codes32 w = {fragment<Code, true, 32, 8, true>(tile, n0, 2 * h), fragment<Code, true, 32, 8, true>(tile, n0, 2 * h + 1)};
-                        acc[0][0] = multiply_add8<T, decltype(far)::value>(w, static_cast<int>(word >> 8 * kb), codes[kb][h], ea[kb], acc[0][0]);
-                    }
+                for (int h = 0; h < 2; ++h) {
+                    const Codes32 w = {fragment<Code, true, 32, 8, true>(tile, n0, 2 * h), fragment<Code, true, 32, 8, true>(tile, n0, 2 * h + 1)};
+                    acc[0][0] = multiply_add8<T, decltype(far)::value>(w, static_cast<int>(word >> 8 * kb), codes[kb][h], ea[kb], acc[0][0]);
                 }
-                store_blocks<T, 1, 1>(tail, acc, m0, n0, 0, turn);
             }
-        });
+            store_blocks<T, 1, 1>(tail, acc, m0, n0, 0, turn);
+        };
+        if constexpr (sizeof(T) == 2) {
+            for (int n0 = 0; n0 < b.extent; n0 += 32) columns_from(std::false_type(), n0);
+        } else {
+            with_exponents<T>(beyond, [&](auto far) {
+                for (int n0 = 0; n0 < b.extent; n0 += 32) columns_from(far, n0);
+            });
+        }
     }
 }
 
