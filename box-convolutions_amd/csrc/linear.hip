@@ -657,7 +657,11 @@ void launch_float8(Coded a, const Coded& b, Tail<T> tail, const ProductPlan& p, 
 }
 
 // The plan of 16-bit products by the same estimate, a stage of 128 bytes being a block here; parts of k are whole words of exponents. (Results in
-// float32: no tiles of 256 x 256, whose fragments do not fit the registers as bfloat16.)
+// float32: no tiles of 256 x 256, whose fragments do not fit the registers as bfloat16.) The constants are those of 16-bit products; measured here, repeated alone,
+// with tiles of 256, 128 and 64 (float32 results 128 and 64), the plan's choice first in brackets: 8192 x 4096 -> 2048 [256] 63, 105, 131 us (float32 [128] 170,
+// 202); 8192 x 2048 -> 4096 [256] 71, 114, 135 ([128] 177, 218); 4096 x 2048 -> 2048 [128] 31, 31, 37 ([128] 50, 58); 2048 x 4096 -> 2048 [128] 37, 47, 36 ([128]
+// 61, 59); 1024 x 4096 -> 1024 [64] 28, 28, 19 ([64] 31, 28); 512 x 4096 -> 512 [64 in four parts] 20, 18, 13 ([same] 20, 15); 300000 x 64 -> 256 [256] 43, 43, 43
+// ([128] 92, 92); 20000 x 256 -> 256 [128] 14, 11, 10 ([128] 17, 14); 1501 x 333 -> 517 [64] 15, 12, 6 ([64] 15, 8).
 template <class T>
 ProductPlan plan_float8(int64_t rows, int64_t K, int64_t N) {
     constexpr ProductShape kSmall[] = {kWide[1], kWide[2]};
@@ -673,7 +677,9 @@ ProductPlan plan_float8(int64_t rows, int64_t K, int64_t N) {
 
 // Few rows take one launch, values too while quantizing them in every workgroup again costs less than another launch: 16 rows of 1024 -> 4096
 // bfloat16 5.5 us as values or codes, of 4096 12.2 and 7.4, of 8192 -> 2048 20.6 and 11.9, where quantizing takes 3 to 4; 32 rows of 2048 -> 4096 11.0 and 7.7.
-// (64 rows this way were no better than tiles: 1024 -> 4096 7.4 and 7.8, 4096 -> 4096 20 and 12.)
+// (64 rows this way were no better than tiles: 1024 -> 4096 7.4 and 7.8, 4096 -> 4096 20 and 12.) Codes in bfloat16 this way and through tiles: 16 rows of 1024 -> 4096
+// 4.3 and 7.7 us, 4096 -> 4096 7.7 and 10.5, 4096 -> 1024 7.2 and 8.9, 8192 -> 2048 12.1 and 11.4; 32 rows of 512 -> 512 4.4 and 6.0, 1024 -> 4096 5.6 and 7.9, 2048 -> 4096
+// 7.9 and 9.3, but 4096 -> 4096 13.6 and 11.9, 4096 -> 1024 13.4 and 9.2, 8192 -> 2048 23.0 and 12.3: the border is one of rows, and long rows pay for it from 17 on.
 constexpr int64_t kFewRows = 32, kFewRowsValues = 2048;
 
 // The bytes of rows in 8 bits, codes and then exponents.

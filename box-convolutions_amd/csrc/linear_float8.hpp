@@ -24,8 +24,8 @@ struct Codes32 { Chunk lo, hi; };
 
 // The 8-bit instructions cut every product of 8 neighbouring k down, towards zero, to a multiple of 2^-13 of the largest of them before they add (found
 // with products of one large and one small pair: one 2^13 times smaller is kept, one 2^14 times smaller is lost, of either sign, from the ninth k on nothing
-// is). Measured against 64 bits: 1.5e-5 to 4e-5 of a sum of random signs, -3e-6 of a sum of one sign (normal values, K 64 to 4096); at worst 7 * 2^-13 of each
-// group's largest product. Half a step of the 16-bit types is 2^-9 to 2^-8 and 2^-12 to 2^-11 of a result, but of the result: where large products cancel, what is
+// is). Measured against 64 bits: 1.5e-5 to 4e-5 of a sum of random signs, -3e-6 of a sum of one sign (normal values, K 64 to 4096), by a model of the
+// cut -1e-5 to -1e-4 where channels differ by factors of e to e^2; at worst 7 * 2^-13 of each group's largest product. Half a step of the 16-bit types is 2^-9 to 2^-8 and 2^-12 to 2^-11 of a result, but of the result: where large products cancel, what is
 // left of small ones beside them can be lost. 16-bit results take these instructions all the same: their operands were rounded to 2^-4. Results in float32 take
 // the bfloat16 instructions instead, at half the rate or less: codes and powers of two fit that type, and its products add up in float32.
 typedef int Eight __attribute__((ext_vector_type(8)));
@@ -113,9 +113,10 @@ __device__ __forceinline__ void word_to_lds(Descriptor d, unsigned offset, unsig
 // codes of every row. A block is two steps of 64 values of k. The barrier stands between them: the second step's fragments are in registers by then, so the
 // stage takes a block RING further on, whose loads go out one at a time between the second step's products. Exponents come four blocks at a time, a
 // word of every row, into a ring of their own; a lane keeps the words of its rows and shifts them by a byte from block to block.
-// Bound by the matrix instructions while tiles go round: 8192 x 8192 -> 8192 bfloat16 2.5 PFLOP/s, where a library's product with one scale a tensor
-// reaches 2.6. With one tile a compute unit its first loads and its epilogue are not hidden: 8192 x 4096 -> 2048 62 us (2.2 PFLOP/s), with silu, bias and a
-// residual 70 to 76, a library's without them 50; 8192 x 2048 -> 4096 69, with gelu 87, a library's 65. Float32 results: at most half of that.
+// Bound by the matrix instructions while tiles go round: 8192 x 8192 -> 8192 bfloat16 486 us (2.3 PFLOP/s; 452 at best), where a library's product with one scale
+// a tensor reaches 2.6. With one tile a compute unit its first loads and its epilogue are not hidden: 8192 x 4096 -> 2048 repeated alone 61 us (2.3 PFLOP/s), with
+// silu, bias and a residual 66, right behind the launch that quantizes its rows 80 to 85, a library's without them 50; 8192 x 2048 -> 4096 69, with gelu 87, behind
+// the norm that writes its rows 102 to 105, a library's 65. Float32 results: 8192 x 8192 -> 8192 1.30 ms (0.85 PFLOP/s), 8192 x 4096 -> 2048 174 to 210 us. (Medians.)
 // No better: parts of k that start at another block in every tile, four waves for a tile of 256 x 256.
 template <class T, int TM, int TN, int WM, int WN, int RING>
 __global__ void __launch_bounds__(WM * WN * 64)
@@ -365,7 +366,8 @@ few_rows_float8_kernel(Coded a, const T* x, int64_t ld_x, int64_t columns, Coded
 // y of many rows through a weight of at most KB blocks a row that LDS holds whole. A wave takes 32 rows at a time with all their columns: its
 // lanes read the row's values (or, CODED, its codes) once, two lanes a row, and quantize them in registers; the codes never go through memory.
 // Then 32 columns at a time: products, epilogue. Workgroups of eight waves go round over the rows. WHOLE: rows of values end with a block.
-// Bound by memory: 131072 x 128 -> 32 bfloat16 with relu 11.4 us, 3.7 TB/s of values in and results out (quantized first and through tiles 24.2).
+// Bound by memory: 131072 x 128 -> 32 bfloat16 with relu 11.4 to 11.9 us repeated alone, 3.6 TB/s of values in and results out, 12.4 to 13.2 among passes on other
+// inputs (quantized first and through tiles 24.2). Float32 22.8 us.
 constexpr int kNarrowBlocks = 4, kNarrowWaves = 8;         // (a row's exponents are one word)
 constexpr size_t kNarrowWeight = 64 * 1024;
 constexpr size_t narrow_float8_lds(int64_t columns, int blocks) { return static_cast<size_t>((columns + 31) / 32 * 32) * (blocks * kBlock + 4) + kNarrowWaves * 4096; }

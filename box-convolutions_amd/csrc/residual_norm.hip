@@ -13,12 +13,13 @@
 // s is formed in float32 and h and the backward take it unrounded: the backward forms it again from x, the residual and the gate.
 // Statistics, sums over rows and every step between a load and a store are float32; what is stored is rounded once.
 //
-// Bound by memory: forward 20, backward 40 operations for each of 4 and 6 elements moved. Where a copy of 1 GiB reaches 5.2 TB/s:
-//   forward   4 x 128 x 256 x 128 bfloat16, layer, gate per item   28 us 4.8 TB/s    8192 x 4096 bfloat16, rms   48 to 54 us 5.0 to 5.6 TB/s
-//   backward                                                        41 us 4.9 TB/s                                 83 to 88 us 4.6 to 4.9 TB/s
-//   2 x 301 x 767 x 52 float16, layer, gate per element             forward 55 to 58 us 4.2 to 4.3 TB/s, backward 89 to 92 us 4.2 to 4.3 TB/s
-// and its sums' join 4 to 5 us. One row of 4096 without gradients 4.4 us. 16384 x 1000 bfloat16 26 and 40 us, x 1001 31 and 52.
-// Still far from it: the backward of more than 4096 channels, whose sums leave the registers (4096 x 8190 bfloat16 145 us, 2.8 TB/s).
+// Bound by memory: forward 20, backward 40 operations for each of 4 and 6 elements moved. Where a copy of 1 GiB reaches 5.2 TB/s (medians of a kernel trace):
+//   forward   4 x 128 x 256 x 128 bfloat16, layer, gate per item   28 us 4.8 TB/s    8192 x 4096 bfloat16, rms   53 us 5.1 TB/s
+//   backward                                                        41 us 4.9 TB/s                                 86 us 4.7 TB/s
+//   2 x 301 x 767 x 52 float16, layer, gate per element             forward 57 us 4.2 TB/s, backward 91 to 93 us 4.1 to 4.2 TB/s
+// and its sums' join 4 to 5 us. One row of 4096 without gradients 4.4 us. Rms without a gate: 16384 x 1000 bfloat16 28 and 37 us, x 1001 31 and 46.
+// Still far from it: the backward of more than 4096 channels, whose sums leave the registers (4096 x 8190 bfloat16 134 us, 3.0 TB/s), and both passes of
+// more than 8192, element by element (4096 x 12288 bfloat16 0.60 and 4.6 ms, where a copy of the same bytes takes 0.08 and 0.12).
 #include <type_traits>
 
 #include "float8_blocks.hpp"
@@ -888,7 +889,9 @@ void known_lanes(const Shape& s, F f) {
 
 // As many workgroups as the chip holds at once: the forward's kernels leave room for four waves a SIMD, the backward's for two, and a workgroup is on one
 // compute unit whole: counted in waves, workgroups of 3, 5, 6 or 7 came in two rounds (8192 x 3500 bfloat16 forward 71 us, backward 139; 53 and 82 this way;
-// 4096 x 6400 backward 162 and 101; with 4 or 8 waves the count is the same). (Fewer where the backward's sums are long and in memory.)
+// 4096 x 6400 backward 162 and 101; with 4 or 8 waves the count is the same). (Fewer where the backward's sums are long and in memory, two read and written
+// for every row: 4096 x 12288 bfloat16 takes it 4.7 ms with 128 workgroups, 2.4 with 256, 512 or 1024; 2048 x 16384 3.2 and 1.6; 64 x 16384 0.16 with any number.
+// Their workspace grows with them, 20 bytes a channel and workgroup.)
 int64_t resident(const Shape& s, int waves) { return 256 * std::max(1, waves * 64 / s.threads); }
 RowPlan forward_plan(const ResidualNormCall& c, const Shape& s) { return plan_rows(c, resident(s, s.big ? 8 : 16), s.rows); }
 RowPlan backward_plan(const ResidualNormCall& c, const Shape& s) { return plan_rows(c, s.lanes == 0 ? 128 : resident(s, 8), s.rows); }
