@@ -894,7 +894,7 @@ void known_lanes(const Shape& s, F f) {
 // Their workspace grows with them, 20 bytes a channel and workgroup.)
 int64_t resident(const Shape& s, int waves) { return 256 * std::max(1, waves * 64 / s.threads); }
 RowPlan forward_plan(const ResidualNormCall& c, const Shape& s) { return plan_rows(c, resident(s, s.big ? 8 : 16), s.rows); }
-RowPlan backward_plan(const ResidualNormCall& c, const Shape& s) { return plan_rows(c, s.lanes == 0 ? 128 : resident(s, 8), s.rows); }
+RowPlan backward_plan(const ResidualNormCall& c, const Shape& s) { return plan_rows(c, backward_target(c, s.rows, s.lanes == 0 ? 128 : resident(s, 8)), s.rows); }
 
 }  // namespace
 

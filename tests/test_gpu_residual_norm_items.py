@@ -40,3 +40,20 @@ def test_float32_gate_per_item_of_rows(hip, monkeypatch, B, C, dtype, side):
     out = run(c)
     assert out["gate"].dtype == torch.float32
     check(out, expected(c))
+
+
+@pytest.mark.parametrize("B,C,pixels,gate", [(1 << 21, 8, 1, "item"), (1 << 20, 12, 2, "item"), (300007, 40, 1, "item"), (1 << 17, 520, 1, "item"), (1 << 22, 8, 1, "channel")])
+def test_sums_over_many_items(hip, B, C, pixels, gate):
+    """Items of a row or two, as many as a tensor of a few dozen megabytes has: the parameters' gradients are no longer chains of additions for that. The same
+    gradients everywhere, so that a chain's roundings would add up; 512 additions in a row are allowed, as everywhere."""
+    from box_convolution import residual_norm
+    g = torch.full((B, C, pixels), 1.1, device="cuda")
+    x, r = (torch.randn(B, C, pixels, device="cuda") for _ in range(2))
+    gate_, w, b = torch.ones(B, C, device="cuda") if gate == "item" else torch.ones(C, device="cuda"), torch.ones(C, device="cuda"), torch.zeros(C, device="cuda")
+    leaves = [t.requires_grad_(True) for t in (w, b, w.detach().clone(), b.detach().clone())]
+    s, h = residual_norm(x, r, gate_, 1.0, (leaves[0], leaves[1]), (leaves[2], leaves[3]), "layer")
+    got = torch.autograd.grad([s, h], leaves[1::2], [g, torch.zeros_like(h)])[0], torch.autograd.grad(residual_norm(x, r, gate_, 1.0, (w, b), (leaves[2], leaves[3]), "layer")[1],
+                                                                                                        leaves[3], g)[0]
+    want = g[0, 0, 0].double().item() * B * pixels
+    for k, sums in enumerate(got):
+        assert (sums.double() - want).abs().max().item() <= 512 * 2.0 ** -24 * want, (k, (sums.double() / want - 1).abs().max().item() * 2 ** 24)

@@ -73,3 +73,44 @@ def test_kernels_walk_as_the_test_does():
         source = file.read()
     calls = source.count("span_of(")
     assert calls == 4 and source.count("i < items_of(a.plan, blockIdx.x); ++i) {\n        const Span span = span_of(a.plan, a.pixels, blockIdx.x, i);") == calls
+
+
+CHAINS = r"""
+#include <cstdio>
+#include "residual_norm.hpp"
+using namespace boxconv;
+
+int main() {
+    long most = 0;
+    for (const int kind : {kGateChannel, kGateItem})
+        for (int64_t batch = 1; batch < 100000000; batch = batch * 3 + 1)
+            for (int64_t pixels = 1; pixels < 100000000 && batch * pixels < 10000000000; pixels = pixels * 5 + 2)
+                for (const int64_t at_once : {1, 4, 32, 256})
+                    for (const int64_t resident : {128, 256, 512, 1024}) {
+                        ResidualNormCall c = {};
+                        c.gate_kind = kind;
+                        c.batch = batch;
+                        c.pixels = pixels;
+                        const RowPlan p = plan_rows(c, backward_target(c, at_once, resident), at_once);
+                        const int64_t chain = p.items * ((p.rows + at_once - 1) / at_once);        // rows that one team adds up
+                        const bool large = batch * pixels / at_once > int64_t(1) << 28;             // (more rows than a GPU's memory holds)
+                        if (chain > most && !large) most = chain;
+                        if ((chain > 512 && !large) || p.groups >= (int64_t(1) << 32) / 512) {
+                            printf("%lld items of %lld rows, %lld at once, %lld workgroups resident: %lld workgroups, a chain of %lld\n", (long long)batch, (long long)pixels,
+                                   (long long)at_once, (long long)resident, (long long)p.groups, (long long)chain);
+                            return 1;
+                        }
+                    }
+    printf("chains of at most %ld\n", most);
+    return most > 1 ? 0 : 1;
+}
+"""
+
+
+def test_sums_over_rows_are_short_chains(tmp_path):
+    """However many rows and items there are, a team of lanes adds few of them up one after the other."""
+    source, program = tmp_path / "chains.cpp", tmp_path / "chains"
+    source.write_text(CHAINS)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-D__HIP_PLATFORM_AMD__=1", "-I/opt/rocm/include", "-I" + CSRC, str(source), "-o", str(program)], check=True)
+    done = subprocess.run([str(program)], capture_output=True, text=True, timeout=100)
+    assert done.returncode == 0, done.stdout
