@@ -889,7 +889,7 @@ void known_lanes(const Shape& s, F f) {
 
 // As many workgroups as the chip holds at once: the forward's kernels leave room for four waves a SIMD, the backward's for two, and a workgroup is on one
 // compute unit whole: counted in waves, workgroups of 3, 5, 6 or 7 came in two rounds (8192 x 3500 bfloat16 forward 71 us, backward 139; 53 and 82 this way;
-// 4096 x 6400 backward 162 and 101; with 4 or 8 waves the count is the same). (Fewer where the backward's sums are long and in memory, two read and written
+// 4096 x 6400 backward 162 and 101; with 4 or 8 waves the count is the same). (Fewer where the backward's sums are long and in memory, read and written
 // for every row: 4096 x 12288 bfloat16 takes it 4.7 ms with 128 workgroups, 2.4 with 256, 512 or 1024; 2048 x 16384 3.2 and 1.6; 64 x 16384 0.16 with any number.
 // Their workspace grows with them, 20 bytes a channel and workgroup.)
 int64_t resident(const Shape& s, int waves) { return 256 * std::max(1, waves * 64 / s.threads); }
