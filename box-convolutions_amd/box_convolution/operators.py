@@ -255,7 +255,8 @@ def residual_norm(input, residual=None, gate=None, scale=1.0, after=None, before
     quantize: the normed rows as ``Float8Blocks``, for ``linear_act_float8`` (inference only: nothing here may require a gradient).
 
     Where nothing is done to the input (no residual, gate or norm behind the block, scale 1), the stream is the input itself.
-    Statistics and sums are float32; ``normed`` is formed from the stream before it is rounded to the input's type.
+    Statistics and sums are float32: a row with a value beyond 1.8e19, whose square float32 does not hold, has an infinite deviation, and is normalised to 0.
+    ``normed`` is formed from the stream before it is rounded to the input's type.
     """
     _native._require_device(input, "residual norm input")
     if kind not in ("rms", "layer"):
